@@ -10,6 +10,7 @@
 #include "cache/cache.h"
 #include "config/config.h"
 #include "engine/generate.h"
+#include "kernels/adapter_plan.h"
 #include "models/decoder.h"
 #include "weights/loader.h"
 
@@ -531,5 +532,15 @@ ILLM_API int illm_plan_batches(const int* prompt_lens, int n, long long max_new_
             a.push(e);
         }
         *out = dup_string(a.dump());
+    });
+}
+
+// The plan of tokens among adapters (csrc/adapters.h): sizes[4] and, unless out is null, its sizes' layout filled in.
+ILLM_API int illm_adapter_plan(const int* index, int T, const int* ranks, int count, int* sizes, int* total, int* out) {
+    return guard([&] {
+        const AdapterPlanSizes s = ops::adapter_plan_sizes(index, T, ranks, count);
+        sizes[0] = s.T, sizes[1] = s.slots, sizes[2] = s.groups, sizes[3] = s.chunks;
+        *total = adapter_plan_layout(s).total;
+        if (out) ops::adapter_plan_fill(index, T, ranks, count, s, out);
     });
 }

@@ -36,6 +36,22 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """For tensors of another device than the current one: kernels are launched on theirs, on its current stream."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 P_, I_, F_, LL_ = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 _KERNEL_SIGNATURES = {
     "illm_embedding": [P_, P_, I_, P_, I_, I_, I_, P_, P_],
@@ -64,6 +80,9 @@ _KERNEL_SIGNATURES = {
     "illm_argmax": [P_, I_, I_, I_, P_, P_, P_, P_],
     "illm_sample": [P_, I_, I_, I_, P_, P_, I_, F_, F_, I_, F_, P_, P_, P_, P_],
     "illm_sample_scratch_elems": [I_, I_, I_, F_],
+    "illm_linear_adapters_ws": [I_, I_, I_, I_, I_, I_, I_],
+    "illm_linear_adapters": [P_, P_, I_, I_, I_, I_, P_, P_, P_, I_, I_, P_, I_, I_, I_, P_, I_, P_, P_, P_],
+    "illm_sample_rows": [P_, I_, I_, I_, LL_, P_, P_, P_, P_, P_, P_, P_],
     "illm_fill_random": [P_, I_, LL_, ctypes.c_ulonglong, F_, F_, P_],
     "illm_poison_pages": [P_, P_, LL_, I_, LL_, P_, I_, P_],
     "illm_selftest_wait_timeout": [P_, P_, LL_, I_, P_],
@@ -80,7 +99,7 @@ def _declare():
     for name, args in _KERNEL_SIGNATURES.items():
         fn = getattr(h, name)
         fn.argtypes = args
-        fn.restype = LL_ if name == "illm_sample_scratch_elems" else I_
+        fn.restype = LL_ if name in ("illm_sample_scratch_elems", "illm_linear_adapters_ws") else I_
     _declared = True
 
 
@@ -754,6 +773,128 @@ def linear(x, w, out_dtype=None, defer_reduce=False, backend=None):
     return _take(dev, out, (M, N), out_dtype, x.device)
 
 
+_error_words = {}
+
+
+def _error_word(device):
+    """The address of the tensor-core kernels' error word on this device (outside an engine)."""
+    at = _error_words.get(device.index)
+    if at is None:
+        dev, n, tc, st = ctypes.c_void_p(), ctypes.c_int(), ctypes.c_void_p(), ctypes.c_void_p()
+        with _on(device):
+            _b.check(_b.lib().illm_test_device(ctypes.c_void_p(1), ctypes.byref(dev)))
+            _b.lib().illm_test_device_info(dev, ctypes.byref(n), ctypes.byref(tc), ctypes.byref(st))
+        at = _error_words[device.index] = tc.value
+    return at
+
+
+ADAPTER_GROUP, MAX_ADAPTER_RANK = 16, 256
+
+
+class Adapters:
+    """Room for `count` low-rank adapters of one projection W [n_out, n_in], each of a rank up to `rank` (at most 256):
+    y += scale * (x A^T) B^T with A [r, n_in] and B [n_out, r].  They are laid out once, as the kernels read them: `a`
+    [count, R, n_in] and `b` [count, R / 16, n_out, 16] with R the rank rounded up to 16.  An adapter that was never put has
+    rank 0 and adds nothing."""
+
+    def __init__(self, count, rank, n_out, n_in, dtype=torch.bfloat16, device=None):
+        if count < 1 or not 1 <= rank <= MAX_ADAPTER_RANK or n_out < 1 or n_in < 1:
+            raise KernelError(f"adapters: {count} adapters of rank {rank} for [{n_out}, {n_in}]: at least one, ranks of 1 to {MAX_ADAPTER_RANK}")
+        act_code(dtype)
+        if dtype == torch.bfloat16 and n_in % 8:
+            raise KernelError(f"adapters: the inner size {n_in} must be a multiple of 8 in bfloat16")
+        self.count, self.rank, self.n_out, self.n_in, self.dtype = count, rank, n_out, n_in, dtype
+        self.R = -(-rank // ADAPTER_GROUP) * ADAPTER_GROUP
+        self.device = torch.empty(0, device="cuda" if device is None else device).device
+        if self.device.type != "cuda":
+            raise KernelError("adapters live on a CUDA device: inferllm_b200 has no CPU path")
+        self.a = torch.zeros((count, self.R, n_in), dtype=dtype, device=self.device)
+        self.b = torch.zeros((count, self.R // ADAPTER_GROUP, n_out, ADAPTER_GROUP), dtype=dtype, device=self.device)
+        self.scales = torch.zeros((count,), dtype=torch.float32, device=self.device)
+        self.ranks = [0] * count
+
+    def put(self, i, a, b, scale=1.0):
+        """Adapter i becomes scale * b a (a [r, n_in], b [n_out, r], any float type); what it was is gone.  Works on torch's
+        current stream, like any torch operation.  A plan made before an adapter got a larger rank is refused."""
+        if not 0 <= i < self.count:
+            raise KernelError(f"adapters: there is no adapter {i} among {self.count}")
+        if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.n_in or b.shape[0] != self.n_out or a.shape[0] != b.shape[1]:
+            raise KernelError(f"adapters: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit [r, {self.n_in}] and [{self.n_out}, r]")
+        r = a.shape[0]
+        if r > self.rank:
+            raise KernelError(f"adapters: rank {r} exceeds the {self.rank} there is room for")
+        if not (a.is_floating_point() and b.is_floating_point()):
+            raise KernelError("adapters: the factors must be floating-point tensors")
+        self.a[i].zero_()
+        self.a[i, :r] = a
+        self.b[i].zero_()
+        for g in range(0, r, ADAPTER_GROUP):
+            e = min(r, g + ADAPTER_GROUP)
+            self.b[i, g // ADAPTER_GROUP, :, :e - g] = b[:, g:e]
+        self.scales[i] = float(scale)
+        self.ranks[i] = r
+
+    def remove(self, i):
+        """Adapter i adds nothing any more."""
+        self.put(i, self.a.new_zeros((0, self.n_in)), self.b.new_zeros((self.n_out, 0)), 0.0)
+
+
+class AdapterRows:
+    """Which adapter each token of a step has: `index` [T] of whole numbers on the host, -1 for none.  Made once per step and
+    used for every projection whose adapters have these ranks (or smaller ones)."""
+
+    def __init__(self, index, ranks, device=None):
+        index = index.tolist() if hasattr(index, "tolist") else list(index)
+        self.T, self.ranks = len(index), list(ranks)
+        self.named = sorted({a for a in index if a >= 0})
+        self.device = torch.empty(0, device="cuda" if device is None else device).device
+        sizes, total, c_index, c_ranks = (ctypes.c_int * 4)(), ctypes.c_int(), _b.ints(index), _b.ints(self.ranks)
+        _b.check(_b.lib().illm_adapter_plan(c_index, self.T, c_ranks, len(self.ranks), sizes, ctypes.byref(total), None))
+        host = torch.zeros(total.value, dtype=torch.int32)
+        _b.check(_b.lib().illm_adapter_plan(c_index, self.T, c_ranks, len(self.ranks), sizes, ctypes.byref(total),
+                                            ctypes.cast(host.data_ptr(), _b.PI)))
+        self.slots, self.groups, self.chunks = sizes[1], sizes[2], sizes[3]
+        self.plan = host.to(self.device)
+        self.most_groups = max((-(-self.ranks[a] // ADAPTER_GROUP) for a in self.named), default=0)
+
+    def fits(self, adapters):
+        """Whether the plan covers these adapters' ranks."""
+        have, need = self.ranks, adapters.ranks
+        return all(a < len(need) and -(-need[a] // ADAPTER_GROUP) <= -(-have[a] // ADAPTER_GROUP) for a in self.named) and self.most_groups * ADAPTER_GROUP <= adapters.R
+
+
+def linear_adapters(x, w, adapters, rows, out_dtype=None):
+    """y[t] = x[t] . W^T + scale_a (x[t] . A_a^T) . B_a^T, a the adapter that `rows` gives token t (none: the product alone).
+    x [T, K], w [N, K] float32 or bfloat16, `adapters` an `Adapters` of [N, K], `rows` an `AdapterRows` of T tokens; sums in
+    float32, rounded once to `out_dtype` (default x's; float32 is the other choice)."""
+    _need(x, "x", None, 2)
+    _need(w, "w", x.dtype, 2)
+    (T, K), (N, wk) = x.shape, w.shape
+    dtype, out_code = act_code(x.dtype), act_code(out_dtype or x.dtype)
+    if wk != K or adapters.n_in != K or adapters.n_out != N or adapters.dtype != x.dtype:
+        raise KernelError(f"linear_adapters: x is {x.dtype} [{T}, {K}], w [{N}, {wk}] and the adapters are {adapters.dtype} for [{adapters.n_out}, {adapters.n_in}]")
+    if rows.T != T:
+        raise KernelError(f"linear_adapters: the plan is of {rows.T} tokens, x has {T}")
+    if w.device != x.device or adapters.device != x.device or rows.device != x.device:
+        raise KernelError("linear_adapters: x, w, the adapters and the plan must be on one device")
+    if not rows.fits(adapters):
+        raise KernelError("linear_adapters: the plan was made for other ranks than the adapters have: make a new one")
+    if x.dtype == torch.bfloat16 and (K % 8 or x.data_ptr() & 15 or w.data_ptr() & 15):
+        raise KernelError(f"linear_adapters: K = {K} must be a multiple of 8 and the operands 16-byte aligned")
+    if x.dtype == torch.float32 and out_code != 0:
+        raise KernelError("linear_adapters: a float32 product stays float32")
+    out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=x.device)
+    if T == 0:
+        return out
+    lib = load()
+    ws = torch.empty((lib.illm_linear_adapters_ws(dtype, T, N, K, adapters.R, rows.groups, rows.chunks),), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _check(lib.illm_linear_adapters(x.data_ptr(), w.data_ptr(), dtype, T, N, K, adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scales.data_ptr(),
+                                        adapters.count, adapters.R, rows.plan.data_ptr(), rows.slots, rows.groups, rows.chunks, out.data_ptr(), out_code,
+                                        ws.data_ptr(), _error_word(x.device), _stream()), "linear_adapters")
+    return out
+
+
 def argmax(logits):
     """float32 [B, V] -> int32 [B], the lowest id among equal maxima (two passes: chunks of 2048
     elements, then the chunks' results)."""
@@ -793,6 +934,45 @@ def sample(logits, uniforms, temp, top_k=0, top_p=1.0, repeat_penalty=1.0, last_
                                   _ptr(last_tokens[b0:b1]) if last_tokens is not None else None, n_last, float(temp),
                                   float(repeat_penalty), int(top_k), float(top_p), _ptr(uniforms[b0:b1]),
                                   _ptr(out[b0:b1]), _ptr(scratch), _stream()), "sample")
+    return out
+
+
+def _per_row(t, name, dtype, B, device):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != B or t.device != device or not t.is_contiguous():
+        raise KernelError(f"sample_rows: {name} must be a contiguous {dtype} tensor [{B}] on {device}, found {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def sample_rows(logits, uniforms, temp=None, top_k=None, top_p=None, min_p=None):
+    """The next token of every row by settings of its own -> int32 [B].
+
+    logits [B, V] float32 or bfloat16 (rows may be further apart than V); uniforms float32 [B] in [0, 1); temp, top_p and
+    min_p float32 [B], top_k int32 [B], each None for "off" in every row (temperature 1).  With w = exp((l - max l) / temp) and
+    the words in descending order of their logit (equal ones in ascending order of their id), a row keeps the first top_k
+    (<= 0: all), of these the shortest prefix whose weight reaches top_p of theirs (>= 1: all, <= 0: the first), of these the
+    words with w >= min_p (<= 0: all, above 1 counts as 1), and takes the first of them, ids ascending, at which the sum of the weights
+    exceeds u times their whole sum.  temp <= 0 or NaN: the lowest id of the largest.  Words at -inf or NaN never come; a row
+    without any other gives -1.  Weights are made in float64 and summed as integers: the result does not depend on the
+    order of a sum."""
+    if not logits.is_cuda:
+        raise KernelError("logits must be a CUDA tensor: inferllm_b200 has no CPU path")
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise KernelError(f"sample_rows: logits must be float32 or bfloat16 [B, V], found {logits.dtype} {tuple(logits.shape)}")
+    B, V = logits.shape
+    device = logits.device
+    if V == 0 or (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
+        raise KernelError(f"sample_rows: rows of at least one word, each contiguous and none within another, found {tuple(logits.shape)} with strides {logits.stride()}")
+    if uniforms is None:
+        raise KernelError("sample_rows: one uniform number per row is needed")
+    u = _per_row(uniforms, "uniforms", torch.float32, B, device)
+    settings = (_per_row(temp, "temp", torch.float32, B, device), _per_row(top_k, "top_k", torch.int32, B, device),
+                _per_row(top_p, "top_p", torch.float32, B, device), _per_row(min_p, "min_p", torch.float32, B, device))
+    out = torch.empty((B,), dtype=torch.int32, device=device)
+    with _on(device):
+        _check(load().illm_sample_rows(logits.data_ptr(), _DT[logits.dtype], B, V, logits.stride(0) if B > 1 else V, u, *settings, out.data_ptr(),
+                                       _stream()), "sample_rows")
     return out
 
 

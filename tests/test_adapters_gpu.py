@@ -1,0 +1,199 @@
+"""Low-rank adapters beside a shared projection, against the formula in 64 bits (GPU).
+
+Tolerances.  float32: the K products of a result, and the R behind them, are added in float32, each addition off by at most
+2^-24 of a partial sum; partial sums stay within the result's own size, that of one normal variable for the shared product, and
+sum |v| |B| for the adapter, so (K + R) 2^-24 times their sum bounds the error.  bfloat16: the result is rounded once, at most
+2^-8 of its value; on the prompt path the intermediate values v are rounded as well, which is at most 2^-8 sum |v| |B|.  In the
+root-mean-square a rounding to bfloat16 is off by 2^-8 / sqrt(3) times the mean square of where a value lies within its power
+of two, 0.0017 of the values; the two of them by 0.0024 of the results, and 2^-8 = 0.0039 is the bound."""
+import numpy as np
+import pytest
+import torch
+
+from inferllm_b200.kernels import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def make(T, K, N, ranks, dtype, seed, scale_of=lambda i: 1.0 + 0.5 * i):
+    g = torch.Generator("cuda").manual_seed(seed)
+
+    def normal(*shape, std):
+        return (torch.randn(shape, generator=g, device="cuda") * std).to(dtype)
+
+    x, w = normal(T, K, std=1.0), normal(N, K, std=K ** -0.5)
+    a, b = [normal(r, K, std=K ** -0.5) for r in ranks], [normal(N, r, std=1.0) for r in ranks]
+    ad = ops.Adapters(len(ranks), max(max(ranks), 1), N, K, dtype)
+    for i, r in enumerate(ranks):
+        if r:
+            ad.put(i, a[i], b[i], scale_of(i))
+    return x, w, a, b, ad, [scale_of(i) for i in range(len(ranks))]
+
+
+def expected(x, w, a, b, scales, index):
+    """(value, |terms| of the adapter) in 64 bits."""
+    y, spread = x.double() @ w.double().t(), torch.zeros((x.shape[0], w.shape[0]), dtype=torch.float64, device="cuda")
+    for t, i in enumerate(index):
+        if i >= 0 and a[i].shape[0]:
+            v = scales[i] * (a[i].double() @ x[t].double())
+            y[t] += b[i].double() @ v
+            spread[t] = b[i].double().abs() @ v.abs()
+    return y, spread
+
+
+def check(got, x, w, a, b, scales, index):
+    want, spread = expected(x, w, a, b, scales, index)
+    err = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    terms = x.shape[1] + max([m.shape[0] for m in a])
+    sums = 2.0 ** -24 * terms * (1.0 + want.abs() + spread)
+    if x.dtype == torch.float32:
+        assert bool((err <= sums).all()), float((err - sums).max())
+    else:
+        out = 2.0 ** -8 * want.abs() if got.dtype == torch.bfloat16 else 0.0
+        bound = sums + out + 2.0 ** -8 * spread
+        assert bool((err <= bound).all()), float((err - bound).max())
+        scale = float((want ** 2).mean().sqrt())
+        assert float((err ** 2).mean().sqrt()) <= 2.0 ** -8 * scale
+
+
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 2, 3, 8, 16, 17, 33, 64, 65, 127, 130, 256, 257, 300, 600])
+def test_tokens(T, dtype):
+    ranks = [16, 8, 1, 64, 20, 0, 33]
+    rng = np.random.default_rng(T)
+    index = rng.integers(-1, len(ranks), T).tolist()
+    x, w, a, b, ad, s = make(T, 328, 520, ranks, dtype, T)
+    check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(8, 1), (64, 192), (72, 130), (1000, 257), (144, 1001), (4096, 136), (2048, 600)])
+def test_sizes(K, N, dtype):
+    for T in (1, 9, 40, 100, 290):
+        ranks = [4, 16, 48]
+        index = [(t * 5) % 4 - 1 for t in range(T)]
+        x, w, a, b, ad, s = make(T, K, N, ranks, dtype, K + T)
+        check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rank", [1, 7, 16, 17, 64, 65, 128, 200, 256])
+def test_ranks(rank, dtype):
+    for T in (5, 64, 150):
+        x, w, a, b, ad, s = make(T, 256, 264, [rank, 3], dtype, rank + T)
+        index = [t % 2 for t in range(T)]
+        check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [4, 64, 200, 512])
+def test_kinds_of_batches(T, dtype):
+    """All with one adapter, none with any, every token with its own, one token with one, prompts one behind another."""
+    ranks = [16] * 64
+    x, w, a, b, ad, s = make(T, 512, 384, ranks, dtype, 7 * T, lambda i: 0.25 + 0.01 * i)
+    for index in ([63] * T, [-1] * T, [t % 64 for t in range(T)], [-1] * (T - 1) + [5], [2] + [-1] * (T - 1), [(t * 4 // T) * 9 - 1 for t in range(T)]):
+        check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+def test_no_adapter_is_the_product():
+    for T in (3, 64, 100, 500):
+        x, w, a, b, ad, s = make(T, 512, 384, [16], torch.float32, T)
+        got = ops.linear_adapters(x, w, ad, ops.AdapterRows([-1] * T, ad.ranks))
+        assert torch.equal(got, ops.gemm_f32(x, w))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_token_does_not_depend_on_adapters_of_others(dtype):
+    """Infinities and NaN in another token's row or adapter stay there."""
+    for T in (6, 64, 200, 300):
+        x, w, a, b, ad, s = make(T, 320, 272, [16, 32, 8], dtype, T)
+        index = [(t * 7) % 4 - 1 for t in range(T)]
+        rows = ops.AdapterRows(index, ad.ranks)
+        want = ops.linear_adapters(x, w, ad, rows)
+        a[1][0, 3], b[1][5, 2] = float("inf"), float("nan")
+        ad.put(1, a[1], b[1], s[1])
+        bad = [t for t in range(T) if index[t] == 1]
+        clean = next(t for t in range(T) if index[t] == 0)
+        x[clean] = float("nan")
+        got = ops.linear_adapters(x, w, ad, rows)
+        ok = [t for t in range(T) if index[t] != 1 and t != clean]
+        assert torch.equal(got[ok], want[ok])
+        assert not torch.isfinite(got[bad]).all() and got[clean].isnan().all()
+
+
+def test_float32_rows_do_not_depend_on_the_batch():
+    T = 70
+    x, w, a, b, ad, s = make(T, 500, 300, [16, 24, 5], torch.float32, 1)
+    index = [(t * 5) % 4 - 1 for t in range(T)]
+    whole = ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks))
+    for t in (0, 1, 2, 3, 33, 69):
+        one = ops.linear_adapters(x[t:t + 1].contiguous(), w, ad, ops.AdapterRows(index[t:t + 1], ad.ranks))
+        assert torch.equal(one[0], whole[t])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_put_replaces_and_remove_removes(dtype):
+    x, w, a, b, ad, s = make(40, 256, 200, [32, 16], dtype, 3)
+    index = [t % 2 for t in range(40)]
+    rows = ops.AdapterRows(index, ad.ranks)
+    ad.put(0, a[1], b[1], 2.0)                          # a smaller rank: the plan still covers it
+    check(ops.linear_adapters(x, w, ad, rows), x, w, [a[1], a[1]], [b[1], b[1]], [2.0, s[1]], index)
+    ad.remove(1)
+    check(ops.linear_adapters(x, w, ad, rows), x, w, [a[1], a[1]], [b[1], b[1]], [2.0, 0.0], index)
+    ad.put(1, a[0], b[0], 1.0)                          # a larger one: it does not
+    with pytest.raises(ops.KernelError):
+        ops.linear_adapters(x, w, ad, rows)
+
+
+def test_float32_results_of_bfloat16():
+    for T in (3, 64, 100, 300):
+        x, w, a, b, ad, s = make(T, 256, 200, [16, 40], torch.bfloat16, T)
+        index = [t % 3 - 1 for t in range(T)]
+        got = ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks), torch.float32)
+        assert got.dtype == torch.float32
+        check(got, x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("T", [5, 64, 300])
+def test_streams_and_graphs(T):
+    x, w, a, b, ad, s = make(T, 512, 384, [16, 32], torch.bfloat16, T)
+    rows = ops.AdapterRows([t % 3 - 1 for t in range(T)], ad.ranks)
+    want = ops.linear_adapters(x, w, ad, rows)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = ops.linear_adapters(x, w, ad, rows)
+    stream.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_adapters(x, w, ad, rows)
+    for seed in (1, 2):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").bfloat16())
+        graph.replay()
+        assert torch.equal(got, ops.linear_adapters(x, w, ad, rows))
+
+
+def test_refusals():
+    x, w, a, b, ad, s = make(4, 64, 32, [8, 8], torch.bfloat16, 1)
+    rows = ops.AdapterRows([0, 1, -1, 0], ad.ranks)
+    other = ops.Adapters(2, 8, 32, 64, torch.float32)
+    bad = [lambda: ops.linear_adapters(x[:3].contiguous(), w, ad, rows), lambda: ops.linear_adapters(x, w[:, :56].contiguous(), ad, rows),
+           lambda: ops.linear_adapters(x, w[:16].contiguous(), ad, rows), lambda: ops.linear_adapters(x, w, other, rows),
+           lambda: ops.linear_adapters(x.float(), w, ad, rows), lambda: ops.linear_adapters(x.cpu(), w, ad, rows),
+           lambda: ops.linear_adapters(x.t().contiguous().t(), w, ad, rows), lambda: ops.linear_adapters(x, w, ad, rows, torch.float16),
+           lambda: ops.linear_adapters(x.float(), w.float(), other, rows, torch.bfloat16),
+           lambda: ops.linear_adapters(x, w, ad, ops.AdapterRows([0, 2, -1, 0], [8, 8, 8])),
+           lambda: ops.linear_adapters(x, w, ad, ops.AdapterRows([0, 1, -1, 0], [8, 0])),
+           lambda: ad.put(2, a[0], b[0]), lambda: ad.put(0, a[0][:, :32], b[0]), lambda: ad.put(0, a[0], b[0][:, :4]),
+           lambda: ad.put(0, torch.zeros(9, 64), torch.zeros(32, 9)), lambda: ad.put(0, a[0].int(), b[0]),
+           lambda: ops.Adapters(0, 8, 32, 64), lambda: ops.Adapters(2, 257, 32, 64), lambda: ops.Adapters(2, 8, 32, 60),
+           lambda: ops.Adapters(2, 8, 32, 64, torch.float16), lambda: ops.Adapters(2, 8, 32, 64, device="cpu"),
+           lambda: ops.AdapterRows([0, 2], [8, 8]), lambda: ops.AdapterRows([-2], [8]), lambda: ops.AdapterRows([0], [300])]
+    for call in bad:
+        with pytest.raises(ops.KernelError):
+            call()
