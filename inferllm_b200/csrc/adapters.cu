@@ -10,21 +10,11 @@
 //            reads a row of A once for the tokens of a slot;
 //   expand   y[t, n] = base[t, n] + v[t] . B_a[n]: a thread per output column, the slot's 16 values of B in registers.
 // Sums are float32 in one order per token, whatever else is in the batch.
-#include "adapters.h"
-#include "common.cuh"
+#include "adapters.cuh"
 #include "kernels.h"
 
 #define AD_TOKENS 8
 #define AD_COLS 128
-
-struct AdPlan {
-    const int *counts, *token_adapter, *order, *slot_begin, *slot_adapter, *slot_group, *groups, *tile_chunk, *chunk_tile, *chunk_groups;
-};
-static AdPlan ad_plan(const int* plan, const AdapterPlanSizes& s) {
-    const AdapterPlanLayout l = adapter_plan_layout(s);
-    return AdPlan{plan + l.counts, plan + l.token_adapter, plan + l.order, plan + l.slot_begin, plan + l.slot_adapter, plan + l.slot_group, plan + l.groups,
-                  plan + l.tile_chunk, plan + l.chunk_tile, plan + l.chunk_groups};
-}
 
 // v[t, 16 g + r] for the ranks of group g of token t's adapter, float32 [T, R]
 template <typename T>
@@ -116,52 +106,328 @@ adapter_expand_kernel(const float* base, int N, const T* __restrict__ b, const f
     }
 }
 
-// Bytes of workspace that illm_linear_adapters needs.
-extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int groups, int chunks) {
-    const long long v = (long long)T * R * 4, base = dtype == ILLM_BF16 ? (long long)T * N * 4 : 0;
-    return (v + 255) / 256 * 256 + base;
+// ---- The rows form (bfloat16, up to 256 tokens): two launches.
+//
+// The first streams W once and, in the same grid, the first factors of the adapters that the tokens name: rank groups are
+// nothing but more rows of the weight.  A block multiplies 128 of those rows (a tile of W, or 8 rank groups fetched by a TMA box
+// of 16 rows each, so that they may come from any adapters) with all tokens over its slice of K on tcgen05, the rows on the
+// 128 lanes, the tokens as the MMA's N, and leaves float32 slices, so that all SMs stream whatever N is.
+// The second adds up the slices and, in the same float32 sum, v[t] . B_a[n]; v, the tokens' rank values, is added up and
+// scaled by every block for the tokens that it works on.  It stays float32: the result is rounded once.
+#define AD_ROWS_MAX_STAGES 8
+
+template <int BN>
+__global__ void __launch_bounds__(TC_THREADS)
+adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x,
+                    float* __restrict__ base, float* __restrict__ vs, int v_ld, int T, int N, int R, int base_tiles, const AdPlan plan, int k_iters_total,
+                    int k_iters_per_split, int STAGES, int early, int* __restrict__ err) {
+    constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = BN * TC_BK * 2, BOX_BYTES = ADAPTER_GROUP * TC_BK * 2;
+    constexpr unsigned TMEM_COLS = BN < 32 ? 32 : BN;
+    constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(BN >> 3) << 17) | ((unsigned)(TC_BM >> 4) << 24);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * AD_ROWS_MAX_STAGES + 1];
+    __shared__ unsigned tmem_holder;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool shrink = (int)blockIdx.x >= base_tiles;
+    const int g0 = shrink ? ((int)blockIdx.x - base_tiles) * (TC_BM / ADAPTER_GROUP) : 0;
+    int boxes = 0;
+    if (shrink) {
+        boxes = min(TC_BM / ADAPTER_GROUP, plan.counts[1] - g0);
+        if (boxes <= 0) return;                         // the grid is sized for more rank groups than there are
+    }
+    const int ra0 = blockIdx.x * TC_BM, rows = shrink ? boxes * ADAPTER_GROUP : min(TC_BM, N - ra0);
+
+    const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + STAGES * A_BYTES;
+    const unsigned full0 = tc_smem_u32(&bars[0]), empty0 = tc_smem_u32(&bars[AD_ROWS_MAX_STAGES]);
+    const unsigned done_bar = tc_smem_u32(&bars[2 * AD_ROWS_MAX_STAGES]);
+    const int k_begin = blockIdx.z * k_iters_per_split, n_k = min(k_iters_total - k_begin, k_iters_per_split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(done_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(&tmem_holder)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_holder;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int group_row[TC_BM / ADAPTER_GROUP];
+#pragma unroll
+            for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++) {
+                const int g = j < boxes ? plan.groups[g0 + j] : 0;
+                group_row[j] = (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
+            }
+            auto arm_and_load_weights = [&](int i, int s) {
+                mbar_expect_tx(full0 + 8 * s, (shrink ? boxes * BOX_BYTES : A_BYTES) + B_BYTES);
+                const int kx = (k_begin + i) * TC_BK;
+                if (!shrink) {
+                    tma_load_2d(a_base + s * A_BYTES, &map_w, kx, ra0, full0 + 8 * s);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++)
+                        if (j < boxes) tma_load_2d(a_base + s * A_BYTES + j * BOX_BYTES, &map_a, kx, group_row[j], full0 + 8 * s);
+                }
+            };
+            // where no kernel before this one makes weights, the first ring of them comes before the wait for the tokens' rows
+            const int n_pre = n_k < STAGES ? n_k : STAGES;
+            if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int i = 0; i < n_pre; i++) arm_and_load_weights(i, i);
+            if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int i = 0; i < n_pre; i++) tma_load_2d(b_base + i * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * i);
+            bool alive = true;
+            for (int i = n_pre; i < n_k && alive; i++) {
+                const int s = i % STAGES;
+                alive = mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, err);
+                if (!alive) break;
+                arm_and_load_weights(i, s);
+                tma_load_2d(b_base + s * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * s);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool alive = true;
+            for (int i = 0; i < n_k && alive; i++) {
+                const int s = i % STAGES;
+                alive = mbar_wait(full0 + 8 * s, (i / STAGES) & 1, err);
+                if (!alive) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < TC_BK / 16; kk++)
+                    umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
+                              (i > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(empty0 + 8 * s);
+            }
+            umma_commit(done_bar);
+        }
+    } else {
+        const int quad = warp & 3, row = quad * 32 + lane;
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // the workspace may still be read by an earlier kernel
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, err));
+        tc_fence_after();
+        const int ld = shrink ? v_ld : N;
+        float* to = (shrink ? vs : base) + (size_t)blockIdx.z * T * ld + (shrink ? g0 * ADAPTER_GROUP : ra0) + row;
+        if (ok)
+#pragma unroll 1
+            for (int c0 = 0; c0 < BN; c0 += 16) {
+                if (c0 >= T) break;
+                float v[16];
+                tmem_ld16(tmem + ((unsigned)(quad * 32) << 16) + (unsigned)c0, v);
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (c0 + j < T && row < rows) to[(size_t)(c0 + j) * ld] = v[j];
+            }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
 }
 
-template <typename TX, typename TOut>
-static int ad_general(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int R, const AdapterPlanSizes& sz,
-                      const int* plan_dev, TOut* out, char* ws, int* err, cudaStream_t s) {
-    const AdPlan plan = ad_plan(plan_dev, sz);
-    float* v = (float*)ws;
-    const int groups = R / ADAPTER_GROUP, tiles = (T + AD_TOKENS - 1) / AD_TOKENS;
-    float* base;
-    int rc;
-    if (sizeof(TX) == 4) {
-        base = (float*)out;
-        rc = illm_gemm_f32_nt((const float*)x, (const float*)w, base, T, N, K, K, K, N, err, s);
-    } else {
-        base = (float*)(ws + ((size_t)T * R * 4 + 255) / 256 * 256);
-        rc = T <= 64 ? illm_gemm_bf16_tc(x, w, base, ILLM_F32, T, N, K, nullptr, 1, err, s, 0) : illm_gemm_bf16_tc2(x, w, base, ILLM_F32, 0, T, N, K, err, s);
+__device__ __forceinline__ float ad_dot16(const float* w, const float* v, float acc) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const float4 f = reinterpret_cast<const float4*>(v)[q];
+        acc = fmaf(f.x, w[4 * q], acc);
+        acc = fmaf(f.y, w[4 * q + 1], acc);
+        acc = fmaf(f.z, w[4 * q + 2], acc);
+        acc = fmaf(f.w, w[4 * q + 3], acc);
     }
-    if (rc != 0) return rc;
-    if (sz.slots > 0)
-        illm_launch(adapter_shrink_kernel<TX>, dim3(tiles, groups), dim3(256), 0, s, (const TX*)x, K, (const TX*)a, scales, R, plan, T, v);
-    illm_launch(adapter_expand_kernel<TX, TOut>, dim3((N + AD_COLS - 1) / AD_COLS, tiles), dim3(AD_COLS), 0, s, (const float*)base, N, (const TX*)b,
-                (const float*)v, R, plan, T, out);
+    return acc;
+}
+
+// TOK places of the plan's order by 128 columns.  SHARED: neighbours mostly have the same adapter, whose values of B are then
+// loaded once for them; otherwise the loads of all places are in flight together.
+template <int TOK, bool SHARED, typename TOut>
+__global__ void __launch_bounds__(AD_COLS)
+adapter_join_kernel(const float* __restrict__ base, int splits, long long stride, int N, const bf16* __restrict__ b, const float* __restrict__ vs, int v_ld,
+                    const float* __restrict__ scales, int R, const int4* __restrict__ places, int T, TOut* __restrict__ out) {
+    pdl_grid_sync();
+    __shared__ __align__(16) float v[TOK][ADAPTER_GROUP * ADAPTER_MAX_GROUPS];
+    const int tid = threadIdx.x, col = blockIdx.x * AD_COLS + tid, p0 = blockIdx.y * TOK;
+    int4 at[TOK];                                       // token, adapter, first group, groups
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < TOK; i++) {
+        at[i] = p0 + i < T ? places[p0 + i] : make_int4(-1, -1, 0, 0);
+        most = max(most, at[i].w);
+    }
+    float acc[TOK];
+#pragma unroll
+    for (int i = 0; i < TOK; i++) acc[i] = 0.f;
+    if (col < N)
+        for (int z = 0; z < splits; z++)
+#pragma unroll
+            for (int i = 0; i < TOK; i++)
+                if (at[i].x >= 0) acc[i] += base[(size_t)z * stride + (size_t)at[i].x * N + col];
+    if (most > 0) {
+#pragma unroll
+        for (int i = 0; i < TOK; i++) {
+            const int n = at[i].w * ADAPTER_GROUP;
+            if (n > 0) {
+                const float s = scales[at[i].y];
+                for (int r = tid; r < n; r += AD_COLS) {
+                    const float* from = vs + (size_t)at[i].x * v_ld + at[i].z * ADAPTER_GROUP + r;
+                    float t = 0.f;
+                    for (int z = 0; z < splits; z++) t += from[(size_t)z * T * v_ld];
+                    v[i][r] = s * t;
+                }
+            }
+        }
+        __syncthreads();
+        if (col < N)
+            for (int g = 0; g < most; g++) {
+                const bf16* bg = b + ((size_t)g * N + col) * ADAPTER_GROUP;
+                const size_t ld = (size_t)(R / ADAPTER_GROUP) * N * ADAPTER_GROUP;
+                if (SHARED) {
+                    float w[ADAPTER_GROUP];
+#pragma unroll
+                    for (int i = 0; i < TOK; i++)
+                        if (g < at[i].w) {
+                            if (i == 0 || at[i].y != at[i - 1].y) {
+                                load8(bg + at[i].y * ld, w);
+                                load8(bg + at[i].y * ld + 8, w + 8);
+                            }
+                            acc[i] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i]);
+                        }
+                } else {
+                    float w[TOK][ADAPTER_GROUP];
+#pragma unroll
+                    for (int i = 0; i < TOK; i++)
+                        if (g < at[i].w) {
+                            load8(bg + at[i].y * ld, w[i]);
+                            load8(bg + at[i].y * ld + 8, w[i] + 8);
+                        }
+#pragma unroll
+                    for (int i = 0; i < TOK; i++)
+                        if (g < at[i].w) acc[i] = ad_dot16(w[i], &v[i][g * ADAPTER_GROUP], acc[i]);
+                }
+            }
+    }
+    if (col < N)
+#pragma unroll
+        for (int i = 0; i < TOK; i++)
+            if (at[i].x >= 0) out[(size_t)at[i].x * N + col] = from_f32<TOut>(acc[i]);
+}
+
+// ---- host side
+
+// How the rows form cuts K: as many slices as bring about two blocks to an SM (one beyond 128 tokens, whose stages are larger),
+// each at least 8 pieces of 64 wide, at most 8 slices (their reader pays for every one).
+struct AdRows { int base_tiles, shrink_tiles, k_iters, per, splits; };
+static AdRows ad_rows(int T, int N, int K, int groups) {
+    AdRows r;
+    r.base_tiles = ad_div(N, TC_BM);
+    r.shrink_tiles = ad_div(groups, TC_BM / ADAPTER_GROUP);
+    r.k_iters = ad_div(K, TC_BK);
+    int s = (T > 128 ? 1 : 2) * illm_sm_count() / (r.base_tiles + r.shrink_tiles);
+    s = s > r.k_iters / 8 ? r.k_iters / 8 : s;
+    s = s > 8 ? 8 : s;
+    s = s < 1 ? 1 : s;
+    r.per = ad_div(r.k_iters, s);
+    r.splits = ad_div(r.k_iters, r.per);
+    return r;
+}
+
+template <int BN>
+static int ad_launch_rows(const CUtensorMap& mw, const CUtensorMap& ma, const CUtensorMap& mx, float* base, float* vs, int v_ld, int T, int N, int R,
+                          const AdRows& r, const AdPlan& plan, int early, int* err, cudaStream_t s) {
+    const int stage = (TC_BM + BN) * TC_BK * 2;
+    const int blocks = (r.base_tiles + r.shrink_tiles) * r.splits, sms = illm_sm_count();
+    const int resident = blocks > 2 * sms ? 3 : (blocks > sms ? 2 : 1);
+    int stages = (227 * 1024 / resident - 2560) / stage;
+    stages = stages > AD_ROWS_MAX_STAGES ? AD_ROWS_MAX_STAGES : (stages < 2 ? 2 : stages);
+    if (stages > r.per) stages = r.per < 2 ? 2 : r.per;
+    const size_t smem = (size_t)stages * stage + 1024;
+    auto kern = adapter_rows_kernel<BN>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    illm_launch(kern, dim3(r.base_tiles + r.shrink_tiles, 1, r.splits), dim3(TC_THREADS), smem, s, mw, ma, mx, base, vs, v_ld, T, N, R, r.base_tiles, plan,
+                r.k_iters, r.per, stages, early, err);
+    return illm_launch_status();
+}
+
+template <typename TOut>
+static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R,
+                        const AdapterPlanSizes& sz, const int* plan_dev, TOut* out, char* ws, int early, int* err, cudaStream_t s) {
+    const AdPlan plan = ad_plan(plan_dev, sz);
+    const AdRows r = ad_rows(T, N, K, sz.groups);
+    const int v_ld = sz.groups * ADAPTER_GROUP, bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    float *vs = (float*)ws, *base = (float*)(ws + ad_round((long long)r.splits * T * v_ld * 4));
+    CUtensorMap mw, ma, mx;
+    int rc;
+    if ((rc = ad_make_map(&mw, w, N, K, TC_BM)) || (rc = ad_make_map(&ma, a, (long long)count * R, K, ADAPTER_GROUP)) || (rc = ad_make_map(&mx, x, T, K, bn)))
+        return rc;
+    switch (bn) {
+        case 16: rc = ad_launch_rows<16>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
+        case 32: rc = ad_launch_rows<32>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
+        case 64: rc = ad_launch_rows<64>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
+        case 128: rc = ad_launch_rows<128>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
+        default: rc = ad_launch_rows<256>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s);
+    }
+    if (rc) return rc;
+    auto join = [&](auto kern, int tok) {
+        illm_launch(kern, dim3(ad_div(N, AD_COLS), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
+                    (const float*)vs, v_ld, scales, R, plan.places, T, out);
+    };
+    // many tokens of few adapters: prompts
+    if (T <= 4) join(adapter_join_kernel<1, false, TOut>, 1);
+    else if (T > 64 && 4 * sz.slots <= T) join(adapter_join_kernel<8, true, TOut>, 8);
+    else join(adapter_join_kernel<4, false, TOut>, 4);
+    return illm_launch_status();
+}
+
+// Bytes of workspace that illm_linear_adapters needs.
+extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int groups, int chunks) {
+    if (dtype == ILLM_BF16 && T <= ADAPTER_ROWS_MAX) {
+        const long long splits = ad_rows(T, N, K, groups).splits;
+        return ad_round(splits * T * groups * ADAPTER_GROUP * 4) + splits * T * N * 4;
+    }
+    return 256 + (dtype == ILLM_BF16 ? ad_prompt_ws(T, N, K, chunks) : (long long)T * R * 4);
+}
+
+static int ad_float32(const float* x, const float* w, int T, int N, int K, const float* a, const float* b, const float* scales, int R,
+                      const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int* err, cudaStream_t s) {
+    const AdPlan plan = ad_plan(plan_dev, sz);
+    const int tiles = ad_div(T, AD_TOKENS);
+    const int rc = illm_gemm_f32_nt(x, w, out, T, N, K, K, K, N, err, s);
+    if (rc != 0 || sz.slots == 0) return rc;
+    illm_launch(adapter_shrink_kernel<float>, dim3(tiles, R / ADAPTER_GROUP), dim3(256), 0, s, x, K, a, scales, R, plan, T, v);
+    illm_launch(adapter_expand_kernel<float, float>, dim3(ad_div(N, AD_COLS), tiles), dim3(AD_COLS), 0, s, (const float*)out, N, b, (const float*)v, R, plan, T,
+                out);
     return illm_launch_status();
 }
 
 // out [T, N] = x W^T + the tokens' adapters.  dtype: of x, W, A and B; out_dtype float32 or that.  plan: the device array laid
 // out by adapter_plan_layout({T, slots, groups, chunks}).  ws: illm_linear_adapters_ws bytes, 256-byte aligned.
 extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales,
-                                    int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int* err,
-                                    void* stream) {
+                                    int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int early,
+                                    int* err, void* stream) {
     if (T <= 0 || N <= 0) return 0;
     if (K <= 0 || count <= 0 || R <= 0 || R % ADAPTER_GROUP || R > ADAPTER_GROUP * ADAPTER_MAX_GROUPS || slots < 0 || groups < 0 || chunks < 0 || !ws || !plan ||
-        T > 65535 * AD_TOKENS)
-        return ILLM_ERR_BAD_ARG;
+        T > 65535 * AD_TOKENS || (long long)count * R * (N / ADAPTER_GROUP + 1) >= (1ll << 31) || (long long)count * R >= (1ll << 31))
+        return ILLM_ERR_BAD_ARG;        // (rows of the factors are counted in 32 bits)
     if (dtype == ILLM_BF16 && ((K & 7) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)a & 15) || ((uintptr_t)b & 15))) return ILLM_ERR_BAD_ARG;
     const AdapterPlanSizes sz{T, slots, groups, chunks};
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == ILLM_F32 && out_dtype == ILLM_F32)
-        return ad_general<float, float>(x, w, T, N, K, a, b, scales, R, sz, plan, (float*)out, (char*)ws, err, s);
-    if (dtype == ILLM_BF16 && out_dtype == ILLM_BF16)
-        return ad_general<bf16, bf16>(x, w, T, N, K, a, b, scales, R, sz, plan, (bf16*)out, (char*)ws, err, s);
-    if (dtype == ILLM_BF16 && out_dtype == ILLM_F32)
-        return ad_general<bf16, float>(x, w, T, N, K, a, b, scales, R, sz, plan, (float*)out, (char*)ws, err, s);
-    return ILLM_ERR_BAD_ARG;
+        return ad_float32((const float*)x, (const float*)w, T, N, K, (const float*)a, (const float*)b, scales, R, sz, plan, (float*)out, (float*)ws, err, s);
+    if (dtype != ILLM_BF16 || (out_dtype != ILLM_BF16 && out_dtype != ILLM_F32)) return ILLM_ERR_BAD_ARG;
+    if (T > ADAPTER_ROWS_MAX)
+        return ad_prompt_form(x, w, T, N, K, a, b, scales, count, R, ad_plan(plan, sz), chunks, out, out_dtype, (char*)ws, early, err, s);
+    if (out_dtype == ILLM_BF16) return ad_rows_form<bf16>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (bf16*)out, (char*)ws, early, err, s);
+    return ad_rows_form<float>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (float*)out, (char*)ws, early, err, s);
 }

@@ -10,6 +10,7 @@
 #define ADAPTER_TILE 256          // tokens of a tile of the prompt product
 #define ADAPTER_CHUNK 4           // groups of a chunk: one 64-wide K piece of the prompt product
 #define ADAPTER_MAX_GROUPS 16     // ranks up to 256
+#define ADAPTER_ROWS_MAX 256      // tokens up to which the rows form runs; above it the plan has tiles
 
 struct AdapterPlanSizes {
     int T;                        // tokens
@@ -22,6 +23,7 @@ struct AdapterPlanLayout {
     int counts;                   // [4] slots, rank groups, chunks that there really are, and the most groups of a slot
     int token_adapter;            // [T] adapter of a token, -1: none
     int order;                    // [T] the tokens by slot
+    int places;                   // [T * 4] per place of `order`: the token, its adapter (-1: none), where its slot begins in `groups`, how many it has
     int slot_begin;               // [slots + 2] where a slot begins in `order` (the last slot: tokens without an adapter)
     int slot_adapter;             // [slots + 1] -1 for the last
     int slot_group;               // [slots + 2] where a slot begins in `groups`
@@ -38,6 +40,7 @@ static inline AdapterPlanLayout adapter_plan_layout(const AdapterPlanSizes& s) {
     l.counts = off;        off += 4;
     l.token_adapter = off; off += adapter_pad4(s.T);
     l.order = off;         off += adapter_pad4(s.T);
+    l.places = off;        off += s.T * 4;
     l.slot_begin = off;    off += adapter_pad4(s.slots + 2);
     l.slot_adapter = off;  off += adapter_pad4(s.slots + 1);
     l.slot_group = off;    off += adapter_pad4(s.slots + 2);

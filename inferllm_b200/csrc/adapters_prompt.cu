@@ -1,0 +1,389 @@
+// Low-rank adapters beside a shared projection, for prompts in bfloat16: the adapters are a longer K.
+//   y[t] = [x[t], v[t]] . [W, B]^T,   v[t] = s_a x[t] A_a^T
+// For a tile of 256 tokens the further columns are the rank groups (16 ranks each) of the adapters that the tile's tokens name, four
+// groups to a chunk of 64 columns; a token's v is zero in the groups of other adapters.  A prompt's tile names one or two
+// adapters: one chunk behind the K / 64 pieces of the shared product, in the same accumulators, rounded once with it.
+//
+// adapter_values_kernel makes the chunks of v: 128 tokens by 64 ranks per cluster, tcgen05 (tokens on the lanes, four TMA boxes of
+// 16 rows of A as the MMA's N), the cluster's blocks share K and add up over distributed shared memory in the order of
+// their ranks; scaled in float32, rounded to bfloat16 (the operand type of the product that follows; 2^-8 of a term that
+// is itself a correction), zero where the token's adapter is another one.  Its bound is reading x once, from L2 behind the first chunk.
+//
+// adapter_pair_kernel is the product on pairs of SMs (256 x 256 tiles, cta_group::2, as gemm_tc2.cu: two blocks hold 128 token
+// rows and 128 weight rows each, persistent over the tiles, two accumulators in tensor memory).  A chunk is one more stage of
+// its ring: 128 rows of v (128-byte swizzle) and four boxes of [128 outputs x 16 ranks] of B (32-byte swizzle, laid out so
+// that a K step of 16 is one rank group of any adapter).  Few tiles: K is cut into slices, whose float32 sums a last kernel adds up.
+// It starts while the first kernel still runs: that one lets it go only when its own wait for the tokens' rows is over, so
+// the shared product may be read at once, and only the chunks wait.
+#include "adapters.cuh"
+#include "kernels.h"
+#include "tc_pair.cuh"
+
+#define AP_VALUE_STAGES 4
+#define AP_COLS (ADAPTER_CHUNK * ADAPTER_GROUP)        // columns of a chunk
+#define AP_PITCH (AP_COLS + 1)
+#define AP_STAGES 6
+#define AP_BN 256
+#define AP_HALF 128
+
+__device__ __forceinline__ float ap_load_remote(const float* local, unsigned rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(tc_smem_u32(local), rank)) : "memory");
+    return v;
+}
+
+// grid: cluster blocks of a half tile, halves, chunks, in this order along x
+__global__ void __launch_bounds__(TC_THREADS)
+adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scales, int R, int T,
+                      int C, int k_iters_total, const AdPlan plan, bf16* __restrict__ v, int* __restrict__ err) {
+    constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = AP_COLS * TC_BK * 2, BOX_BYTES = ADAPTER_GROUP * TC_BK * 2;
+    constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AP_COLS >> 3) << 17) | ((unsigned)(TC_BM >> 4) << 24);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * AP_VALUE_STAGES + 1];
+    __shared__ unsigned tmem_holder;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunk = (int)blockIdx.x / (2 * C), half = (int)blockIdx.x / C & 1;
+    const unsigned rank = cluster_ctarank();
+    if (chunk >= plan.counts[2]) return;                // the grid is sized for more chunks than there are (all blocks of the cluster leave)
+    const int t0 = plan.chunk_tile[chunk] * ADAPTER_TILE + half * TC_BM;
+
+    const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + AP_VALUE_STAGES * A_BYTES;
+    float* partial = reinterpret_cast<float*>(smem_raw + (a_base - tc_smem_u32(smem_raw)));     // [128][AP_PITCH] over the ring, when it is done
+    const unsigned full0 = tc_smem_u32(&bars[0]), empty0 = tc_smem_u32(&bars[AP_VALUE_STAGES]), done_bar = tc_smem_u32(&bars[2 * AP_VALUE_STAGES]);
+    const int per = (k_iters_total + C - 1) / C, k_begin = (int)rank * per, n_k = max(0, min(per, k_iters_total - k_begin));
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < AP_VALUE_STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(done_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(&tmem_holder)), "r"((unsigned)AP_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int row[ADAPTER_CHUNK], boxes = 0;
+#pragma unroll
+            for (int j = 0; j < ADAPTER_CHUNK; j++) {
+                const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + j];
+                row[j] = g < 0 ? -1 : (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
+                boxes += g >= 0;
+            }
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            // only now may the product begin: it reads the tokens' rows without a wait of its own
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            bool alive = true;
+            for (int i = 0; i < n_k && alive; i++) {
+                const int s = i % AP_VALUE_STAGES;
+                if (i >= AP_VALUE_STAGES) alive = mbar_wait(empty0 + 8 * s, ((i / AP_VALUE_STAGES) - 1) & 1, err);
+                if (!alive) break;
+                mbar_expect_tx(full0 + 8 * s, A_BYTES + boxes * BOX_BYTES);
+                const int kx = (k_begin + i) * TC_BK;
+                tma_load_2d(a_base + s * A_BYTES, &map_x, kx, t0, full0 + 8 * s);
+#pragma unroll
+                for (int j = 0; j < ADAPTER_CHUNK; j++)
+                    if (row[j] >= 0) tma_load_2d(b_base + s * B_BYTES + j * BOX_BYTES, &map_a, kx, row[j], full0 + 8 * s);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool alive = true;
+            for (int i = 0; i < n_k && alive; i++) {
+                const int s = i % AP_VALUE_STAGES;
+                alive = mbar_wait(full0 + 8 * s, (i / AP_VALUE_STAGES) & 1, err);
+                if (!alive) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < TC_BK / 16; kk++)
+                    umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
+                              (i > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(empty0 + 8 * s);
+            }
+            umma_commit(done_bar);
+        }
+    } else {
+        const int quad = warp & 3, r = quad * 32 + lane;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, err));
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < AP_COLS; c0 += 16) {
+            float f[16];
+            if (ok && n_k > 0) tmem_ld16(tmem + ((unsigned)(quad * 32) << 16) + (unsigned)c0, f);
+#pragma unroll
+            for (int j = 0; j < 16; j++) partial[r * AP_PITCH + c0 + j] = ok && n_k > 0 ? f[j] : 0.f;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                 // every block's sums are there
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)AP_COLS) : "memory");
+    }
+    // each block finishes its share of the rows, four columns a thread
+    const int rows = TC_BM / C;
+    for (int i = threadIdx.x; i < rows * (AP_COLS / 4); i += TC_THREADS) {
+        const int r = (int)rank * rows + i / (AP_COLS / 4), c = i % (AP_COLS / 4) * 4, t = t0 + r;
+        const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + c / ADAPTER_GROUP], ad = t < T ? plan.token_adapter[t] : -1;
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        if (g >= 0 && g / ADAPTER_MAX_GROUPS == ad) {
+            for (int b = 0; b < C; b++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) f[j] += ap_load_remote(&partial[r * AP_PITCH + c + j], b);
+            const float s = scales[ad];
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] *= s;
+        }
+        __nv_bfloat162 o[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+        *reinterpret_cast<uint2*>(v + ((size_t)chunk * ADAPTER_TILE + half * TC_BM + r) * AP_COLS + c) = *reinterpret_cast<uint2*>(o);
+    }
+    cluster_sync_all();                                 // no block leaves while another may still read its sums
+}
+
+// Descriptor of a K-major tile whose rows are 32 bytes, 32-byte swizzled: 8-row groups 256 bytes apart.
+__device__ __forceinline__ unsigned long long umma_desc_sw32(unsigned smem_addr) {
+    return (unsigned long long)((smem_addr & 0x3FFFF) >> 4) | (1ull << 16) | ((unsigned long long)(256 >> 4) << 32) | (1ull << 46) | (6ull << 61);
+}
+
+// C = x . W^T + the chunks.  splits > 1: C is float32 [splits, T, N], slice z the z-th run of K pieces, the last with the chunks.
+template <typename TOut>
+__global__ void __launch_bounds__(TC_THREADS)
+adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_b, TOut* __restrict__ C, int T, int N, int R, int k_iters_total, int splits, const AdPlan plan,
+                    int chunked, int* __restrict__ err) {
+    constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = AP_HALF * TC_BK * 2, BOX_BYTES = AP_HALF * ADAPTER_GROUP * 2;
+    constexpr unsigned TMEM_COLS = 512;
+    constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AP_BN >> 3) << 17) | ((unsigned)(256 >> 4) << 24);
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const unsigned base = tc_smem_u32(smem_raw);
+    const unsigned a_base = base, b_base = a_base + AP_STAGES * A_BYTES;
+    const unsigned bars = b_base + AP_STAGES * B_BYTES;
+    const unsigned full0 = bars, empty0 = bars + 8 * AP_STAGES;
+    const unsigned acc_full0 = bars + 16 * AP_STAGES, acc_empty0 = acc_full0 + 16;
+    unsigned* tmem_holder = reinterpret_cast<unsigned*>(smem_raw + (bars - base) + 16 * AP_STAGES + 32);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int n_m = (T + 255) / 256, n_tiles = n_m * ((N + AP_BN - 1) / AP_BN), n_items = n_tiles * splits;
+    const int per = (k_iters_total + splits - 1) / splits;
+
+    if ((base & 1023u) != 0) {          // no static shared memory is declared: cannot happen; never run misaligned
+        if (threadIdx.x == 0) atomicExch(err, TC_ERR_MISALIGNED_SMEM);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < AP_STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(acc_full0 + 8 * b, 1);
+            mbar_init(acc_empty0 + 8 * b, 8);      // four epilogue warps in each of the two blocks
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(tmem_holder)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                 // the peer's barriers exist before anything arrives on them
+    tc_fence_after();
+    const unsigned tmem = *tmem_holder;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // item -> its tile, its run of K pieces and its chunks
+    auto item = [&](int i, int& m, int& n, int& k0, int& k1, int& c0, int& c1) {
+        const int z = i / n_tiles, t = i - z * n_tiles;
+        m = t % n_m, n = t / n_m;
+        k0 = z * per, k1 = min(k_iters_total, k0 + per);
+        c0 = c1 = 0;
+        if (chunked && z == splits - 1) c0 = plan.tile_chunk[m], c1 = plan.tile_chunk[m + 1];
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            bool alive = true, waited = false;
+            int it = 0;
+            const unsigned full_leader = map_to_cta(full0, 0);      // block 0 counts the bytes of both
+            if (!chunked) asm volatile("griddepcontrol.wait;" ::: "memory");       // no kernel of ours has waited for the tokens' rows
+            for (int i = pair; i < n_items && alive; i += n_pairs) {
+                int m, n, k0, k1, c0, c1;
+                item(i, m, n, k0, k1, c0, c1);
+                const int ra0 = m * 256 + (int)rank * 128, rb0 = n * AP_BN + (int)rank * AP_HALF;
+                for (int k = k0; k < k1 + (c1 - c0); k++, it++) {
+                    const int s = it % AP_STAGES;
+                    if (it >= AP_STAGES) alive = mbar_wait(empty0 + 8 * s, ((it / AP_STAGES) - 1) & 1, err);
+                    if (!alive) break;
+                    if (k < k1) {
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + B_BYTES));
+                        tma_load_2d_pair(b_base + s * B_BYTES, &map_w, k * TC_BK, rb0, full_leader + 8 * s);
+                        tma_load_2d_pair(a_base + s * A_BYTES, &map_x, k * TC_BK, ra0, full_leader + 8 * s);
+                    } else {
+                        const int c = c0 + (k - k1);
+                        int g[ADAPTER_CHUNK], boxes = 0;
+#pragma unroll
+                        for (int j = 0; j < ADAPTER_CHUNK; j++) {
+                            g[j] = plan.chunk_groups[c * ADAPTER_CHUNK + j];
+                            boxes += g[j] >= 0;
+                        }
+                        if (!waited) {
+                            asm volatile("griddepcontrol.wait;" ::: "memory");     // the values are there
+                            waited = true;
+                        }
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + boxes * BOX_BYTES));
+                        tma_load_2d_pair(a_base + s * A_BYTES, &map_v, 0, c * ADAPTER_TILE + (int)rank * 128, full_leader + 8 * s);
+#pragma unroll
+                        for (int j = 0; j < ADAPTER_CHUNK; j++)
+                            if (g[j] >= 0) {
+                                const int row = ((g[j] / ADAPTER_MAX_GROUPS) * (R / ADAPTER_GROUP) + g[j] % ADAPTER_MAX_GROUPS) * N + rb0;
+                                tma_load_2d_pair(b_base + s * B_BYTES + j * BOX_BYTES, &map_b, 0, row, full_leader + 8 * s);
+                            }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            bool alive = true;
+            int it = 0, ti = 0;
+            for (int i = pair; i < n_items && alive; i += n_pairs, ti++) {
+                int m, n, k0, k1, c0, c1;
+                item(i, m, n, k0, k1, c0, c1);
+                const int buf = ti & 1;
+                if (ti >= 2) alive = mbar_wait(acc_empty0 + 8 * buf, ((ti >> 1) - 1) & 1, err);
+                tc_fence_after();
+                for (int k = k0; k < k1 + (c1 - c0) && alive; k++, it++) {
+                    const int s = it % AP_STAGES;
+                    alive = mbar_wait(full0 + 8 * s, (it / AP_STAGES) & 1, err);
+                    if (!alive) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < TC_BK / 16; kk++) {
+                        const unsigned long long da = umma_desc_sw128(a_base + s * A_BYTES + kk * 32);
+                        if (k < k1)
+                            umma_bf16_pair(tmem + buf * AP_BN, da, umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC, (k > k0 || kk > 0) ? 1u : 0u);
+                        else if (plan.chunk_groups[(c0 + k - k1) * ADAPTER_CHUNK + kk] >= 0)
+                            umma_bf16_pair(tmem + buf * AP_BN, da, umma_desc_sw32(b_base + s * B_BYTES + kk * BOX_BYTES), IDESC, 1u);
+                    }
+                    umma_commit_pair(empty0 + 8 * s);
+                }
+                umma_commit_pair(acc_full0 + 8 * buf);
+            }
+        }
+    } else {
+        const int quad = warp & 3;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const unsigned acc_empty_leader = map_to_cta(acc_empty0, 0);
+        bool alive = true;
+        int ti = 0;
+        for (int i = pair; i < n_items && alive; i += n_pairs, ti++) {
+            int m, n, k0, k1, c0, c1;
+            item(i, m, n, k0, k1, c0, c1);
+            const int buf = ti & 1, ra = m * 256 + (int)rank * 128 + quad * 32 + lane, rb0 = n * AP_BN;
+            TOut* Cz = C + (size_t)(i / n_tiles) * T * N;
+            // lanes leave the polling loop one by one: together again before the warp-wide tcgen05.ld
+            alive = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (ti >> 1) & 1, err));
+            if (!alive) break;
+            tc_fence_after();
+            const unsigned tbase = tmem + ((unsigned)(quad * 32) << 16) + (unsigned)(buf * AP_BN);
+#pragma unroll 1
+            for (int c = 0; c < AP_BN; c += 16) {
+                if (rb0 + c >= N) break;
+                float v[16];
+                tmem_ld16(tbase + c, v);
+                if (ra < T) {
+                    TOut* dst = Cz + (size_t)ra * N + rb0 + c;
+                    if (rb0 + c + 16 <= N && ((N & 7) == 0)) {
+                        store8(dst, v);
+                        store8(dst + 8, v + 8);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (rb0 + c + j < N) store_out<TOut>(dst + j, v[j]);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8 * buf);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                 // neither block leaves while the other may still touch it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// ---- host side
+
+// Slices of K: as many as there are pairs of SMs for the tiles, each of at least 16 pieces, at most 4.
+static int ap_splits(int T, int N, int K) {
+    const int tiles = ad_div(T, 256) * ad_div(N, AP_BN), k_iters = ad_div(K, TC_BK);
+    int s = illm_sm_count() / 2 / tiles;
+    s = s > k_iters / 16 ? k_iters / 16 : s;
+    s = s > 4 ? 4 : (s < 1 ? 1 : s);
+    return ad_div(k_iters, ad_div(k_iters, s));
+}
+long long ad_prompt_ws(int T, int N, int K, int chunks) {
+    const int s = ap_splits(T, N, K);
+    return ad_round((long long)chunks * ADAPTER_TILE * AP_COLS * 2) + (s > 1 ? (long long)s * T * N * 4 : 0);
+}
+
+template <typename TOut>
+static int ap_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mv, const CUtensorMap& mb, TOut* out, int T, int N, int R, int k_iters,
+                          int splits, const AdPlan& plan, int chunked, int* err, cudaStream_t s) {
+    const size_t smem = (size_t)AP_STAGES * (TC_BM + AP_HALF) * TC_BK * 2 + 16 * AP_STAGES + 32 + 16;
+    auto kern = adapter_pair_kernel<TOut>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    const int items = ad_div(T, 256) * ad_div(N, AP_BN) * splits, most = illm_sm_count() / 2, pairs = items < most ? items : most;
+    return illm_launch_cluster(kern, dim3(2 * pairs), dim3(TC_THREADS), 2, smem, s, mx, mw, mv, mb, out, T, N, R, k_iters, splits, plan, chunked, err);
+}
+
+int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R,
+                   const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int early, int* err, cudaStream_t s) {
+    (void)early;
+    const int k_iters = ad_div(K, TC_BK), splits = ap_splits(T, N, K);
+    bf16* v = (bf16*)ws;
+    float* slices = (float*)(ws + ad_round((long long)chunks * ADAPTER_TILE * AP_COLS * 2));
+    CUtensorMap mx, ma, mw, mv, mb;
+    int rc;
+    if ((rc = ad_make_map(&mx, x, T, K, TC_BM)) || (rc = ad_make_map(&mw, w, N, K, AP_HALF))) return rc;
+    mv = mb = mx;
+    if (chunks > 0) {
+        if ((rc = ad_make_map(&ma, a, (long long)count * R, K, ADAPTER_GROUP)) || (rc = ad_make_map(&mv, v, (long long)chunks * ADAPTER_TILE, AP_COLS, TC_BM)) ||
+            (rc = ad_make_map(&mb, b, (long long)count * (R / ADAPTER_GROUP) * N, ADAPTER_GROUP, AP_HALF, ADAPTER_GROUP, CU_TENSOR_MAP_SWIZZLE_32B)))
+            return rc;
+        // as many blocks share a chunk's K as bring about two blocks to an SM
+        int C = 1;
+        while (C < 8 && chunks * 2 * C * 2 <= 2 * illm_sm_count() && k_iters >= 4 * C) C *= 2;
+        const size_t smem = (size_t)AP_VALUE_STAGES * (TC_BM + AP_COLS) * TC_BK * 2 + 1024;
+        cudaError_t e = cudaFuncSetAttribute(adapter_values_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        rc = illm_launch_cluster(adapter_values_kernel, dim3((unsigned)C * 2 * chunks), dim3(TC_THREADS), C, smem, s, mx, ma, scales, R, T, C, k_iters, plan, v, err);
+        if (rc) return rc;
+    }
+    if (splits > 1) {
+        rc = ap_launch_pair<float>(mx, mw, mv, mb, slices, T, N, R, k_iters, splits, plan, chunks > 0, err, s);
+        return rc ? rc : illm_splitk_reduce(slices, out, out_dtype, (long long)T * N, splits, s);
+    }
+    if (out_dtype == ILLM_BF16) return ap_launch_pair<bf16>(mx, mw, mv, mb, (bf16*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
+    return ap_launch_pair<float>(mx, mw, mv, mb, (float*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
+}

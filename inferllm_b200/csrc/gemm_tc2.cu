@@ -23,51 +23,12 @@
 // silu(gate) * up (formula src/kern/naive/naive.cpp:80-89; the reference runs w3, w1, Silu and Mul
 // as four operators, src/core/graph.cpp:57-79), so the packed projection never goes to memory.
 // Every wait is bounded and raises the error word.
-#include "tc_common.cuh"
+#include "tc_pair.cuh"
 
 #define T2_BN 256
 #define T2_HALF 128
 #define T2_STAGES 6
 #define T2_THREADS 192
-
-__device__ __forceinline__ unsigned cluster_ctarank() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// address of the same shared-memory location in block `rank` of the cluster
-__device__ __forceinline__ unsigned map_to_cta(unsigned addr, unsigned rank) {
-    unsigned out;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-    return out;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(unsigned cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// TMA load into this block's shared memory whose completion is counted on `bar`, a barrier of
-// either block of the pair given by its cluster address
-__device__ __forceinline__ void tma_load_2d_pair(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void umma_bf16_pair(unsigned tmem_d, unsigned long long da, unsigned long long db,
-                                               unsigned idesc, unsigned accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
-}
-// arrives, when the MMAs issued so far are done, on the barrier at this offset in both blocks
-__device__ __forceinline__ void umma_commit_pair(unsigned bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(bar), "h"((unsigned short)3) : "memory");
-}
 
 // the activation of a gated epilogue: EPI 1 silu, 2 relu, 3 tanh-form gelu
 template <int EPI> __device__ __forceinline__ float t2_gate_act(float g) {

@@ -210,7 +210,7 @@ int illm_moe_gemm_split(const void* x, int x_dtype, const void* w, int w_dtype, 
 
 // adapters.cu
 long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int groups, int chunks);
-int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int* err, void* stream);
+int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int early, int* err, void* stream);
 
 // sample_rows.cu
 int illm_sample_rows(const void* logits, int dtype, int B, int V, long long ld, const float* uniforms, const float* temp, const int* top_k, const float* top_p, const float* min_p, int* out, void* stream);

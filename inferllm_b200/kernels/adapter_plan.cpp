@@ -32,7 +32,7 @@ AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, i
         s.slots++;
         s.groups += groups_of(ranks[a]);
     }
-    if (T > kAdapterRowsMaxTokens)
+    if (T > ADAPTER_ROWS_MAX)
         for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE) {
             int g = 0;
             for (int a : named(index, t0, tile_end(t0, T))) g += groups_of(ranks[a]);
@@ -44,7 +44,7 @@ AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, i
 AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool tiles) {
     const int slots = tiles ? std::min(1, T) : std::min(T, count);
     AdapterPlanSizes s{T, slots, slots * groups_of(max_rank), 0};
-    if (tiles && T > kAdapterRowsMaxTokens)
+    if (tiles && T > ADAPTER_ROWS_MAX)
         s.chunks = (T + ADAPTER_TILE - 1) / ADAPTER_TILE * ((groups_of(max_rank) + ADAPTER_CHUNK - 1) / ADAPTER_CHUNK);
     return s;
 }
@@ -77,7 +77,14 @@ void adapter_plan_fill(const int* index, int T, const int* ranks, int count, con
     begin[slots.size() + 1] = T;
     out[l.slot_group + slots.size() + 1] = g;
     std::vector<int> next(begin, begin + slots.size() + 1);
-    for (int t = 0; t < T; t++) out[l.order + next[(size_t)slot(t)]++] = t;
+    for (int t = 0; t < T; t++) {
+        const int i = slot(t), place = next[(size_t)i]++;
+        int* rec = out + l.places + 4 * place;
+        out[l.order + place] = rec[0] = t;
+        rec[1] = index[t];
+        rec[2] = out[l.slot_group + i];
+        rec[3] = out[l.slot_group + i + 1] - rec[2];
+    }
     int chunks = 0, tile = 0;
     if (sizes.chunks > 0) {
         for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE, tile++) {

@@ -7,9 +7,6 @@
 namespace illm {
 namespace ops {
 
-// Tokens up to which the rows form of the product runs; above it the plan has tiles.
-constexpr int kAdapterRowsMaxTokens = 64;
-
 // The smallest sizes that hold the plan of these tokens.  index[t] is a token's adapter, -1 for none; ranks[a] the rank of
 // adapter a.  KernelError for an index outside the adapters, a rank outside [0, 256] or too many tokens.
 AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, int count);

@@ -10,6 +10,7 @@ policy functions here ask it, so the choices tested are the ones that run.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -81,7 +82,7 @@ _KERNEL_SIGNATURES = {
     "illm_sample": [P_, I_, I_, I_, P_, P_, I_, F_, F_, I_, F_, P_, P_, P_, P_],
     "illm_sample_scratch_elems": [I_, I_, I_, F_],
     "illm_linear_adapters_ws": [I_, I_, I_, I_, I_, I_, I_],
-    "illm_linear_adapters": [P_, P_, I_, I_, I_, I_, P_, P_, P_, I_, I_, P_, I_, I_, I_, P_, I_, P_, P_, P_],
+    "illm_linear_adapters": [P_, P_, I_, I_, I_, I_, P_, P_, P_, I_, I_, P_, I_, I_, I_, P_, I_, P_, I_, P_, P_],
     "illm_sample_rows": [P_, I_, I_, I_, LL_, P_, P_, P_, P_, P_, P_, P_],
     "illm_fill_random": [P_, I_, LL_, ctypes.c_ulonglong, F_, F_, P_],
     "illm_poison_pages": [P_, P_, LL_, I_, LL_, P_, I_, P_],
@@ -805,6 +806,8 @@ class Adapters:
             raise KernelError(f"adapters: the inner size {n_in} must be a multiple of 8 in bfloat16")
         self.count, self.rank, self.n_out, self.n_in, self.dtype = count, rank, n_out, n_in, dtype
         self.R = -(-rank // ADAPTER_GROUP) * ADAPTER_GROUP
+        if count * self.R * (n_out // ADAPTER_GROUP + 1) >= 2 ** 31:
+            raise KernelError(f"adapters: {count} adapters of {n_out} outputs and rank {self.R} have more than 2^31 rows")
         self.device = torch.empty(0, device="cuda" if device is None else device).device
         if self.device.type != "cuda":
             raise KernelError("adapters live on a CUDA device: inferllm_b200 has no CPU path")
@@ -815,7 +818,7 @@ class Adapters:
 
     def put(self, i, a, b, scale=1.0):
         """Adapter i becomes scale * b a (a [r, n_in], b [n_out, r], any float type); what it was is gone.  Works on torch's
-        current stream, like any torch operation.  A plan made before an adapter got a larger rank is refused."""
+        current stream, like any torch operation, and looks at the numbers, which have to be finite in the adapters' type.  A plan made before an adapter got a larger rank is refused."""
         if not 0 <= i < self.count:
             raise KernelError(f"adapters: there is no adapter {i} among {self.count}")
         if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.n_in or b.shape[0] != self.n_out or a.shape[0] != b.shape[1]:
@@ -825,13 +828,17 @@ class Adapters:
             raise KernelError(f"adapters: rank {r} exceeds the {self.rank} there is room for")
         if not (a.is_floating_point() and b.is_floating_point()):
             raise KernelError("adapters: the factors must be floating-point tensors")
+        a, b, scale = a.to(self.device, self.dtype), b.to(self.device, self.dtype), float(scale)
+        # (the prompt product multiplies an adapter's b with the zeros of its neighbours' tokens)
+        if not (math.isfinite(scale) and bool(a.isfinite().all()) and bool(b.isfinite().all())):
+            raise KernelError(f"adapters: adapter {i} is not finite in {self.dtype}")
         self.a[i].zero_()
         self.a[i, :r] = a
         self.b[i].zero_()
         for g in range(0, r, ADAPTER_GROUP):
             e = min(r, g + ADAPTER_GROUP)
             self.b[i, g // ADAPTER_GROUP, :, :e - g] = b[:, g:e]
-        self.scales[i] = float(scale)
+        self.scales[i] = scale
         self.ranks[i] = r
 
     def remove(self, i):
@@ -891,7 +898,7 @@ def linear_adapters(x, w, adapters, rows, out_dtype=None):
     with _on(x.device):
         _check(lib.illm_linear_adapters(x.data_ptr(), w.data_ptr(), dtype, T, N, K, adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scales.data_ptr(),
                                         adapters.count, adapters.R, rows.plan.data_ptr(), rows.slots, rows.groups, rows.chunks, out.data_ptr(), out_code,
-                                        ws.data_ptr(), _error_word(x.device), _stream()), "linear_adapters")
+                                        ws.data_ptr(), 0, _error_word(x.device), _stream()), "linear_adapters")
     return out
 
 

@@ -20,7 +20,7 @@ def plan(index, ranks):
 def unpack(index, ranks):
     (T, slots, groups, chunks), out = plan(index, ranks)
     at, fields = 0, {}
-    for name, n in (("counts", 4), ("token_adapter", T), ("order", T), ("slot_begin", slots + 2), ("slot_adapter", slots + 1), ("slot_group", slots + 2),
+    for name, n in (("counts", 4), ("token_adapter", T), ("order", T), ("places", 4 * T), ("slot_begin", slots + 2), ("slot_adapter", slots + 1), ("slot_group", slots + 2),
                     ("groups", groups), ("tile_chunk", -(-T // 256) + 1), ("chunk_tile", chunks), ("chunk_groups", chunks * 4)):
         fields[name] = out[at:at + n]
         at += -(-n // 4) * 4
@@ -38,7 +38,7 @@ def test_every_token_and_every_rank_group_once(T, count):
     named = sorted(set(index) - {-1})
     g_of = lambda a: -(-ranks[a] // 16)  # noqa: E731
     assert slots == len(named) and f["slot_adapter"] == named + [-1]
-    assert f["counts"] == [slots, groups, chunks if T > 64 else 0, max([g_of(a) for a in named], default=0)]
+    assert f["counts"] == [slots, groups, chunks if T > 256 else 0, max([g_of(a) for a in named], default=0)]
     assert f["token_adapter"] == index and sorted(f["order"]) == list(range(T))
     assert f["slot_begin"][-1] == T
     for i, a in enumerate(f["slot_adapter"]):
@@ -46,7 +46,10 @@ def test_every_token_and_every_rank_group_once(T, count):
         assert tokens == [t for t in range(T) if index[t] == a]
         mine = f["groups"][f["slot_group"][i]:f["slot_group"][i + 1]]
         assert mine == ([a * 16 + g for g in range(g_of(a))] if a >= 0 else [])
-    if T <= 64:
+    for place, t in enumerate(f["order"]):
+        slot = max(i for i in range(slots + 1) if f["slot_begin"][i] <= place < f["slot_begin"][i + 1])
+        assert f["places"][4 * place:4 * place + 4] == [t, index[t], f["slot_group"][slot], g_of(index[t]) if index[t] >= 0 else 0]
+    if T <= 256:
         assert chunks == 0
         return
     for tile in range(-(-T // 256)):

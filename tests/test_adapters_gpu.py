@@ -108,13 +108,14 @@ def test_no_adapter_is_the_product():
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_token_does_not_depend_on_adapters_of_others(dtype):
-    """Infinities and NaN in another token's row or adapter stay there."""
+    """Infinities and NaN in another token's row stay there, and so does an adapter whose values overflow; one that is not
+    finite itself is refused."""
     for T in (6, 64, 200, 300):
         x, w, a, b, ad, s = make(T, 320, 272, [16, 32, 8], dtype, T)
         index = [(t * 7) % 4 - 1 for t in range(T)]
         rows = ops.AdapterRows(index, ad.ranks)
         want = ops.linear_adapters(x, w, ad, rows)
-        a[1][0, 3], b[1][5, 2] = float("inf"), float("nan")
+        a[1][0] = 3e38
         ad.put(1, a[1], b[1], s[1])
         bad = [t for t in range(T) if index[t] == 1]
         clean = next(t for t in range(T) if index[t] == 0)
@@ -191,6 +192,8 @@ def test_refusals():
            lambda: ops.linear_adapters(x, w, ad, ops.AdapterRows([0, 1, -1, 0], [8, 0])),
            lambda: ad.put(2, a[0], b[0]), lambda: ad.put(0, a[0][:, :32], b[0]), lambda: ad.put(0, a[0], b[0][:, :4]),
            lambda: ad.put(0, torch.zeros(9, 64), torch.zeros(32, 9)), lambda: ad.put(0, a[0].int(), b[0]),
+           lambda: ad.put(0, a[0] * float("inf"), b[0]), lambda: ad.put(0, a[0], b[0] * float("nan")), lambda: ad.put(0, a[0], b[0], float("inf")),
+           lambda: ad.put(0, a[0].double() * 1e39, b[0]),
            lambda: ops.Adapters(0, 8, 32, 64), lambda: ops.Adapters(2, 257, 32, 64), lambda: ops.Adapters(2, 8, 32, 60),
            lambda: ops.Adapters(2, 8, 32, 64, torch.float16), lambda: ops.Adapters(2, 8, 32, 64, device="cpu"),
            lambda: ops.AdapterRows([0, 2], [8, 8]), lambda: ops.AdapterRows([-2], [8]), lambda: ops.AdapterRows([0], [300])]
