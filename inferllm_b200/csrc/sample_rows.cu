@@ -18,8 +18,8 @@
 // 2^-50) and rounded to integers in units of 2^-S with S = 62 - log2 V (at most 50): sums of integers are the same in
 // every order, and are off by at most V / 2 units of 2^-S, in the mean sqrt(V) / 4 of them.
 //
-// One launch, a cluster of blocks per row: every block keeps its run of the row in shared memory (the row is read once; rows
-// too long for that are read again where they are needed), and the blocks exchange sums through distributed shared memory.
+// One launch, a cluster of blocks per row: every block keeps its run of the row in shared memory (the row is read once), and the
+// blocks exchange sums through distributed shared memory.
 //   1. the largest word.  T <= 0 ends here.
 //   2. a cut: a histogram over 2048 bins of the distance m - l (128 bins to an octave from 2^-8 to 2^8, whatever the
 //      temperature: the bins are only a partition that keeps the order), of counts for top_k and of weights for top_p; each
@@ -87,7 +87,7 @@ struct __align__(16) SrShared {
     u64 warp_sum[SR_WARPS];
     struct { unsigned count[256], lo[256], hi[256]; } digits[2];
     union {
-        struct { unsigned lo[SR_BINS], hi[SR_BINS]; };  // histogram: a sum's halves, or a count in lo
+        unsigned part[3][SR_BINS];                      // histogram: a sum's bits in three parts, or a count in the first
         struct { float value[SR_LIST]; int id[SR_LIST]; };      // the first block's list
     };
 };
@@ -109,9 +109,12 @@ struct SrRow {
 // A float as a double by integer instructions: the conversion instruction does 16 of them per clock and SM, a quarter of the rate
 // of the float64 arithmetic behind it, and was what bound the sums.
 __device__ __forceinline__ double sr_double(float f) {
-    const unsigned b = __float_as_uint(f);
-    if ((b & 0x7f800000u) == 0u) return (double)f;      // zero, subnormal
-    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29));
+    const unsigned b = __float_as_uint(f), sign = b & 0x80000000u, high = b & 0x7fffffffu;
+    // zero and subnormals have no leading one: it is added with the smallest normal exponent and taken off again
+    const bool small = high < 0x00800000u;
+    const unsigned e = small ? 897u << 20 : 896u << 20;
+    const double off = __hiloint2double((int)(small ? sign | (897u << 20) : 0u), 0);
+    return __hiloint2double((int)(sign | ((high >> 3) + e)), (int)(b << 29)) - off;
 }
 // w of a word that can come, in units of 2^-S; 0 as well if it is below min_p (CUT).  With x = 16 (l - m) log2(e) / T = j + f, |f| <= 1/2:
 // w = 2^(j / 16) exp(f ln2 / 16); the table's 16 entries lie in 32 different banks, and the series' first term left out is
@@ -139,7 +142,8 @@ __device__ __forceinline__ u64 sr_weight(const SrRow& r, const double* table, fl
     if (x < -1024.0) units = 0ull;                      // less than 2^-64
     return l == r.max_value ? r.one : units;
 }
-__device__ __forceinline__ bool sr_kept(const SrRow& r, float l, int id) { return l > r.cut || (l == r.cut && id <= r.cut_id); }
+// whether a word can come and is still kept (no branch: the loops over the row are bound by how many of their loads and chains overlap)
+__device__ __forceinline__ bool sr_kept(const SrRow& r, float l, int id) { return (l > r.low) & ((l > r.cut) | ((l == r.cut) & (id <= r.cut_id))); }
 
 // sum over the warp by three 32-bit reductions of 22 bits each (32 of them stay below 2^27)
 __device__ __forceinline__ u64 sr_warp_sum(u64 v) {
@@ -202,12 +206,14 @@ __device__ __forceinline__ u64 sr_block_before(SrShared& sh, u64 v, u64& whole) 
     return before;
 }
 
-// A list of at most SR_LIST words in ascending order of their id, dealt to the block's threads in runs: word tid * per + e.
+// A list of at most SR_LIST words in ascending order of their id, dealt to the block's threads in runs: word w.at + e.
 // order: key above the list's smallest key, and below it the complement of the place: larger means earlier in the row's order.
 struct SrList {
-    u64 order[SR_PER];
-    float l[SR_PER];
-    int n;                  // words of this thread
+    unsigned key[SR_PER];   // above the list's smallest
+    unsigned least;         // that one
+    int n, at;              // words of this thread, place of the first
+    __device__ __forceinline__ u64 order(int e) const { return ((u64)key[e] << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - at - e); }
+    __device__ __forceinline__ float value(int e) const { return sr_value(key[e] + least); }
 };
 // The cut of the shortest prefix, largest order first, whose measure (m[e] of word e) reaches `target`, which all of them do: kept
 // are the words with order >= the result, and `last` is the smallest of them.  Digit by digit, 8 bits at a time, until a digit
@@ -223,8 +229,8 @@ __device__ __forceinline__ u64 sr_list_cut(SrShared& sh, const SrList& w, const 
         const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
 #pragma unroll
         for (int e = 0; e < SR_PER; e++)
-            if (e < w.n && m[e] != 0ull && (shift == 64 ? 0ull : w.order[e] >> shift) == prefix) {
-                const int d = (int)(w.order[e] >> down) & ((1 << width) - 1);
+            if (e < w.n && m[e] != 0ull && w.order(e) >> shift == prefix) {
+                const int d = (int)(w.order(e) >> down) & ((1 << width) - 1);
                 const unsigned low = (unsigned)m[e], carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
                 if ((unsigned)(m[e] >> 32) + carry != 0u) atomicAdd(&hi[d], (unsigned)(m[e] >> 32) + carry);
                 atomicAdd(&count[d], 1u);
@@ -267,14 +273,15 @@ __device__ __forceinline__ u64 sr_draw_target(float u, u64 total) {
     return t < total ? t : total - 1;
 }
 
-template <typename TIn, bool RESIDENT>
+template <typename TIn>
 __global__ void __launch_bounds__(SR_THREADS, 2)
-sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chunk, int C, int S, const float* __restrict__ uniforms,
+sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chunk, int C, int S, int part_bits, const float* __restrict__ uniforms,
                    const float* __restrict__ temps, const int* __restrict__ top_ks, const float* __restrict__ top_ps,
                    const float* __restrict__ min_ps, int* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char sr_smem[];
     SrShared& sh = *reinterpret_cast<SrShared*>(sr_smem);
     float* resident = reinterpret_cast<float*>(sr_smem + sizeof(SrShared));
+    unsigned* taken_mask = reinterpret_cast<unsigned*>(resident + chunk);       // a bit per word
     pdl_grid_sync();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned rank = C > 1 ? sr_rank() : 0;
@@ -287,7 +294,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     int turn = 0;
     const float temp = temps ? temps[row] : 1.0f, top_p = top_ps ? top_ps[row] : 1.0f, min_p = min_ps ? min_ps[row] : 0.f, u = uniforms[row];
     const int top_k = top_ks ? top_ks[row] : 0;
-    auto value = [&](int i) { return RESIDENT ? resident[i] : to_f32(src[first + i]); };
+    auto value = [&](int i) { return resident[i]; };
 
     // 1. the row and its largest word
     float top = -INFINITY;
@@ -301,14 +308,13 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             else *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(src + first + i);
 #pragma unroll
             for (int e = 0; e < W; e++) top = fmaxf(top, f[e]);
-            if (RESIDENT)
 #pragma unroll
                 for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(resident + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
         }
 #pragma unroll 4
         for (int i = whole + tid; i < n; i += SR_THREADS) {
             const float f = to_f32(src[first + i]);
-            if (RESIDENT) resident[i] = f;
+            resident[i] = f;
             top = fmaxf(top, f);                        // (the other one of a NaN)
         }
     }
@@ -384,7 +390,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             u64 mine = 0;
             for (int i = tid; i < n; i += SR_THREADS) {
                 const float l = value(i);
-                if (l > r.low && sr_kept(r, l, first + i)) {
+                if (sr_kept(r, l, first + i)) {
                     const unsigned k = sr_key(l);
                     if (k >= mid && k < hi) mine += measure(l);
                 }
@@ -408,73 +414,83 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     // The kept words that `pick` takes, in ascending order of their id, into the first block's list; how many there are.  More
     // than the list holds: nothing is written.
     auto gather = [&](auto pick) {
-        auto taken = [&](int i) {
-            if (i >= s1) return false;
-            const float l = value(i);
-            return l > r.low && sr_kept(r, l, first + i) && pick(l);
-        };
         unsigned count = 0;
 #pragma unroll 4
-        for (int i = s0; i < s1; i += 32) count += __popc(__ballot_sync(0xffffffffu, taken(i + lane)));
+        for (int i = s0; i < s1; i += 32) {
+            const float l = i + lane < s1 ? value(i + lane) : -INFINITY;
+            const unsigned all = __ballot_sync(0xffffffffu, sr_kept(r, l, first + i + lane) & pick(l));
+            count += __popc(all);
+            if (lane == 0) taken_mask[i >> 5] = all;
+        }
         const u64 block = sr_block_sum(sh, lane == 0 ? count : 0u);
         unsigned at = 0, total = 0;
-        for (int q = 0; q < warp; q++) at += (unsigned)sh.warp_sum[q];
+#pragma unroll
+        for (int q = 0; q < SR_WARPS; q++) at += q < warp ? (unsigned)sh.warp_sum[q] : 0u;
         const u64* e = sr_exchange(sh, turn, block, C, rank);
         for (int c = 0; c < C; c++) {
             if (c < (int)rank) at += (unsigned)e[c];
             total += (unsigned)e[c];
         }
         if (total > SR_LIST) return total;
-        if (count != 0)
-            for (int i = s0; i < s1; i += 32) {
-                const bool t = taken(i + lane);
-                const unsigned all = __ballot_sync(0xffffffffu, t);
-                if (t) {
-                    const int to = at + __popc(all & ((1u << lane) - 1u));
-                    sr_store_remote(&sh.value[to], 0, __float_as_uint(value(i + lane)));
-                    sr_store_remote(&sh.id[to], 0, (unsigned)(first + i + lane));
-                }
-                at += __popc(all);
+        // a lane per 32 words
+        for (int i0 = s0; i0 < s1 && count != 0; i0 += 1024) {
+            const int i = i0 + lane * 32;
+            unsigned mask = i < s1 ? taken_mask[i >> 5] : 0u;
+            const unsigned mine = __popc(mask);
+            unsigned run = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += v;
             }
+            unsigned to = at + run - mine;
+            at += __shfl_sync(0xffffffffu, run, 31);
+            for (; mask; mask &= mask - 1, to++) {
+                const int k = i + __ffs(mask) - 1;
+                sr_store_remote(&sh.value[to], 0, __float_as_uint(value(k)));
+                sr_store_remote(&sh.id[to], 0, (unsigned)(first + k));
+            }
+        }
         sr_cluster_sync();
         return total;
     };
     // the first block's list in its registers; `bits` how many of an order's bits differ among them
-    auto take_list = [&](SrList& w, int words, int& per, int& bits) {
-        per = (words + SR_THREADS - 1) / SR_THREADS;
-        w.n = max(0, min(per, words - tid * per));
+    auto take_list = [&](SrList& w, int words, int& bits) {
+        const int per = (words + SR_THREADS - 1) / SR_THREADS;
+        w.at = tid * per;
+        w.n = max(0, min(per, words - w.at));
         unsigned most = 0, least = 0;                   // the smallest key's complement
 #pragma unroll
         for (int e = 0; e < SR_PER; e++)
             if (e < w.n) {
-                w.l[e] = sh.value[tid * per + e];
-                const unsigned k = sr_key(w.l[e]);
-                most = max(most, k);
-                least = max(least, ~k);
+                w.key[e] = sr_key(sh.value[w.at + e]);
+                most = max(most, w.key[e]);
+                least = max(least, ~w.key[e]);
             }
         most = sr_block_max(sh, most);
-        least = ~sr_block_max(sh, least);
+        w.least = ~sr_block_max(sh, least);
 #pragma unroll
-        for (int e = 0; e < SR_PER; e++)
-            if (e < w.n) w.order[e] = ((u64)(sr_key(w.l[e]) - least) << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - (tid * per + e));
-        bits = 64 - __clzll(((u64)(most - least) << SR_LIST_BITS) | (SR_LIST - 1));
+        for (int e = 0; e < SR_PER; e++) w.key[e] -= w.least;
+        bits = 64 - __clzll(((u64)(most - w.least) << SR_LIST_BITS) | (SR_LIST - 1));
     };
     // Histogram of the kept words by bins.  Finds the bin in which the sum of measure reaches target_of(whole sum); `above` is the
     // sum over the bins before it.  false if the whole does not reach the target.
     auto bin_of = [&](auto target_of, auto measure, bool wide, int& bin, u64& above, u64& inside, u64& target) {
-        for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.lo[i] = sh.hi[i] = 0u;
+        for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.part[0][i] = sh.part[1][i] = sh.part[2][i] = 0u;
         __syncthreads();
-#pragma unroll 2
+        const unsigned low_bits = (1u << part_bits) - 1u;
+#pragma unroll 4
         for (int i = tid; i < n; i += SR_THREADS) {
             const float l = value(i);
-            if (l > r.low && sr_kept(r, l, first + i)) {
-                const u64 m = measure(l);
-                const int b = sr_bin(r.max_value, l);
-                if (!wide) atomicAdd(&sh.lo[b], (unsigned)m);
-                else if (m != 0ull) {
-                    const unsigned low = (unsigned)m, carry = atomicAdd(&sh.lo[b], low) > ~low ? 1u : 0u;
-                    if ((unsigned)(m >> 32) + carry != 0u) atomicAdd(&sh.hi[b], (unsigned)(m >> 32) + carry);
-                }
+            const u64 m = sr_kept(r, l, first + i) ? measure(l) : 0ull;
+            const int b = sr_bin(r.max_value, l);
+            if (!wide) {
+                if (m != 0ull) atomicAdd(&sh.part[0][b], 1u);
+            } else {
+                const unsigned p0 = (unsigned)m & low_bits, p1 = (unsigned)(m >> part_bits) & low_bits, p2 = (unsigned)(m >> (2 * part_bits));
+                if (p0) atomicAdd(&sh.part[0][b], p0);
+                if (p1) atomicAdd(&sh.part[1][b], p1);
+                if (p2) atomicAdd(&sh.part[2][b], p2);
             }
         }
         sr_cluster_sync();
@@ -487,8 +503,8 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             if (j < q && tid * q + j < share)
                 for (int c = 0; c < C; c++) {
                     const int b = (int)rank * share + tid * q + j;
-                    sum[j] += sr_load_remote(&sh.lo[b], c);
-                    if (wide) sum[j] += (u64)sr_load_remote(&sh.hi[b], c) << 32;
+                    sum[j] += sr_load_remote(&sh.part[0][b], c);
+                    if (wide) sum[j] += ((u64)sr_load_remote(&sh.part[1][b], c) << part_bits) + ((u64)sr_load_remote(&sh.part[2][b], c) << (2 * part_bits));
                 }
             mine += sum[j];
         }
@@ -523,21 +539,21 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
         if (words <= SR_LIST) {
             if (rank == 0) {
                 SrList w;
-                int per, bits;
-                take_list(w, (int)words, per, bits);
+                int bits;
+                take_list(w, (int)words, bits);
                 u64 m[SR_PER], last = ~0ull;
 #pragma unroll
-                for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? measure(w.l[e]) : 0ull;
+                for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? measure(w.value(e)) : 0ull;
                 const u64 cut = sr_list_cut(sh, w, m, target - above, bits);
                 // the last word of the prefix: the smallest order that is kept
 #pragma unroll
                 for (int e = 0; e < SR_PER; e++)
-                    if (e < w.n && m[e] != 0ull && w.order[e] >= cut && w.order[e] < last) last = w.order[e];
+                    if (e < w.n && m[e] != 0ull && w.order(e) >= cut && w.order(e) < last) last = w.order(e);
                 const unsigned high = ~sr_block_max(sh, ~(unsigned)(last >> 32)), low = ~sr_block_max(sh, (unsigned)(last >> 32) == high ? ~(unsigned)last : 0u);
 #pragma unroll
                 for (int e = 0; e < SR_PER; e++)
-                    if (e < w.n && w.order[e] == (((u64)high << 32) | low))
-                        tell_all(1, ((u64)__float_as_uint(w.l[e]) << 32) | (unsigned)sh.id[tid * per + e]);
+                    if (e < w.n && w.order(e) == (((u64)high << 32) | low))
+                        tell_all(1, ((u64)__float_as_uint(w.value(e)) << 32) | (unsigned)sh.id[w.at + e]);
             }
             sr_cluster_sync();
             r.cut = __uint_as_float((unsigned)(sh.found[1] >> 32));
@@ -547,7 +563,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
         unsigned hi = 0, lo = 0;                        // the bin's largest key, and its smallest one's complement
         for (int i = tid; i < n; i += SR_THREADS) {
             const float l = value(i);
-            if (l > r.low && sr_kept(r, l, first + i) && sr_bin(r.max_value, l) == bin) {
+            if (sr_kept(r, l, first + i) && sr_bin(r.max_value, l) == bin) {
                 const unsigned k = sr_key(l);
                 hi = max(hi, k);
                 lo = max(lo, ~k);
@@ -572,26 +588,26 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             const int words = (int)gather([&](float l) { return sr_bin(r.max_value, l) <= bin; });
             if (rank != 0) return;
             SrList w;
-            int per, bits;
-            take_list(w, words, per, bits);
+            int bits;
+            take_list(w, words, bits);
             u64 m[SR_PER], mine = 0, whole;
 #pragma unroll
             for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? 1ull : 0ull;
             u64 cut = sr_list_cut(sh, w, m, target, bits);
             if (top_p < 1.0f) {
 #pragma unroll
-                for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order[e] >= cut ? weight_of(w.l[e]) : 0ull;
+                for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= cut ? weight_of(w.value(e)) : 0ull;
                 cut = sr_list_cut(sh, w, m, sr_top_p_target(top_p, sr_block_sum(sh, mine)), bits);
             }
             mine = 0;
 #pragma unroll
-            for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order[e] >= cut ? sr_weight<true>(r, sh.table, w.l[e]) : 0ull;
+            for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= cut ? sr_weight<true>(r, sh.table, w.value(e)) : 0ull;
             u64 before = sr_block_before(sh, mine, whole);
             const u64 t = sr_draw_target(u, whole);
             if (before <= t && before + mine > t) {
 #pragma unroll
                 for (int e = 0; e < SR_PER; e++) {
-                    if (before <= t && before + m[e] > t) out[row] = sh.id[tid * per + e];
+                    if (before <= t && before + m[e] > t) out[row] = sh.id[w.at + e];
                     before += m[e];
                 }
             }
@@ -605,7 +621,8 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     // 3. the draw
     auto weight = [&](int i) {
         const float l = value(i);
-        return l > r.low && sr_kept(r, l, first + i) ? sr_weight<true>(r, sh.table, l) : 0ull;
+        const u64 w = sr_weight<true>(r, sh.table, l);
+        return sr_kept(r, l, first + i) ? w : 0ull;
     };
     u64 mine = 0;
 #pragma unroll 4
@@ -617,37 +634,37 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     if (rank == 0 && tid == 0) out[row] = id;
 }
 
-template <typename TIn, bool RESIDENT>
+template <typename TIn>
 static int sr_launch(const void* logits, long long ld, int B, int V, int C, const float* u, const float* temp, const int* top_k, const float* top_p,
                      const float* min_p, int* out, cudaStream_t s) {
-    int S = 62;
-    while (S > 0 && (1ll << (62 - S)) < V) S--;
-    if (S > 50) S = 50;
     const int chunk = ((V + C - 1) / C + 7) / 8 * 8;        // whole 16-byte pieces of either type
-    const size_t smem = sizeof(SrShared) + (RESIDENT ? (size_t)chunk * sizeof(float) : 0);
-    auto kern = sample_rows_kernel<TIn, RESIDENT>;
+    int log_v = 0, log_chunk = 0;
+    while ((1 << log_v) < V) log_v++;
+    while ((1 << log_chunk) < chunk) log_chunk++;
+    // a row's sum stays below 2^62; a part of the histogram, times a block's words, below 2^32
+    const int part_bits = 32 - log_chunk - 1;
+    int S = 62 - log_v;
+    S = S > 50 ? 50 : S;
+    S = S > 3 * part_bits ? 3 * part_bits : S;
+    const size_t smem = sizeof(SrShared) + (size_t)chunk * sizeof(float) + (size_t)(chunk / 32 + SR_WARPS + 1) * sizeof(unsigned);
+    auto kern = sample_rows_kernel<TIn>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return illm_launch_cluster(kern, dim3((unsigned)B * C), dim3(SR_THREADS), C, smem, s, (const TIn*)logits, ld, V, chunk, C, S, u, temp, top_k, top_p,
-                               min_p, out);
+    return illm_launch_cluster(kern, dim3((unsigned)B * C), dim3(SR_THREADS), C, smem, s, (const TIn*)logits, ld, V, chunk, C, S, part_bits, u, temp, top_k,
+                               top_p, min_p, out);
 }
 
-// logits [B, V] (dtype ILLM_F32 or ILLM_BF16, rows ld elements apart), one uniform number in [0, 1) per row; temp, top_k, top_p and
-// min_p [B] or nullptr (1, all, 1, 0) -> out int32 [B].
+// logits [B, V] (dtype ILLM_F32 or ILLM_BF16, rows ld elements apart), V at most 360,448; one uniform number in [0, 1) per row; temp,
+// top_k, top_p and min_p [B] or nullptr (1, all, 1, 0) -> out int32 [B].
 extern "C" int illm_sample_rows(const void* logits, int dtype, int B, int V, long long ld, const float* uniforms, const float* temp,
                                 const int* top_k, const float* top_p, const float* min_p, int* out, void* stream) {
     if (B <= 0) return 0;
-    if (V <= 0 || V > 0x7ffffff0 || B > (1 << 24) || ld < V || !logits || !uniforms || !out) return ILLM_ERR_BAD_ARG;
+    if (V <= 0 || V > SR_MAX_CLUSTER * SR_MAX_RESIDENT || B > (1 << 24) || ld < V || !logits || !uniforms || !out) return ILLM_ERR_BAD_ARG;
     // blocks to a row: more while there are fewer than four to an SM and a block's run is worth a block, or does not fit it
     int C = 1;
     while (C < SR_MAX_CLUSTER && (((V + C - 1) / C > 2048 && (long long)B * C < 4 * illm_sm_count()) || (V + C - 1) / C > SR_MAX_RESIDENT / 2)) C *= 2;
-    const bool resident = (V + C - 1) / C <= SR_MAX_RESIDENT;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == ILLM_F32)
-        return resident ? sr_launch<float, true>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s)
-                        : sr_launch<float, false>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
-    if (dtype == ILLM_BF16)
-        return resident ? sr_launch<bf16, true>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s)
-                        : sr_launch<bf16, false>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
+    if (dtype == ILLM_F32) return sr_launch<float>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
+    if (dtype == ILLM_BF16) return sr_launch<bf16>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
     return ILLM_ERR_BAD_ARG;
 }

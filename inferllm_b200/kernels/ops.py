@@ -23,6 +23,7 @@ def load():
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 MAX_HEAD_DIM_GENERIC = 256
+MAX_SAMPLE_WORDS = 8 * 45056
 MAX_NORM_WIDTH = 200 * 1024 // 4
 
 
@@ -971,6 +972,8 @@ def sample_rows(logits, uniforms, temp=None, top_k=None, top_p=None, min_p=None)
     device = logits.device
     if V == 0 or (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
         raise KernelError(f"sample_rows: rows of at least one word, each contiguous and none within another, found {tuple(logits.shape)} with strides {logits.stride()}")
+    if V > MAX_SAMPLE_WORDS:
+        raise KernelError(f"sample_rows: rows of {V} words exceed the {MAX_SAMPLE_WORDS} that a cluster's shared memory holds")
     if uniforms is None:
         raise KernelError("sample_rows: one uniform number per row is needed")
     u = _per_row(uniforms, "uniforms", torch.float32, B, device)

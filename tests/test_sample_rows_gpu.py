@@ -125,11 +125,14 @@ def test_a_row_does_not_depend_on_the_batch():
         assert ops.sample_rows(logits[i:i + 1], u[i:i + 1], temp[i:i + 1], k[i:i + 1], p[i:i + 1]).tolist() == whole[i:i + 1]
 
 
-def test_rows_longer_than_shared_memory():
+def test_the_longest_rows():
     g = torch.Generator("cuda").manual_seed(8)
-    V = 450001
+    V = 360448
     logits = torch.randn((3, V), generator=g, device="cuda")
     check(logits, [0.2, 0.6, 0.9], [1.0, 0.8, 0.0], [0, 5000, 3], [0.9, 0.95, 1.0], [0.0, 0.01, 0.0])
+    check(torch.zeros((2, V), device="cuda"), [0.2, 0.6], [1.0, 0.8], [0, 5000], [0.9, 1.0], [0.0, 0.01])
+    with pytest.raises(ops.KernelError):
+        ops.sample_rows(torch.zeros((1, V + 1), device="cuda"), f32([0.5]))
 
 
 def test_random_numbers_outside_their_range():
