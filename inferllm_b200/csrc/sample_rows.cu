@@ -21,13 +21,17 @@
 // One launch, a cluster of blocks per row: every block keeps its run of the row in shared memory (the row is read once), and the
 // blocks exchange sums through distributed shared memory.
 //   1. the largest word.  T <= 0 ends here.
-//   2. a cut: a histogram over 2048 bins of the distance m - l (128 bins to an octave from 2^-8 to 2^8, whatever the
-//      temperature: the bins are only a partition that keeps the order), of counts for top_k and of weights for top_p; each
-//      block adds up its share of the bins for all blocks and one of them finds the bin in which the cut falls.  That bin's words
-//      (some hundreds) go to the first block, which finds the cut among them, 8 bits of (value, id) at a time.  Where top_k
-//      leaves at most 4096 words down to that bin, it takes all of them and finishes the row by itself.  A bin of more words
-//      (many equal ones) is bisected by the whole cluster.
-//   3. the kept weights' sum, then the block, the warp's run and the word in which it passes u times the whole.
+//   2. top_k: a histogram of counts over 2048 bins of the distance m - l (128 bins to an octave from 2^-8 to 2^8, whatever the
+//      temperature: the bins are only a partition that keeps the order); the blocks tell one another the sums of 32 groups of bins,
+//      then the bins of the group in which the cut falls.  Where at most 4096 words lie down to that bin (any usual top_k) the
+//      first block takes them all and finishes the row by itself; otherwise it finds the cut among the bin's words.
+//   3. top_p: the same histogram of float32 weights (relative to the bin's, in integers, so that their order does not matter) says
+//      in which bin the cut falls, up to a rounding; one pass over the row then adds up the exact weights, all of them and those
+//      before that bin, which proves the bin right or says which way to move, and notes the bin's words for the first block, which
+//      finds the cut among them.
+//   4. the draw: the block, the warp's run and the word in which the kept weights' sum passes u times the whole.  Behind top_p the
+//      runs' sums are known from its pass.
+// A bin of more than 4096 words (many equal ones) is bisected by the whole cluster.
 #include <math.h>
 
 #include "common.cuh"
@@ -37,9 +41,12 @@
 #define SR_MAX_CLUSTER 8
 #define SR_MAX_RESIDENT 45056       // words of a row that one block keeps
 #define SR_BINS 2048
+#define SR_GROUPS 32                // groups of bins
+#define SR_GROUP (SR_BINS / SR_GROUPS)
 #define SR_PER 8
 #define SR_LIST (SR_THREADS * SR_PER)       // words that one block takes to itself
 #define SR_LIST_BITS 12
+#define SR_FEW 128                  // words that are ranked by comparing each with each
 
 typedef unsigned long long u64;
 
@@ -62,11 +69,7 @@ __device__ __forceinline__ void sr_store_remote(void* local, unsigned rank, u64 
 __device__ __forceinline__ void sr_store_remote(void* local, unsigned rank, unsigned v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(sr_remote(local, rank)), "r"(v) : "memory");
 }
-__device__ __forceinline__ unsigned sr_load_remote(const unsigned* local, unsigned rank) {
-    unsigned v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sr_remote(local, rank)) : "memory");
-    return v;
-}
+__device__ __forceinline__ void sr_store_remote(void* local, unsigned rank, float v) { sr_store_remote(local, rank, __float_as_uint(v)); }
 
 // order-preserving image of a float, both zeros alike, and back
 __device__ __forceinline__ unsigned sr_key(float f) {
@@ -74,24 +77,26 @@ __device__ __forceinline__ unsigned sr_key(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float sr_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
-// bin of a word: 0 the nearest to the largest
-__device__ __forceinline__ int sr_bin(float max_value, float l) {
-    const float d = l == max_value ? 0.f : max_value - l;
-    return min(max((int)(__float_as_uint(d) >> 16) - 15231, 0), SR_BINS - 1);
-}
+// distance from the largest word (0 for an infinite one), its bin (0 the nearest) and where a bin begins
+__device__ __forceinline__ float sr_distance(float max_value, float l) { return l == max_value ? 0.f : max_value - l; }
+__device__ __forceinline__ int sr_bin(float d) { return min(max((int)(__float_as_uint(d) >> 16) - 15231, 0), SR_BINS - 1); }
+__device__ __forceinline__ float sr_edge(int bin) { return bin <= 0 ? 0.f : bin >= SR_BINS ? INFINITY : __uint_as_float((unsigned)(bin + 15231) << 16); }
 
 struct __align__(16) SrShared {
     double table[16];                                   // 2^(i / 16)
-    u64 slot[2][SR_MAX_CLUSTER];                        // what the blocks of the cluster exchange, two in turn
-    u64 found[4];                                       // what one block tells all
-    u64 warp_sum[SR_WARPS];
+    u64 slot[2][4][SR_MAX_CLUSTER];                     // what the blocks of the cluster exchange, two sets in turn
+    u64 found;                                          // what one block tells all
+    u64 warp_sum[SR_WARPS], warp_above[SR_WARPS];
+    float group_sum[SR_MAX_CLUSTER][SR_GROUPS];         // every block's histogram: sums of the groups,
+    float bin_sum[SR_MAX_CLUSTER][SR_GROUP];            // bins of one group
     struct { unsigned count[256], lo[256], hi[256]; } digits[2];
+    u64 few_order[SR_FEW], few_weight[SR_FEW];
+    unsigned n_few, few_at[SR_FEW];
     union {
-        unsigned part[3][SR_BINS];                      // histogram: a sum's bits in three parts, or a count in the first
+        unsigned bins[SR_BINS];
         struct { float value[SR_LIST]; int id[SR_LIST]; };      // the first block's list
     };
 };
-
 static_assert(sizeof(SrShared) % 16 == 0, "the row behind it is written 16 bytes at a time");
 
 struct SrRow {
@@ -106,22 +111,12 @@ struct SrRow {
     int cut_id;
 };
 
-// A float as a double by integer instructions: the conversion instruction does 16 of them per clock and SM, a quarter of the rate
-// of the float64 arithmetic behind it, and was what bound the sums.
-__device__ __forceinline__ double sr_double(float f) {
-    const unsigned b = __float_as_uint(f), sign = b & 0x80000000u, high = b & 0x7fffffffu;
-    // zero and subnormals have no leading one: it is added with the smallest normal exponent and taken off again
-    const bool small = high < 0x00800000u;
-    const unsigned e = small ? 897u << 20 : 896u << 20;
-    const double off = __hiloint2double((int)(small ? sign | (897u << 20) : 0u), 0);
-    return __hiloint2double((int)(sign | ((high >> 3) + e)), (int)(b << 29)) - off;
-}
 // w of a word that can come, in units of 2^-S; 0 as well if it is below min_p (CUT).  With x = 16 (l - m) log2(e) / T = j + f, |f| <= 1/2:
 // w = 2^(j / 16) exp(f ln2 / 16); the table's 16 entries lie in 32 different banks, and the series' first term left out is
 // below 2^-51 of the sum.
 template <bool CUT>
 __device__ __forceinline__ u64 sr_weight(const SrRow& r, const double* table, float l) {
-    const double x = (sr_double(l) - r.max_wide) * r.inv_temp;
+    const double x = ((double)l - r.max_wide) * r.inv_temp;
     const double shift = 6755399441055744.0;            // 1.5 * 2^52: rounds to an integer, which the low bits then hold
     const double t = x + shift;
     const int j = (int)(unsigned)__double_as_longlong(t);
@@ -139,7 +134,7 @@ __device__ __forceinline__ u64 sr_weight(const SrRow& r, const double* table, fl
     const double two52 = 4503599627370496.0;
     u64 units = (u64)__double_as_longlong(w * r.unit + two52) & 0xFFFFFFFFFFFFFull;      // rounded to nearest
     if (CUT && w < r.min_p) units = 0ull;
-    if (x < -1024.0) units = 0ull;                      // less than 2^-64
+    if ((unsigned)__double2hiint(x) > 0xC0900000u) units = 0ull;      // x < -1024: less than 2^-64
     return l == r.max_value ? r.one : units;
 }
 // whether a word can come and is still kept (no branch: the loops over the row are bound by how many of their loads and chains overlap)
@@ -151,23 +146,14 @@ __device__ __forceinline__ u64 sr_warp_sum(u64 v) {
                    c = __reduce_add_sync(0xffffffffu, (unsigned)(v >> 44));
     return (u64)a + ((u64)b << 22) + ((u64)c << 44);
 }
-__device__ __forceinline__ u64 sr_warp_scan(u64 v) {        // inclusive
+template <typename T> __device__ __forceinline__ T sr_warp_scan(T v) {        // inclusive
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+        const T x = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += x;
     }
     return v;
-}
-// The blocks' values side by side; every thread of every block may read them in the slots that come back.  The two sets of
-// slots take turns, so that a block that is behind still reads the one while the next exchange fills the other.
-__device__ __forceinline__ const u64* sr_exchange(SrShared& sh, int& turn, u64 mine, int C, unsigned rank) {
-    u64* s = sh.slot[turn & 1];
-    turn++;
-    if ((int)threadIdx.x < C) sr_store_remote(&s[rank], threadIdx.x, mine);
-    sr_cluster_sync();
-    return s;
 }
 // sum over the block (every thread gets it); the warps' sums stay in sh.warp_sum
 __device__ __forceinline__ u64 sr_block_sum(SrShared& sh, u64 v) {
@@ -205,64 +191,6 @@ __device__ __forceinline__ u64 sr_block_before(SrShared& sh, u64 v, u64& whole) 
     }
     return before;
 }
-
-// A list of at most SR_LIST words in ascending order of their id, dealt to the block's threads in runs: word w.at + e.
-// order: key above the list's smallest key, and below it the complement of the place: larger means earlier in the row's order.
-struct SrList {
-    unsigned key[SR_PER];   // above the list's smallest
-    unsigned least;         // that one
-    int n, at;              // words of this thread, place of the first
-    __device__ __forceinline__ u64 order(int e) const { return ((u64)key[e] << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - at - e); }
-    __device__ __forceinline__ float value(int e) const { return sr_value(key[e] + least); }
-};
-// The cut of the shortest prefix, largest order first, whose measure (m[e] of word e) reaches `target`, which all of them do: kept
-// are the words with order >= the result, and `last` is the smallest of them.  Digit by digit, 8 bits at a time, until a digit
-// has one word.
-__device__ __forceinline__ u64 sr_list_cut(SrShared& sh, const SrList& w, const u64* m, u64 target, int bits) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    u64 prefix = 0, above = 0;
-    int shift = bits;
-    for (int turn = 0;; turn ^= 1) {
-        unsigned *count = sh.digits[turn].count, *lo = sh.digits[turn].lo, *hi = sh.digits[turn].hi;
-        for (int i = tid; i < 256; i += SR_THREADS) count[i] = lo[i] = hi[i] = 0u;
-        __syncthreads();
-        const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
-#pragma unroll
-        for (int e = 0; e < SR_PER; e++)
-            if (e < w.n && m[e] != 0ull && w.order(e) >> shift == prefix) {
-                const int d = (int)(w.order(e) >> down) & ((1 << width) - 1);
-                const unsigned low = (unsigned)m[e], carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
-                if ((unsigned)(m[e] >> 32) + carry != 0u) atomicAdd(&hi[d], (unsigned)(m[e] >> 32) + carry);
-                atomicAdd(&count[d], 1u);
-            }
-        __syncthreads();
-        // every warp by itself: 8 digits a lane, the largest first
-        u64 sum[8], mine = 0;
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-            const int d = 255 - (lane * 8 + q);
-            mine += sum[q] = ((u64)hi[d] << 32) | lo[d];
-        }
-        u64 before = above + sr_warp_scan(mine) - mine;
-        const int owner = __ffs(__ballot_sync(0xffffffffu, before + mine >= target)) - 1;
-        int digit = 0;
-        bool open = true;
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-            if (open && before + sum[q] >= target) {
-                digit = 255 - (lane * 8 + q);
-                open = false;
-            }
-            if (open) before += sum[q];
-        }
-        digit = __shfl_sync(0xffffffffu, digit, owner);
-        above = __shfl_sync(0xffffffffu, before, owner);
-        prefix = (prefix << width) | (unsigned)digit;
-        shift = down;
-        if (shift == 0 || count[digit] == 1u) return prefix << shift;
-    }
-}
-
 __device__ __forceinline__ u64 sr_top_p_target(float top_p, u64 total) {
     const u64 t = (u64)ceil((double)top_p * (double)total);
     return !(top_p > 0.f) || t == 0ull ? 1ull : t;
@@ -273,92 +201,48 @@ __device__ __forceinline__ u64 sr_draw_target(float u, u64 total) {
     return t < total ? t : total - 1;
 }
 
-template <typename TIn>
-__global__ void __launch_bounds__(SR_THREADS, 2)
-sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chunk, int C, int S, int part_bits, const float* __restrict__ uniforms,
-                   const float* __restrict__ temps, const int* __restrict__ top_ks, const float* __restrict__ top_ps,
-                   const float* __restrict__ min_ps, int* __restrict__ out) {
-    extern __shared__ __align__(16) unsigned char sr_smem[];
-    SrShared& sh = *reinterpret_cast<SrShared*>(sr_smem);
-    float* resident = reinterpret_cast<float*>(sr_smem + sizeof(SrShared));
-    unsigned* taken_mask = reinterpret_cast<unsigned*>(resident + chunk);       // a bit per word
-    pdl_grid_sync();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned rank = C > 1 ? sr_rank() : 0;
-    const int row = blockIdx.x / C;
-    const TIn* src = logits + (long long)row * ld;
-    const int first = (int)rank * chunk, n = max(0, min(V - first, chunk));     // this block's run of the row
-    const int seg = ((chunk + SR_WARPS - 1) / SR_WARPS + 31) & ~31;            // a warp's run of the block's
-    const int s0 = min(warp * seg, n), s1 = min(s0 + seg, n);
-    if (tid < 16) sh.table[tid] = exp2((double)tid / 16.0);
-    int turn = 0;
-    const float temp = temps ? temps[row] : 1.0f, top_p = top_ps ? top_ps[row] : 1.0f, min_p = min_ps ? min_ps[row] : 0.f, u = uniforms[row];
-    const int top_k = top_ks ? top_ks[row] : 0;
-    auto value = [&](int i) { return resident[i]; };
+// A block's view of its row.
+struct SrBlock {
+    SrShared& sh;
+    const float* row;       // its run of the row
+    unsigned* mask;         // a bit per word of it
+    int n, first, seg, s0, s1, C, tid, lane, warp;     // s0 .. s1: the warp's run of that
+    unsigned rank;
+    int turn;
 
-    // 1. the row and its largest word
-    float top = -INFINITY;
-    {
-        constexpr int W = 16 / sizeof(TIn);
-        const int whole = ((uintptr_t)(src + first) & 15) == 0 ? n / W * W : 0;
-#pragma unroll 4
-        for (int i = tid * W; i < whole; i += SR_THREADS * W) {
-            float f[W];
-            if (W == 8) load8(reinterpret_cast<const bf16*>(src + first + i), f);
-            else *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(src + first + i);
+    // The blocks' values side by side; every thread of every block may read them in the slots that come back.  The two sets of
+    // slots take turns, so that a block that is behind still reads the one while the next exchange fills the other.
+    template <int N> __device__ __forceinline__ const u64 (*exchange(const u64 (&mine)[N]))[SR_MAX_CLUSTER] {
+        u64(*s)[SR_MAX_CLUSTER] = sh.slot[turn & 1];
+        turn++;
+        const int i = tid / SR_MAX_CLUSTER, c = tid % SR_MAX_CLUSTER;
 #pragma unroll
-            for (int e = 0; e < W; e++) top = fmaxf(top, f[e]);
-#pragma unroll
-                for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(resident + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-        }
-#pragma unroll 4
-        for (int i = whole + tid; i < n; i += SR_THREADS) {
-            const float f = to_f32(src[first + i]);
-            resident[i] = f;
-            top = fmaxf(top, f);                        // (the other one of a NaN)
-        }
+        for (int j = 0; j < N; j++)
+            if (i == j && c < C) sr_store_remote(&s[j][rank], c, mine[j]);
+        sr_cluster_sync();
+        return s;
     }
-    const u64* ex = sr_exchange(sh, turn, sr_block_max(sh, sr_key(top)), C, rank);
-    u64 best = 0;
-    for (int c = 0; c < C; c++) best = ex[c] > best ? ex[c] : best;
-    SrRow r;
-    r.max_value = sr_value((unsigned)best);
-    if (r.max_value == -INFINITY) {                     // nothing can come: the same in all blocks
-        if (rank == 0 && tid == 0) out[row] = -1;
-        return;
-    }
-    if (!(temp > 0.f)) {                                // the largest comes, the lowest id of equals
-        unsigned least = 0;                             // its complement, for a maximum
-        for (int i = tid; i < n; i += SR_THREADS)
-            if (value(i) == r.max_value) { least = 0x7fffffff - (first + i); break; }
-        ex = sr_exchange(sh, turn, sr_block_max(sh, least), C, rank);
-        if (rank == 0 && tid == 0) {
-            for (int c = 0; c < C; c++) least = max(least, (unsigned)ex[c]);
-            out[row] = 0x7fffffff - (int)least;
-        }
-        return;
-    }
-    r.inv_temp = 16.0 * 1.44269504088896340736 / (double)temp;
-    r.max_wide = (double)r.max_value;
-    r.one = 1ull << S;
-    r.unit = (double)r.one;
-    r.min_p = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
-    r.low = r.max_value == INFINITY ? 3.402823466e38f : -INFINITY;
-    r.cut = -INFINITY;
-    r.cut_id = -1;
-
-    auto cluster_sum = [&](u64 mine) {
-        const u64* e = sr_exchange(sh, turn, sr_block_sum(sh, mine), C, rank);
+    __device__ __forceinline__ u64 cluster_sum(u64 mine) {
+        const u64 m[1] = {sr_block_sum(sh, mine)};
+        const u64(*e)[SR_MAX_CLUSTER] = exchange(m);
         u64 t = 0;
-        for (int c = 0; c < C; c++) t += e[c];
+        for (int c = 0; c < C; c++) t += e[0][c];
         return t;
-    };
-    auto tell_all = [&](int i, u64 v) {                 // by one thread
-        for (int c = 0; c < C; c++) sr_store_remote(&sh.found[i], c, v);
-    };
+    }
+    __device__ __forceinline__ unsigned cluster_max(unsigned mine) {
+        const u64 m[1] = {sr_block_max(sh, mine)};
+        const u64(*e)[SR_MAX_CLUSTER] = exchange(m);
+        unsigned t = 0;
+        for (int c = 0; c < C; c++) t = max(t, (unsigned)e[0][c]);
+        return t;
+    }
+    __device__ __forceinline__ void tell_all(u64 v) {      // by one thread
+        for (int c = 0; c < C; c++) sr_store_remote(&sh.found, c, v);
+    }
+
     // The first id, ascending, at which the sum of measure(i) over the ids up to it exceeds t; every thread of the cluster
     // gets it.  totals: the blocks' sums, sh.warp_sum the warps'.  The whole sum must exceed t.
-    auto find = [&](u64 t, const u64* totals, auto measure) {
+    template <typename F> __device__ __forceinline__ int find(u64 t, const u64* totals, F measure) {
         u64 before = 0;
         int owner = 0;
         for (; owner < C - 1 && before + totals[owner] <= t; owner++) before += totals[owner];
@@ -375,263 +259,513 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
                 mine = i < e ? measure(i) : 0ull;
                 u64 whole;
                 const u64 prior = before + sr_block_before(sh, mine, whole);
-                if (prior <= t && prior + mine > t) tell_all(0, (u64)(first + i));
+                if (prior <= t && prior + mine > t) tell_all((u64)(first + i));
                 before += whole;
                 if (before > t) break;
             }
         }
         sr_cluster_sync();
-        return (int)sh.found[0];
-    };
-    // The whole cluster's bisection: words with keys in [lo, hi), above = the sum over larger ones.
-    auto cut_by_cluster = [&](u64 lo, u64 hi, u64 above, u64 target, auto measure) {
+        return (int)sh.found;
+    }
+
+    // Histogram of the kept words over the bins, of counts or (WEIGHTS) of float32 weights, and the bin in which the sum reaches
+    // `share` of the whole (WEIGHTS) or `share` words; `before` is the sum over the bins ahead of it, `inside` its own.  Counts
+    // are exact.  false if there are fewer words.  The same in every block.
+    template <bool WEIGHTS> __device__ __forceinline__ bool bin_of(const SrRow& r, float share, int part_bits, int& bin, float& before, float& inside) {
+        for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.bins[i] = 0u;
+        __syncthreads();
+        const float rate = fmaxf((float)(r.inv_temp * -0.0625), -1e30f), scale = (float)(1u << part_bits);       // log2 of a weight per distance
+        const bool all = r.cut == -INFINITY;
+#pragma unroll 4
+        for (int i = tid; i < n; i += SR_THREADS) {
+            const float l = row[i], d = sr_distance(r.max_value, l);
+            const int b = sr_bin(d);
+            unsigned m = 1u;
+            // (2^23 as the ulp's unit: the sum's low bits are the rounded weight)
+            if (WEIGHTS) m = __float_as_uint(fmaf(fast_exp2((d - sr_edge(b)) * rate), scale, 8388608.0f)) & 0x7fffffu;
+            if ((l > r.low) & (all || sr_kept(r, l, first + i)) & (m != 0u)) atomicAdd(&sh.bins[b], m);
+        }
+        __syncthreads();
+        auto mass = [&](int b) { return WEIGHTS ? (float)sh.bins[b] * fast_exp2(sr_edge(b) * rate) : (float)sh.bins[b]; };
+        // groups: 16 threads each
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < SR_BINS / SR_THREADS; j++) v += mass(tid * (SR_BINS / SR_THREADS) + j);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if ((tid & 15) < C) sr_store_remote(&sh.group_sum[rank][tid >> 4], tid & 15, v);
+        sr_cluster_sync();
+        // every warp by itself, and alike: the group, then the bin
+        v = 0.f;
+        for (int c = 0; c < C; c++) v += sh.group_sum[c][lane];
+        float upto = sr_warp_scan(v);
+        const float whole = __shfl_sync(0xffffffffu, upto, 31), target = WEIGHTS ? share * whole : share;
+        if (!WEIGHTS && whole < target) return false;
+        auto first_lane = [&](float m) {                // where the sum reaches the target, or the last with anything in it
+            const unsigned reach = __ballot_sync(0xffffffffu, (upto >= target) & (m > 0.f)), some = __ballot_sync(0xffffffffu, m > 0.f);
+            return reach ? __ffs(reach) - 1 : 31 - __clz(some | 1u);
+        };
+        const int g = first_lane(v);
+        const float ahead = __shfl_sync(0xffffffffu, upto - v, g);
+        if (tid < SR_GROUP * C) sr_store_remote(&sh.bin_sum[rank][tid % SR_GROUP], tid / SR_GROUP, mass(g * SR_GROUP + tid % SR_GROUP));
+        sr_cluster_sync();
+        float a = 0.f, b = 0.f;
+        for (int c = 0; c < C; c++) {
+            a += sh.bin_sum[c][2 * lane];
+            b += sh.bin_sum[c][2 * lane + 1];
+        }
+        upto = ahead + sr_warp_scan(a + b);
+        const int p = first_lane(a + b);
+        a = __shfl_sync(0xffffffffu, a, p);
+        b = __shfl_sync(0xffffffffu, b, p);
+        before = __shfl_sync(0xffffffffu, upto, p) - (a + b);
+        const bool second = (before + a < target && b > 0.f) || !(a > 0.f);
+        bin = g * SR_GROUP + 2 * p + second;
+        before += second ? a : 0.f;
+        inside = second ? b : a;
+        return true;
+    }
+
+    // The words that a mask marks, in ascending order of their id, into the first block's list.  count: of this warp's run, at: words
+    // of all runs before it.
+    __device__ __forceinline__ void push(unsigned count, unsigned at) {
+        // a lane per 32 words
+        for (int i0 = s0; i0 < s1 && count != 0; i0 += 1024) {
+            const int i = i0 + lane * 32;
+            unsigned m = i < s1 ? mask[i >> 5] : 0u;
+            const unsigned mine = __popc(m), run = sr_warp_scan(mine);
+            unsigned to = at + run - mine;
+            at += __shfl_sync(0xffffffffu, run, 31);
+            for (; m; m &= m - 1, to++) {
+                const int k = i + __ffs(m) - 1;
+                sr_store_remote(&sh.value[to], 0, row[k]);
+                sr_store_remote(&sh.id[to], 0, (unsigned)(first + k));
+            }
+        }
+        sr_cluster_sync();
+    }
+    // The kept words at distances of [from, to) into the first block's list; how many there are.  More than the list holds: nothing
+    // is written.
+    __device__ __forceinline__ unsigned gather(const SrRow& r, float from, float to) {
+        unsigned count = 0;
+#pragma unroll 4
+        for (int i = s0; i < s1; i += 32) {
+            const float l = i + lane < s1 ? row[i + lane] : -INFINITY, d = sr_distance(r.max_value, l);
+            const unsigned all = __ballot_sync(0xffffffffu, sr_kept(r, l, first + i + lane) & (d >= from) & ((d < to) | (to == INFINITY)));
+            count += __popc(all);
+            if (lane == 0) mask[i >> 5] = all;
+        }
+        const u64 m[1] = {sr_block_sum(sh, lane == 0 ? count : 0u)};
+        unsigned at = 0, total = 0;
+#pragma unroll
+        for (int q = 0; q < SR_WARPS; q++) at += q < warp ? (unsigned)sh.warp_sum[q] : 0u;
+        const u64(*e)[SR_MAX_CLUSTER] = exchange(m);
+        for (int c = 0; c < C; c++) {
+            if (c < (int)rank) at += (unsigned)e[0][c];
+            total += (unsigned)e[0][c];
+        }
+        if (total <= SR_LIST) push(count, at);
+        return total;
+    }
+
+    // The whole cluster's bisection among the kept words at distances of [from, to), for bins that no list holds: the cut of the
+    // shortest prefix whose measure reaches `target`, `above` being the measure of the words before these.
+    template <typename F> __device__ __forceinline__ void cut_by_cluster(SrRow& r, float from, float to, u64 above, u64 target, F measure) {
+        unsigned most = 0, least = 0;                   // the largest key, and the smallest one's complement
+        for (int i = tid; i < n; i += SR_THREADS) {
+            const float l = row[i], d = sr_distance(r.max_value, l);
+            if (sr_kept(r, l, first + i) & (d >= from) & ((d < to) | (to == INFINITY))) {
+                const unsigned k = sr_key(l);
+                most = max(most, k);
+                least = max(least, ~k);
+            }
+        }
+        u64 hi = (u64)cluster_max(most) + 1, lo = (u64)(unsigned)~cluster_max(least);
         while (hi - lo > 1) {
             const u64 mid = lo + (hi - lo) / 2;
             u64 mine = 0;
             for (int i = tid; i < n; i += SR_THREADS) {
-                const float l = value(i);
-                if (sr_kept(r, l, first + i)) {
-                    const unsigned k = sr_key(l);
-                    if (k >= mid && k < hi) mine += measure(l);
-                }
+                const float l = row[i];
+                const unsigned k = sr_key(l);
+                if (sr_kept(r, l, first + i) & (k >= mid) & (k < hi)) mine += measure(l);
             }
             const u64 m = cluster_sum(mine);
             if (above + m >= target) lo = mid;
             else { hi = mid; above += m; }
         }
+        // of the words with this very value as many as are needed, in ascending order of their id
         const float cut = sr_value((unsigned)lo);
         const u64 each = measure(cut), need = (target - above + each - 1) / each;
-        auto tie = [&](int i) {
-            const float l = value(i);
-            return l == cut && sr_kept(r, l, first + i) ? 1ull : 0ull;
-        };
+        auto tie = [&](int i) { return (row[i] == cut) & sr_kept(r, row[i], first + i) ? 1ull : 0ull; };
         u64 mine = 0;
         for (int i = s0 + lane; i < s1; i += 32) mine += tie(i);
-        const u64* totals = sr_exchange(sh, turn, sr_block_sum(sh, mine), C, rank);
-        r.cut_id = find(need - 1, totals, tie);
+        const u64 m[1] = {sr_block_sum(sh, mine)};
+        const u64(*e)[SR_MAX_CLUSTER] = exchange(m);
+        const int id = find(need - 1, e[0], tie);
         r.cut = cut;
-    };
-    // The kept words that `pick` takes, in ascending order of their id, into the first block's list; how many there are.  More
-    // than the list holds: nothing is written.
-    auto gather = [&](auto pick) {
-        unsigned count = 0;
-#pragma unroll 4
-        for (int i = s0; i < s1; i += 32) {
-            const float l = i + lane < s1 ? value(i + lane) : -INFINITY;
-            const unsigned all = __ballot_sync(0xffffffffu, sr_kept(r, l, first + i + lane) & pick(l));
-            count += __popc(all);
-            if (lane == 0) taken_mask[i >> 5] = all;
-        }
-        const u64 block = sr_block_sum(sh, lane == 0 ? count : 0u);
-        unsigned at = 0, total = 0;
-#pragma unroll
-        for (int q = 0; q < SR_WARPS; q++) at += q < warp ? (unsigned)sh.warp_sum[q] : 0u;
-        const u64* e = sr_exchange(sh, turn, block, C, rank);
-        for (int c = 0; c < C; c++) {
-            if (c < (int)rank) at += (unsigned)e[c];
-            total += (unsigned)e[c];
-        }
-        if (total > SR_LIST) return total;
-        // a lane per 32 words
-        for (int i0 = s0; i0 < s1 && count != 0; i0 += 1024) {
-            const int i = i0 + lane * 32;
-            unsigned mask = i < s1 ? taken_mask[i >> 5] : 0u;
-            const unsigned mine = __popc(mask);
-            unsigned run = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned v = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += v;
-            }
-            unsigned to = at + run - mine;
-            at += __shfl_sync(0xffffffffu, run, 31);
-            for (; mask; mask &= mask - 1, to++) {
-                const int k = i + __ffs(mask) - 1;
-                sr_store_remote(&sh.value[to], 0, __float_as_uint(value(k)));
-                sr_store_remote(&sh.id[to], 0, (unsigned)(first + k));
-            }
-        }
-        sr_cluster_sync();
-        return total;
-    };
-    // the first block's list in its registers; `bits` how many of an order's bits differ among them
-    auto take_list = [&](SrList& w, int words, int& bits) {
+        r.cut_id = id;
+    }
+};
+
+// A list of at most SR_LIST words in ascending order of their id, dealt to the block's threads in runs.  order: key above the list's
+// smallest key, and below it the complement of the place: larger means earlier in the row's order.
+struct SrList {
+    unsigned key[SR_PER];   // above the list's smallest
+    unsigned least;         // that one
+    int n, at, bits;        // words of this thread, place of the first, bits of an order
+    __device__ __forceinline__ u64 order(int e) const { return ((u64)key[e] << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - at - e); }
+    __device__ __forceinline__ float value(int e) const { return sr_value(key[e] + least); }
+    __device__ __forceinline__ void take(SrShared& sh, int words) {
         const int per = (words + SR_THREADS - 1) / SR_THREADS;
-        w.at = tid * per;
-        w.n = max(0, min(per, words - w.at));
-        unsigned most = 0, least = 0;                   // the smallest key's complement
+        at = threadIdx.x * per;
+        n = max(0, min(per, words - at));
+        unsigned most = 0, low = 0;                     // the smallest key's complement
 #pragma unroll
         for (int e = 0; e < SR_PER; e++)
-            if (e < w.n) {
-                w.key[e] = sr_key(sh.value[w.at + e]);
-                most = max(most, w.key[e]);
-                least = max(least, ~w.key[e]);
+            if (e < n) {
+                key[e] = sr_key(sh.value[at + e]);
+                most = max(most, key[e]);
+                low = max(low, ~key[e]);
             }
         most = sr_block_max(sh, most);
-        w.least = ~sr_block_max(sh, least);
+        least = ~sr_block_max(sh, low);
 #pragma unroll
-        for (int e = 0; e < SR_PER; e++) w.key[e] -= w.least;
-        bits = 64 - __clzll(((u64)(most - w.least) << SR_LIST_BITS) | (SR_LIST - 1));
-    };
-    // Histogram of the kept words by bins.  Finds the bin in which the sum of measure reaches target_of(whole sum); `above` is the
-    // sum over the bins before it.  false if the whole does not reach the target.
-    auto bin_of = [&](auto target_of, auto measure, bool wide, int& bin, u64& above, u64& inside, u64& target) {
-        for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.part[0][i] = sh.part[1][i] = sh.part[2][i] = 0u;
-        __syncthreads();
-        const unsigned low_bits = (1u << part_bits) - 1u;
+        for (int e = 0; e < SR_PER; e++) key[e] -= least;
+        bits = 64 - __clzll(((u64)(most - least) << SR_LIST_BITS) | (SR_LIST - 1));
+    }
+    // The order of the last word of the shortest prefix, largest order first, whose measure (m[e] of word e) reaches `target`,
+    // which all of them do.  By digits of 8 bits, until one holds at most 32 words, which every warp ranks by itself.
+    __device__ __forceinline__ u64 cut(SrShared& sh, const u64* m, u64 target) const {
+        const int tid = threadIdx.x, lane = tid & 31;
+        u64 prefix = 0, above = 0;
+        int shift = bits;
+        for (int turn = 0;; turn ^= 1) {
+            unsigned *count = sh.digits[turn].count, *lo = sh.digits[turn].lo, *hi = sh.digits[turn].hi;
+            for (int i = tid; i < 256; i += SR_THREADS) count[i] = lo[i] = hi[i] = 0u;
+            if (tid == 0) sh.n_few = 0;
+            __syncthreads();
+            const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++)
+                if (e < n && m[e] != 0ull && order(e) >> shift == prefix) {
+                    const int d = (int)(order(e) >> down) & ((1 << width) - 1);
+                    const unsigned low = (unsigned)m[e], carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
+                    if ((unsigned)(m[e] >> 32) + carry != 0u) atomicAdd(&hi[d], (unsigned)(m[e] >> 32) + carry);
+                    atomicAdd(&count[d], 1u);
+                }
+            __syncthreads();
+            // every warp by itself: 8 digits a lane, the largest first
+            u64 mine = 0;
+#pragma unroll
+            for (int q = 0; q < 8; q++) mine += ((u64)hi[255 - (lane * 8 + q)] << 32) + lo[255 - (lane * 8 + q)];
+            u64 before = above + sr_warp_scan(mine) - mine;
+            const int owner = __ffs(__ballot_sync(0xffffffffu, before + mine >= target)) - 1;
+            int digit = 0;
+            bool open = true;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const u64 s = ((u64)hi[255 - (lane * 8 + q)] << 32) + lo[255 - (lane * 8 + q)];
+                if (open && before + s >= target) {
+                    digit = 255 - (lane * 8 + q);
+                    open = false;
+                }
+                if (open) before += s;
+            }
+            digit = __shfl_sync(0xffffffffu, digit, owner);
+            above = __shfl_sync(0xffffffffu, before, owner);
+            prefix = (prefix << width) | (unsigned)digit;
+            shift = down;
+            const unsigned words = count[digit];
+            if (words <= 32) {
+#pragma unroll
+                for (int e = 0; e < SR_PER; e++)
+                    if (e < n && m[e] != 0ull && order(e) >> shift == prefix) {
+                        const unsigned to = atomicAdd(&sh.n_few, 1u);
+                        sh.few_order[to] = order(e);
+                        sh.few_weight[to] = m[e];
+                    }
+                __syncthreads();
+                const u64 o = lane < (int)words ? sh.few_order[lane] : 0ull, w = lane < (int)words ? sh.few_weight[lane] : 0ull;
+                u64 sum = above;
+                for (int j = 0; j < (int)words; j++) sum += sh.few_order[j] > o ? sh.few_weight[j] : 0ull;
+                const int last = __ffs(__ballot_sync(0xffffffffu, lane < (int)words && sum < target && sum + w >= target)) - 1;
+                const u64 result = __shfl_sync(0xffffffffu, o, last);
+                __syncthreads();
+                return result;
+            }
+        }
+    }
+};
+
+template <typename TIn>
+__global__ void __launch_bounds__(SR_THREADS, 2)
+sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chunk, int C, int S, int part_bits, const float* __restrict__ uniforms,
+                   const float* __restrict__ temps, const int* __restrict__ top_ks, const float* __restrict__ top_ps,
+                   const float* __restrict__ min_ps, int* __restrict__ out) {
+    extern __shared__ __align__(16) unsigned char sr_smem[];
+    SrShared& sh = *reinterpret_cast<SrShared*>(sr_smem);
+    float* resident = reinterpret_cast<float*>(sr_smem + sizeof(SrShared));
+    pdl_grid_sync();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned rank = C > 1 ? sr_rank() : 0;
+    const int at_row = blockIdx.x / C;
+    const TIn* src = logits + (long long)at_row * ld;
+    const int first = (int)rank * chunk, n = max(0, min(V - first, chunk)), seg = ((chunk + SR_WARPS - 1) / SR_WARPS + 31) & ~31;
+    const int s0 = min(warp * seg, n), s1 = min(s0 + seg, n);
+    SrBlock k{sh, resident, reinterpret_cast<unsigned*>(resident + chunk), n, first, seg, s0, s1, C, tid, lane, warp, rank, 0};
+    if (tid < 16) sh.table[tid] = exp2((double)tid / 16.0);
+    const float temp = temps ? temps[at_row] : 1.0f, top_p = top_ps ? top_ps[at_row] : 1.0f, min_p = min_ps ? min_ps[at_row] : 0.f, u = uniforms[at_row];
+    const int top_k = top_ks ? top_ks[at_row] : 0;
+
+    // 1. the row and its largest word
+    float top = -INFINITY;
+    {
+        constexpr int W = 16 / sizeof(TIn);
+        const int whole = ((uintptr_t)(src + first) & 15) == 0 ? n / W * W : 0;
+#pragma unroll 8
+        for (int i = tid * W; i < whole; i += SR_THREADS * W) {
+            float f[W];
+            if (W == 8) load8(reinterpret_cast<const bf16*>(src + first + i), f);
+            else *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(src + first + i);
+#pragma unroll
+            for (int e = 0; e < W; e++) top = fmaxf(top, f[e]);
+#pragma unroll
+            for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(resident + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        }
 #pragma unroll 4
-        for (int i = tid; i < n; i += SR_THREADS) {
-            const float l = value(i);
-            const u64 m = sr_kept(r, l, first + i) ? measure(l) : 0ull;
-            const int b = sr_bin(r.max_value, l);
-            if (!wide) {
-                if (m != 0ull) atomicAdd(&sh.part[0][b], 1u);
-            } else {
-                const unsigned p0 = (unsigned)m & low_bits, p1 = (unsigned)(m >> part_bits) & low_bits, p2 = (unsigned)(m >> (2 * part_bits));
-                if (p0) atomicAdd(&sh.part[0][b], p0);
-                if (p1) atomicAdd(&sh.part[1][b], p1);
-                if (p2) atomicAdd(&sh.part[2][b], p2);
-            }
+        for (int i = whole + tid; i < n; i += SR_THREADS) {
+            const float f = to_f32(src[first + i]);
+            resident[i] = f;
+            top = fmaxf(top, f);                        // (the other one of a NaN)
         }
-        sr_cluster_sync();
-        // this block's share of the bins, for all blocks: up to 4 neighbouring ones a thread
-        const int share = SR_BINS / C, q = share < SR_THREADS ? 1 : share / SR_THREADS;
-        u64 sum[SR_BINS / SR_THREADS], mine = 0;
-#pragma unroll
-        for (int j = 0; j < SR_BINS / SR_THREADS; j++) {
-            sum[j] = 0;
-            if (j < q && tid * q + j < share)
-                for (int c = 0; c < C; c++) {
-                    const int b = (int)rank * share + tid * q + j;
-                    sum[j] += sr_load_remote(&sh.part[0][b], c);
-                    if (wide) sum[j] += ((u64)sr_load_remote(&sh.part[1][b], c) << part_bits) + ((u64)sr_load_remote(&sh.part[2][b], c) << (2 * part_bits));
-                }
-            mine += sum[j];
-        }
-        const u64 block = sr_block_sum(sh, mine), *totals = sr_exchange(sh, turn, block, C, rank);
-        u64 whole = 0, before = 0;
-        for (int c = 0; c < C; c++) {
-            if (c < (int)rank) before += totals[c];
-            whole += totals[c];
-        }
-        target = target_of(whole);
-        if (whole < target) return false;
-        if (before < target && before + block >= target) {          // the block in whose share it falls
-            for (int w = 0; w < warp; w++) before += sh.warp_sum[w];
-            before += sr_warp_scan(mine) - mine;
-#pragma unroll
-            for (int j = 0; j < SR_BINS / SR_THREADS; j++) {
-                if (j < q && before < target && before + sum[j] >= target) {
-                    tell_all(1, (u64)((int)rank * share + tid * q + j));
-                    tell_all(2, before);
-                    tell_all(3, sum[j]);
-                }
-                before += sum[j];
-            }
-        }
-        sr_cluster_sync();
-        bin = (int)sh.found[1], above = sh.found[2], inside = sh.found[3];
-        return true;
-    };
-    // Narrows the cut to the shortest prefix of the kept words whose measure reaches the target, given its bin.
-    auto cut_in_bin = [&](int bin, u64 above, u64 target, auto measure) {
-        const unsigned words = gather([&](float l) { return sr_bin(r.max_value, l) == bin; });
-        if (words <= SR_LIST) {
-            if (rank == 0) {
-                SrList w;
-                int bits;
-                take_list(w, (int)words, bits);
-                u64 m[SR_PER], last = ~0ull;
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? measure(w.value(e)) : 0ull;
-                const u64 cut = sr_list_cut(sh, w, m, target - above, bits);
-                // the last word of the prefix: the smallest order that is kept
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++)
-                    if (e < w.n && m[e] != 0ull && w.order(e) >= cut && w.order(e) < last) last = w.order(e);
-                const unsigned high = ~sr_block_max(sh, ~(unsigned)(last >> 32)), low = ~sr_block_max(sh, (unsigned)(last >> 32) == high ? ~(unsigned)last : 0u);
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++)
-                    if (e < w.n && w.order(e) == (((u64)high << 32) | low))
-                        tell_all(1, ((u64)__float_as_uint(w.value(e)) << 32) | (unsigned)sh.id[w.at + e]);
-            }
-            sr_cluster_sync();
-            r.cut = __uint_as_float((unsigned)(sh.found[1] >> 32));
-            r.cut_id = (int)(unsigned)sh.found[1];
-            return;
-        }
-        unsigned hi = 0, lo = 0;                        // the bin's largest key, and its smallest one's complement
-        for (int i = tid; i < n; i += SR_THREADS) {
-            const float l = value(i);
-            if (sr_kept(r, l, first + i) && sr_bin(r.max_value, l) == bin) {
-                const unsigned k = sr_key(l);
-                hi = max(hi, k);
-                lo = max(lo, ~k);
-            }
-        }
-        const u64* e = sr_exchange(sh, turn, sr_block_max(sh, hi), C, rank);
-        for (int c = 0; c < C; c++) hi = max(hi, (unsigned)e[c]);
-        e = sr_exchange(sh, turn, sr_block_max(sh, lo), C, rank);
-        for (int c = 0; c < C; c++) lo = max(lo, (unsigned)e[c]);
-        // (a thread's own maximum is not above the cluster's)
-        cut_by_cluster((u64)~lo, (u64)hi + 1, above, target, measure);
-    };
+    }
+    SrRow r;
+    r.max_value = sr_value(k.cluster_max(sr_key(top)));
+    if (r.max_value == -INFINITY) {                     // nothing can come: the same in all blocks
+        if (rank == 0 && tid == 0) out[at_row] = -1;
+        return;
+    }
+    if (!(temp > 0.f)) {                                // the largest comes, the lowest id of equals
+        unsigned least = 0;                             // its complement, for a maximum
+        for (int i = tid; i < n; i += SR_THREADS)
+            if (resident[i] == r.max_value) { least = 0x7fffffff - (first + i); break; }
+        least = k.cluster_max(least);
+        if (rank == 0 && tid == 0) out[at_row] = 0x7fffffff - (int)least;
+        return;
+    }
+    r.inv_temp = 16.0 * 1.44269504088896340736 / (double)temp;
+    r.max_wide = (double)r.max_value;
+    r.one = 1ull << S;
+    r.unit = (double)r.one;
+    r.min_p = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
+    r.low = r.max_value == INFINITY ? 3.402823466e38f : -INFINITY;
+    r.cut = -INFINITY;
+    r.cut_id = -1;
     auto one = [](float) { return 1ull; };
     auto weight_of = [&](float l) { return sr_weight<false>(r, sh.table, l); };
-    int bin;
-    u64 above, inside, target;
-
-    // 2. the cuts
-    if (top_k > 0 && top_k < V && bin_of([&](u64) { return (u64)top_k; }, one, false, bin, above, inside, target)) {
-        if (above + inside <= SR_LIST) {
-            // few words: the first block takes them all and finishes the row
-            const int words = (int)gather([&](float l) { return sr_bin(r.max_value, l) <= bin; });
-            if (rank != 0) return;
-            SrList w;
-            int bits;
-            take_list(w, words, bits);
-            u64 m[SR_PER], mine = 0, whole;
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? 1ull : 0ull;
-            u64 cut = sr_list_cut(sh, w, m, target, bits);
-            if (top_p < 1.0f) {
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= cut ? weight_of(w.value(e)) : 0ull;
-                cut = sr_list_cut(sh, w, m, sr_top_p_target(top_p, sr_block_sum(sh, mine)), bits);
-            }
-            mine = 0;
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= cut ? sr_weight<true>(r, sh.table, w.value(e)) : 0ull;
-            u64 before = sr_block_before(sh, mine, whole);
-            const u64 t = sr_draw_target(u, whole);
-            if (before <= t && before + mine > t) {
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++) {
-                    if (before <= t && before + m[e] > t) out[row] = sh.id[w.at + e];
-                    before += m[e];
-                }
-            }
-            return;
-        }
-        cut_in_bin(bin, above, target, one);
-    }
-    if (top_p < 1.0f && bin_of([&](u64 whole) { return sr_top_p_target(top_p, whole); }, weight_of, true, bin, above, inside, target))
-        cut_in_bin(bin, above, target, weight_of);
-
-    // 3. the draw
     auto weight = [&](int i) {
-        const float l = value(i);
+        const float l = resident[i];
         const u64 w = sr_weight<true>(r, sh.table, l);
         return sr_kept(r, l, first + i) ? w : 0ull;
     };
+    // In the first block, the cut among its list's words.
+    auto cut_in_list = [&](int words, u64 target, auto measure) {
+        if (rank == 0) {
+            SrList w;
+            w.take(sh, words);
+            u64 m[SR_PER];
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? measure(w.value(e)) : 0ull;
+            const u64 last = w.cut(sh, m, target);
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++)
+                if (e < w.n && w.order(e) == last) k.tell_all(((u64)__float_as_uint(w.value(e)) << 32) | (unsigned)sh.id[w.at + e]);
+        }
+        sr_cluster_sync();
+        r.cut = __uint_as_float((unsigned)(sh.found >> 32));
+        r.cut_id = (int)(unsigned)sh.found;
+    };
+    // The token, from this thread's part of its warp's run's sum.
+    auto draw = [&](u64 mine) {
+        const u64 block[1] = {sr_block_sum(sh, mine)};
+        const u64(*e)[SR_MAX_CLUSTER] = k.exchange(block);
+        u64 total = 0;
+        for (int c = 0; c < C; c++) total += e[0][c];
+        const int id = k.find(sr_draw_target(u, total), e[0], weight);
+        if (rank == 0 && tid == 0) out[at_row] = id;
+    };
+    int bin;
+    float before, inside;
+
+    // 2. top_k
+    if (top_k > 0 && top_k < V && k.bin_of<false>(r, (float)top_k, part_bits, bin, before, inside)) {
+        const float to = sr_edge(bin + 1);
+        if (before + inside <= (float)SR_LIST) {
+            // few words: the first block takes them all and finishes the row
+            const int words = (int)k.gather(r, 0.f, to);
+            if (rank != 0) return;
+            SrList w;
+            w.take(sh, words);
+            u64 m[SR_PER], mine = 0, whole;
+            if (words <= SR_FEW) {
+                // few enough to compare each with each (a word to a thread's place, 4 threads to a word)
+                if (w.n) sh.few_order[w.at] = w.order(0);
+                __syncthreads();
+                const u64 o = tid / 4 < words ? sh.few_order[tid / 4] : 0ull;
+                unsigned ahead = 0;
+                for (int j = tid & 3; j < words; j += 4) ahead += sh.few_order[j] > o;
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
+                if ((tid & 3) == 0 && tid / 4 < words) sh.few_at[ahead] = tid / 4;
+                __syncthreads();
+                if (warp != 0) return;
+                // a warp over the words in the row's order, 4 a lane, ...
+                constexpr int Q = SR_FEW / 32;
+                const int kept = min(top_k, words);
+                int at[Q];
+                u64 q[Q];
+#pragma unroll
+                for (int e = 0; e < Q; e++) {
+                    const int i = lane * Q + e;
+                    at[e] = i < words ? (int)sh.few_at[i] : -1;
+                    mine += q[e] = i < kept ? weight_of(sh.value[at[e]]) : 0ull;
+                }
+                u64 run = sr_warp_scan(mine);
+                const u64 target = top_p < 1.0f ? sr_top_p_target(top_p, __shfl_sync(0xffffffffu, run, 31)) : ~0ull;
+                run -= mine;
+                // ... their weights back into ascending order of the id
+#pragma unroll
+                for (int e = 0; e < Q; e++)
+                    if (at[e] >= 0) {
+                        sh.few_weight[at[e]] = lane * Q + e < kept && run < target ? sr_weight<true>(r, sh.table, sh.value[at[e]]) : 0ull;
+                        run += q[e];
+                    }
+                __syncwarp();
+                mine = 0;
+#pragma unroll
+                for (int e = 0; e < Q; e++) mine += q[e] = lane * Q + e < words ? sh.few_weight[lane * Q + e] : 0ull;
+                run = sr_warp_scan(mine);
+                const u64 t = sr_draw_target(u, __shfl_sync(0xffffffffu, run, 31));
+                run -= mine;
+#pragma unroll
+                for (int e = 0; e < Q; e++) {
+                    if (run <= t && run + q[e] > t) out[at_row] = sh.id[lane * Q + e];
+                    run += q[e];
+                }
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? 1ull : 0ull;
+            u64 last = w.cut(sh, m, (u64)top_k);
+            if (top_p < 1.0f) {
+#pragma unroll
+                for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= last ? weight_of(w.value(e)) : 0ull;
+                last = w.cut(sh, m, sr_top_p_target(top_p, sr_block_sum(sh, mine)));
+            }
+            mine = 0;
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= last ? sr_weight<true>(r, sh.table, w.value(e)) : 0ull;
+            u64 run = sr_block_before(sh, mine, whole);
+            const u64 t = sr_draw_target(u, whole);
+#pragma unroll
+            for (int e = 0; e < SR_PER; e++) {
+                if (run <= t && run + m[e] > t) out[at_row] = sh.id[w.at + e];
+                run += m[e];
+            }
+            return;
+        }
+        const float from = sr_edge(bin);
+        const unsigned words = k.gather(r, from, to);
+        if (words <= SR_LIST) cut_in_list((int)words, (u64)top_k - (u64)before, one);
+        else k.cut_by_cluster(r, from, to, (u64)before, (u64)top_k, one);
+    }
+
+    // 3. top_p
+    if (top_p < 1.0f) {
+        k.bin_of<true>(r, fmaxf(top_p, 0.f), part_bits, bin, before, inside);
+        u64 target;
+        float from, to;
+        const u64(*e)[SR_MAX_CLUSTER];
+        u64 above = 0, within = 0;
+        unsigned count, at, words;
+        for (;;) {
+            from = sr_edge(bin), to = sr_edge(bin + 1);
+            u64 sum = 0, ahead = 0, own = 0;
+            count = 0;
+#pragma unroll 2
+            for (int i = s0; i < s1; i += 32) {
+                const float l = i + lane < s1 ? resident[i + lane] : -INFINITY, d = sr_distance(r.max_value, l);
+                const bool kept = sr_kept(r, l, first + i + lane), here = kept & (d >= from) & ((d < to) | (to == INFINITY));
+                const u64 w = sr_weight<false>(r, sh.table, l), m = kept ? w : 0ull;
+                sum += m;
+                ahead += d < from ? m : 0ull;
+                own += here ? m : 0ull;
+                const unsigned all = __ballot_sync(0xffffffffu, here);
+                count += __popc(all);
+                if (lane == 0) k.mask[i >> 5] = all;
+            }
+            u64 mine[4];
+            mine[0] = sr_block_sum(sh, sum);
+            mine[2] = sr_block_sum(sh, own);
+            mine[3] = sr_block_sum(sh, lane == 0 ? count : 0u);
+            at = 0;
+#pragma unroll
+            for (int q = 0; q < SR_WARPS; q++) at += q < warp ? (unsigned)sh.warp_sum[q] : 0u;
+            mine[1] = sr_block_sum(sh, ahead);
+            if (tid < SR_WARPS) sh.warp_above[tid] = sh.warp_sum[tid];
+            e = k.exchange(mine);
+            u64 total = 0;
+            above = within = 0;
+            words = 0;
+            for (int c = 0; c < C; c++) {
+                total += e[0][c];
+                above += e[1][c];
+                within += e[2][c];
+                if (c < (int)rank) at += (unsigned)e[3][c];
+                words += (unsigned)e[3][c];
+            }
+            target = sr_top_p_target(top_p, total);
+            if (above >= target) bin--;                 // (the histogram's rounding, at a bin's border)
+            else if (above + within < target) bin++;
+            else break;
+        }
+        if (words > SR_LIST) {
+            k.cut_by_cluster(r, from, to, above, target, weight_of);
+        } else {
+            k.push(count, at);
+            cut_in_list((int)words, target - above, weight_of);
+            if (!(min_p > 0.f)) {
+                // the runs' sums: what is ahead of the bin, and the bin's words that are kept
+                u64 mine = lane == 0 ? sh.warp_above[warp] : 0ull;
+                for (int i0 = s0; i0 < s1 && count != 0; i0 += 1024) {
+                    const int i = i0 + lane * 32;
+                    for (unsigned m = i < s1 ? k.mask[i >> 5] : 0u; m; m &= m - 1) mine += weight(i + __ffs(m) - 1);
+                }
+                draw(mine);
+                return;
+            }
+        }
+    }
+
+    // 4. the draw.  Words so far that min_p leaves them out are passed over without their weight (a margin of 2^-16 for the rounding).
+    float far = min_p > 0.f ? (float)(log(1.0 / r.min_p) * (double)temp) * 1.0000153f + 1e-30f : INFINITY;
+    if (!(far < INFINITY)) far = INFINITY;              // (an infinite temperature)
     u64 mine = 0;
+    if (far == INFINITY) {
 #pragma unroll 4
-    for (int i = s0 + lane; i < s1; i += 32) mine += weight(i);
-    const u64* totals = sr_exchange(sh, turn, sr_block_sum(sh, mine), C, rank);
-    u64 total = 0;
-    for (int c = 0; c < C; c++) total += totals[c];
-    const int id = find(sr_draw_target(u, total), totals, weight);
-    if (rank == 0 && tid == 0) out[row] = id;
+        for (int i = s0 + lane; i < s1; i += 32) mine += weight(i);
+        draw(mine);
+        return;
+    }
+    for (int i = s0; i < s1; i += 32) {
+        const float l = i + lane < s1 ? resident[i + lane] : -INFINITY;
+        const bool kept = sr_kept(r, l, first + i + lane) & (sr_distance(r.max_value, l) <= far);
+        if (__any_sync(0xffffffffu, kept)) {
+            const u64 w = sr_weight<true>(r, sh.table, l);
+            mine += kept ? w : 0ull;
+        }
+    }
+    draw(mine);
 }
 
 template <typename TIn>
@@ -641,11 +775,8 @@ static int sr_launch(const void* logits, long long ld, int B, int V, int C, cons
     int log_v = 0, log_chunk = 0;
     while ((1 << log_v) < V) log_v++;
     while ((1 << log_chunk) < chunk) log_chunk++;
-    // a row's sum stays below 2^62; a part of the histogram, times a block's words, below 2^32
-    const int part_bits = 32 - log_chunk - 1;
-    int S = 62 - log_v;
-    S = S > 50 ? 50 : S;
-    S = S > 3 * part_bits ? 3 * part_bits : S;
+    // a row's sum stays below 2^62; a bin's float32 weights in units of 2^-part_bits, a block's words at most, below 2^32
+    const int part_bits = log_chunk > 9 ? 31 - log_chunk : 22, S = log_v > 12 ? 62 - log_v : 50;
     const size_t smem = sizeof(SrShared) + (size_t)chunk * sizeof(float) + (size_t)(chunk / 32 + SR_WARPS + 1) * sizeof(unsigned);
     auto kern = sample_rows_kernel<TIn>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
