@@ -43,8 +43,7 @@
 #define SR_BINS 2048
 #define SR_GROUPS 32                // groups of bins
 #define SR_GROUP (SR_BINS / SR_GROUPS)
-#define SR_PER 8
-#define SR_LIST (SR_THREADS * SR_PER)       // words that one block takes to itself
+#define SR_LIST 4096                 // words that one block takes to itself
 #define SR_LIST_BITS 12
 #define SR_FEW 128                  // words that are ranked by comparing each with each
 
@@ -137,6 +136,7 @@ __device__ __forceinline__ u64 sr_weight(const SrRow& r, const double* table, fl
     if ((unsigned)__double2hiint(x) > 0xC0900000u) units = 0ull;      // x < -1024: less than 2^-64
     return l == r.max_value ? r.one : units;
 }
+__device__ __forceinline__ u64 sr_measure(const SrRow& r, const double* table, float l, bool weights) { return weights ? sr_weight<false>(r, table, l) : 1ull; }
 // whether a word can come and is still kept (no branch: the loops over the row are bound by how many of their loads and chains overlap)
 __device__ __forceinline__ bool sr_kept(const SrRow& r, float l, int id) { return (l > r.low) & ((l > r.cut) | ((l == r.cut) & (id <= r.cut_id))); }
 
@@ -240,9 +240,17 @@ struct SrBlock {
         for (int c = 0; c < C; c++) sr_store_remote(&sh.found, c, v);
     }
 
-    // The first id, ascending, at which the sum of measure(i) over the ids up to it exceeds t; every thread of the cluster
+    // What word i adds to a sum in ascending order of the id: its weight if it is kept, or (ties) 1 if it equals `value` and is kept.
+    __device__ __forceinline__ u64 part(const SrRow& r, bool ties, float value, int i) const {
+        const float l = row[i];
+        const bool kept = sr_kept(r, l, first + i);
+        if (ties) return (l == value) & kept ? 1ull : 0ull;
+        const u64 w = sr_weight<true>(r, sh.table, l);
+        return kept ? w : 0ull;
+    }
+    // The first id, ascending, at which the sum of part(i) over the ids up to it exceeds t; every thread of the cluster
     // gets it.  totals: the blocks' sums, sh.warp_sum the warps'.  The whole sum must exceed t.
-    template <typename F> __device__ __forceinline__ int find(u64 t, const u64* totals, F measure) {
+    __device__ __forceinline__ int find(const SrRow& r, u64 t, const u64* totals, bool ties, float value) {
         u64 before = 0;
         int owner = 0;
         for (; owner < C - 1 && before + totals[owner] <= t; owner++) before += totals[owner];
@@ -256,7 +264,7 @@ struct SrBlock {
             const int e = min(n, (w + 1) * seg);
             for (int i0 = w * seg; i0 < e; i0 += SR_THREADS) {
                 const int i = i0 + tid;
-                mine = i < e ? measure(i) : 0ull;
+                mine = i < e ? part(r, ties, value, i) : 0ull;
                 u64 whole;
                 const u64 prior = before + sr_block_before(sh, mine, whole);
                 if (prior <= t && prior + mine > t) tell_all((u64)(first + i));
@@ -369,8 +377,8 @@ struct SrBlock {
     }
 
     // The whole cluster's bisection among the kept words at distances of [from, to), for bins that no list holds: the cut of the
-    // shortest prefix whose measure reaches `target`, `above` being the measure of the words before these.
-    template <typename F> __device__ __forceinline__ void cut_by_cluster(SrRow& r, float from, float to, u64 above, u64 target, F measure) {
+    // shortest prefix whose count, or weight, reaches `target`, `above` being that of the words before these.
+    __device__ __forceinline__ void cut_by_cluster(SrRow& r, float from, float to, u64 above, u64 target, bool weights) {
         unsigned most = 0, least = 0;                   // the largest key, and the smallest one's complement
         for (int i = tid; i < n; i += SR_THREADS) {
             const float l = row[i], d = sr_distance(r.max_value, l);
@@ -387,7 +395,7 @@ struct SrBlock {
             for (int i = tid; i < n; i += SR_THREADS) {
                 const float l = row[i];
                 const unsigned k = sr_key(l);
-                if (sr_kept(r, l, first + i) & (k >= mid) & (k < hi)) mine += measure(l);
+                if (sr_kept(r, l, first + i) & (k >= mid) & (k < hi)) mine += sr_measure(r, sh.table, l, weights);
             }
             const u64 m = cluster_sum(mine);
             if (above + m >= target) lo = mid;
@@ -395,107 +403,112 @@ struct SrBlock {
         }
         // of the words with this very value as many as are needed, in ascending order of their id
         const float cut = sr_value((unsigned)lo);
-        const u64 each = measure(cut), need = (target - above + each - 1) / each;
-        auto tie = [&](int i) { return (row[i] == cut) & sr_kept(r, row[i], first + i) ? 1ull : 0ull; };
+        const u64 each = sr_measure(r, sh.table, cut, weights), need = (target - above + each - 1) / each;
         u64 mine = 0;
-        for (int i = s0 + lane; i < s1; i += 32) mine += tie(i);
+        for (int i = s0 + lane; i < s1; i += 32) mine += part(r, true, cut, i);
         const u64 m[1] = {sr_block_sum(sh, mine)};
         const u64(*e)[SR_MAX_CLUSTER] = exchange(m);
-        const int id = find(need - 1, e[0], tie);
+        const int id = find(r, need - 1, e[0], true, cut);
         r.cut = cut;
         r.cut_id = id;
     }
 };
 
-// A list of at most SR_LIST words in ascending order of their id, dealt to the block's threads in runs.  order: key above the list's
-// smallest key, and below it the complement of the place: larger means earlier in the row's order.
+// The two out of line, by value: what a function takes by its address stays in memory for the loops over the row as well.
+__device__ __noinline__ int sr_find(SrBlock k, SrRow r, u64 t, const u64* totals) { return k.find(r, t, totals, false, 0.f); }
+struct SrCut {
+    float cut;
+    int id, turn;
+};
+__device__ __noinline__ SrCut sr_cut_by_cluster(SrBlock k, SrRow r, float from, float to, u64 above, u64 target, bool weights) {
+    k.cut_by_cluster(r, from, to, above, target, weights);
+    return SrCut{r.cut, r.cut_id, k.turn};
+}
+
+// The first block's list: `words` of them in sh.value and sh.id, in ascending order of the id.  A word's order is its key above the
+// list's smallest, and below that the complement of its place: larger means earlier in the row's order.
+// (This part runs once per row, on one block: short code counts, since it comes from memory, not from the instruction cache.)
 struct SrList {
-    unsigned key[SR_PER];   // above the list's smallest
-    unsigned least;         // that one
-    int n, at, bits;        // words of this thread, place of the first, bits of an order
-    __device__ __forceinline__ u64 order(int e) const { return ((u64)key[e] << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - at - e); }
-    __device__ __forceinline__ float value(int e) const { return sr_value(key[e] + least); }
-    __device__ __forceinline__ void take(SrShared& sh, int words) {
-        const int per = (words + SR_THREADS - 1) / SR_THREADS;
-        at = threadIdx.x * per;
-        n = max(0, min(per, words - at));
-        unsigned most = 0, low = 0;                     // the smallest key's complement
-#pragma unroll
-        for (int e = 0; e < SR_PER; e++)
-            if (e < n) {
-                key[e] = sr_key(sh.value[at + e]);
-                most = max(most, key[e]);
-                low = max(low, ~key[e]);
-            }
-        most = sr_block_max(sh, most);
-        least = ~sr_block_max(sh, low);
-#pragma unroll
-        for (int e = 0; e < SR_PER; e++) key[e] -= least;
-        bits = 64 - __clzll(((u64)(most - least) << SR_LIST_BITS) | (SR_LIST - 1));
+    unsigned least;         // the smallest key
+    int bits;               // of an order
+};
+__device__ __forceinline__ u64 sr_order(const SrShared& sh, const SrList& w, int i) {
+    return ((u64)(sr_key(sh.value[i]) - w.least) << SR_LIST_BITS) | (unsigned)(SR_LIST - 1 - i);
+}
+__device__ __noinline__ SrList sr_list(SrShared& sh, int words) {
+    unsigned most = 0, low = 0;                         // the largest key, and the smallest one's complement
+#pragma unroll 1
+    for (int i = threadIdx.x; i < words; i += SR_THREADS) {
+        const unsigned k = sr_key(sh.value[i]);
+        most = max(most, k);
+        low = max(low, ~k);
     }
-    // The order of the last word of the shortest prefix, largest order first, whose measure (m[e] of word e) reaches `target`,
-    // which all of them do.  By digits of 8 bits, until one holds at most 32 words, which every warp ranks by itself.
-    __device__ __forceinline__ u64 cut(SrShared& sh, const u64* m, u64 target) const {
-        const int tid = threadIdx.x, lane = tid & 31;
-        u64 prefix = 0, above = 0;
-        int shift = bits;
-        for (int turn = 0;; turn ^= 1) {
-            unsigned *count = sh.digits[turn].count, *lo = sh.digits[turn].lo, *hi = sh.digits[turn].hi;
-            for (int i = tid; i < 256; i += SR_THREADS) count[i] = lo[i] = hi[i] = 0u;
-            if (tid == 0) sh.n_few = 0;
-            __syncthreads();
-            const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++)
-                if (e < n && m[e] != 0ull && order(e) >> shift == prefix) {
-                    const int d = (int)(order(e) >> down) & ((1 << width) - 1);
-                    const unsigned low = (unsigned)m[e], carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
-                    if ((unsigned)(m[e] >> 32) + carry != 0u) atomicAdd(&hi[d], (unsigned)(m[e] >> 32) + carry);
-                    atomicAdd(&count[d], 1u);
-                }
-            __syncthreads();
-            // every warp by itself: 8 digits a lane, the largest first
-            u64 mine = 0;
-#pragma unroll
-            for (int q = 0; q < 8; q++) mine += ((u64)hi[255 - (lane * 8 + q)] << 32) + lo[255 - (lane * 8 + q)];
-            u64 before = above + sr_warp_scan(mine) - mine;
-            const int owner = __ffs(__ballot_sync(0xffffffffu, before + mine >= target)) - 1;
-            int digit = 0;
-            bool open = true;
-#pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const u64 s = ((u64)hi[255 - (lane * 8 + q)] << 32) + lo[255 - (lane * 8 + q)];
-                if (open && before + s >= target) {
-                    digit = 255 - (lane * 8 + q);
-                    open = false;
-                }
-                if (open) before += s;
+    most = sr_block_max(sh, most);
+    const unsigned least = ~sr_block_max(sh, low);
+    return SrList{least, 64 - __clzll(((u64)(most - least) << SR_LIST_BITS) | (SR_LIST - 1))};
+}
+// The order of the last word of the shortest prefix, largest order first, whose count, or weight, reaches `target`, which that of
+// the words with an order of at least `from` does.  By digits of 8 bits, until one holds at most 32 words, which every warp
+// ranks by itself.
+__device__ __noinline__ u64 sr_list_cut(SrShared& sh, SrRow r, SrList w, int words, u64 from, bool weights, u64 target) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    u64 prefix = 0, above = 0;
+    int shift = w.bits;
+#pragma unroll 1
+    for (int turn = 0;; turn ^= 1) {
+        unsigned *count = sh.digits[turn].count, *lo = sh.digits[turn].lo, *hi = sh.digits[turn].hi;
+        if (tid < 256) count[tid] = lo[tid] = hi[tid] = 0u;
+        if (tid == 0) sh.n_few = 0;
+        __syncthreads();
+        const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
+#pragma unroll 1
+        for (int i = tid; i < words; i += SR_THREADS) {
+            const u64 o = sr_order(sh, w, i);
+            if (o < from || o >> shift != prefix) continue;
+            const u64 m = sr_measure(r, sh.table, sh.value[i], weights);
+            const int d = (int)(o >> down) & ((1 << width) - 1);
+            const unsigned low = (unsigned)m, carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
+            if ((unsigned)(m >> 32) + carry != 0u) atomicAdd(&hi[d], (unsigned)(m >> 32) + carry);
+            atomicAdd(&count[d], 1u);
+        }
+        __syncthreads();
+        // every warp by itself: 8 digits a lane, the largest first
+        u64 mine = 0;
+#pragma unroll 1
+        for (int q = 0; q < 8; q++) mine += ((u64)hi[255 - (lane * 8 + q)] << 32) + lo[255 - (lane * 8 + q)];
+        u64 before = above + sr_warp_scan(mine) - mine;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, before + mine >= target)) - 1;
+        int digit = 255 - lane * 8;
+#pragma unroll 1
+        for (int q = 0; q < 7; q++, digit--) {
+            const u64 s = ((u64)hi[digit] << 32) + lo[digit];
+            if (before + s >= target) break;
+            before += s;
+        }
+        digit = __shfl_sync(0xffffffffu, digit, owner);
+        above = __shfl_sync(0xffffffffu, before, owner);
+        prefix = (prefix << width) | (unsigned)digit;
+        shift = down;
+        const int few = (int)count[digit];
+        if (few <= 32) {
+#pragma unroll 1
+            for (int i = tid; i < words; i += SR_THREADS) {
+                const u64 o = sr_order(sh, w, i);
+                if (o < from || o >> shift != prefix) continue;
+                const unsigned to = atomicAdd(&sh.n_few, 1u);
+                sh.few_order[to] = o;
+                sh.few_weight[to] = sr_measure(r, sh.table, sh.value[i], weights);
             }
-            digit = __shfl_sync(0xffffffffu, digit, owner);
-            above = __shfl_sync(0xffffffffu, before, owner);
-            prefix = (prefix << width) | (unsigned)digit;
-            shift = down;
-            const unsigned words = count[digit];
-            if (words <= 32) {
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++)
-                    if (e < n && m[e] != 0ull && order(e) >> shift == prefix) {
-                        const unsigned to = atomicAdd(&sh.n_few, 1u);
-                        sh.few_order[to] = order(e);
-                        sh.few_weight[to] = m[e];
-                    }
-                __syncthreads();
-                const u64 o = lane < (int)words ? sh.few_order[lane] : 0ull, w = lane < (int)words ? sh.few_weight[lane] : 0ull;
-                u64 sum = above;
-                for (int j = 0; j < (int)words; j++) sum += sh.few_order[j] > o ? sh.few_weight[j] : 0ull;
-                const int last = __ffs(__ballot_sync(0xffffffffu, lane < (int)words && sum < target && sum + w >= target)) - 1;
-                const u64 result = __shfl_sync(0xffffffffu, o, last);
-                __syncthreads();
-                return result;
-            }
+            __syncthreads();
+            const u64 o = lane < few ? sh.few_order[lane] : 0ull, m = lane < few ? sh.few_weight[lane] : 0ull;
+            u64 sum = above;
+#pragma unroll 1
+            for (int q = 0; q < few; q++) sum += sh.few_order[q] > o ? sh.few_weight[q] : 0ull;
+            const int last = __ffs(__ballot_sync(0xffffffffu, lane < few && sum < target && sum + m >= target)) - 1;
+            return __shfl_sync(0xffffffffu, o, last);
         }
     }
-};
+}
 
 template <typename TIn>
 __global__ void __launch_bounds__(SR_THREADS, 2)
@@ -561,41 +574,27 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     r.low = r.max_value == INFINITY ? 3.402823466e38f : -INFINITY;
     r.cut = -INFINITY;
     r.cut_id = -1;
-    auto one = [](float) { return 1ull; };
-    auto weight_of = [&](float l) { return sr_weight<false>(r, sh.table, l); };
-    auto weight = [&](int i) {
-        const float l = resident[i];
-        const u64 w = sr_weight<true>(r, sh.table, l);
-        return sr_kept(r, l, first + i) ? w : 0ull;
+    auto cut_by_cluster = [&](float from, float to, u64 above, u64 target, bool weights) {
+        const SrCut c = sr_cut_by_cluster(k, r, from, to, above, target, weights);
+        r.cut = c.cut;
+        r.cut_id = c.id;
+        k.turn = c.turn;
     };
-    // In the first block, the cut among its list's words.
-    auto cut_in_list = [&](int words, u64 target, auto measure) {
+    // The cut among the first block's list, by that block.
+    auto cut_in_list = [&](int words, bool weights, u64 target) {
         if (rank == 0) {
-            SrList w;
-            w.take(sh, words);
-            u64 m[SR_PER];
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? measure(w.value(e)) : 0ull;
-            const u64 last = w.cut(sh, m, target);
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++)
-                if (e < w.n && w.order(e) == last) k.tell_all(((u64)__float_as_uint(w.value(e)) << 32) | (unsigned)sh.id[w.at + e]);
+            const SrList w = sr_list(sh, words);
+            const int i = SR_LIST - 1 - (int)(sr_list_cut(sh, r, w, words, 0ull, weights, target) & (SR_LIST - 1));
+            if (tid < C) sr_store_remote(&sh.found, tid, ((u64)__float_as_uint(sh.value[i]) << 32) | (unsigned)sh.id[i]);
         }
         sr_cluster_sync();
         r.cut = __uint_as_float((unsigned)(sh.found >> 32));
         r.cut_id = (int)(unsigned)sh.found;
     };
-    // The token, from this thread's part of its warp's run's sum.
-    auto draw = [&](u64 mine) {
-        const u64 block[1] = {sr_block_sum(sh, mine)};
-        const u64(*e)[SR_MAX_CLUSTER] = k.exchange(block);
-        u64 total = 0;
-        for (int c = 0; c < C; c++) total += e[0][c];
-        const int id = k.find(sr_draw_target(u, total), e[0], weight);
-        if (rank == 0 && tid == 0) out[at_row] = id;
-    };
     int bin;
     float before, inside;
+    u64 mine = 0;               // of this thread, of the kept words of its warp's run
+    bool summed = false;
 
     // 2. top_k
     if (top_k > 0 && top_k < V && k.bin_of<false>(r, (float)top_k, part_bits, bin, before, inside)) {
@@ -604,80 +603,64 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             // few words: the first block takes them all and finishes the row
             const int words = (int)k.gather(r, 0.f, to);
             if (rank != 0) return;
-            SrList w;
-            w.take(sh, words);
-            u64 m[SR_PER], mine = 0, whole;
+            const SrList w = sr_list(sh, words);
             if (words <= SR_FEW) {
-                // few enough to compare each with each (a word to a thread's place, 4 threads to a word)
-                if (w.n) sh.few_order[w.at] = w.order(0);
+                // few enough to compare each with each, 4 threads to a word
+                if (tid < words) sh.few_order[tid] = sr_order(sh, w, tid);
                 __syncthreads();
                 const u64 o = tid / 4 < words ? sh.few_order[tid / 4] : 0ull;
                 unsigned ahead = 0;
+#pragma unroll 1
                 for (int j = tid & 3; j < words; j += 4) ahead += sh.few_order[j] > o;
                 ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
                 ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
                 if ((tid & 3) == 0 && tid / 4 < words) sh.few_at[ahead] = tid / 4;
                 __syncthreads();
-                if (warp != 0) return;
-                // a warp over the words in the row's order, 4 a lane, ...
-                constexpr int Q = SR_FEW / 32;
-                const int kept = min(top_k, words);
-                int at[Q];
-                u64 q[Q];
-#pragma unroll
-                for (int e = 0; e < Q; e++) {
-                    const int i = lane * Q + e;
-                    at[e] = i < words ? (int)sh.few_at[i] : -1;
-                    mine += q[e] = i < kept ? weight_of(sh.value[at[e]]) : 0ull;
-                }
-                u64 run = sr_warp_scan(mine);
-                const u64 target = top_p < 1.0f ? sr_top_p_target(top_p, __shfl_sync(0xffffffffu, run, 31)) : ~0ull;
-                run -= mine;
+                // the words in the row's order, one to a thread, ...
+                const int kept = min(top_k, words), at = tid < words ? (int)sh.few_at[tid] : -1;
+                const float l = at >= 0 ? sh.value[at] : r.max_value;
+                u64 m = tid < kept ? sr_weight<false>(r, sh.table, l) : 0ull, whole = 0, ahead_of = 0;
+                if (top_p < 1.0f) ahead_of = sr_block_before(sh, m, whole);
                 // ... their weights back into ascending order of the id
-#pragma unroll
-                for (int e = 0; e < Q; e++)
-                    if (at[e] >= 0) {
-                        sh.few_weight[at[e]] = lane * Q + e < kept && run < target ? sr_weight<true>(r, sh.table, sh.value[at[e]]) : 0ull;
-                        run += q[e];
-                    }
-                __syncwarp();
-                mine = 0;
-#pragma unroll
-                for (int e = 0; e < Q; e++) mine += q[e] = lane * Q + e < words ? sh.few_weight[lane * Q + e] : 0ull;
-                run = sr_warp_scan(mine);
-                const u64 t = sr_draw_target(u, __shfl_sync(0xffffffffu, run, 31));
-                run -= mine;
-#pragma unroll
-                for (int e = 0; e < Q; e++) {
-                    if (run <= t && run + q[e] > t) out[at_row] = sh.id[lane * Q + e];
-                    run += q[e];
-                }
+                if (at >= 0) sh.few_weight[at] = tid < kept && (top_p >= 1.0f || ahead_of < sr_top_p_target(top_p, whole)) ? sr_weight<true>(r, sh.table, l) : 0ull;
+                __syncthreads();
+                m = tid < words ? sh.few_weight[tid] : 0ull;
+                ahead_of = sr_block_before(sh, m, whole);
+                const u64 t = sr_draw_target(u, whole);
+                if (ahead_of <= t && ahead_of + m > t) out[at_row] = sh.id[tid];
                 return;
             }
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) m[e] = e < w.n ? 1ull : 0ull;
-            u64 last = w.cut(sh, m, (u64)top_k);
+            u64 last = sr_list_cut(sh, r, w, words, 0ull, false, (u64)top_k);
+            auto sum = [&] {
+                u64 mine = 0;
+#pragma unroll 1
+                for (int i = tid; i < words; i += SR_THREADS)
+                    if (sr_order(sh, w, i) >= last) mine += sr_weight<true>(r, sh.table, sh.value[i]);
+                return sr_block_sum(sh, mine);
+            };
+            const double min_p_given = r.min_p;
             if (top_p < 1.0f) {
-#pragma unroll
-                for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= last ? weight_of(w.value(e)) : 0ull;
-                last = w.cut(sh, m, sr_top_p_target(top_p, sr_block_sum(sh, mine)));
+                r.min_p = 0.0;                          // (it does not count for top_p's share)
+                last = sr_list_cut(sh, r, w, words, last, true, sr_top_p_target(top_p, sum()));
+                r.min_p = min_p_given;
             }
-            mine = 0;
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) mine += m[e] = e < w.n && w.order(e) >= last ? sr_weight<true>(r, sh.table, w.value(e)) : 0ull;
-            u64 run = sr_block_before(sh, mine, whole);
-            const u64 t = sr_draw_target(u, whole);
-#pragma unroll
-            for (int e = 0; e < SR_PER; e++) {
-                if (run <= t && run + m[e] > t) out[at_row] = sh.id[w.at + e];
-                run += m[e];
+            const u64 t = sr_draw_target(u, sum());
+            u64 ahead = 0;
+#pragma unroll 1
+            for (int i0 = 0; i0 < words; i0 += SR_THREADS) {
+                const int i = i0 + tid;
+                const u64 m = i < words && sr_order(sh, w, i) >= last ? sr_weight<true>(r, sh.table, sh.value[i]) : 0ull;
+                u64 whole;
+                const u64 prior = ahead + sr_block_before(sh, m, whole);
+                if (prior <= t && prior + m > t) out[at_row] = sh.id[i];
+                ahead += whole;
             }
             return;
         }
         const float from = sr_edge(bin);
         const unsigned words = k.gather(r, from, to);
-        if (words <= SR_LIST) cut_in_list((int)words, (u64)top_k - (u64)before, one);
-        else k.cut_by_cluster(r, from, to, (u64)before, (u64)top_k, one);
+        if (words <= SR_LIST) cut_in_list((int)words, false, (u64)top_k - (u64)before);
+        else cut_by_cluster(from, to, (u64)before, (u64)top_k, false);
     }
 
     // 3. top_p
@@ -704,16 +687,16 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
                 count += __popc(all);
                 if (lane == 0) k.mask[i >> 5] = all;
             }
-            u64 mine[4];
-            mine[0] = sr_block_sum(sh, sum);
-            mine[2] = sr_block_sum(sh, own);
-            mine[3] = sr_block_sum(sh, lane == 0 ? count : 0u);
+            u64 sums[4];
+            sums[0] = sr_block_sum(sh, sum);
+            sums[2] = sr_block_sum(sh, own);
+            sums[3] = sr_block_sum(sh, lane == 0 ? count : 0u);
             at = 0;
 #pragma unroll
             for (int q = 0; q < SR_WARPS; q++) at += q < warp ? (unsigned)sh.warp_sum[q] : 0u;
-            mine[1] = sr_block_sum(sh, ahead);
+            sums[1] = sr_block_sum(sh, ahead);
             if (tid < SR_WARPS) sh.warp_above[tid] = sh.warp_sum[tid];
-            e = k.exchange(mine);
+            e = k.exchange(sums);
             u64 total = 0;
             above = within = 0;
             words = 0;
@@ -730,42 +713,43 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             else break;
         }
         if (words > SR_LIST) {
-            k.cut_by_cluster(r, from, to, above, target, weight_of);
+            cut_by_cluster(from, to, above, target, true);
         } else {
             k.push(count, at);
-            cut_in_list((int)words, target - above, weight_of);
+            cut_in_list((int)words, true, target - above);
             if (!(min_p > 0.f)) {
                 // the runs' sums: what is ahead of the bin, and the bin's words that are kept
-                u64 mine = lane == 0 ? sh.warp_above[warp] : 0ull;
+                summed = true;
+                mine = lane == 0 ? sh.warp_above[warp] : 0ull;
                 for (int i0 = s0; i0 < s1 && count != 0; i0 += 1024) {
                     const int i = i0 + lane * 32;
-                    for (unsigned m = i < s1 ? k.mask[i >> 5] : 0u; m; m &= m - 1) mine += weight(i + __ffs(m) - 1);
+#pragma unroll 1
+                    for (unsigned m = i < s1 ? k.mask[i >> 5] : 0u; m; m &= m - 1) mine += k.part(r, false, 0.f, i + __ffs(m) - 1);
                 }
-                draw(mine);
-                return;
             }
         }
     }
 
     // 4. the draw.  Words so far that min_p leaves them out are passed over without their weight (a margin of 2^-16 for the rounding).
-    float far = min_p > 0.f ? (float)(log(1.0 / r.min_p) * (double)temp) * 1.0000153f + 1e-30f : INFINITY;
-    if (!(far < INFINITY)) far = INFINITY;              // (an infinite temperature)
-    u64 mine = 0;
-    if (far == INFINITY) {
+    if (!summed) {
+        float far = min_p > 0.f ? (float)(log(1.0 / r.min_p) * (double)temp) * 1.0000153f + 1e-30f : INFINITY;
+        if (!(far < INFINITY)) {                        // (or an infinite temperature)
 #pragma unroll 4
-        for (int i = s0 + lane; i < s1; i += 32) mine += weight(i);
-        draw(mine);
-        return;
-    }
-    for (int i = s0; i < s1; i += 32) {
-        const float l = i + lane < s1 ? resident[i + lane] : -INFINITY;
-        const bool kept = sr_kept(r, l, first + i + lane) & (sr_distance(r.max_value, l) <= far);
-        if (__any_sync(0xffffffffu, kept)) {
-            const u64 w = sr_weight<true>(r, sh.table, l);
-            mine += kept ? w : 0ull;
+            for (int i = s0 + lane; i < s1; i += 32) mine += k.part(r, false, 0.f, i);
+        } else {
+#pragma unroll 1
+            for (int i = s0; i < s1; i += 32) {
+                const float l = i + lane < s1 ? resident[i + lane] : -INFINITY;
+                if (sr_kept(r, l, first + i + lane) & (sr_distance(r.max_value, l) <= far)) mine += sr_weight<true>(r, sh.table, l);
+            }
         }
     }
-    draw(mine);
+    const u64 block[1] = {sr_block_sum(sh, mine)};
+    const u64(*e)[SR_MAX_CLUSTER] = k.exchange(block);
+    u64 total = 0;
+    for (int c = 0; c < C; c++) total += e[0][c];
+    const int id = sr_find(k, r, sr_draw_target(u, total), e[0]);
+    if (rank == 0 && tid == 0) out[at_row] = id;
 }
 
 template <typename TIn>
