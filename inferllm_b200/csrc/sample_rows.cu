@@ -775,9 +775,11 @@ extern "C" int illm_sample_rows(const void* logits, int dtype, int B, int V, lon
                                 const int* top_k, const float* top_p, const float* min_p, int* out, void* stream) {
     if (B <= 0) return 0;
     if (V <= 0 || V > SR_MAX_CLUSTER * SR_MAX_RESIDENT || B > (1 << 24) || ld < V || !logits || !uniforms || !out) return ILLM_ERR_BAD_ARG;
-    // blocks to a row: more while there are fewer than four to an SM and a block's run is worth a block, or does not fit it
+    // blocks to a row: more while there are fewer than two to an SM (which is what its registers hold) and a block's run is worth a
+    // block, or is more than two of them on an SM can keep.  256 rows of 32,000 words on 1, 2, 4, 8 blocks each: 72, 64, 76, 107 us;
+    // one row: 25, 21, 17, 16; 64 rows of 128,256 words on 4 and 8: 80 and 74.
     int C = 1;
-    while (C < SR_MAX_CLUSTER && (((V + C - 1) / C > 2048 && (long long)B * C < 4 * illm_sm_count()) || (V + C - 1) / C > SR_MAX_RESIDENT / 2)) C *= 2;
+    while (C < SR_MAX_CLUSTER && (((V + C - 1) / C > 2048 && (long long)B * C < 2 * illm_sm_count()) || (V + C - 1) / C > SR_MAX_RESIDENT / 2)) C *= 2;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == ILLM_F32) return sr_launch<float>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
     if (dtype == ILLM_BF16) return sr_launch<bf16>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
