@@ -6,7 +6,7 @@
 // Which token has which adapter comes as a plan (adapters.h).
 //
 // The general form (both types): the shared product by the package's own kernels into float32, then
-//   shrink   v[t] = s_a x[t] A_a^T: a block per 8 tokens of the plan's order and rank group, a warp per two ranks, which
+//   shrink   v[t] = s_a x[t] A_a^T: a block per 4 tokens of the plan's order and rank group, a warp per two ranks, which
 //            reads a row of A once for the tokens of a slot;
 //   expand   y[t, n] = base[t, n] + v[t] . B_a[n]: a thread per output column, the slot's 16 values of B in registers.
 // Sums are float32 in one order per token, whatever else is in the batch.
@@ -14,96 +14,95 @@
 #include "kernels.h"
 
 #define AD_TOKENS 8
+#define AD_SHRINK 4
 #define AD_COLS 128
 
-// v[t, 16 g + r] for the ranks of group g of token t's adapter, float32 [T, R]
-template <typename T>
+// v[t, 16 g + r] for the ranks of group g of token t's adapter, float32 [T, R]; W floats of a row at a time
+template <int W>
 __global__ void __launch_bounds__(256)
-adapter_shrink_kernel(const T* __restrict__ x, int K, const T* __restrict__ a, const float* __restrict__ scales, int R, const AdPlan plan, int tokens,
-                      float* __restrict__ v) {
+adapter_shrink_kernel(const float* __restrict__ x, int K, const float* __restrict__ a, const float* __restrict__ scales, int R, const int4* __restrict__ places,
+                      int tokens, float* __restrict__ v) {
     pdl_grid_sync();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
-    const int n_slots = plan.counts[0], p0 = blockIdx.x * AD_TOKENS, p1 = min(tokens, p0 + AD_TOKENS);
-    int slot = 0;
-    for (int p = p0; p < p1;) {
-        while (slot < n_slots && plan.slot_begin[slot + 1] <= p) slot++;
-        if (slot >= n_slots) return;                    // the rest has no adapter
-        const int e = min(p1, plan.slot_begin[slot + 1]), n = e - p;
-        if (g < plan.slot_group[slot + 1] - plan.slot_group[slot]) {
-            const int ad = plan.slot_adapter[slot];
-            const T* a0 = a + ((long long)ad * R + g * ADAPTER_GROUP + warp * 2) * K;
-            const T* xr[AD_TOKENS];
-            float acc[2][AD_TOKENS];
+    const int lane = threadIdx.x & 31, rank = blockIdx.y * ADAPTER_GROUP + (threadIdx.x >> 5) * 2, p0 = blockIdx.x * AD_SHRINK;
+    for (int i = 0; i < AD_SHRINK;) {
+        if (p0 + i >= tokens) return;
+        // the neighbours with this token's adapter share its rows
+        const int4 at = places[p0 + i];
+        if (at.y < 0) return;                           // the rest has no adapter
+        int n = 1;
+        while (i + n < AD_SHRINK && p0 + i + n < tokens && places[p0 + i + n].y == at.y) n++;
+        if ((int)blockIdx.y < at.w) {
+            const float* a0 = a + ((long long)at.y * R + rank) * K;
+            const float* xr[AD_SHRINK];
+            float acc[2][AD_SHRINK];
 #pragma unroll
-            for (int i = 0; i < AD_TOKENS; i++) {
-                xr[i] = x + (long long)plan.order[p + min(i, n - 1)] * K;
-                acc[0][i] = acc[1][i] = 0.f;
+            for (int e = 0; e < AD_SHRINK; e++) {
+                xr[e] = x + (long long)places[p0 + i + min(e, n - 1)].x * K;
+                acc[0][e] = acc[1][e] = 0.f;
             }
-            for (int k = lane; k < K; k += 32) {
-                const float w0 = to_f32(a0[k]), w1 = to_f32(a0[K + k]);
+#pragma unroll 2
+            for (int k = lane * W; k < K; k += 32 * W) {
+                float w0[W], w1[W], f[W];
+                AdColumns<W>::load(a0 + k, w0);
+                AdColumns<W>::load(a0 + K + k, w1);
 #pragma unroll
-                for (int i = 0; i < AD_TOKENS; i++) {
-                    const float xv = to_f32(xr[i][k]);
-                    acc[0][i] = fmaf(xv, w0, acc[0][i]);
-                    acc[1][i] = fmaf(xv, w1, acc[1][i]);
+                for (int e = 0; e < AD_SHRINK; e++) {
+                    AdColumns<W>::load(xr[e] + k, f);
+#pragma unroll
+                    for (int q = 0; q < W; q++) {
+                        acc[0][e] = fmaf(f[q], w0[q], acc[0][e]);
+                        acc[1][e] = fmaf(f[q], w1[q], acc[1][e]);
+                    }
                 }
             }
+            const float s = scales[at.y];
 #pragma unroll
-            for (int i = 0; i < AD_TOKENS; i++) {
-                acc[0][i] = warp_sum(acc[0][i]);
-                acc[1][i] = warp_sum(acc[1][i]);
+            for (int e = 0; e < AD_SHRINK; e++) {
+                const float s0 = warp_sum(acc[0][e]), s1 = warp_sum(acc[1][e]);
+                if (lane == 0 && e < n) {
+                    float* to = v + (long long)places[p0 + i + e].x * R + rank;
+                    to[0] = s * s0;
+                    to[1] = s * s1;
+                }
             }
-            const float s = scales[ad];
-            if (lane == 0)
-#pragma unroll
-                for (int i = 0; i < AD_TOKENS; i++)
-                    if (i < n) {
-                        float* to = v + (long long)plan.order[p + i] * R + g * ADAPTER_GROUP + warp * 2;
-                        to[0] = s * acc[0][i];
-                        to[1] = s * acc[1][i];
-                    }
         }
-        p = e;
+        i += n;
     }
 }
 
-template <typename T, typename TOut>
+// out[t, n] += v[t] . B_a[n]
 __global__ void __launch_bounds__(AD_COLS)
-adapter_expand_kernel(const float* base, int N, const T* __restrict__ b, const float* __restrict__ v, int R, const AdPlan plan, int tokens, TOut* out) {
+adapter_expand_kernel(int N, const float* __restrict__ b, const float* __restrict__ v, int R, const int4* __restrict__ places, int tokens, float* out) {
     pdl_grid_sync();
-    const int col = blockIdx.x * AD_COLS + threadIdx.x;
-    const int n_slots = plan.counts[0], p0 = blockIdx.y * AD_TOKENS, p1 = min(tokens, p0 + AD_TOKENS);
+    const int col = blockIdx.x * AD_COLS + threadIdx.x, p0 = blockIdx.y * AD_TOKENS;
     if (col >= N) return;
-    int slot = 0;
-    for (int p = p0; p < p1;) {
-        while (slot < n_slots && plan.slot_begin[slot + 1] <= p) slot++;
-        const int e = slot < n_slots ? min(p1, plan.slot_begin[slot + 1]) : p1, n = e - p;
-        float acc[AD_TOKENS];
-        for (int i = 0; i < AD_TOKENS; i++) acc[i] = 0.f;
-        if (slot < n_slots) {
-            const int ad = plan.slot_adapter[slot], n_g = plan.slot_group[slot + 1] - plan.slot_group[slot];
-            for (int g = 0; g < n_g; g++) {
-                float w[ADAPTER_GROUP];
-                const T* bw = b + (((long long)ad * (R / ADAPTER_GROUP) + g) * N + col) * ADAPTER_GROUP;
-                load8(bw, w);
-                load8(bw + 8, w + 8);
+    int4 at[AD_TOKENS];
+    float acc[AD_TOKENS];
+    int most = 0;
 #pragma unroll
-                for (int i = 0; i < AD_TOKENS; i++)
-                    if (i < n) {
-                        const float* vt = v + (long long)plan.order[p + i] * R + g * ADAPTER_GROUP;
-#pragma unroll
-                        for (int r = 0; r < ADAPTER_GROUP; r++) acc[i] = fmaf(vt[r], w[r], acc[i]);
-                    }
-            }
-        }
+    for (int i = 0; i < AD_TOKENS; i++) {
+        at[i] = p0 + i < tokens ? places[p0 + i] : make_int4(-1, -1, 0, 0);
+        most = max(most, at[i].w);
+        acc[i] = at[i].w > 0 ? out[(long long)at[i].x * N + col] : 0.f;
+    }
+    for (int g = 0; g < most; g++) {
+        float w[ADAPTER_GROUP];
 #pragma unroll
         for (int i = 0; i < AD_TOKENS; i++)
-            if (i < n) {
-                const long long at = (long long)plan.order[p + i] * N + col;
-                out[at] = from_f32<TOut>(base[at] + acc[i]);
+            if (g < at[i].w) {
+                if (i == 0 || at[i].y != at[i - 1].y) {
+                    const float* bw = b + (((long long)at[i].y * (R / ADAPTER_GROUP) + g) * N + col) * ADAPTER_GROUP;
+                    load8(bw, w);
+                    load8(bw + 8, w + 8);
+                }
+                const float* vt = v + (long long)at[i].x * R + g * ADAPTER_GROUP;
+#pragma unroll
+                for (int r = 0; r < ADAPTER_GROUP; r++) acc[i] = fmaf(vt[r], w[r], acc[i]);
             }
-        p = e;
     }
+#pragma unroll
+    for (int i = 0; i < AD_TOKENS; i++)
+        if (at[i].w > 0) out[(long long)at[i].x * N + col] = acc[i];
 }
 
 // ---- The rows form (bfloat16, up to 256 tokens): two launches.
@@ -159,10 +158,11 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_holder;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0) {
         if (lane == 0) {
+            // the join reads second factors before its wait: not before this kernel's own wait, unless no kernel before made them
+            if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             int group_row[TC_BM / ADAPTER_GROUP];
 #pragma unroll
             for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++) {
@@ -182,25 +182,29 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             };
             // where no kernel before this one makes weights, the first ring of them comes before the wait for the tokens' rows
             const int n_pre = n_k < STAGES ? n_k : STAGES;
-            if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (!early) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            }
             for (int i = 0; i < n_pre; i++) arm_and_load_weights(i, i);
             if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int i = 0; i < n_pre; i++) tma_load_2d(b_base + i * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * i);
             bool alive = true;
-            for (int i = n_pre; i < n_k && alive; i++) {
-                const int s = i % STAGES;
-                alive = mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, err);
+            int s = 0, phase = 0;
+            for (int i = n_pre; i < n_k; i++) {
+                alive = mbar_wait(empty0 + 8 * s, phase, err);
                 if (!alive) break;
                 arm_and_load_weights(i, s);
                 tma_load_2d(b_base + s * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * s);
+                if (++s == STAGES) s = 0, phase ^= 1;
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             bool alive = true;
-            for (int i = 0; i < n_k && alive; i++) {
-                const int s = i % STAGES;
-                alive = mbar_wait(full0 + 8 * s, (i / STAGES) & 1, err);
+            int s = 0, phase = 0;
+            for (int i = 0; i < n_k; i++) {
+                alive = mbar_wait(full0 + 8 * s, phase, err);
                 if (!alive) break;
                 tc_fence_after();
 #pragma unroll
@@ -208,6 +212,7 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                     umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
                               (i > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(empty0 + 8 * s);
+                if (++s == STAGES) s = 0, phase ^= 1;
             }
             umma_commit(done_bar);
         }
@@ -249,81 +254,111 @@ __device__ __forceinline__ float ad_dot16(const float* w, const float* v, float 
     return acc;
 }
 
-// TOK places of the plan's order by 128 columns.  SHARED: neighbours mostly have the same adapter, whose values of B are then
-// loaded once for them; otherwise the loads of all places are in flight together.
-template <int TOK, bool SHARED, typename TOut>
+// TOK places of the plan's order by 128 threads of VEC columns.  SHARED: neighbours mostly have the same adapter, whose values of B
+// are then loaded once for them; otherwise the loads of all places are in flight together.
+template <int TOK, bool SHARED, int VEC, typename TOut>
 __global__ void __launch_bounds__(AD_COLS)
 adapter_join_kernel(const float* __restrict__ base, int splits, long long stride, int N, const bf16* __restrict__ b, const float* __restrict__ vs, int v_ld,
                     const float* __restrict__ scales, int R, const int4* __restrict__ places, int T, TOut* __restrict__ out) {
-    pdl_grid_sync();
     __shared__ __align__(16) float v[TOK][ADAPTER_GROUP * ADAPTER_MAX_GROUPS];
-    const int tid = threadIdx.x, col = blockIdx.x * AD_COLS + tid, p0 = blockIdx.y * TOK;
+    const int tid = threadIdx.x, col = (blockIdx.x * AD_COLS + tid) * VEC, p0 = blockIdx.y * TOK;
     int4 at[TOK];                                       // token, adapter, first group, groups
     int most = 0;
 #pragma unroll
-    for (int i = 0; i < TOK; i++) {
+    for (int i = 0; i < TOK; i++) {                     // (the plan comes with a copy, not from a kernel)
         at[i] = p0 + i < T ? places[p0 + i] : make_int4(-1, -1, 0, 0);
         most = max(most, at[i].w);
     }
-    float acc[TOK];
+    // the second factors as well: the first groups' values come before the wait for the kernel that makes the slices
+    const size_t ld = (size_t)(R / ADAPTER_GROUP) * N * ADAPTER_GROUP;
+    uint4 head[SHARED ? 1 : TOK][SHARED ? 1 : VEC][2];
+    if (!SHARED && col < N)
 #pragma unroll
-    for (int i = 0; i < TOK; i++) acc[i] = 0.f;
+        for (int i = 0; i < TOK; i++)
+            if (at[i].w > 0)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) head[i][e][h] = reinterpret_cast<const uint4*>(b + at[i].y * ld + (size_t)(col + e) * ADAPTER_GROUP)[h];
+    pdl_grid_sync();
+    float acc[TOK][VEC];
+#pragma unroll
+    for (int i = 0; i < TOK; i++)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[i][e] = 0.f;
     if (col < N)
+#pragma unroll 4
         for (int z = 0; z < splits; z++)
 #pragma unroll
             for (int i = 0; i < TOK; i++)
-                if (at[i].x >= 0) acc[i] += base[(size_t)z * stride + (size_t)at[i].x * N + col];
-    if (most > 0) {
+                if (at[i].x >= 0) {
+                    float f[VEC];
+                    AdColumns<VEC>::load(base + (size_t)z * stride + (size_t)at[i].x * N + col, f);
 #pragma unroll
-        for (int i = 0; i < TOK; i++) {
-            const int n = at[i].w * ADAPTER_GROUP;
-            if (n > 0) {
-                const float s = scales[at[i].y];
-                for (int r = tid; r < n; r += AD_COLS) {
-                    const float* from = vs + (size_t)at[i].x * v_ld + at[i].z * ADAPTER_GROUP + r;
-                    float t = 0.f;
-                    for (int z = 0; z < splits; z++) t += from[(size_t)z * T * v_ld];
-                    v[i][r] = s * t;
+                    for (int e = 0; e < VEC; e++) acc[i][e] += f[e];
                 }
+    if (most > 0) {
+        // the places' rank values, a thread per rank of a place
+        for (int q = tid; q < TOK * most * ADAPTER_GROUP; q += AD_COLS) {
+            const int i = q / (most * ADAPTER_GROUP), rank = q - i * (most * ADAPTER_GROUP);
+            int4 a = at[0];
+#pragma unroll
+            for (int e = 1; e < TOK; e++)
+                if (i == e) a = at[e];
+            if (rank < a.w * ADAPTER_GROUP) {
+                const float* from = vs + (size_t)a.x * v_ld + a.z * ADAPTER_GROUP + rank;
+                const float s = scales[a.y];
+                float t = 0.f;
+#pragma unroll 4
+                for (int z = 0; z < splits; z++) t += from[(size_t)z * T * v_ld];
+                v[i][rank] = s * t;
             }
         }
         __syncthreads();
         if (col < N)
             for (int g = 0; g < most; g++) {
                 const bf16* bg = b + ((size_t)g * N + col) * ADAPTER_GROUP;
-                const size_t ld = (size_t)(R / ADAPTER_GROUP) * N * ADAPTER_GROUP;
                 if (SHARED) {
-                    float w[ADAPTER_GROUP];
 #pragma unroll
-                    for (int i = 0; i < TOK; i++)
-                        if (g < at[i].w) {
-                            if (i == 0 || at[i].y != at[i - 1].y) {
-                                load8(bg + at[i].y * ld, w);
-                                load8(bg + at[i].y * ld + 8, w + 8);
+                    for (int e = 0; e < VEC; e++) {
+                        float w[ADAPTER_GROUP];
+#pragma unroll
+                        for (int i = 0; i < TOK; i++)
+                            if (g < at[i].w) {
+                                if (i == 0 || at[i].y != at[i - 1].y) {
+                                    load8(bg + at[i].y * ld + e * ADAPTER_GROUP, w);
+                                    load8(bg + at[i].y * ld + e * ADAPTER_GROUP + 8, w + 8);
+                                }
+                                acc[i][e] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i][e]);
                             }
-                            acc[i] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i]);
-                        }
+                    }
                 } else {
-                    float w[TOK][ADAPTER_GROUP];
 #pragma unroll
                     for (int i = 0; i < TOK; i++)
-                        if (g < at[i].w) {
-                            load8(bg + at[i].y * ld, w[i]);
-                            load8(bg + at[i].y * ld + 8, w[i] + 8);
-                        }
+                        if (g < at[i].w)
+#pragma unroll
+                            for (int e = 0; e < VEC; e++) {
+                                float w[ADAPTER_GROUP];
+                                load8(reinterpret_cast<const bf16*>(&head[i][e][0]), w);
+                                load8(reinterpret_cast<const bf16*>(&head[i][e][1]), w + 8);
+                                acc[i][e] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i][e]);
+                            }
 #pragma unroll
                     for (int i = 0; i < TOK; i++)
-                        if (g < at[i].w) acc[i] = ad_dot16(w[i], &v[i][g * ADAPTER_GROUP], acc[i]);
+                        if (g + 1 < at[i].w)
+#pragma unroll
+                            for (int e = 0; e < VEC; e++)
+#pragma unroll
+                                for (int h = 0; h < 2; h++)
+                                    head[i][e][h] = reinterpret_cast<const uint4*>(bg + at[i].y * ld + (size_t)N * ADAPTER_GROUP + e * ADAPTER_GROUP)[h];
                 }
             }
     }
     if (col < N)
 #pragma unroll
         for (int i = 0; i < TOK; i++)
-            if (at[i].x >= 0) out[(size_t)at[i].x * N + col] = from_f32<TOut>(acc[i]);
+            if (at[i].x >= 0) AdColumns<VEC>::store(out + (size_t)at[i].x * N + col, acc[i]);
 }
-
-// ---- host side
 
 // How the rows form cuts K: as many slices as bring about two blocks to an SM (one beyond 128 tokens, whose stages are larger),
 // each at least 8 pieces of 64 wide, at most 8 slices (their reader pays for every one).
@@ -379,14 +414,14 @@ static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const
         default: rc = ad_launch_rows<256>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s);
     }
     if (rc) return rc;
-    auto join = [&](auto kern, int tok) {
-        illm_launch(kern, dim3(ad_div(N, AD_COLS), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
+    auto join = [&](auto kern, int tok, int vec) {
+        illm_launch(kern, dim3(ad_div(N, AD_COLS * vec), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
                     (const float*)vs, v_ld, scales, R, plan.places, T, out);
     };
-    // many tokens of few adapters: prompts
-    if (T <= 4) join(adapter_join_kernel<1, false, TOut>, 1);
-    else if (T > 64 && 4 * sz.slots <= T) join(adapter_join_kernel<8, true, TOut>, 8);
-    else join(adapter_join_kernel<4, false, TOut>, 4);
+    // few tokens: many blocks; many tokens of few adapters: prompts
+    if (T <= 4) join(adapter_join_kernel<1, false, 1, TOut>, 1, 1);
+    else if (T > 64 && 4 * sz.slots <= T && N % 4 == 0) join(adapter_join_kernel<4, true, 4, TOut>, 4, 4);
+    else join(adapter_join_kernel<4, false, 1, TOut>, 4, 1);
     return illm_launch_status();
 }
 
@@ -402,12 +437,12 @@ extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int
 static int ad_float32(const float* x, const float* w, int T, int N, int K, const float* a, const float* b, const float* scales, int R,
                       const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int* err, cudaStream_t s) {
     const AdPlan plan = ad_plan(plan_dev, sz);
-    const int tiles = ad_div(T, AD_TOKENS);
     const int rc = illm_gemm_f32_nt(x, w, out, T, N, K, K, K, N, err, s);
     if (rc != 0 || sz.slots == 0) return rc;
-    illm_launch(adapter_shrink_kernel<float>, dim3(tiles, R / ADAPTER_GROUP), dim3(256), 0, s, x, K, a, scales, R, plan, T, v);
-    illm_launch(adapter_expand_kernel<float, float>, dim3(ad_div(N, AD_COLS), tiles), dim3(AD_COLS), 0, s, (const float*)out, N, b, (const float*)v, R, plan, T,
-                out);
+    const bool wide = K % 4 == 0 && !(((uintptr_t)x | (uintptr_t)a) & 15);
+    auto shrink = wide ? adapter_shrink_kernel<4> : adapter_shrink_kernel<1>;
+    illm_launch(shrink, dim3(ad_div(T, AD_SHRINK), R / ADAPTER_GROUP), dim3(256), 0, s, x, K, a, scales, R, plan.places, T, v);
+    illm_launch(adapter_expand_kernel, dim3(ad_div(N, AD_COLS), ad_div(T, AD_TOKENS)), dim3(AD_COLS), 0, s, N, b, (const float*)v, R, plan.places, T, out);
     return illm_launch_status();
 }
 
@@ -418,7 +453,7 @@ extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int
                                     int* err, void* stream) {
     if (T <= 0 || N <= 0) return 0;
     if (K <= 0 || count <= 0 || R <= 0 || R % ADAPTER_GROUP || R > ADAPTER_GROUP * ADAPTER_MAX_GROUPS || slots < 0 || groups < 0 || chunks < 0 || !ws || !plan ||
-        T > 65535 * AD_TOKENS || (long long)count * R * (N / ADAPTER_GROUP + 1) >= (1ll << 31) || (long long)count * R >= (1ll << 31))
+        T > 65535 * AD_SHRINK || (long long)count * R * (N / ADAPTER_GROUP + 1) >= (1ll << 31) || (long long)count * R >= (1ll << 31))
         return ILLM_ERR_BAD_ARG;        // (rows of the factors are counted in 32 bits)
     if (dtype == ILLM_BF16 && ((K & 7) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)a & 15) || ((uintptr_t)b & 15))) return ILLM_ERR_BAD_ARG;
     const AdapterPlanSizes sz{T, slots, groups, chunks};

@@ -14,6 +14,21 @@ static inline AdPlan ad_plan(const int* plan, const AdapterPlanSizes& s) {
                   plan + l.tile_chunk, plan + l.chunk_tile, plan + l.chunk_groups};
 }
 
+// VEC neighbouring columns
+template <int VEC> struct AdColumns;
+template <> struct AdColumns<1> {
+    __device__ static void load(const float* p, float* f) { f[0] = *p; }
+    template <typename T> __device__ static void store(T* p, const float* f) { *p = from_f32<T>(f[0]); }
+};
+template <> struct AdColumns<4> {
+    __device__ static void load(const float* p, float* f) { *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p); }
+    __device__ static void store(float* p, const float* f) { *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(f); }
+    __device__ static void store(bf16* p, const float* f) {
+        __nv_bfloat162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
+    }
+};
+
 typedef CUresult (*AdEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                     const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 

@@ -10,7 +10,7 @@
 #define ADAPTER_TILE 256          // tokens of a tile of the prompt product
 #define ADAPTER_CHUNK 4           // groups of a chunk: one 64-wide K piece of the prompt product
 #define ADAPTER_MAX_GROUPS 16     // ranks up to 256
-#define ADAPTER_ROWS_MAX 256      // tokens up to which the rows form runs; above it the plan has tiles
+#define ADAPTER_ROWS_MAX 128      // tokens up to which the rows form runs; above it the plan has tiles
 
 struct AdapterPlanSizes {
     int T;                        // tokens

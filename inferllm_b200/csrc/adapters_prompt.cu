@@ -5,7 +5,7 @@
 // adapters: one chunk behind the K / 64 pieces of the shared product, in the same accumulators, rounded once with it.
 //
 // adapter_values_kernel makes the chunks of v: 128 tokens by 64 ranks per cluster, tcgen05 (tokens on the lanes, four TMA boxes of
-// 16 rows of A as the MMA's N), the cluster's blocks share K and add up over distributed shared memory in the order of
+// 16 rows of A, or one of 64, as the MMA's N), the cluster's blocks share K and add up over distributed shared memory in the order of
 // their ranks; scaled in float32, rounded to bfloat16 (the operand type of the product that follows; 2^-8 of a term that
 // is itself a correction), zero where the token's adapter is another one.  Its bound is reading x once, from L2 behind the first chunk.
 //
@@ -19,24 +19,28 @@
 #include "kernels.h"
 #include "tc_pair.cuh"
 
-#define AP_VALUE_STAGES 4
+#define AP_VALUE_STAGES 8
+#define AP_VALUE_THREADS 256
 #define AP_COLS (ADAPTER_CHUNK * ADAPTER_GROUP)        // columns of a chunk
-#define AP_PITCH (AP_COLS + 1)
+#define AP_PITCH (AP_COLS + 4)      // floats: rows start on 16 bytes, and 8 neighbouring ones in different banks
 #define AP_STAGES 6
 #define AP_BN 256
 #define AP_HALF 128
 
-__device__ __forceinline__ float ap_load_remote(const float* local, unsigned rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(tc_smem_u32(local), rank)) : "memory");
+__device__ __forceinline__ float4 ap_load_remote(const float* local, unsigned rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(map_to_cta(tc_smem_u32(local), rank)) : "memory");
     return v;
 }
 
 // grid: cluster blocks of a half tile, halves, chunks, in this order along x
-__global__ void __launch_bounds__(TC_THREADS)
-adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scales, int R, int T,
-                      int C, int k_iters_total, const AdPlan plan, bf16* __restrict__ v, int* __restrict__ err) {
+template <int AP_ITEMS>
+__global__ void __launch_bounds__(AP_VALUE_THREADS)
+adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a4, const float* __restrict__ scales, int R, int T,
+                      int C, int k_iters_total, int STAGES, const AdPlan plan, bf16* __restrict__ v, int* __restrict__ err) {
     constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = AP_COLS * TC_BK * 2, BOX_BYTES = ADAPTER_GROUP * TC_BK * 2;
+    static_assert((A_BYTES + B_BYTES) * 2 >= TC_BM * AP_PITCH * 4, "two stages hold the sums");
     constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AP_COLS >> 3) << 17) | ((unsigned)(TC_BM >> 4) << 24);
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * AP_VALUE_STAGES + 1];
@@ -47,21 +51,21 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     if (chunk >= plan.counts[2]) return;                // the grid is sized for more chunks than there are (all blocks of the cluster leave)
     const int t0 = plan.chunk_tile[chunk] * ADAPTER_TILE + half * TC_BM;
 
-    const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + AP_VALUE_STAGES * A_BYTES;
+    const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + STAGES * A_BYTES;
     float* partial = reinterpret_cast<float*>(smem_raw + (a_base - tc_smem_u32(smem_raw)));     // [128][AP_PITCH] over the ring, when it is done
     const unsigned full0 = tc_smem_u32(&bars[0]), empty0 = tc_smem_u32(&bars[AP_VALUE_STAGES]), done_bar = tc_smem_u32(&bars[2 * AP_VALUE_STAGES]);
     const int per = (k_iters_total + C - 1) / C, k_begin = (int)rank * per, n_k = max(0, min(per, k_iters_total - k_begin));
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < AP_VALUE_STAGES; s++) {
-            mbar_init(full0 + 8 * s, 1);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 2);
             mbar_init(empty0 + 8 * s, 1);
         }
         mbar_init(done_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(&tmem_holder)), "r"((unsigned)AP_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -70,80 +74,103 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     tc_fence_after();
     const unsigned tmem = tmem_holder;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int row[ADAPTER_CHUNK], boxes = 0;
+    if (warp <= 1 && lane == 0) {
+        // warp 0 fetches the tokens' rows (and hears from the MMAs when a stage is free), warp 1 the adapters'; a stage is full when
+        // both have arrived
+        int row[ADAPTER_CHUNK], boxes = 0;
+        bool joined = true;                             // the four groups lie one behind another: one box instead of four
 #pragma unroll
-            for (int j = 0; j < ADAPTER_CHUNK; j++) {
-                const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + j];
-                row[j] = g < 0 ? -1 : (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
-                boxes += g >= 0;
-            }
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            // only now may the product begin: it reads the tokens' rows without a wait of its own
-            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            bool alive = true;
-            for (int i = 0; i < n_k && alive; i++) {
-                const int s = i % AP_VALUE_STAGES;
-                if (i >= AP_VALUE_STAGES) alive = mbar_wait(empty0 + 8 * s, ((i / AP_VALUE_STAGES) - 1) & 1, err);
-                if (!alive) break;
-                mbar_expect_tx(full0 + 8 * s, A_BYTES + boxes * BOX_BYTES);
-                const int kx = (k_begin + i) * TC_BK;
-                tma_load_2d(a_base + s * A_BYTES, &map_x, kx, t0, full0 + 8 * s);
-#pragma unroll
-                for (int j = 0; j < ADAPTER_CHUNK; j++)
-                    if (row[j] >= 0) tma_load_2d(b_base + s * B_BYTES + j * BOX_BYTES, &map_a, kx, row[j], full0 + 8 * s);
-            }
+        for (int j = 0; j < ADAPTER_CHUNK; j++) {
+            const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + j];
+            row[j] = g < 0 ? -1 : (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
+            boxes += g >= 0;
+            joined = joined && row[j] == row[0] + j * ADAPTER_GROUP && g >= 0;
         }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            bool alive = true;
-            for (int i = 0; i < n_k && alive; i++) {
-                const int s = i % AP_VALUE_STAGES;
-                alive = mbar_wait(full0 + 8 * s, (i / AP_VALUE_STAGES) & 1, err);
-                if (!alive) break;
-                tc_fence_after();
-#pragma unroll
-                for (int kk = 0; kk < TC_BK / 16; kk++)
-                    umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
-                              (i > 0 || kk > 0) ? 1u : 0u);
-                umma_commit(empty0 + 8 * s);
-            }
-            umma_commit(done_bar);
-        }
-    } else {
-        const int quad = warp & 3, r = quad * 32 + lane;
         asm volatile("griddepcontrol.wait;" ::: "memory");
+        // only now may the product begin: it reads the tokens' rows without a wait of its own
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        bool alive = true;
+        int s = 0, phase = 1;
+        for (int i = 0; i < n_k; i++) {
+            if (i >= STAGES) alive = mbar_wait(empty0 + 8 * s, phase, err);
+            if (!alive) break;
+            const int kx = (k_begin + i) * TC_BK;
+            if (warp == 0) {
+                mbar_expect_tx(full0 + 8 * s, A_BYTES);
+                tma_load_2d(a_base + s * A_BYTES, &map_x, kx, t0, full0 + 8 * s);
+            } else {
+                mbar_expect_tx(full0 + 8 * s, boxes * BOX_BYTES);
+                if (joined) {
+                    tma_load_2d(b_base + s * B_BYTES, &map_a4, kx, row[0], full0 + 8 * s);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < ADAPTER_CHUNK; j++)
+                        if (row[j] >= 0) tma_load_2d(b_base + s * B_BYTES + j * BOX_BYTES, &map_a, kx, row[j], full0 + 8 * s);
+                }
+            }
+            if (++s == STAGES) s = 0, phase ^= 1;
+        }
+    } else if (warp == 2 && lane == 0) {
+        bool alive = true;
+        int s = 0, phase = 0;
+        for (int i = 0; i < n_k; i++) {
+            alive = mbar_wait(full0 + 8 * s, phase, err);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TC_BK / 16; kk++)
+                umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
+                          (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(empty0 + 8 * s);
+            if (++s == STAGES) s = 0, phase ^= 1;
+        }
+        umma_commit(done_bar);
+    }
+    // each block finishes its share of the rows, four columns to a thread: what it needs for that, while the products run
+    const int rows = TC_BM / C, items = rows * (AP_COLS / 4);
+    float factor[AP_ITEMS];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < AP_ITEMS; q++) {
+        const int i = threadIdx.x + q * AP_VALUE_THREADS, t = t0 + (int)rank * rows + i / (AP_COLS / 4);
+        const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + i % (AP_COLS / 4) / (ADAPTER_GROUP / 4)], ad = i < items && t < T ? plan.token_adapter[t] : -1;
+        factor[q] = g >= 0 && g / ADAPTER_MAX_GROUPS == ad ? scales[ad] : NAN;        // NaN: the token's adapter is another one
+    }
+    __syncwarp();
+    if (warp >= AP_VALUE_THREADS / 32 - 4) {
+        const int quad = warp & 3, r = quad * 32 + lane;
         const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, err));
         tc_fence_after();
-#pragma unroll 1
+#pragma unroll
         for (int c0 = 0; c0 < AP_COLS; c0 += 16) {
             float f[16];
             if (ok && n_k > 0) tmem_ld16(tmem + ((unsigned)(quad * 32) << 16) + (unsigned)c0, f);
 #pragma unroll
-            for (int j = 0; j < 16; j++) partial[r * AP_PITCH + c0 + j] = ok && n_k > 0 ? f[j] : 0.f;
+            for (int j = 0; j < 16; j++) f[j] = ok && n_k > 0 ? f[j] : 0.f;
+            store8(partial + r * AP_PITCH + c0, f);
+            store8(partial + r * AP_PITCH + c0 + 8, f + 8);
         }
     }
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();                                 // every block's sums are there
-    if (warp == 1) {
+    if (warp == 2) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)AP_COLS) : "memory");
     }
-    // each block finishes its share of the rows, four columns a thread
-    const int rows = TC_BM / C;
-    for (int i = threadIdx.x; i < rows * (AP_COLS / 4); i += TC_THREADS) {
-        const int r = (int)rank * rows + i / (AP_COLS / 4), c = i % (AP_COLS / 4) * 4, t = t0 + r;
-        const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + c / ADAPTER_GROUP], ad = t < T ? plan.token_adapter[t] : -1;
+#pragma unroll
+    for (int q = 0; q < AP_ITEMS; q++) {
+        const int i = threadIdx.x + q * AP_VALUE_THREADS, r = (int)rank * rows + i / (AP_COLS / 4), c = i % (AP_COLS / 4) * 4;
+        if (i >= items) break;
         float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (g >= 0 && g / ADAPTER_MAX_GROUPS == ad) {
-            for (int b = 0; b < C; b++)
+        if (factor[q] == factor[q]) {
+            float4 p[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) f[j] += ap_load_remote(&partial[r * AP_PITCH + c + j], b);
-            const float s = scales[ad];
+            for (int b = 0; b < 8; b++) p[b] = b < C ? ap_load_remote(&partial[r * AP_PITCH + c], b) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[j] *= s;
+            for (int b = 0; b < 8; b++) f[0] += p[b].x, f[1] += p[b].y, f[2] += p[b].z, f[3] += p[b].w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] *= factor[q];
         }
         __nv_bfloat162 o[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
         *reinterpret_cast<uint2*>(v + ((size_t)chunk * ADAPTER_TILE + half * TC_BM + r) * AP_COLS + c) = *reinterpret_cast<uint2*>(o);
@@ -331,6 +358,20 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
 }
 
+// out[i] = the slices' sum in ascending order, four neighbours a thread
+template <typename TOut> __global__ void __launch_bounds__(256) adapter_sum_kernel(const float* __restrict__ slices, int splits, long long n, TOut* __restrict__ out) {
+    pdl_grid_sync();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 f[4];                                        // (at most 4 slices)
+#pragma unroll
+    for (int z = 0; z < 4; z++) f[z] = z < splits ? *reinterpret_cast<const float4*>(slices + z * n + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float a[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+    for (int z = 1; z < 4; z++) a[0] += f[z].x, a[1] += f[z].y, a[2] += f[z].z, a[3] += f[z].w;
+    AdColumns<4>::store(out + i, a);
+}
+
 // ---- host side
 
 // Slices of K: as many as there are pairs of SMs for the tiles, each of at least 16 pieces, at most 4.
@@ -363,26 +404,37 @@ int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void
     const int k_iters = ad_div(K, TC_BK), splits = ap_splits(T, N, K);
     bf16* v = (bf16*)ws;
     float* slices = (float*)(ws + ad_round((long long)chunks * ADAPTER_TILE * AP_COLS * 2));
-    CUtensorMap mx, ma, mw, mv, mb;
+    CUtensorMap mx, ma, ma4, mw, mv, mb;
     int rc;
     if ((rc = ad_make_map(&mx, x, T, K, TC_BM)) || (rc = ad_make_map(&mw, w, N, K, AP_HALF))) return rc;
     mv = mb = mx;
     if (chunks > 0) {
-        if ((rc = ad_make_map(&ma, a, (long long)count * R, K, ADAPTER_GROUP)) || (rc = ad_make_map(&mv, v, (long long)chunks * ADAPTER_TILE, AP_COLS, TC_BM)) ||
+        if ((rc = ad_make_map(&ma, a, (long long)count * R, K, ADAPTER_GROUP)) || (rc = ad_make_map(&ma4, a, (long long)count * R, K, AP_COLS)) ||
+            (rc = ad_make_map(&mv, v, (long long)chunks * ADAPTER_TILE, AP_COLS, TC_BM)) ||
             (rc = ad_make_map(&mb, b, (long long)count * (R / ADAPTER_GROUP) * N, ADAPTER_GROUP, AP_HALF, ADAPTER_GROUP, CU_TENSOR_MAP_SWIZZLE_32B)))
             return rc;
         // as many blocks share a chunk's K as bring about two blocks to an SM
         int C = 1;
         while (C < 8 && chunks * 2 * C * 2 <= 2 * illm_sm_count() && k_iters >= 4 * C) C *= 2;
-        const size_t smem = (size_t)AP_VALUE_STAGES * (TC_BM + AP_COLS) * TC_BK * 2 + 1024;
-        cudaError_t e = cudaFuncSetAttribute(adapter_values_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // the ring holds a block's whole share of K where one block has an SM to itself
+        const int per = ad_div(k_iters, C), most = chunks * 2 * C > illm_sm_count() ? 4 : AP_VALUE_STAGES, stages = per < 2 ? 2 : per < most ? per : most;
+        const size_t smem = (size_t)stages * (TC_BM + AP_COLS) * TC_BK * 2 + 1024;
+        // rows and columns that a thread finishes: 128 / C x 64 in fours, 256 threads
+        auto kern = C == 8 ? adapter_values_kernel<1> : C == 4 ? adapter_values_kernel<2> : C == 2 ? adapter_values_kernel<4> : adapter_values_kernel<8>;
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
-        rc = illm_launch_cluster(adapter_values_kernel, dim3((unsigned)C * 2 * chunks), dim3(TC_THREADS), C, smem, s, mx, ma, scales, R, T, C, k_iters, plan, v, err);
+        rc = illm_launch_cluster(kern, dim3((unsigned)C * 2 * chunks), dim3(AP_VALUE_THREADS), C, smem, s, mx, ma, ma4, scales, R, T, C, k_iters, stages, plan, v, err);
         if (rc) return rc;
     }
     if (splits > 1) {
         rc = ap_launch_pair<float>(mx, mw, mv, mb, slices, T, N, R, k_iters, splits, plan, chunks > 0, err, s);
-        return rc ? rc : illm_splitk_reduce(slices, out, out_dtype, (long long)T * N, splits, s);
+        if (rc) return rc;
+        const long long n = (long long)T * N;
+        if (n % 4 || ((uintptr_t)out & 15)) return illm_splitk_reduce(slices, out, out_dtype, n, splits, s);
+        const dim3 blocks((unsigned)((n / 4 + 255) / 256));
+        if (out_dtype == ILLM_BF16) illm_launch(adapter_sum_kernel<bf16>, blocks, dim3(256), 0, s, (const float*)slices, splits, n, (bf16*)out);
+        else illm_launch(adapter_sum_kernel<float>, blocks, dim3(256), 0, s, (const float*)slices, splits, n, (float*)out);
+        return illm_launch_status();
     }
     if (out_dtype == ILLM_BF16) return ap_launch_pair<bf16>(mx, mw, mv, mb, (bf16*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
     return ap_launch_pair<float>(mx, mw, mv, mb, (float*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);

@@ -9,6 +9,7 @@ policy functions here ask it, so the choices tested are the ones that run.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -38,15 +39,7 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
+_HERE = contextlib.nullcontext()
 
 
 def _on(device):
@@ -816,6 +809,8 @@ class Adapters:
         self.b = torch.zeros((count, self.R // ADAPTER_GROUP, n_out, ADAPTER_GROUP), dtype=dtype, device=self.device)
         self.scales = torch.zeros((count,), dtype=torch.float32, device=self.device)
         self.ranks = [0] * count
+        self.changes = 0        # how often a rank has changed
+        self.pointers = self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr()
 
     def put(self, i, a, b, scale=1.0):
         """Adapter i becomes scale * b a (a [r, n_in], b [n_out, r], any float type); what it was is gone.  Works on torch's
@@ -840,7 +835,9 @@ class Adapters:
             e = min(r, g + ADAPTER_GROUP)
             self.b[i, g // ADAPTER_GROUP, :, :e - g] = b[:, g:e]
         self.scales[i] = scale
-        self.ranks[i] = r
+        if self.ranks[i] != r:
+            self.ranks[i] = r
+            self.changes += 1
 
     def remove(self, i):
         """Adapter i adds nothing any more."""
@@ -863,43 +860,51 @@ class AdapterRows:
                                             ctypes.cast(host.data_ptr(), _b.PI)))
         self.slots, self.groups, self.chunks = sizes[1], sizes[2], sizes[3]
         self.plan = host.to(self.device)
+        self.plan_ptr = self.plan.data_ptr()
+        self._fitted = None
         self.most_groups = max((-(-self.ranks[a] // ADAPTER_GROUP) for a in self.named), default=0)
 
     def fits(self, adapters):
         """Whether the plan covers these adapters' ranks."""
+        if self._fitted is not None and self._fitted[0] is adapters and self._fitted[1] == adapters.changes:
+            return True
         have, need = self.ranks, adapters.ranks
-        return all(a < len(need) and -(-need[a] // ADAPTER_GROUP) <= -(-have[a] // ADAPTER_GROUP) for a in self.named) and self.most_groups * ADAPTER_GROUP <= adapters.R
+        ok = all(a < len(need) and -(-need[a] // ADAPTER_GROUP) <= -(-have[a] // ADAPTER_GROUP) for a in self.named) and self.most_groups * ADAPTER_GROUP <= adapters.R
+        if ok:
+            self._fitted = adapters, adapters.changes
+        return ok
 
 
 def linear_adapters(x, w, adapters, rows, out_dtype=None):
     """y[t] = x[t] . W^T + scale_a (x[t] . A_a^T) . B_a^T, a the adapter that `rows` gives token t (none: the product alone).
     x [T, K], w [N, K] float32 or bfloat16, `adapters` an `Adapters` of [N, K], `rows` an `AdapterRows` of T tokens; sums in
     float32, rounded once to `out_dtype` (default x's; float32 is the other choice)."""
-    _need(x, "x", None, 2)
-    _need(w, "w", x.dtype, 2)
+    if x.dim() != 2 or w.dim() != 2 or not (x.is_contiguous() and w.is_contiguous()):
+        raise KernelError(f"linear_adapters: x and w must be contiguous matrices, found {tuple(x.shape)} and {tuple(w.shape)}")
     (T, K), (N, wk) = x.shape, w.shape
-    dtype, out_code = act_code(x.dtype), act_code(out_dtype or x.dtype)
-    if wk != K or adapters.n_in != K or adapters.n_out != N or adapters.dtype != x.dtype:
-        raise KernelError(f"linear_adapters: x is {x.dtype} [{T}, {K}], w [{N}, {wk}] and the adapters are {adapters.dtype} for [{adapters.n_out}, {adapters.n_in}]")
+    device, dtype, out_dtype = x.device, x.dtype, out_dtype or x.dtype
+    if adapters.device != device or w.device != device or rows.device != device:
+        raise KernelError(f"linear_adapters: x is on {device}, w on {w.device}, the adapters on {adapters.device} and the plan on {rows.device}: one CUDA device is needed")
+    if wk != K or adapters.n_in != K or adapters.n_out != N or adapters.dtype != dtype or w.dtype != dtype:
+        raise KernelError(f"linear_adapters: x is {dtype} [{T}, {K}], w {w.dtype} [{N}, {wk}] and the adapters are {adapters.dtype} for [{adapters.n_out}, {adapters.n_in}]")
     if rows.T != T:
         raise KernelError(f"linear_adapters: the plan is of {rows.T} tokens, x has {T}")
-    if w.device != x.device or adapters.device != x.device or rows.device != x.device:
-        raise KernelError("linear_adapters: x, w, the adapters and the plan must be on one device")
     if not rows.fits(adapters):
         raise KernelError("linear_adapters: the plan was made for other ranks than the adapters have: make a new one")
-    if x.dtype == torch.bfloat16 and (K % 8 or x.data_ptr() & 15 or w.data_ptr() & 15):
-        raise KernelError(f"linear_adapters: K = {K} must be a multiple of 8 and the operands 16-byte aligned")
-    if x.dtype == torch.float32 and out_code != 0:
-        raise KernelError("linear_adapters: a float32 product stays float32")
-    out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=x.device)
+    if out_dtype not in _DT or (dtype == torch.float32 and out_dtype != dtype):
+        raise KernelError(f"linear_adapters: a result in {out_dtype} of {dtype} operands (float32, or the operands' type)")
+    px, pw = x.data_ptr(), w.data_ptr()
+    if (px | pw) & 15 and (dtype == torch.bfloat16 or K % 4 == 0):
+        raise KernelError("linear_adapters: x and w must start on a 16-byte boundary")
+    out = torch.empty((T, N), dtype=out_dtype, device=device)
     if T == 0:
         return out
-    lib = load()
-    ws = torch.empty((lib.illm_linear_adapters_ws(dtype, T, N, K, adapters.R, rows.groups, rows.chunks),), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        _check(lib.illm_linear_adapters(x.data_ptr(), w.data_ptr(), dtype, T, N, K, adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scales.data_ptr(),
-                                        adapters.count, adapters.R, rows.plan.data_ptr(), rows.slots, rows.groups, rows.chunks, out.data_ptr(), out_code,
-                                        ws.data_ptr(), 0, _error_word(x.device), _stream()), "linear_adapters")
+    lib, code = load(), _DT[dtype]
+    ws = torch.empty((lib.illm_linear_adapters_ws(code, T, N, K, adapters.R, rows.groups, rows.chunks),), dtype=torch.uint8, device=device)
+    a, b, scales = adapters.pointers
+    with _on(device):
+        _check(lib.illm_linear_adapters(px, pw, code, T, N, K, a, b, scales, adapters.count, adapters.R, rows.plan_ptr, rows.slots, rows.groups, rows.chunks,
+                                        out.data_ptr(), _DT[out_dtype], ws.data_ptr(), 0, _error_word(device), _stream()), "linear_adapters")
     return out
 
 
@@ -948,7 +953,7 @@ def sample(logits, uniforms, temp, top_k=0, top_p=1.0, repeat_penalty=1.0, last_
 def _per_row(t, name, dtype, B, device):
     if t is None:
         return None
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != B or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (B,) or not t.is_contiguous() or t.device != device:
         raise KernelError(f"sample_rows: {name} must be a contiguous {dtype} tensor [{B}] on {device}, found {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
