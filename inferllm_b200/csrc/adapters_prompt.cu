@@ -48,8 +48,9 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunk = (int)blockIdx.x / (2 * C), half = (int)blockIdx.x / C & 1;
     const unsigned rank = cluster_ctarank();
-    if (chunk >= plan.counts[2]) return;                // the grid is sized for more chunks than there are (all blocks of the cluster leave)
-    const int t0 = plan.chunk_tile[chunk] * ADAPTER_TILE + half * TC_BM;
+    const int n_chunks = plan.counts[2], t0 = plan.chunk_tile[chunk] * ADAPTER_TILE + half * TC_BM;
+    const int4 groups = *reinterpret_cast<const int4*>(plan.chunk_groups + chunk * ADAPTER_CHUNK);
+    if (chunk >= n_chunks) return;                      // the grid is sized for more chunks than there are (all blocks of the cluster leave)
 
     const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + STAGES * A_BYTES;
     float* partial = reinterpret_cast<float*>(smem_raw + (a_base - tc_smem_u32(smem_raw)));     // [128][AP_PITCH] over the ring, when it is done
@@ -81,7 +82,7 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         bool joined = true;                             // the four groups lie one behind another: one box instead of four
 #pragma unroll
         for (int j = 0; j < ADAPTER_CHUNK; j++) {
-            const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + j];
+            const int g = j == 0 ? groups.x : j == 1 ? groups.y : j == 2 ? groups.z : groups.w;
             row[j] = g < 0 ? -1 : (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
             boxes += g >= 0;
             joined = joined && row[j] == row[0] + j * ADAPTER_GROUP && g >= 0;
@@ -133,7 +134,7 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 #pragma unroll
     for (int q = 0; q < AP_ITEMS; q++) {
         const int i = threadIdx.x + q * AP_VALUE_THREADS, t = t0 + (int)rank * rows + i / (AP_COLS / 4);
-        const int g = plan.chunk_groups[chunk * ADAPTER_CHUNK + i % (AP_COLS / 4) / (ADAPTER_GROUP / 4)], ad = i < items && t < T ? plan.token_adapter[t] : -1;
+        const int j = i % (AP_COLS / 4) / (ADAPTER_GROUP / 4), g = j == 0 ? groups.x : j == 1 ? groups.y : j == 2 ? groups.z : groups.w, ad = i < items && t < T ? plan.token_adapter[t] : -1;
         factor[q] = g >= 0 && g / ADAPTER_MAX_GROUPS == ad ? scales[ad] : NAN;        // NaN: the token's adapter is another one
     }
     __syncwarp();
@@ -184,21 +185,23 @@ __device__ __forceinline__ unsigned long long umma_desc_sw32(unsigned smem_addr)
 }
 
 // C = x . W^T + the chunks.  splits > 1: C is float32 [splits, T, N], slice z the z-th run of K pieces, the last with the chunks.
+// (Tiles of 512 outputs, which need 48 KB instead of 64 for the same work but cannot hide their epilogue, were 3 to 15 % slower.)
 template <typename TOut>
 __global__ void __launch_bounds__(TC_THREADS)
 adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_b, TOut* __restrict__ C, int T, int N, int R, int k_iters_total, int splits, const AdPlan plan,
                     int chunked, int* __restrict__ err) {
+    constexpr int STAGES = AP_STAGES;
     constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = AP_HALF * TC_BK * 2, BOX_BYTES = AP_HALF * ADAPTER_GROUP * 2;
     constexpr unsigned TMEM_COLS = 512;
     constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AP_BN >> 3) << 17) | ((unsigned)(256 >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const unsigned base = tc_smem_u32(smem_raw);
-    const unsigned a_base = base, b_base = a_base + AP_STAGES * A_BYTES;
-    const unsigned bars = b_base + AP_STAGES * B_BYTES;
-    const unsigned full0 = bars, empty0 = bars + 8 * AP_STAGES;
-    const unsigned acc_full0 = bars + 16 * AP_STAGES, acc_empty0 = acc_full0 + 16;
-    unsigned* tmem_holder = reinterpret_cast<unsigned*>(smem_raw + (bars - base) + 16 * AP_STAGES + 32);
+    const unsigned a_base = base, b_base = a_base + STAGES * A_BYTES;
+    const unsigned bars = b_base + STAGES * B_BYTES;
+    const unsigned full0 = bars, empty0 = bars + 8 * STAGES;
+    const unsigned acc_full0 = bars + 16 * STAGES, acc_empty0 = acc_full0 + 16;
+    unsigned* tmem_holder = reinterpret_cast<unsigned*>(smem_raw + (bars - base) + 16 * STAGES + 32);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_ctarank();
@@ -211,7 +214,7 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         return;
     }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < AP_STAGES; s++) {
+        for (int s = 0; s < STAGES; s++) {
             mbar_init(full0 + 8 * s, 1);
             mbar_init(empty0 + 8 * s, 1);
         }
@@ -244,7 +247,7 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (warp == 0) {
         if (lane == 0) {
             bool alive = true, waited = false;
-            int it = 0;
+            int s = 0, phase = 1, it = 0;
             const unsigned full_leader = map_to_cta(full0, 0);      // block 0 counts the bytes of both
             if (!chunked) asm volatile("griddepcontrol.wait;" ::: "memory");       // no kernel of ours has waited for the tokens' rows
             for (int i = pair; i < n_items && alive; i += n_pairs) {
@@ -252,13 +255,13 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 item(i, m, n, k0, k1, c0, c1);
                 const int ra0 = m * 256 + (int)rank * 128, rb0 = n * AP_BN + (int)rank * AP_HALF;
                 for (int k = k0; k < k1 + (c1 - c0); k++, it++) {
-                    const int s = it % AP_STAGES;
-                    if (it >= AP_STAGES) alive = mbar_wait(empty0 + 8 * s, ((it / AP_STAGES) - 1) & 1, err);
+                    if (it >= STAGES) alive = mbar_wait(empty0 + 8 * s, phase, err);
                     if (!alive) break;
+                    const unsigned a_s = a_base + s * A_BYTES, b_s = b_base + s * B_BYTES, full = full_leader + 8 * s;
                     if (k < k1) {
                         if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + B_BYTES));
-                        tma_load_2d_pair(b_base + s * B_BYTES, &map_w, k * TC_BK, rb0, full_leader + 8 * s);
-                        tma_load_2d_pair(a_base + s * A_BYTES, &map_x, k * TC_BK, ra0, full_leader + 8 * s);
+                        tma_load_2d_pair(b_s, &map_w, k * TC_BK, rb0, full);
+                        tma_load_2d_pair(a_s, &map_x, k * TC_BK, ra0, full);
                     } else {
                         const int c = c0 + (k - k1);
                         int g[ADAPTER_CHUNK], boxes = 0;
@@ -272,41 +275,53 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                             waited = true;
                         }
                         if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + boxes * BOX_BYTES));
-                        tma_load_2d_pair(a_base + s * A_BYTES, &map_v, 0, c * ADAPTER_TILE + (int)rank * 128, full_leader + 8 * s);
+                        tma_load_2d_pair(a_s, &map_v, 0, c * ADAPTER_TILE + (int)rank * 128, full);
 #pragma unroll
                         for (int j = 0; j < ADAPTER_CHUNK; j++)
                             if (g[j] >= 0) {
                                 const int row = ((g[j] / ADAPTER_MAX_GROUPS) * (R / ADAPTER_GROUP) + g[j] % ADAPTER_MAX_GROUPS) * N + rb0;
-                                tma_load_2d_pair(b_base + s * B_BYTES + j * BOX_BYTES, &map_b, 0, row, full_leader + 8 * s);
+                                tma_load_2d_pair(b_s + j * BOX_BYTES, &map_b, 0, row, full);
                             }
                     }
+                    if (++s == STAGES) s = 0, phase ^= 1;
                 }
             }
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             bool alive = true;
-            int it = 0, ti = 0;
+            int s = 0, phase = 0, ti = 0;
+            // descriptors of the first stage; 16 bytes are one unit of their address
+            const unsigned long long da0 = umma_desc_sw128(a_base), db0 = umma_desc_sw128(b_base);
             for (int i = pair; i < n_items && alive; i += n_pairs, ti++) {
                 int m, n, k0, k1, c0, c1;
                 item(i, m, n, k0, k1, c0, c1);
                 const int buf = ti & 1;
+                const unsigned d = tmem + buf * AP_BN;
                 if (ti >= 2) alive = mbar_wait(acc_empty0 + 8 * buf, ((ti >> 1) - 1) & 1, err);
                 tc_fence_after();
-                for (int k = k0; k < k1 + (c1 - c0) && alive; k++, it++) {
-                    const int s = it % AP_STAGES;
-                    alive = mbar_wait(full0 + 8 * s, (it / AP_STAGES) & 1, err);
+                // (one thread issues every MMA of the pair: its loop over K holds nothing but waits and MMAs, and the chunks have
+                // their own; with a choice between the two inside, 4,096 tokens of 4096 x 22016 took 610 us instead of 479)
+                for (int k = k0; k < k1 && alive; k++) {
+                    alive = mbar_wait(full0 + 8 * s, phase, err);
                     if (!alive) break;
                     tc_fence_after();
+                    const unsigned long long da = da0 + s * (A_BYTES >> 4), db = db0 + s * (B_BYTES >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < TC_BK / 16; kk++) {
-                        const unsigned long long da = umma_desc_sw128(a_base + s * A_BYTES + kk * 32);
-                        if (k < k1)
-                            umma_bf16_pair(tmem + buf * AP_BN, da, umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC, (k > k0 || kk > 0) ? 1u : 0u);
-                        else if (plan.chunk_groups[(c0 + k - k1) * ADAPTER_CHUNK + kk] >= 0)
-                            umma_bf16_pair(tmem + buf * AP_BN, da, umma_desc_sw32(b_base + s * B_BYTES + kk * BOX_BYTES), IDESC, 1u);
-                    }
+                    for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16_pair(d, da + 2 * kk, db + 2 * kk, IDESC, (k > k0 || kk > 0) ? 1u : 0u);
                     umma_commit_pair(empty0 + 8 * s);
+                    if (++s == STAGES) s = 0, phase ^= 1;
+                }
+                for (int c = c0; c < c1 && alive; c++) {
+                    alive = mbar_wait(full0 + 8 * s, phase, err);
+                    if (!alive) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int kk = 0; kk < ADAPTER_CHUNK; kk++)
+                        if (plan.chunk_groups[c * ADAPTER_CHUNK + kk] >= 0)
+                            umma_bf16_pair(d, da0 + s * (A_BYTES >> 4) + 2 * kk, umma_desc_sw32(b_base + s * B_BYTES + kk * BOX_BYTES), IDESC, 1u);
+                    umma_commit_pair(empty0 + 8 * s);
+                    if (++s == STAGES) s = 0, phase ^= 1;
                 }
                 umma_commit_pair(acc_full0 + 8 * buf);
             }

@@ -33,11 +33,12 @@ def make(T, K, N, ranks, dtype, seed, scale_of=lambda i: 1.0 + 0.5 * i):
 def expected(x, w, a, b, scales, index):
     """(value, |terms| of the adapter) in 64 bits."""
     y, spread = x.double() @ w.double().t(), torch.zeros((x.shape[0], w.shape[0]), dtype=torch.float64, device="cuda")
-    for t, i in enumerate(index):
-        if i >= 0 and a[i].shape[0]:
-            v = scales[i] * (a[i].double() @ x[t].double())
-            y[t] += b[i].double() @ v
-            spread[t] = b[i].double().abs() @ v.abs()
+    index = torch.tensor(index, device="cuda")
+    for i in range(len(a)):
+        rows = (index == i).nonzero()[:, 0]
+        v = scales[i] * (x[rows].double() @ a[i].double().t())
+        y[rows] += v @ b[i].double().t()
+        spread[rows] = v.abs() @ b[i].double().abs().t()
     return y, spread
 
 
@@ -97,6 +98,16 @@ def test_kinds_of_batches(T, dtype):
     x, w, a, b, ad, s = make(T, 512, 384, ranks, dtype, 7 * T, lambda i: 0.25 + 0.01 * i)
     for index in ([63] * T, [-1] * T, [t % 64 for t in range(T)], [-1] * (T - 1) + [5], [2] + [-1] * (T - 1), [(t * 4 // T) * 9 - 1 for t in range(T)]):
         check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("T,K,N", [(2300, 72, 2304), (2305, 200, 2301), (4097, 64, 1500), (200, 2048, 300), (700, 1104, 520), (5000, 136, 5000)])
+def test_large_products(T, K, N):
+    """More tiles than pairs of SMs, K in slices; sizes that fill no tile."""
+    ranks = [16, 8, 40, 64]
+    x, w, a, b, ad, s = make(T, K, N, ranks, torch.bfloat16, T)
+    index = [(t // 90) % 5 - 1 for t in range(T)]
+    for dtype in (torch.bfloat16, torch.float32):
+        check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks), dtype), x, w, a, b, s, index)
 
 
 def test_no_adapter_is_the_product():
