@@ -80,15 +80,17 @@ static cudaStream_t caller_stream(void* s) { return (cudaStream_t)s; }
 // stream on which the caller made device_ids and will read logits_out (nullptr: none): the engine's
 // stream waits for it before the step, and it waits for the engine's stream after the step; the host
 // waits for neither.
-ILLM_API int illm_engine_step(void* e, int n_items, const int* slots, const int* n_tokens, const int* tokens, const int* n_want,
-                              const int* want, const int* device_ids, float* logits_out, const float** logits_dev, void* caller) {
+static int engine_step(void* e, int n_items, const int* slots, const int* n_tokens, const int* tokens, const int* n_want, const int* want,
+                       const int* adapters, const int* device_ids, float* logits_out, const float** logits_dev, void* caller) {
     return guard([&] {
         Engine* eng = (Engine*)e;
         eng->device().make_current();
         // the step itself waits for the caller only if it reads the caller's memory; the copy into the
         // caller's buffer waits in any case (the buffer may still be in use on the caller's stream)
         if (caller && device_ids) eng->device().wait_for(caller_stream(caller));
-        LogitsRef lg = eng->step(items_from(n_items, slots, n_tokens, tokens, n_want, want), device_ids);
+        std::vector<StepItem> items = items_from(n_items, slots, n_tokens, tokens, n_want, want);
+        for (int i = 0; adapters && i < n_items; i++) items[(size_t)i].adapter = adapters[i];
+        LogitsRef lg = eng->step(items, device_ids);
         if (logits_dev) *logits_dev = lg.p;
         if (caller && !device_ids && logits_out && lg.rows > 0) eng->device().wait_for(caller_stream(caller));
         if (logits_out && lg.rows > 0)
@@ -96,6 +98,41 @@ ILLM_API int illm_engine_step(void* e, int n_items, const int* slots, const int*
                                        eng->device().stream()),
                        "copying the logits");
         if (caller) eng->device().signal_to(caller_stream(caller));
+    });
+}
+ILLM_API int illm_engine_step(void* e, int n_items, const int* slots, const int* n_tokens, const int* tokens, const int* n_want,
+                              const int* want, const int* device_ids, float* logits_out, const float** logits_dev, void* caller) {
+    return engine_step(e, n_items, slots, n_tokens, tokens, n_want, want, nullptr, device_ids, logits_out, logits_dev, caller);
+}
+// The same with a low-rank adapter per item (-1: none).
+ILLM_API int illm_engine_step_adapters(void* e, int n_items, const int* slots, const int* n_tokens, const int* tokens, const int* n_want,
+                                       const int* want, const int* adapters, const int* device_ids, float* logits_out, const float** logits_dev,
+                                       void* caller) {
+    return engine_step(e, n_items, slots, n_tokens, tokens, n_want, want, adapters, device_ids, logits_out, logits_dev, caller);
+}
+// names[n] with their factors a[i] (float32 [ranks[i], n_in[i]]) and b[i] ([n_out[i], ranks[i]]) on the host.  *out: the adapter's number.
+ILLM_API int illm_engine_add_adapter(void* e, int n, const char** names, const float** a, const float** b, const int* ranks, const long long* n_in,
+                                     const long long* n_out, float scale, int* out) {
+    return guard([&] {
+        AdapterFactors f;
+        f.scale = scale;
+        for (int i = 0; i < n; i++) f.of[names[i]] = AdapterFactors::One{a[i], b[i], ranks[i], n_in[i], n_out[i]};
+        *out = ((Engine*)e)->add_adapter(f);
+    });
+}
+ILLM_API int illm_engine_remove_adapter(void* e, int i) {
+    return guard([&] { ((Engine*)e)->remove_adapter(i); });
+}
+// {name: [out, in]} of the projections beside which adapters run
+ILLM_API int illm_engine_adapted(void* e, char** out) {
+    return guard([&] {
+        Json j = Json::object();
+        for (auto& p : ((Engine*)e)->adapted()) {
+            Json a = Json::array();
+            for (long long v : p.second) a.push(v);
+            j.set(p.first, a);
+        }
+        *out = dup_string(j.dump());
     });
 }
 // Orders the engine's stream against a caller's: direction 0: the engine waits for the caller;
@@ -161,16 +198,26 @@ static SamplingParams params_from(const Json& j) {
     if (j.at("temp").is_number()) p.temp = (float)j.at("temp").as_double();
     if (j.at("top_k").is_int()) p.top_k = (int)j.at("top_k").as_int();
     if (j.at("top_p").is_number()) p.top_p = (float)j.at("top_p").as_double();
+    if (j.at("min_p").is_number()) p.min_p = (float)j.at("min_p").as_double();
     if (j.at("repeat_penalty").is_number()) p.repeat_penalty = (float)j.at("repeat_penalty").as_double();
     if (j.at("repeat_last_n").is_int()) p.repeat_last_n = (int)j.at("repeat_last_n").as_int();
     if (j.at("seed").is_int()) p.seed = j.at("seed").as_int();
     return p;
 }
+static std::vector<SamplingParams> each_from(const Json& j) {
+    std::vector<SamplingParams> out;
+    for (const Json& p : j.items()) out.push_back(params_from(p));
+    return out;
+}
 ILLM_API int illm_sampling_params_validate(const char* params_json) {
     return guard([&] { params_from(parse_json_arg(params_json, "sampling parameters")).validate(); });
 }
 ILLM_API int illm_sampler_create(void* engine, const char* params_json, void** out) {
-    return guard([&] { *out = new Sampler(&((Engine*)engine)->device(), params_from(parse_json_arg(params_json, "sampling parameters"))); });
+    return guard([&] {
+        const Json j = parse_json_arg(params_json, "sampling parameters");      // an object, or a list: one per request number
+        Device* dev = &((Engine*)engine)->device();
+        *out = j.kind() == Json::Array ? new Sampler(dev, each_from(j)) : new Sampler(dev, params_from(j));
+    });
 }
 ILLM_API void illm_sampler_free(void* s) { delete (Sampler*)s; }
 // logits: float32 [B, V] on the device; hist_lens == nullptr: no histories.  *tokens: int32 [B] on the
@@ -208,6 +255,8 @@ ILLM_API int illm_model_create(const char* config_json, const char* model_name, 
         if (j.at("max_batch").is_int()) c.max_batch = (int)j.at("max_batch").as_int();
         if (j.at("page_size").is_int()) c.page_size = (int)j.at("page_size").as_int();
         if (j.at("cuda_graphs").is_bool()) c.cuda_graphs = j.at("cuda_graphs").as_bool();
+        if (j.at("max_adapters").is_int()) c.max_adapters = (int)j.at("max_adapters").as_int();
+        if (j.at("adapter_rank").is_int()) c.adapter_rank = (int)j.at("adapter_rank").as_int();
         if (j.at("gemm").is_string()) c.gemm = j.at("gemm").as_string();
         if (j.at("poison_freed_pages").is_bool()) c.poison_freed_pages = j.at("poison_freed_pages").as_bool();
         if (j.at("stream").is_int()) c.stream = (void*)(uintptr_t)j.at("stream").as_int();
@@ -263,8 +312,8 @@ ILLM_API int illm_model_warm_up(void* m, long long prompt_tokens, const int* bat
 }
 typedef void (*illm_token_fn)(void* user, int request, int token);
 // stop_ids == nullptr: the default stop set (see Model::generate).
-ILLM_API int illm_model_generate(void* m, int n_prompts, const int* prompt_lens, const int* prompts, long long max_new_tokens,
-                                 const int* stop_ids, int n_stop, illm_token_fn on_token, void* user, char** result_json) {
+static int model_generate(void* m, int n_prompts, const int* prompt_lens, const int* prompts, long long max_new_tokens, const int* stop_ids, int n_stop,
+                          const char* sampling_json, const int* adapters, illm_token_fn on_token, void* user, char** result_json) {
     return guard([&] {
         std::vector<std::vector<int>> ps;
         size_t off = 0;
@@ -276,9 +325,23 @@ ILLM_API int illm_model_generate(void* m, int n_prompts, const int* prompt_lens,
         if (stop_ids) stop.assign(stop_ids, stop_ids + n_stop);
         TokenCallback cb;
         if (on_token) cb = [&](int r, int t) { on_token(user, r, t); };
-        GenerationResult res = ((Model*)m)->generate(ps, max_new_tokens, stop_ids ? &stop : nullptr, cb);
+        std::vector<SamplingParams> each;
+        if (sampling_json) each = each_from(parse_json_arg(sampling_json, "sampling parameters"));
+        std::vector<int> ad;
+        if (adapters) ad.assign(adapters, adapters + n_prompts);
+        GenerationResult res = ((Model*)m)->generate(ps, max_new_tokens, stop_ids ? &stop : nullptr, cb, sampling_json ? &each : nullptr, adapters ? &ad : nullptr);
         *result_json = dup_string(res.to_json().dump());
     });
+}
+ILLM_API int illm_model_generate(void* m, int n_prompts, const int* prompt_lens, const int* prompts, long long max_new_tokens,
+                                 const int* stop_ids, int n_stop, illm_token_fn on_token, void* user, char** result_json) {
+    return model_generate(m, n_prompts, prompt_lens, prompts, max_new_tokens, stop_ids, n_stop, nullptr, nullptr, on_token, user, result_json);
+}
+// The same with settings (a JSON list, one per request; nullptr: those of init) and a low-rank adapter (-1: none) per request.
+ILLM_API int illm_model_generate_each(void* m, int n_prompts, const int* prompt_lens, const int* prompts, long long max_new_tokens,
+                                      const int* stop_ids, int n_stop, const char* sampling_json, const int* adapters, illm_token_fn on_token, void* user,
+                                      char** result_json) {
+    return model_generate(m, n_prompts, prompt_lens, prompts, max_new_tokens, stop_ids, n_stop, sampling_json, adapters, on_token, user, result_json);
 }
 
 // ---- single kernels through their C++ faces (tests and kernel benchmarks)

@@ -50,7 +50,10 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const unsigned rank = cluster_ctarank();
     const int n_chunks = plan.counts[2], t0 = plan.chunk_tile[chunk] * ADAPTER_TILE + half * TC_BM;
     const int4 groups = *reinterpret_cast<const int4*>(plan.chunk_groups + chunk * ADAPTER_CHUNK);
-    if (chunk >= n_chunks) return;                      // the grid is sized for more chunks than there are (all blocks of the cluster leave)
+    if (chunk >= n_chunks) {                            // the grid is sized for more chunks than there are (all blocks of the cluster leave)
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // (the product relies on this kernel's wait)
+        return;
+    }
 
     const unsigned a_base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, b_base = a_base + STAGES * A_BYTES;
     float* partial = reinterpret_cast<float*>(smem_raw + (a_base - tc_smem_u32(smem_raw)));     // [128][AP_PITCH] over the ring, when it is done

@@ -213,6 +213,7 @@ long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int gro
 int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int early, int* err, void* stream);
 
 // sample_rows.cu
+int illm_penalise(float* logits, int B, int V, const int* last, int n_last, const float* penalty, void* stream);
 int illm_sample_rows(const void* logits, int dtype, int B, int V, long long ld, const float* uniforms, const float* temp, const int* top_k, const float* top_p, const float* min_p, int* out, void* stream);
 
 #ifdef __cplusplus

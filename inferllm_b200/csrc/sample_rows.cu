@@ -785,3 +785,25 @@ extern "C" int illm_sample_rows(const void* logits, int dtype, int B, int V, lon
     if (dtype == ILLM_BF16) return sr_launch<bf16>(logits, ld, B, V, C, uniforms, temp, top_k, top_p, min_p, out, s);
     return ILLM_ERR_BAD_ARG;
 }
+
+// The repetition penalty of rows with settings of their own: a block per row, a thread per word of its last ones, each word once.
+__global__ void __launch_bounds__(128) penalise_kernel(float* __restrict__ logits, int V, const int* __restrict__ last, int n_last, const float* __restrict__ penalty) {
+    pdl_grid_sync();
+    const float p = penalty[blockIdx.x];
+    const int* mine = last + (size_t)blockIdx.x * n_last;
+    float* row = logits + (size_t)blockIdx.x * V;
+    if (p == 1.0f) return;
+    for (int j = threadIdx.x; j < n_last; j += 128) {
+        const int id = mine[j];
+        if (id < 0 || id >= V) continue;
+        bool first = true;
+        for (int e = 0; e < j && first; e++) first = mine[e] != id;
+        if (first) row[id] = row[id] < 0.f ? row[id] * p : row[id] / p;
+    }
+}
+extern "C" int illm_penalise(float* logits, int B, int V, const int* last, int n_last, const float* penalty, void* stream) {
+    if (B <= 0 || n_last <= 0) return 0;
+    if (V <= 0 || !logits || !last || !penalty) return ILLM_ERR_BAD_ARG;
+    illm_launch(penalise_kernel, dim3((unsigned)B), dim3(128), 0, (cudaStream_t)stream, logits, V, last, n_last, penalty);
+    return illm_launch_status();
+}

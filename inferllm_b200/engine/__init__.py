@@ -29,6 +29,8 @@ class EngineOptions:
     page_size: int = 64
     cuda_graphs: bool = True       # replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     gemm: str = "auto"             # bfloat16 products: "auto" | "tc" | "library"
+    max_adapters: int = 0          # low-rank adapters that may be loaded together (`Engine.add_adapter`)
+    adapter_rank: int = 16         # the largest rank of one (at most 85)
     poison_freed_pages: bool = False    # fill pages that go back to the pool with NaN (a check, not for serving)
 
     def to_json(self, stream: int) -> str:
@@ -53,6 +55,7 @@ class StepItem:
     slot: int
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=list)  # places among `tokens` whose logits are asked for
+    adapter: int = -1          # the low-rank adapter these tokens run with (`Engine.add_adapter`); -1: none
 
 
 def _need_cuda(device_id: int) -> None:
@@ -162,10 +165,46 @@ class Engine:
         if device_ids is not None and (device_ids.dtype != torch.int32 or device_ids.numel() != len(items)):
             raise EngineError("device_ids needs one int32 id per item and items of one token each")
         out = torch.empty((len(want), self.vocab_size), dtype=torch.float32, device=f"cuda:{self.device_id}")
-        _b.check(_b.lib().illm_engine_step(self._ptr, len(slots), _b.ints(slots), _b.ints(n_tok), _b.ints(toks), _b.ints(n_want),
-                                           _b.ints(want), device_ids.data_ptr() if device_ids is not None else None,
-                                           out.data_ptr() if len(want) else None, None, caller_stream(self.device_id)))
+        adapters = [int(it.adapter) for it in items]
+        _b.check(_b.lib().illm_engine_step_adapters(self._ptr, len(slots), _b.ints(slots), _b.ints(n_tok), _b.ints(toks), _b.ints(n_want),
+                                                    _b.ints(want), _b.ints(adapters) if any(a != -1 for a in adapters) else None,
+                                                    device_ids.data_ptr() if device_ids is not None else None,
+                                                    out.data_ptr() if len(want) else None, None, caller_stream(self.device_id)))
         return out
+
+    # ---- low-rank adapters
+
+    def adapted(self) -> dict:
+        """The projections beside which adapters run: name as in the weight file -> [out, in]."""
+        return {k: tuple(v) for k, v in _b.call_json(_b.lib().illm_engine_adapted, self._ptr).items()}
+
+    def add_adapter(self, factors: dict, scale: float = 1.0) -> int:
+        """Load a low-rank adapter; its number is what `StepItem.adapter` and `Model.generate(adapters=...)` take.
+        `factors`: name of a projection (as in the weight file) -> (a [r, in], b [out, r]), anything that turns into a
+        float32 array; the projection's output gets scale * (x a^T) b^T added.  Items of one step may each have another
+        adapter, or none."""
+        import numpy as np
+
+        def host(t):
+            t = t.detach().float().cpu().numpy() if hasattr(t, "detach") else np.asarray(t)
+            return np.ascontiguousarray(t, np.float32)
+
+        pairs = {name: (host(a), host(b)) for name, (a, b) in factors.items()}
+        for name, (a, b) in pairs.items():
+            if a.ndim != 2 or b.ndim != 2 or a.shape[0] != b.shape[1]:
+                raise EngineError(f"adapter: the factors of '{name}' are {a.shape} and {b.shape}, not [r, in] and [out, r]")
+        n, out = len(pairs), ctypes.c_int()
+        P, LL = ctypes.c_void_p, ctypes.c_longlong
+        _b.check(_b.lib().illm_engine_add_adapter(
+            self._ptr, n, (ctypes.c_char_p * max(n, 1))(*[k.encode() for k in pairs]), (P * max(n, 1))(*[a.ctypes.data for a, _ in pairs.values()]),
+            (P * max(n, 1))(*[b.ctypes.data for _, b in pairs.values()]), _b.ints(a.shape[0] for a, _ in pairs.values()),
+            (LL * max(n, 1))(*[a.shape[1] for a, _ in pairs.values()]), (LL * max(n, 1))(*[b.shape[0] for _, b in pairs.values()]), float(scale),
+            ctypes.byref(out)))
+        return out.value
+
+    def remove_adapter(self, adapter: int) -> None:
+        """Free an adapter's place; a step that names it afterwards is refused."""
+        _b.check(_b.lib().illm_engine_remove_adapter(self._ptr, int(adapter)))
 
     def warm_up(self, prompt_tokens: int = 0, batch_sizes: Sequence[int] = ()) -> None:
         sizes = list(batch_sizes)
@@ -394,6 +433,8 @@ class ModelConfig:
     page_size: int = 64
     cuda_graphs: bool = True
     gemm: str = "auto"
+    max_adapters: int = 0
+    adapter_rank: int = 16
     poison_freed_pages: bool = False
 
 
@@ -483,15 +524,20 @@ class Model:
         _b.check(_b.lib().illm_model_warm_up(self._ptr, int(prompt_tokens), _b.ints(sizes), len(sizes)))
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 128, stop_ids: Optional[Sequence[int]] = None,
-                 on_token=None) -> GenerationResult:
+                 on_token=None, sampling: Optional[Sequence] = None, adapters: Optional[Sequence[int]] = None) -> GenerationResult:
         """Generate for many requests.  `stop_ids` default to the end token given to `init`; where that
-        is one of the configuration's end tokens, to all of them."""
+        is one of the configuration's end tokens, to all of them.  `sampling`: `SamplingParams` per request (default: those of
+        `init` for all); `adapters`: a low-rank adapter per request (`engine.add_adapter`), -1 for none."""
         lens = [len(p) for p in prompts]
         flat = [int(t) for p in prompts for t in p]
         stop = None if stop_ids is None else _b.ints(int(s) for s in stop_ids)
         cb = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int, ctypes.c_int)(lambda _u, r, t: on_token(r, t)) if on_token else None
         out = ctypes.c_void_p()
-        _b.check(_b.lib().illm_model_generate(self._ptr, len(lens), _b.ints(lens), _b.ints(flat), int(max_new_tokens), stop,
-                                              0 if stop_ids is None else len(list(stop_ids)),
-                                              ctypes.cast(cb, ctypes.c_void_p) if cb else None, None, ctypes.byref(out)))
+        if adapters is not None and len(adapters) != len(lens):
+            raise ValueError("generate: one adapter per request is needed (-1 for none)")
+        each = None if sampling is None else json.dumps([asdict(p) for p in sampling]).encode()
+        _b.check(_b.lib().illm_model_generate_each(self._ptr, len(lens), _b.ints(lens), _b.ints(flat), int(max_new_tokens), stop,
+                                                   0 if stop_ids is None else len(list(stop_ids)), each,
+                                                   None if adapters is None else _b.ints(adapters),
+                                                   ctypes.cast(cb, ctypes.c_void_p) if cb else None, None, ctypes.byref(out)))
         return GenerationResult(**json.loads(_b.take_string(out)))

@@ -1,9 +1,11 @@
 #include "engine/engine.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <set>
 
+#include "kernels/adapter_plan.h"
 #include "util/log.h"
 #include "weights/loader.h"
 
@@ -19,6 +21,8 @@ EngineOptions EngineOptions::from_json(const Json& j) {
     if (j.at("max_seq_len").is_int()) o.max_seq_len = j.at("max_seq_len").as_int();
     if (j.at("max_batch").is_int()) o.max_batch = (int)j.at("max_batch").as_int();
     if (j.at("page_size").is_int()) o.page_size = (int)j.at("page_size").as_int();
+    if (j.at("max_adapters").is_int()) o.max_adapters = (int)j.at("max_adapters").as_int();
+    if (j.at("adapter_rank").is_int()) o.adapter_rank = (int)j.at("adapter_rank").as_int();
     if (j.at("cuda_graphs").is_bool()) o.cuda_graphs = j.at("cuda_graphs").as_bool();
     if (j.at("gemm").is_string()) o.gemm = j.at("gemm").as_string();
     if (j.at("poison_freed_pages").is_bool()) o.poison_freed_pages = j.at("poison_freed_pages").as_bool();
@@ -45,6 +49,9 @@ static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options) : config_(std::move(config)), options_(options) {
     const DType dtype = engine_dtype(options.dtype);
     if (options.page_size <= 0) throw EngineError("page_size must be positive");
+    if (options.max_adapters < 0 || options.max_adapters > 4096) throw EngineError("max_adapters must be in [0, 4096]");
+    if (options.max_adapters > 0 && (options.adapter_rank < 1 || options.adapter_rank > ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces))
+        throw EngineError("adapter_rank must be in [1, " + std::to_string(ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces) + "]");
     device_.reset(new Device(options.device_id, (cudaStream_t)options.stream));
     rt_.dev = device_.get();
     rt_.dtype = dtype;
@@ -60,6 +67,11 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     cache_.reset(new SequenceCache(model_->cache_requests(), num_slots, num_pages, options.page_size, max_seq, device_.get(), dtype,
                                    options.poison_freed_pages));
     builder_.reset(new StepContextBuilder(device_.get(), &rt_));
+    if (options.max_adapters > 0) {
+        if (model_->adapted().empty()) throw EngineError("max_adapters: no layer of this model runs low-rank adapters");
+        model_->make_adapters(options.max_adapters, options.adapter_rank);
+        adapter_ranks_.assign((size_t)options.max_adapters, 0);
+    }
     for (TokRead& t : tok_reads_) check_cuda(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming), "cudaEventCreate");
     // say once which attention kernels the model's layers get: a head size that the tensor-core kernels
     // do not take falls to the general kernel, which is right but far slower on prompts
@@ -156,9 +168,62 @@ size_t Engine::context_ints(int T, int B, int K) const {
     return StepContextBuilder::ints(T, B, K, cache_->paged.size(), cache_->width);
 }
 
+int Engine::add_adapter(const AdapterFactors& f) {
+    device_->make_current();
+    const auto free = std::find(adapter_ranks_.begin(), adapter_ranks_.end(), 0);
+    if (free == adapter_ranks_.end())
+        throw EngineError("there is room for " + std::to_string(adapter_ranks_.size()) + " adapters (EngineOptions::max_adapters), and all are in use");
+    const auto names = model_->adapted();
+    std::string wrong;
+    int rank = 0;
+    if (f.of.empty()) wrong = " it has no factors;";
+    if (!std::isfinite(f.scale)) wrong += " its scale is not finite;";
+    for (auto& o : f.of) {
+        const AdapterFactors::One& one = o.second;
+        auto it = names.find(o.first);
+        if (it == names.end()) {
+            wrong += " '" + o.first + "' is no projection that runs adapters;";
+            continue;
+        }
+        if (one.n_out != it->second[0] || one.n_in != it->second[1])
+            wrong += " '" + o.first + "' is [" + std::to_string(it->second[0]) + ", " + std::to_string(it->second[1]) + "], the factors are for [" +
+                     std::to_string(one.n_out) + ", " + std::to_string(one.n_in) + "];";
+        else if (one.r < 1 || one.r > options_.adapter_rank)
+            wrong += " '" + o.first + "': rank " + std::to_string(one.r) + " is outside [1, " + std::to_string(options_.adapter_rank) + "];";
+        else {
+            // (the prompt product multiplies an adapter's second factor with the zeros of its neighbours' tokens)
+            const float most = rt_.is_f32() ? 3.4028235e38f : 3.3895314e38f;       // the largest that stays finite
+            bool finite = true;
+            for (long long k = 0; k < one.r * one.n_in; k++) finite = finite && std::fabs(one.a[k]) <= most;
+            for (long long k = 0; k < one.r * one.n_out; k++) finite = finite && std::fabs(one.b[k]) <= most;
+            if (!finite) wrong += " '" + o.first + "' is not finite;";
+        }
+        rank = std::max(rank, one.r);
+    }
+    if (!wrong.empty()) throw EngineError("the adapter does not fit the model:" + wrong);
+    AdapterFactors own = f;
+    own.rank = rank;
+    const int i = (int)(free - adapter_ranks_.begin());
+    model_->put_adapter(i, own);
+    adapter_ranks_[(size_t)i] = rank;
+    return i;
+}
+void Engine::remove_adapter(int i) {
+    if (i < 0 || i >= (int)adapter_ranks_.size() || adapter_ranks_[(size_t)i] == 0) throw EngineError("adapter " + std::to_string(i) + " is not there");
+    adapter_ranks_[(size_t)i] = 0;
+}
+// What is set aside for the plans: as much as these tokens need, or (a captured step) as any step of its kind can.
+void Engine::size_adapters(StepAdapters& a, bool fixed, bool one_sequence) const {
+    for (int p = 1; p <= kAdapterPieces; p++) {
+        const std::vector<int> ranks = a.packed_ranks(p);
+        a.sizes[p - 1] = fixed ? ops::adapter_plan_bound((int)a.index.size(), (int)ranks.size(), p * options_.adapter_rank, one_sequence)
+                               : ops::adapter_plan_sizes(a.index.data(), (int)a.index.size(), ranks.data(), (int)ranks.size());
+    }
+}
+
 StepContext Engine::make_context(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows, int* into,
-                                 std::vector<const int*>* tables_dev) {
-    StepContext ctx = builder_->build(*cache_, plan, ids, want_rows, into, tables_dev);
+                                 std::vector<const int*>* tables_dev, const StepAdapters* adapters) {
+    StepContext ctx = builder_->build(*cache_, plan, ids, want_rows, into, tables_dev, adapters);
     last_upload_bytes_ = builder_->last_upload_bytes;
     return ctx;
 }
@@ -176,6 +241,7 @@ LogitsRef Engine::step(const std::vector<StepItem>& items, const int* device_ids
     device_->make_current();
     const long long V = vocab_size();
     std::vector<int> ids, want_rows, slots, q_lens;
+    StepAdapters step_adapters, *adapters = nullptr;
     int off = 0;
     for (const StepItem& it : items) {
         const int n = (int)it.tokens.size();
@@ -190,27 +256,36 @@ LogitsRef Engine::step(const std::vector<StepItem>& items, const int* device_ids
                                   std::to_string(n) + " tokens");
             want_rows.push_back(off + w);
         }
+        if (it.adapter != -1) {
+            if (it.adapter < 0 || it.adapter >= (int)adapter_ranks_.size() || adapter_ranks_[(size_t)it.adapter] == 0)
+                throw EngineError("slot " + std::to_string(it.slot) + ": adapter " + std::to_string(it.adapter) + " is not there");
+            adapters = &step_adapters;
+        }
+        step_adapters.index.insert(step_adapters.index.end(), it.tokens.size(), it.adapter);
         ids.insert(ids.end(), it.tokens.begin(), it.tokens.end());
         slots.push_back(it.slot);
         q_lens.push_back(n);
         off += n;
     }
     if (device_ids && ids.size() != items.size()) throw EngineError("device_ids needs one int32 id per item and items of one token each");
+    if (adapters) adapters->ranks = adapter_ranks_;
     if (graph_safe_ < 0) graph_safe_ = model_->graph_safe() ? 1 : 0;
     if (options_.cuda_graphs && items.size() == 1 && ids.size() > 1 && ids.size() <= (size_t)kPromptGraphMaxTokens) {
         if (pad_safe_ < 0) pad_safe_ = model_->pad_safe() ? 1 : 0;
         LogitsRef out;
-        if (pad_safe_ && prompt_step_graphed(items[0].slot, ids, want_rows, &out)) return out;
+        if (pad_safe_ && prompt_step_graphed(items[0].slot, ids, want_rows, adapters, &out)) return out;
     }
     StepPlan plan = cache_->plan_step(slots, q_lens);
     LogitsRef logits;
     try {
         if (options_.cuda_graphs && ids.size() == items.size() && graph_safe_) {
-            logits = decode_step_graphed(plan, ids, want_rows, device_ids);
+            if (adapters) size_adapters(*adapters, true, false);
+            logits = decode_step_graphed(plan, ids, want_rows, device_ids, adapters);
         } else {
+            if (adapters) size_adapters(*adapters, false, false);
             device_->arena_rewind();
             std::vector<const int*> tables;
-            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables);
+            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
             if (device_ids)
                 check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                            "copying the step's token ids");
@@ -240,16 +315,16 @@ void Engine::drop_graphs(bool keep_seen) {
 }
 
 LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, const std::vector<int>& ids,
-                                  const std::vector<int>& want_rows, const int* device_ids) {
+                                  const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters) {
     if (graphs_.size() > 64) drop_graphs(true);
     std::unique_ptr<GraphEntry> e(new GraphEntry);
     int T = 0;
     for (int q : plan.q_lens) T += q;
-    e->ctx_buf = (int*)device_->alloc_persistent(context_ints(T, (int)plan.slots.size(), (int)want_rows.size()) * sizeof(int),
-                                                 "the inputs of a captured step");
+    e->ctx_buf = (int*)device_->alloc_persistent(
+            (context_ints(T, (int)plan.slots.size(), (int)want_rows.size()) + (adapters ? adapters->ints() : 0)) * sizeof(int), "the inputs of a captured step");
     device_->arena_rewind();
     std::vector<const int*> tables;
-    StepContext ctx = make_context(plan, ids, want_rows, e->ctx_buf, &tables);
+    StepContext ctx = make_context(plan, ids, want_rows, e->ctx_buf, &tables, adapters);
     if (device_ids)
         check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                    "copying the step's token ids");
@@ -286,9 +361,9 @@ LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, 
 }
 
 LogitsRef Engine::replay(GraphEntry& e, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                         const int* device_ids) {
+                         const int* device_ids, const StepAdapters* adapters) {
     std::vector<const int*> tables;
-    StepContext ctx = make_context(plan, ids, want_rows, e.ctx_buf, &tables);
+    StepContext ctx = make_context(plan, ids, want_rows, e.ctx_buf, &tables, adapters);
     if (device_ids)
         check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                    "copying the step's token ids");
@@ -305,7 +380,7 @@ LogitsRef Engine::replay(GraphEntry& e, const StepPlan& plan, const std::vector<
 // page that the step would not need anyway and stays within the longest sequence; false otherwise (the
 // caller then runs the step as it is).  The logits of the real tokens do not depend on the padding
 // beyond rounding, and in float32 not at all.
-bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const std::vector<int>& want_rows, LogitsRef* out) {
+bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const std::vector<int>& want_rows, StepAdapters* adapters, LogitsRef* out) {
     SequenceCache& c = *cache_;
     const int T = (int)ids_in.size();
     const int padded = (int)ceil_div(T, kPromptBucket) * kPromptBucket;
@@ -317,19 +392,23 @@ bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const
     StepPlan plan = c.plan_step({slot}, {padded});
     std::vector<int> ids = ids_in;
     ids.resize((size_t)padded, 0);
-    const std::string key = "p/" + std::to_string(padded) + "/" + std::to_string(want_rows.size());
+    const std::string key = std::string(adapters ? "pa/" : "p/") + std::to_string(padded) + "/" + std::to_string(want_rows.size());
     try {
+        if (adapters) {
+            adapters->index.resize((size_t)padded, adapters->index.back());
+            size_adapters(*adapters, true, true);
+        }
         auto it = graphs_.find(key);
         if (it == graphs_.end()) {
             graphs_[key].reset(new GraphEntry);       // seen once
             device_->arena_rewind();
             std::vector<const int*> tables;
-            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables);
+            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
             *out = run_forward(ctx, tables);
         } else if (!it->second->exec) {
-            *out = capture_and_run(key, plan, ids, want_rows, nullptr);
+            *out = capture_and_run(key, plan, ids, want_rows, nullptr, adapters);
         } else {
-            *out = replay(*it->second, plan, ids, want_rows, nullptr);
+            *out = replay(*it->second, plan, ids, want_rows, nullptr, adapters);
         }
     } catch (...) {
         c.abandon_step(plan);
@@ -344,21 +423,21 @@ bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const
 // in device memory), so the step is captured in a CUDA graph the second time a batch size is seen and
 // replayed from then on.
 LogitsRef Engine::decode_step_graphed(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                                      const int* device_ids) {
-    const std::string key = "d/" + std::to_string(ids.size()) + "/" + std::to_string(want_rows.size());
+                                      const int* device_ids, const StepAdapters* adapters) {
+    const std::string key = std::string(adapters ? "da/" : "d/") + std::to_string(ids.size()) + "/" + std::to_string(want_rows.size());
     auto it = graphs_.find(key);
     if (it == graphs_.end()) {
         graphs_[key].reset(new GraphEntry);
         device_->arena_rewind();
         std::vector<const int*> tables;
-        StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables);
+        StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
         if (device_ids)
             check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                        "copying the step's token ids");
         return run_forward(ctx, tables);
     }
-    if (!it->second->exec) return capture_and_run(key, plan, ids, want_rows, device_ids);
-    return replay(*it->second, plan, ids, want_rows, device_ids);
+    if (!it->second->exec) return capture_and_run(key, plan, ids, want_rows, device_ids, adapters);
+    return replay(*it->second, plan, ids, want_rows, device_ids, adapters);
 }
 
 void Engine::read_logits(const LogitsRef& logits, float* host) {

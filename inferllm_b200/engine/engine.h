@@ -32,6 +32,8 @@ struct EngineOptions {
     int max_batch = 0;                  // slots; 0: max_tokens / page_size
     int page_size = 64;
     bool cuda_graphs = true;            // replay one-token-per-sequence steps and single prompts from captured CUDA graphs
+    int max_adapters = 0;               // low-rank adapters that may be loaded together (Engine::add_adapter)
+    int adapter_rank = 16;              // the largest rank of one (at most 85: q, k and v stand side by side)
     std::string gemm = "auto";          // bfloat16 products: "auto" | "tc" | "library" (see ops::GemmBackend)
     bool poison_freed_pages = false;    // fill pages that go back to the pool with NaN (a check, not for serving)
     void* stream = nullptr;             // the CUDA stream to work on; nullptr: one of the engine's own
@@ -50,6 +52,7 @@ struct StepItem {
     int slot = 0;
     std::vector<int> tokens;
     std::vector<int> want;      // places among `tokens` whose logits are asked for
+    int adapter = -1;           // the low-rank adapter that these tokens run with (Engine::add_adapter); -1: none
 };
 
 // Logits of a step on the device: float32 [rows, vocab], valid until the engine's next step.
@@ -89,6 +92,13 @@ public:
     // size replay.  Uses free slots and pages only and gives them back; sizes that do not fit the cache
     // are left out.
     void warm_up(long long prompt_tokens, const std::vector<int>& batch_sizes);
+    // Low-rank adapters: every item of a step may run with one of its own, all in one batch.  add_adapter takes factors by the names
+    // (as in the weight file) of the projections that they stand beside and returns the adapter's number, the lowest free one;
+    // remove_adapter frees it.  Both wait for the steps that the stream holds.
+    int add_adapter(const AdapterFactors& factors);
+    void remove_adapter(int i);
+    std::map<std::string, std::vector<long long>> adapted() const { return model_->adapted(); }
+
     // Read the kernels' error words (synchronises); EngineError naming what a kernel reported.
     void check_device_errors();
 
@@ -115,15 +125,16 @@ private:
     struct GraphEntry;
     long long tokens_that_fit(double fraction) const;
     StepContext make_context(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows, int* into,
-                             std::vector<const int*>* tables_dev);
+                             std::vector<const int*>* tables_dev, const StepAdapters* adapters);
+    void size_adapters(StepAdapters& a, bool fixed, bool one_sequence) const;
     LogitsRef run_forward(const StepContext& ctx, const std::vector<const int*>& tables);
-    bool prompt_step_graphed(int slot, const std::vector<int>& ids, const std::vector<int>& want_rows, LogitsRef* out);
+    bool prompt_step_graphed(int slot, const std::vector<int>& ids, const std::vector<int>& want_rows, StepAdapters* adapters, LogitsRef* out);
     LogitsRef decode_step_graphed(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                                  const int* device_ids);
+                                  const int* device_ids, const StepAdapters* adapters);
     LogitsRef capture_and_run(const std::string& key, const StepPlan& plan, const std::vector<int>& ids,
-                              const std::vector<int>& want_rows, const int* device_ids);
+                              const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters);
     LogitsRef replay(GraphEntry& e, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                     const int* device_ids);
+                     const int* device_ids, const StepAdapters* adapters);
     void drop_graphs(bool keep_seen);
     size_t context_ints(int T, int B, int K) const;
 
@@ -134,6 +145,7 @@ private:
     std::unique_ptr<DecoderModel> model_;
     std::unique_ptr<SequenceCache> cache_;
     bool loaded_ = false;
+    std::vector<int> adapter_ranks_;        // 0: free
     int pad_safe_ = -1, graph_safe_ = -1;
     size_t last_upload_bytes_ = 0;
 

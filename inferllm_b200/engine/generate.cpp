@@ -75,11 +75,13 @@ static double wall_clock() {
 }
 
 GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int>>& prompts, Chooser& chooser, long long max_new_tokens,
-                          const std::vector<int>& stop_ids, const TokenCallback& on_token, const std::function<double()>& clock_in) {
+                          const std::vector<int>& stop_ids, const TokenCallback& on_token, const std::function<double()>& clock_in,
+                          const std::vector<int>* adapters) {
     const std::function<double()> clock = clock_in ? clock_in : std::function<double()>(wall_clock);
     const Limits limits = backend.limits();
     const std::set<int> stop(stop_ids.begin(), stop_ids.end());
     const size_t n = prompts.size();
+    if (adapters && adapters->size() != n) throw ValueError("generate: one adapter per request is needed (-1 for none)");
     GenerationResult res;
     res.tokens.resize(n);
     res.finish.assign(n, "");
@@ -111,6 +113,7 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
                 it.slot = slots[r];
                 it.tokens = prompts[(size_t)r];
                 it.want = {(int)prompts[(size_t)r].size() - 1};
+                if (adapters) it.adapter = (*adapters)[(size_t)r];
                 items.push_back(std::move(it));
                 hist.push_back(prompts[(size_t)r]);
             }
@@ -148,6 +151,7 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
                         it.slot = slots[r];
                         it.tokens = {0};
                         it.want = {0};
+                        if (adapters) it.adapter = (*adapters)[(size_t)r];
                         its.push_back(std::move(it));
                         steps.push_back(n_tok[r]);
                     }

@@ -69,7 +69,8 @@ std::vector<std::vector<int>> plan_batches(const std::vector<int>& prompt_lens, 
 using TokenCallback = std::function<void(int request, int token)>;
 GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int>>& prompts, Chooser& chooser, long long max_new_tokens,
                           const std::vector<int>& stop_ids, const TokenCallback& on_token = nullptr,
-                          const std::function<double()>& clock = nullptr);
+                          const std::function<double()>& clock = nullptr,
+                          const std::vector<int>* adapters = nullptr /* per request, -1: none (StepItem::adapter) */);
 
 // The engine and the sampler behind the loop's interfaces.
 class EngineBackend : public GenBackend {

@@ -32,6 +32,8 @@ EngineOptions Model::options() const {
     o.page_size = config_.page_size;
     o.cuda_graphs = config_.cuda_graphs;
     o.gemm = config_.gemm;
+    o.max_adapters = config_.max_adapters;
+    o.adapter_rank = config_.adapter_rank;
     o.poison_freed_pages = config_.poison_freed_pages;
     o.stream = config_.stream;
     return o;
@@ -148,7 +150,8 @@ std::string Model::decode_summary() const {
 void Model::warm_up(long long prompt_tokens, const std::vector<int>& batch_sizes) { engine().warm_up(prompt_tokens, batch_sizes); }
 
 GenerationResult Model::generate(const std::vector<std::vector<int>>& prompts, long long max_new_tokens, const std::vector<int>* stop_ids,
-                                 const TokenCallback& on_token) {
+                                 const TokenCallback& on_token, const std::vector<SamplingParams>* sampling, const std::vector<int>* adapters) {
+    if (sampling && sampling->size() != prompts.size()) throw ValueError("generate: one set of sampling parameters per request is needed");
     std::vector<int> stop;
     if (stop_ids) {
         stop = *stop_ids;
@@ -158,11 +161,12 @@ GenerationResult Model::generate(const std::vector<std::vector<int>>& prompts, l
         stop = {end_token_};
     }
     Engine& e = engine();
-    Sampler sampler(&e.device(), sampling_);
+    if (prompts.empty()) sampling = nullptr;
+    std::unique_ptr<Sampler> sampler(sampling ? new Sampler(&e.device(), *sampling) : new Sampler(&e.device(), sampling_));
     // the sampler keeps the windows of last tokens for the repetition penalty on the device
-    SamplerChooser chooser(&sampler);
+    SamplerChooser chooser(sampler.get());
     EngineBackend backend(&e);
-    GenerationResult res = illm::generate(backend, prompts, chooser, max_new_tokens, stop, on_token);
+    GenerationResult res = illm::generate(backend, prompts, chooser, max_new_tokens, stop, on_token, nullptr, adapters);
     e.check_device_errors();
     return res;
 }

@@ -33,6 +33,7 @@ struct ModelConfig {
     int page_size = 64;
     bool cuda_graphs = true;
     std::string gemm = "auto";
+    int max_adapters = 0, adapter_rank = 16;
     bool poison_freed_pages = false;
     void* stream = nullptr;
 };
@@ -66,7 +67,9 @@ public:
     // tokens (or init() was given none), all of them: the reference ends a turn on its one end token
     // (application/llama/llama.cpp:237), a config.json may name several.
     GenerationResult generate(const std::vector<std::vector<int>>& prompts, long long max_new_tokens = 128,
-                              const std::vector<int>* stop_ids = nullptr, const TokenCallback& on_token = nullptr);
+                              const std::vector<int>* stop_ids = nullptr, const TokenCallback& on_token = nullptr,
+                              const std::vector<SamplingParams>* sampling = nullptr /* per request; nullptr: as given to init() */,
+                              const std::vector<int>* adapters = nullptr /* per request, -1: none (Engine::add_adapter) */);
     void warm_up(long long prompt_tokens, const std::vector<int>& batch_sizes);
 
     Engine& engine();

@@ -2,6 +2,8 @@
 
 #include <algorithm>
 
+#include "kernels/adapter_plan.h"
+
 namespace illm {
 
 StepContextBuilder::StepContextBuilder(Device* dev, Runtime* rt) : dev_(dev), rt_(rt) {
@@ -21,7 +23,8 @@ size_t StepContextBuilder::ints(int T, int B, int K, size_t n_groups, int width)
 }
 
 StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan& plan, const std::vector<int>& ids,
-                                      const std::vector<int>& want_rows, int* into, std::vector<const int*>* tables_dev) {
+                                      const std::vector<int>& want_rows, int* into, std::vector<const int*>* tables_dev,
+                                      const StepAdapters* adapters) {
     const int B = (int)plan.slots.size(), K = (int)want_rows.size();
     int T = 0, max_q = 0;
     long long max_len = 0;
@@ -30,7 +33,7 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
         max_q = std::max(max_q, plan.q_lens[i]);
         max_len = std::max(max_len, plan.past[i] + plan.q_lens[i]);
     }
-    const size_t total = ints(T, B, K, cache.paged.size(), cache.width);
+    const size_t own = ints(T, B, K, cache.paged.size(), cache.width), total = own + (adapters ? adapters->ints() : 0);
     // one asynchronous copy for all of a step's index arrays, from a small ring of pinned staging
     // buffers: the host may prepare the next steps while the GPU still runs this one, and waits only
     // when it comes back to a buffer whose copy has not left yet
@@ -70,6 +73,16 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
         std::copy(tab.begin(), tab.end(), h + off);
         off += pad4(tab.size());
     }
+    size_t o_plan[kAdapterPieces] = {};
+    if (adapters) {
+        off = own;
+        for (int p = 0; p < kAdapterPieces; p++) {
+            const std::vector<int> ranks = adapters->packed_ranks(p + 1);
+            ops::adapter_plan_fill(adapters->index.data(), T, ranks.data(), (int)ranks.size(), adapters->sizes[p], h + off);
+            o_plan[p] = off;
+            off += (size_t)adapter_plan_layout(adapters->sizes[p]).total;
+        }
+    }
     int* buf = into ? into : dev_->alloc_n<int>(total);
     check_cuda(cudaMemcpyAsync(buf, h, total * sizeof(int), cudaMemcpyHostToDevice, dev_->stream()), "uploading a step's index arrays");
     check_cuda(cudaEventRecord(st.busy, dev_->stream()), "cudaEventRecord");
@@ -93,6 +106,8 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
     ctx.max_seq_len = cache.max_seq_len;
     ctx.is_decode = max_q == 1;
     ctx.err = dev_->step_error_word();
+    ctx.adapted = adapters != nullptr;
+    for (int p = 0; adapters && p < kAdapterPieces; p++) ctx.adapters[p] = AdapterView{buf + o_plan[p], adapters->sizes[p]};
     ctx.dev = dev_;
     ctx.rt = rt_;
     ctx.q_lens = plan.q_lens;

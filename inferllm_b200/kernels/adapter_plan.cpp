@@ -41,11 +41,14 @@ AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, i
     return s;
 }
 
-AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool tiles) {
-    const int slots = tiles ? std::min(1, T) : std::min(T, count);
+AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool one_sequence) {
+    const int slots = one_sequence ? std::min(1, T) : std::min(T, count);
     AdapterPlanSizes s{T, slots, slots * groups_of(max_rank), 0};
-    if (tiles && T > ADAPTER_ROWS_MAX)
-        s.chunks = (T + ADAPTER_TILE - 1) / ADAPTER_TILE * ((groups_of(max_rank) + ADAPTER_CHUNK - 1) / ADAPTER_CHUNK);
+    if (T > ADAPTER_ROWS_MAX)
+        for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE) {
+            const int adapters = std::min(tile_end(t0, T) - t0, slots);
+            s.chunks += (adapters * groups_of(max_rank) + ADAPTER_CHUNK - 1) / ADAPTER_CHUNK;
+        }
     return s;
 }
 

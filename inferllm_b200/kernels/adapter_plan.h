@@ -11,8 +11,8 @@ namespace ops {
 // adapter a.  KernelError for an index outside the adapters, a rank outside [0, 256] or too many tokens.
 AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, int count);
 // Sizes that hold any plan of T tokens over `count` adapters of ranks up to max_rank (for captured steps, whose arrays must
-// not move): single tokens of many sequences (tiles == false) or one sequence's tokens (tiles == true: one adapter).
-AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool tiles);
+// not move): of one sequence, which has one adapter, or of any.
+AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool one_sequence);
 // Fills out[0 .. layout(sizes).total).
 void adapter_plan_fill(const int* index, int T, const int* ranks, int count, const AdapterPlanSizes& sizes, int* out);
 

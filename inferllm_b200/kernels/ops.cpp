@@ -414,6 +414,38 @@ Mat linear_gated(Device& dev, GemmBackend backend, const Mat& x, const Mat& w, i
     return out;
 }
 
+// ---- low-rank adapters
+
+Mat linear_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, DType out_dtype) {
+    need(x, "x");
+    need(w, "w", true, x.dtype);
+    const long long T = x.rows, K = x.cols, N = w.rows;
+    if (w.cols != K) throw KernelError("linear_adapters: the operands' inner sizes differ");
+    if (view.sizes.T != T || !view.plan || !set.a || !set.b || !set.scales)
+        throw KernelError("linear_adapters: the plan is of " + std::to_string(view.sizes.T) + " tokens, x has " + std::to_string(T));
+    if (x.dtype == DType::BF16 && K % 8) throw KernelError("linear_adapters: K = " + std::to_string(K) + " must be a multiple of 8 in bfloat16");
+    if (x.dtype == DType::F32 && out_dtype != DType::F32) throw KernelError("linear_adapters: a float32 product stays float32");
+    Mat out = new_mat(dev, T, N, out_dtype);
+    if (T == 0) return out;
+    const int code = code_of(x.dtype, "linear_adapters");
+    void* ws = dev.alloc((size_t)illm_linear_adapters_ws(code, (int)T, (int)N, (int)K, set.R, view.sizes.groups, view.sizes.chunks));
+    check_kernel(illm_linear_adapters(x.p, w.p, code, (int)T, (int)N, (int)K, set.a, set.b, set.scales, set.count, set.R, view.plan, view.sizes.slots,
+                                      view.sizes.groups, view.sizes.chunks, out.p, code_of(out_dtype, "linear_adapters"), ws, 1, dev.tc_error_word(),
+                                      dev.stream()),
+                 "linear_adapters");
+    return out;
+}
+
+Mat linear_gated_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, int act, float act_limit) {
+    MatOrPartials gu;
+    gu.m = linear_adapters(dev, x, w, set, view, x.dtype);
+    if (act == kActSilu) return swiglu(dev, gu);
+    if (gu.m.cols % 2) throw KernelError("gated activation: the packed projection must have an even number of columns");
+    Mat out = new_mat(dev, gu.m.rows, gu.m.cols / 2, gu.m.dtype);
+    check_kernel(illm_gated_act_ex(gu.m.p, out.p, code_of(out.dtype, "gated_act"), (int)out.rows, (int)out.cols, act, act_limit, dev.stream()), "gated_act");
+    return out;
+}
+
 // ---- rotation and attention
 
 static void check_cache(const KVView& kv, DType want, Geometry g, const char* what) {
@@ -1430,6 +1462,17 @@ int* sample(Device& dev, const float* logits, long long B, long long V, const fl
                      "sample");
     }
     return out;
+}
+
+int* sample_rows(Device& dev, const float* logits, long long B, long long V, const float* uniforms, const float* temp, const int* top_k, const float* top_p,
+                 const float* min_p, int* out) {
+    if (!out) out = dev.alloc_n<int>((size_t)std::max<long long>(B, 1));
+    check_kernel(illm_sample_rows(logits, 0, (int)B, (int)V, V, uniforms, temp, top_k, top_p, min_p, out, dev.stream()), "sample_rows");
+    return out;
+}
+
+void penalise(Device& dev, float* logits, long long B, long long V, const int* last, int n_last, const float* penalty) {
+    check_kernel(illm_penalise(logits, (int)B, (int)V, last, n_last, penalty, dev.stream()), "penalise");
 }
 
 void fill_random(Device& dev, void* out, DType dtype, long long n, unsigned long long key, float std, float mean) {

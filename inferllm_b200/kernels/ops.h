@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "cache/cache.h"
+#include "csrc/adapters.h"
 #include "device/device.h"
 
 namespace illm {
@@ -53,6 +54,21 @@ struct MatOrPartials {
     long long stride() const { return is_partials() ? part.rows * part.cols : 0; }
 };
 
+// The low-rank adapters beside one projection [n_out, n_in]: a [count, R, n_in], b [count, R / 16, n_out, 16] in the projection's
+// dtype, scales float32 [count]; R the largest rank rounded up to 16 (csrc/adapters.cu).
+struct AdapterSet {
+    const void *a = nullptr, *b = nullptr;
+    const float* scales = nullptr;
+    int count = 0, R = 0;
+};
+// The plan of a step's tokens among adapters (csrc/adapters.h), on the device.
+struct AdapterView {
+    const int* plan = nullptr;
+    AdapterPlanSizes sizes{0, 0, 0, 0};
+};
+// Projections are packed (q, k, v; gate, up): an adapter's ranks beside a packed one are those of its pieces side by side.
+constexpr int kAdapterPieces = 3;
+
 // What every part sees of a step, on the device: int32 arrays in one buffer.
 struct StepView {
     const int* ids = nullptr;         // [T] token id
@@ -69,6 +85,8 @@ struct StepView {
     long long max_seq_len = 0;        // the longest sequence the cache allows (sizes decode grids and scratch)
     bool is_decode = false;           // one token per sequence
     int* err = nullptr;               // the step's error word
+    bool adapted = false;             // some of the step's sequences have a low-rank adapter: adapters[p - 1] is the plan for
+    AdapterView adapters[kAdapterPieces];      // projections packed of p pieces
 };
 
 namespace ops {
@@ -172,6 +190,13 @@ MatOrPartials linear(Device& dev, GemmBackend backend, const Mat& x, const Mat& 
 // by default); the product kernels of the package apply it in their epilogues.
 // act_limit: the limit of kActSwishClamped.
 Mat linear_gated(Device& dev, GemmBackend backend, const Mat& x, const Mat& w, int act = 1 /* kActSilu */, float act_limit = 0.f);
+
+// x [T, K] . w [N, K]^T plus every token's adapter, scale_a (x[t] . a_a^T) . b_a^T, in one float32 sum, rounded once: few tokens as
+// further rows of the weight, prompts as a longer K, float32 behind the product (csrc/adapters.cu, adapters_prompt.cu).  The weights
+// and the adapters must not come from the kernel that runs before.
+Mat linear_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, DType out_dtype);
+// act(gate) * up of it, for a weight whose rows 2i, 2i + 1 are the gate and the up row of output i.
+Mat linear_gated_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, int act, float act_limit);
 
 struct Geometry { int n_heads, n_kv_heads, head_dim; };
 // Rotate Q (and K) of the packed projection and store K, V in the cache pages.  cos_sin: float32
@@ -507,6 +532,11 @@ int* argmax(Device& dev, const float* logits, long long B, long long V, int* out
 // src/utils.cpp:31-115).  uniforms float32 [B] in [0, 1); last_tokens int32 [B, n_last] (-1 pads) or nullptr.
 int* sample(Device& dev, const float* logits, long long B, long long V, const float* uniforms, float temp, int top_k, float top_p,
             float repeat_penalty, const int* last_tokens, int n_last, int* out /* nullptr: from the arena */);
+// One token per row by settings of the row's own (csrc/sample_rows.cu): temp, top_k, top_p, min_p [B] on the device.
+int* sample_rows(Device& dev, const float* logits, long long B, long long V, const float* uniforms, const float* temp, const int* top_k, const float* top_p,
+                 const float* min_p, int* out);
+// logits [B, V] in place: of the words in last[b, 0 .. n_last) (-1: none) each once, l < 0 ? l * penalty[b] : l / penalty[b].
+void penalise(Device& dev, float* logits, long long B, long long V, const int* last, int n_last, const float* penalty);
 void fill_random(Device& dev, void* out, DType dtype, long long n, unsigned long long key, float std, float mean);
 void convert(Device& dev, const void* src, DType src_dtype, void* dst, DType dst_dtype, long long n);
 // x in another dtype, as a new activation (x itself if it has that dtype already)

@@ -1,5 +1,7 @@
 #include "models/decoder.h"
 
+#include <algorithm>
+
 #include "cache/cache.h"
 
 namespace illm {
@@ -66,6 +68,32 @@ void DecoderModel::load_tensors(const std::function<std::unique_ptr<TensorSource
         o.second->load(*src);
     }
     if (head_->tied()) head_->tie(*embedding_);
+}
+
+std::map<std::string, std::vector<long long>> DecoderModel::adapted() const {
+    std::map<std::string, std::vector<long long>> out;
+    for (auto& o : owners()) {
+        const std::vector<std::string> names = o.second->adapted();
+        for (auto& d : o.second->tensors())
+            if (std::find(names.begin(), names.end(), d.first) != names.end()) out[o.first + d.first] = d.second.shape;
+    }
+    return out;
+}
+void DecoderModel::make_adapters(int count, int rank) {
+    for (auto& o : owners()) o.second->make_adapters(count, rank);
+}
+void DecoderModel::put_adapter(int i, const AdapterFactors& f) {
+    for (auto& o : owners()) {
+        if (o.second->adapted().empty()) continue;
+        AdapterFactors own;
+        own.scale = f.scale;
+        own.rank = f.rank;
+        for (const std::string& n : o.second->adapted()) {
+            auto it = f.of.find(o.first + n);
+            if (it != f.of.end()) own.of[n] = it->second;
+        }
+        o.second->put_adapter(i, own);
+    }
 }
 
 std::map<int, CacheRequest> DecoderModel::cache_requests() const {

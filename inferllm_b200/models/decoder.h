@@ -42,6 +42,11 @@ public:
     std::map<int, CacheRequest> cache_requests() const;
     // Run the tokens of one step; float32 logits [ctx.K, vocab] (rows == 0 when nothing is wanted).
     Mat forward(const StepContext& ctx, const SequenceCache& cache, const std::vector<const int*>& tables_dev);
+    // Low-rank adapters: the names (as in the weight file) of the matrices beside which they can stand, with their shapes; room
+    // for `count` of rank up to `rank`; adapter i's factors by those names.
+    std::map<std::string, std::vector<long long>> adapted() const;
+    void make_adapters(int count, int rank);
+    void put_adapter(int i, const AdapterFactors& f);
     // true if a one-token-per-sequence step launches the same kernels every time, i.e. no part reads
     // host-side fields of the step context.
     bool graph_safe() const;

@@ -1,5 +1,7 @@
 #include "parts/parts.h"
 
+#include "parts/adapted.h"
+
 #include <cmath>
 
 namespace illm {
@@ -775,16 +777,46 @@ struct Attention : Mixer {
         if (ctx.is_decode && rotation && rot % 16 == 0 && ops::attention_decode_ring_supported(h.dtype, n_heads, n_kv_heads, head_dim, kv.page_size)) {
             // one token per sequence: the attention kernel itself adds up the K slices of the projection,
             // rotates Q and the new K row and writes K and V into the cache
-            MatOrPartials qkv = ops::linear(dev, rt->gemm, h, w_qkv, rt->dtype, true);
+            MatOrPartials qkv = project_qkv(h, ctx, true);
             ops::FusedRope fr{table, rot, n_pos, writes, ctx.err};
             Mat o = ops::attention_decode_ring(dev, qkv, kv, ctx, g, scale, ctx.max_seq_len, 0, &fr);
-            return ops::linear(dev, rt->gemm, o, w_o, rt->dtype, may_defer);
+            return project_o(o, ctx, may_defer);
         }
         // the packed projection may stay in K slices if the position encoding's kernel adds them up
-        MatOrPartials qkv = ops::linear(dev, rt->gemm, h, w_qkv, rt->dtype, position->takes_partials());
+        MatOrPartials qkv = project_qkv(h, ctx, position->takes_partials());
         Mat q = position->encode_and_store(qkv, g, ctx, kv);
         Mat o = ops::attention(dev, q, kv, ctx, g, scale);
-        return ops::linear(dev, rt->gemm, o, w_o, rt->dtype, may_defer);
+        return project_o(o, ctx, may_defer);
+    }
+
+    // The plain layer's projections, with the low-rank adapters of the step's sequences beside them.
+    AdaptedProjection ad_qkv, ad_o;
+    MatOrPartials project_qkv(const Mat& h, const StepContext& ctx, bool may_defer) {
+        if (!ctx.adapted || ad_qkv.empty()) return ops::linear(*rt->dev, rt->gemm, h, w_qkv, rt->dtype, may_defer);
+        MatOrPartials r;
+        r.m = ops::linear_adapters(*rt->dev, h, w_qkv, ad_qkv.set(), ad_qkv.view(ctx), rt->dtype);
+        return r;
+    }
+    MatOrPartials project_o(const Mat& o, const StepContext& ctx, bool may_defer) {
+        if (!ctx.adapted || ad_o.empty()) return ops::linear(*rt->dev, rt->gemm, o, w_o, rt->dtype, may_defer);
+        MatOrPartials r;
+        r.m = ops::linear_adapters(*rt->dev, o, w_o, ad_o.set(), ad_o.view(ctx), rt->dtype);
+        return r;
+    }
+    std::vector<std::string> adapted() const override {
+        if (values_are_keys || general()) return {};
+        return {names.at("q"), names.at("k"), names.at("v"), names.at("o")};
+    }
+    void make_adapters(int count, int rank) override {
+        if (adapted().empty()) return;
+        const long long q = (long long)n_heads * head_dim, kv = (long long)n_kv_heads * head_dim;
+        ad_qkv = AdaptedProjection(rt, "an attention layer's q, k and v", hidden,
+                                   {{names.at("q"), q, 0, 1}, {names.at("k"), kv, q, 1}, {names.at("v"), kv, q + kv, 1}}, count, rank);
+        ad_o = AdaptedProjection(rt, "an attention layer's output", q, {{names.at("o"), hidden, 0, 1}}, count, rank);
+    }
+    void put_adapter(int i, const AdapterFactors& f) override {
+        if (!ad_qkv.empty()) ad_qkv.put(i, f);
+        if (!ad_o.empty()) ad_o.put(i, f);
     }
 };
 
@@ -833,8 +865,25 @@ struct GatedMLP : FeedForward {
         w_down = Mat{down_buf.get(), hidden, inter, rt->dtype, hidden};
         src.fetch_into(n_down, w_down.p, rt->dtype);
     }
-    MatOrPartials forward(const Mat& h, const StepContext&, bool may_defer) override {
+    // low-rank adapters beside gate and up (whose rows take turns) and beside down
+    AdaptedProjection ad_gate_up, ad_down;
+    std::vector<std::string> adapted() const override { return {n_gate, n_up, n_down}; }
+    void make_adapters(int count, int rank) override {
+        ad_gate_up = AdaptedProjection(rt, "a feed-forward layer's gate and up", hidden, {{n_gate, inter, 0, 2}, {n_up, inter, 1, 2}}, count, rank);
+        ad_down = AdaptedProjection(rt, "a feed-forward layer's down", inter, {{n_down, hidden, 0, 1}}, count, rank);
+    }
+    void put_adapter(int i, const AdapterFactors& f) override {
+        ad_gate_up.put(i, f);
+        ad_down.put(i, f);
+    }
+    MatOrPartials forward(const Mat& h, const StepContext& ctx, bool may_defer) override {
         Device& dev = *rt->dev;
+        if (ctx.adapted && !ad_gate_up.empty()) {
+            MatOrPartials r;
+            r.m = ops::linear_adapters(dev, ops::linear_gated_adapters(dev, h, w_gate_up, ad_gate_up.set(), ad_gate_up.view(ctx), act, act_limit), w_down,
+                                       ad_down.set(), ad_down.view(ctx), out_f32 ? DType::F32 : rt->dtype);
+            return r;
+        }
         return ops::linear(dev, rt->gemm, ops::linear_gated(dev, rt->gemm, h, w_gate_up, act, act_limit), w_down, out_f32 ? DType::F32 : rt->dtype,
                            may_defer);
     }

@@ -96,6 +96,15 @@ struct OwnedMat {
 };
 OwnedMat fetch_owned(Runtime* rt, TensorSource& src, const std::string& name, DType want, const char* what);
 
+// One request kind's low-rank adapter: factors by the names of the tensors that they stand beside, on the host in float32,
+// a [r, in] and b [out, r]; y += scale * (x . a^T) . b^T.
+struct AdapterFactors {
+    struct One { const float *a, *b; int r; long long n_in, n_out; };
+    std::map<std::string, One> of;
+    float scale = 1.f;
+    int rank = 0;               // the largest r of the whole adapter
+};
+
 class Part {
 public:
     Part(PartSpec s, Runtime* runtime) : spec(std::move(s)), rt(runtime) {}
@@ -103,6 +112,11 @@ public:
     virtual TensorDecls tensors() const { return {}; }
     // Receive the declared tensors and bring them into the form the kernels want.
     virtual void load(TensorSource&) {}
+    // The declared tensors beside which this part runs low-rank adapters ([out, in] matrices), room for `count` of them of
+    // rank up to `rank`, and adapter i's factors (names among adapted(); what is not named adds nothing).
+    virtual std::vector<std::string> adapted() const { return {}; }
+    virtual void make_adapters(int count, int rank) {}
+    virtual void put_adapter(int i, const AdapterFactors& f) {}
     PartSpec spec;
     Runtime* rt;      // nullptr: the part only declares its tensors (checking a folder, writing a random one)
 };

@@ -18,6 +18,7 @@ class SamplingParams:
     repeat_penalty: float = 1.0   # 1 = off
     repeat_last_n: int = 64
     seed: int = 0
+    min_p: float = 0.0            # 0 = off: words less than min_p times as likely as the likeliest are left out
 
     def validate(self):
         _b.check(_b.lib().illm_sampling_params_validate(json.dumps(asdict(self)).encode()))
@@ -34,14 +35,17 @@ def uniform_for(seed: int, request: int, step: int) -> float:
 
 class Sampler:
     """Chooses one token per row of float32 logits on the device (a torch tensor [B, V]); returns an
-    int32 torch tensor [B].  See `sampling/sampler.h` for `histories`."""
+    int32 torch tensor [B].  `params`: the settings of all requests, or a list with one per request number.
+    See `sampling/sampler.h` for `histories`."""
 
-    def __init__(self, engine, params: SamplingParams):
-        params.validate()
+    def __init__(self, engine, params):
+        each = isinstance(params, (list, tuple))
+        for p in params if each else [params]:
+            p.validate()
         self.params = params
         self._engine = engine
         out = ctypes.c_void_p()
-        _b.check(_b.lib().illm_sampler_create(engine._ptr, json.dumps(asdict(params)).encode(), ctypes.byref(out)))
+        _b.check(_b.lib().illm_sampler_create(engine._ptr, json.dumps([asdict(p) for p in params] if each else asdict(params)).encode(), ctypes.byref(out)))
         self._ptr = out
         engine._adopt(self)
 

@@ -1,6 +1,7 @@
 #include "sampling/sampler.h"
 
 #include <algorithm>
+#include <cstring>
 
 #include "csrc/kernels.h"
 
@@ -9,6 +10,7 @@ namespace illm {
 void SamplingParams::validate() const {
     if (temp < 0) throw ValueError("temp must be >= 0");
     if (!(top_p > 0 && top_p <= 1)) throw ValueError("top_p must be in (0, 1]");
+    if (!(min_p >= 0 && min_p <= 1)) throw ValueError("min_p must be in [0, 1]");
     if (!(repeat_penalty > 0)) throw ValueError("repeat_penalty must be > 0");
     if (top_k < 0 || repeat_last_n < 0) throw ValueError("top_k and repeat_last_n must be >= 0");
 }
@@ -27,6 +29,54 @@ float uniform_for(long long seed, long long request, long long step) {
 }
 
 Sampler::Sampler(Device* dev, const SamplingParams& params) : dev_(dev), params_(params) { params.validate(); }
+
+Sampler::Sampler(Device* dev, const std::vector<SamplingParams>& per_request) : dev_(dev), each_(per_request) {
+    if (each_.empty()) throw ValueError("a sampler needs settings for at least one request");
+    for (const SamplingParams& p : each_) {
+        p.validate();
+        if (p.repeat_penalty == 1.0f || p.repeat_last_n == 0) continue;
+        if (params_.repeat_penalty != 1.0f && params_.repeat_last_n != p.repeat_last_n)
+            throw ValueError("requests of one batch that penalise repetitions need the same repeat_last_n");
+        params_.repeat_penalty = p.repeat_penalty;      // (that some request does)
+        params_.repeat_last_n = p.repeat_last_n;
+    }
+}
+
+const SamplingParams& Sampler::params_of(int request) const {
+    if (each_.empty()) return params_;
+    if (request < 0 || request >= (int)each_.size())
+        throw ValueError("the sampler has settings for " + std::to_string(each_.size()) + " requests, not for number " + std::to_string(request));
+    return each_[(size_t)request];
+}
+
+// Rows with settings of their own.  last: int32 [rows, params_.repeat_last_n] on the device, or nullptr.
+void Sampler::choose_rows(const LogitsRef& logits, const std::vector<int>& requests, const std::vector<int>& steps, const int* last, int* out) {
+    const size_t B = requests.size();
+    std::vector<float> host(6 * B);                     // uniform numbers, temp, top_k (an int), top_p, min_p, penalties
+    bool penalised = false;
+    for (size_t i = 0; i < B; i++) {
+        const SamplingParams& p = params_of(requests[i]);
+        const int k = p.top_k;
+        host[i] = uniform_for(p.seed, requests[i], steps[i]);
+        host[B + i] = p.temp;
+        memcpy(&host[2 * B + i], &k, sizeof k);
+        host[3 * B + i] = p.top_p;
+        host[4 * B + i] = p.min_p;
+        host[5 * B + i] = p.repeat_last_n > 0 ? p.repeat_penalty : 1.0f;
+        penalised = penalised || host[5 * B + i] != 1.0f;
+    }
+    float* dev = dev_->alloc_n<float>(6 * B);
+    dev_->upload_small(dev, host.data(), host.size() * sizeof(float));
+    const float* l = logits.p;
+    if (penalised && last) {
+        // the caller's logits stay as they are
+        float* own = dev_->alloc_n<float>(B * (size_t)logits.vocab);
+        check_cuda(cudaMemcpyAsync(own, l, B * (size_t)logits.vocab * sizeof(float), cudaMemcpyDeviceToDevice, dev_->stream()), "copying the logits");
+        ops::penalise(*dev_, own, (long long)B, logits.vocab, last, params_.repeat_last_n, dev + 5 * B);
+        l = own;
+    }
+    ops::sample_rows(*dev_, l, (long long)B, logits.vocab, dev, dev + B, (const int*)(dev + 2 * B), dev + 3 * B, dev + 4 * B, out);
+}
 
 Sampler::~Sampler() {
     if (window_) dev_->free_persistent(window_);
@@ -58,7 +108,8 @@ TokensRef Sampler::choose(const LogitsRef& logits, const std::vector<int>& reque
     dev_->make_current();
     if ((int)requests.size() != B || (int)steps.size() != B) throw ValueError("the sampler needs a request number and a step per row of logits");
     int* out = out_buffer(B);
-    if (p.greedy() && p.repeat_penalty == 1.0f) {
+    const bool rows_apart = !each_.empty() || p.min_p > 0;
+    if (!rows_apart && p.greedy() && p.repeat_penalty == 1.0f) {
         ops::argmax(*dev_, logits.p, B, logits.vocab, out);
         return TokensRef{out, B};
     }
@@ -114,8 +165,10 @@ TokensRef Sampler::choose(const LogitsRef& logits, const std::vector<int>& reque
             on_device = true;
         }
     }
-    float* u = dev_->alloc_n<float>((size_t)B);
-    if (p.greedy()) {
+    float* u = rows_apart ? nullptr : dev_->alloc_n<float>((size_t)B);
+    if (rows_apart) {
+        choose_rows(logits, requests, steps, last, out);
+    } else if (p.greedy()) {
         // greedy with a repetition penalty: the penalised maximum; top_k = 1 keeps exactly it
         check_cuda(cudaMemsetAsync(u, 0, (size_t)B * sizeof(float), dev_->stream()), "zeroing the uniform numbers");
         ops::sample(*dev_, logits.p, B, logits.vocab, u, 1.0f, 1, 1.0f, p.repeat_penalty, last, n_last, out);

@@ -20,6 +20,7 @@ struct SamplingParams {
     float temp = 0.0f;              // 0 = greedy
     int top_k = 0;                  // 0 = off
     float top_p = 1.0f;             // 1 = off
+    float min_p = 0.0f;             // 0 = off: words less than min_p times as likely as the likeliest are left out
     float repeat_penalty = 1.0f;    // 1 = off
     int repeat_last_n = 64;
     long long seed = 0;
@@ -50,6 +51,10 @@ struct TokensRef {
 class Sampler {
 public:
     Sampler(Device* dev, const SamplingParams& params);
+    // Settings per request number.  Rows then go through csrc/sample_rows.cu in one batch, whatever their settings (as they do with
+    // min_p): equal logits count by their id, and top_k keeps exactly k words.  Requests that penalise repetitions share one
+    // repeat_last_n.
+    Sampler(Device* dev, const std::vector<SamplingParams>& per_request);
     ~Sampler();
     TokensRef choose(const LogitsRef& logits, const std::vector<int>& requests, const std::vector<int>& steps,
                      const std::vector<std::vector<int>>* histories);
@@ -57,10 +62,13 @@ public:
 
 private:
     bool wants_history() const { return params_.repeat_penalty != 1.0f && params_.repeat_last_n > 0; }
+    const SamplingParams& params_of(int request) const;
+    void choose_rows(const LogitsRef& logits, const std::vector<int>& requests, const std::vector<int>& steps, const int* last, int* out);
     int* out_buffer(int n);
     const int* upload_ints(const std::vector<int>& v);
     Device* dev_;
-    SamplingParams params_;
+    SamplingParams params_;                     // of all requests, or what they share
+    std::vector<SamplingParams> each_;          // per request number; empty: all alike
     int* window_ = nullptr;         // int32 [window_rows_, repeat_last_n] on the device
     int window_rows_ = 0, window_cap_ = 0;
     std::map<int, int> row_of_;     // request -> its row of the window
