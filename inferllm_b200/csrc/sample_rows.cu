@@ -518,6 +518,8 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     extern __shared__ __align__(16) unsigned char sr_smem[];
     SrShared& sh = *reinterpret_cast<SrShared*>(sr_smem);
     float* resident = reinterpret_cast<float*>(sr_smem + sizeof(SrShared));
+    // a block's shared memory may be written by the others of its cluster once it runs: they wait for this before the first exchange
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_grid_sync();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned rank = C > 1 ? sr_rank() : 0;
@@ -552,6 +554,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             top = fmaxf(top, f);                        // (the other one of a NaN)
         }
     }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     SrRow r;
     r.max_value = sr_value(k.cluster_max(sr_key(top)));
     if (r.max_value == -INFINITY) {                     // nothing can come: the same in all blocks

@@ -190,6 +190,26 @@ def test_streams_and_graphs(T):
         assert torch.equal(got, ops.linear_adapters(x, w, ad, rows))
 
 
+def test_calls_back_to_back():
+    """Many calls with nothing between them but the kernel that makes their input: what each waits for, it waits for."""
+    cases = []
+    for T, K, N, dtype in ((1, 512, 600, torch.bfloat16), (20, 1024, 520, torch.bfloat16), (100, 512, 384, torch.bfloat16), (200, 2048, 512, torch.bfloat16),
+                           (600, 512, 2304, torch.bfloat16), (2500, 128, 2304, torch.bfloat16), (30, 300, 200, torch.float32)):
+        x, w, a, b, ad, s = make(T, K, N, [16, 40, 8], dtype, T + K)
+        rows = ops.AdapterRows([(t // 3) % 4 - 1 for t in range(T)], ad.ranks)
+        cases.append((x, w, ad, rows, [ops.linear_adapters(x * f, w, ad, rows) for f in (1.0, 2.0)]))
+    torch.cuda.synchronize()
+    got = []
+    for i in range(700):
+        x, w, ad, rows, want = cases[i % 7]
+        f = i // 7 % 2
+        got.append((ops.linear_adapters(x * (1.0 + f), w, ad, rows), want[f]))
+        if i % 140 == 139:
+            torch.cuda.synchronize()
+            assert all(torch.equal(g, v) for g, v in got)
+            got = []
+
+
 def test_refusals():
     x, w, a, b, ad, s = make(4, 64, 32, [8, 8], torch.bfloat16, 1)
     rows = ops.AdapterRows([0, 1, -1, 0], ad.ranks)

@@ -170,6 +170,23 @@ def test_on_another_stream_and_replayed():
         assert got.tolist() == ops.sample_rows(logits, u, temp, k).tolist()
 
 
+def test_passes_back_to_back():
+    """Many calls with nothing between them, so that their blocks start while others still run."""
+    g = torch.Generator("cuda").manual_seed(10)
+    cases = []
+    for B, V in ((1, 32000), (7, 128256), (64, 32000), (200, 4099), (33, 700)):
+        logits, u = torch.randn((B, V), generator=g, device="cuda") * 2, torch.rand(B, generator=g, device="cuda")
+        temp, k = torch.rand(B, generator=g, device="cuda") + 0.2, torch.randint(0, 60, (B,), generator=g, device="cuda").int()
+        p = torch.rand(B, generator=g, device="cuda") * 0.5 + 0.6
+        args = (logits, u, temp, k * (k > 20), p)
+        want = ops.sample_rows(*args)
+        torch.cuda.synchronize()
+        cases.append((args, want))
+    got = [ops.sample_rows(*cases[i % 5][0]) for i in range(2000)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, cases[i % 5][1]) for i, t in enumerate(got))
+
+
 def test_nothing_to_do():
     assert ops.sample_rows(torch.zeros((0, 10), device="cuda"), torch.zeros(0, device="cuda")).shape == (0,)
 
