@@ -5,11 +5,12 @@
 // R the largest rank rounded up to 16, rows beyond an adapter's own rank zero and, where they fill a group, never read.
 // Which token has which adapter comes as a plan (adapters.h).
 //
-// The general form (both types): the shared product by the package's own kernels into float32, then
+// Float32: the package's product, which adds up every output in one chain over K, then
 //   shrink   v[t] = s_a x[t] A_a^T: a block per 4 tokens of the plan's order and rank group, a warp per two ranks, which
 //            reads a row of A once for the tokens of a slot;
-//   expand   y[t, n] = base[t, n] + v[t] . B_a[n]: a thread per output column, the slot's 16 values of B in registers.
-// Sums are float32 in one order per token, whatever else is in the batch.
+//   expand   y[t, n] += v[t] . B_a[n]: a thread per output column, 16 values of B in registers for neighbours with one adapter.
+// A token's sums have one order whatever else is in the batch, and one without an adapter keeps the plain product's bits.
+// Bfloat16: up to 128 tokens below, prompts in adapters_prompt.cu.
 #include "adapters.cuh"
 #include "kernels.h"
 
@@ -105,7 +106,7 @@ adapter_expand_kernel(int N, const float* __restrict__ b, const float* __restric
         if (at[i].w > 0) out[(long long)at[i].x * N + col] = acc[i];
 }
 
-// ---- The rows form (bfloat16, up to 256 tokens): two launches.
+// ---- The rows form (bfloat16, up to 128 tokens): two launches.
 //
 // The first streams W once and, in the same grid, the first factors of the adapters that the tokens name: rank groups are
 // nothing but more rows of the weight.  A block multiplies 128 of those rows (a tile of W, or 8 rank groups fetched by a TMA box
@@ -360,15 +361,14 @@ adapter_join_kernel(const float* __restrict__ base, int splits, long long stride
             if (at[i].x >= 0) AdColumns<VEC>::store(out + (size_t)at[i].x * N + col, acc[i]);
 }
 
-// How the rows form cuts K: as many slices as bring about two blocks to an SM (one beyond 128 tokens, whose stages are larger),
-// each at least 8 pieces of 64 wide, at most 8 slices (their reader pays for every one).
+// How the rows form cuts K: as many slices as bring about two blocks to an SM, each at least 8 pieces of 64 wide, at most 8 slices (their reader pays for every one).
 struct AdRows { int base_tiles, shrink_tiles, k_iters, per, splits; };
 static AdRows ad_rows(int T, int N, int K, int groups) {
     AdRows r;
     r.base_tiles = ad_div(N, TC_BM);
     r.shrink_tiles = ad_div(groups, TC_BM / ADAPTER_GROUP);
     r.k_iters = ad_div(K, TC_BK);
-    int s = (T > 128 ? 1 : 2) * illm_sm_count() / (r.base_tiles + r.shrink_tiles);
+    int s = 2 * illm_sm_count() / (r.base_tiles + r.shrink_tiles);
     s = s > r.k_iters / 8 ? r.k_iters / 8 : s;
     s = s > 8 ? 8 : s;
     s = s < 1 ? 1 : s;
@@ -400,7 +400,7 @@ static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const
                         const AdapterPlanSizes& sz, const int* plan_dev, TOut* out, char* ws, int early, int* err, cudaStream_t s) {
     const AdPlan plan = ad_plan(plan_dev, sz);
     const AdRows r = ad_rows(T, N, K, sz.groups);
-    const int v_ld = sz.groups * ADAPTER_GROUP, bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    const int v_ld = sz.groups * ADAPTER_GROUP, bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     float *vs = (float*)ws, *base = (float*)(ws + ad_round((long long)r.splits * T * v_ld * 4));
     CUtensorMap mw, ma, mx;
     int rc;
@@ -410,8 +410,7 @@ static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const
         case 16: rc = ad_launch_rows<16>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
         case 32: rc = ad_launch_rows<32>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
         case 64: rc = ad_launch_rows<64>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
-        case 128: rc = ad_launch_rows<128>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s); break;
-        default: rc = ad_launch_rows<256>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s);
+        default: rc = ad_launch_rows<128>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s);
     }
     if (rc) return rc;
     auto join = [&](auto kern, int tok, int vec) {
@@ -437,8 +436,15 @@ extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int
 static int ad_float32(const float* x, const float* w, int T, int N, int K, const float* a, const float* b, const float* scales, int R,
                       const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int* err, cudaStream_t s) {
     const AdPlan plan = ad_plan(plan_dev, sz);
-    const int rc = illm_gemm_f32_nt(x, w, out, T, N, K, K, K, N, err, s);
-    if (rc != 0 || sz.slots == 0) return rc;
+    // The product's bits do not depend on how its rows are taken (one chain of additions over K per output).  Nine to sixteen go
+    // by eights through the kernel that streams the weight for up to eight, where its tiles would leave SMs without one: 9 tokens of
+    // 11008 x 4096 take 179 us instead of 501, 16 of 5120 x 5120 125 instead of 222; of 4096 x 22016, which fill them, 296 and 251.
+    const int by = T > 8 && T <= 16 && N < 64 * illm_sm_count() ? 8 : T;
+    for (int t = 0; t < T; t += by) {
+        const int rc = illm_gemm_f32_nt(x + (size_t)t * K, w, out + (size_t)t * N, T - t < by ? T - t : by, N, K, K, K, N, err, s);
+        if (rc != 0) return rc;
+    }
+    if (sz.slots == 0) return 0;
     const bool wide = K % 4 == 0 && !(((uintptr_t)x | (uintptr_t)a) & 15);
     auto shrink = wide ? adapter_shrink_kernel<4> : adapter_shrink_kernel<1>;
     illm_launch(shrink, dim3(ad_div(T, AD_SHRINK), R / ADAPTER_GROUP), dim3(256), 0, s, x, K, a, scales, R, plan.places, T, v);

@@ -24,6 +24,7 @@
 #define AP_COLS (ADAPTER_CHUNK * ADAPTER_GROUP)        // columns of a chunk
 #define AP_PITCH (AP_COLS + 4)      // floats: rows start on 16 bytes, and 8 neighbouring ones in different banks
 #define AP_STAGES 6
+#define AP_OUT_PITCH 33
 #define AP_BN 256
 #define AP_HALF 128
 
@@ -205,6 +206,7 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const unsigned full0 = bars, empty0 = bars + 8 * STAGES;
     const unsigned acc_full0 = bars + 16 * STAGES, acc_empty0 = acc_full0 + 16;
     unsigned* tmem_holder = reinterpret_cast<unsigned*>(smem_raw + (bars - base) + 16 * STAGES + 32);
+    float* stage_out = reinterpret_cast<float*>(smem_raw + (bars - base) + 16 * STAGES + 48);       // [4][32][AP_OUT_PITCH], only for odd N
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_ctarank();
@@ -345,21 +347,40 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             if (!alive) break;
             tc_fence_after();
             const unsigned tbase = tmem + ((unsigned)(quad * 32) << 16) + (unsigned)(buf * AP_BN);
+            if ((N & 7) == 0) {
 #pragma unroll 1
-            for (int c = 0; c < AP_BN; c += 16) {
-                if (rb0 + c >= N) break;
-                float v[16];
-                tmem_ld16(tbase + c, v);
-                if (ra < T) {
-                    TOut* dst = Cz + (size_t)ra * N + rb0 + c;
-                    if (rb0 + c + 16 <= N && ((N & 7) == 0)) {
+                for (int c = 0; c < AP_BN; c += 16) {
+                    if (rb0 + c >= N) break;
+                    float v[16];
+                    tmem_ld16(tbase + c, v);
+                    if (ra < T) {
+                        TOut* dst = Cz + (size_t)ra * N + rb0 + c;
                         store8(dst, v);
-                        store8(dst + 8, v + 8);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            if (rb0 + c + j < N) store_out<TOut>(dst + j, v[j]);
+                        if (rb0 + c + 8 < N) store8(dst + 8, v + 8);
                     }
+                }
+            } else {
+                // rows that start anywhere: 32 of them by 32 columns through shared memory, so that a warp stores a row's neighbours
+                // together (element by element, a row to a thread, 260 tokens of 2048 x 32001 took 205 us)
+                float* mine = stage_out + (warp - 2) * 32 * AP_OUT_PITCH;
+                const int rows = min(32, T - (ra - lane));
+#pragma unroll 1
+                for (int c = 0; c < AP_BN; c += 32) {
+                    if (rb0 + c >= N) break;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float v[16];
+                        tmem_ld16(tbase + c + 16 * h, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) mine[lane * AP_OUT_PITCH + 16 * h + j] = v[j];
+                    }
+                    __syncwarp();
+                    if (rb0 + c + lane < N) {
+                        TOut* dst = Cz + (size_t)(ra - lane) * N + rb0 + c + lane;
+#pragma unroll 4
+                        for (int q = 0; q < rows; q++) store_out<TOut>(dst + (size_t)q * N, mine[q * AP_OUT_PITCH + lane]);
+                    }
+                    __syncwarp();
                 }
             }
             tc_fence_before();
@@ -408,7 +429,7 @@ long long ad_prompt_ws(int T, int N, int K, int chunks) {
 template <typename TOut>
 static int ap_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mv, const CUtensorMap& mb, TOut* out, int T, int N, int R, int k_iters,
                           int splits, const AdPlan& plan, int chunked, int* err, cudaStream_t s) {
-    const size_t smem = (size_t)AP_STAGES * (TC_BM + AP_HALF) * TC_BK * 2 + 16 * AP_STAGES + 32 + 16;
+    const size_t smem = (size_t)AP_STAGES * (TC_BM + AP_HALF) * TC_BK * 2 + 16 * AP_STAGES + 32 + 16 + ((N & 7) ? 4 * 32 * AP_OUT_PITCH * 4 : 0);
     auto kern = adapter_pair_kernel<TOut>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
