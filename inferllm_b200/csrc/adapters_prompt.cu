@@ -452,9 +452,18 @@ int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void
             (rc = ad_make_map(&mv, v, (long long)chunks * ADAPTER_TILE, AP_COLS, TC_BM)) ||
             (rc = ad_make_map(&mb, b, (long long)count * (R / ADAPTER_GROUP) * N, ADAPTER_GROUP, AP_HALF, ADAPTER_GROUP, CU_TENSOR_MAP_SWIZZLE_32B)))
             return rc;
-        // as many blocks share a chunk's K as bring about two blocks to an SM
-        int C = 1;
-        while (C < 8 && chunks * 2 * C * 2 <= 2 * illm_sm_count() && k_iters >= 4 * C) C *= 2;
+        // Blocks that share a chunk's K: the product's pairs of SMs start at once where this kernel leaves SMs free, and those that start
+        // behind it should be the ones that the last round of tiles would leave idle (2,048 tokens of 4096 x 4096: 57 us, 67 with
+        // blocks everywhere), as long as a block's share of K is no longer than a tile's; else about two blocks to an SM.
+        const int most_pairs = illm_sm_count() / 2, items = ad_div(T, 256) * ad_div(N, AP_BN) * splits;
+        const int idle = 2 * (items <= most_pairs ? most_pairs - items : (most_pairs - items % most_pairs) % most_pairs);
+        auto share = [&](int room) {
+            int c = 1;
+            while (c < 8 && chunks * 2 * c * 2 <= room && k_iters >= 4 * c) c *= 2;
+            return c;
+        };
+        int C = share(idle);
+        if (chunks * 2 * C > idle || ad_div(k_iters, C) > ad_div(k_iters, splits)) C = share(2 * illm_sm_count());
         // the ring holds a block's whole share of K where one block has an SM to itself
         const int per = ad_div(k_iters, C), most = chunks * 2 * C > illm_sm_count() ? 4 : AP_VALUE_STAGES, stages = per < 2 ? 2 : per < most ? per : most;
         const size_t smem = (size_t)stages * (TC_BM + AP_COLS) * TC_BK * 2 + 1024;
