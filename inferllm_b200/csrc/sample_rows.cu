@@ -447,24 +447,30 @@ __device__ __noinline__ SrList sr_list(SrShared& sh, int words) {
     const unsigned least = ~sr_block_max(sh, low);
     return SrList{least, 64 - __clzll(((u64)(most - least) << SR_LIST_BITS) | (SR_LIST - 1))};
 }
-// The order of the last word of the shortest prefix, largest order first, whose count, or weight, reaches `target`, which that of
-// the words with an order of at least `from` does.  By digits of 8 bits, until one holds at most 32 words, which every warp
-// ranks by itself.
-__device__ __noinline__ u64 sr_list_cut(SrShared& sh, SrRow r, SrList w, int words, u64 from, bool weights, u64 target) {
+// The order of the last word of the shortest prefix, largest order first, whose count, or weight, reaches `target`, among the words
+// with an order of at least `from` at distances of at least `edge`; they are at most `few` and reach it.  By digits of 8 bits,
+// until one holds at most 32 words, which every warp ranks by itself: a top_k's words in question are the last bin's, mostly so
+// few that no digit is taken (1 to 2 us less than over the whole list, for rows with a top_k of 1000 in clusters).
+__device__ __noinline__ u64 sr_list_cut(SrShared& sh, SrRow r, SrList w, int words, u64 from, float edge, int few, bool weights, u64 target) {
     const int tid = threadIdx.x, lane = tid & 31;
     u64 prefix = 0, above = 0;
     int shift = w.bits;
+    // whether word i is still in question, and its order
+    auto open = [&](int i, u64& o) {
+        o = sr_order(sh, w, i);
+        return o >= from && o >> shift == prefix && sr_distance(r.max_value, sh.value[i]) >= edge;
+    };
+    if (tid == 0) sh.n_few = 0;
 #pragma unroll 1
-    for (int turn = 0;; turn ^= 1) {
+    for (int turn = 0; few > 32; turn ^= 1) {
         unsigned *count = sh.digits[turn].count, *lo = sh.digits[turn].lo, *hi = sh.digits[turn].hi;
         if (tid < 256) count[tid] = lo[tid] = hi[tid] = 0u;
-        if (tid == 0) sh.n_few = 0;
         __syncthreads();
         const int down = shift > 8 ? shift - 8 : 0, width = shift - down;
 #pragma unroll 1
         for (int i = tid; i < words; i += SR_THREADS) {
-            const u64 o = sr_order(sh, w, i);
-            if (o < from || o >> shift != prefix) continue;
+            u64 o;
+            if (!open(i, o)) continue;
             const u64 m = sr_measure(r, sh.table, sh.value[i], weights);
             const int d = (int)(o >> down) & ((1 << width) - 1);
             const unsigned low = (unsigned)m, carry = atomicAdd(&lo[d], low) > ~low ? 1u : 0u;
@@ -489,25 +495,27 @@ __device__ __noinline__ u64 sr_list_cut(SrShared& sh, SrRow r, SrList w, int wor
         above = __shfl_sync(0xffffffffu, before, owner);
         prefix = (prefix << width) | (unsigned)digit;
         shift = down;
-        const int few = (int)count[digit];
-        if (few <= 32) {
-#pragma unroll 1
-            for (int i = tid; i < words; i += SR_THREADS) {
-                const u64 o = sr_order(sh, w, i);
-                if (o < from || o >> shift != prefix) continue;
-                const unsigned to = atomicAdd(&sh.n_few, 1u);
-                sh.few_order[to] = o;
-                sh.few_weight[to] = sr_measure(r, sh.table, sh.value[i], weights);
-            }
-            __syncthreads();
-            const u64 o = lane < few ? sh.few_order[lane] : 0ull, m = lane < few ? sh.few_weight[lane] : 0ull;
-            u64 sum = above;
-#pragma unroll 1
-            for (int q = 0; q < few; q++) sum += sh.few_order[q] > o ? sh.few_weight[q] : 0ull;
-            const int last = __ffs(__ballot_sync(0xffffffffu, lane < few && sum < target && sum + m >= target)) - 1;
-            return __shfl_sync(0xffffffffu, o, last);
-        }
+        few = (int)count[digit];
     }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < words; i += SR_THREADS) {
+        u64 o;
+        if (!open(i, o)) continue;
+        const unsigned to = atomicAdd(&sh.n_few, 1u);
+        sh.few_order[to] = o;
+        sh.few_weight[to] = sr_measure(r, sh.table, sh.value[i], weights);
+    }
+    __syncthreads();
+    few = (int)sh.n_few;
+    const u64 o = lane < few ? sh.few_order[lane] : 0ull, m = lane < few ? sh.few_weight[lane] : 0ull;
+    u64 sum = above;
+#pragma unroll 1
+    for (int q = 0; q < few; q++) sum += sh.few_order[q] > o ? sh.few_weight[q] : 0ull;
+    const int last = __ffs(__ballot_sync(0xffffffffu, lane < few && sum < target && sum + m >= target)) - 1;
+    const u64 result = __shfl_sync(0xffffffffu, o, last);
+    __syncthreads();                                    // (the next call begins with the counter)
+    return result;
 }
 
 template <typename TIn>
@@ -587,7 +595,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
     auto cut_in_list = [&](int words, bool weights, u64 target) {
         if (rank == 0) {
             const SrList w = sr_list(sh, words);
-            const int i = SR_LIST - 1 - (int)(sr_list_cut(sh, r, w, words, 0ull, weights, target) & (SR_LIST - 1));
+            const int i = SR_LIST - 1 - (int)(sr_list_cut(sh, r, w, words, 0ull, 0.f, words, weights, target) & (SR_LIST - 1));
             if (tid < C) sr_store_remote(&sh.found, tid, ((u64)__float_as_uint(sh.value[i]) << 32) | (unsigned)sh.id[i]);
         }
         sr_cluster_sync();
@@ -633,7 +641,8 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
                 if (ahead_of <= t && ahead_of + m > t) out[at_row] = sh.id[tid];
                 return;
             }
-            u64 last = sr_list_cut(sh, r, w, words, 0ull, false, (u64)top_k);
+            // (only the bin's words are in question: mostly few)
+            u64 last = sr_list_cut(sh, r, w, words, 0ull, sr_edge(bin), (int)inside, false, (u64)top_k - (u64)before);
             auto sum = [&] {
                 u64 mine = 0;
 #pragma unroll 1
@@ -644,7 +653,7 @@ sample_rows_kernel(const TIn* __restrict__ logits, long long ld, int V, int chun
             const double min_p_given = r.min_p;
             if (top_p < 1.0f) {
                 r.min_p = 0.0;                          // (it does not count for top_p's share)
-                last = sr_list_cut(sh, r, w, words, last, true, sr_top_p_target(top_p, sum()));
+                last = sr_list_cut(sh, r, w, words, last, 0.f, words, true, sr_top_p_target(top_p, sum()));
                 r.min_p = min_p_given;
             }
             const u64 t = sr_draw_target(u, sum());
