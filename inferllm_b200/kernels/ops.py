@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 
 import torch
 
@@ -811,10 +810,13 @@ class Adapters:
         self.ranks = [0] * count
         self.changes = 0        # how often a rank has changed
         self.pointers = self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr()
+        _error_word(self.device)    # (made here: a call that is captured first of all could not)
 
     def put(self, i, a, b, scale=1.0):
         """Adapter i becomes scale * b a (a [r, n_in], b [n_out, r], any float type); what it was is gone.  Works on torch's
-        current stream, like any torch operation, and looks at the numbers, which have to be finite in the adapters' type.  A plan made before an adapter got a larger rank is refused."""
+        current stream, like any torch operation, and looks at the numbers, which have to be finite in the adapters' type.  A plan
+        made before an adapter got a larger rank is refused; a captured call keeps the plan, and with it the ranks, that it was
+        captured with."""
         if not 0 <= i < self.count:
             raise KernelError(f"adapters: there is no adapter {i} among {self.count}")
         if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.n_in or b.shape[0] != self.n_out or a.shape[0] != b.shape[1]:
@@ -824,9 +826,11 @@ class Adapters:
             raise KernelError(f"adapters: rank {r} exceeds the {self.rank} there is room for")
         if not (a.is_floating_point() and b.is_floating_point()):
             raise KernelError("adapters: the factors must be floating-point tensors")
-        a, b, scale = a.to(self.device, self.dtype), b.to(self.device, self.dtype), float(scale)
+        # (copies: they may be parameters, or the place's own factors)
+        a, b = (f.detach().to(self.device, self.dtype, copy=True) for f in (a, b))
+        scale = float(scale)
         # (the prompt product multiplies an adapter's b with the zeros of its neighbours' tokens)
-        if not (math.isfinite(scale) and bool(a.isfinite().all()) and bool(b.isfinite().all())):
+        if not (abs(scale) <= torch.finfo(torch.float32).max and bool(a.isfinite().all()) and bool(b.isfinite().all())):
             raise KernelError(f"adapters: adapter {i} is not finite in {self.dtype}")
         self.a[i].zero_()
         self.a[i, :r] = a

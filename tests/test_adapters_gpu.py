@@ -6,6 +6,10 @@ sum |v| |B| for the adapter, so (K + R) 2^-24 times their sum bounds the error. 
 2^-8 of its value; on the prompt path the intermediate values v are rounded as well, which is at most 2^-8 sum |v| |B|.  In the
 root-mean-square a rounding to bfloat16 is off by 2^-8 / sqrt(3) times the mean square of where a value lies within its power
 of two, 0.0017 of the values; the two of them by 0.0024 of the results, and 2^-8 = 0.0039 is the bound."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -231,3 +235,66 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ops.KernelError):
             call()
+
+
+def test_put_takes_parameters_and_its_own_factors():
+    x, w, a, b, ad, s = make(6, 64, 48, [16, 8], torch.bfloat16, 3)
+    rows = ops.AdapterRows([0, 1, -1, 0, 1, 1], ad.ranks)
+    want = ops.linear_adapters(x, w, ad, rows)
+    ad.put(0, torch.nn.Parameter(a[0].clone()), torch.nn.Parameter(b[0].clone()), s[0])
+    assert not (ad.a.requires_grad or ad.b.requires_grad)
+    assert torch.equal(ops.linear_adapters(x, w, ad, rows), want)
+    ad.put(0, ad.a[0], ad.b[0, 0], s[0])
+    ad.put(1, ad.a[1, :8], ad.b[1, 0, :, :8], s[1])
+    assert torch.equal(ops.linear_adapters(x, w, ad, rows), want)
+    with pytest.raises(ops.KernelError, match="not finite"):
+        ad.put(0, a[0], b[0], 1e39)                     # (no float32)
+    assert torch.equal(ops.linear_adapters(x, w, ad, rows), want)
+
+
+@pytest.mark.parametrize("T", [7, 100, 400])
+def test_two_streams_at_once(T):
+    x, w, a, b, ad, s = make(T, 512, 1000, [16, 40, 8], torch.bfloat16, T)
+    rows = ops.AdapterRows([t % 4 - 1 for t in range(T)], ad.ranks)
+    xs = [x, x * 2.0, x * -1.0]
+    want = [ops.linear_adapters(v, w, ad, rows) for v in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+    for i in range(40):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[j].append(ops.linear_adapters(xs[j], w, ad, rows))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[j]) for j in range(3) for g in got[j])
+
+
+@pytest.mark.parametrize("dtype,N", [(torch.bfloat16, 16400), (torch.bfloat16, 16401), (torch.float32, 16400)])
+def test_more_results_than_32_bits_count(dtype, N):
+    T, K = 140000, 32
+    x, w, a, b, ad, s = make(T, K, N, [8, 24], dtype, N)
+    index = [(t // 1000) % 3 - 1 for t in range(T)]
+    out = ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks))
+    for t in (0, 2 ** 31 // N - 100, T - 200):
+        check(out[t:t + 200], x[t:t + 200], w, a, b, s, index[t:t + 200])
+
+
+def test_captured_first_of_all():
+    """A process whose first call is a captured one."""
+    code = """
+import torch
+from inferllm_b200.kernels import ops
+x, w = torch.randn(5, 64, device="cuda").bfloat16(), torch.randn(40, 64, device="cuda").bfloat16()
+ad = ops.Adapters(1, 8, 40, 64)
+ad.put(0, torch.randn(8, 64), torch.randn(40, 8))
+rows = ops.AdapterRows([0, -1, 0, 0, -1], ad.ranks)
+u = torch.rand(5, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.linear_adapters(x, w, ad, rows, torch.float32)
+    ids = ops.sample_rows(y, u)
+g.replay()
+assert torch.equal(y, ops.linear_adapters(x, w, ad, rows, torch.float32)) and torch.equal(ids, ops.sample_rows(y, u))
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr

@@ -201,3 +201,33 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ops.KernelError):
             call()
+
+
+def test_more_words_than_32_bits_count():
+    B, V = 17000, 128256
+    g = torch.Generator("cuda").manual_seed(9)
+    logits = torch.empty((B, V), dtype=torch.bfloat16, device="cuda")
+    for r in range(0, B, 1000):
+        logits[r:r + 1000] = torch.randn((min(1000, B - r), V), generator=g, device="cuda")
+    u, temp = torch.rand(B, generator=g, device="cuda"), torch.full((B,), 0.7, device="cuda")
+    top_k = (torch.arange(B, device="cuda") % 3 * 40).int()
+    got = ops.sample_rows(logits, u, temp, top_k)
+    for r in (0, 2 ** 31 // V - 30, B - 60):
+        e = slice(r, r + 60)
+        assert torch.equal(got[e], ops.sample_rows(logits[e], u[e].contiguous(), temp[e].contiguous(), top_k[e].contiguous()))
+
+
+def test_streams_at_once():
+    g = torch.Generator("cuda").manual_seed(10)
+    logits = torch.randn((24, 40000), generator=g, device="cuda") * 3
+    u = torch.rand(24, generator=g, device="cuda")
+    top_p = torch.full((24,), 0.9, device="cuda")
+    want = ops.sample_rows(logits, u, None, None, top_p)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(ops.sample_rows(logits, u, None, None, top_p))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want) for v in got)
