@@ -459,7 +459,7 @@ extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int
                                     int* err, void* stream) {
     if (T <= 0 || N <= 0) return 0;
     if (K <= 0 || count <= 0 || R <= 0 || R % ADAPTER_GROUP || R > ADAPTER_GROUP * ADAPTER_MAX_GROUPS || slots < 0 || groups < 0 || chunks < 0 || !ws || !plan ||
-        T > 65535 * AD_SHRINK || (long long)count * R * (N / ADAPTER_GROUP + 1) >= (1ll << 31) || (long long)count * R >= (1ll << 31))
+        T > 65535 * AD_TOKENS || (long long)count * R * (N / ADAPTER_GROUP + 1) >= (1ll << 31) || (long long)count * R >= (1ll << 31))
         return ILLM_ERR_BAD_ARG;        // (rows of the factors are counted in 32 bits)
     if (dtype == ILLM_BF16 && ((K & 7) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)a & 15) || ((uintptr_t)b & 15))) return ILLM_ERR_BAD_ARG;
     const AdapterPlanSizes sz{T, slots, groups, chunks};

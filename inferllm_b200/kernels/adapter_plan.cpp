@@ -20,7 +20,7 @@ static std::vector<int> named(const int* index, int from, int to) {
 static int tile_end(int t0, int T) { return std::min(T, t0 + ADAPTER_TILE); }
 
 AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, int count) {
-    if (T < 0 || T > (1 << 19)) throw KernelError("adapters: a step of " + std::to_string(T) + " tokens is outside [0, 524288]");
+    if (T < 0 || T > 524280) throw KernelError("adapters: a step of " + std::to_string(T) + " tokens is outside [0, 524280]");
     for (int a = 0; a < count; a++)
         if (ranks[a] < 0 || ranks[a] > ADAPTER_GROUP * ADAPTER_MAX_GROUPS)
             throw KernelError("adapters: adapter " + std::to_string(a) + " has rank " + std::to_string(ranks[a]) + ", outside [0, 256]");

@@ -65,3 +65,11 @@ def test_refusals():
     for index, ranks in (([0], []), ([2], [8, 8]), ([-2], [8]), ([0], [257]), ([0], [-1])):
         with pytest.raises(KernelError):
             plan(index, ranks)
+
+
+def test_the_longest_step():
+    index = np.full(524280, -1, dtype=np.int32)
+    index[-1] = 0
+    assert plan(index, [5])[0][0] == 524280
+    with pytest.raises(Exception, match="524281"):
+        plan(np.full(524281, -1, dtype=np.int32), [5])
