@@ -231,3 +231,18 @@ def test_streams_at_once():
             got.append(ops.sample_rows(logits, u, None, None, top_p))
     torch.cuda.synchronize()
     assert all(torch.equal(v, want) for v in got)
+
+
+@pytest.mark.parametrize("B,V", [(512, 3000), (300, 9000), (513, 3000), (64, 128256)])
+def test_more_blocks_than_run_at_once(B, V):
+    """Where rows of much work come first, every row still comes, and once: each is what it is in a small batch."""
+    g = torch.Generator("cuda").manual_seed(B)
+    logits = torch.randn((B, V), generator=g, device="cuda") * 3
+    u = torch.rand(B, generator=g, device="cuda")
+    kind = torch.randint(0, 5, (B,), generator=g, device="cuda")
+    temp = torch.where(kind == 0, 0.0, 0.9)
+    top_k = torch.where(kind == 1, 40, torch.where(kind == 2, 700, 0)).int()
+    top_p = torch.where((kind == 3) | (kind == 1), 0.8, 1.0)
+    out = ops.sample_rows(logits, u, temp, top_k, top_p)
+    want = torch.cat([ops.sample_rows(*[v[r:r + 16].contiguous() for v in (logits, u, temp, top_k, top_p)]) for r in range(0, B, 16)])
+    assert torch.equal(out, want)
