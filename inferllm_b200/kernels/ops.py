@@ -865,8 +865,15 @@ class AdapterRows:
         self.slots, self.groups, self.chunks = sizes[1], sizes[2], sizes[3]
         self.plan = host.to(self.device)
         self.plan_ptr = self.plan.data_ptr()
-        self._fitted = None
+        self._fitted, self._ws = None, {}
         self.most_groups = max((-(-self.ranks[a] // ADAPTER_GROUP) for a in self.named), default=0)
+
+    def ws_bytes(self, code, N, K, R):
+        """The workspace of a product by this plan."""
+        n = self._ws.get((code, N, K, R))
+        if n is None:
+            n = self._ws[code, N, K, R] = load().illm_linear_adapters_ws(code, self.T, N, K, R, self.groups, self.chunks)
+        return n
 
     def fits(self, adapters):
         """Whether the plan covers these adapters' ranks."""
@@ -904,7 +911,7 @@ def linear_adapters(x, w, adapters, rows, out_dtype=None):
     if T == 0:
         return out
     lib, code = load(), _DT[dtype]
-    ws = torch.empty((lib.illm_linear_adapters_ws(code, T, N, K, adapters.R, rows.groups, rows.chunks),), dtype=torch.uint8, device=device)
+    ws = torch.empty((rows.ws_bytes(code, N, K, adapters.R),), dtype=torch.uint8, device=device)
     a, b, scales = adapters.pointers
     with _on(device):
         _check(lib.illm_linear_adapters(px, pw, code, T, N, K, a, b, scales, adapters.count, adapters.R, rows.plan_ptr, rows.slots, rows.groups, rows.chunks,
