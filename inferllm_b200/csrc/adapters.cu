@@ -160,63 +160,68 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     tc_fence_after();
     const unsigned tmem = tmem_holder;
 
+    // (the two warps stay together around what one lane issues: what every lane agrees on then lies in uniform registers)
     if (warp == 0) {
-        if (lane == 0) {
-            // the join reads second factors before its wait: not before this kernel's own wait, unless no kernel before made them
-            if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            int group_row[TC_BM / ADAPTER_GROUP];
+        const bool elected = elect_one();
+        // the join reads second factors before its wait: not before this kernel's own wait, unless no kernel before made them
+        if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        int group_row[TC_BM / ADAPTER_GROUP];
 #pragma unroll
-            for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++) {
-                const int g = j < boxes ? plan.groups[g0 + j] : 0;
-                group_row[j] = (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
-            }
-            auto arm_and_load_weights = [&](int i, int s) {
-                mbar_expect_tx(full0 + 8 * s, (shrink ? boxes * BOX_BYTES : A_BYTES) + B_BYTES);
-                const int kx = (k_begin + i) * TC_BK;
-                if (!shrink) {
-                    tma_load_2d(a_base + s * A_BYTES, &map_w, kx, ra0, full0 + 8 * s);
-                } else {
+        for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++) {
+            const int g = j < boxes ? plan.groups[g0 + j] : 0;
+            group_row[j] = (g / ADAPTER_MAX_GROUPS) * R + (g % ADAPTER_MAX_GROUPS) * ADAPTER_GROUP;
+        }
+        auto arm_and_load_weights = [&](int i, int s) {
+            mbar_expect_tx(full0 + 8 * s, (shrink ? boxes * BOX_BYTES : A_BYTES) + B_BYTES);
+            const int kx = (k_begin + i) * TC_BK;
+            if (!shrink) {
+                tma_load_2d(a_base + s * A_BYTES, &map_w, kx, ra0, full0 + 8 * s);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++)
-                        if (j < boxes) tma_load_2d(a_base + s * A_BYTES + j * BOX_BYTES, &map_a, kx, group_row[j], full0 + 8 * s);
-                }
-            };
-            // where no kernel before this one makes weights, the first ring of them comes before the wait for the tokens' rows
-            const int n_pre = n_k < STAGES ? n_k : STAGES;
-            if (!early) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");
-                asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+                for (int j = 0; j < TC_BM / ADAPTER_GROUP; j++)
+                    if (j < boxes) tma_load_2d(a_base + s * A_BYTES + j * BOX_BYTES, &map_a, kx, group_row[j], full0 + 8 * s);
             }
+        };
+        // where no kernel before this one makes weights, the first ring of them comes before the wait for the tokens' rows
+        const int n_pre = n_k < STAGES ? n_k : STAGES;
+        if (!early) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        }
+        if (elected)
             for (int i = 0; i < n_pre; i++) arm_and_load_weights(i, i);
-            if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (elected)
             for (int i = 0; i < n_pre; i++) tma_load_2d(b_base + i * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * i);
-            bool alive = true;
-            int s = 0, phase = 0;
-            for (int i = n_pre; i < n_k; i++) {
-                alive = mbar_wait(empty0 + 8 * s, phase, err);
-                if (!alive) break;
+        bool alive = true;
+        int s = 0, phase = 0;
+        for (int i = n_pre; i < n_k; i++) {
+            alive = mbar_wait_warp(empty0 + 8 * s, phase, err);
+            if (!alive) break;
+            if (elected) {
                 arm_and_load_weights(i, s);
                 tma_load_2d(b_base + s * B_BYTES, &map_x, (k_begin + i) * TC_BK, 0, full0 + 8 * s);
-                if (++s == STAGES) s = 0, phase ^= 1;
             }
+            if (++s == STAGES) s = 0, phase ^= 1;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            bool alive = true;
-            int s = 0, phase = 0;
-            for (int i = 0; i < n_k; i++) {
-                alive = mbar_wait(full0 + 8 * s, phase, err);
-                if (!alive) break;
-                tc_fence_after();
+        const bool elected = elect_one();
+        const unsigned long long da0 = umma_desc_sw128(a_base), db0 = umma_desc_sw128(b_base);
+        bool alive = true;
+        int s = 0, phase = 0;
+        for (int i = 0; i < n_k; i++) {
+            alive = mbar_wait_warp(full0 + 8 * s, phase, err);
+            if (!alive) break;
+            tc_fence_after();
+            if (elected) {
+                const unsigned long long da = da0 + s * (A_BYTES >> 4), db = db0 + s * (B_BYTES >> 4);
 #pragma unroll
-                for (int kk = 0; kk < TC_BK / 16; kk++)
-                    umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
-                              (i > 0 || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16(tmem, da + 2 * kk, db + 2 * kk, IDESC, (i > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(empty0 + 8 * s);
-                if (++s == STAGES) s = 0, phase ^= 1;
             }
-            umma_commit(done_bar);
+            if (++s == STAGES) s = 0, phase ^= 1;
         }
+        if (elected) umma_commit(done_bar);
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;
         asm volatile("griddepcontrol.wait;" ::: "memory");      // the workspace may still be read by an earlier kernel

@@ -9,12 +9,16 @@
 // their ranks; scaled in float32, rounded to bfloat16 (the operand type of the product that follows; 2^-8 of a term that
 // is itself a correction), zero where the token's adapter is another one.  Its bound is reading x once, from L2 behind the first chunk.
 //
-// adapter_pair_kernel is the product on pairs of SMs (256 x 256 tiles, cta_group::2, as gemm_tc2.cu: two blocks hold 128 token
-// rows and 128 weight rows each, persistent over the tiles, two accumulators in tensor memory).  A chunk is one more stage of
-// its ring: 128 rows of v (128-byte swizzle) and four boxes of [128 outputs x 16 ranks] of B (32-byte swizzle, laid out so
-// that a K step of 16 is one rank group of any adapter).  Few tiles: K is cut into slices, whose float32 sums a last kernel adds up.
-// It starts while the first kernel still runs: that one lets it go only when its own wait for the tokens' rows is over, so
-// the shared product may be read at once, and only the chunks wait.
+// adapter_pair_kernel is the product on pairs of SMs (tiles of 256 tokens by 96 to 256 outputs, cta_group::2, as gemm_tc2.cu: two
+// blocks hold 128 token rows and half the weight rows each, persistent over the tiles, two accumulators in tensor memory).  A chunk
+// is one more stage of its ring: 128 rows of v (128-byte swizzle) and four boxes of [half the outputs x 16 ranks] of B (32-byte
+// swizzle, laid out so that a K step of 16 is one rank group of any adapter).  Few tiles: narrower ones, or slices of K, whose
+// float32 sums a last kernel adds up (ap_shape).  It starts while the first kernel still runs: that one lets it go only when its own
+// wait for the tokens' rows is over, so the shared product may be read at once, and only the chunks wait.
+// Measured on one B200: 2,048 tokens of 4096 x 4096 with 12 adapters of mixed ranks 62 us (1,110 TFLOP/s, the product alone 51 to
+// 55), 4,096 of 4096 x 22016 with rank 64 569 us (1,320 TFLOP/s, 94 % of what the library's product keeps up), 200 of
+// 4096 x 6144 20.6 us, of which reading the weight takes 7.7.  Bound: the tensor cores from about 1,000 tokens on, below that
+// the latency of launching, filling and draining two dependent kernels.
 #include "adapters.cuh"
 #include "kernels.h"
 #include "tc_pair.cuh"
@@ -23,10 +27,8 @@
 #define AP_VALUE_THREADS 256
 #define AP_COLS (ADAPTER_CHUNK * ADAPTER_GROUP)        // columns of a chunk
 #define AP_PITCH (AP_COLS + 4)      // floats: rows start on 16 bytes, and 8 neighbouring ones in different banks
-#define AP_STAGES 6
 #define AP_OUT_PITCH 33
-#define AP_BN 256
-#define AP_HALF 128
+#define AP_THREADS 224             // of the product: two warps fetch, one multiplies, four finish
 
 __device__ __forceinline__ float4 ap_load_remote(const float* local, unsigned rank) {
     float4 v;
@@ -79,7 +81,9 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     tc_fence_after();
     const unsigned tmem = tmem_holder;
 
-    if (warp <= 1 && lane == 0) {
+    if (warp <= 1) {
+        // (the warps stay together around what one lane issues: what every lane agrees on then lies in uniform registers)
+        const bool elected = elect_one();
         // warp 0 fetches the tokens' rows (and hears from the MMAs when a stage is free), warp 1 the adapters'; a stage is full when
         // both have arrived
         int row[ADAPTER_CHUNK], boxes = 0;
@@ -97,10 +101,11 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         bool alive = true;
         int s = 0, phase = 1;
         for (int i = 0; i < n_k; i++) {
-            if (i >= STAGES) alive = mbar_wait(empty0 + 8 * s, phase, err);
+            if (i >= STAGES) alive = mbar_wait_warp(empty0 + 8 * s, phase, err);
             if (!alive) break;
             const int kx = (k_begin + i) * TC_BK;
-            if (warp == 0) {
+            if (!elected) {
+            } else if (warp == 0) {
                 mbar_expect_tx(full0 + 8 * s, A_BYTES);
                 tma_load_2d(a_base + s * A_BYTES, &map_x, kx, t0, full0 + 8 * s);
             } else {
@@ -115,21 +120,24 @@ adapter_values_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             }
             if (++s == STAGES) s = 0, phase ^= 1;
         }
-    } else if (warp == 2 && lane == 0) {
+    } else if (warp == 2) {
+        const bool elected = elect_one();
+        const unsigned long long da0 = umma_desc_sw128(a_base), db0 = umma_desc_sw128(b_base);
         bool alive = true;
         int s = 0, phase = 0;
         for (int i = 0; i < n_k; i++) {
-            alive = mbar_wait(full0 + 8 * s, phase, err);
+            alive = mbar_wait_warp(full0 + 8 * s, phase, err);
             if (!alive) break;
             tc_fence_after();
+            if (elected) {
+                const unsigned long long da = da0 + s * (A_BYTES >> 4), db = db0 + s * (B_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < TC_BK / 16; kk++)
-                umma_bf16(tmem, umma_desc_sw128(a_base + s * A_BYTES + kk * 32), umma_desc_sw128(b_base + s * B_BYTES + kk * 32), IDESC,
-                          (i > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(empty0 + 8 * s);
+                for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16(tmem, da + 2 * kk, db + 2 * kk, IDESC, (i > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(empty0 + 8 * s);
+            }
             if (++s == STAGES) s = 0, phase ^= 1;
         }
-        umma_commit(done_bar);
+        if (elected) umma_commit(done_bar);
     }
     // each block finishes its share of the rows, four columns to a thread: what it needs for that, while the products run
     const int rows = TC_BM / C, items = rows * (AP_COLS / 4);
@@ -190,15 +198,17 @@ __device__ __forceinline__ unsigned long long umma_desc_sw32(unsigned smem_addr)
 
 // C = x . W^T + the chunks.  splits > 1: C is float32 [splits, T, N], slice z the z-th run of K pieces, the last with the chunks.
 // (Tiles of 512 outputs, which need 48 KB instead of 64 for the same work but cannot hide their epilogue, were 3 to 15 % slower.)
-template <typename TOut>
-__global__ void __launch_bounds__(TC_THREADS)
+// Even, so that a stage is always the same warp's to fill: a wait by parity holds only for one that has seen the phase before.
+template <int BN> constexpr int ap_stages() { return 192 * 1024 / ((TC_BM + BN / 2) * TC_BK * 2) / 2 * 2; }
+template <int BN, typename TOut>
+__global__ void __launch_bounds__(AP_THREADS)
 adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_b, TOut* __restrict__ C, int T, int N, int R, int k_iters_total, int splits, const AdPlan plan,
                     int chunked, int* __restrict__ err) {
-    constexpr int STAGES = AP_STAGES;
-    constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = AP_HALF * TC_BK * 2, BOX_BYTES = AP_HALF * ADAPTER_GROUP * 2;
+    constexpr int STAGES = ap_stages<BN>(), HALF = BN / 2;
+    constexpr unsigned A_BYTES = TC_BM * TC_BK * 2, B_BYTES = HALF * TC_BK * 2, BOX_BYTES = HALF * ADAPTER_GROUP * 2;
     constexpr unsigned TMEM_COLS = 512;
-    constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AP_BN >> 3) << 17) | ((unsigned)(256 >> 4) << 24);
+    constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(BN >> 3) << 17) | ((unsigned)(256 >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const unsigned base = tc_smem_u32(smem_raw);
     const unsigned a_base = base, b_base = a_base + STAGES * A_BYTES;
@@ -211,7 +221,7 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-    const int n_m = (T + 255) / 256, n_tiles = n_m * ((N + AP_BN - 1) / AP_BN), n_items = n_tiles * splits;
+    const int n_m = (T + 255) / 256, n_tiles = n_m * ((N + BN - 1) / BN), n_items = n_tiles * splits;
     const int per = (k_iters_total + splits - 1) / splits;
 
     if ((base & 1023u) != 0) {          // no static shared memory is declared: cannot happen; never run misaligned
@@ -249,36 +259,43 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         c0 = c1 = 0;
         if (chunked && z == splits - 1) c0 = plan.tile_chunk[m], c1 = plan.tile_chunk[m + 1];
     };
-    if (warp == 0) {
-        if (lane == 0) {
-            bool alive = true, waited = false;
-            int s = 0, phase = 1, it = 0;
-            const unsigned full_leader = map_to_cta(full0, 0);      // block 0 counts the bytes of both
-            if (!chunked) asm volatile("griddepcontrol.wait;" ::: "memory");       // no kernel of ours has waited for the tokens' rows
-            for (int i = pair; i < n_items && alive; i += n_pairs) {
-                int m, n, k0, k1, c0, c1;
-                item(i, m, n, k0, k1, c0, c1);
-                const int ra0 = m * 256 + (int)rank * 128, rb0 = n * AP_BN + (int)rank * AP_HALF;
-                for (int k = k0; k < k1 + (c1 - c0); k++, it++) {
-                    if (it >= STAGES) alive = mbar_wait(empty0 + 8 * s, phase, err);
-                    if (!alive) break;
-                    const unsigned a_s = a_base + s * A_BYTES, b_s = b_base + s * B_BYTES, full = full_leader + 8 * s;
-                    if (k < k1) {
+    if (warp == 0 || warp == 6) {
+        // two warps that fetch, each every other piece (one of them takes about 0.22 us for a piece's wait, its announcement and its
+        // two loads; a warp stays together around what one lane issues, which costs it a third less than a lane by itself)
+        const bool elected = elect_one();
+        const int turn = warp == 6;
+        bool alive = true, waited = false;
+        int s = turn, phase = 1, it = 0;
+        const unsigned full_leader = map_to_cta(full0, 0);      // block 0 counts the bytes of both
+        if (!chunked) asm volatile("griddepcontrol.wait;" ::: "memory");       // no kernel of ours has waited for the tokens' rows
+        for (int i = pair; i < n_items && alive; i += n_pairs) {
+            int m, n, k0, k1, c0, c1;
+            item(i, m, n, k0, k1, c0, c1);
+            const int ra0 = m * 256 + (int)rank * 128, rb0 = n * BN + (int)rank * HALF, end = k1 + (c1 - c0);
+            // `it` counts the pieces of all items
+            for (int k = k0 + ((it ^ turn) & 1); k < end; k += 2) {
+                if (it + (k - k0) >= STAGES) alive = mbar_wait_warp(empty0 + 8 * s, phase, err);
+                if (!alive) break;
+                const unsigned a_s = a_base + s * A_BYTES, b_s = b_base + s * B_BYTES, full = full_leader + 8 * s;
+                if (k < k1) {
+                    if (elected) {
                         if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + B_BYTES));
                         tma_load_2d_pair(b_s, &map_w, k * TC_BK, rb0, full);
                         tma_load_2d_pair(a_s, &map_x, k * TC_BK, ra0, full);
-                    } else {
-                        const int c = c0 + (k - k1);
-                        int g[ADAPTER_CHUNK], boxes = 0;
+                    }
+                } else {
+                    const int c = c0 + (k - k1);
+                    int g[ADAPTER_CHUNK], boxes = 0;
 #pragma unroll
-                        for (int j = 0; j < ADAPTER_CHUNK; j++) {
-                            g[j] = plan.chunk_groups[c * ADAPTER_CHUNK + j];
-                            boxes += g[j] >= 0;
-                        }
-                        if (!waited) {
-                            asm volatile("griddepcontrol.wait;" ::: "memory");     // the values are there
-                            waited = true;
-                        }
+                    for (int j = 0; j < ADAPTER_CHUNK; j++) {
+                        g[j] = plan.chunk_groups[c * ADAPTER_CHUNK + j];
+                        boxes += g[j] >= 0;
+                    }
+                    if (!waited) {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");     // the values are there
+                        waited = true;
+                    }
+                    if (elected) {
                         if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (A_BYTES + boxes * BOX_BYTES));
                         tma_load_2d_pair(a_s, &map_v, 0, c * ADAPTER_TILE + (int)rank * 128, full);
 #pragma unroll
@@ -288,12 +305,15 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                                 tma_load_2d_pair(b_s + j * BOX_BYTES, &map_b, 0, row, full);
                             }
                     }
-                    if (++s == STAGES) s = 0, phase ^= 1;
                 }
+                s += 2;
+                if (s >= STAGES) s -= STAGES, phase ^= 1;
             }
+            it += end - k0;
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool elected = elect_one();
             bool alive = true;
             int s = 0, phase = 0, ti = 0;
             // descriptors of the first stage; 16 bytes are one unit of their address
@@ -302,33 +322,35 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 int m, n, k0, k1, c0, c1;
                 item(i, m, n, k0, k1, c0, c1);
                 const int buf = ti & 1;
-                const unsigned d = tmem + buf * AP_BN;
-                if (ti >= 2) alive = mbar_wait(acc_empty0 + 8 * buf, ((ti >> 1) - 1) & 1, err);
+                const unsigned d = tmem + buf * 256;
+                if (ti >= 2) alive = mbar_wait_warp(acc_empty0 + 8 * buf, ((ti >> 1) - 1) & 1, err);
                 tc_fence_after();
                 // (one thread issues every MMA of the pair: its loop over K holds nothing but waits and MMAs, and the chunks have
                 // their own; with a choice between the two inside, 4,096 tokens of 4096 x 22016 took 610 us instead of 479)
                 for (int k = k0; k < k1 && alive; k++) {
-                    alive = mbar_wait(full0 + 8 * s, phase, err);
+                    alive = mbar_wait_warp(full0 + 8 * s, phase, err);
                     if (!alive) break;
                     tc_fence_after();
                     const unsigned long long da = da0 + s * (A_BYTES >> 4), db = db0 + s * (B_BYTES >> 4);
+                    if (elected) {
 #pragma unroll
-                    for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16_pair(d, da + 2 * kk, db + 2 * kk, IDESC, (k > k0 || kk > 0) ? 1u : 0u);
-                    umma_commit_pair(empty0 + 8 * s);
+                        for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16_pair(d, da + 2 * kk, db + 2 * kk, IDESC, (k > k0 || kk > 0) ? 1u : 0u);
+                        umma_commit_pair(empty0 + 8 * s);
+                    }
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
                 for (int c = c0; c < c1 && alive; c++) {
-                    alive = mbar_wait(full0 + 8 * s, phase, err);
+                    alive = mbar_wait_warp(full0 + 8 * s, phase, err);
                     if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int kk = 0; kk < ADAPTER_CHUNK; kk++)
-                        if (plan.chunk_groups[c * ADAPTER_CHUNK + kk] >= 0)
+                        if (elected && plan.chunk_groups[c * ADAPTER_CHUNK + kk] >= 0)
                             umma_bf16_pair(d, da0 + s * (A_BYTES >> 4) + 2 * kk, umma_desc_sw32(b_base + s * B_BYTES + kk * BOX_BYTES), IDESC, 1u);
-                    umma_commit_pair(empty0 + 8 * s);
+                    if (elected) umma_commit_pair(empty0 + 8 * s);
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
-                umma_commit_pair(acc_full0 + 8 * buf);
+                if (elected) umma_commit_pair(acc_full0 + 8 * buf);
             }
         }
     } else {
@@ -340,16 +362,16 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         for (int i = pair; i < n_items && alive; i += n_pairs, ti++) {
             int m, n, k0, k1, c0, c1;
             item(i, m, n, k0, k1, c0, c1);
-            const int buf = ti & 1, ra = m * 256 + (int)rank * 128 + quad * 32 + lane, rb0 = n * AP_BN;
+            const int buf = ti & 1, ra = m * 256 + (int)rank * 128 + quad * 32 + lane, rb0 = n * BN;
             TOut* Cz = C + (size_t)(i / n_tiles) * T * N;
             // lanes leave the polling loop one by one: together again before the warp-wide tcgen05.ld
             alive = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (ti >> 1) & 1, err));
             if (!alive) break;
             tc_fence_after();
-            const unsigned tbase = tmem + ((unsigned)(quad * 32) << 16) + (unsigned)(buf * AP_BN);
+            const unsigned tbase = tmem + ((unsigned)(quad * 32) << 16) + (unsigned)(buf * 256);
             if ((N & 7) == 0) {
 #pragma unroll 1
-                for (int c = 0; c < AP_BN; c += 16) {
+                for (int c = 0; c < BN; c += 16) {
                     if (rb0 + c >= N) break;
                     float v[16];
                     tmem_ld16(tbase + c, v);
@@ -365,7 +387,7 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 float* mine = stage_out + (warp - 2) * 32 * AP_OUT_PITCH;
                 const int rows = min(32, T - (ra - lane));
 #pragma unroll 1
-                for (int c = 0; c < AP_BN; c += 32) {
+                for (int c = 0; c < BN; c += 32) {
                     if (rb0 + c >= N) break;
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -413,57 +435,90 @@ template <typename TOut> __global__ void __launch_bounds__(256) adapter_sum_kern
 
 // ---- host side
 
-// Slices of K: as many as there are pairs of SMs for the tiles, each of at least 16 pieces, at most 4.
-static int ap_splits(int T, int N, int K) {
-    const int tiles = ad_div(T, 256) * ad_div(N, AP_BN), k_iters = ad_div(K, TC_BK);
-    int s = illm_sm_count() / 2 / tiles;
-    s = s > k_iters / 16 ? k_iters / 16 : s;
-    s = s > 4 ? 4 : (s < 1 ? 1 : s);
-    return ad_div(k_iters, ad_div(k_iters, s));
+// How the shared product is cut: the width of its tiles, the slices of K and the blocks that share a chunk's values.
+struct ApShape { int bn, splits, C; };
+
+// Blocks that share a chunk's K: the product's pairs of SMs start at once where the kernel of the values leaves SMs free, and those
+// that start behind it should be the ones that the last round of tiles would leave idle (2,048 tokens of 4096 x 4096: 57 us, 67
+// with blocks everywhere), as long as a block's share of K is no longer than a tile's; else about two blocks to an SM.
+static int ap_values_blocks(int items, int chunks, int k_iters, int splits) {
+    const int most_pairs = illm_sm_count() / 2;
+    const int idle = 2 * (items <= most_pairs ? most_pairs - items : (most_pairs - items % most_pairs) % most_pairs);
+    auto share = [&](int room) {
+        int c = 1;
+        while (c < 8 && chunks * 2 * c * 2 <= room && k_iters >= 4 * c) c *= 2;
+        return c;
+    };
+    const int c = share(idle);
+    return chunks * 2 * c > idle || ad_div(k_iters, c) > ad_div(k_iters, splits) ? share(2 * illm_sm_count()) : c;
+}
+
+// The least of an estimate in us over widths of 96 to 256 and up to 4 slices.  A pair of SMs takes max(0.18, 0.045 + 0.0011 width) for
+// a piece of 64 (from 96 on it is bound by the waits and the issue of the pieces), the tiles come in rounds of as many as there are
+// pairs; the values of the last chunk take 3 and 0.42 a piece, beside it or before it; slices cost their kernel, 2, and their bytes twice.
+// Measured with 256 wide tiles (with slices where they do not fill the pairs) and with the choice: 200 tokens of 4096 x 6144 29.0
+// and 18.7 us, 512 of 4096 x 4096 24.9 and 18.8, 1,000 of 4096 x 6144 47.2 and 42.3, 257 of 1024 x 1024 14.8 and 9.3.
+static ApShape ap_shape(int T, int N, int K, int chunks) {
+    const int k_iters = ad_div(K, TC_BK), pairs = illm_sm_count() / 2;
+    ApShape best{256, 1, 1};
+    float least = 0.f;
+    for (int bn = 256; bn >= 96; bn -= 32)
+        for (int want = 1; want <= 4; want++) {
+            const int pieces = ad_div(k_iters, want), splits = ad_div(k_iters, pieces), items = ad_div(T, 256) * ad_div(N, bn) * splits;
+            if (splits != want || (splits > 1 && (items > pairs || pieces < 8))) continue;
+            const int C = chunks > 0 ? ap_values_blocks(items, chunks, k_iters, splits) : 1;
+            const float piece = 0.045f + 0.001075f * bn, product = ad_div(items, pairs) * pieces * (piece < 0.18f ? 0.18f : piece);
+            // (where they find no SM left free the product's blocks wait for theirs)
+            const float values = chunks > 0 ? 3.f + 0.42f * ad_div(k_iters, C) : 0.f;
+            const bool beside = chunks * 2 * C <= 2 * (pairs - items % pairs) % (2 * pairs);
+            const float time = (!beside ? product + values : product < values ? values : product) + (splits > 1 ? 2.f + (float)splits * T * N * 1.6e-6f : 0.f);
+            if (least == 0.f || time < least) least = time, best = ApShape{bn, splits, C};
+        }
+    return best;
 }
 long long ad_prompt_ws(int T, int N, int K, int chunks) {
-    const int s = ap_splits(T, N, K);
+    const int s = ap_shape(T, N, K, chunks).splits;
     return ad_round((long long)chunks * ADAPTER_TILE * AP_COLS * 2) + (s > 1 ? (long long)s * T * N * 4 : 0);
 }
 
-template <typename TOut>
+template <int BN, typename TOut>
 static int ap_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mv, const CUtensorMap& mb, TOut* out, int T, int N, int R, int k_iters,
                           int splits, const AdPlan& plan, int chunked, int* err, cudaStream_t s) {
-    const size_t smem = (size_t)AP_STAGES * (TC_BM + AP_HALF) * TC_BK * 2 + 16 * AP_STAGES + 32 + 16 + ((N & 7) ? 4 * 32 * AP_OUT_PITCH * 4 : 0);
-    auto kern = adapter_pair_kernel<TOut>;
+    const size_t smem = (size_t)ap_stages<BN>() * (TC_BM + BN / 2) * TC_BK * 2 + 16 * ap_stages<BN>() + 32 + 16 + ((N & 7) ? 4 * 32 * AP_OUT_PITCH * 4 : 0);
+    auto kern = adapter_pair_kernel<BN, TOut>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    const int items = ad_div(T, 256) * ad_div(N, AP_BN) * splits, most = illm_sm_count() / 2, pairs = items < most ? items : most;
-    return illm_launch_cluster(kern, dim3(2 * pairs), dim3(TC_THREADS), 2, smem, s, mx, mw, mv, mb, out, T, N, R, k_iters, splits, plan, chunked, err);
+    const int items = ad_div(T, 256) * ad_div(N, BN) * splits, most = illm_sm_count() / 2, pairs = items < most ? items : most;
+    return illm_launch_cluster(kern, dim3(2 * pairs), dim3(AP_THREADS), 2, smem, s, mx, mw, mv, mb, out, T, N, R, k_iters, splits, plan, chunked, err);
+}
+
+template <typename TOut>
+static int ap_launch(int bn, const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mv, const CUtensorMap& mb, TOut* out, int T, int N, int R, int k_iters,
+                     int splits, const AdPlan& plan, int chunked, int* err, cudaStream_t s) {
+    switch (bn) {
+#define AP_CASE(W) case W: return ap_launch_pair<W>(mx, mw, mv, mb, out, T, N, R, k_iters, splits, plan, chunked, err, s);
+        AP_CASE(96) AP_CASE(128) AP_CASE(160) AP_CASE(192) AP_CASE(224)
+#undef AP_CASE
+        default: return ap_launch_pair<256>(mx, mw, mv, mb, out, T, N, R, k_iters, splits, plan, chunked, err, s);
+    }
 }
 
 int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R,
                    const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int early, int* err, cudaStream_t s) {
     (void)early;
-    const int k_iters = ad_div(K, TC_BK), splits = ap_splits(T, N, K);
+    const ApShape shape = ap_shape(T, N, K, chunks);
+    const int k_iters = ad_div(K, TC_BK), splits = shape.splits, bn = shape.bn, C = shape.C;
     bf16* v = (bf16*)ws;
     float* slices = (float*)(ws + ad_round((long long)chunks * ADAPTER_TILE * AP_COLS * 2));
     CUtensorMap mx, ma, ma4, mw, mv, mb;
     int rc;
-    if ((rc = ad_make_map(&mx, x, T, K, TC_BM)) || (rc = ad_make_map(&mw, w, N, K, AP_HALF))) return rc;
+    if ((rc = ad_make_map(&mx, x, T, K, TC_BM)) || (rc = ad_make_map(&mw, w, N, K, bn / 2))) return rc;
     mv = mb = mx;
     if (chunks > 0) {
         if ((rc = ad_make_map(&ma, a, (long long)count * R, K, ADAPTER_GROUP)) || (rc = ad_make_map(&ma4, a, (long long)count * R, K, AP_COLS)) ||
             (rc = ad_make_map(&mv, v, (long long)chunks * ADAPTER_TILE, AP_COLS, TC_BM)) ||
-            (rc = ad_make_map(&mb, b, (long long)count * (R / ADAPTER_GROUP) * N, ADAPTER_GROUP, AP_HALF, ADAPTER_GROUP, CU_TENSOR_MAP_SWIZZLE_32B)))
+            (rc = ad_make_map(&mb, b, (long long)count * (R / ADAPTER_GROUP) * N, ADAPTER_GROUP, bn / 2, ADAPTER_GROUP, CU_TENSOR_MAP_SWIZZLE_32B)))
             return rc;
-        // Blocks that share a chunk's K: the product's pairs of SMs start at once where this kernel leaves SMs free, and those that start
-        // behind it should be the ones that the last round of tiles would leave idle (2,048 tokens of 4096 x 4096: 57 us, 67 with
-        // blocks everywhere), as long as a block's share of K is no longer than a tile's; else about two blocks to an SM.
-        const int most_pairs = illm_sm_count() / 2, items = ad_div(T, 256) * ad_div(N, AP_BN) * splits;
-        const int idle = 2 * (items <= most_pairs ? most_pairs - items : (most_pairs - items % most_pairs) % most_pairs);
-        auto share = [&](int room) {
-            int c = 1;
-            while (c < 8 && chunks * 2 * c * 2 <= room && k_iters >= 4 * c) c *= 2;
-            return c;
-        };
-        int C = share(idle);
-        if (chunks * 2 * C > idle || ad_div(k_iters, C) > ad_div(k_iters, splits)) C = share(2 * illm_sm_count());
         // the ring holds a block's whole share of K where one block has an SM to itself
         const int per = ad_div(k_iters, C), most = chunks * 2 * C > illm_sm_count() ? 4 : AP_VALUE_STAGES, stages = per < 2 ? 2 : per < most ? per : most;
         const size_t smem = (size_t)stages * (TC_BM + AP_COLS) * TC_BK * 2 + 1024;
@@ -475,7 +530,7 @@ int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void
         if (rc) return rc;
     }
     if (splits > 1) {
-        rc = ap_launch_pair<float>(mx, mw, mv, mb, slices, T, N, R, k_iters, splits, plan, chunks > 0, err, s);
+        rc = ap_launch<float>(bn, mx, mw, mv, mb, slices, T, N, R, k_iters, splits, plan, chunks > 0, err, s);
         if (rc) return rc;
         const long long n = (long long)T * N;
         if (n % 4 || ((uintptr_t)out & 15)) return illm_splitk_reduce(slices, out, out_dtype, n, splits, s);
@@ -484,6 +539,6 @@ int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void
         else illm_launch(adapter_sum_kernel<float>, blocks, dim3(256), 0, s, (const float*)slices, splits, n, (float*)out);
         return illm_launch_status();
     }
-    if (out_dtype == ILLM_BF16) return ap_launch_pair<bf16>(mx, mw, mv, mb, (bf16*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
-    return ap_launch_pair<float>(mx, mw, mv, mb, (float*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
+    if (out_dtype == ILLM_BF16) return ap_launch<bf16>(bn, mx, mw, mv, mb, (bf16*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
+    return ap_launch<float>(bn, mx, mw, mv, mb, (float*)out, T, N, R, k_iters, 1, plan, chunks > 0, err, s);
 }

@@ -47,6 +47,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int* er
     atomicExch(err, code);
     return false;
 }
+// one lane of a warp that is together
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// a wait of a whole warp, which is together behind it and agrees on its outcome
+__device__ __forceinline__ bool mbar_wait_warp(unsigned bar, unsigned parity, int* err) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); }
 __device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
