@@ -826,18 +826,25 @@ class Adapters:
             raise KernelError(f"adapters: rank {r} exceeds the {self.rank} there is room for")
         if not (a.is_floating_point() and b.is_floating_point()):
             raise KernelError("adapters: the factors must be floating-point tensors")
-        # (copies: they may be parameters, or the place's own factors)
-        a, b = (f.detach().to(self.device, self.dtype, copy=True) for f in (a, b))
         scale = float(scale)
-        # (the prompt product multiplies an adapter's b with the zeros of its neighbours' tokens)
-        if not (abs(scale) <= torch.finfo(torch.float32).max and bool(a.isfinite().all()) and bool(b.isfinite().all())):
+        finite = abs(scale) <= torch.finfo(torch.float32).max
+        a, b = (f.detach().to(self.device, self.dtype) for f in (a, b))
+        if r > 0:
+            # (the prompt product multiplies an adapter's b with the zeros of its neighbours' tokens; NaN is its own least and largest)
+            finite = finite and bool(torch.stack(torch.aminmax(a) + torch.aminmax(b)).isfinite().all())
+        if not finite:
             raise KernelError(f"adapters: adapter {i} is not finite in {self.dtype}")
-        self.a[i].zero_()
+        own = self.a.untyped_storage().data_ptr(), self.b.untyped_storage().data_ptr()
+        a, b = (f.clone() if f.untyped_storage().data_ptr() in own else f for f in (a, b))      # (an adapter's factors, put again)
         self.a[i, :r] = a
-        self.b[i].zero_()
-        for g in range(0, r, ADAPTER_GROUP):
-            e = min(r, g + ADAPTER_GROUP)
-            self.b[i, g // ADAPTER_GROUP, :, :e - g] = b[:, g:e]
+        self.a[i, r:].zero_()
+        whole, rest = divmod(r, ADAPTER_GROUP)
+        to = self.b[i]
+        if whole:
+            to[:whole] = b[:, :r - rest].unflatten(1, (whole, ADAPTER_GROUP)).transpose(0, 1)
+        to[whole:].zero_()
+        if rest:
+            to[whole, :, :rest] = b[:, r - rest:]
         self.scales[i] = scale
         if self.ranks[i] != r:
             self.ranks[i] = r
