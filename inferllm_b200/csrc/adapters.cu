@@ -10,7 +10,8 @@
 //            reads a row of A once for the tokens of a slot;
 //   expand   y[t, n] += v[t] . B_a[n]: a thread per output column, 16 values of B in registers for neighbours with one adapter.
 // A token's sums have one order whatever else is in the batch, and one without an adapter keeps the plain product's bits.
-// Bfloat16: up to 128 tokens below, prompts in adapters_prompt.cu.
+// 257 tokens of 1024 x 5632: 97 us of product (bound by its FMAs: 41 at full rate, and three rounds of tiles), 12 of adapters.
+// Bfloat16: token by token below, tiles of tokens in adapters_prompt.cu (ad_tiled).
 #include "adapters.cuh"
 #include "kernels.h"
 
@@ -114,6 +115,8 @@ adapter_expand_kernel(int N, const float* __restrict__ b, const float* __restric
 // 128 lanes, the tokens as the MMA's N, and leaves float32 slices, so that all SMs stream whatever N is.
 // The second adds up the slices and, in the same float32 sum, v[t] . B_a[n]; v, the tokens' rank values, is added up and
 // scaled by every block for the tokens that it works on.  It stays float32: the result is rounded once.
+// Bound: reading the weight and the factors, and two starts and ends.  One token of 4096 x 4096 9.9 us on the GPU (the weight's 33 MB
+// at the copy rate: 5.1), 8 tokens with 8 adapters of 4096 x 12288 22.6 (16.0), 64 tokens with 48 of 11008 x 4096 31.4 (19.4).
 #define AD_ROWS_MAX_STAGES 8
 
 template <int BN>
@@ -260,14 +263,13 @@ __device__ __forceinline__ float ad_dot16(const float* w, const float* v, float 
     return acc;
 }
 
-// TOK places of the plan's order by 128 threads of VEC columns.  SHARED: neighbours mostly have the same adapter, whose values of B
-// are then loaded once for them; otherwise the loads of all places are in flight together.
-template <int TOK, bool SHARED, int VEC, typename TOut>
+// TOK places of the plan's order by 128 threads, a column each; the loads of all places are in flight together.
+template <int TOK, typename TOut>
 __global__ void __launch_bounds__(AD_COLS)
 adapter_join_kernel(const float* __restrict__ base, int splits, long long stride, int N, const bf16* __restrict__ b, const float* __restrict__ vs, int v_ld,
                     const float* __restrict__ scales, int R, const int4* __restrict__ places, int T, TOut* __restrict__ out) {
     __shared__ __align__(16) float v[TOK][ADAPTER_GROUP * ADAPTER_MAX_GROUPS];
-    const int tid = threadIdx.x, col = (blockIdx.x * AD_COLS + tid) * VEC, p0 = blockIdx.y * TOK;
+    const int tid = threadIdx.x, col = blockIdx.x * AD_COLS + tid, p0 = blockIdx.y * TOK;
     int4 at[TOK];                                       // token, adapter, first group, groups
     int most = 0;
 #pragma unroll
@@ -277,32 +279,23 @@ adapter_join_kernel(const float* __restrict__ base, int splits, long long stride
     }
     // the second factors as well: the first groups' values come before the wait for the kernel that makes the slices
     const size_t ld = (size_t)(R / ADAPTER_GROUP) * N * ADAPTER_GROUP;
-    uint4 head[SHARED ? 1 : TOK][SHARED ? 1 : VEC][2];
-    if (!SHARED && col < N)
+    uint4 head[TOK][2];
+    if (col < N)
 #pragma unroll
         for (int i = 0; i < TOK; i++)
             if (at[i].w > 0)
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) head[i][e][h] = reinterpret_cast<const uint4*>(b + at[i].y * ld + (size_t)(col + e) * ADAPTER_GROUP)[h];
+                for (int h = 0; h < 2; h++) head[i][h] = reinterpret_cast<const uint4*>(b + at[i].y * ld + (size_t)col * ADAPTER_GROUP)[h];
     pdl_grid_sync();
-    float acc[TOK][VEC];
+    float acc[TOK];
 #pragma unroll
-    for (int i = 0; i < TOK; i++)
-#pragma unroll
-        for (int e = 0; e < VEC; e++) acc[i][e] = 0.f;
+    for (int i = 0; i < TOK; i++) acc[i] = 0.f;
     if (col < N)
 #pragma unroll 4
         for (int z = 0; z < splits; z++)
 #pragma unroll
             for (int i = 0; i < TOK; i++)
-                if (at[i].x >= 0) {
-                    float f[VEC];
-                    AdColumns<VEC>::load(base + (size_t)z * stride + (size_t)at[i].x * N + col, f);
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) acc[i][e] += f[e];
-                }
+                if (at[i].x >= 0) acc[i] += base[(size_t)z * stride + (size_t)at[i].x * N + col];
     if (most > 0) {
         // the places' rank values, a thread per rank of a place
         for (int q = tid; q < TOK * most * ADAPTER_GROUP; q += AD_COLS) {
@@ -323,47 +316,26 @@ adapter_join_kernel(const float* __restrict__ base, int splits, long long stride
         __syncthreads();
         if (col < N)
             for (int g = 0; g < most; g++) {
-                const bf16* bg = b + ((size_t)g * N + col) * ADAPTER_GROUP;
-                if (SHARED) {
+                const bf16* next = b + ((size_t)(g + 1) * N + col) * ADAPTER_GROUP;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) {
+                for (int i = 0; i < TOK; i++)
+                    if (g < at[i].w) {
                         float w[ADAPTER_GROUP];
-#pragma unroll
-                        for (int i = 0; i < TOK; i++)
-                            if (g < at[i].w) {
-                                if (i == 0 || at[i].y != at[i - 1].y) {
-                                    load8(bg + at[i].y * ld + e * ADAPTER_GROUP, w);
-                                    load8(bg + at[i].y * ld + e * ADAPTER_GROUP + 8, w + 8);
-                                }
-                                acc[i][e] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i][e]);
-                            }
+                        load8(reinterpret_cast<const bf16*>(&head[i][0]), w);
+                        load8(reinterpret_cast<const bf16*>(&head[i][1]), w + 8);
+                        acc[i] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i]);
                     }
-                } else {
 #pragma unroll
-                    for (int i = 0; i < TOK; i++)
-                        if (g < at[i].w)
+                for (int i = 0; i < TOK; i++)
+                    if (g + 1 < at[i].w)
 #pragma unroll
-                            for (int e = 0; e < VEC; e++) {
-                                float w[ADAPTER_GROUP];
-                                load8(reinterpret_cast<const bf16*>(&head[i][e][0]), w);
-                                load8(reinterpret_cast<const bf16*>(&head[i][e][1]), w + 8);
-                                acc[i][e] = ad_dot16(w, &v[i][g * ADAPTER_GROUP], acc[i][e]);
-                            }
-#pragma unroll
-                    for (int i = 0; i < TOK; i++)
-                        if (g + 1 < at[i].w)
-#pragma unroll
-                            for (int e = 0; e < VEC; e++)
-#pragma unroll
-                                for (int h = 0; h < 2; h++)
-                                    head[i][e][h] = reinterpret_cast<const uint4*>(bg + at[i].y * ld + (size_t)N * ADAPTER_GROUP + e * ADAPTER_GROUP)[h];
-                }
+                        for (int h = 0; h < 2; h++) head[i][h] = reinterpret_cast<const uint4*>(next + at[i].y * ld)[h];
             }
     }
     if (col < N)
 #pragma unroll
         for (int i = 0; i < TOK; i++)
-            if (at[i].x >= 0) AdColumns<VEC>::store(out + (size_t)at[i].x * N + col, acc[i]);
+            if (at[i].x >= 0) out[(size_t)at[i].x * N + col] = from_f32<TOut>(acc[i]);
 }
 
 // How the rows form cuts K: as many slices as bring about two blocks to an SM, each at least 8 pieces of 64 wide, at most 8 slices (their reader pays for every one).
@@ -418,20 +390,27 @@ static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const
         default: rc = ad_launch_rows<128>(mw, ma, mx, base, vs, v_ld, T, N, R, r, plan, early, err, s);
     }
     if (rc) return rc;
-    auto join = [&](auto kern, int tok, int vec) {
-        illm_launch(kern, dim3(ad_div(N, AD_COLS * vec), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
+    auto join = [&](auto kern, int tok) {
+        illm_launch(kern, dim3(ad_div(N, AD_COLS), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
                     (const float*)vs, v_ld, scales, R, plan.places, T, out);
     };
-    // few tokens: many blocks; many tokens of few adapters: prompts
-    if (T <= 4) join(adapter_join_kernel<1, false, 1, TOut>, 1, 1);
-    else if (T > 64 && 4 * sz.slots <= T && N % 4 == 0) join(adapter_join_kernel<4, true, 4, TOut>, 4, 4);
-    else join(adapter_join_kernel<4, false, 1, TOut>, 4, 1);
+    // A place to a block while that makes no more than some 14 blocks to an SM, else four.  One and four, us: 32 tokens with 8
+    // adapters of rank 64 beside 4096 x 4096 13.4 and 15.1; 64 tokens with 48 adapters, their factors in memory, beside 11008 x 4096
+    // 31.4 and 34.2 (with 8 in L2 32.1 and 30.5); 16 tokens with 64 of rank 16 beside 4096 x 22016 41.4 and 38.8.
+    if (T * ad_div(N, AD_COLS) < 14 * illm_sm_count()) join(adapter_join_kernel<1, TOut>, 1);
+    else join(adapter_join_kernel<4, TOut>, 4);
     return illm_launch_status();
 }
 
+// Where both forms can run, tiles are the faster one from 65 tokens on, and for wide products from 33 (rows form and tiles, us: 80
+// tokens, 8 adapters of rank 64 beside 4096 x 4096 27.6 and 20.9, one of rank 16 beside 4096 x 12288 30.9 and 26.4; 64 tokens, 8 of
+// rank 64 beside 11008 x 4096 30.5 and 36.0, beside 4096 x 12288 41.8 and 31.2; 32 with one beside 4096 x 22016 38.3 and 41.3).  With an adapter to every
+// token they are not: 80 tokens with 64 of rank 16 beside 4096 x 4096 16.5 and 27.5.
+static bool ad_tiled(int T, int slots, int N) { return adapter_tiled(T, slots) && (T > 64 || N > 64 * illm_sm_count()); }
+
 // Bytes of workspace that illm_linear_adapters needs.
-extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int groups, int chunks) {
-    if (dtype == ILLM_BF16 && T <= ADAPTER_ROWS_MAX) {
+extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int slots, int groups, int chunks) {
+    if (dtype == ILLM_BF16 && !ad_tiled(T, slots, N)) {
         const long long splits = ad_rows(T, N, K, groups).splits;
         return ad_round(splits * T * groups * ADAPTER_GROUP * 4) + splits * T * N * 4;
     }
@@ -472,7 +451,7 @@ extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int
     if (dtype == ILLM_F32 && out_dtype == ILLM_F32)
         return ad_float32((const float*)x, (const float*)w, T, N, K, (const float*)a, (const float*)b, scales, R, sz, plan, (float*)out, (float*)ws, err, s);
     if (dtype != ILLM_BF16 || (out_dtype != ILLM_BF16 && out_dtype != ILLM_F32)) return ILLM_ERR_BAD_ARG;
-    if (T > ADAPTER_ROWS_MAX)
+    if (ad_tiled(T, slots, N))
         return ad_prompt_form(x, w, T, N, K, a, b, scales, count, R, ad_plan(plan, sz), chunks, out, out_dtype, (char*)ws, early, err, s);
     if (out_dtype == ILLM_BF16) return ad_rows_form<bf16>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (bf16*)out, (char*)ws, early, err, s);
     return ad_rows_form<float>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (float*)out, (char*)ws, early, err, s);

@@ -10,7 +10,7 @@
 #define ADAPTER_TILE 256          // tokens of a tile of the prompt product
 #define ADAPTER_CHUNK 4           // groups of a chunk: one 64-wide K piece of the prompt product
 #define ADAPTER_MAX_GROUPS 16     // ranks up to 256
-#define ADAPTER_ROWS_MAX 128      // tokens up to which the rows form runs; above it the plan has tiles
+#define ADAPTER_ROWS_MAX 128      // tokens up to which the rows form can run
 
 struct AdapterPlanSizes {
     int T;                        // tokens
@@ -18,6 +18,9 @@ struct AdapterPlanSizes {
     int groups;                   // rank groups of all slots (a bound)
     int chunks;                   // chunks of all tiles (a bound; 0: the plan has no tiles)
 };
+// Whether a step's products in bfloat16 may run as a prompt's, by tiles of tokens (the plan then has chunks): where there are more
+// tokens than the rows form takes, or at least four to an adapter.
+static inline bool adapter_tiled(int T, int slots) { return T > ADAPTER_ROWS_MAX || (T > 32 && 4 * slots <= T); }
 // Places of the arrays in the plan; each starts on a 16-byte boundary.
 struct AdapterPlanLayout {
     int counts;                   // [4] slots, rank groups, chunks that there really are, and the most groups of a slot

@@ -209,7 +209,7 @@ int illm_moe_down_splits(int T, int top, int E, int N, int K, int n_sms);
 int illm_moe_gemm_split(const void* x, int x_dtype, const void* w, int w_dtype, void* y, int T, int top, int E, int N, int K, int gated, int act, float act_limit, int bm, int tensor_cores, int splits, long long slice_stride, const int* pair_of_row, const int* tile_expert, const int* tile_row0, const int* tile_rows, void* stream);
 
 // adapters.cu
-long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int groups, int chunks);
+long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int R, int slots, int groups, int chunks);
 int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int early, int* err, void* stream);
 
 // sample_rows.cu

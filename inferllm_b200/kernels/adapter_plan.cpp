@@ -32,7 +32,7 @@ AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, i
         s.slots++;
         s.groups += groups_of(ranks[a]);
     }
-    if (T > ADAPTER_ROWS_MAX)
+    if (adapter_tiled(T, s.slots))
         for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE) {
             int g = 0;
             for (int a : named(index, t0, tile_end(t0, T))) g += groups_of(ranks[a]);
@@ -44,7 +44,7 @@ AdapterPlanSizes adapter_plan_sizes(const int* index, int T, const int* ranks, i
 AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool one_sequence) {
     const int slots = one_sequence ? std::min(1, T) : std::min(T, count);
     AdapterPlanSizes s{T, slots, slots * groups_of(max_rank), 0};
-    if (T > ADAPTER_ROWS_MAX)
+    if (adapter_tiled(T, slots))
         for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE) {
             const int adapters = std::min(tile_end(t0, T) - t0, slots);
             s.chunks += (adapters * groups_of(max_rank) + ADAPTER_CHUNK - 1) / ADAPTER_CHUNK;
@@ -54,7 +54,8 @@ AdapterPlanSizes adapter_plan_bound(int T, int count, int max_rank, bool one_seq
 
 void adapter_plan_fill(const int* index, int T, const int* ranks, int count, const AdapterPlanSizes& sizes, int* out) {
     const AdapterPlanSizes least = adapter_plan_sizes(index, T, ranks, count);
-    if (sizes.T != T || sizes.slots < least.slots || sizes.groups < least.groups || sizes.chunks < least.chunks)
+    const bool tiled = adapter_tiled(T, sizes.slots);       // (room for more adapters than there are may mean rows)
+    if (sizes.T != T || sizes.slots < least.slots || sizes.groups < least.groups || (tiled && sizes.chunks < least.chunks))
         throw KernelError("adapters: the plan does not fit the sizes that were set aside for it");
     const AdapterPlanLayout l = adapter_plan_layout(sizes);
     std::fill(out, out + l.total, 0);
@@ -89,7 +90,7 @@ void adapter_plan_fill(const int* index, int T, const int* ranks, int count, con
         rec[3] = out[l.slot_group + i + 1] - rec[2];
     }
     int chunks = 0, tile = 0;
-    if (sizes.chunks > 0) {
+    if (tiled && sizes.chunks > 0) {
         for (int t0 = 0; t0 < T; t0 += ADAPTER_TILE, tile++) {
             out[l.tile_chunk + tile] = chunks;
             int in = ADAPTER_CHUNK;         // groups in the last chunk

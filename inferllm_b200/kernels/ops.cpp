@@ -428,7 +428,7 @@ Mat linear_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& s
     Mat out = new_mat(dev, T, N, out_dtype);
     if (T == 0) return out;
     const int code = code_of(x.dtype, "linear_adapters");
-    void* ws = dev.alloc((size_t)illm_linear_adapters_ws(code, (int)T, (int)N, (int)K, set.R, view.sizes.groups, view.sizes.chunks));
+    void* ws = dev.alloc((size_t)illm_linear_adapters_ws(code, (int)T, (int)N, (int)K, set.R, view.sizes.slots, view.sizes.groups, view.sizes.chunks));
     check_kernel(illm_linear_adapters(x.p, w.p, code, (int)T, (int)N, (int)K, set.a, set.b, set.scales, set.count, set.R, view.plan, view.sizes.slots,
                                       view.sizes.groups, view.sizes.chunks, out.p, code_of(out_dtype, "linear_adapters"), ws, 1, dev.tc_error_word(),
                                       dev.stream()),

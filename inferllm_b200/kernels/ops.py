@@ -74,7 +74,7 @@ _KERNEL_SIGNATURES = {
     "illm_argmax": [P_, I_, I_, I_, P_, P_, P_, P_],
     "illm_sample": [P_, I_, I_, I_, P_, P_, I_, F_, F_, I_, F_, P_, P_, P_, P_],
     "illm_sample_scratch_elems": [I_, I_, I_, F_],
-    "illm_linear_adapters_ws": [I_, I_, I_, I_, I_, I_, I_],
+    "illm_linear_adapters_ws": [I_, I_, I_, I_, I_, I_, I_, I_],
     "illm_linear_adapters": [P_, P_, I_, I_, I_, I_, P_, P_, P_, I_, I_, P_, I_, I_, I_, P_, I_, P_, I_, P_, P_],
     "illm_sample_rows": [P_, I_, I_, I_, LL_, P_, P_, P_, P_, P_, P_, P_],
     "illm_fill_random": [P_, I_, LL_, ctypes.c_ulonglong, F_, F_, P_],
@@ -879,7 +879,7 @@ class AdapterRows:
         """The workspace of a product by this plan."""
         n = self._ws.get((code, N, K, R))
         if n is None:
-            n = self._ws[code, N, K, R] = load().illm_linear_adapters_ws(code, self.T, N, K, R, self.groups, self.chunks)
+            n = self._ws[code, N, K, R] = load().illm_linear_adapters_ws(code, self.T, N, K, R, self.slots, self.groups, self.chunks)
         return n
 
     def fits(self, adapters):

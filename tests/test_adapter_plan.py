@@ -28,7 +28,7 @@ def unpack(index, ranks):
     return (T, slots, groups, chunks), fields
 
 
-@pytest.mark.parametrize("T", [0, 1, 5, 64, 65, 256, 257, 1000])
+@pytest.mark.parametrize("T", [0, 1, 5, 64, 65, 100, 128, 256, 257, 1000])
 @pytest.mark.parametrize("count", [1, 3, 70])
 def test_every_token_and_every_rank_group_once(T, count):
     rng = np.random.default_rng(T + count)
@@ -38,7 +38,7 @@ def test_every_token_and_every_rank_group_once(T, count):
     named = sorted(set(index) - {-1})
     g_of = lambda a: -(-ranks[a] // 16)  # noqa: E731
     assert slots == len(named) and f["slot_adapter"] == named + [-1]
-    assert f["counts"] == [slots, groups, chunks if T > 128 else 0, max([g_of(a) for a in named], default=0)]
+    assert f["counts"] == [slots, groups, chunks, max([g_of(a) for a in named], default=0)]
     assert f["token_adapter"] == index and sorted(f["order"]) == list(range(T))
     assert f["slot_begin"][-1] == T
     for i, a in enumerate(f["slot_adapter"]):
@@ -49,7 +49,7 @@ def test_every_token_and_every_rank_group_once(T, count):
     for place, t in enumerate(f["order"]):
         slot = max(i for i in range(slots + 1) if f["slot_begin"][i] <= place < f["slot_begin"][i + 1])
         assert f["places"][4 * place:4 * place + 4] == [t, index[t], f["slot_group"][slot], g_of(index[t]) if index[t] >= 0 else 0]
-    if T <= 128:
+    if T <= 32 or (T <= 128 and 4 * slots > T):
         assert chunks == 0
         return
     for tile in range(-(-T // 256)):

@@ -298,3 +298,29 @@ assert torch.equal(y, ops.linear_adapters(x, w, ad, rows, torch.float32)) and to
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.parametrize("T", [65, 70, 100, 128])
+def test_from_65_to_128_tokens(T):
+    """Few adapters (tiles of tokens), many (token by token), and the two on either side of the rule."""
+    ranks = [16] * 64
+    x, w, a, b, ad, s = make(T, 512, 388, ranks, torch.bfloat16, 5 * T, lambda i: 0.25 + 0.01 * i)
+    for used in (1, 2, T // 4, T // 4 + 1, 64):
+        for index in ([t % used for t in range(T)], [(t * used // T) if t % 9 else -1 for t in range(T)]):
+            check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+    rows = ops.AdapterRows([t % 3 - 1 for t in range(T)], ad.ranks)
+    want = ops.linear_adapters(x, w, ad, rows)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_adapters(x, w, ad, rows)
+    graph.replay()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T", [33, 48, 64])
+def test_wide_products_of_33_to_64_tokens(T):
+    ranks = [16, 64, 40, 8] + [16] * 20
+    x, w, a, b, ad, s = make(T, 128, 9600, ranks, torch.bfloat16, 3 * T, lambda i: 0.25 + 0.05 * i)
+    for used in (1, 4, T // 4, T // 4 + 1):
+        index = [t % used if t % 7 else -1 for t in range(T)]
+        check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)

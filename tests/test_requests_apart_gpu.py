@@ -300,3 +300,23 @@ def test_the_operators_one_behind_another():
         assert torch.equal(l, logits) and torch.equal(t, tokens)
         host = logits.double().cpu().numpy()
         assert tokens.tolist() == [choose(host[i], float(u[i]), float(np.float32(0.8)), 30, float(np.float32(0.9))) for i in range(T)]
+
+
+@pytest.mark.parametrize("max_adapters", [4, 40])
+def test_captured_steps_of_72_sequences(max_adapters, model_folders, plain_models):
+    """Room for few adapters (tiles of tokens) or for many (token by token, whatever the step names)."""
+    name, n = "A", 72
+    cfg, w = plain_models[name]
+    e = Engine.from_folder(model_folders[name], EngineOptions(dtype="bfloat16", max_tokens=n * 64, max_batch=n, max_adapters=max_adapters, adapter_rank=12))
+    adapters = [factors(cfg, w, 12, s) for s in (1, 2, 3)]
+    for a in adapters:
+        e.add_adapter(*a)
+    p = random_prompt(name, 5, 4)
+    slots = [e.new_sequence() for _ in range(n)]
+    for s in range(0, n, 36):
+        e.step([StepItem(x, p[:1], [], -1 if x % 4 == 3 else x % 4) for x in slots[s:s + 36]])
+    want = [plain.forward(cfg, merged(w, a), p) for a in adapters + [None]]
+    for j in (1, 2, 3, 4):
+        got = e.step([StepItem(x, [p[j]], [0], -1 if x % 4 == 3 else x % 4) for x in slots]).cpu().numpy()
+        for i, x in enumerate(slots):
+            assert_close(got[i:i + 1], want[x % 4][j:j + 1], "bfloat16", f"sequence {x}, token {j}")
