@@ -420,14 +420,8 @@ extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int
 static int ad_float32(const float* x, const float* w, int T, int N, int K, const float* a, const float* b, const float* scales, int R,
                       const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int* err, cudaStream_t s) {
     const AdPlan plan = ad_plan(plan_dev, sz);
-    // The product's bits do not depend on how its rows are taken (one chain of additions over K per output).  Nine to sixteen go
-    // by eights through the kernel that streams the weight for up to eight, where its tiles would leave SMs without one: 9 tokens of
-    // 11008 x 4096 take 179 us instead of 501, 16 of 5120 x 5120 125 instead of 222; of 4096 x 22016, which fill them, 296 and 251.
-    const int by = T > 8 && T <= 16 && N < 64 * illm_sm_count() ? 8 : T;
-    for (int t = 0; t < T; t += by) {
-        const int rc = illm_gemm_f32_nt(x + (size_t)t * K, w, out + (size_t)t * N, T - t < by ? T - t : by, N, K, K, K, N, err, s);
-        if (rc != 0) return rc;
-    }
+    const int rc = illm_gemm_f32_nt(x, w, out, T, N, K, K, K, N, err, s);
+    if (rc != 0) return rc;
     if (sz.slots == 0) return 0;
     const bool wide = K % 4 == 0 && !(((uintptr_t)x | (uintptr_t)a) & 15);
     auto shrink = wide ? adapter_shrink_kernel<4> : adapter_shrink_kernel<1>;

@@ -194,7 +194,7 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     constexpr unsigned X_BYTES = MR * GS_KT * 4, STAGE_TX = GS_W_BYTES + X_BYTES;
     const unsigned w_base = (tc_smem_u32(gs_raw) + 1023u) & ~1023u, x_base = w_base + S * GS_W_BYTES;
     const unsigned char* w_gen = gs_raw + (w_base - tc_smem_u32(gs_raw));
-    const int lane = threadIdx.x, n0 = blockIdx.x * 32;
+    const int lane = threadIdx.x, n0 = blockIdx.x * 32, m0 = blockIdx.y * MR;
     const int n_tiles = (K + GS_KT - 1) / GS_KT;
     if (lane == 0) {
         for (int s = 0; s < S; s++) mbar_init(tc_smem_u32(&gs_full[s]), 1);
@@ -212,7 +212,7 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     };
     auto issue_x = [&](int t) {
         const int s = t % S;
-        tma_load_2d(x_base + s * X_BYTES, &map_a, t * GS_KT, 0, tc_smem_u32(&gs_full[s]));
+        tma_load_2d(x_base + s * X_BYTES, &map_a, t * GS_KT, m0, tc_smem_u32(&gs_full[s]));
     };
     const int n_pre = n_tiles < S - 1 ? n_tiles : S - 1;
     if (lane == 0)
@@ -263,7 +263,106 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     if (n < N) {
 #pragma unroll
         for (int m = 0; m < MR; m++)
-            if (m < M) C[(size_t)m * ldc + n] = acc[m];
+            if (m0 + m < M) C[(size_t)(m0 + m) * ldc + n] = acc[m];
+    }
+}
+
+// The same for some 9 to 200 rows, where the tile kernel has few blocks, each of which waits for one 16-wide slice of K at a time: the
+// stages of the kernel above, blocks of two warps with 16 rows each and 32 outputs.  A lane owns four rows and four outputs (rows
+// rg, rg + 4, ...; outputs cg, cg + 8, ...; 4 x 8 lanes), so that 16 bytes from shared memory, which take a quarter of their lines'
+// bandwidth even where lanes share them, serve 8 multiply-adds; both operands lie swizzled, and the lanes' distinct rows of one read
+// differ in the low three bits.  Every sum is the one chain over k again.  (32 rows to a warp, a lane with 8 x 4: 336 to 573 us where
+// this takes 212 to 443, 9 to 128 rows of 11008 x 4096: half as many warps, and code that does not stay in the instruction cache.)
+#define GM_KT 64
+#define GM_STAGES 4
+#define GM_RI 4
+#define GM_ROWS (8 * GM_RI)
+#define GM_STAGE_BYTES ((32 + GM_ROWS) * GM_KT * 4)
+
+__global__ void __launch_bounds__(64)
+gemm_f32_mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, float* __restrict__ C, int M, int N, int K,
+                    int ldc, int* __restrict__ err) {
+    extern __shared__ unsigned char gs_raw[];
+    __shared__ __align__(8) unsigned long long full[GM_STAGES];
+    constexpr int ROWS = GM_ROWS, BYTES = GM_STAGE_BYTES, BOX_W = 32 * 128, BOX_X = ROWS * 128, BOXES = GM_KT / 32;
+    const unsigned base = (tc_smem_u32(gs_raw) + 1023u) & ~1023u;
+    const unsigned char* gen = gs_raw + (base - tc_smem_u32(gs_raw));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cg = lane & 7, rg = lane >> 3, n0 = blockIdx.x * 32, m0 = blockIdx.y * ROWS;
+    const int n_tiles = (K + GM_KT - 1) / GM_KT;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < GM_STAGES; s++) mbar_init(tc_smem_u32(&full[s]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto issue_w = [&](int t) {
+        const unsigned bar = tc_smem_u32(&full[t % GM_STAGES]), to = base + t % GM_STAGES * BYTES;
+        mbar_expect_tx(bar, BYTES);
+#pragma unroll
+        for (int q = 0; q < BOXES; q++) tma_load_2d(to + q * BOX_W, &map_w, t * GM_KT + q * 32, n0, bar);
+    };
+    auto issue_x = [&](int t) {
+        const unsigned bar = tc_smem_u32(&full[t % GM_STAGES]), to = base + t % GM_STAGES * BYTES + BOXES * BOX_W;
+#pragma unroll
+        for (int q = 0; q < BOXES; q++) tma_load_2d(to + q * BOX_X, &map_a, t * GM_KT + q * 32, m0, bar);
+    };
+    const int n_pre = n_tiles < GM_STAGES - 1 ? n_tiles : GM_STAGES - 1;
+    if (threadIdx.x == 0)
+        for (int t = 0; t < n_pre; t++) issue_w(t);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (threadIdx.x == 0)
+        for (int t = 0; t < n_pre; t++) issue_x(t);
+    float acc[GM_RI][4];
+#pragma unroll
+    for (int i = 0; i < GM_RI; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
+    bool alive = true;
+    int t = 0;
+    for (; t < n_tiles; t++) {
+        // the stage that was read in the round before is free (the barrier below)
+        if (threadIdx.x == 0 && t + GM_STAGES - 1 < n_tiles) {
+            issue_w(t + GM_STAGES - 1);
+            issue_x(t + GM_STAGES - 1);
+        }
+        alive = __all_sync(0xffffffffu, mbar_wait(tc_smem_u32(&full[t % GM_STAGES]), (t / GM_STAGES) & 1, err));
+        const unsigned char *ws = gen + t % GM_STAGES * BYTES + cg * 128, *xs = gen + t % GM_STAGES * BYTES + BOXES * BOX_W + (warp * 4 * GM_RI + rg) * 128;
+        if (alive)
+#pragma unroll
+            for (int at = 0; at < GM_KT / 4; at++) {
+                const int q = at >> 3, c = at & 7;
+                float4 w[4], x[GM_RI];
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = *reinterpret_cast<const float4*>(ws + q * BOX_W + j * 1024 + ((c ^ cg) << 4));
+#pragma unroll
+                for (int i = 0; i < GM_RI; i++) x[i] = *reinterpret_cast<const float4*>(xs + q * BOX_X + i * 512 + ((c ^ ((i & 1) * 4 + rg)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int i = 0; i < GM_RI; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            acc[i][j] = fmaf(e == 0 ? x[i].x : e == 1 ? x[i].y : e == 2 ? x[i].z : x[i].w,
+                                             e == 0 ? w[j].x : e == 1 ? w[j].y : e == 2 ? w[j].z : w[j].w, acc[i][j]);
+            }
+        // the stage is refilled by the next round's requests (and a warp whose wait ran out takes the other with it)
+        alive = __syncthreads_and(alive);
+        if (!alive) break;
+    }
+    if (!alive) {
+        // no result; the copies in flight are waited for, each with a short limit, before the block gives its shared memory back
+        for (int u = t; u < n_tiles && u < t + GM_STAGES; u++) mbar_wait(tc_smem_u32(&full[u % GM_STAGES]), (u / GM_STAGES) & 1, err, TC_ERR_TIMEOUT, 1LL << 24);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < GM_RI; i++) {
+        const int m = m0 + warp * 4 * GM_RI + i * 4 + rg;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int n = n0 + j * 8 + cg;
+            if (m < M && n < N) C[(size_t)m * ldc + n] = acc[i][j];
+        }
     }
 }
 
@@ -302,7 +401,20 @@ static int launch_gemm_f32_small(const float* A, const float* W, float* C, int M
     auto kern = gemm_f32_small_kernel<MR>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GS_SMEM(MR));
     if (e != cudaSuccess) return (int)e;
-    illm_launch(kern, dim3((N + 31) / 32), dim3(32), (size_t)GS_SMEM(MR), s, mw, ma, C, M, N, K, ldc, err);
+    illm_launch(kern, dim3((N + 31) / 32, (M + MR - 1) / MR), dim3(32), (size_t)GS_SMEM(MR), s, mw, ma, C, M, N, K, ldc, err);
+    return illm_launch_status();
+}
+
+static int launch_gemm_f32_mid(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int* err, cudaStream_t s) {
+    CUtensorMap mw, ma;
+    int rc;
+    if ((rc = gs_make_map(&mw, W, N, K, ldw, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B)) != 0) return rc;
+    if ((rc = gs_make_map(&ma, A, M, K, lda, GM_ROWS, 32, CU_TENSOR_MAP_SWIZZLE_128B)) != 0) return rc;
+    auto kern = gemm_f32_mid_kernel;
+    constexpr int SMEM = GM_STAGES * GM_STAGE_BYTES + 1024;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return (int)e;
+    illm_launch(kern, dim3((N + 31) / 32, (M + GM_ROWS - 1) / GM_ROWS), dim3(64), (size_t)SMEM, s, mw, ma, C, M, N, K, ldc, err);
     return illm_launch_status();
 }
 
@@ -312,9 +424,12 @@ extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M,
                                 int lda, int ldw, int ldc, int* err, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return ILLM_ERR_BAD_ARG;
-    if (err != nullptr && M <= 8 && (K & 3) == 0 && (lda & 3) == 0 && (ldw & 3) == 0 &&
-        ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(W)) & 15) == 0) {
-        cudaStream_t s = (cudaStream_t)stream;
+    const int sms = illm_sm_count();
+    const bool staged = err != nullptr && (K & 3) == 0 && (lda & 3) == 0 && (ldw & 3) == 0 &&
+                        ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(W)) & 15) == 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    // (9 to 16 rows as two blocks of 8, while they all run at once)
+    if (staged && (M <= 8 || (M <= 16 && (N + 31) / 32 <= sms))) {
         if (M == 1) return launch_gemm_f32_small<1>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
         if (M == 2) return launch_gemm_f32_small<2>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
         if (M <= 4) return launch_gemm_f32_small<4>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
@@ -324,10 +439,13 @@ extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M,
     // rows beyond M: the tile with the least work on the busiest SM, per output 1 : 1.2 : 1.6.  (512 rows of 7B size: Q/K/V and
     // gate/up 47 TF/s, output and down products 41; over 294 shapes of 9 to 2,048 rows 0.55 of the time of one 64 x 64 tile of 4 x 4
     // outputs a thread, 0.83 where it gains least.)
-    cudaStream_t s = (cudaStream_t)stream;
-    const int sms = illm_sm_count();
     auto rounds = [&](long long bm, long long bn) { return (double)(((M + bm - 1) / bm * ((N + bn - 1) / bn) + sms - 1) / sms); };
     const double c0 = rounds(128, 128) * 128 * 128, c1 = rounds(64, 64) * 64 * 64 * 1.2, c2 = rounds(32, 64) * 32 * 64 * 1.6;
+    // Few tiles: the staged kernel by what both were measured to take for a step of k, in ns (48 to 96 rows of 11008 x 4096: 316 to 335 us
+    // instead of 466 to 500, 32 of 4096 x 4096 80 instead of 137; 128 of 4096 x 22016 would take 689 instead of 582).
+    const double least = c0 < c1 ? (c0 < c2 ? c0 : c2) : (c1 < c2 ? c1 : c2), blocks = (double)((N + 31) / 32) * ((M + GM_ROWS - 1) / GM_ROWS) / sms;
+    const double mid = 10 + 9.3 * blocks < 19.4 ? 19.4 : 10 + 9.3 * blocks;
+    if (staged && (M + GM_ROWS - 1) / GM_ROWS <= 65535 && mid < 12 + 5.3e-3 * least) return launch_gemm_f32_mid(A, W, C, M, N, K, lda, ldw, ldc, err, s);
     if (c0 <= c1 && c0 <= c2) return launch_gemm_f32_tile<128, 128, 8, 16>(A, W, C, M, N, K, lda, ldw, ldc, s);
     if (c1 <= c2) return launch_gemm_f32_tile<64, 64, 8, 4>(A, W, C, M, N, K, lda, ldw, ldc, s);
     return launch_gemm_f32_tile<32, 64, 4, 4>(A, W, C, M, N, K, lda, ldw, ldc, s);
