@@ -446,7 +446,7 @@ extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int
         return ad_float32((const float*)x, (const float*)w, T, N, K, (const float*)a, (const float*)b, scales, R, sz, plan, (float*)out, (float*)ws, err, s);
     if (dtype != ILLM_BF16 || (out_dtype != ILLM_BF16 && out_dtype != ILLM_F32)) return ILLM_ERR_BAD_ARG;
     if (ad_tiled(T, slots, N))
-        return ad_prompt_form(x, w, T, N, K, a, b, scales, count, R, ad_plan(plan, sz), chunks, out, out_dtype, (char*)ws, early, err, s);
+        return ad_prompt_form(x, w, T, N, K, a, b, scales, count, R, ad_plan(plan, sz), chunks, out, out_dtype, (char*)ws, err, s);
     if (out_dtype == ILLM_BF16) return ad_rows_form<bf16>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (bf16*)out, (char*)ws, early, err, s);
     return ad_rows_form<float>(x, w, T, N, K, a, b, scales, count, R, sz, plan, (float*)out, (char*)ws, early, err, s);
 }

@@ -56,4 +56,4 @@ static inline int ad_div(long long a, long long b) { return (int)((a + b - 1) / 
 // adapters_prompt.cu: the prompt form (bfloat16, a plan with tiles)
 long long ad_prompt_ws(int T, int N, int K, int chunks);
 int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R,
-                   const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int early, int* err, cudaStream_t s);
+                   const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int* err, cudaStream_t s);

@@ -504,8 +504,7 @@ static int ap_launch(int bn, const CUtensorMap& mx, const CUtensorMap& mw, const
 }
 
 int ad_prompt_form(const void* x, const void* w, int T, int N, int K, const void* a, const void* b, const float* scales, int count, int R,
-                   const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int early, int* err, cudaStream_t s) {
-    (void)early;
+                   const AdPlan& plan, int chunks, void* out, int out_dtype, char* ws, int* err, cudaStream_t s) {
     const ApShape shape = ap_shape(T, N, K, chunks);
     const int k_iters = ad_div(K, TC_BK), splits = shape.splits, bn = shape.bn, C = shape.C;
     bf16* v = (bf16*)ws;

@@ -918,9 +918,9 @@ def linear_adapters(x, w, adapters, rows, out_dtype=None):
     if T == 0:
         return out
     lib, code = load(), _DT[dtype]
-    ws = torch.empty((rows.ws_bytes(code, N, K, adapters.R),), dtype=torch.uint8, device=device)
     a, b, scales = adapters.pointers
     with _on(device):
+        ws = torch.empty((rows.ws_bytes(code, N, K, adapters.R),), dtype=torch.uint8, device=device)
         _check(lib.illm_linear_adapters(px, pw, code, T, N, K, a, b, scales, adapters.count, adapters.R, rows.plan_ptr, rows.slots, rows.groups, rows.chunks,
                                         out.data_ptr(), _DT[out_dtype], ws.data_ptr(), 0, _error_word(device), _stream()), "linear_adapters")
     return out
