@@ -324,3 +324,17 @@ def test_wide_products_of_33_to_64_tokens(T):
     for used in (1, 4, T // 4, T // 4 + 1):
         index = [t % used if t % 7 else -1 for t in range(T)]
         check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+
+
+@pytest.mark.parametrize("K,N", [(2752, 160), (1000, 2049), (2048, 4096), (260, 9000), (72, 130), (514, 300)])
+def test_float32_rows_by_any_kernel(K, N):
+    """A row's bits are the same in products of any number of rows, whichever kernel they take, and an infinite row stays alone."""
+    x, w, a, b, ad, s = make(200, K, N, [16, 5], torch.float32, K + N)
+    x[7, 3] = float("inf")
+    none = [ops.linear_adapters(x[t:t + 8].clone(), w, ad, ops.AdapterRows([-1] * len(x[t:t + 8]), ad.ranks)) for t in range(0, 200, 8)]
+    want = torch.cat(none)
+    for T in (9, 16, 17, 32, 33, 64, 65, 96, 128, 161, 200):
+        got = ops.linear_adapters(x[:T].clone(), w, ad, ops.AdapterRows([-1] * T, ad.ranks))
+        same = (got == want[:T]) | (got.isnan() & want[:T].isnan())
+        assert bool(same.all()), T
+        assert torch.isfinite(got[:7]).all()
