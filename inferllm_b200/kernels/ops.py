@@ -914,13 +914,14 @@ def linear_adapters(x, w, adapters, rows, out_dtype=None):
     px, pw = x.data_ptr(), w.data_ptr()
     if (px | pw) & 15 and (dtype == torch.bfloat16 or K % 4 == 0):
         raise KernelError("linear_adapters: x and w must start on a 16-byte boundary")
-    out = torch.empty((T, N), dtype=out_dtype, device=device)
+    # (new_empty with plain arguments: half the host's time of torch.empty, and a call of few tokens is bound by the host)
+    out = x.new_empty(T, N) if out_dtype is dtype else x.new_empty(T, N, dtype=out_dtype)
     if T == 0:
         return out
     lib, code = load(), _DT[dtype]
     a, b, scales = adapters.pointers
     with _on(device):
-        ws = torch.empty((rows.ws_bytes(code, N, K, adapters.R),), dtype=torch.uint8, device=device)
+        ws = x.new_empty(rows.ws_bytes(code, N, K, adapters.R), dtype=torch.uint8)
         _check(lib.illm_linear_adapters(px, pw, code, T, N, K, a, b, scales, adapters.count, adapters.R, rows.plan_ptr, rows.slots, rows.groups, rows.chunks,
                                         out.data_ptr(), _DT[out_dtype], ws.data_ptr(), 0, _error_word(device), _stream()), "linear_adapters")
     return out
@@ -1002,7 +1003,7 @@ def sample_rows(logits, uniforms, temp=None, top_k=None, top_p=None, min_p=None)
     u = _per_row(uniforms, "uniforms", torch.float32, B, device)
     settings = (_per_row(temp, "temp", torch.float32, B, device), _per_row(top_k, "top_k", torch.int32, B, device),
                 _per_row(top_p, "top_p", torch.float32, B, device), _per_row(min_p, "min_p", torch.float32, B, device))
-    out = torch.empty((B,), dtype=torch.int32, device=device)
+    out = logits.new_empty(B, dtype=torch.int32)
     with _on(device):
         _check(load().illm_sample_rows(logits.data_ptr(), _DT[logits.dtype], B, V, logits.stride(0) if B > 1 else V, u, *settings, out.data_ptr(),
                                        _stream()), "sample_rows")
