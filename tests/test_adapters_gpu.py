@@ -338,3 +338,16 @@ def test_float32_rows_by_any_kernel(K, N):
         same = (got == want[:T]) | (got.isnan() & want[:T].isnan())
         assert bool(same.all()), T
         assert torch.isfinite(got[:7]).all()
+
+
+@pytest.mark.parametrize("T,K,N", [(200, 4096, 6144), (512, 4096, 4096), (257, 1024, 1024), (1000, 4096, 6144), (2048, 1024, 1024), (2048, 4096, 4096),
+                                   (1024, 8192, 1024), (70, 11008, 4096), (200, 4096, 6143), (500, 4096, 4093), (257, 1024, 1021), (1000, 2048, 6139),
+                                   (1024, 8192, 1019)])
+def test_widths_of_tiles(T, K, N):
+    """Sizes for which the estimate takes tiles of every width, some with K in slices; outputs that fill no tile."""
+    ranks = [16, 40, 8]
+    x, w, a, b, ad, s = make(T, K, N, ranks, torch.bfloat16, T + N)
+    index = [(t // 37) % 4 - 1 for t in range(T)]
+    check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
+    one = [1] * T
+    check(ops.linear_adapters(x, w, ad, ops.AdapterRows(one, ad.ranks), torch.float32), x, w, a, b, s, one)
