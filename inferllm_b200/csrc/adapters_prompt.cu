@@ -17,7 +17,7 @@
 // wait for the tokens' rows is over, so the shared product may be read at once, and only the chunks wait.
 // Measured on one B200: 2,048 tokens of 4096 x 4096 with 12 adapters of mixed ranks 62 us (1,110 TFLOP/s, the product alone 51 to
 // 55), 4,096 of 4096 x 22016 with rank 64 569 us (1,320 TFLOP/s, 94 % of what the library's product keeps up), 200 of
-// 4096 x 6144 20.6 us, of which reading the weight takes 7.7.  Bound: the tensor cores from about 1,000 tokens on, below that
+// 4096 x 6144 20.2 us, of which reading the weight takes 7.7.  Bound: the tensor cores from about 1,000 tokens on, below that
 // the latency of launching, filling and draining two dependent kernels.
 #include "adapters.cuh"
 #include "kernels.h"
@@ -326,17 +326,31 @@ adapter_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 if (ti >= 2) alive = mbar_wait_warp(acc_empty0 + 8 * buf, ((ti >> 1) - 1) & 1, err);
                 tc_fence_after();
                 // (one thread issues every MMA of the pair: its loop over K holds nothing but waits and MMAs, and the chunks have
-                // their own; with a choice between the two inside, 4,096 tokens of 4096 x 22016 took 610 us instead of 479)
-                for (int k = k0; k < k1 && alive; k++) {
-                    alive = mbar_wait_warp(full0 + 8 * s, phase, err);
+                // their own; with a choice between the two inside, 4,096 tokens of 4096 x 22016 took 610 us instead of 479.  Two pieces
+                // to a round of it: 200 tokens of 2048 x 2048 9.6 us instead of 11.1, of 4096 x 6144 18.0 instead of 18.7)
+                auto multiply = [&](int stage, unsigned accumulate) {
+                    const unsigned long long da = da0 + stage * (A_BYTES >> 4), db = db0 + stage * (B_BYTES >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16_pair(d, da + 2 * kk, db + 2 * kk, IDESC, kk > 0 ? 1u : accumulate);
+                    umma_commit_pair(empty0 + 8 * stage);
+                };
+                int k = k0;
+                for (; k + 1 < k1 && alive; k += 2) {
+                    const int s2 = s + 1 == STAGES ? 0 : s + 1, phase2 = s2 == 0 ? phase ^ 1 : phase;
+                    alive = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase, err) && mbar_wait(full0 + 8 * s2, phase2, err));
                     if (!alive) break;
                     tc_fence_after();
-                    const unsigned long long da = da0 + s * (A_BYTES >> 4), db = db0 + s * (B_BYTES >> 4);
                     if (elected) {
-#pragma unroll
-                        for (int kk = 0; kk < TC_BK / 16; kk++) umma_bf16_pair(d, da + 2 * kk, db + 2 * kk, IDESC, (k > k0 || kk > 0) ? 1u : 0u);
-                        umma_commit_pair(empty0 + 8 * s);
+                        multiply(s, k > k0 ? 1u : 0u);
+                        multiply(s2, 1u);
                     }
+                    s = s2 + 1 == STAGES ? 0 : s2 + 1;
+                    phase = s == 0 ? phase2 ^ 1 : phase2;
+                }
+                if (k < k1 && alive) {
+                    alive = mbar_wait_warp(full0 + 8 * s, phase, err);
+                    tc_fence_after();
+                    if (elected && alive) multiply(s, k > k0 ? 1u : 0u);
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
                 for (int c = c0; c < c1 && alive; c++) {
