@@ -308,7 +308,11 @@ struct SrBlock {
         for (int c = 0; c < C; c++) v += sh.group_sum[c][lane];
         float upto = sr_warp_scan(v);
         const float whole = __shfl_sync(0xffffffffu, upto, 31), target = WEIGHTS ? share * whole : share;
-        if (!WEIGHTS && whole < target) return false;
+        if (!WEIGHTS && whole < target) {
+            // (the same in every block; the next histogram's sums go where slower warps still read these)
+            sr_cluster_sync();
+            return false;
+        }
         auto first_lane = [&](float m) {                // where the sum reaches the target, or the last with anything in it
             const unsigned reach = __ballot_sync(0xffffffffu, (upto >= target) & (m > 0.f)), some = __ballot_sync(0xffffffffu, m > 0.f);
             return reach ? __ffs(reach) - 1 : 31 - __clz(some | 1u);

@@ -246,3 +246,26 @@ def test_more_blocks_than_run_at_once(B, V):
     out = ops.sample_rows(logits, u, temp, top_k, top_p)
     want = torch.cat([ops.sample_rows(*[v[r:r + 16].contiguous() for v in (logits, u, temp, top_k, top_p)]) for r in range(0, B, 16)])
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V", [(200, 4099), (100, 9001), (16, 32000), (60, 32000), (40, 128256)])
+def test_fewer_words_than_top_k_with_top_p(B, V, dtype):
+    """Rows of 1 to 39 words that can come, a top_k of 40 and a top_p: the count over the words finds no cut, and a sum of weights
+    follows it at once.  On 2, 4 and 8 blocks to a row, few and more of them than run at once, the words all in one block's part
+    of the row or in every one, many calls with nothing between them."""
+    rng = np.random.default_rng(V + B)
+    host = np.full((B, V), -INF)
+    for r in range(B):
+        n = 1 + r % 39
+        at = rng.choice(V, n, replace=False) if r % 3 else (0 if r % 2 else V - 64) + rng.choice(64, n, replace=False)
+        host[r, at] = rng.standard_normal(n) * 2
+    logits = torch.from_numpy(host.astype(np.float32)).cuda().to(dtype)
+    u, top_p = rng.random(B).astype(np.float32).tolist(), [(0.9, 0.5, 0.99)[r % 3] for r in range(B)]
+    temp, top_k = [0.8] * B, [40] * B
+    check(logits, u, temp, top_k, top_p, [0.0] * B)
+    args = logits, f32(u), f32(temp), torch.tensor(top_k, dtype=torch.int32, device="cuda"), f32(top_p)
+    want = ops.sample_rows(*args)
+    got = [ops.sample_rows(*args) for _ in range(200)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in got)
