@@ -418,9 +418,9 @@ extern "C" long long illm_linear_adapters_ws(int dtype, int T, int N, int K, int
 }
 
 static int ad_float32(const float* x, const float* w, int T, int N, int K, const float* a, const float* b, const float* scales, int R,
-                      const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int* err, cudaStream_t s) {
+                      const AdapterPlanSizes& sz, const int* plan_dev, float* out, float* v, int early, int* err, cudaStream_t s) {
     const AdPlan plan = ad_plan(plan_dev, sz);
-    const int rc = illm_gemm_f32_nt(x, w, out, T, N, K, K, K, N, err, s);
+    const int rc = illm_gemm_f32_nt_ex(x, w, out, T, N, K, K, K, N, early, err, s);
     if (rc != 0) return rc;
     if (sz.slots == 0) return 0;
     const bool wide = K % 4 == 0 && !(((uintptr_t)x | (uintptr_t)a) & 15);
@@ -431,7 +431,8 @@ static int ad_float32(const float* x, const float* w, int T, int N, int K, const
 }
 
 // out [T, N] = x W^T + the tokens' adapters.  dtype: of x, W, A and B; out_dtype float32 or that.  plan: the device array laid
-// out by adapter_plan_layout({T, slots, groups, chunks}).  ws: illm_linear_adapters_ws bytes, 256-byte aligned.
+// out by adapter_plan_layout({T, slots, groups, chunks}).  ws: illm_linear_adapters_ws bytes, 256-byte aligned.  early: no kernel ahead in
+// the stream makes W, A or B, so that they may be read before the wait for it.
 extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int T, int N, int K, const void* a, const void* b, const float* scales,
                                     int count, int R, const int* plan, int slots, int groups, int chunks, void* out, int out_dtype, void* ws, int early,
                                     int* err, void* stream) {
@@ -443,7 +444,7 @@ extern "C" int illm_linear_adapters(const void* x, const void* w, int dtype, int
     const AdapterPlanSizes sz{T, slots, groups, chunks};
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == ILLM_F32 && out_dtype == ILLM_F32)
-        return ad_float32((const float*)x, (const float*)w, T, N, K, (const float*)a, (const float*)b, scales, R, sz, plan, (float*)out, (float*)ws, err, s);
+        return ad_float32((const float*)x, (const float*)w, T, N, K, (const float*)a, (const float*)b, scales, R, sz, plan, (float*)out, (float*)ws, early, err, s);
     if (dtype != ILLM_BF16 || (out_dtype != ILLM_BF16 && out_dtype != ILLM_F32)) return ILLM_ERR_BAD_ARG;
     if (ad_tiled(T, slots, N))
         return ad_prompt_form(x, w, T, N, K, a, b, scales, count, R, ad_plan(plan, sz), chunks, out, out_dtype, (char*)ws, err, s);

@@ -109,7 +109,8 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // Some kernels issue the two instructions by themselves and read what no kernel writes before the wait: weights (the product
 // kernels, the row kernels of norms, sums and q/k/v), and the step's positions, sequences and page table (the q/k/v preparation,
 // the ring kernel with the fused rotation), which the engine brings with a copy.  A caller of the raw entry points that makes
-// one of those with a kernel puts something between the two that is no such launch, or waits for that kernel.
+// one of those with a kernel puts something between the two that is no such launch, or waits for that kernel.  (The float32 products
+// and the products with adapters ask: their `early` says that no kernel makes the weights.)
 __device__ __forceinline__ void pdl_grid_sync() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

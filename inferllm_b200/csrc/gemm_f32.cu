@@ -177,7 +177,7 @@ static int launch_gemm_f32_tile(const float* A, const float* W, float* C, int M,
 // one fused multiply-add per k, starting from zero: the chain of the tile kernel, so the result is
 // the same bits.  A lane reads its own row of a box, 16 bytes at a time, at the swizzled place
 // (chunk c of row r lies at chunk c ^ (r & 7)): eight lanes then touch all 32 banks once.  The
-// weights are requested before the wait for the kernels ahead (they are nobody's result), the
+// weights are requested before the wait for the kernels ahead where the caller says that they are nobody's result (`early`), the
 // activations after it.  The waits are bounded like those of the tensor-core kernels.
 #define GS_STAGES(MR) ((MR) > 4 ? 5 : 6)             // two blocks per SM: at most 113 KB each
 #define GS_KT 128                                   // values of k per stage
@@ -187,7 +187,7 @@ static int launch_gemm_f32_tile(const float* A, const float* W, float* C, int M,
 template <int MR>
 __global__ void __launch_bounds__(32)
 gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                      float* __restrict__ C, int M, int N, int K, int ldc, int* __restrict__ err) {
+                      float* __restrict__ C, int M, int N, int K, int ldc, int early, int* __restrict__ err) {
     constexpr int S = GS_STAGES(MR);
     extern __shared__ unsigned char gs_raw[];
     __shared__ __align__(8) unsigned long long gs_full[S];
@@ -215,9 +215,11 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         tma_load_2d(x_base + s * X_BYTES, &map_a, t * GS_KT, m0, tc_smem_u32(&gs_full[s]));
     };
     const int n_pre = n_tiles < S - 1 ? n_tiles : S - 1;
+    // the first stages of the weights come before the wait only where no kernel ahead can have made them
+    if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (lane == 0)
         for (int t = 0; t < n_pre; t++) issue_w(t);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (lane == 0)
         for (int t = 0; t < n_pre; t++) issue_x(t);
     float acc[MR];
@@ -281,7 +283,7 @@ gemm_f32_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
 __global__ void __launch_bounds__(64)
 gemm_f32_mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, float* __restrict__ C, int M, int N, int K,
-                    int ldc, int* __restrict__ err) {
+                    int ldc, int early, int* __restrict__ err) {
     extern __shared__ unsigned char gs_raw[];
     __shared__ __align__(8) unsigned long long full[GM_STAGES];
     constexpr int ROWS = GM_ROWS, BYTES = GM_STAGE_BYTES, BOX_W = 32 * 128, BOX_X = ROWS * 128, BOXES = GM_KT / 32;
@@ -308,9 +310,10 @@ gemm_f32_mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int q = 0; q < BOXES; q++) tma_load_2d(to + q * BOX_X, &map_a, t * GM_KT + q * 32, m0, bar);
     };
     const int n_pre = n_tiles < GM_STAGES - 1 ? n_tiles : GM_STAGES - 1;
+    if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0)
         for (int t = 0; t < n_pre; t++) issue_w(t);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0)
         for (int t = 0; t < n_pre; t++) issue_x(t);
     float acc[GM_RI][4];
@@ -393,7 +396,7 @@ static int gs_make_map(CUtensorMap* map, const float* ptr, long long rows, long 
 
 template <int MR>
 static int launch_gemm_f32_small(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc,
-                                 int* err, cudaStream_t s) {
+                                 int early, int* err, cudaStream_t s) {
     CUtensorMap mw, ma;
     int rc;
     if ((rc = gs_make_map(&mw, W, N, K, ldw, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B)) != 0) return rc;
@@ -401,11 +404,11 @@ static int launch_gemm_f32_small(const float* A, const float* W, float* C, int M
     auto kern = gemm_f32_small_kernel<MR>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GS_SMEM(MR));
     if (e != cudaSuccess) return (int)e;
-    illm_launch(kern, dim3((N + 31) / 32, (M + MR - 1) / MR), dim3(32), (size_t)GS_SMEM(MR), s, mw, ma, C, M, N, K, ldc, err);
+    illm_launch(kern, dim3((N + 31) / 32, (M + MR - 1) / MR), dim3(32), (size_t)GS_SMEM(MR), s, mw, ma, C, M, N, K, ldc, early, err);
     return illm_launch_status();
 }
 
-static int launch_gemm_f32_mid(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int* err, cudaStream_t s) {
+static int launch_gemm_f32_mid(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int early, int* err, cudaStream_t s) {
     CUtensorMap mw, ma;
     int rc;
     if ((rc = gs_make_map(&mw, W, N, K, ldw, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B)) != 0) return rc;
@@ -414,14 +417,15 @@ static int launch_gemm_f32_mid(const float* A, const float* W, float* C, int M, 
     constexpr int SMEM = GM_STAGES * GM_STAGE_BYTES + 1024;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
-    illm_launch(kern, dim3((N + 31) / 32, (M + GM_ROWS - 1) / GM_ROWS), dim3(64), (size_t)SMEM, s, mw, ma, C, M, N, K, ldc, err);
+    illm_launch(kern, dim3((N + 31) / 32, (M + GM_ROWS - 1) / GM_ROWS), dim3(64), (size_t)SMEM, s, mw, ma, C, M, N, K, ldc, early, err);
     return illm_launch_status();
 }
 
 // err: the device's error word for the bounded waits of the few-rows kernel (null: that kernel is
-// not used and every size takes the tile kernel).
-extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M, int N, int K,
-                                int lda, int ldw, int ldc, int* err, void* stream) {
+// not used and every size takes the tile kernel).  early: no kernel ahead in the stream makes W, so that the staged kernels may read
+// it before their wait (an engine's weights); 0: any order of kernels is kept.
+extern "C" int illm_gemm_f32_nt_ex(const float* A, const float* W, float* C, int M, int N, int K,
+                                   int lda, int ldw, int ldc, int early, int* err, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return ILLM_ERR_BAD_ARG;
     const int sms = illm_sm_count();
@@ -430,10 +434,10 @@ extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M,
     cudaStream_t s = (cudaStream_t)stream;
     // (9 to 16 rows as two blocks of 8, while they all run at once)
     if (staged && (M <= 8 || (M <= 16 && (N + 31) / 32 <= sms))) {
-        if (M == 1) return launch_gemm_f32_small<1>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
-        if (M == 2) return launch_gemm_f32_small<2>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
-        if (M <= 4) return launch_gemm_f32_small<4>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
-        return launch_gemm_f32_small<8>(A, W, C, M, N, K, lda, ldw, ldc, err, s);
+        if (M == 1) return launch_gemm_f32_small<1>(A, W, C, M, N, K, lda, ldw, ldc, early, err, s);
+        if (M == 2) return launch_gemm_f32_small<2>(A, W, C, M, N, K, lda, ldw, ldc, early, err, s);
+        if (M <= 4) return launch_gemm_f32_small<4>(A, W, C, M, N, K, lda, ldw, ldc, early, err, s);
+        return launch_gemm_f32_small<8>(A, W, C, M, N, K, lda, ldw, ldc, early, err, s);
     }
     // A larger thread tile reads less shared memory per FMA, a smaller block leaves fewer SMs idle in the last round and fewer
     // rows beyond M: the tile with the least work on the busiest SM, per output 1 : 1.2 : 1.6.  (512 rows of 7B size: Q/K/V and
@@ -445,8 +449,11 @@ extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M,
     // instead of 466 to 500, 32 of 4096 x 4096 80 instead of 137; 128 of 4096 x 22016 would take 689 instead of 582).
     const double least = c0 < c1 ? (c0 < c2 ? c0 : c2) : (c1 < c2 ? c1 : c2), blocks = (double)((N + 31) / 32) * ((M + GM_ROWS - 1) / GM_ROWS) / sms;
     const double mid = 10 + 9.3 * blocks < 19.4 ? 19.4 : 10 + 9.3 * blocks;
-    if (staged && (M + GM_ROWS - 1) / GM_ROWS <= 65535 && mid < 12 + 5.3e-3 * least) return launch_gemm_f32_mid(A, W, C, M, N, K, lda, ldw, ldc, err, s);
+    if (staged && (M + GM_ROWS - 1) / GM_ROWS <= 65535 && mid < 12 + 5.3e-3 * least) return launch_gemm_f32_mid(A, W, C, M, N, K, lda, ldw, ldc, early, err, s);
     if (c0 <= c1 && c0 <= c2) return launch_gemm_f32_tile<128, 128, 8, 16>(A, W, C, M, N, K, lda, ldw, ldc, s);
     if (c1 <= c2) return launch_gemm_f32_tile<64, 64, 8, 4>(A, W, C, M, N, K, lda, ldw, ldc, s);
     return launch_gemm_f32_tile<32, 64, 4, 4>(A, W, C, M, N, K, lda, ldw, ldc, s);
+}
+extern "C" int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int* err, void* stream) {
+    return illm_gemm_f32_nt_ex(A, W, C, M, N, K, lda, ldw, ldc, 0, err, stream);
 }

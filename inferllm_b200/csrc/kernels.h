@@ -108,6 +108,7 @@ long long illm_launch_count();
 
 // gemm_f32.cu
 int illm_gemm_f32_nt(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int* err, void* stream);
+int illm_gemm_f32_nt_ex(const float* A, const float* W, float* C, int M, int N, int K, int lda, int ldw, int ldc, int early, int* err, void* stream);
 
 // gemm_tc.cu
 int illm_gemm_bf16_tc_tune(int stages);

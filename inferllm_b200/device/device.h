@@ -48,6 +48,10 @@ public:
     // memory (6.6e6 on a B200).  The policies that weigh a kernel's stream against its fixed costs use it.
     double stream_bytes_per_us() const { return stream_bytes_per_us_; }
     cudaStream_t stream() const { return stream_; }
+    // Whether weights are there before any kernel on the stream runs, so that a product may read them before its wait for the kernels
+    // ahead of it: an engine's are; what a caller of single operators multiplies by may be the result of the call before.
+    bool weights_settled() const { return weights_settled_; }
+    void set_weights_settled(bool on) { weights_settled_ = on; }
     void set_stream(cudaStream_t s);
     // Ordering against another stream of the same device (a caller that exchanges device memory with
     // the engine works on its own stream): this stream waits for what `other` holds now / `other` waits
@@ -103,7 +107,7 @@ private:
     int ordinal_, n_sms_ = 148;
     double stream_bytes_per_us_ = 6.6e6;
     cudaStream_t stream_ = nullptr;
-    bool own_stream_ = false;
+    bool own_stream_ = false, weights_settled_ = false;
     Lane lanes_[kLanes];
     int lane_ = 0;
     unsigned long long arena_generation_ = 0;

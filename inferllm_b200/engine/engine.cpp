@@ -53,6 +53,7 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     if (options.max_adapters > 0 && (options.adapter_rank < 1 || options.adapter_rank > ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces))
         throw EngineError("adapter_rank must be in [1, " + std::to_string(ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces) + "]");
     device_.reset(new Device(options.device_id, (cudaStream_t)options.stream));
+    device_->set_weights_settled(true);
     rt_.dev = device_.get();
     rt_.dtype = dtype;
     rt_.page_size = options.page_size;

@@ -304,8 +304,8 @@ Mat gemm_f32(Device& dev, const Mat& x, const Mat& w) {
     Mat out = new_mat_exact(dev, M, N, DType::F32);
     for (long long m0 = 0; m0 < M; m0 += 65535LL * 64) {
         const long long m1 = std::min(M, m0 + 65535LL * 64);
-        check_kernel(illm_gemm_f32_nt((const float*)row_ptr(x, m0), (const float*)w.p, (float*)row_ptr(out, m0), (int)(m1 - m0), (int)N, (int)K,
-                                      (int)K, (int)K, (int)N, dev.tc_error_word(), dev.stream()),
+        check_kernel(illm_gemm_f32_nt_ex((const float*)row_ptr(x, m0), (const float*)w.p, (float*)row_ptr(out, m0), (int)(m1 - m0), (int)N, (int)K,
+                                         (int)K, (int)K, (int)N, dev.weights_settled(), dev.tc_error_word(), dev.stream()),
                      "gemm_f32");
     }
     return out;
@@ -430,8 +430,8 @@ Mat linear_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& s
     const int code = code_of(x.dtype, "linear_adapters");
     void* ws = dev.alloc((size_t)illm_linear_adapters_ws(code, (int)T, (int)N, (int)K, set.R, view.sizes.slots, view.sizes.groups, view.sizes.chunks));
     check_kernel(illm_linear_adapters(x.p, w.p, code, (int)T, (int)N, (int)K, set.a, set.b, set.scales, set.count, set.R, view.plan, view.sizes.slots,
-                                      view.sizes.groups, view.sizes.chunks, out.p, code_of(out_dtype, "linear_adapters"), ws, 1, dev.tc_error_word(),
-                                      dev.stream()),
+                                      view.sizes.groups, view.sizes.chunks, out.p, code_of(out_dtype, "linear_adapters"), ws, dev.weights_settled(),
+                                      dev.tc_error_word(), dev.stream()),
                  "linear_adapters");
     return out;
 }
@@ -1168,8 +1168,9 @@ MatOrPartials group_linear(Device& dev, GemmBackend backend, const Mat& x, long 
         long long row = 0;
         for (long long g = 0; g < G; row += n[g++])
             for (long long m0 = 0; m0 < M; m0 += 65535LL * 64)
-                check_kernel(illm_gemm_f32_nt((const float*)row_ptr(x, g * group_rows + m0), (const float*)row_ptr(w, row), (float*)row_ptr(r.m, m0) + row,
-                                              (int)std::min(M - m0, 65535LL * 64), n[g], (int)K, (int)K, (int)K, (int)N, dev.tc_error_word(), dev.stream()),
+                check_kernel(illm_gemm_f32_nt_ex((const float*)row_ptr(x, g * group_rows + m0), (const float*)row_ptr(w, row), (float*)row_ptr(r.m, m0) + row,
+                                                 (int)std::min(M - m0, 65535LL * 64), n[g], (int)K, (int)K, (int)K, (int)N, dev.weights_settled(),
+                                                 dev.tc_error_word(), dev.stream()),
                              "gemm_f32");
         return r;
     }

@@ -192,8 +192,7 @@ MatOrPartials linear(Device& dev, GemmBackend backend, const Mat& x, const Mat& 
 Mat linear_gated(Device& dev, GemmBackend backend, const Mat& x, const Mat& w, int act = 1 /* kActSilu */, float act_limit = 0.f);
 
 // x [T, K] . w [N, K]^T plus every token's adapter, scale_a (x[t] . a_a^T) . b_a^T, in one float32 sum, rounded once: few tokens as
-// further rows of the weight, prompts as a longer K, float32 behind the product (csrc/adapters.cu, adapters_prompt.cu).  The weights
-// and the adapters must not come from the kernel that runs before.
+// further rows of the weight, prompts as a longer K, float32 behind the product (csrc/adapters.cu, adapters_prompt.cu).
 Mat linear_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, DType out_dtype);
 // act(gate) * up of it, for a weight whose rows 2i, 2i + 1 are the gate and the up row of output i.
 Mat linear_gated_adapters(Device& dev, const Mat& x, const Mat& w, const AdapterSet& set, const AdapterView& view, int act, float act_limit);

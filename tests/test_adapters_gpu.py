@@ -351,3 +351,49 @@ def test_widths_of_tiles(T, K, N):
     check(ops.linear_adapters(x, w, ad, ops.AdapterRows(index, ad.ranks)), x, w, a, b, s, index)
     one = [1] * T
     check(ops.linear_adapters(x, w, ad, ops.AdapterRows(one, ad.ranks), torch.float32), x, w, a, b, s, one)
+
+
+@pytest.mark.parametrize("T", [1, 3, 8, 12, 16, 40, 100, 150, 300])
+def test_a_weight_that_the_call_before_makes(T):
+    """A float32 weight filled by the kernel just before each product, new numbers every time and nothing between the calls: the
+    products, which let the weights come before the activations in an engine, wait for it."""
+    K, N, n = 512, 4096, 40
+    g = torch.Generator("cuda").manual_seed(T)
+    x = torch.randn((T, K), generator=g, device="cuda")
+    ad = ops.Adapters(1, 16, N, K, torch.float32)
+    rows = ops.AdapterRows([-1] * T, ad.ranks)
+    w = torch.empty((N, K), device="cuda")
+    calls = [lambda: ops.linear_adapters(x, w, ad, rows), lambda: ops.gemm_f32(x, w), lambda: ops.linear(x, w)]
+    want = []
+    for i in range(n):
+        ops.fill_random(w, 1000 * T + i, 1.0)
+        torch.cuda.synchronize()
+        want.append(ops.gemm_f32(x, w))
+        torch.cuda.synchronize()
+    for call in calls:
+        got = []
+        for i in range(n):
+            ops.fill_random(w, 1000 * T + i, 1.0)
+            got.append(call())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("T", [1, 20, 70, 128, 200, 600])
+def test_a_bfloat16_weight_that_the_call_before_makes(T):
+    """The same with adapters, in each form of the bfloat16 product."""
+    K, N, n = 1024, 4096, 40
+    x, _, _, _, ad, _ = make(T, K, N, [16, 40], torch.bfloat16, T)
+    rows = ops.AdapterRows([t % 3 - 1 for t in range(T)], ad.ranks)
+    w = torch.empty((N, K), dtype=torch.bfloat16, device="cuda")
+    want, got = [], []
+    for i in range(n):
+        ops.fill_random(w, 1000 * T + i, 1.0)
+        torch.cuda.synchronize()
+        want.append(ops.linear_adapters(x, w, ad, rows))
+        torch.cuda.synchronize()
+    for i in range(n):
+        ops.fill_random(w, 1000 * T + i, 1.0)
+        got.append(ops.linear_adapters(x, w, ad, rows))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
