@@ -22,7 +22,7 @@ class EngineOptions:
     dtype: str = "bfloat16"        # "bfloat16": serving kernels; "float32": everything in true 32-bit
     device_id: int = 0
     max_tokens: Optional[int] = 4096    # tokens that live sequences may hold together (sizes the cache);
-                                        # None: what `mem_fraction` of the memory left beside the weights holds
+                                        # None: what `mem_fraction` of the memory left beside the weights and the adapters holds
     mem_fraction: float = 0.9
     max_seq_len: Optional[int] = None   # longest sequence; default the model's max positions
     max_batch: Optional[int] = None     # slots; default max_tokens / page_size

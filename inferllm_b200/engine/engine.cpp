@@ -61,6 +61,12 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     model_.reset(new DecoderModel(config_->model_spec(), &rt_));
     const ModelSpec& spec = model_->spec;
     const long long max_seq = std::min(options.max_seq_len > 0 ? options.max_seq_len : spec.max_positions, spec.max_positions);
+    // (before the cache, which may take its share of what is left)
+    if (options.max_adapters > 0) {
+        if (model_->adapted().empty()) throw EngineError("max_adapters: no layer of this model runs low-rank adapters");
+        model_->make_adapters(options.max_adapters, options.adapter_rank);
+        adapter_ranks_.assign((size_t)options.max_adapters, 0);
+    }
     long long max_tokens = options.max_tokens;
     if (max_tokens <= 0) max_tokens = tokens_that_fit(options.mem_fraction);
     const int num_pages = (int)std::max<long long>(1, ceil_div(max_tokens, options.page_size));
@@ -68,11 +74,6 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     cache_.reset(new SequenceCache(model_->cache_requests(), num_slots, num_pages, options.page_size, max_seq, device_.get(), dtype,
                                    options.poison_freed_pages));
     builder_.reset(new StepContextBuilder(device_.get(), &rt_));
-    if (options.max_adapters > 0) {
-        if (model_->adapted().empty()) throw EngineError("max_adapters: no layer of this model runs low-rank adapters");
-        model_->make_adapters(options.max_adapters, options.adapter_rank);
-        adapter_ranks_.assign((size_t)options.max_adapters, 0);
-    }
     for (TokRead& t : tok_reads_) check_cuda(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming), "cudaEventCreate");
     // say once which attention kernels the model's layers get: a head size that the tensor-core kernels
     // do not take falls to the general kernel, which is right but far slower on prompts
@@ -138,8 +139,8 @@ long long Engine::tokens_that_fit(double fraction) const {
     const double room = ((double)free_b - (double)weights) * fraction;
     if (room < (double)per_token * options_.page_size) {
         char msg[200];
-        snprintf(msg, sizeof msg, "the weights (%.1f GiB) leave no room for a cache on this device (%.1f GiB free)",
-                 weights / 1073741824.0, free_b / 1073741824.0);
+        snprintf(msg, sizeof msg, "the weights (%.1f GiB) leave no room for a cache on this device (%.1f GiB free%s)",
+                 weights / 1073741824.0, free_b / 1073741824.0, options_.max_adapters > 0 ? " beside the room for adapters" : "");
         throw EngineError(msg);
     }
     return (long long)(room / (double)per_token);

@@ -26,7 +26,7 @@ struct EngineOptions {
     std::string dtype = "bfloat16";     // "bfloat16": serving kernels; "float32": everything in true 32-bit
     int device_id = 0;
     long long max_tokens = 4096;        // tokens that live sequences may hold together (sizes the cache);
-                                        // <= 0: what mem_fraction of the memory left beside the weights holds
+                                        // <= 0: what mem_fraction of the memory left beside the weights and the room for adapters holds
     double mem_fraction = 0.9;
     long long max_seq_len = 0;          // longest sequence; 0: the model's max positions
     int max_batch = 0;                  // slots; 0: max_tokens / page_size

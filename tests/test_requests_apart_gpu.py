@@ -320,3 +320,25 @@ def test_captured_steps_of_72_sequences(max_adapters, model_folders, plain_model
         got = e.step([StepItem(x, [p[j]], [0], -1 if x % 4 == 3 else x % 4) for x in slots]).cpu().numpy()
         for i, x in enumerate(slots):
             assert_close(got[i:i + 1], want[x % 4][j:j + 1], "bfloat16", f"sequence {x}, token {j}")
+
+
+def test_cache_sized_from_the_memory_that_adapters_leave(model_folders):
+    """Where the cache takes a share of the free memory, it is of what the room for adapters leaves."""
+    import gc
+
+    def made(**kw):
+        """Pages of the cache, and bytes of device memory that the engine took."""
+        gc.collect()
+        torch.cuda.empty_cache()
+        free = torch.cuda.mem_get_info()[0]
+        e = Engine.from_folder(model_folders["C"], EngineOptions(dtype="bfloat16", max_batch=4, adapter_rank=85, **kw))
+        out = e.limits().num_pages, free - torch.cuda.mem_get_info()[0]
+        del e
+        return out
+
+    made(max_tokens=64)
+    room = made(max_tokens=64, max_adapters=4096)[1] - made(max_tokens=64)[1]
+    page = 64 * 2 * 2 * 2 * 128 * 2         # tokens, layers, keys and values, heads, channels, bytes
+    assert room > 10e9
+    without, beside = made(max_tokens=None, mem_fraction=0.05)[0], made(max_tokens=None, mem_fraction=0.05, max_adapters=4096)[0]
+    assert abs((without - beside) * page - 0.05 * room) < 0.1 * 0.05 * room
