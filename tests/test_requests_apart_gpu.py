@@ -342,3 +342,61 @@ def test_cache_sized_from_the_memory_that_adapters_leave(model_folders):
     assert room > 10e9
     without, beside = made(max_tokens=None, mem_fraction=0.05)[0], made(max_tokens=None, mem_fraction=0.05, max_adapters=4096)[0]
     assert abs((without - beside) * page - 0.05 * room) < 0.1 * 0.05 * room
+
+
+def test_requests_that_end_at_different_times(model_folders):
+    """Settings, windows of last tokens and adapters of their own while requests leave the batch one after another, against one
+    request at a time with its choices written out (float32: the logits do not depend on the batch)."""
+    name, n_new = "B", 12
+    m = Model(ModelConfig(compt_type="float32", nr_ctx=TINY[name]["max_position_embeddings"], max_tokens=2048, max_adapters=3, adapter_rank=8))
+    m.load(model_folders[name])
+    m.init(top_k=0, top_p=1.0, temp=0.0, repeat_penalty=1.0, repeat_last_n=0, seed=0, end_token=-1)
+    import plain_llama
+    cfg, w = plain_llama.load_weights(model_folders[name])
+    numbers = [m.engine.add_adapter(*factors(cfg, w, 8, s)) for s in (3, 6)]
+    prompts = [random_prompt(name, n, 400 + n) for n in (9, 30, 4, 17, 22, 6, 13)]
+    which = [numbers[i % 3] if i % 3 < 2 else -1 for i in range(7)]
+    each = [SamplingParams(temp=(0.0, 0.8, 1.2, 1.0)[i % 4], top_k=(0, 30)[i % 2], top_p=(1.0, 0.9, 0.7)[i % 3], min_p=(0.0, 0.03)[i // 2 % 2], seed=20 + i,
+                           repeat_penalty=(1.4, 1.0, 2.0, 0.7)[(i + 1) % 4], repeat_last_n=(5, 0)[(i + 1) % 4 == 1]) for i in range(7)]
+
+    def alone(r, stop):
+        slot, history, out = m.engine.new_sequence(), list(prompts[r]), []
+        feed = history
+        for step in range(n_new):
+            logits = m.engine.step([StepItem(slot, feed, [len(feed) - 1], which[r])])[0].cpu().numpy()
+            out.append(expect(logits, each[r], r, step, history))
+            history, feed = history + out[-1:], out[-1:]
+            if out[-1] in stop:
+                break
+        m.engine.end_sequence(slot)
+        return out
+
+    free = m.generate(prompts, max_new_tokens=n_new, stop_ids=[], sampling=each, adapters=which)
+    assert free.tokens == [alone(r, ()) for r in range(7)]
+    stop = {free.tokens[r][at] for r, at in ((0, 2), (3, 0), (4, 5), (6, 8), (1, 3))}
+    got = m.generate(prompts, max_new_tokens=n_new, stop_ids=sorted(stop), sampling=each, adapters=which)
+    assert got.tokens == [alone(r, stop) for r in range(7)]
+    assert len({len(t) for t in got.tokens}) >= 4
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("max_adapters", [30, 64])
+def test_many_sequences_with_many_adapters(max_adapters, dtype, model_folders, plain_models):
+    """Single tokens of 150 sequences with 30 adapters among them, then of ever fewer of these."""
+    name, n, used = "A", 150, 30
+    cfg, w = plain_models[name]
+    e = Engine.from_folder(model_folders[name], EngineOptions(dtype=dtype, max_tokens=n * 64, max_batch=n, max_adapters=max_adapters, adapter_rank=12))
+    adapters = [factors(cfg, w, 12, s) for s in range(used)]
+    for a in adapters:
+        e.add_adapter(*a)
+    p = random_prompt(name, 9, 4)
+    which = [(x * 7) % (used + 1) - 1 for x in range(n)]
+    want = [plain.forward(cfg, merged(w, a), p) for a in adapters + [None]]
+    slots = [e.new_sequence() for _ in range(n)]
+    for s in range(0, n, 50):
+        e.step([StepItem(x, p[:1], [], which[x]) for x in slots[s:s + 50]])
+    for j, live in ((1, 150), (2, 150), (3, 150), (4, 130), (5, 120), (6, 61), (7, 60), (8, 2)):
+        got = e.step([StepItem(x, [p[j]], [0], which[x]) for x in slots[:live]]).cpu().numpy()
+        for i in range(live):
+            assert_close(got[i:i + 1], want[which[i]][j:j + 1], dtype, f"sequence {i}, token {j}")
+    e.check_device_errors()
