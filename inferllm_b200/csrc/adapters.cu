@@ -394,10 +394,12 @@ static int ad_rows_form(const void* x, const void* w, int T, int N, int K, const
         illm_launch(kern, dim3(ad_div(N, AD_COLS), ad_div(T, tok)), dim3(AD_COLS), 0, s, (const float*)base, r.splits, (long long)T * N, N, (const bf16*)b,
                     (const float*)vs, v_ld, scales, R, plan.places, T, out);
     };
-    // A place to a block while that makes no more than some 14 blocks to an SM, else four.  One and four, us: 32 tokens with 8
-    // adapters of rank 64 beside 4096 x 4096 13.4 and 15.1; 64 tokens with 48 adapters, their factors in memory, beside 11008 x 4096
-    // 31.4 and 34.2 (with 8 in L2 32.1 and 30.5); 16 tokens with 64 of rank 16 beside 4096 x 22016 41.4 and 38.8.
-    if (T * ad_div(N, AD_COLS) < 14 * illm_sm_count()) join(adapter_join_kernel<1, TOut>, 1);
+    // A place to a block while that makes no more than some 11 blocks to an SM, else four.  One and four, us, L2 flushed, 4096 x N: 32
+    // tokens of 4096 with 8 adapters of rank 64 19.0 and 20.8; of 6144 (10.4 blocks) with 32 of rank 16 20.6 and 20.7, of rank 64 28.5
+    // and 30.3; 64 tokens of 3584 (12.1 blocks) with 64 of rank 16 20.8 and 18.9, of rank 64 31.8 and 31.8; of 4096 (13.8) 22.9 and 20.7,
+    // 33.4 and 33.2; of 5120 25.0 and 22.8, 36.6 and 37.1.  (Mixed ranks fill four places unevenly: 64 tokens with 48 adapters of 11008 x
+    // 4096 43.6 both ways, with the host between calls 31.4 and 33.2; far beyond the border they gain by one: of 4096 x 8192 37.5 and 40.3.)
+    if (T * ad_div(N, AD_COLS) < 11 * illm_sm_count()) join(adapter_join_kernel<1, TOut>, 1);
     else join(adapter_join_kernel<4, TOut>, 4);
     return illm_launch_status();
 }
