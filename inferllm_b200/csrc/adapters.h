@@ -21,7 +21,8 @@ struct AdapterPlanSizes {
 // Whether a step's products in bfloat16 may run as a prompt's, by tiles of tokens (the plan then has chunks): where there are more
 // tokens than the rows form takes, or at least four to an adapter.
 static inline bool adapter_tiled(int T, int slots) { return T > ADAPTER_ROWS_MAX || (T > 32 && 4 * slots <= T); }
-// Places of the arrays in the plan; each starts on a 16-byte boundary.
+// Places of the arrays in the plan; each starts on a 16-byte boundary.  The kernels read counts[1] and [2], token_adapter, places, groups
+// and the tiles' arrays; the other counts and the slots' arrays say the same by slot, for whoever reads a plan on the host.
 struct AdapterPlanLayout {
     int counts;                   // [4] slots, rank groups, chunks that there really are, and the most groups of a slot
     int token_adapter;            // [T] adapter of a token, -1: none

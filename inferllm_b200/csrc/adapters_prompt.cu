@@ -467,11 +467,14 @@ static int ap_values_blocks(int items, int chunks, int k_iters, int splits) {
     return chunks * 2 * c > idle || ad_div(k_iters, c) > ad_div(k_iters, splits) ? share(2 * illm_sm_count()) : c;
 }
 
-// The least of an estimate in us over widths of 96 to 256 and up to 4 slices.  A pair of SMs takes max(0.18, 0.045 + 0.0011 width) for
-// a piece of 64 (from 96 on it is bound by the waits and the issue of the pieces), the tiles come in rounds of as many as there are
+// The least of an estimate in us over widths of 96 to 256 and up to 4 slices.  A pair of SMs counts max(0.18, 0.045 + 0.0011 width) for
+// a piece of 64 (the narrow ones are bound by the waits and the issue of the pieces; measured before the multiplying warp took two
+// to a round, which leaves the order of the widths), the tiles come in rounds of as many as there are
 // pairs; the values of the last chunk take 3 and 0.42 a piece, beside it or before it; slices cost their kernel, 2, and their bytes twice.
 // Measured with 256 wide tiles (with slices where they do not fill the pairs) and with the choice: 200 tokens of 4096 x 6144 29.0
-// and 18.7 us, 512 of 4096 x 4096 24.9 and 18.8, 1,000 of 4096 x 6144 47.2 and 42.3, 257 of 1024 x 1024 14.8 and 9.3.
+// and 18.7 us, 512 of 4096 x 4096 24.9 and 18.8, 1,000 of 4096 x 6144 47.2 and 42.3, 257 of 1024 x 1024 14.8 and 9.3.  Against the
+// best of all widths and slices over 14 sizes of 150 to 2,048 tokens, replayed behind a flush of L2: up to 3 % more in 13 of them, 12 %
+// (17.9 and 16.0 us) at 257 of 1024 x 1024.
 static ApShape ap_shape(int T, int N, int K, int chunks) {
     const int k_iters = ad_div(K, TC_BK), pairs = illm_sm_count() / 2;
     ApShape best{256, 1, 1};

@@ -10,7 +10,8 @@
 // T <= 0: the lowest id among the maxima.  A row with no word at all gives -1.
 //
 // All three cuts are prefixes of one order, so a cut is one pair (key, id): an element is kept if its order-preserving
-// integer key is above the cut's, or equal and its id not above the cut's.  Nothing is sorted; a cut is found by bisection.
+// integer key is above the cut's, or equal and its id not above the cut's.  The row is not sorted: a histogram says in which bin a cut
+// falls, and the bin's words are ranked (only where they are very many, a bisection takes them).
 //
 // Sums.  A vocabulary of 128k words has neighbouring partial sums nearer than float32 tells apart, and a sum whose order
 // depends on timing would move a choice.  Weights are therefore made in float64 (2^(i/16) from a table times Taylor's series
@@ -821,8 +822,9 @@ extern "C" int illm_sample_rows(const void* logits, int dtype, int B, int V, lon
     if (B <= 0) return 0;
     if (V <= 0 || V > SR_MAX_CLUSTER * SR_MAX_RESIDENT || B > (1 << 24) || ld < V || !logits || !uniforms || !out) return ILLM_ERR_BAD_ARG;
     // blocks to a row: more while there are fewer than two to an SM (which is what its registers hold) and a block's run is worth a
-    // block, or is more than two of them on an SM can keep.  256 rows of 32,000 words on 1, 2, 4, 8 blocks each: 72, 64, 76, 107 us;
-    // one row: 25, 21, 17, 16; 64 rows of 128,256 words on 4 and 8: 80 and 74.
+    // block, or is more than two of them on an SM can keep.  Mixed settings, a replayed graph behind a flush of L2: 256 rows of 32,000
+    // words (bfloat16) on 1, 2, 4, 8 blocks each 69, 52, 65, 106 us; one row 25, 21, 16, 16; 64 rows of 128,256 words on 4 and 8 73 and
+    // 55; 16 rows of as many, temperature alone, 25 on both.
     int C = 1;
     while (C < SR_MAX_CLUSTER && (((V + C - 1) / C > 2048 && (long long)B * C < 2 * illm_sm_count()) || (V + C - 1) / C > SR_MAX_RESIDENT / 2)) C *= 2;
     cudaStream_t s = (cudaStream_t)stream;

@@ -527,7 +527,7 @@ class Model:
                  on_token=None, sampling: Optional[Sequence] = None, adapters: Optional[Sequence[int]] = None) -> GenerationResult:
         """Generate for many requests.  `stop_ids` default to the end token given to `init`; where that
         is one of the configuration's end tokens, to all of them.  `sampling`: `SamplingParams` per request (default: those of
-        `init` for all); `adapters`: a low-rank adapter per request (`engine.add_adapter`), -1 for none."""
+        `init` for all; the ones with a repetition penalty share one `repeat_last_n`); `adapters`: a low-rank adapter per request (`engine.add_adapter`), -1 for none."""
         lens = [len(p) for p in prompts]
         flat = [int(t) for p in prompts for t in p]
         stop = None if stop_ids is None else _b.ints(int(s) for s in stop_ids)

@@ -94,7 +94,8 @@ public:
     void warm_up(long long prompt_tokens, const std::vector<int>& batch_sizes);
     // Low-rank adapters: every item of a step may run with one of its own, all in one batch.  add_adapter takes factors by the names
     // (as in the weight file) of the projections that they stand beside and returns the adapter's number, the lowest free one;
-    // remove_adapter frees it.  Both wait for the steps that the stream holds.
+    // remove_adapter frees it.  add_adapter returns when the factors are in place, behind the steps that the stream holds; remove_adapter
+    // only gives the number back: steps that were issued before still run with the adapter.
     int add_adapter(const AdapterFactors& factors);
     void remove_adapter(int i);
     std::map<std::string, std::vector<long long>> adapted() const { return model_->adapted(); }

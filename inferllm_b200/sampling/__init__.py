@@ -35,7 +35,8 @@ def uniform_for(seed: int, request: int, step: int) -> float:
 
 class Sampler:
     """Chooses one token per row of float32 logits on the device (a torch tensor [B, V]); returns an
-    int32 torch tensor [B].  `params`: the settings of all requests, or a list with one per request number.
+    int32 torch tensor [B].  `params`: the settings of all requests, or a list with one per request number (of
+    which those with a repetition penalty share one `repeat_last_n`; a batch of others is refused).
     See `sampling/sampler.h` for `histories`."""
 
     def __init__(self, engine, params):
