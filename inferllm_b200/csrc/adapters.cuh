@@ -4,14 +4,13 @@
 #include "tc_common.cuh"
 
 struct AdPlan {
-    const int *counts, *token_adapter, *order;
+    const int *counts, *token_adapter;
     const int4* places;
-    const int *slot_begin, *slot_adapter, *slot_group, *groups, *tile_chunk, *chunk_tile, *chunk_groups;
+    const int *groups, *tile_chunk, *chunk_tile, *chunk_groups;
 };
 static inline AdPlan ad_plan(const int* plan, const AdapterPlanSizes& s) {
     const AdapterPlanLayout l = adapter_plan_layout(s);
-    return AdPlan{plan + l.counts, plan + l.token_adapter, plan + l.order, (const int4*)(plan + l.places), plan + l.slot_begin, plan + l.slot_adapter, plan + l.slot_group, plan + l.groups,
-                  plan + l.tile_chunk, plan + l.chunk_tile, plan + l.chunk_groups};
+    return AdPlan{plan + l.counts, plan + l.token_adapter, (const int4*)(plan + l.places), plan + l.groups, plan + l.tile_chunk, plan + l.chunk_tile, plan + l.chunk_groups};
 }
 
 // VEC neighbouring columns
