@@ -116,7 +116,7 @@ adapter_expand_kernel(int N, const float* __restrict__ b, const float* __restric
 // The second adds up the slices and, in the same float32 sum, v[t] . B_a[n]; v, the tokens' rank values, is added up and
 // scaled by every block for the tokens that it works on.  It stays float32: the result is rounded once.
 // Bound: reading the weight and the factors, and two starts and ends.  One token of 4096 x 4096 9.9 us on the GPU (the weight's 33 MB
-// at the copy rate: 5.1), 8 tokens with 8 adapters of 4096 x 12288 22.6 (16.0), 64 tokens with 48 of 11008 x 4096 31.4 (19.4).
+// at the copy rate: 5.1), 8 tokens with 8 adapters of 4096 x 12288 22.6 (16.0), 64 tokens with 48 of 11008 x 4096 33.2 (19.4).
 #define AD_ROWS_MAX_STAGES 8
 
 template <int BN>
