@@ -242,7 +242,7 @@ def prepare(case, seed):
         members = {}
         for t, a in enumerate(group):
             members.setdefault(a, []).append(t)
-        state["plan"] = ops.SharedPrefixes([(common[m[0]], m) for a, m in members.items() if a >= 0], len(group), case["heads"] // case["kv_heads"])
+        state["plan"] = ops.SharedPrefixes([(common[m[0]], m) for a, m in members.items() if a >= 0], lens, case["heads"] // case["kv_heads"])
     return state
 
 
