@@ -410,6 +410,11 @@ ILLM_API int illm_policy_gemm_tc_splits(long long M, long long N, long long K, i
 ILLM_API int illm_policy_ring_splits(long long T, int n_kv_heads, long long max_len, int head_dim, int n_sms) {
     return ops::attention_decode_ring_splits(T, n_kv_heads, max_len, head_dim, n_sms);
 }
+// blocks per (token, kv head) of attention_pages, or (wide) parts of a common prefix of attention_tiles; pairs: blocks without either
+ILLM_API int illm_policy_pages_splits(long long pairs, long long keys, int wide, int n_sms) {
+    return wide ? ops::attention_prefix_splits(pairs, keys, n_sms) : ops::attention_pages_splits(pairs, keys, n_sms);
+}
+ILLM_API int illm_policy_tile_rows(int B, int max_q, int nh, int nkv, int n_sms) { return ops::attention_tile_rows(B, max_q, nh, nkv, n_sms); }
 ILLM_API int illm_policy_attention_diff_splits(long long T, int head_groups, long long max_seq_len, int n_sms) {
     return ops::attention_diff_splits(T, head_groups, max_seq_len, n_sms);
 }

@@ -11,6 +11,7 @@
 #include "config/config.h"
 #include "engine/generate.h"
 #include "kernels/adapter_plan.h"
+#include "kernels/prefix_plan.h"
 #include "models/decoder.h"
 #include "weights/loader.h"
 
@@ -542,5 +543,23 @@ ILLM_API int illm_adapter_plan(const int* index, int T, const int* ranks, int co
         sizes[0] = s.T, sizes[1] = s.slots, sizes[2] = s.groups, sizes[3] = s.chunks;
         *total = adapter_plan_layout(s).total;
         if (out) ops::adapter_plan_fill(index, T, ranks, count, s, out);
+    });
+}
+
+// The plan of a step's common prefixes: n_groups groups, group i with prefixes[i] positions and counts[i] members, which follow one another in
+// `members`; lens [T].  sizes: tiles, wide, longest prefix, longest rest, and where start and members begin; out: nullptr, or `total` ints.
+ILLM_API int illm_prefix_plan(int n_groups, const int* prefixes, const int* counts, const int* members, const int* lens, int T, int G, int* sizes, int* total, int* out) {
+    return guard([&] {
+        std::vector<ops::PrefixGroup> groups((size_t)std::max(n_groups, 0));
+        for (auto& g : groups) {
+            const size_t i = (size_t)(&g - groups.data());
+            g.prefix = prefixes[i];
+            g.members.assign(members, members + std::max(counts[i], 0));
+            members += std::max(counts[i], 0);
+        }
+        const ops::PrefixPlanSizes s = ops::prefix_plan_sizes(groups, lens, T, G);
+        sizes[0] = s.tiles, sizes[1] = s.wide ? 1 : 0, sizes[2] = s.longest_prefix, sizes[3] = s.longest_rest, sizes[4] = s.start_at(), sizes[5] = s.members_at();
+        *total = s.ints();
+        if (out) ops::prefix_plan_fill(groups, s, G, out);
     });
 }

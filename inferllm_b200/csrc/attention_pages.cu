@@ -1,0 +1,561 @@
+// Attention of single tokens over paged caches on warp-level tensor instructions, the keys as a stream: over rows of eight bits
+// (kv_int8.cu) or bfloat16, and over positions that several sequences hold in common, which are read once for all of them.
+//
+//   o = sum_j p_j v_j,  p = softmax over the visible j of scale q . k_j       (src/kern/naive/naive.cpp:576-604, :531-553, :209-240, :634-662)
+//
+// The rows of a block's products are queries that walk the same keys: the heads of one token that share a key/value head or, for
+// a common prefix, those of up to 16 / group of its tokens.  A block takes every n-th tile of 64 keys of its range.  One thread
+// brings them by TMA into a ring of stages (swizzled; pages are multiples of 64 positions, so a tile lies in one page), four warps
+// take 16 keys of a tile each, with a running maximum and sum of their own, and are joined at the end; the shares of all blocks of a
+// head are joined by a second kernel in ascending order.  With a plan (common prefixes) the first blocks of the grid walk the
+// prefixes and the others what every token has for itself behind its prefix, in one launch.
+//
+// Eight-bit rows.  A key's products are made from the bytes: 0x64 in front of a byte is 1024 + u in half precision, minus 1152 is
+// u - 128 exactly, so a pair of elements costs a byte permutation and a subtraction, and for the values the permutation also makes
+// the transposition that the product wants.  The queries are scaled by a power of two per row so that bfloat16 turns into
+// half precision without loss (elements below 2^-24 of the row's largest lose bits), the key's scale is a factor of its score.  The
+// values' scale goes into the softmax weight: w_j = 2^(s_j + log2 s^v_j - m'), with a maximum m' of its own next to the softmax's m,
+// so that the largest weight of a row is 1 whatever the scales are; weights are rounded to half precision (2^-12 of a weight; those below 2^-24 of
+// the largest to 2^-25 of it).  The sum of 2^(s_j - m), scores and accumulators are float32.
+// A tile's hidden keys have weight 0 whatever lies there: bytes are finite, scales of hidden keys are not used.
+// bfloat16 rows go as in attention_decode_ring.cu, which is the faster one without a plan (it also rotates and writes).
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "tc_common.cuh"
+
+#define PG_BN 64                        // keys per tile
+#define PG_CONSUMERS 4
+#define PG_THREADS ((PG_CONSUMERS + 1) * 32)
+#define PG_MAX_SPLITS 32
+#define PG_ERR_PAGE 8                   // a visible position without a page
+
+namespace {
+
+__device__ __forceinline__ void pg_ldm(unsigned* r, unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void pg_ldm_t(unsigned* r, unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <bool HALF> __device__ __forceinline__ void pg_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+    if (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pg_half2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned pg_bf162(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+// two bytes of w (the selector names them; 4 is the 0x64 above them) as u - 128 in half precision
+__device__ __forceinline__ unsigned pg_widen(unsigned w, unsigned selector) {
+    unsigned r = __byte_perm(w, 0x64646464u, selector);
+    const unsigned bias = 0x64806480u;       // 1152, twice
+    __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float pg_log2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Byte offset of the 16-byte piece c of key row r inside a tile.  bfloat16: boxes of 64 channels of 8 KB, rows of 128 bytes, the
+// piece's number XORed with the row's; eight bits: rows of D bytes, the same swizzle for 128 and the 64-byte one for 64.
+template <int D, bool Q8> __device__ __forceinline__ unsigned pg_off(int r, int c) {
+    if (!Q8) return (unsigned)((c >> 3) * (PG_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    if (D == 128) return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4));
+    return (unsigned)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ void pg_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+}  // namespace
+
+// A plan of common prefixes (attention_decode_shared): int32 on the device.  `start` [T]: the positions that a token leaves to its
+// group; `tiles` [n_tiles][4]: first member, number of members, positions of the prefix, 0; `members`: tokens.
+struct PgPlan {
+    const int* start;
+    const int4* tiles;
+    const int* members;
+    int n_tiles;
+};
+
+// stages that leave two blocks to an SM
+template <int D, bool Q8> struct PgRing {
+    static constexpr int TILE = PG_BN * D * (Q8 ? 1 : 2), SCALES = Q8 ? 2 * PG_BN * 4 : 0;
+    static constexpr int STAGES = (Q8 ? 768 : 384) / D, BYTES = STAGES * (2 * TILE + SCALES) + 1024;
+};
+
+// grid: (splits, kv heads, prefix tiles and tokens).  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
+// a token's own first.  out: written here where there is one slot.
+template <int D, bool Q8>
+__global__ void __launch_bounds__(PG_THREADS)
+attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
+                       const __grid_constant__ CUtensorMap map_v16, const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ q,
+                       int q_stride, const int* __restrict__ block_table, int max_pages, int n_pages, const int* __restrict__ token_pos,
+                       const int* __restrict__ token_seq, const PgPlan plan, float* __restrict__ part_acc, float* __restrict__ part_ml, bf16* __restrict__ out,
+                       int own_splits, int pre_splits, int nh, int nkv, int page_size, int span, float scale_log2e, int* __restrict__ err) {
+    using R = PgRing<D, Q8>;
+    constexpr int KS = D / 16, STAGES = R::STAGES, TILE = R::TILE;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned base = (tc_smem_u32(smem_raw) + 1023u) & ~1023u, scales = base + STAGES * 2 * TILE;
+    unsigned char* gbase = smem_raw + (base - tc_smem_u32(smem_raw));
+    const unsigned full0 = tc_smem_u32(bars), empty0 = full0 + 8 * STAGES;
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, PG_CONSUMERS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_grid_sync();
+
+    // ---- which rows and keys
+    const int split = blockIdx.x, hk = blockIdx.y, G = nh / nkv, slots = own_splits + pre_splits;
+    const bool prefix = (int)blockIdx.z < plan.n_tiles;
+    const int n_splits = prefix ? pre_splits : own_splits;
+    if (split >= n_splits) return;
+    int t = 0, first = 0, count = 1, p, lo = 0;
+    if (prefix) {
+        const int4 tile = plan.tiles[blockIdx.z];
+        first = tile.x;
+        count = tile.y;
+        p = tile.z - 1;
+        if (count <= 0 || p < 0) return;
+        t = plan.members[first];
+    } else {
+        t = blockIdx.z - plan.n_tiles;
+        p = token_pos[t];
+        lo = p < 0 ? 0 : first_visible(p, span);
+        if (plan.start) lo = max(lo, plan.start[t]);
+    }
+    const int rows = count * G;
+    auto row_head = [&](int r) -> size_t {      // of a row below `rows`: which row of [T, nh]
+        const int tok = prefix ? plan.members[first + r / G] : t;
+        return (size_t)tok * nh + hk * G + r % G;
+    };
+    const int tile_lo = lo / PG_BN, n_tiles = p < lo ? 0 : p / PG_BN - tile_lo + 1;
+    const int n_my = n_tiles > split ? (n_tiles - split + n_splits - 1) / n_splits : 0;
+    const int slot = prefix ? own_splits + split : split;
+    if (n_my == 0) {
+        if (slots == 1) {
+            for (int i = tid; i < rows * D; i += PG_THREADS) out[row_head(i / D) * D + i % D] = __float2bfloat16_rn(0.f);
+        } else if (tid < rows) {
+            *reinterpret_cast<float2*>(part_ml + (row_head(tid) * slots + slot) * 2) = make_float2(-INFINITY, 0.f);
+        }
+        return;
+    }
+
+    if (warp == PG_CONSUMERS) {
+        // ---- producer.  A page that the sequence does not hold is reported and another one read in its place.
+        if (lane == 0) {
+            const int* bt = block_table + (size_t)token_seq[t] * max_pages;
+            for (int i = 0; i < n_my; i++) {
+                const int s = i % STAGES;
+                if (i >= STAGES && !mbar_wait(empty0 + 8 * s, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_DECODE)) break;
+                const int key0 = (tile_lo + split + i * n_splits) * PG_BN;
+                int page = key0 / page_size < max_pages ? bt[key0 / page_size] : -1;
+                if (page < 0 || page >= n_pages) {
+                    atomicExch(err, PG_ERR_PAGE);
+                    page = 0;
+                }
+                const int row = (page * nkv + hk) * page_size + key0 % page_size;
+                const unsigned kdst = base + (unsigned)s * 2 * TILE, vdst = kdst + TILE, bar = full0 + 8 * s;
+                const int groups = min(PG_BN / 16, (p - key0) / 16 + 1);       // of 16 keys, as many as hold a visible one
+                mbar_expect_tx(bar, (unsigned)groups * (2 * TILE / (PG_BN / 16)) + (unsigned)R::SCALES);
+                if (Q8) {
+                    pg_bulk(scales + s * R::SCALES, ksc + row, PG_BN * 4, bar);
+                    pg_bulk(scales + s * R::SCALES + PG_BN * 4, vsc + row, PG_BN * 4, bar);
+                }
+#pragma unroll
+                for (int hx = 0; hx < (Q8 ? 1 : D / 64); hx++) {
+                    const int box = hx * (PG_BN * 128), line = Q8 ? D : 128;
+                    if (groups == PG_BN / 16) {
+                        tma_load_2d(kdst + box, &map_k, hx * 64, row, bar);
+                        tma_load_2d(vdst + box, &map_v, hx * 64, row, bar);
+                    } else {
+                        for (int u = 0; u < groups; u++) {
+                            tma_load_2d(kdst + box + u * 16 * line, &map_k16, hx * 64, row + u * 16, bar);
+                            tma_load_2d(vdst + box + u * 16 * line, &map_v16, hx * 64, row + u * 16, bar);
+                        }
+                    }
+                }
+            }
+        }
+        return;
+    }
+
+    // ---- consumers: warp w owns keys 16w .. 16w+15 of every tile
+    const int g = lane >> 2, t4 = lane & 3, mtx = lane >> 3;
+    // The queries as fragments: row g and g + 8.  With eight bits a thread's four elements of 16 are neighbours (4 t4 ..), as the
+    // bytes of the keys come; any order of the summed index is as good as another.
+    unsigned qf[KS][4];
+    float row_scale[2] = {scale_log2e, scale_log2e};
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int r = g + e * 8;
+        const bool ok = r < rows;
+        const size_t head = ok ? row_head(r) : 0;
+        const bf16* src = q + (head / nh) * (size_t)q_stride + (head % nh) * D;
+        uint2 raw[KS];
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            raw[k] = make_uint2(0u, 0u);
+            if (!ok) continue;
+            if (Q8) {
+                raw[k] = *reinterpret_cast<const uint2*>(src + k * 16 + t4 * 4);
+            } else {
+                raw[k].x = *reinterpret_cast<const unsigned*>(src + k * 16 + t4 * 2);
+                raw[k].y = *reinterpret_cast<const unsigned*>(src + k * 16 + 8 + t4 * 2);
+            }
+        }
+        if (Q8) {
+            unsigned top = 0;           // the largest magnitude's bits
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+                top = max(max(top, max(raw[k].x & 0x7fffu, (raw[k].x >> 16) & 0x7fffu)), max(raw[k].y & 0x7fffu, (raw[k].y >> 16) & 0x7fffu));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // a power of two that brings the largest to [2^10, 2^11): 128 products with 127 stay below 2^25
+            const int ex = max((int)(top >> 7) - 127, -116);
+            const float up = __int_as_float((10 - ex + 127) << 23), down = __int_as_float((ex - 10 + 127) << 23);
+            row_scale[e] = scale_log2e * down;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                qf[k][e] = pg_half2(__uint_as_float(raw[k].x << 16) * up, __uint_as_float(raw[k].x & 0xffff0000u) * up);
+                qf[k][e + 2] = pg_half2(__uint_as_float(raw[k].y << 16) * up, __uint_as_float(raw[k].y & 0xffff0000u) * up);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                qf[k][e] = raw[k].x;
+                qf[k][e + 2] = raw[k].y;
+            }
+        }
+    }
+
+    // m, l: maximum and sum of the softmax; mv: the maximum that the accumulators are relative to (m itself for bfloat16 rows)
+    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[2 * KS][4];
+#pragma unroll
+    for (int i = 0; i < 2 * KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+    for (int i = 0; i < n_my; i++) {
+        const int s = i % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_DECODE))) break;
+        const int key0 = (tile_lo + split + i * n_splits) * PG_BN + warp * 16;
+        if (key0 <= p && key0 + 15 >= lo) {
+            const unsigned kbase = base + (unsigned)s * 2 * TILE, vbase = kbase + TILE;
+            float sa[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sb[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            if (Q8) {
+                const int krow = warp * 16 + (mtx & 1) * 8 + (lane & 7);
+#pragma unroll
+                for (int k = 0; k < KS; k += 2) {
+                    unsigned b[4];
+                    pg_ldm(b, kbase + pg_off<D, Q8>(krow, k + (mtx >> 1)));
+                    pg_mma<true>(sa[0], qf[k], pg_widen(b[0], 0x4140), pg_widen(b[0], 0x4342));
+                    pg_mma<true>(sa[1], qf[k], pg_widen(b[1], 0x4140), pg_widen(b[1], 0x4342));
+                    pg_mma<true>(sb[0], qf[k + 1], pg_widen(b[2], 0x4140), pg_widen(b[2], 0x4342));
+                    pg_mma<true>(sb[1], qf[k + 1], pg_widen(b[3], 0x4140), pg_widen(b[3], 0x4342));
+                }
+            } else {
+                const int krow = warp * 16 + (mtx >> 1) * 8 + (lane & 7);
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    unsigned b[4];
+                    pg_ldm(b, kbase + pg_off<D, Q8>(krow, k * 2 + (mtx & 1)));
+                    pg_mma<false>(k & 1 ? sb[0] : sa[0], qf[k], b[0], b[1]);
+                    pg_mma<false>(k & 1 ? sb[1] : sa[1], qf[k], b[2], b[3]);
+                }
+            }
+            float lv[2][2];                 // log2 of the values' scales
+            float mx[2] = {-INFINITY, -INFINITY}, mxv[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                float kf[2] = {1.f, 1.f};
+                if (Q8) {
+                    const unsigned at = scales + s * R::SCALES + (warp * 16 + nt * 8 + t4 * 2) * 4;
+                    float v0, v1;
+                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(kf[0]), "=f"(kf[1]) : "r"(at));
+                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v0), "=f"(v1) : "r"(at + PG_BN * 4));
+                    lv[nt][0] = pg_log2(v0);
+                    lv[nt][1] = pg_log2(v1);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int key = key0 + nt * 8 + t4 * 2 + (e & 1);
+                    const bool hidden = key > p || key < lo;
+                    float v = (sa[nt][e] + sb[nt][e]) * row_scale[e >> 1];
+                    if (Q8) v *= kf[e & 1];
+                    if (hidden) v = -INFINITY;
+                    sa[nt][e] = v;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], v);
+                    if (Q8) {
+                        const float w = hidden ? -INFINITY : v + lv[nt][e & 1];
+                        sb[nt][e] = w;
+                        mxv[e >> 1] = fmaxf(mxv[e >> 1], w);
+                    }
+                }
+            }
+            float ref[2], refv[2], alpha[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                const float top = fmaxf(m[e], mx[e]);
+                ref[e] = top == -INFINITY ? 0.f : top;
+                const float keep = fast_exp2(m[e] - ref[e]);
+                l[e] *= keep;
+                m[e] = top;
+                if (Q8) {
+                    mxv[e] = fmaxf(mxv[e], __shfl_xor_sync(0xffffffffu, mxv[e], 1));
+                    mxv[e] = fmaxf(mxv[e], __shfl_xor_sync(0xffffffffu, mxv[e], 2));
+                    const float topv = fmaxf(mv[e], mxv[e]);
+                    refv[e] = topv == -INFINITY ? 0.f : topv;
+                    alpha[e] = fast_exp2(mv[e] - refv[e]);
+                    mv[e] = topv;
+                } else {
+                    refv[e] = ref[e];
+                    alpha[e] = keep;
+                    mv[e] = top;
+                }
+            }
+            unsigned pf[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                const float p0 = fast_exp2(sa[nt][0] - ref[0]), p1 = fast_exp2(sa[nt][1] - ref[0]);
+                const float p2 = fast_exp2(sa[nt][2] - ref[1]), p3 = fast_exp2(sa[nt][3] - ref[1]);
+                l[0] += p0 + p1;
+                l[1] += p2 + p3;
+                if (Q8) {
+                    pf[nt * 2] = pg_half2(fast_exp2(sb[nt][0] - refv[0]), fast_exp2(sb[nt][1] - refv[0]));
+                    pf[nt * 2 + 1] = pg_half2(fast_exp2(sb[nt][2] - refv[1]), fast_exp2(sb[nt][3] - refv[1]));
+                } else {
+                    pf[nt * 2] = pg_bf162(p0, p1);
+                    pf[nt * 2 + 1] = pg_bf162(p2, p3);
+                }
+            }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+                for (int j = 0; j < 2 * KS; j++) {
+                    o[j][0] *= alpha[0];
+                    o[j][1] *= alpha[0];
+                    o[j][2] *= alpha[1];
+                    o[j][3] *= alpha[1];
+                }
+            }
+            const int vrow = warp * 16 + (mtx & 1) * 8 + (lane & 7);
+            if (Q8) {
+#pragma unroll
+                for (int c = 0; c < KS; c += 2) {
+                    unsigned b[4];
+                    pg_ldm_t(b, vbase + pg_off<D, Q8>(vrow, c + (mtx >> 1)));
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {           // channels 16 (c + u) + 2 n and + 2 n + 1 of column n
+                        pg_mma<true>(o[(c + u) * 2], pf, pg_widen(b[u * 2], 0x4240), pg_widen(b[u * 2 + 1], 0x4240));
+                        pg_mma<true>(o[(c + u) * 2 + 1], pf, pg_widen(b[u * 2], 0x4341), pg_widen(b[u * 2 + 1], 0x4341));
+                    }
+                }
+            } else {
+                if (key0 + 15 > p || key0 < lo) {
+                    // rows of hidden keys may hold anything, and 0 x NaN would not be 0
+                    unsigned char* v = gbase + (size_t)s * 2 * TILE + TILE;
+                    for (int j = lane; j < 16 * 2 * KS; j += 32) {
+                        const int r = j / (2 * KS), c = j % (2 * KS);
+                        if (key0 + r > p || key0 + r < lo) *reinterpret_cast<uint4*>(v + pg_off<D, Q8>(warp * 16 + r, c)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the stage is filled again
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    unsigned b[4];
+                    pg_ldm_t(b, vbase + pg_off<D, Q8>(vrow, c * 2 + (mtx >> 1)));
+                    pg_mma<false>(o[c * 2], pf, b[0], b[1]);
+                    pg_mma<false>(o[c * 2 + 1], pf, b[2], b[3]);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * s) : "memory");
+    }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+
+    // ---- join the warps (ascending) through the ring's memory: every load has landed and been read
+    asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
+    float* joined = reinterpret_cast<float*>(gbase);            // [PG_CONSUMERS][16][D + 4]: accumulators, m, l, mv
+    constexpr int ROW = D + 4;
+    static_assert(PG_CONSUMERS * 16 * ROW * 4 <= STAGES * 2 * TILE, "the joined rows must fit the ring");
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int r = g + e * 8;
+        if (r >= rows) continue;
+        float* dst = joined + ((size_t)warp * 16 + r) * ROW;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if (Q8) {
+                *reinterpret_cast<float4*>(dst + k * 16 + t4 * 4) = make_float4(o[k * 2][e * 2], o[k * 2 + 1][e * 2], o[k * 2][e * 2 + 1], o[k * 2 + 1][e * 2 + 1]);
+            } else {
+                *reinterpret_cast<float2*>(dst + k * 16 + t4 * 2) = make_float2(o[k * 2][e * 2], o[k * 2][e * 2 + 1]);
+                *reinterpret_cast<float2*>(dst + k * 16 + 8 + t4 * 2) = make_float2(o[k * 2 + 1][e * 2], o[k * 2 + 1][e * 2 + 1]);
+            }
+        }
+        if (t4 == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m[e], l[e], mv[e], 0.f);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
+    for (int idx = tid; idx < rows * D; idx += PG_CONSUMERS * 32) {
+        const int r = idx / D, c = idx - r * D;
+        float4 w[PG_CONSUMERS];
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < PG_CONSUMERS; k++) {
+            w[k] = *reinterpret_cast<const float4*>(joined + ((size_t)k * 16 + r) * ROW + D);
+            M = fmaxf(M, w[k].x);
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
+        float num = 0.f, den = 0.f;
+#pragma unroll
+        for (int k = 0; k < PG_CONSUMERS; k++) {
+            if (w[k].y == 0.f) continue;                        // no visible keys; a sum that is no number goes on
+            num += joined[((size_t)k * 16 + r) * ROW + c] * (w[k].z == -INFINITY ? 1.f : fast_exp2(w[k].z - ref));
+            den += w[k].y * (w[k].x == -INFINITY ? 1.f : fast_exp2(w[k].x - ref));
+        }
+        const size_t head = row_head(r);
+        if (slots == 1) {
+            out[head * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+        } else {
+            part_acc[(head * slots + slot) * D + c] = num;
+            if (c == 0) *reinterpret_cast<float2*>(part_ml + (head * slots + slot) * 2) = make_float2(M, den);
+        }
+    }
+}
+
+// out[t, h] = sum over the shares (ascending) of acc 2^(m - M) / sum of l 2^(m - M): a token's own and, where it has a prefix in common with
+// others, the prefix's.  A share without keys has l = 0 and no accumulators; a token without any gets zeros.
+template <int D>
+__global__ void __launch_bounds__(D)
+attention_pages_join_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, bf16* __restrict__ out, int own_splits, int pre_splits,
+                            const int* __restrict__ start, int nh) {
+    pdl_grid_sync();
+    const int h = blockIdx.x, t = blockIdx.y, c = threadIdx.x, lane = threadIdx.x & 31, slots = own_splits + pre_splits;
+    const int n = start && start[t] > 0 ? slots : own_splits;
+    const size_t o = ((size_t)t * nh + h) * slots;
+    float2 ml[2];           // share `lane` and share 32 + `lane`
+#pragma unroll
+    for (int k = 0; k < 2; k++) ml[k] = lane + 32 * k < n ? *reinterpret_cast<const float2*>(part_ml + (o + lane + 32 * k) * 2) : make_float2(-INFINITY, 0.f);
+    const float M = warp_max(fmaxf(ml[0].x, ml[1].x)), ref = M == -INFINITY ? 0.f : M;
+    float w[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) w[k] = ml[k].y == 0.f ? 0.f : ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - ref);
+    float num = 0.f, den = 0.f;
+    for (int s0 = 0; s0 < n; s0 += 8) {
+        float v[8], f[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int s = s0 + k;
+            f[k] = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+            const float l = __shfl_sync(0xffffffffu, s < 32 ? ml[0].y : ml[1].y, s & 31);
+            if (f[k] != 0.f) den += f[k] * l;
+            v[k] = s < n && f[k] != 0.f ? part_acc[(o + s) * D + c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) num += f[k] * v[k];
+    }
+    out[((size_t)t * nh + h) * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+}
+
+// ---- host side
+
+typedef CUresult (*PgEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static PgEncodeTiledFn pg_encode_fn() {
+    static const PgEncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess ? (PgEncodeTiledFn)p
+                                                                                                                                         : (PgEncodeTiledFn) nullptr;
+    }();
+    return fn;
+}
+// an entry's pages as a matrix [pages * kv heads * page_size, d]; boxes of `box_rows` rows of 128 bytes (eight bits: of d)
+static int pg_make_map(CUtensorMap* map, const void* ptr, long long rows, int d, int box_rows, bool q8) {
+    PgEncodeTiledFn fn = pg_encode_fn();
+    if (!fn) return ILLM_ERR_BAD_ARG;
+    cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)d * (q8 ? 1 : 2)};
+    cuuint32_t box[2] = {q8 ? (cuuint32_t)d : 64u, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, q8 && d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : ILLM_ERR_BAD_ARG;
+}
+
+template <int D, bool Q8>
+static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages,
+                     const int* token_pos, const int* token_seq, const PgPlan& plan, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int page_size,
+                     int span, float scale, int own_splits, int pre_splits, int* err, cudaStream_t s) {
+    CUtensorMap mk, mv, mk16, mv16;
+    const long long rows = n_pages * nkv * page_size;
+    int rc;
+    if ((rc = pg_make_map(&mk, kc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mv, vc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mk16, kc, rows, D, 16, Q8)) ||
+        (rc = pg_make_map(&mv16, vc, rows, D, 16, Q8)))
+        return rc;
+    auto kern = attention_pages_kernel<D, Q8>;
+    const int smem = PgRing<D, Q8>::BYTES;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    illm_launch(kern, dim3(own_splits > pre_splits ? own_splits : pre_splits, nkv, plan.n_tiles + T), dim3(PG_THREADS), smem, s, mk, mv, mk16, mv16, ksc, vsc, (const bf16*)q,
+                q_stride, block_table, max_pages, (int)n_pages, token_pos, token_seq, plan, part_acc, part_ml, (bf16*)out, own_splits, pre_splits, nh, nkv, page_size,
+                span, scale * 1.4426950408889634f, err);
+    if ((rc = illm_launch_status()) || own_splits + pre_splits == 1) return rc;
+    illm_launch(attention_pages_join_kernel<D>, dim3(nh, T), dim3(D), 0, s, (const float*)part_acc, (const float*)part_ml, (bf16*)out, own_splits, pre_splits,
+                plan.start, nh);
+    return illm_launch_status();
+}
+
+// Single tokens: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages
+// [n_pages, nkv, page_size, d] of bytes with their scales ksc, vsc, or (ksc, vsc nullptr) of bfloat16; page_size a multiple of 64, d 64
+// or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most 16 rows (members times nh / nkv),
+// are walked here, with n_tiles 0 their shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  Scratch where own_splits +
+// pre_splits > 1 (each at most 32, pre_splits 0 without a plan): part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  err: 7 a wait ran out,
+// 8 a visible position without a page.
+extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
+                                    const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles,
+                                    const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,
+                                    int span, float scale, int own_splits, int pre_splits, int* err, void* stream) {
+    if (T <= 0) return 0;
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || T > 65535 || nkv > 65535 || n_tiles < 0 || n_tiles + T > 65535 || (q_stride & 7) || page_size <= 0 ||
+        page_size % PG_BN || max_pages <= 0 || n_pages <= 0 || n_pages * nkv * page_size > 0x7fffffffLL || own_splits < 1 || own_splits > PG_MAX_SPLITS || pre_splits < 0 ||
+        pre_splits > PG_MAX_SPLITS || !q || ((uintptr_t)q & 15) || !kc || !vc || ((uintptr_t)kc & 15) || ((uintptr_t)vc & 15) || (!ksc) != (!vsc) || ((uintptr_t)ksc & 15) ||
+        ((uintptr_t)vsc & 15) || !err || (plan_start && (span != 0 || pre_splits < 1)) || (!plan_start && (n_tiles > 0 || pre_splits != 0)) ||
+        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || (own_splits + pre_splits > 1 && (!part_acc || !part_ml || ((uintptr_t)part_ml & 7))))
+        return ILLM_ERR_BAD_ARG;
+    const PgPlan plan = {plan_start, reinterpret_cast<const int4*>(plan_tiles), plan_members, n_tiles};
+    cudaStream_t s = (cudaStream_t)stream;
+#define PG_CASE(DD, QQ)                                                                                                                                        \
+    if (d == DD && (ksc != nullptr) == QQ)                                                                                                                     \
+        return pg_launch<DD, QQ>(q, q_stride, kc, vc, ksc, vsc, n_pages, block_table, max_pages, token_pos, token_seq, plan, part_acc, part_ml, out, T, nh, nkv, \
+                                 page_size, span, scale, own_splits, pre_splits, err, s);
+    PG_CASE(128, true) PG_CASE(64, true) PG_CASE(128, false) PG_CASE(64, false)
+#undef PG_CASE
+    return ILLM_ERR_BAD_ARG;
+}

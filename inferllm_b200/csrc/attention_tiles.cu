@@ -1,0 +1,537 @@
+// Attention of many queries over paged caches on the 5th-generation tensor cores where the rows of the products are (token, head)
+// pairs that share a key/value head: prompts over rows of eight bits (kv_int8.cu), and the tokens of a step over a prefix that their
+// sequences hold in common (eight bits or bfloat16), which is then read once for all of them.
+//
+//   o = sum_j p_j v_j,  p = softmax over the visible j of scale q . k_j       (src/kern/naive/naive.cpp:606-632, :531-553, :209-240, :664-691)
+//
+// A block has two tiles of 128 rows over the same keys and is alone on its SM.  Eight softmax warps (a thread is a row of a tile and a lane of
+// tensor memory), a thread that issues the products, one that brings pages by TMA and, for eight bits, four warps that widen them:
+// bytes from a ring of four raw stages become (u - 128) s in bfloat16, in the swizzled layout that the products read.  Widening
+// costs about ten instructions for four elements, as much as the softmax of half a tile, which is why the tiles share it; two rows five apart
+// (r and r XOR 5) go to a quarter of a warp, so that neither its loads nor its stores meet in a bank.
+// Tensor memory of a tile, 256 columns: two score buffers of 64 and the output.  As in attention_prefill_tc.cu the scores
+// of the next 64 keys are made while the softmax works on the last ones, the weights stay in tensor memory in place of their scores,
+// and the output is rescaled only when a row's maximum has grown by more than 2^8.
+// Rounded to bfloat16: the widened rows (2^-9 of an element, next to the eight bits' own 1/254 of the row's largest), the softmax weights
+// and the results.  Scores, sums and the running output are float32.
+// A key whose row reads back as NaN has its score NaN instead, so that it reaches the queries that see it and no others.
+#include <cuda.h>
+#include <math.h>
+
+#include "attention_tc.cuh"
+#include "tc_common.cuh"
+
+#define TL_BM 128
+#define TL_BN 64
+#define TL_RAW 4                        // raw stages (eight bits)
+#define TL_SOFTMAX 8                    // warps
+#define TL_MMA_WARP 8
+#define TL_TMA_WARP 9
+#define TL_WIDEN_WARP 10                // the first of four
+#define TL_ERR_PAGE 8
+#define TL_RESCALE_STEP 8.0f
+
+// Which rows and keys: prompts (PREFIX false) or the tiles of a plan of common prefixes (attention_pages.cu).
+struct TlWork {
+    const int *cu_q, *seq_lens;         // prompts: [B + 1], [B]
+    int span, tile_rows;                // tile_rows: rows of a block, 128 (its first tile alone) or 256
+    const int4* tiles;                  // prefixes: first member, number of members, positions, 0
+    const int *members, *token_seq;
+    int slots, slot0;                   // shares of a (token, head) and the first of them that is the prefix's
+    float *part_acc, *part_ml;
+};
+
+template <int D, bool Q8> struct TlSizes {
+    static constexpr int STAGES = Q8 ? 2 : 4, TILE = TL_BN * D * 2, Q_TILE = TL_BM * D * 2;
+    static constexpr int RAW_TILE = TL_BN * D, RAW = Q8 ? TL_RAW : 0, SCALES = 2 * TL_BN * 4;
+    static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + RAW * (2 * RAW_TILE + SCALES) + 512;
+    static constexpr int THREADS = (Q8 ? 14 : 10) * 32;
+};
+
+namespace {
+
+__device__ __forceinline__ void tl_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tl_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tl_store16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// sixteen bytes as (u - 128) s in bfloat16: a byte below 0x4b0000 is 2^23 + u in float32
+__device__ __forceinline__ void tl_widen(const unsigned (&w)[4], float s, unsigned (&out)[8]) {
+    const unsigned long long bias = f2_pack(-8388736.f, -8388736.f), ss = f2_pack(s, s);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const unsigned lo = __byte_perm(w[i], 0x4b000000u, h ? 0x7652 : 0x7650), hi = __byte_perm(w[i], 0x4b000000u, h ? 0x7653 : 0x7651);
+            float a, b;
+            f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(lo), __uint_as_float(hi)), bias), ss), a, b);
+            out[i * 2 + h] = pack_bf16(a, b);
+        }
+}
+
+}  // namespace
+
+template <int D, bool Q8, bool PREFIX>
+__global__ void __launch_bounds__((TlSizes<D, Q8>::THREADS), 1)
+attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const float* __restrict__ ksc, const float* __restrict__ vsc,
+                       const bf16* __restrict__ q, int q_stride, const int* __restrict__ block_table, int max_pages, int n_pages, const TlWork work, bf16* __restrict__ out,
+                       int nh, int nkv, int page_size, float scale_log2e, int* __restrict__ err) {
+    using Z = TlSizes<D, Q8>;
+    constexpr int STAGES = Z::STAGES, TILE = Z::TILE, NA = D / 64;
+    constexpr unsigned ATOM = TL_BN * 128, Q_ATOM = TL_BM * 128, S_COLS = TL_BN, O_COL = 2 * TL_BN, TILE_COLS = 256;
+    constexpr unsigned IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TL_BN >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
+    constexpr unsigned IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(D >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const unsigned base = tc_smem_u32(smem_raw);
+    const unsigned q_s = base, kv_s = q_s + 2 * Z::Q_TILE, raw_s = kv_s + STAGES * 2 * TILE, sc_s = raw_s + Z::RAW * 2 * Z::RAW_TILE;
+    const unsigned bars0 = sc_s + Z::RAW * Z::SCALES;
+    const unsigned q_full = bars0, k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * STAGES, v_full0 = k_empty0 + 8 * STAGES, v_empty0 = v_full0 + 8 * STAGES;
+    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32;
+    unsigned* holder = reinterpret_cast<unsigned*>(smem_raw + (pv_done0 + 16 - base));
+    if ((base & 1023u) != 0) {          // cannot happen without static shared memory; never run misaligned
+        if (threadIdx.x == 0) atomicExch(err, TC_ERR_MISALIGNED_SMEM);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, TL_SOFTMAX * 32);
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(k_full0 + 8 * i, Q8 ? 128 : 1);
+            mbar_init(v_full0 + 8 * i, Q8 ? 128 : 1);
+            mbar_init(k_empty0 + 8 * i, 1);
+            mbar_init(v_empty0 + 8 * i, 1);
+        }
+        for (int i = 0; i < TL_RAW; i++) {
+            mbar_init(raw_full0 + 8 * i, 1);
+            mbar_init(raw_empty0 + 8 * i, 128);
+        }
+        for (int i = 0; i < 4; i++) {
+            mbar_init(s_full0 + 8 * i, 1);
+            mbar_init(p_full0 + 8 * i, TL_BM);
+        }
+        for (int w = 0; w < 2; w++) mbar_init(pv_done0 + 8 * w, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == TL_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(holder)), "r"(2 * TILE_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = *holder;
+    pdl_grid_sync();
+
+    // ---- which rows and keys
+    const int G = nh / nkv;
+    int hk, row0 = 0, n_rows, token0, past = 0, seq, jb0, last_key, nb[2], first_key;       // of the block: its rows, from row0 of its (sequence or tile)'s
+    int4 tile = make_int4(0, 0, 0, 0);
+    if (PREFIX) {
+        hk = blockIdx.y;
+        tile = work.tiles[blockIdx.z];
+        n_rows = tile.y > 0 && tile.z > 0 ? tile.y * G : 0;
+        token0 = 0;
+        seq = n_rows ? work.token_seq[work.members[tile.x]] : 0;
+        const int all = (tile.z + TL_BN - 1) / TL_BN, per = (all + gridDim.x - 1) / gridDim.x;
+        jb0 = blockIdx.x * per;
+        first_key = jb0 * TL_BN;
+        last_key = tile.z - 1;
+        const int n = max(0, min(per, all - jb0));
+        nb[0] = n_rows > 0 ? n : 0;
+        nb[1] = n_rows > TL_BM ? n : 0;
+    } else {
+        // blocks with the most keys before them start first
+        hk = blockIdx.x;
+        seq = blockIdx.z;
+        token0 = work.cu_q[seq];
+        const int q_len = work.cu_q[seq + 1] - token0, all_rows = q_len * G;
+        past = work.seq_lens[seq] - q_len;
+        const int at = (all_rows + work.tile_rows - 1) / work.tile_rows - 1 - (int)blockIdx.y;
+        row0 = at * work.tile_rows;
+        n_rows = at < 0 ? 0 : min(work.tile_rows, all_rows - row0);
+        first_key = n_rows > 0 ? max(0, first_visible(past + row0 / G, work.span)) : 0;
+        jb0 = first_key / TL_BN;
+        last_key = n_rows > 0 ? past + (row0 + n_rows - 1) / G : -1;
+        nb[0] = n_rows > 0 ? (past + (row0 + min(n_rows, TL_BM) - 1) / G) / TL_BN - jb0 + 1 : 0;
+        nb[1] = n_rows > TL_BM ? last_key / TL_BN - jb0 + 1 : 0;
+    }
+    const int n_blocks = max(nb[0], nb[1]);         // the second tile, where it has rows, sees at least as far as the first
+
+    if (warp == TL_TMA_WARP) {
+        // ---- pages.  One that the sequence does not hold is reported and another read in its place.
+        if (lane == 0) {
+            const int* bt = block_table + (size_t)seq * max_pages;
+            for (int i = 0; i < n_blocks; i++) {
+                const int key0 = (jb0 + i) * TL_BN;
+                int page = key0 / page_size < max_pages ? bt[key0 / page_size] : -1;
+                if (page < 0 || page >= n_pages) {
+                    atomicExch(err, TL_ERR_PAGE);
+                    page = 0;
+                }
+                const int row = (page * nkv + hk) * page_size + key0 % page_size;
+                if (Q8) {
+                    const int st = i % TL_RAW;
+                    if (i >= TL_RAW && !mbar_wait(raw_empty0 + 8 * st, ((i / TL_RAW) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+                    const unsigned bar = raw_full0 + 8 * st, dst = raw_s + st * 2 * Z::RAW_TILE;
+                    mbar_expect_tx(bar, 2 * Z::RAW_TILE + Z::SCALES);
+                    tma_load_2d(dst, &map_k, 0, row, bar);
+                    tl_bulk(sc_s + st * Z::SCALES, ksc + row, TL_BN * 4, bar);
+                    tma_load_2d(dst + Z::RAW_TILE, &map_v, 0, row, bar);
+                    tl_bulk(sc_s + st * Z::SCALES + TL_BN * 4, vsc + row, TL_BN * 4, bar);
+                } else {
+                    const int st = i % STAGES;
+                    const unsigned kd = kv_s + st * 2 * TILE, vd = kd + TILE;
+                    if (i >= STAGES && !mbar_wait(k_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+                    mbar_expect_tx(k_full0 + 8 * st, TILE);
+                    for (int a = 0; a < NA; a++) tma_load_2d(kd + a * ATOM, &map_k, 64 * a, row, k_full0 + 8 * st);
+                    if (i >= STAGES && !mbar_wait(v_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+                    mbar_expect_tx(v_full0 + 8 * st, TILE);
+                    for (int a = 0; a < NA; a++) tma_load_2d(vd + a * ATOM, &map_v, 64 * a, row, v_full0 + 8 * st);
+                }
+            }
+        }
+    } else if (warp == TL_MMA_WARP) {
+        // ---- products: the scores of a tile one block ahead of its softmax
+        if (lane == 0 && n_blocks > 0) {
+            bool alive = mbar_wait(q_full, 0, err, TC_ERR_TIMEOUT_PREFILL);
+            auto issue_s = [&](int w, int i) {
+                const int st = i % STAGES;
+                if (!mbar_wait(k_full0 + 8 * st, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_PREFILL)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++)
+                    mma_bf16_ss(tmem + w * TILE_COLS + (i & 1) * S_COLS, desc_kmajor(q_s + w * Z::Q_TILE + (kk >> 2) * Q_ATOM + (kk & 3) * 32),
+                                desc_kmajor(kv_s + st * 2 * TILE + (kk >> 2) * ATOM + (kk & 3) * 32), IDESC_S, kk > 0);
+                mma_commit(s_full0 + 8 * (2 * w + (i & 1)));
+                if (w == (i < nb[1] ? 1 : 0)) mma_commit(k_empty0 + 8 * st);        // the last tile that reads the stage
+                return true;
+            };
+            for (int w = 0; w < 2 && alive; w++)
+                if (nb[w] > 0) alive = issue_s(w, 0);
+            for (int i = 0; i < n_blocks && alive; i++)
+                for (int w = 0; w < 2 && alive; w++) {
+                    if (i >= nb[w]) continue;
+                    if (i + 1 < nb[w] && !(alive = issue_s(w, i + 1))) break;
+                    const int st = i % STAGES;
+                    if (!(alive = mbar_wait(p_full0 + 8 * (2 * w + (i & 1)), (i >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL))) break;
+                    if (!(alive = mbar_wait(v_full0 + 8 * st, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_PREFILL))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TL_BN / 16; ks++)
+                        mma_bf16_ts(tmem + w * TILE_COLS + O_COL, tmem + w * TILE_COLS + (i & 1) * S_COLS + ks * 8,
+                                    desc_mnmajor(kv_s + st * 2 * TILE + TILE + ks * 16 * 128, ATOM), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
+                    if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
+                    mma_commit(pv_done0 + 8 * w);
+                }
+        }
+    } else if (Q8 && warp >= TL_WIDEN_WARP) {
+        // ---- bytes to bfloat16.  Keys outside the block's range get zero rows: what lies there may be another sequence's.
+        const int ct = threadIdx.x - TL_WIDEN_WARP * 32;
+        auto widen = [&](const unsigned char* raw, const float* own, const float* other, unsigned dst, int key0, bool keys) {
+#pragma unroll
+            for (int it = 0; it < TL_BN * D / 16 / 128; it++) {
+                const int id = ct + it * 128, rest = id >> 3;
+                const int r = (D == 128 ? rest >> 1 : rest) * 2 ^ ((id & 4) ? 5 : 0), c = (id & 3) + (D == 128 ? (rest & 1) * 4 : 0);
+                const uint4 v = *reinterpret_cast<const uint4*>(raw + (D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + c * 16));
+                const int key = key0 + r;
+                float s = own[r];
+                const float s2 = other[r];
+                const bool in = key >= first_key && key <= last_key, number = fabsf(s) < INFINITY && fabsf(s2) < INFINITY;
+                if (!in || !number) s = in && keys ? __uint_as_float(0x7fffffffu) : 0.f;
+                const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                unsigned o[8];
+                tl_widen(w, s, o);
+                const unsigned at = dst + (c >> 2) * ATOM + r * 128, p = (c & 3) * 2;
+                tl_store16(at + ((p ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+                tl_store16(at + (((p + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
+            }
+        };
+        for (int i = 0; i < n_blocks; i++) {
+            const int rs = i % TL_RAW, st = i % STAGES, key0 = (jb0 + i) * TL_BN;
+            const unsigned char* raw = smem_raw + (raw_s - base) + rs * 2 * Z::RAW_TILE;
+            const float* ks = reinterpret_cast<const float*>(smem_raw + (sc_s - base) + rs * Z::SCALES);
+            const float* vs = ks + TL_BN;
+            const unsigned kd = kv_s + st * 2 * TILE, vd = kd + TILE;
+            if (!mbar_wait(raw_full0 + 8 * rs, (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+            if (i >= STAGES && !mbar_wait(k_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+            widen(raw, ks, vs, kd, key0, true);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tl_arrive(k_full0 + 8 * st);
+            if (i >= STAGES && !mbar_wait(v_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+            widen(raw + Z::RAW_TILE, vs, ks, vd, key0, false);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tl_arrive(v_full0 + 8 * st);
+            tl_arrive(raw_empty0 + 8 * rs);
+        }
+    } else if (warp < TL_SOFTMAX) {
+        // ---- softmax: thread = row = lane of tensor memory
+        const int w = warp >> 2, r = threadIdx.x & 127, br = w * TL_BM + r;       // br: row of the block
+        const bool valid = br < n_rows;
+        int token = 0, h = hk * G, pos = last_key;
+        if (valid) {
+            if (PREFIX) {
+                token = work.members[tile.x + br / G];
+                h = hk * G + br % G;
+            } else {
+                const int i = (row0 + br) / G;
+                token = token0 + i;
+                h = hk * G + (row0 + br) % G;
+                pos = past + i;
+            }
+        }
+        // the row's query into the swizzled tile; rows behind the last one are zeros
+        {
+            const bf16* src = q + (size_t)token * q_stride + (size_t)h * D;
+#pragma unroll
+            for (int c = 0; c < D / 8; c++) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (valid) v = *reinterpret_cast<const uint4*>(src + c * 8);
+                tl_store16(q_s + w * Z::Q_TILE + (c >> 3) * Q_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tl_arrive(q_full);
+        }
+        const unsigned lane_addr = tmem + w * TILE_COLS + ((unsigned)((warp & 3) * 32) << 16);
+        const int nbw = nb[w];
+        // what the tile's rows see: everything in blocks between the last row's first key and the first row's last one
+        const int tile_first = PREFIX ? last_key : past + (row0 + w * TL_BM) / G, tile_last = PREFIX ? last_key : past + (row0 + min(n_rows, (w + 1) * TL_BM) - 1) / G;
+        const int lo_pos = PREFIX ? 0 : nbw > 0 ? first_visible(pos, work.span) : 0, lo_last = PREFIX || nbw == 0 ? 0 : first_visible(tile_last, work.span);
+        float m_ref = -INFINITY, l_run = 0.f;
+        bool alive = true;
+        for (int i = 0; i < nbw; i++) {
+            const int key0 = (jb0 + i) * TL_BN;
+            alive = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (2 * w + (i & 1)), (i >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+            if (!alive) break;
+            tc_fence_after();
+            const unsigned s_addr = lane_addr + (i & 1) * S_COLS;
+            unsigned sr[TL_BN];
+            tmem_ld32_issue(s_addr, sr);
+            tmem_ld32_issue(s_addr + 32, sr + 32);
+            tmem_wait_ld<TL_BN>(sr);
+            if (key0 + TL_BN - 1 > tile_first || key0 < lo_last) {
+#pragma unroll
+                for (int c = 0; c < TL_BN; c++)
+                    if (key0 + c > pos || key0 + c < lo_pos) sr[c] = 0xff800000u;      // -inf
+            }
+            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < TL_BN; c += 8) {
+                mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+                mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+                mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
+                mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+            }
+            const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale_log2e);
+            const bool grown = m_new > m_ref + TL_RESCALE_STEP;      // true for m_ref = -inf, m_new finite
+            bool pv_seen = false;
+            if (__any_sync(0xffffffffu, grown)) {
+                if (i > 0) {
+                    pv_seen = true;
+                    const float corr = m_new == -INFINITY ? 1.f : m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new);
+                    alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (i - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+                    if (!alive) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        unsigned o[32];
+                        tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                        tmem_wait_ld<32>(o);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+                        tmem_st32(lane_addr + O_COL + c0, o);
+                    }
+                    tmem_wait_st();
+                    l_run *= corr;
+                }
+                m_ref = m_new;
+            }
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            unsigned pr[TL_BN / 2];
+            const unsigned long long scale2 = f2_pack(scale_log2e, scale_log2e), neg_m2 = f2_pack(-m_use, -m_use);
+            unsigned long long psa = f2_pack(0.f, 0.f), psb = psa;
+#pragma unroll
+            for (int c = 0; c < TL_BN; c += 4) {
+                float x0, x1, x2, x3;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, neg_m2), x0, x1);
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, neg_m2), x2, x3);
+                const float p0 = fast_exp2(x0), p1 = fast_exp2(x1), p2 = fast_exp2(x2), p3 = fast_exp2(x3);
+                psa = f2_add(psa, f2_pack(p0, p1));
+                psb = f2_add(psb, f2_pack(p2, p3));
+                pr[c >> 1] = pack_bf16(p0, p1);
+                pr[(c >> 1) + 1] = pack_bf16(p2, p3);
+            }
+            {
+                float a0, a1, b0, b1;
+                f2_unpack(psa, a0, a1);
+                f2_unpack(psb, b0, b1);
+                l_run += (a0 + a1) + (b0 + b1);
+            }
+            tmem_st32(s_addr, pr);
+            tmem_wait_st();
+            if (!Q8 && key0 + TL_BN - 1 > last_key) {
+                // behind the prefix the page may hold anything: those rows of V are cleared (both tiles write the same zeros)
+                const int st = i % STAGES;
+                alive = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * st, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+                if (r < TL_BN && key0 + r > last_key)
+#pragma unroll
+                    for (int a = 0; a < NA; a++)
+#pragma unroll
+                        for (int c = 0; c < 8; c++) tl_store16(kv_s + st * 2 * TILE + TILE + a * ATOM + r * 128 + c * 16, 0u, 0u, 0u, 0u);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            // (every phase of pv_done is observed, in order, before this thread lets the next one begin)
+            if (i > 0 && !pv_seen) alive = __all_sync(0xffffffffu, alive && mbar_wait(pv_done0 + 8 * w, (i - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+            if (!alive) break;
+            tc_fence_before();
+            tl_arrive(p_full0 + 8 * (2 * w + (i & 1)));
+        }
+        if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (nbw - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+        const size_t head = (size_t)token * nh + h;
+        if (PREFIX) {
+            const size_t share = head * work.slots + work.slot0 + blockIdx.x;
+            if (valid) *reinterpret_cast<float2*>(work.part_ml + share * 2) = nbw > 0 ? make_float2(m_ref, l_run) : make_float2(-INFINITY, 0.f);
+            if (alive && nbw > 0) {
+                tc_fence_after();
+                float* dst = work.part_acc + share * D;
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    unsigned o[32];
+                    tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                    tmem_wait_ld<32>(o);
+                    if (valid)
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            *reinterpret_cast<float4*>(dst + c0 + c) =
+                                make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+                }
+            }
+        } else if (alive && nbw > 0) {
+            tc_fence_after();
+            const float inv = 1.0f / l_run;
+            bf16* dst = out + head * D;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                unsigned o[32];
+                tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                tmem_wait_ld<32>(o);
+                if (valid)
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] = __uint_as_float(o[c + e]) * inv;
+                        store8(dst + c0 + c, f);
+                    }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == TL_MMA_WARP) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE_COLS) : "memory");
+    }
+}
+
+// ---- host side
+
+typedef CUresult (*TlEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// an entry's pages as a matrix [pages * kv heads * page_size, d]; boxes of 64 rows of 128 bytes (eight bits: of d)
+static int tl_make_map(CUtensorMap* map, const void* ptr, long long rows, int d, bool q8) {
+    static const TlEncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess ? (TlEncodeTiledFn)p
+                                                                                                                                         : (TlEncodeTiledFn) nullptr;
+    }();
+    if (!fn) return ILLM_ERR_BAD_ARG;
+    cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)d * (q8 ? 1 : 2)};
+    cuuint32_t box[2] = {q8 ? (cuuint32_t)d : 64u, TL_BN};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, q8 && d == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : ILLM_ERR_BAD_ARG;
+}
+
+template <int D, bool Q8, bool PREFIX>
+static int tl_launch(dim3 grid, const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table,
+                     int max_pages, const TlWork& work, void* out, int nh, int nkv, int page_size, float scale, int* err, cudaStream_t s) {
+    CUtensorMap mk, mv;
+    const long long rows = n_pages * nkv * page_size;
+    int rc;
+    if ((rc = tl_make_map(&mk, kc, rows, D, Q8)) || (rc = tl_make_map(&mv, vc, rows, D, Q8))) return rc;
+    auto kern = attention_tiles_kernel<D, Q8, PREFIX>;
+    const int smem = TlSizes<D, Q8>::SMEM;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    illm_launch(kern, grid, dim3(TlSizes<D, Q8>::THREADS), smem, s, mk, mv, ksc, vsc, (const bf16*)q, q_stride, block_table, max_pages, (int)n_pages, work, (bf16*)out, nh, nkv,
+                page_size, scale * 1.4426950408889634f, err);
+    return illm_launch_status();
+}
+
+static bool tl_bad(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, int max_pages, int nh, int nkv, int page_size,
+                   const int* err) {
+    return nkv <= 0 || nh <= 0 || nh % nkv || nkv > 65535 || (q_stride & 7) || page_size <= 0 || page_size % TL_BN || max_pages <= 0 || n_pages <= 0 ||
+           n_pages * nkv * page_size > 0x7fffffffLL || !q || ((uintptr_t)q & 15) || !kc || !vc || ((uintptr_t)kc & 15) || ((uintptr_t)vc & 15) || (!ksc) != (!vsc) ||
+           ((uintptr_t)ksc & 15) || ((uintptr_t)vsc & 15) || !err;
+}
+
+// Prompts over rows of eight bits: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages of bytes
+// [n_pages, nkv, page_size, d] and their scales; cu_q [B + 1], seq_lens [B] as for attention_prefill_tc; out [T, nh * d].  tile_rows: 128 or 256.
+// d 64 or 128, page_size a multiple of 64.  span: see first_visible.  err: 5 a wait ran out, 6 shared memory, 8 a visible position without a page.
+extern "C" int illm_attention_tiles_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
+                                         const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d,
+                                         int page_size, int span, float scale, int tile_rows, int* err, void* stream) {
+    if (B <= 0 || max_q <= 0) return 0;
+    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || !ksc || B > 65535 || (tile_rows != TL_BM && tile_rows != 2 * TL_BM) || !out ||
+        ((uintptr_t)out & 15))
+        return ILLM_ERR_BAD_ARG;
+    const long long tiles = ((long long)max_q * (nh / nkv) + tile_rows - 1) / tile_rows;
+    if (tiles > 65535 || (long long)max_q * (nh / nkv) > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;
+    TlWork work = {};
+    work.cu_q = cu_q;
+    work.seq_lens = seq_lens;
+    work.span = span;
+    work.tile_rows = tile_rows;
+    const dim3 grid((unsigned)nkv, (unsigned)tiles, (unsigned)B);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (d == 128) return tl_launch<128, true, false>(grid, q, q_stride, kc, vc, ksc, vsc, n_pages, block_table, max_pages, work, out, nh, nkv, page_size, scale, err, s);
+    if (d == 64) return tl_launch<64, true, false>(grid, q, q_stride, kc, vc, ksc, vsc, n_pages, block_table, max_pages, work, out, nh, nkv, page_size, scale, err, s);
+    return ILLM_ERR_BAD_ARG;
+}
+
+// The shares of common prefixes (ksc, vsc nullptr: bfloat16 pages): for every tile of the plan (at most 256 / (nh / nkv) members) and every one of `splits` parts of its
+// positions, for every (member, head) the accumulators, maximum (in units of log2) and sum at share slot0 + part of `slots`: part_acc float [T, nh, slots, d],
+// part_ml float [T, nh, slots, 2].  illm_attention_pages_join adds them up with the others.
+extern "C" int illm_attention_tiles_prefix(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
+                                           const int* block_table, int max_pages, const int* token_seq, const int* plan_tiles, const int* plan_members, int n_tiles,
+                                           float* part_acc, float* part_ml, int nh, int nkv, int d, int page_size, float scale, int slots, int slot0, int splits, int* err,
+                                           void* stream) {
+    if (n_tiles <= 0) return 0;
+    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || nh / nkv > 2 * TL_BM || n_tiles > 65535 || splits < 1 || splits > 65535 || slot0 < 0 ||
+        slot0 + splits > slots || !part_acc || !part_ml || ((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || !plan_tiles || ((uintptr_t)plan_tiles & 15) || !plan_members)
+        return ILLM_ERR_BAD_ARG;
+    TlWork work = {};
+    work.tiles = reinterpret_cast<const int4*>(plan_tiles);
+    work.members = plan_members;
+    work.token_seq = token_seq;
+    work.slots = slots;
+    work.slot0 = slot0;
+    work.part_acc = part_acc;
+    work.part_ml = part_ml;
+    const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)n_tiles);
+    cudaStream_t s = (cudaStream_t)stream;
+#define TL_CASE(DD, QQ)                                                                                                                                           \
+    if (d == DD && (ksc != nullptr) == QQ)                                                                                                                        \
+        return tl_launch<DD, QQ, true>(grid, q, q_stride, kc, vc, ksc, vsc, n_pages, block_table, max_pages, work, nullptr, nh, nkv, page_size, scale, err, s);
+    TL_CASE(128, true) TL_CASE(64, true) TL_CASE(128, false) TL_CASE(64, false)
+#undef TL_CASE
+    return ILLM_ERR_BAD_ARG;
+}

@@ -37,6 +37,20 @@ int illm_attention_mixed_keys_per_tile(int nh, int nkv, int d, int esize, int ha
 int illm_attention_mixed_tc_supported(int nh, int nkv, int d);
 int illm_attention_mixed_tc(const void* q, int q_stride, const void* kc, const int* block_table, int max_pages, const int* token_pos, const int* cu_q, int B, void* out, int T, int nh, int nkv, int d, int page_size, int window, float scale, const float* r1, const float* r2, const float* mix, const float* gate, int gate_stride, int n_sms, void* stream);
 
+// kv_int8.cu
+int illm_kv_write_int8(const void* qkv, const float* partials, int splits, long long split_stride, void* q_out, const float* cos_sin, const int* token_pos, const int* token_seq, const int* block_table, int max_pages, long long n_pages, void* kc, void* vc, float* ksc, float* vsc, int act_dtype, int T, int nh, int nkv, int d, int rot, int page_size, int write_kv, int table_positions, int* err, void* stream);
+int illm_kv_read_int8(const void* kc, const void* vc, const float* ksc, const float* vsc, const int* token_pos, const int* token_seq, const int* block_table, int max_pages, long long n_pages, void* k_out, void* v_out, int dtype, long long n, int nkv, int d, int page_size, void* stream);
+
+// attention_int8.cu
+int illm_attention_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, const int* block_table, int max_pages, long long n_pages, const int* token_pos, const int* token_seq, void* out, int act_dtype, int T, int nh, int nkv, int d, int page_size, int span, float scale, int* err, void* stream);
+
+// attention_pages.cu
+int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles, const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size, int span, float scale, int own_splits, int pre_splits, int* err, void* stream);
+
+// attention_tiles.cu
+int illm_attention_tiles_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d, int page_size, int span, float scale, int tile_rows, int* err, void* stream);
+int illm_attention_tiles_prefix(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* token_seq, const int* plan_tiles, const int* plan_members, int n_tiles, float* part_acc, float* part_ml, int nh, int nkv, int d, int page_size, float scale, int slots, int slot0, int splits, int* err, void* stream);
+
 // attention_prefill.cu
 int illm_attention_prefill(const void* q, int q_stride, const void* kc, const void* vc, const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d, int page_size, int window, float scale, void* stream);
 

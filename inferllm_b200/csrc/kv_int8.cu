@@ -1,0 +1,228 @@
+// Rows of keys and values in eight bits: rotated, rounded and written into the paged cache in one pass, and read back.
+//
+// A row is the d values of one position and kv head.  With a = max |x| over it, its scale is s = a / 127 and a value is kept as
+// u = 128 + round(x / s) (ties to even), so that it stands for (u - 128) s: at most a / 254 from x.  Pages: u
+// [pages, kv heads, page_size, d] bytes, scales float32 [pages, kv heads, page_size] beside them.  The zero point of 128 keeps u
+// unsigned: an attention kernel makes 1024 + u in half precision by putting the byte into the mantissa.
+// One scale per row, not per page: rows come one at a time and are never rounded again.  A row whose largest value is below
+// 2^-100 stands for zeros (s = 0; its quotients would leave float32), one with an infinity or a NaN reads back as NaN.
+//
+// The write does what rope_kv.cu does for a cache of wider rows (src/kern/naive/naive.cpp:389-414 for the rotation, src/core/op.cpp:414-416 for
+// the rows' way into the cache; the reference keeps float32 rows only): pair (j, j + rot / 2) of every query and key head is turned by the position's angle,
+// from a table; the arithmetic is float32, and keys and values are rounded once, to eight bits.  The queries leave in the
+// activations' type, in a matrix of their own.
+// Memory bounds it: a projection row is read once, 1 + 4 / d bytes per element are written.  A row belongs to the fewest lanes
+// (8, 16 or 32) that hold it with eight channels each, so that the maximum is a few shuffles, and a thread keeps its channels'
+// cos and sin for several heads of its token.
+#include "common.cuh"
+
+#define KQ_THREADS 256
+#define KQ_TINY 7.888609e-31f       // 2^-100
+
+// channels 8c .. 8c+7 of a row of d values that starts at element `row` of the projection (or the sum of its K slices)
+template <typename TA, bool PARTIALS>
+__device__ __forceinline__ void kq_fetch(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at, float* f) {
+    if (!PARTIALS) {
+        load8(x + at, f);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) f[k] = 0.f;
+    for (int z = 0; z < splits; z++) {
+        float p[8];
+        load8(partials + (size_t)z * stride + at, p);
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[k] += p[k];
+    }
+}
+template <typename TA, bool PARTIALS>
+__device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
+    if (!PARTIALS) return to_f32(x[at]);
+    float f = 0.f;
+    for (int z = 0; z < splits; z++) f += partials[(size_t)z * stride + at];
+    return f;
+}
+
+// LANES: lanes of a row.  WIDE: the rotated halves are whole pieces of eight channels (rot a multiple of 16); otherwise a thread
+// fetches its channels' partners one by one.  A block takes `per_block` heads of one token.
+template <typename TA, bool PARTIALS, bool WIDE, int LANES>
+__global__ void __launch_bounds__(KQ_THREADS)
+kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ partials, int splits, long long split_stride, TA* __restrict__ q_out,
+                     const float2* __restrict__ cs, const int* __restrict__ token_pos, const int* __restrict__ token_seq,
+                     const int* __restrict__ block_table, int max_pages, int n_pages, unsigned char* __restrict__ kc, unsigned char* __restrict__ vc,
+                     float* __restrict__ ksc, float* __restrict__ vsc, int nh, int nkv, int d, int rot, int page_size, int write_kv,
+                     int table_positions, int per_block, int* __restrict__ err) {
+    pdl_grid_sync();
+    const int t = blockIdx.x, c = threadIdx.x & (LANES - 1), half = rot >> 1, n_slots = nh + 2 * nkv;
+    const bool active = c * 8 < d;
+    const int p = token_pos[t];
+    if (p < 0 || (half > 0 && p >= table_positions)) {
+        if (threadIdx.x == 0) atomicExch(err, 3);
+        return;
+    }
+    int page = -1;
+    if (write_kv) {
+        if (p / page_size < max_pages) page = block_table[(size_t)token_seq[t] * max_pages + p / page_size];
+        if (page < 0 || page >= n_pages) {
+            if (threadIdx.x == 0) atomicExch(err, 2);
+            page = -1;
+        }
+    }
+    const int hc = half >> 3;                   // WIDE: pieces of a rotated half
+    const bool turned = active && c * 8 < rot;
+    float2 turn[8];
+    if (WIDE && turned) {
+        const float2* row = cs + (size_t)p * half + (c < hc ? c : c - hc) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            const float4 v = *reinterpret_cast<const float4*>(row + k);
+            turn[k] = make_float2(v.x, v.y);
+            turn[k + 1] = make_float2(v.z, v.w);
+        }
+    }
+    const int s0 = blockIdx.y * per_block + threadIdx.x / LANES, s1 = min(n_slots, (int)(blockIdx.y + 1) * per_block);
+    // (the lanes of a row run together: s0 is the same for all of them, and shuffles stay within the row)
+    const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) & ~(LANES - 1));
+    for (int slot = s0; slot < s1; slot += KQ_THREADS / LANES) {
+        const bool is_q = slot < nh, is_k = !is_q && slot < nh + nkv;
+        if (!is_q && page < 0) break;           // queries come first
+        const size_t at = ((size_t)t * n_slots + slot) * d;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (active) kq_fetch<TA, PARTIALS>(qkv, partials, splits, split_stride, at + c * 8, x);
+        if (turned && (is_q || is_k)) {
+            if (WIDE) {
+                float y[8];
+                kq_fetch<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (c < hc ? c + hc : c - hc) * 8, y);
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = c < hc ? x[k] * turn[k].x - y[k] * turn[k].y : y[k] * turn[k].y + x[k] * turn[k].x;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int i = c * 8 + k, j = i < half ? i : i - half;
+                    if (i >= rot) continue;
+                    const float2 w = cs[(size_t)p * half + j];
+                    const float y = kq_fetch1<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (i < half ? i + half : j));
+                    x[k] = i < half ? x[k] * w.x - y * w.y : y * w.y + x[k] * w.x;
+                }
+            }
+        }
+        if (is_q) {
+            if (active) store8(q_out + ((size_t)t * nh + slot) * d + c * 8, x);
+            continue;
+        }
+        // the largest magnitude as bits: unsigned order is that of the values, with infinities and then NaNs above them
+        unsigned top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+        const float a = __uint_as_float(top);
+        const bool finite = top < 0x7f800000u, tiny = finite && a < KQ_TINY;
+        const float scale = !finite ? __uint_as_float(0x7fffffffu) : tiny ? 0.f : a / 127.f, inv = !finite || tiny ? 0.f : 127.f / a;
+        const int hk = is_k ? slot - nh : slot - nh - nkv;
+        const size_t row = ((size_t)page * nkv + hk) * page_size + p % page_size;
+        unsigned u[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) u[k] = finite ? (unsigned)(128 + min(127, max(-127, __float2int_rn(x[k] * inv)))) : 128u;
+        if (active)
+            *reinterpret_cast<uint2*>((is_k ? kc : vc) + row * d + c * 8) =
+                make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24, u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
+        if (c == 0) (is_k ? ksc : vsc)[row] = scale;
+    }
+}
+
+// rows of given positions, (u - 128) s in the activations' type: k, v [T, kv heads, d]; a position without a page reads back as NaN
+template <typename TA>
+__global__ void __launch_bounds__(KQ_THREADS)
+kv_read_int8_kernel(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, const float* __restrict__ ksc, const float* __restrict__ vsc,
+                    const int* __restrict__ token_pos, const int* __restrict__ token_seq, const int* __restrict__ block_table, int max_pages, int n_pages,
+                    TA* __restrict__ k_out, TA* __restrict__ v_out, long long n, int nkv, int d, int page_size) {
+    pdl_grid_sync();
+    const long long i = (long long)blockIdx.x * KQ_THREADS + threadIdx.x;
+    const int pieces = d >> 3;
+    if (i >= n * nkv * pieces) return;
+    const int c = (int)(i % pieces), hk = (int)(i / pieces % nkv);
+    const long long t = i / pieces / nkv;
+    const int p = token_pos[t];
+    const int page = p >= 0 && p / page_size < max_pages ? block_table[(size_t)token_seq[t] * max_pages + p / page_size] : -1;
+    const bool held = page >= 0 && page < n_pages;
+    const size_t row = held ? ((size_t)page * nkv + hk) * page_size + p % page_size : 0;
+    const float nan = __uint_as_float(0x7fffffffu);
+    auto one = [&](const unsigned char* cache, const float* scales, TA* out) {
+        const uint2 v = *reinterpret_cast<const uint2*>(cache + row * d + c * 8);
+        const float s = held ? scales[row] : nan;
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[k] = (float)((int)((k < 4 ? v.x : v.y) >> (8 * (k & 3)) & 255u) - 128) * s;
+        store8(out + (t * nkv + hk) * d + c * 8, f);
+    };
+    one(kc, ksc, k_out);
+    one(vc, vsc, v_out);
+}
+
+// qkv: the packed projection [T, (nh + 2 nkv) d] of dtype act_dtype, or (partials) its float32 K slices [splits][T][...], added in
+// ascending order.  q_out [T, nh d].  kc, vc: one entry's pages; ksc, vsc their scales.  d a multiple of 8 up to 256; rot even, up to d;
+// write_kv 0: the rotation alone.  err: 2 a position without a page, 3 one outside the table.
+extern "C" int illm_kv_write_int8(const void* qkv, const float* partials, int splits, long long split_stride, void* q_out, const float* cos_sin,
+                                  const int* token_pos, const int* token_seq, const int* block_table, int max_pages, long long n_pages, void* kc, void* vc,
+                                  float* ksc, float* vsc, int act_dtype, int T, int nh, int nkv, int d, int rot, int page_size, int write_kv,
+                                  int table_positions, int* err, void* stream) {
+    if (T <= 0) return 0;
+    if (nh <= 0 || nkv <= 0 || d <= 0 || d > 256 || (d & 7) || rot < 0 || rot > d || (rot & 1) || (rot > 0 && !cos_sin) || page_size <= 0 || max_pages <= 0 ||
+        n_pages > 0x7fffffffLL || (act_dtype != ILLM_BF16 && act_dtype != ILLM_F32) || (partials ? splits < 1 : !qkv) || !q_out || !err)
+        return ILLM_ERR_BAD_ARG;
+    if (write_kv && (!kc || !vc || !ksc || !vsc || ((uintptr_t)kc & 7) || ((uintptr_t)vc & 7))) return ILLM_ERR_BAD_ARG;
+    if (((uintptr_t)qkv & 15) || ((uintptr_t)partials & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)cos_sin & 15)) return ILLM_ERR_BAD_ARG;
+    const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, at_once = KQ_THREADS / lanes;
+    const int n_slots = nh + (write_kv ? 2 * nkv : 0), rounds_all = (n_slots + at_once - 1) / at_once;
+    // several heads to a thread once that leaves eight blocks to every SM
+    int rounds = 1;
+    while (rounds < rounds_all && (long long)T * ((rounds_all + rounds) / (rounds + 1)) >= 8LL * illm_sm_count()) rounds++;
+    const dim3 grid((unsigned)T, (unsigned)((rounds_all + rounds - 1) / rounds));
+    if (grid.y > 65535) return ILLM_ERR_BAD_ARG;
+    cudaStream_t s = (cudaStream_t)stream;
+    const bool wide = (rot & 15) == 0;
+#define KQ_RUN(TA, PART, W, L)                                                                                                                  \
+    illm_launch(kv_write_int8_kernel<TA, PART, W, L>, grid, dim3(KQ_THREADS), 0, s, (const TA*)qkv, partials, splits, split_stride, (TA*)q_out, \
+                (const float2*)cos_sin, token_pos, token_seq, block_table, max_pages, (int)n_pages, (unsigned char*)kc, (unsigned char*)vc, ksc, vsc, nh, \
+                nkv, d, rot, page_size, write_kv, table_positions, rounds * at_once, err)
+#define KQ_LANES(TA, PART, W)                  \
+    do {                                       \
+        if (lanes == 8) KQ_RUN(TA, PART, W, 8); \
+        else if (lanes == 16) KQ_RUN(TA, PART, W, 16); \
+        else KQ_RUN(TA, PART, W, 32);          \
+    } while (0)
+#define KQ_WIDE(TA, PART)                  \
+    do {                                   \
+        if (wide) KQ_LANES(TA, PART, true); \
+        else KQ_LANES(TA, PART, false);    \
+    } while (0)
+    if (act_dtype == ILLM_BF16 && partials) KQ_WIDE(bf16, true);
+    else if (act_dtype == ILLM_BF16) KQ_WIDE(bf16, false);
+    else if (partials) return ILLM_ERR_BAD_ARG;
+    else KQ_WIDE(float, false);
+#undef KQ_WIDE
+#undef KQ_LANES
+#undef KQ_RUN
+    return illm_launch_status();
+}
+
+// k_out, v_out [n, nkv, d] of dtype `dtype`: the rows of n positions (token_pos, token_seq int32 [n]).
+extern "C" int illm_kv_read_int8(const void* kc, const void* vc, const float* ksc, const float* vsc, const int* token_pos, const int* token_seq,
+                                 const int* block_table, int max_pages, long long n_pages, void* k_out, void* v_out, int dtype, long long n, int nkv, int d,
+                                 int page_size, void* stream) {
+    if (n <= 0) return 0;
+    if (nkv <= 0 || d <= 0 || d > 256 || (d & 7) || page_size <= 0 || max_pages <= 0 || n_pages <= 0 || n_pages > 0x7fffffffLL || !kc || !vc || !ksc || !vsc || ((uintptr_t)kc & 7) ||
+        ((uintptr_t)vc & 7) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || (dtype != ILLM_BF16 && dtype != ILLM_F32))
+        return ILLM_ERR_BAD_ARG;
+    const long long blocks = (n * nkv * (d / 8) + KQ_THREADS - 1) / KQ_THREADS;
+    if (blocks > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == ILLM_BF16)
+        illm_launch(kv_read_int8_kernel<bf16>, dim3((unsigned)blocks), dim3(KQ_THREADS), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
+                    token_seq, block_table, max_pages, (int)n_pages, (bf16*)k_out, (bf16*)v_out, n, nkv, d, page_size);
+    else
+        illm_launch(kv_read_int8_kernel<float>, dim3((unsigned)blocks), dim3(KQ_THREADS), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
+                    token_seq, block_table, max_pages, (int)n_pages, (float*)k_out, (float*)v_out, n, nkv, d, page_size);
+    return illm_launch_status();
+}

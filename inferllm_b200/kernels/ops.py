@@ -61,6 +61,12 @@ _KERNEL_SIGNATURES = {
     "illm_attention_decode_ring": [P_, I_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, I_, I_, I_, I_, I_, F_, I_, P_, P_],
     "illm_attention_decode_ring_rope": [P_, P_, I_, LL_, P_, I_, I_, I_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, I_, I_, I_, I_, I_,
                                         F_, I_, P_, P_, P_],
+    "illm_kv_write_int8": [P_, P_, I_, LL_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, I_, I_, P_, P_],
+    "illm_kv_read_int8": [P_, P_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, I_, LL_, I_, I_, I_, P_],
+    "illm_attention_int8": [P_, I_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, P_, P_],
+    "illm_attention_pages": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, F_, I_, I_, P_, P_],
+    "illm_attention_tiles_int8": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, I_, P_, P_],
+    "illm_attention_tiles_prefix": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, P_, P_, I_, I_, I_, I_, F_, I_, I_, I_, P_, P_],
     "illm_attention_prefill": [P_, I_, P_, P_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, P_],
     "illm_gemm_bf16_tc": [P_, P_, P_, I_, I_, I_, I_, P_, I_, P_, P_, I_],
     "illm_splitk_reduce": [P_, P_, I_, LL_, I_, P_],
@@ -924,6 +930,281 @@ def linear_adapters(x, w, adapters, rows, out_dtype=None):
         ws = x.new_empty(rows.ws_bytes(code, N, K, adapters.R), dtype=torch.uint8)
         _check(lib.illm_linear_adapters(px, pw, code, T, N, K, a, b, scales, adapters.count, adapters.R, rows.plan_ptr, rows.slots, rows.groups, rows.chunks,
                                         out.data_ptr(), _DT[out_dtype], ws.data_ptr(), 0, _error_word(device), _stream()), "linear_adapters")
+    return out
+
+
+# ---- a cache of eight-bit rows, and positions that sequences hold in common
+
+class CacheInt8:
+    """Keys and values of one cache entry in eight bits: `k`, `v` uint8 [pages, kv heads, page_size, head_dim] and `k_scale`,
+    `v_scale` float32 [pages, kv heads, page_size].  A row (the values of one position and kv head) stands for
+    (u - 128) * scale; `kv_write_int8` makes it with scale = max|x| / 127."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        for name, t in (("k", k), ("v", v)):
+            _need(t, name, torch.uint8, 4)
+            if t.shape != k.shape or t.device != k.device:
+                raise KernelError(f"cache: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _need(t, name, torch.float32, 3)
+            if t.shape != k.shape[:3] or t.device != k.device:
+                raise KernelError(f"cache: {name} {tuple(t.shape)} does not fit pages {tuple(k.shape)}")
+        if any(t.data_ptr() & 15 for t in (k, v, k_scale, v_scale)):
+            raise KernelError("cache: pages and scales must start on 16-byte boundaries")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        if min(k.shape) < 1 or self.head_dim % 8 or self.head_dim > MAX_HEAD_DIM_GENERIC:
+            raise KernelError(f"cache: pages {tuple(k.shape)}: head sizes are multiples of 8 up to {MAX_HEAD_DIM_GENERIC}")
+        if k.numel() // self.head_dim >= 2 ** 31:
+            raise KernelError(f"cache: pages {tuple(k.shape)} have more than 2^31 rows")
+        self.device = k.device
+        self.pointers = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+
+    @classmethod
+    def empty(cls, pages, n_kv_heads, page_size, head_dim, device="cuda"):
+        """Room for so many pages; what lies in them is nobody's."""
+        def rows(dtype, *more):
+            return torch.empty((pages, n_kv_heads, page_size) + more, dtype=dtype, device=device)
+        return cls(rows(torch.uint8, head_dim), rows(torch.uint8, head_dim), rows(torch.float32), rows(torch.float32))
+
+
+def _page_entry(cache):
+    """Of a cache entry (CacheInt8 or a bfloat16 pair (k, v)): its device, pages, kv heads, page size, head size and pointers."""
+    if isinstance(cache, CacheInt8):
+        return cache.device, cache.pages, cache.n_kv_heads, cache.page_size, cache.head_dim, cache.pointers
+    k, v = cache
+    _need(k, "k", torch.bfloat16, 4)
+    _need(v, "v", torch.bfloat16, 4)
+    if k.shape != v.shape or k.device != v.device or min(k.shape) < 1:
+        raise KernelError(f"cache: k {tuple(k.shape)} and v {tuple(v.shape)} must be alike and not empty")
+    return (k.device,) + tuple(k.shape) + ((k.data_ptr(), v.data_ptr(), None, None),)
+
+
+def _step_arrays(device, T, block_table, **arrays):
+    if block_table.device != device:
+        raise KernelError(f"block_table is on {block_table.device}, the cache on {device}")
+    _need(block_table, "block_table", torch.int32, 2)
+    if block_table.shape[1] < 1:
+        raise KernelError("block_table must have at least one page per sequence")
+    for name, t in arrays.items():
+        _need(t, name, torch.int32, 1)
+        if t.device != device or (T is not None and t.numel() != T):
+            raise KernelError(f"{name} must be int32 [{T}] on {device}, found {tuple(t.shape)} on {t.device}")
+
+
+def _query_rows(q, device, n_heads, n_kv_heads, head_dim):
+    """The query heads in the first n_heads * head_dim columns of q (rows may lie further apart): rows and their distance."""
+    if not q.is_cuda or q.dim() != 2 or q.device != device:
+        raise KernelError(f"q must be a matrix on {device}, found shape {tuple(q.shape)} on {q.device}")
+    act_code(q.dtype)
+    if n_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"attention: {n_heads} heads are no multiple of {n_kv_heads} kv heads")
+    if q.shape[1] < n_heads * head_dim:
+        raise KernelError(f"q has {q.shape[1]} columns, {n_heads} heads of {head_dim} need {n_heads * head_dim}")
+    if q.shape[0] and (q.stride(1) != 1 or q.stride(0) < q.shape[1]):
+        raise KernelError("q: a row's elements must lie side by side")
+    if q.numel() and (q.data_ptr() & 15 or (q.shape[0] > 1 and q.stride(0) * q.element_size() & 15)):
+        raise KernelError("q: rows must start on 16-byte boundaries")
+    return q.shape[0], max(q.stride(0), q.shape[1])
+
+
+def kv_write_int8(qkv, cos_sin, rot_dim, token_pos, token_seq, block_table, cache, n_heads, err):
+    """Rotate the queries and keys of the packed projection [T, (heads + 2 kv heads) * head_dim] and write keys and values into
+    the pages of `cache` (CacheInt8) in eight bits.
+    `cos_sin` float32 [positions, rot_dim/2, 2] or None with rot_dim 0.  Returns the rotated queries [T, heads * head_dim], a
+    new tensor; `qkv` may be `SplitKPartials`.  `err` (int32 [1]): 2 for a position without a page, 3 for one beyond the table;
+    such a token's rows are not written.  Two tokens of one call must not name the same position."""
+    if not isinstance(cache, CacheInt8):
+        raise KernelError("kv_write_int8 writes a CacheInt8")
+    d, nkv = cache.head_dim, cache.n_kv_heads
+    partials = qkv if isinstance(qkv, SplitKPartials) else None
+    dtype = torch.bfloat16 if partials is not None else qkv.dtype
+    if partials is None:
+        _need(qkv, "qkv", None, 2)
+    code = act_code(dtype)
+    if tuple(qkv.shape)[1] != (n_heads + 2 * nkv) * d or n_heads < 1:
+        raise KernelError(f"qkv width {tuple(qkv.shape)[1]} is not (heads + 2 kv heads) * head_dim")
+    if qkv.device != cache.device or err.device != cache.device:
+        raise KernelError("qkv, err and the cache must be on one device")
+    T = qkv.shape[0]
+    _need(err, "err", torch.int32)
+    _step_arrays(cache.device, T, block_table, token_pos=token_pos, token_seq=token_seq)
+    if rot_dim < 0 or rot_dim > d or rot_dim % 2:
+        raise KernelError(f"rot_dim {rot_dim} must be even and at most the head size {d}")
+    n_pos = 0
+    if rot_dim:
+        if cos_sin is None:
+            raise KernelError("a rotation needs its cos/sin table")
+        _need(cos_sin, "cos_sin", torch.float32, 3)
+        if cos_sin.shape[1] != rot_dim // 2 or cos_sin.shape[2] != 2 or cos_sin.device != cache.device:
+            raise KernelError("cos_sin table does not match rot_dim")
+        if cos_sin.data_ptr() & 15:
+            raise KernelError("cos_sin must start on a 16-byte boundary")
+        n_pos = cos_sin.shape[0]
+    with _on(cache.device):
+        q = _rows(T, n_heads * d, dtype, cache.device)
+        _check(load().illm_kv_write_int8(
+            None if partials is not None else _ptr(qkv), None if partials is None else _ptr(partials.ws), 0 if partials is None else partials.splits,
+            0 if partials is None else partials.rows * partials.cols, _ptr(q), _ptr(cos_sin) if rot_dim else None, _ptr(token_pos), _ptr(token_seq),
+            _ptr(block_table), block_table.shape[1], cache.pages, *cache.pointers, code, T, n_heads, nkv, d, rot_dim, cache.page_size, 1, n_pos, _ptr(err),
+            _stream()), "kv_write_int8")
+    return q
+
+
+def kv_read_int8(cache, token_pos, token_seq, block_table, dtype=torch.bfloat16):
+    """What the rows of given positions stand for: keys and values [n, kv heads, head_dim] of `dtype`.  A position without a page reads as
+    NaN."""
+    if not isinstance(cache, CacheInt8):
+        raise KernelError("kv_read_int8 reads a CacheInt8")
+    n, code = token_pos.numel(), act_code(dtype)
+    _step_arrays(cache.device, n, block_table, token_pos=token_pos, token_seq=token_seq)
+    with _on(cache.device):
+        k = torch.empty((n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+        v = torch.empty_like(k)
+        _check(load().illm_kv_read_int8(*cache.pointers, _ptr(token_pos), _ptr(token_seq), _ptr(block_table), block_table.shape[1], cache.pages, _ptr(k), _ptr(v),
+                                        code, n, cache.n_kv_heads, cache.head_dim, cache.page_size, _stream()), "kv_read_int8")
+    return k, v
+
+
+def attention_int8_tc_supported(dtype, n_heads, n_kv_heads, head_dim, page_size, decode) -> bool:
+    """Whether the tensor-core kernels take these sizes (the engine's rule); the others go to the plain kernel."""
+    return (dtype == torch.bfloat16 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and page_size % 64 == 0
+            and (not decode or n_heads // n_kv_heads <= 16))
+
+
+def _attention_int8_plain(q, stride, cache, block_table, token_pos, token_seq, n_heads, span, scale):
+    T = q.shape[0]
+    out = _rows(T, n_heads * cache.head_dim, q.dtype, cache.device)
+    _check(load().illm_attention_int8(_ptr(q), stride, *cache.pointers, _ptr(block_table), block_table.shape[1], cache.pages, _ptr(token_pos), _ptr(token_seq), _ptr(out),
+                                      act_code(q.dtype), T, n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size, span, float(scale),
+                                      _error_word(cache.device), _stream()), "attention_int8")
+    return out
+
+
+def _pages_splits(pairs, keys, wide=False) -> int:
+    return int(_b.lib().illm_policy_pages_splits(int(pairs), int(keys), int(wide), n_sms_of_device()))
+
+
+def _check_max_len(max_len):
+    if int(max_len) < 1:
+        raise KernelError(f"max_len must be positive, found {max_len}")
+
+
+def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, window, scale, max_len, splits=None):
+    """Attention of single tokens over a cache of eight-bit rows: q [T, >= heads * head_dim] (rotated query heads first), the token's own position
+    included.  `window` as elsewhere (0 all, negative: chunks).  `max_len` bounds the sequences' lengths (it sizes the grid, not the result).
+    Returns [T, heads * head_dim].  bfloat16 with head sizes 64 and 128 and pages of a multiple of 64 positions runs on tensor cores, everything else
+    (float32 among it) on a plain kernel."""
+    if not isinstance(cache, CacheInt8):
+        raise KernelError("attention_decode_int8 reads a CacheInt8")
+    d, nkv, span = cache.head_dim, cache.n_kv_heads, int(window or 0)
+    T, stride = _query_rows(q, cache.device, n_heads, nkv, d)
+    _step_arrays(cache.device, T, block_table, token_pos=token_pos, token_seq=token_seq)
+    _check_max_len(max_len)
+    with _on(cache.device):
+        if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, cache.page_size, True):
+            return _attention_int8_plain(q, stride, cache, block_table, token_pos, token_seq, n_heads, span, scale)
+        out = torch.empty((T, n_heads * d), dtype=torch.bfloat16, device=cache.device)
+        keys = min(int(max_len), abs(span)) if span else int(max_len)
+        for t0 in range(0, T, 65535):
+            t1 = min(T, t0 + 65535)
+            n = _pages_splits((t1 - t0) * nkv, keys) if splits is None else int(splits)
+            acc, ml = _shares(t1 - t0, n_heads, n, d, cache.device)
+            _check(load().illm_attention_pages(_ptr(q[t0:t1]), stride, *cache.pointers, cache.pages, _ptr(block_table), block_table.shape[1], _ptr(token_pos[t0:t1]),
+                                               _ptr(token_seq[t0:t1]), None, None, None, 0, _ptr(acc), _ptr(ml), _ptr(out[t0:t1]), t1 - t0, n_heads, nkv, d,
+                                               cache.page_size, span, float(scale), n, 0, _error_word(cache.device), _stream()), "attention_decode_int8")
+    return out
+
+
+def _shares(T, n_heads, slots, d, device):
+    """Scratch of attention_pages."""
+    if slots == 1:
+        return None, None
+    ws = torch.empty(T * n_heads * slots * (d + 2), dtype=torch.float32, device=device)
+    cut = T * n_heads * slots * d
+    return ws[:cut], ws[cut:]
+
+
+def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads, window, scale, tile_rows=None):
+    """Attention of whole prompts (or chunks that continue a sequence) over a cache of eight-bit rows, the step's own rows written already.
+    `cu_q` int32 [B + 1], `seq_lens` int32 [B] (after the step) and `max_q` as for `attention_prefill_tc`.  Returns [T, heads * head_dim].  bfloat16 with head
+    sizes 64 and 128 and pages of a multiple of 64 positions."""
+    if not isinstance(cache, CacheInt8):
+        raise KernelError("attention_prompts_int8 reads a CacheInt8")
+    d, nkv, B = cache.head_dim, cache.n_kv_heads, seq_lens.numel()
+    T, stride = _query_rows(q, cache.device, n_heads, nkv, d)
+    _step_arrays(cache.device, B, block_table, seq_lens=seq_lens)
+    _step_arrays(cache.device, B + 1, block_table, cu_q=cu_q)
+    if int(max_q) < 0 or int(max_q) > T:
+        raise KernelError(f"max_q {max_q} is outside the step's {T} tokens")
+    if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, cache.page_size, False):
+        raise KernelError(f"attention_prompts_int8 takes bfloat16, head sizes 64 and 128 and pages of a multiple of 64 positions, found {q.dtype}, {d} and "
+                          f"{cache.page_size} (attention_decode_int8 takes prompts of other sizes token by token)")
+    with _on(cache.device):
+        out = _rows(T, n_heads * d, torch.bfloat16, cache.device)
+        if T and B:
+            rows = int(_b.lib().illm_policy_tile_rows(B, int(max_q), n_heads, nkv, n_sms_of_device())) if tile_rows is None else int(tile_rows)
+            _check(load().illm_attention_tiles_int8(_ptr(q), stride, *cache.pointers, cache.pages, _ptr(block_table), block_table.shape[1], _ptr(cu_q), _ptr(seq_lens),
+                                                    _ptr(out), B, int(max_q), n_heads, nkv, d, cache.page_size, int(window or 0), float(scale), rows,
+                                                    _error_word(cache.device), _stream()), "attention_prompts_int8")
+    return out
+
+
+class SharedPrefixes:
+    """Which tokens of a step (one per sequence) see their first positions in common: `groups` of (positions, [tokens]), whose block tables name
+    the same pages for those positions; `lens` [T] on the host: the positions that each token sees, its own included; `group_heads`: query heads per kv
+    head (at most 16).  Made once per step and used for every layer.  Tokens in no group are served too."""
+
+    def __init__(self, groups, lens, group_heads, device=None):
+        groups = [(int(p), [int(t) for t in m]) for p, m in groups]
+        lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
+        self.T, self.group_heads = len(lens), int(group_heads)
+        self.device = torch.empty(0, device="cuda" if device is None else device).device
+        sizes, total = (ctypes.c_int * 6)(), ctypes.c_int()
+        args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), self.T,
+                self.group_heads, sizes, ctypes.byref(total))
+        _b.check(_b.lib().illm_prefix_plan(*args, None))
+        host = torch.zeros(max(1, total.value), dtype=torch.int32)
+        _b.check(_b.lib().illm_prefix_plan(*args, ctypes.cast(host.data_ptr(), _b.PI)))
+        self.tiles, self.wide, self.longest_prefix, self.longest_rest = sizes[0], bool(sizes[1]), sizes[2], sizes[3]
+        self.longest = max(lens)
+        self.host = host
+        self.plan = host.to(self.device)
+        at = self.plan.data_ptr()
+        self.pointers = at + 4 * sizes[4], at, at + 4 * sizes[5]         # start, tiles, members
+
+
+def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n_heads, scale, max_len, own_splits=None, pre_splits=None):
+    """Attention of single tokens whose sequences hold first positions in common (`plan`, SharedPrefixes): a group's common keys are read once for all of
+    its tokens.  `cache`: CacheInt8 or a bfloat16 pair (k, v) of pages [pages, kv heads, page_size, head_dim]; all positions are visible (no window).
+    `token_pos` must be those that the plan was made for, `max_len` at least the longest.  bfloat16 queries, head sizes 64 and 128, pages of a multiple of 64
+    positions, at most 16 query heads per kv head; others are refused."""
+    device, pages, nkv, page_size, d, pointers = _page_entry(cache)
+    T, stride = _query_rows(q, device, n_heads, nkv, d)
+    _step_arrays(device, T, block_table, token_pos=token_pos, token_seq=token_seq)
+    _check_max_len(max_len)
+    if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, page_size, True):
+        raise KernelError(f"attention_decode_shared takes bfloat16, head sizes 64 and 128, pages of a multiple of 64 positions and up to 16 query heads per kv head, "
+                          f"found {q.dtype}, {d}, {page_size} and {n_heads} over {nkv}")
+    if plan.T != T or plan.device != device or plan.group_heads != n_heads // nkv:
+        raise KernelError(f"attention_decode_shared: the plan is for {plan.T} tokens with {plan.group_heads} query heads per kv head on {plan.device}")
+    if int(max_len) < plan.longest:
+        raise KernelError(f"attention_decode_shared: max_len {max_len} is below the plan's longest sequence {plan.longest}")
+    with _on(device):
+        out = torch.empty((T, n_heads * d), dtype=torch.bfloat16, device=device)
+        common = plan.tiles > 0
+        own = _pages_splits(T * nkv, max(1, plan.longest_rest)) if own_splits is None else int(own_splits)
+        pre = (_pages_splits(plan.tiles * nkv, plan.longest_prefix, plan.wide) if pre_splits is None else int(pre_splits)) if common else 0
+        acc, ml = _shares(T, n_heads, own + pre, d, device)
+        start, tiles, members = plan.pointers if common else (None, None, None)
+        err = _error_word(device)
+        if common and plan.wide:
+            _check(load().illm_attention_tiles_prefix(_ptr(q), stride, *pointers, pages, _ptr(block_table), block_table.shape[1], _ptr(token_seq), tiles, members,
+                                                      plan.tiles, _ptr(acc), _ptr(ml), n_heads, nkv, d, page_size, float(scale), own + pre, own, pre, err,
+                                                      _stream()), "attention_decode_shared")
+        _check(load().illm_attention_pages(_ptr(q), stride, *pointers, pages, _ptr(block_table), block_table.shape[1], _ptr(token_pos), _ptr(token_seq), start, tiles,
+                                           members, 0 if plan.wide else plan.tiles, _ptr(acc), _ptr(ml), _ptr(out), T, n_heads, nkv, d, page_size, 0, float(scale),
+                                           own, pre, err, _stream()), "attention_decode_shared")
     return out
 
 

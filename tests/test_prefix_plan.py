@@ -1,0 +1,79 @@
+"""The plan of a step's common prefixes, on the host: which tokens walk which positions together."""
+import ctypes
+
+import pytest
+
+from inferllm_b200 import binding as _b
+from inferllm_b200.binding import KernelError
+
+
+def plan(groups, lens, G):
+    sizes, total = (ctypes.c_int * 6)(), ctypes.c_int()
+    args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), len(lens), G,
+            sizes, ctypes.byref(total))
+    _b.check(_b.lib().illm_prefix_plan(*args, None))
+    out = (ctypes.c_int * max(1, total.value))()
+    _b.check(_b.lib().illm_prefix_plan(*args, out))
+    flat = list(out)[:total.value]
+    tiles = [flat[4 * i:4 * i + 4] for i in range(sizes[0])]
+    return dict(tiles=tiles, wide=bool(sizes[1]), longest_prefix=sizes[2], longest_rest=sizes[3], start=flat[sizes[4]:sizes[4] + len(lens)], members=flat[sizes[5]:])
+
+
+def covered(p):
+    """token -> positions of the prefix that a tile walks for it."""
+    got = {}
+    for first, n, length, zero in p["tiles"]:
+        assert zero == 0
+        for t in p["members"][first:first + n]:
+            assert t not in got
+            got[t] = length
+    return got
+
+
+@pytest.mark.parametrize("G", [1, 3, 4, 7, 16])
+@pytest.mark.parametrize("counts", [(1,), (2,), (5, 9), (64,), (300, 17, 1)])
+def test_every_member_is_in_one_tile_that_fits(G, counts):
+    tokens = sum(counts) + 3
+    order = [(i * 7919) % tokens for i in range(tokens)] if tokens % 7919 else list(range(tokens))
+    assert sorted(order) == list(range(tokens))
+    groups, at = [], 0
+    for i, c in enumerate(counts):
+        groups.append((64 * (i + 1), order[at:at + c]))
+        at += c
+    lens = [64 * len(counts) + 1 + t for t in range(tokens)]
+    p = plan(groups, lens, G)
+    want = {t: length for length, m in groups for t in m}
+    assert covered(p) == want
+    assert p["start"] == [want.get(t, 0) for t in range(tokens)]
+    most = 256 if p["wide"] else 16
+    assert all(1 <= n and n * G <= most for _, n, _, _ in p["tiles"])
+    assert p["longest_prefix"] == 64 * len(counts)
+    assert p["longest_rest"] == max(n - want.get(t, 0) for t, n in enumerate(lens))
+
+
+def test_groups_of_many_rows_take_wide_tiles():
+    assert not plan([(64, [0, 1])], [65, 65], 16)["wide"]
+    assert plan([(64, list(range(64)))], [65] * 64, 4)["wide"]
+
+
+def test_no_groups_is_a_plan():
+    p = plan([], [5, 9], 4)
+    assert p["tiles"] == [] and p["start"] == [0, 0] and p["longest_rest"] == 9
+
+
+@pytest.mark.parametrize("groups, lens, G, words", [
+    ([(64, [0, 0])], [65, 65], 1, "in two groups"),
+    ([(64, [0]), (64, [0])], [65, 65], 1, "in two groups"),
+    ([(64, [2])], [65, 65], 1, "outside the step"),
+    ([(64, [-1])], [65, 65], 1, "outside the step"),
+    ([(64, [])], [65, 65], 1, "at least one token"),
+    ([(0, [0])], [65, 65], 1, "at least one position"),
+    ([(64, [0, 1])], [65, 63], 1, "fewer than the common prefix"),
+    ([], [0], 1, "sees no position"),
+    ([], [], 1, "1 to 65535 tokens"),
+    ([(64, [0])], [65], 17, "1 to 16 query heads"),
+    ([(64, [0])], [65], 0, "1 to 16 query heads"),
+])
+def test_refusals(groups, lens, G, words):
+    with pytest.raises(KernelError, match=words):
+        plan(groups, lens, G)
