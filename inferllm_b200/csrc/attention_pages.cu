@@ -30,6 +30,7 @@
 #define PG_THREADS ((PG_CONSUMERS + 1) * 32)
 #define PG_MAX_SPLITS 32
 #define PG_ERR_PAGE 8                   // a visible position without a page
+#define PG_AHEAD 8.0f                   // how far (in powers of two) a score may run ahead of what its weights are relative to
 
 namespace {
 
@@ -61,6 +62,12 @@ __device__ __forceinline__ unsigned pg_widen(unsigned w, unsigned selector) {
     const unsigned bias = 0x64806480u;       // 1152, twice
     __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const unsigned*>(&v);
+}
+// an 8 x 8 matrix of 16-bit elements, transposed
+__device__ __forceinline__ unsigned pg_transpose(unsigned x) {
+    unsigned y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float pg_log2(float x) {
     float y;
@@ -97,7 +104,7 @@ template <int D, bool Q8> struct PgRing {
 
 // grid: (splits, kv heads, prefix tiles and tokens).  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
 // a token's own first.  out: written here where there is one slot.
-template <int D, bool Q8>
+template <int D, bool Q8, int NT>
 __global__ void __launch_bounds__(PG_THREADS)
 attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
                        const __grid_constant__ CUtensorMap map_v16, const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ q,
@@ -198,15 +205,16 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         return;
     }
 
-    // ---- consumers: warp w owns keys 16w .. 16w+15 of every tile
+    // ---- consumers: warp w owns keys 16w .. 16w+15 of every tile.  Keys (and channels of the values) are the 16 rows of a product, queries its
+    // 8 columns, NT times.
     const int g = lane >> 2, t4 = lane & 3, mtx = lane >> 3;
-    // The queries as fragments: row g and g + 8.  With eight bits a thread's four elements of 16 are neighbours (4 t4 ..), as the
-    // bytes of the keys come; any order of the summed index is as good as another.
-    unsigned qf[KS][4];
-    float row_scale[2] = {scale_log2e, scale_log2e};
+    // The queries as fragments of column g.  With eight bits a thread's four elements of 16 are neighbours (4 t4 ..), as the bytes of the keys come;
+    // any order of the summed index is as good as another.
+    unsigned qf[NT][KS][2];
+    float row_scale[NT][2];             // of the thread's columns 2 t4 and 2 t4 + 1 of the scores
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int r = g + e * 8;
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = nt * 8 + g;
         const bool ok = r < rows;
         const size_t head = ok ? row_head(r) : 0;
         const bf16* src = q + (head / nh) * (size_t)q_stride + (head % nh) * D;
@@ -222,6 +230,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 raw[k].y = *reinterpret_cast<const unsigned*>(src + k * 16 + 8 + t4 * 2);
             }
         }
+        float down = 1.f;
         if (Q8) {
             unsigned top = 0;           // the largest magnitude's bits
 #pragma unroll
@@ -231,27 +240,34 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // a power of two that brings the largest to [2^10, 2^11): 128 products with 127 stay below 2^25
             const int ex = max((int)(top >> 7) - 127, -116);
-            const float up = __int_as_float((10 - ex + 127) << 23), down = __int_as_float((ex - 10 + 127) << 23);
-            row_scale[e] = scale_log2e * down;
+            const float up = __int_as_float((10 - ex + 127) << 23);
+            down = __int_as_float((ex - 10 + 127) << 23);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                qf[k][e] = pg_half2(__uint_as_float(raw[k].x << 16) * up, __uint_as_float(raw[k].x & 0xffff0000u) * up);
-                qf[k][e + 2] = pg_half2(__uint_as_float(raw[k].y << 16) * up, __uint_as_float(raw[k].y & 0xffff0000u) * up);
+                qf[nt][k][0] = pg_half2(__uint_as_float(raw[k].x << 16) * up, __uint_as_float(raw[k].x & 0xffff0000u) * up);
+                qf[nt][k][1] = pg_half2(__uint_as_float(raw[k].y << 16) * up, __uint_as_float(raw[k].y & 0xffff0000u) * up);
             }
         } else {
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                qf[k][e] = raw[k].x;
-                qf[k][e + 2] = raw[k].y;
+                qf[nt][k][0] = raw[k].x;
+                qf[nt][k][1] = raw[k].y;
             }
         }
+        row_scale[nt][0] = scale_log2e * __shfl_sync(0xffffffffu, down, t4 * 8);
+        row_scale[nt][1] = scale_log2e * __shfl_sync(0xffffffffu, down, t4 * 8 + 4);
     }
 
-    // m, l: maximum and sum of the softmax; mv: the maximum that the accumulators are relative to (m itself for bfloat16 rows)
-    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float o[2 * KS][4];
+    // Per column: m, what the sums l are relative to, and mv, what the accumulators are (m itself for bfloat16 rows); both follow the largest score
+    // only once it is 2^8 ahead, which a vote finds, so that the maxima cost no shuffles otherwise.  A weight is at most 2^8 that way.
+    float m[NT][2], mv[NT][2], l[NT][2], o[NT][KS][4];
 #pragma unroll
-    for (int i = 0; i < 2 * KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt][0] = m[nt][1] = mv[nt][0] = mv[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
 
     for (int i = 0; i < n_my; i++) {
         const int s = i % STAGES;
@@ -259,118 +275,115 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const int key0 = (tile_lo + split + i * n_splits) * PG_BN + warp * 16;
         if (key0 <= p && key0 + 15 >= lo) {
             const unsigned kbase = base + (unsigned)s * 2 * TILE, vbase = kbase + TILE;
-            float sa[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sb[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            float sc[NT][4], sv[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[nt][e] = sv[nt][e] = 0.f;
+            const int krow = warp * 16 + (mtx & 1) * 8 + (lane & 7);
             if (Q8) {
-                const int krow = warp * 16 + (mtx & 1) * 8 + (lane & 7);
 #pragma unroll
                 for (int k = 0; k < KS; k += 2) {
                     unsigned b[4];
                     pg_ldm(b, kbase + pg_off<D, Q8>(krow, k + (mtx >> 1)));
-                    pg_mma<true>(sa[0], qf[k], pg_widen(b[0], 0x4140), pg_widen(b[0], 0x4342));
-                    pg_mma<true>(sa[1], qf[k], pg_widen(b[1], 0x4140), pg_widen(b[1], 0x4342));
-                    pg_mma<true>(sb[0], qf[k + 1], pg_widen(b[2], 0x4140), pg_widen(b[2], 0x4342));
-                    pg_mma<true>(sb[1], qf[k + 1], pg_widen(b[3], 0x4140), pg_widen(b[3], 0x4342));
-                }
-            } else {
-                const int krow = warp * 16 + (mtx >> 1) * 8 + (lane & 7);
 #pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    unsigned b[4];
-                    pg_ldm(b, kbase + pg_off<D, Q8>(krow, k * 2 + (mtx & 1)));
-                    pg_mma<false>(k & 1 ? sb[0] : sa[0], qf[k], b[0], b[1]);
-                    pg_mma<false>(k & 1 ? sb[1] : sa[1], qf[k], b[2], b[3]);
-                }
-            }
-            float lv[2][2];                 // log2 of the values' scales
-            float mx[2] = {-INFINITY, -INFINITY}, mxv[2] = {-INFINITY, -INFINITY};
+                    for (int u = 0; u < 2; u++) {
+                        const unsigned a[4] = {pg_widen(b[2 * u], 0x4140), pg_widen(b[2 * u + 1], 0x4140), pg_widen(b[2 * u], 0x4342), pg_widen(b[2 * u + 1], 0x4342)};
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                float kf[2] = {1.f, 1.f};
-                if (Q8) {
-                    const unsigned at = scales + s * R::SCALES + (warp * 16 + nt * 8 + t4 * 2) * 4;
-                    float v0, v1;
-                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(kf[0]), "=f"(kf[1]) : "r"(at));
-                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v0), "=f"(v1) : "r"(at + PG_BN * 4));
-                    lv[nt][0] = pg_log2(v0);
-                    lv[nt][1] = pg_log2(v1);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int key = key0 + nt * 8 + t4 * 2 + (e & 1);
-                    const bool hidden = key > p || key < lo;
-                    float v = (sa[nt][e] + sb[nt][e]) * row_scale[e >> 1];
-                    if (Q8) v *= kf[e & 1];
-                    if (hidden) v = -INFINITY;
-                    sa[nt][e] = v;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], v);
-                    if (Q8) {
-                        const float w = hidden ? -INFINITY : v + lv[nt][e & 1];
-                        sb[nt][e] = w;
-                        mxv[e >> 1] = fmaxf(mxv[e >> 1], w);
+                        for (int nt = 0; nt < NT; nt++) pg_mma<true>(u ? sv[nt] : sc[nt], a, qf[nt][k + u][0], qf[nt][k + u][1]);
                     }
                 }
-            }
-            float ref[2], refv[2], alpha[2];
+            } else {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                const float top = fmaxf(m[e], mx[e]);
-                ref[e] = top == -INFINITY ? 0.f : top;
-                const float keep = fast_exp2(m[e] - ref[e]);
-                l[e] *= keep;
-                m[e] = top;
-                if (Q8) {
-                    mxv[e] = fmaxf(mxv[e], __shfl_xor_sync(0xffffffffu, mxv[e], 1));
-                    mxv[e] = fmaxf(mxv[e], __shfl_xor_sync(0xffffffffu, mxv[e], 2));
-                    const float topv = fmaxf(mv[e], mxv[e]);
-                    refv[e] = topv == -INFINITY ? 0.f : topv;
-                    alpha[e] = fast_exp2(mv[e] - refv[e]);
-                    mv[e] = topv;
-                } else {
-                    refv[e] = ref[e];
-                    alpha[e] = keep;
-                    mv[e] = top;
+                for (int k = 0; k < KS; k++) {
+                    unsigned a[4];
+                    pg_ldm(a, kbase + pg_off<D, Q8>(krow, k * 2 + (mtx >> 1)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) pg_mma<false>(k & 1 ? sv[nt] : sc[nt], a, qf[nt][k][0], qf[nt][k][1]);
                 }
             }
-            unsigned pf[4];
+            // scores in units of log2: element e of a thread is key g + 8 (e / 2), column 2 t4 + e % 2
+            float lv[2] = {0.f, 0.f}, kf[2] = {1.f, 1.f};       // log2 of the values' scales, the keys' scales
+            if (Q8) {
+                const unsigned at = scales + s * R::SCALES + (warp * 16 + g) * 4;
+                float v[2];
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                const float p0 = fast_exp2(sa[nt][0] - ref[0]), p1 = fast_exp2(sa[nt][1] - ref[0]);
-                const float p2 = fast_exp2(sa[nt][2] - ref[1]), p3 = fast_exp2(sa[nt][3] - ref[1]);
-                l[0] += p0 + p1;
-                l[1] += p2 + p3;
-                if (Q8) {
-                    pf[nt * 2] = pg_half2(fast_exp2(sb[nt][0] - refv[0]), fast_exp2(sb[nt][1] - refv[0]));
-                    pf[nt * 2 + 1] = pg_half2(fast_exp2(sb[nt][2] - refv[1]), fast_exp2(sb[nt][3] - refv[1]));
-                } else {
-                    pf[nt * 2] = pg_bf162(p0, p1);
-                    pf[nt * 2 + 1] = pg_bf162(p2, p3);
+                for (int e = 0; e < 2; e++) {
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(kf[e]) : "r"(at + e * 32));
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[e]) : "r"(at + e * 32 + PG_BN * 4));
+                    lv[e] = pg_log2(v[e]);
                 }
             }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+            const bool edge = key0 + 15 > p || key0 < lo;
+            bool over = false;
 #pragma unroll
-                for (int j = 0; j < 2 * KS; j++) {
-                    o[j][0] *= alpha[0];
-                    o[j][1] *= alpha[0];
-                    o[j][2] *= alpha[1];
-                    o[j][3] *= alpha[1];
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float v = (sc[nt][e] + sv[nt][e]) * row_scale[nt][e & 1];
+                    if (Q8) v *= kf[e >> 1];
+                    float w = v + lv[e >> 1];
+                    if (edge) {
+                        const int key = key0 + g + (e >> 1) * 8;
+                        if (key > p || key < lo) v = w = -INFINITY;
+                    }
+                    sc[nt][e] = v;
+                    sv[nt][e] = w;
+                    over |= v > m[nt][e & 1] + PG_AHEAD;
+                    if (Q8) over |= w > mv[nt][e & 1] + PG_AHEAD;
                 }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(sc[nt][e], sc[nt][e + 2]), topv = fmaxf(sv[nt][e], sv[nt][e + 2]);
+#pragma unroll
+                        for (int k = 4; k < 32; k *= 2) {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                            if (Q8) topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, k));
+                        }
+                        top = fmaxf(top, m[nt][e]);
+                        topv = Q8 ? fmaxf(topv, mv[nt][e]) : top;
+                        l[nt][e] *= top == -INFINITY ? 1.f : fast_exp2(m[nt][e] - top);
+                        const float keep = topv == -INFINITY ? 1.f : fast_exp2(mv[nt][e] - topv);
+                        m[nt][e] = top;
+                        mv[nt][e] = topv;
+#pragma unroll
+                        for (int c = 0; c < KS; c++) {
+                            o[nt][c][e] *= keep;
+                            o[nt][c][e + 2] *= keep;
+                        }
+                    }
             }
-            const int vrow = warp * 16 + (mtx & 1) * 8 + (lane & 7);
+            unsigned pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float pw[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float ref = m[nt][e & 1], refv = mv[nt][e & 1];
+                    const float pe = fast_exp2(sc[nt][e] - (ref == -INFINITY ? 0.f : ref));
+                    l[nt][e & 1] += pe;
+                    pw[e] = Q8 ? fast_exp2(sv[nt][e] - (refv == -INFINITY ? 0.f : refv)) : pe;
+                }
+                pf[nt][0] = pg_transpose(Q8 ? pg_half2(pw[0], pw[1]) : pg_bf162(pw[0], pw[1]));
+                pf[nt][1] = pg_transpose(Q8 ? pg_half2(pw[2], pw[3]) : pg_bf162(pw[2], pw[3]));
+            }
             if (Q8) {
 #pragma unroll
                 for (int c = 0; c < KS; c += 2) {
                     unsigned b[4];
-                    pg_ldm_t(b, vbase + pg_off<D, Q8>(vrow, c + (mtx >> 1)));
+                    pg_ldm_t(b, vbase + pg_off<D, Q8>(krow, c + (mtx >> 1)));
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {           // channels 16 (c + u) + 2 n and + 2 n + 1 of column n
-                        pg_mma<true>(o[(c + u) * 2], pf, pg_widen(b[u * 2], 0x4240), pg_widen(b[u * 2 + 1], 0x4240));
-                        pg_mma<true>(o[(c + u) * 2 + 1], pf, pg_widen(b[u * 2], 0x4341), pg_widen(b[u * 2 + 1], 0x4341));
+                    for (int u = 0; u < 2; u++) {           // rows n and n + 8: channels 16 (c + u) + 2 n and + 2 n + 1
+                        const unsigned a[4] = {pg_widen(b[2 * u], 0x4240), pg_widen(b[2 * u], 0x4341), pg_widen(b[2 * u + 1], 0x4240), pg_widen(b[2 * u + 1], 0x4341)};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) pg_mma<true>(o[nt][c + u], a, pf[nt][0], pf[nt][1]);
                     }
                 }
             } else {
-                if (key0 + 15 > p || key0 < lo) {
+                if (edge) {
                     // rows of hidden keys may hold anything, and 0 x NaN would not be 0
                     unsigned char* v = gbase + (size_t)s * 2 * TILE + TILE;
                     for (int j = lane; j < 16 * 2 * KS; j += 32) {
@@ -380,22 +393,18 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the stage is filled again
                     __syncwarp();
                 }
+                const int vrow = warp * 16 + (mtx >> 1) * 8 + (lane & 7);
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
-                    unsigned b[4];
-                    pg_ldm_t(b, vbase + pg_off<D, Q8>(vrow, c * 2 + (mtx >> 1)));
-                    pg_mma<false>(o[c * 2], pf, b[0], b[1]);
-                    pg_mma<false>(o[c * 2 + 1], pf, b[2], b[3]);
+                    unsigned a[4];
+                    pg_ldm_t(a, vbase + pg_off<D, Q8>(vrow, c * 2 + (mtx & 1)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) pg_mma<false>(o[nt][c], a, pf[nt][0], pf[nt][1]);
                 }
             }
         }
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * s) : "memory");
-    }
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
 
     // ---- join the warps (ascending) through the ring's memory: every load has landed and been read
@@ -404,21 +413,25 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     constexpr int ROW = D + 4;
     static_assert(PG_CONSUMERS * 16 * ROW * 4 <= STAGES * 2 * TILE, "the joined rows must fit the ring");
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int r = g + e * 8;
-        if (r >= rows) continue;
-        float* dst = joined + ((size_t)warp * 16 + r) * ROW;
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            if (Q8) {
-                *reinterpret_cast<float4*>(dst + k * 16 + t4 * 4) = make_float4(o[k * 2][e * 2], o[k * 2 + 1][e * 2], o[k * 2][e * 2 + 1], o[k * 2 + 1][e * 2 + 1]);
-            } else {
-                *reinterpret_cast<float2*>(dst + k * 16 + t4 * 2) = make_float2(o[k * 2][e * 2], o[k * 2][e * 2 + 1]);
-                *reinterpret_cast<float2*>(dst + k * 16 + 8 + t4 * 2) = make_float2(o[k * 2 + 1][e * 2], o[k * 2 + 1][e * 2 + 1]);
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+            for (int k = 4; k < 32; k *= 2) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], k);
+            const int r = nt * 8 + t4 * 2 + e;
+            if (r >= rows) continue;
+            float* dst = joined + ((size_t)warp * 16 + r) * ROW;
+#pragma unroll
+            for (int c = 0; c < KS; c++) {
+                if (Q8) {
+                    *reinterpret_cast<float2*>(dst + c * 16 + g * 2) = make_float2(o[nt][c][e], o[nt][c][e + 2]);
+                } else {
+                    dst[c * 16 + g] = o[nt][c][e];
+                    dst[c * 16 + 8 + g] = o[nt][c][e + 2];
+                }
             }
+            if (g == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m[nt][e], l[nt][e], mv[nt][e], 0.f);
         }
-        if (t4 == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m[e], l[e], mv[e], 0.f);
-    }
     asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
     for (int idx = tid; idx < rows * D; idx += PG_CONSUMERS * 32) {
         const int r = idx / D, c = idx - r * D;
@@ -519,7 +532,8 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
     if ((rc = pg_make_map(&mk, kc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mv, vc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mk16, kc, rows, D, 16, Q8)) ||
         (rc = pg_make_map(&mv16, vc, rows, D, 16, Q8)))
         return rc;
-    auto kern = attention_pages_kernel<D, Q8>;
+    // eight rows in a block's products where no block has more
+    auto kern = plan.n_tiles == 0 && nh / nkv <= 8 ? attention_pages_kernel<D, Q8, 1> : attention_pages_kernel<D, Q8, 2>;
     const int smem = PgRing<D, Q8>::BYTES;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;

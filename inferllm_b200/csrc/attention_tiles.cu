@@ -6,14 +6,14 @@
 //
 // A block has two tiles of 128 rows over the same keys and is alone on its SM.  Eight softmax warps (a thread is a row of a tile and a lane of
 // tensor memory), a thread that issues the products, one that brings pages by TMA and, for eight bits, four warps that widen them:
-// bytes from a ring of four raw stages become (u - 128) s in bfloat16, in the swizzled layout that the products read.  Widening
-// costs about ten instructions for four elements, as much as the softmax of half a tile, which is why the tiles share it; two rows five apart
-// (r and r XOR 5) go to a quarter of a warp, so that neither its loads nor its stores meet in a bank.
+// bytes from a ring of four raw stages become u - 128 in bfloat16, exactly, in the swizzled layout that the products read.  Widening
+// costs about two instructions an element, which is why the tiles share it; two rows five apart (r and r XOR 5) go to a quarter of a warp, so that neither
+// its loads nor its stores meet in a bank.  The rows' scales are factors of the scores and, the values', of the softmax weights.
 // Tensor memory of a tile, 256 columns: two score buffers of 64 and the output.  As in attention_prefill_tc.cu the scores
 // of the next 64 keys are made while the softmax works on the last ones, the weights stay in tensor memory in place of their scores,
 // and the output is rescaled only when a row's maximum has grown by more than 2^8.
-// Rounded to bfloat16: the widened rows (2^-9 of an element, next to the eight bits' own 1/254 of the row's largest), the softmax weights
-// and the results.  Scores, sums and the running output are float32.
+// Rounded to bfloat16 are the softmax weights (times the value's scale) and the results; scores, sums and the running output are float32.  (Rows
+// widened with their scales in them, and so rounded, put the results 0.006 of their norm off at scores of spread 2; like this it is 0.002.)
 // A key whose row reads back as NaN has its score NaN instead, so that it reaches the queries that see it and no others.
 #include <cuda.h>
 #include <math.h>
@@ -44,7 +44,7 @@ struct TlWork {
 template <int D, bool Q8> struct TlSizes {
     static constexpr int STAGES = Q8 ? 2 : 4, TILE = TL_BN * D * 2, Q_TILE = TL_BM * D * 2;
     static constexpr int RAW_TILE = TL_BN * D, RAW = Q8 ? TL_RAW : 0, SCALES = 2 * TL_BN * 4;
-    static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + RAW * (2 * RAW_TILE + SCALES) + 512;
+    static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + RAW * (2 * RAW_TILE + 2 * SCALES) + 512;
     static constexpr int THREADS = (Q8 ? 14 : 10) * 32;
 };
 
@@ -57,18 +57,23 @@ __device__ __forceinline__ void tl_arrive(unsigned bar) { asm volatile("mbarrier
 __device__ __forceinline__ void tl_store16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// sixteen bytes as (u - 128) s in bfloat16: a byte below 0x4b0000 is 2^23 + u in float32
-__device__ __forceinline__ void tl_widen(const unsigned (&w)[4], float s, unsigned (&out)[8]) {
-    const unsigned long long bias = f2_pack(-8388736.f, -8388736.f), ss = f2_pack(s, s);
+// sixteen bytes as u - 128 in bfloat16, exactly: a byte below 0x4b0000 is 2^23 + u in float32, and the difference has at most seven bits, which
+// are the upper half of its word
+__device__ __forceinline__ void tl_widen(const unsigned (&w)[4], unsigned (&out)[8]) {
+    const unsigned long long bias = f2_pack(-8388736.f, -8388736.f);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const unsigned lo = __byte_perm(w[i], 0x4b000000u, h ? 0x7652 : 0x7650), hi = __byte_perm(w[i], 0x4b000000u, h ? 0x7653 : 0x7651);
             float a, b;
-            f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(lo), __uint_as_float(hi)), bias), ss), a, b);
-            out[i * 2 + h] = pack_bf16(a, b);
+            f2_unpack(f2_add(f2_pack(__uint_as_float(lo), __uint_as_float(hi)), bias), a, b);
+            out[i * 2 + h] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
         }
+}
+// four floats of shared memory, the same for all lanes
+__device__ __forceinline__ void tl_load4(unsigned at, float* f) {
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(at));
 }
 
 }  // namespace
@@ -86,10 +91,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const unsigned base = tc_smem_u32(smem_raw);
     const unsigned q_s = base, kv_s = q_s + 2 * Z::Q_TILE, raw_s = kv_s + STAGES * 2 * TILE, sc_s = raw_s + Z::RAW * 2 * Z::RAW_TILE;
-    const unsigned bars0 = sc_s + Z::RAW * Z::SCALES;
+    const unsigned f_s = sc_s + Z::RAW * Z::SCALES;         // the factors of a block's scores and weights
+    const unsigned bars0 = f_s + Z::RAW * Z::SCALES;
     const unsigned q_full = bars0, k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * STAGES, v_full0 = k_empty0 + 8 * STAGES, v_empty0 = v_full0 + 8 * STAGES;
-    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32;
-    unsigned* holder = reinterpret_cast<unsigned*>(smem_raw + (pv_done0 + 16 - base));
+    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32, f_full0 = pv_done0 + 16;
+    unsigned* holder = reinterpret_cast<unsigned*>(smem_raw + (f_full0 + 8 * TL_RAW - base));
     if ((base & 1023u) != 0) {          // cannot happen without static shared memory; never run misaligned
         if (threadIdx.x == 0) atomicExch(err, TC_ERR_MISALIGNED_SMEM);
         return;
@@ -106,6 +112,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < TL_RAW; i++) {
             mbar_init(raw_full0 + 8 * i, 1);
             mbar_init(raw_empty0 + 8 * i, 128);
+            mbar_init(f_full0 + 8 * i, TL_BN);
         }
         for (int i = 0; i < 4; i++) {
             mbar_init(s_full0 + 8 * i, 1);
@@ -228,22 +235,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 }
         }
     } else if (Q8 && warp >= TL_WIDEN_WARP) {
-        // ---- bytes to bfloat16.  Keys outside the block's range get zero rows: what lies there may be another sequence's.
+        // ---- bytes to bfloat16, and the factors of the scores (with the softmax's scale) and of the weights.  Keys outside the block's range, where
+        // another sequence's may lie, have factors of zero.  The ring of factors has four places: those of block i + 4 come once the
+        // products of block i + 1 are done (v_empty), so behind every softmax of block i.
         const int ct = threadIdx.x - TL_WIDEN_WARP * 32;
-        auto widen = [&](const unsigned char* raw, const float* own, const float* other, unsigned dst, int key0, bool keys) {
+        auto widen = [&](const unsigned char* raw, unsigned dst) {
 #pragma unroll
             for (int it = 0; it < TL_BN * D / 16 / 128; it++) {
                 const int id = ct + it * 128, rest = id >> 3;
                 const int r = (D == 128 ? rest >> 1 : rest) * 2 ^ ((id & 4) ? 5 : 0), c = (id & 3) + (D == 128 ? (rest & 1) * 4 : 0);
                 const uint4 v = *reinterpret_cast<const uint4*>(raw + (D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + c * 16));
-                const int key = key0 + r;
-                float s = own[r];
-                const float s2 = other[r];
-                const bool in = key >= first_key && key <= last_key, number = fabsf(s) < INFINITY && fabsf(s2) < INFINITY;
-                if (!in || !number) s = in && keys ? __uint_as_float(0x7fffffffu) : 0.f;
                 const unsigned w[4] = {v.x, v.y, v.z, v.w};
                 unsigned o[8];
-                tl_widen(w, s, o);
+                tl_widen(w, o);
                 const unsigned at = dst + (c >> 2) * ATOM + r * 128, p = (c & 3) * 2;
                 tl_store16(at + ((p ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
                 tl_store16(at + (((p + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
@@ -256,12 +260,19 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const float* vs = ks + TL_BN;
             const unsigned kd = kv_s + st * 2 * TILE, vd = kd + TILE;
             if (!mbar_wait(raw_full0 + 8 * rs, (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+            if (ct < TL_BN) {
+                const bool in = key0 + ct >= first_key && key0 + ct <= last_key, number = fabsf(ks[ct]) < INFINITY && fabsf(vs[ct]) < INFINITY;
+                float* f = reinterpret_cast<float*>(smem_raw + (f_s - base) + rs * Z::SCALES);
+                f[ct] = !in ? 0.f : number ? ks[ct] * scale_log2e : __uint_as_float(0x7fffffffu);
+                f[TL_BN + ct] = in && number ? vs[ct] : 0.f;
+                tl_arrive(f_full0 + 8 * rs);
+            }
             if (i >= STAGES && !mbar_wait(k_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
-            widen(raw, ks, vs, kd, key0, true);
+            widen(raw, kd);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tl_arrive(k_full0 + 8 * st);
             if (i >= STAGES && !mbar_wait(v_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
-            widen(raw + Z::RAW_TILE, vs, ks, vd, key0, false);
+            widen(raw + Z::RAW_TILE, vd);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tl_arrive(v_full0 + 8 * st);
             tl_arrive(raw_empty0 + 8 * rs);
@@ -299,6 +310,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // what the tile's rows see: everything in blocks between the last row's first key and the first row's last one
         const int tile_first = PREFIX ? last_key : past + (row0 + w * TL_BM) / G, tile_last = PREFIX ? last_key : past + (row0 + min(n_rows, (w + 1) * TL_BM) - 1) / G;
         const int lo_pos = PREFIX ? 0 : nbw > 0 ? first_visible(pos, work.span) : 0, lo_last = PREFIX || nbw == 0 ? 0 : first_visible(tile_last, work.span);
+        const float unit = Q8 ? 1.f : scale_log2e;
         float m_ref = -INFINITY, l_run = 0.f;
         bool alive = true;
         for (int i = 0; i < nbw; i++) {
@@ -311,6 +323,20 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             tmem_ld32_issue(s_addr, sr);
             tmem_ld32_issue(s_addr + 32, sr + 32);
             tmem_wait_ld<TL_BN>(sr);
+            const unsigned f_at = f_s + (i % TL_RAW) * Z::SCALES;
+            if (Q8) {
+                alive = __all_sync(0xffffffffu, mbar_wait(f_full0 + 8 * (i % TL_RAW), (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+                if (!alive) break;
+#pragma unroll
+                for (int c = 0; c < TL_BN; c += 4) {
+                    float f[4], x[4];
+                    tl_load4(f_at + c * 4, f);
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), f2_pack(f[0], f[1])), x[0], x[1]);
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), f2_pack(f[2], f[3])), x[2], x[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sr[c + e] = __float_as_uint(x[e]);
+                }
+            }
             if (key0 + TL_BN - 1 > tile_first || key0 < lo_last) {
 #pragma unroll
                 for (int c = 0; c < TL_BN; c++)
@@ -324,7 +350,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
                 mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
             }
-            const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale_log2e);
+            const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * unit);
             const bool grown = m_new > m_ref + TL_RESCALE_STEP;      // true for m_ref = -inf, m_new finite
             bool pv_seen = false;
             if (__any_sync(0xffffffffu, grown)) {
@@ -350,7 +376,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
             unsigned pr[TL_BN / 2];
-            const unsigned long long scale2 = f2_pack(scale_log2e, scale_log2e), neg_m2 = f2_pack(-m_use, -m_use);
+            const unsigned long long scale2 = f2_pack(unit, unit), neg_m2 = f2_pack(-m_use, -m_use);
             unsigned long long psa = f2_pack(0.f, 0.f), psb = psa;
 #pragma unroll
             for (int c = 0; c < TL_BN; c += 4) {
@@ -360,8 +386,17 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const float p0 = fast_exp2(x0), p1 = fast_exp2(x1), p2 = fast_exp2(x2), p3 = fast_exp2(x3);
                 psa = f2_add(psa, f2_pack(p0, p1));
                 psb = f2_add(psb, f2_pack(p2, p3));
-                pr[c >> 1] = pack_bf16(p0, p1);
-                pr[(c >> 1) + 1] = pack_bf16(p2, p3);
+                if (Q8) {
+                    float f[4], w0, w1, w2, w3;
+                    tl_load4(f_at + TL_BN * 4 + c * 4, f);
+                    f2_unpack(f2_mul(f2_pack(p0, p1), f2_pack(f[0], f[1])), w0, w1);
+                    f2_unpack(f2_mul(f2_pack(p2, p3), f2_pack(f[2], f[3])), w2, w3);
+                    pr[c >> 1] = pack_bf16(w0, w1);
+                    pr[(c >> 1) + 1] = pack_bf16(w2, w3);
+                } else {
+                    pr[c >> 1] = pack_bf16(p0, p1);
+                    pr[(c >> 1) + 1] = pack_bf16(p2, p3);
+                }
             }
             {
                 float a0, a1, b0, b1;
