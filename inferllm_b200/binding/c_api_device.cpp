@@ -414,7 +414,6 @@ ILLM_API int illm_policy_ring_splits(long long T, int n_kv_heads, long long max_
 ILLM_API int illm_policy_pages_splits(long long pairs, long long keys, int wide, int n_sms) {
     return wide ? ops::attention_prefix_splits(pairs, keys, n_sms) : ops::attention_pages_splits(pairs, keys, n_sms);
 }
-ILLM_API int illm_policy_tile_rows(int B, int max_q, int nh, int nkv, int n_sms) { return ops::attention_tile_rows(B, max_q, nh, nkv, n_sms); }
 ILLM_API int illm_policy_attention_diff_splits(long long T, int head_groups, long long max_seq_len, int n_sms) {
     return ops::attention_diff_splits(T, head_groups, max_seq_len, n_sms);
 }

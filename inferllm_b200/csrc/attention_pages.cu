@@ -29,6 +29,7 @@
 #define PG_CONSUMERS 4
 #define PG_THREADS ((PG_CONSUMERS + 1) * 32)
 #define PG_MAX_SPLITS 32
+#define PG_MAX_CLUSTER 8               // blocks whose shares are joined through shared memory
 #define PG_ERR_PAGE 8                   // a visible position without a page
 #define PG_AHEAD 8.0f                   // how far (in powers of two) a score may run ahead of what its weights are relative to
 
@@ -81,6 +82,17 @@ template <int D, bool Q8> __device__ __forceinline__ unsigned pg_off(int r, int 
     if (D == 128) return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4));
     return (unsigned)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
+// a float of the same place in another block of the cluster
+__device__ __forceinline__ float pg_remote(unsigned at, unsigned rank) {
+    unsigned a;
+    float f;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    return f;
+}
+__device__ __forceinline__ void pg_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void pg_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -99,11 +111,11 @@ struct PgPlan {
 // stages that leave two blocks to an SM
 template <int D, bool Q8> struct PgRing {
     static constexpr int TILE = PG_BN * D * (Q8 ? 1 : 2), SCALES = Q8 ? 2 * PG_BN * 4 : 0;
-    static constexpr int STAGES = (Q8 ? 768 : 384) / D, BYTES = STAGES * (2 * TILE + SCALES) + 1024;
+    static constexpr int STAGES = Q8 ? (D == 128 ? 4 : 6) : 256 / D, BYTES = STAGES * (2 * TILE + SCALES) + 1024;
 };
 
 // grid: (splits, kv heads, prefix tiles and tokens).  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
-// a token's own first.  out: written here where there is one slot.
+// a token's own first.  No part_acc: the blocks of a (token, kv head) are a cluster that joins them through shared memory and writes `out`.
 template <int D, bool Q8, int NT>
 __global__ void __launch_bounds__(PG_THREADS)
 attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
@@ -157,12 +169,8 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int tile_lo = lo / PG_BN, n_tiles = p < lo ? 0 : p / PG_BN - tile_lo + 1;
     const int n_my = n_tiles > split ? (n_tiles - split + n_splits - 1) / n_splits : 0;
     const int slot = prefix ? own_splits + split : split;
-    if (n_my == 0) {
-        if (slots == 1) {
-            for (int i = tid; i < rows * D; i += PG_THREADS) out[row_head(i / D) * D + i % D] = __float2bfloat16_rn(0.f);
-        } else if (tid < rows) {
-            *reinterpret_cast<float2*>(part_ml + (row_head(tid) * slots + slot) * 2) = make_float2(-INFINITY, 0.f);
-        }
+    if (part_acc && n_my == 0) {
+        if (tid < rows) *reinterpret_cast<float2*>(part_ml + (row_head(tid) * slots + slot) * 2) = make_float2(-INFINITY, 0.f);
         return;
     }
 
@@ -201,6 +209,11 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     }
                 }
             }
+        }
+        __syncwarp();
+        if (!part_acc && n_splits > 1) {        // the cluster's two meetings, at the end
+            pg_cluster_sync();
+            pg_cluster_sync();
         }
         return;
     }
@@ -411,7 +424,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
     float* joined = reinterpret_cast<float*>(gbase);            // [PG_CONSUMERS][16][D + 4]: accumulators, m, l, mv
     constexpr int ROW = D + 4;
-    static_assert(PG_CONSUMERS * 16 * ROW * 4 <= STAGES * 2 * TILE, "the joined rows must fit the ring");
+    static_assert((PG_CONSUMERS + 1) * 16 * ROW * 4 <= STAGES * 2 * TILE, "the joined rows and the share must fit the ring");
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -433,6 +446,9 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (g == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m[nt][e], l[nt][e], mv[nt][e], 0.f);
         }
     asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
+    // the block's share of every row: accumulators relative to m, m and l; a row without keys has l = 0
+    float* share = joined + (size_t)PG_CONSUMERS * 16 * ROW;        // [16][ROW]
+    const bool alone = !part_acc && n_splits == 1;
     for (int idx = tid; idx < rows * D; idx += PG_CONSUMERS * 32) {
         const int r = idx / D, c = idx - r * D;
         float4 w[PG_CONSUMERS];
@@ -450,14 +466,44 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             num += joined[((size_t)k * 16 + r) * ROW + c] * (w[k].z == -INFINITY ? 1.f : fast_exp2(w[k].z - ref));
             den += w[k].y * (w[k].x == -INFINITY ? 1.f : fast_exp2(w[k].x - ref));
         }
-        const size_t head = row_head(r);
-        if (slots == 1) {
-            out[head * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+        if (alone) {
+            out[row_head(r) * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+        } else if (part_acc) {
+            const size_t at = row_head(r) * slots + slot;
+            part_acc[at * D + c] = num;
+            if (c == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(M, den);
         } else {
-            part_acc[(head * slots + slot) * D + c] = num;
-            if (c == 0) *reinterpret_cast<float2*>(part_ml + (head * slots + slot) * 2) = make_float2(M, den);
+            share[r * ROW + c] = num;
+            if (c == 0) *reinterpret_cast<float2*>(share + r * ROW + D) = make_float2(M, den);
         }
     }
+    if (alone || part_acc) return;
+    // ---- join the cluster's shares (ascending): every block writes a part of the rows
+    pg_cluster_sync();
+    const unsigned share_at = tc_smem_u32(share);
+    for (int idx = split * (PG_CONSUMERS * 32) + tid; idx < rows * D; idx += n_splits * (PG_CONSUMERS * 32)) {
+        const int r = idx / D, c = idx - r * D;
+        const unsigned row_at = share_at + r * ROW * 4;
+        float ms[PG_MAX_CLUSTER], ls[PG_MAX_CLUSTER], v[PG_MAX_CLUSTER], M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < PG_MAX_CLUSTER; k++) {
+            ms[k] = k < n_splits ? pg_remote(row_at + D * 4, k) : -INFINITY;
+            ls[k] = k < n_splits ? pg_remote(row_at + D * 4 + 4, k) : 0.f;
+            v[k] = k < n_splits ? pg_remote(row_at + c * 4, k) : 0.f;
+            M = fmaxf(M, ms[k]);
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
+        float num = 0.f, den = 0.f;
+#pragma unroll
+        for (int k = 0; k < PG_MAX_CLUSTER; k++) {
+            if (k >= n_splits || ls[k] == 0.f) continue;
+            const float f = ms[k] == -INFINITY ? 1.f : fast_exp2(ms[k] - ref);
+            num += f * v[k];
+            den += f * ls[k];
+        }
+        out[row_head(r) * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+    }
+    pg_cluster_sync();              // the others may still read this block's shares
 }
 
 // out[t, h] = sum over the shares (ascending) of acc 2^(m - M) / sum of l 2^(m - M): a token's own and, where it has a prefix in common with
@@ -537,10 +583,12 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
     const int smem = PgRing<D, Q8>::BYTES;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    illm_launch(kern, dim3(own_splits > pre_splits ? own_splits : pre_splits, nkv, plan.n_tiles + T), dim3(PG_THREADS), smem, s, mk, mv, mk16, mv16, ksc, vsc, (const bf16*)q,
-                q_stride, block_table, max_pages, (int)n_pages, token_pos, token_seq, plan, part_acc, part_ml, (bf16*)out, own_splits, pre_splits, nh, nkv, page_size,
-                span, scale * 1.4426950408889634f, err);
-    if ((rc = illm_launch_status()) || own_splits + pre_splits == 1) return rc;
+    const bool shares = own_splits > PG_MAX_CLUSTER || plan.start;
+    if (!shares) part_acc = part_ml = nullptr;
+    rc = illm_launch_cluster(kern, dim3(own_splits > pre_splits ? own_splits : pre_splits, nkv, plan.n_tiles + T), dim3(PG_THREADS), shares ? 1 : own_splits, smem, s, mk, mv, mk16,
+                             mv16, ksc, vsc, (const bf16*)q, q_stride, block_table, max_pages, (int)n_pages, token_pos, token_seq, plan, part_acc, part_ml, (bf16*)out,
+                             own_splits, pre_splits, nh, nkv, page_size, span, scale * 1.4426950408889634f, err);
+    if (rc || !shares) return rc;
     illm_launch(attention_pages_join_kernel<D>, dim3(nh, T), dim3(D), 0, s, (const float*)part_acc, (const float*)part_ml, (bf16*)out, own_splits, pre_splits,
                 plan.start, nh);
     return illm_launch_status();
@@ -549,9 +597,9 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 // Single tokens: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages
 // [n_pages, nkv, page_size, d] of bytes with their scales ksc, vsc, or (ksc, vsc nullptr) of bfloat16; page_size a multiple of 64, d 64
 // or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most 16 rows (members times nh / nkv),
-// are walked here, with n_tiles 0 their shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  Scratch where own_splits +
-// pre_splits > 1 (each at most 32, pre_splits 0 without a plan): part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  err: 7 a wait ran out,
-// 8 a visible position without a page.
+// are walked here, with n_tiles 0 their shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  own_splits, pre_splits: at most 32 each,
+// pre_splits 0 without a plan.  Scratch with a plan or more than 8 splits: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  err: 7 a wait
+// ran out, 8 a visible position without a page.
 extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                     const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles,
                                     const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,
@@ -561,7 +609,7 @@ extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc,
         page_size % PG_BN || max_pages <= 0 || n_pages <= 0 || n_pages * nkv * page_size > 0x7fffffffLL || own_splits < 1 || own_splits > PG_MAX_SPLITS || pre_splits < 0 ||
         pre_splits > PG_MAX_SPLITS || !q || ((uintptr_t)q & 15) || !kc || !vc || ((uintptr_t)kc & 15) || ((uintptr_t)vc & 15) || (!ksc) != (!vsc) || ((uintptr_t)ksc & 15) ||
         ((uintptr_t)vsc & 15) || !err || (plan_start && (span != 0 || pre_splits < 1)) || (!plan_start && (n_tiles > 0 || pre_splits != 0)) ||
-        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || (own_splits + pre_splits > 1 && (!part_acc || !part_ml || ((uintptr_t)part_ml & 7))))
+        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || ((own_splits > PG_MAX_CLUSTER || plan_start) && (!part_acc || !part_ml || ((uintptr_t)part_ml & 7))) || !out || !token_pos || !token_seq || !block_table)
         return ILLM_ERR_BAD_ARG;
     const PgPlan plan = {plan_start, reinterpret_cast<const int4*>(plan_tiles), plan_members, n_tiles};
     cudaStream_t s = (cudaStream_t)stream;

@@ -519,15 +519,17 @@ static bool tl_bad(const void* q, int q_stride, const void* kc, const void* vc, 
 }
 
 // Prompts over rows of eight bits: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages of bytes
-// [n_pages, nkv, page_size, d] and their scales; cu_q [B + 1], seq_lens [B] as for attention_prefill_tc; out [T, nh * d].  tile_rows: 128 or 256.
+// [n_pages, nkv, page_size, d] and their scales; cu_q [B + 1], seq_lens [B] as for attention_prefill_tc; out [T, nh * d].  tile_rows: 128, 256 or 0 (by a rule).
 // d 64 or 128, page_size a multiple of 64.  span: see first_visible.  err: 5 a wait ran out, 6 shared memory, 8 a visible position without a page.
 extern "C" int illm_attention_tiles_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                          const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d,
                                          int page_size, int span, float scale, int tile_rows, int* err, void* stream) {
     if (B <= 0 || max_q <= 0) return 0;
-    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || !ksc || B > 65535 || (tile_rows != TL_BM && tile_rows != 2 * TL_BM) || !out ||
+    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || !ksc || B > 65535 || (tile_rows && tile_rows != TL_BM && tile_rows != 2 * TL_BM) || !out ||
         ((uintptr_t)out & 15))
         return ILLM_ERR_BAD_ARG;
+    // two tiles a block over the same keys, or one while that leaves SMs without a block
+    if (tile_rows == 0) tile_rows = ((long long)max_q * (nh / nkv) + 2 * TL_BM - 1) / (2 * TL_BM) * nkv * B < illm_sm_count() ? TL_BM : 2 * TL_BM;
     const long long tiles = ((long long)max_q * (nh / nkv) + tile_rows - 1) / tile_rows;
     if (tiles > 65535 || (long long)max_q * (nh / nkv) > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;
     TlWork work = {};

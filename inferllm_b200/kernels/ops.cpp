@@ -126,10 +126,6 @@ int attention_prefix_splits(long long pairs, long long keys, int n_sms) {
     const long long most = std::min<long long>(kRingDecodeMaxSplits, std::max<long long>(1, ceil_div(keys, 128)));
     return (int)std::max<long long>(1, std::min<long long>(most, (long long)n_sms / std::max<long long>(1, pairs)));
 }
-int attention_tile_rows(int B, int max_q, int nh, int nkv, int n_sms) {
-    const long long rows = (long long)max_q * (nkv > 0 ? nh / nkv : 1);
-    return ceil_div(rows, 256) * nkv * B < n_sms ? 128 : 256;
-}
 bool attention_int8_tc_supported(DType dtype, int nh, int nkv, int d, int page_size, bool decode) {
     return dtype == DType::BF16 && nkv > 0 && nh % nkv == 0 && (d == 64 || d == 128) && page_size > 0 && page_size % 64 == 0 && (!decode || nh / nkv <= 16);
 }

@@ -137,8 +137,6 @@ int attention_decode_ring_splits(long long T, int n_kv_heads, long long max_len,
 int attention_pages_splits(long long pairs, long long keys, int n_sms);
 // Parts of a common prefix of `keys` positions that attention_tiles walks for `pairs` (tile, kv head): a block is alone on its SM.
 int attention_prefix_splits(long long pairs, long long keys, int n_sms);
-// Rows of a block of attention_tiles for prompts: 256 (two tiles over the same keys), or 128 while that leaves SMs without a block.
-int attention_tile_rows(int B, int max_q, int nh, int nkv, int n_sms);
 // The tensor-core kernels over rows of eight bits: bfloat16 queries, head size 64 or 128, pages of a multiple of 64 positions; single tokens
 // also need at most 16 query heads per kv head.
 bool attention_int8_tc_supported(DType dtype, int nh, int nkv, int d, int page_size, bool decode);

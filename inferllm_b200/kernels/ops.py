@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -980,32 +981,33 @@ def _page_entry(cache):
     return (k.device,) + tuple(k.shape) + ((k.data_ptr(), v.data_ptr(), None, None),)
 
 
-def _step_arrays(device, T, block_table, **arrays):
-    if block_table.device != device:
-        raise KernelError(f"block_table is on {block_table.device}, the cache on {device}")
-    _need(block_table, "block_table", torch.int32, 2)
-    if block_table.shape[1] < 1:
-        raise KernelError("block_table must have at least one page per sequence")
-    for name, t in arrays.items():
-        _need(t, name, torch.int32, 1)
-        if t.device != device or (T is not None and t.numel() != T):
-            raise KernelError(f"{name} must be int32 [{T}] on {device}, found {tuple(t.shape)} on {t.device}")
+def _step_array(t, name, T, device):
+    # (these run before every small kernel: one look at what is almost always right, the words only where it is not)
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != T or t.device != device or not t.is_contiguous():
+        raise KernelError(f"{name} must be int32 [{T}] on {device}, found {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _block_table(t, device):
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[1] < 1 or t.device != device or not t.is_contiguous():
+        raise KernelError(f"block_table must be int32 [sequences, pages] with at least one page, on {device}, found {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.shape[1]
 
 
 def _query_rows(q, device, n_heads, n_kv_heads, head_dim):
     """The query heads in the first n_heads * head_dim columns of q (rows may lie further apart): rows and their distance."""
-    if not q.is_cuda or q.dim() != 2 or q.device != device:
+    if q.dim() != 2 or q.device != device:
         raise KernelError(f"q must be a matrix on {device}, found shape {tuple(q.shape)} on {q.device}")
     act_code(q.dtype)
     if n_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"attention: {n_heads} heads are no multiple of {n_kv_heads} kv heads")
-    if q.shape[1] < n_heads * head_dim:
-        raise KernelError(f"q has {q.shape[1]} columns, {n_heads} heads of {head_dim} need {n_heads * head_dim}")
-    if q.shape[0] and (q.stride(1) != 1 or q.stride(0) < q.shape[1]):
-        raise KernelError("q: a row's elements must lie side by side")
-    if q.numel() and (q.data_ptr() & 15 or (q.shape[0] > 1 and q.stride(0) * q.element_size() & 15)):
+    (T, width), (apart, side) = q.shape, q.stride()
+    if width < n_heads * head_dim:
+        raise KernelError(f"q has {width} columns, {n_heads} heads of {head_dim} need {n_heads * head_dim}")
+    if T and (side != 1 or (T > 1 and apart < width)):
+        raise KernelError("q: a row's elements must lie side by side, and rows apart")
+    if T and (q.data_ptr() & 15 or (T > 1 and apart * q.element_size() & 15)):
         raise KernelError("q: rows must start on 16-byte boundaries")
-    return q.shape[0], max(q.stride(0), q.shape[1])
+    return T, apart if T > 1 else -(-width // 8) * 8
 
 
 def kv_write_int8(qkv, cos_sin, rot_dim, token_pos, token_seq, block_table, cache, n_heads, err):
@@ -1028,7 +1030,9 @@ def kv_write_int8(qkv, cos_sin, rot_dim, token_pos, token_seq, block_table, cach
         raise KernelError("qkv, err and the cache must be on one device")
     T = qkv.shape[0]
     _need(err, "err", torch.int32)
-    _step_arrays(cache.device, T, block_table, token_pos=token_pos, token_seq=token_seq)
+    width = _block_table(block_table, cache.device)
+    _step_array(token_pos, "token_pos", T, cache.device)
+    _step_array(token_seq, "token_seq", T, cache.device)
     if rot_dim < 0 or rot_dim > d or rot_dim % 2:
         raise KernelError(f"rot_dim {rot_dim} must be even and at most the head size {d}")
     n_pos = 0
@@ -1046,7 +1050,7 @@ def kv_write_int8(qkv, cos_sin, rot_dim, token_pos, token_seq, block_table, cach
         _check(load().illm_kv_write_int8(
             None if partials is not None else _ptr(qkv), None if partials is None else _ptr(partials.ws), 0 if partials is None else partials.splits,
             0 if partials is None else partials.rows * partials.cols, _ptr(q), _ptr(cos_sin) if rot_dim else None, _ptr(token_pos), _ptr(token_seq),
-            _ptr(block_table), block_table.shape[1], cache.pages, *cache.pointers, code, T, n_heads, nkv, d, rot_dim, cache.page_size, 1, n_pos, _ptr(err),
+            _ptr(block_table), width, cache.pages, *cache.pointers, code, T, n_heads, nkv, d, rot_dim, cache.page_size, 1, n_pos, _ptr(err),
             _stream()), "kv_write_int8")
     return q
 
@@ -1056,12 +1060,13 @@ def kv_read_int8(cache, token_pos, token_seq, block_table, dtype=torch.bfloat16)
     NaN."""
     if not isinstance(cache, CacheInt8):
         raise KernelError("kv_read_int8 reads a CacheInt8")
-    n, code = token_pos.numel(), act_code(dtype)
-    _step_arrays(cache.device, n, block_table, token_pos=token_pos, token_seq=token_seq)
+    n, code, width = token_pos.numel(), act_code(dtype), _block_table(block_table, cache.device)
+    _step_array(token_pos, "token_pos", n, cache.device)
+    _step_array(token_seq, "token_seq", n, cache.device)
     with _on(cache.device):
         k = torch.empty((n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
         v = torch.empty_like(k)
-        _check(load().illm_kv_read_int8(*cache.pointers, _ptr(token_pos), _ptr(token_seq), _ptr(block_table), block_table.shape[1], cache.pages, _ptr(k), _ptr(v),
+        _check(load().illm_kv_read_int8(*cache.pointers, _ptr(token_pos), _ptr(token_seq), _ptr(block_table), width, cache.pages, _ptr(k), _ptr(v),
                                         code, n, cache.n_kv_heads, cache.head_dim, cache.page_size, _stream()), "kv_read_int8")
     return k, v
 
@@ -1081,13 +1086,32 @@ def _attention_int8_plain(q, stride, cache, block_table, token_pos, token_seq, n
     return out
 
 
-def _pages_splits(pairs, keys, wide=False) -> int:
-    return int(_b.lib().illm_policy_pages_splits(int(pairs), int(keys), int(wide), n_sms_of_device()))
+_sms = {}
 
 
-def _check_max_len(max_len):
-    if int(max_len) < 1:
-        raise KernelError(f"max_len must be positive, found {max_len}")
+def _splits(pairs, keys, wide, device) -> int:
+    n_sms = _sms.get(device.index)
+    if n_sms is None:
+        n_sms = _sms[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
+    return pages_splits(pairs, keys, wide, n_sms)
+
+
+@functools.lru_cache(maxsize=4096)
+def pages_splits(pairs, keys, wide, n_sms) -> int:
+    """Blocks per (token, kv head) of `attention_decode_int8`, or (`wide`) parts of a common prefix that 256 rows walk together: the engine's policies
+    (`ops::attention_pages_splits`, `ops::attention_prefix_splits`)."""
+    return int(_b.lib().illm_policy_pages_splits(int(pairs), int(keys), int(wide), int(n_sms)))
+
+
+MAX_CLUSTER_SPLITS = 8      # of attention_pages: more of them leave their shares in memory
+
+
+def _shares(T, n_heads, slots, d, device):
+    """Scratch of attention_pages and where its two parts begin."""
+    cut = T * n_heads * slots * d
+    ws = torch.empty(cut + T * n_heads * slots * 2, dtype=torch.float32, device=device)
+    at = ws.data_ptr()
+    return ws, at, at + 4 * cut
 
 
 def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, window, scale, max_len, splits=None):
@@ -1097,32 +1121,27 @@ def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, 
     (float32 among it) on a plain kernel."""
     if not isinstance(cache, CacheInt8):
         raise KernelError("attention_decode_int8 reads a CacheInt8")
-    d, nkv, span = cache.head_dim, cache.n_kv_heads, int(window or 0)
-    T, stride = _query_rows(q, cache.device, n_heads, nkv, d)
-    _step_arrays(cache.device, T, block_table, token_pos=token_pos, token_seq=token_seq)
-    _check_max_len(max_len)
-    with _on(cache.device):
+    device, d, nkv, span = cache.device, cache.head_dim, cache.n_kv_heads, int(window or 0)
+    T, stride = _query_rows(q, device, n_heads, nkv, d)
+    width = _block_table(block_table, device)
+    _step_array(token_pos, "token_pos", T, device)
+    _step_array(token_seq, "token_seq", T, device)
+    max_len = int(max_len)
+    if max_len < 1:
+        raise KernelError(f"max_len must be positive, found {max_len}")
+    with _on(device):
         if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, cache.page_size, True):
             return _attention_int8_plain(q, stride, cache, block_table, token_pos, token_seq, n_heads, span, scale)
-        out = torch.empty((T, n_heads * d), dtype=torch.bfloat16, device=cache.device)
-        keys = min(int(max_len), abs(span)) if span else int(max_len)
+        out = torch.empty((T, n_heads * d), dtype=torch.bfloat16, device=device)
+        run, keys, err, stream = load().illm_attention_pages, min(max_len, abs(span)) if span else max_len, _error_word(device), _stream()
         for t0 in range(0, T, 65535):
-            t1 = min(T, t0 + 65535)
-            n = _pages_splits((t1 - t0) * nkv, keys) if splits is None else int(splits)
-            acc, ml = _shares(t1 - t0, n_heads, n, d, cache.device)
-            _check(load().illm_attention_pages(_ptr(q[t0:t1]), stride, *cache.pointers, cache.pages, _ptr(block_table), block_table.shape[1], _ptr(token_pos[t0:t1]),
-                                               _ptr(token_seq[t0:t1]), None, None, None, 0, _ptr(acc), _ptr(ml), _ptr(out[t0:t1]), t1 - t0, n_heads, nkv, d,
-                                               cache.page_size, span, float(scale), n, 0, _error_word(cache.device), _stream()), "attention_decode_int8")
+            n = min(T - t0, 65535)
+            s = _splits(n * nkv, keys, False, device) if splits is None else int(splits)
+            ws, acc, ml = _shares(n, n_heads, s, d, device) if s > MAX_CLUSTER_SPLITS else (None, None, None)
+            _check(run(q.data_ptr() + t0 * stride * 2, stride, *cache.pointers, cache.pages, block_table.data_ptr(), width, token_pos.data_ptr() + 4 * t0,
+                       token_seq.data_ptr() + 4 * t0, None, None, None, 0, acc, ml, out.data_ptr() + t0 * n_heads * d * 2, n, n_heads, nkv, d, cache.page_size, span,
+                       float(scale), s, 0, err, stream), "attention_decode_int8")
     return out
-
-
-def _shares(T, n_heads, slots, d, device):
-    """Scratch of attention_pages."""
-    if slots == 1:
-        return None, None
-    ws = torch.empty(T * n_heads * slots * (d + 2), dtype=torch.float32, device=device)
-    cut = T * n_heads * slots * d
-    return ws[:cut], ws[cut:]
 
 
 def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads, window, scale, tile_rows=None):
@@ -1131,22 +1150,22 @@ def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads
     sizes 64 and 128 and pages of a multiple of 64 positions."""
     if not isinstance(cache, CacheInt8):
         raise KernelError("attention_prompts_int8 reads a CacheInt8")
-    d, nkv, B = cache.head_dim, cache.n_kv_heads, seq_lens.numel()
-    T, stride = _query_rows(q, cache.device, n_heads, nkv, d)
-    _step_arrays(cache.device, B, block_table, seq_lens=seq_lens)
-    _step_arrays(cache.device, B + 1, block_table, cu_q=cu_q)
-    if int(max_q) < 0 or int(max_q) > T:
+    device, d, nkv, B, max_q = cache.device, cache.head_dim, cache.n_kv_heads, seq_lens.numel(), int(max_q)
+    T, stride = _query_rows(q, device, n_heads, nkv, d)
+    width = _block_table(block_table, device)
+    _step_array(seq_lens, "seq_lens", B, device)
+    _step_array(cu_q, "cu_q", B + 1, device)
+    if max_q < 0 or max_q > T:
         raise KernelError(f"max_q {max_q} is outside the step's {T} tokens")
     if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, cache.page_size, False):
         raise KernelError(f"attention_prompts_int8 takes bfloat16, head sizes 64 and 128 and pages of a multiple of 64 positions, found {q.dtype}, {d} and "
                           f"{cache.page_size} (attention_decode_int8 takes prompts of other sizes token by token)")
-    with _on(cache.device):
-        out = _rows(T, n_heads * d, torch.bfloat16, cache.device)
+    with _on(device):
+        out = _rows(T, n_heads * d, torch.bfloat16, device)
         if T and B:
-            rows = int(_b.lib().illm_policy_tile_rows(B, int(max_q), n_heads, nkv, n_sms_of_device())) if tile_rows is None else int(tile_rows)
-            _check(load().illm_attention_tiles_int8(_ptr(q), stride, *cache.pointers, cache.pages, _ptr(block_table), block_table.shape[1], _ptr(cu_q), _ptr(seq_lens),
-                                                    _ptr(out), B, int(max_q), n_heads, nkv, d, cache.page_size, int(window or 0), float(scale), rows,
-                                                    _error_word(cache.device), _stream()), "attention_prompts_int8")
+            _check(load().illm_attention_tiles_int8(q.data_ptr(), stride, *cache.pointers, cache.pages, block_table.data_ptr(), width, cu_q.data_ptr(), seq_lens.data_ptr(),
+                                                    out.data_ptr(), B, max_q, n_heads, nkv, d, cache.page_size, int(window or 0), float(scale), int(tile_rows or 0),
+                                                    _error_word(device), _stream()), "attention_prompts_int8")
     return out
 
 
@@ -1181,8 +1200,9 @@ def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n
     positions, at most 16 query heads per kv head; others are refused."""
     device, pages, nkv, page_size, d, pointers = _page_entry(cache)
     T, stride = _query_rows(q, device, n_heads, nkv, d)
-    _step_arrays(device, T, block_table, token_pos=token_pos, token_seq=token_seq)
-    _check_max_len(max_len)
+    width = _block_table(block_table, device)
+    _step_array(token_pos, "token_pos", T, device)
+    _step_array(token_seq, "token_seq", T, device)
     if not attention_int8_tc_supported(q.dtype, n_heads, nkv, d, page_size, True):
         raise KernelError(f"attention_decode_shared takes bfloat16, head sizes 64 and 128, pages of a multiple of 64 positions and up to 16 query heads per kv head, "
                           f"found {q.dtype}, {d}, {page_size} and {n_heads} over {nkv}")
@@ -1193,18 +1213,17 @@ def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n
     with _on(device):
         out = torch.empty((T, n_heads * d), dtype=torch.bfloat16, device=device)
         common = plan.tiles > 0
-        own = _pages_splits(T * nkv, max(1, plan.longest_rest)) if own_splits is None else int(own_splits)
-        pre = (_pages_splits(plan.tiles * nkv, plan.longest_prefix, plan.wide) if pre_splits is None else int(pre_splits)) if common else 0
-        acc, ml = _shares(T, n_heads, own + pre, d, device)
+        own = _splits(T * nkv, max(1, plan.longest_rest), False, device) if own_splits is None else int(own_splits)
+        pre = (_splits(plan.tiles * nkv, plan.longest_prefix, plan.wide, device) if pre_splits is None else int(pre_splits)) if common else 0
+        ws, acc, ml = _shares(T, n_heads, own + pre, d, device) if common or own > MAX_CLUSTER_SPLITS else (None, None, None)
         start, tiles, members = plan.pointers if common else (None, None, None)
-        err = _error_word(device)
+        h, err, stream = load(), _error_word(device), _stream()
+        at, table, pos, seq = q.data_ptr(), block_table.data_ptr(), token_pos.data_ptr(), token_seq.data_ptr()
         if common and plan.wide:
-            _check(load().illm_attention_tiles_prefix(_ptr(q), stride, *pointers, pages, _ptr(block_table), block_table.shape[1], _ptr(token_seq), tiles, members,
-                                                      plan.tiles, _ptr(acc), _ptr(ml), n_heads, nkv, d, page_size, float(scale), own + pre, own, pre, err,
-                                                      _stream()), "attention_decode_shared")
-        _check(load().illm_attention_pages(_ptr(q), stride, *pointers, pages, _ptr(block_table), block_table.shape[1], _ptr(token_pos), _ptr(token_seq), start, tiles,
-                                           members, 0 if plan.wide else plan.tiles, _ptr(acc), _ptr(ml), _ptr(out), T, n_heads, nkv, d, page_size, 0, float(scale),
-                                           own, pre, err, _stream()), "attention_decode_shared")
+            _check(h.illm_attention_tiles_prefix(at, stride, *pointers, pages, table, width, seq, tiles, members, plan.tiles, acc, ml, n_heads, nkv, d, page_size,
+                                                 float(scale), own + pre, own, pre, err, stream), "attention_decode_shared")
+        _check(h.illm_attention_pages(at, stride, *pointers, pages, table, width, pos, seq, start, tiles, members, 0 if plan.wide else plan.tiles, acc, ml,
+                                      out.data_ptr(), T, n_heads, nkv, d, page_size, 0, float(scale), own, pre, err, stream), "attention_decode_shared")
     return out
 
 
