@@ -201,38 +201,55 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
         }
     } else if (warp == TL_MMA_WARP) {
-        // ---- products: the scores of a tile one block ahead of its softmax
-        if (lane == 0 && n_blocks > 0) {
-            bool alive = mbar_wait(q_full, 0, err, TC_ERR_TIMEOUT_PREFILL);
-            auto issue_s = [&](int w, int i) {
-                const int st = i % STAGES;
-                if (!mbar_wait(k_full0 + 8 * st, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_PREFILL)) return false;
+        // ---- products: the scores of both tiles one block ahead of their softmax.  The warp stays together around what one lane issues, so that
+        // descriptors lie in uniform registers (a lane by itself took 95 clocks for each instruction).
+        const bool elected = elect_one();
+        const unsigned long long q_desc = desc_kmajor(q_s), k_desc = desc_kmajor(kv_s), v_desc = desc_mnmajor(kv_s + TILE, ATOM);
+        auto wait = [&](unsigned bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, err, TC_ERR_TIMEOUT_PREFILL)) != 0; };
+        auto issue_s = [&](int w, int i, int st) {
+            if (!elected) return;
+            const unsigned long long qd = q_desc + w * (Z::Q_TILE >> 4), kd = k_desc + (unsigned)st * (2 * TILE >> 4);
+            const unsigned to = tmem + w * TILE_COLS + (i & 1) * S_COLS;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++)
+                mma_bf16_ss(to, qd + (kk >> 2) * (Q_ATOM >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (ATOM >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
+            mma_commit(s_full0 + 8 * (2 * w + (i & 1)));
+            if (w == (i < nb[1] ? 1 : 0)) mma_commit(k_empty0 + 8 * st);            // the last tile that reads the stage
+        };
+        bool alive = n_blocks > 0 && wait(q_full, 0) && wait(k_full0, 0);
+        if (alive) {
+            tc_fence_after();
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+                if (nb[w] > 0) issue_s(w, 0, 0);
+        }
+        for (int i = 0; i < n_blocks && alive; i++) {
+            if (i + 1 < n_blocks) {
+                const int st = (i + 1) % STAGES;
+                if (!(alive = wait(k_full0 + 8 * st, (i + 1) / STAGES))) break;
                 tc_fence_after();
+                // (both tiles' next scores before the wait for either's weights: otherwise the second tile's softmax stands still until the first
+                // one's is through)
 #pragma unroll
-                for (int kk = 0; kk < D / 16; kk++)
-                    mma_bf16_ss(tmem + w * TILE_COLS + (i & 1) * S_COLS, desc_kmajor(q_s + w * Z::Q_TILE + (kk >> 2) * Q_ATOM + (kk & 3) * 32),
-                                desc_kmajor(kv_s + st * 2 * TILE + (kk >> 2) * ATOM + (kk & 3) * 32), IDESC_S, kk > 0);
-                mma_commit(s_full0 + 8 * (2 * w + (i & 1)));
-                if (w == (i < nb[1] ? 1 : 0)) mma_commit(k_empty0 + 8 * st);        // the last tile that reads the stage
-                return true;
-            };
-            for (int w = 0; w < 2 && alive; w++)
-                if (nb[w] > 0) alive = issue_s(w, 0);
-            for (int i = 0; i < n_blocks && alive; i++)
-                for (int w = 0; w < 2 && alive; w++) {
-                    if (i >= nb[w]) continue;
-                    if (i + 1 < nb[w] && !(alive = issue_s(w, i + 1))) break;
-                    const int st = i % STAGES;
-                    if (!(alive = mbar_wait(p_full0 + 8 * (2 * w + (i & 1)), (i >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL))) break;
-                    if (!(alive = mbar_wait(v_full0 + 8 * st, (i / STAGES) & 1, err, TC_ERR_TIMEOUT_PREFILL))) break;
-                    tc_fence_after();
+                for (int w = 0; w < 2; w++)
+                    if (i + 1 < nb[w]) issue_s(w, i + 1, st);
+            }
+            const int st = i % STAGES;
+            if (!(alive = wait(v_full0 + 8 * st, i / STAGES))) break;
 #pragma unroll
-                    for (int ks = 0; ks < TL_BN / 16; ks++)
-                        mma_bf16_ts(tmem + w * TILE_COLS + O_COL, tmem + w * TILE_COLS + (i & 1) * S_COLS + ks * 8,
-                                    desc_mnmajor(kv_s + st * 2 * TILE + TILE + ks * 16 * 128, ATOM), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
-                    if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
-                    mma_commit(pv_done0 + 8 * w);
-                }
+            for (int w = 0; w < 2; w++) {
+                if (i >= nb[w] || !alive) continue;
+                if (!(alive = wait(p_full0 + 8 * (2 * w + (i & 1)), i >> 1))) continue;
+                tc_fence_after();
+                if (!elected) continue;
+                const unsigned long long vd = v_desc + (unsigned)st * (2 * TILE >> 4);
+                const unsigned p_at = tmem + w * TILE_COLS + (i & 1) * S_COLS;
+#pragma unroll
+                for (int ks = 0; ks < TL_BN / 16; ks++)
+                    mma_bf16_ts(tmem + w * TILE_COLS + O_COL, p_at + ks * 8, vd + ks * (16 * 128 >> 4), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
+                if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
+                mma_commit(pv_done0 + 8 * w);
+            }
         }
     } else if (Q8 && warp >= TL_WIDEN_WARP) {
         // ---- bytes to bfloat16, and the factors of the scores (with the softmax's scale) and of the weights.  Keys outside the block's range, where
