@@ -10,7 +10,7 @@
 // costs about two instructions an element, which is why the tiles share it; two rows five apart (r and r XOR 5) go to a quarter of a warp, so that neither
 // its loads nor its stores meet in a bank.  The rows' scales are factors of the scores and, the values', of the softmax weights.
 // Tensor memory of a tile, 256 columns: two score buffers of 64 and the output.  As in attention_prefill_tc.cu the scores
-// of the next 64 keys are made while the softmax works on the last ones, the weights stay in tensor memory in place of their scores,
+// of the next keys are made while the softmax works on the last ones, the weights stay in tensor memory in place of their scores,
 // and the output is rescaled only when a row's maximum has grown by more than 2^8.
 // Rounded to bfloat16 are the softmax weights (times the value's scale) and the results; scores, sums and the running output are float32.  (Rows
 // widened with their scales in them, and so rounded, put the results 0.006 of their norm off at scores of spread 2; like this it is 0.002.)
@@ -94,7 +94,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const unsigned f_s = sc_s + Z::RAW * Z::SCALES;         // the factors of a block's scores and weights
     const unsigned bars0 = f_s + Z::RAW * Z::SCALES;
     const unsigned q_full = bars0, k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * STAGES, v_full0 = k_empty0 + 8 * STAGES, v_empty0 = v_full0 + 8 * STAGES;
-    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32, f_full0 = pv_done0 + 16;
+    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32, f_full0 = pv_done0 + 32;
     unsigned* holder = reinterpret_cast<unsigned*>(smem_raw + (f_full0 + 8 * TL_RAW - base));
     if ((base & 1023u) != 0) {          // cannot happen without static shared memory; never run misaligned
         if (threadIdx.x == 0) atomicExch(err, TC_ERR_MISALIGNED_SMEM);
@@ -118,7 +118,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             mbar_init(s_full0 + 8 * i, 1);
             mbar_init(p_full0 + 8 * i, TL_BM);
         }
-        for (int w = 0; w < 2; w++) mbar_init(pv_done0 + 8 * w, 1);
+        for (int i = 0; i < 4; i++) mbar_init(pv_done0 + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -201,13 +201,16 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
         }
     } else if (warp == TL_MMA_WARP) {
-        // ---- products: the scores of both tiles one block ahead of their softmax.  The warp stays together around what one lane issues, so that
-        // descriptors lie in uniform registers (a lane by itself took 95 clocks for each instruction).
+        // ---- products, in this order: S(0, 0) S(1, 0) S(0, 1) S(1, 1), then per block i and tile w  O(w) += P(w, i) V(i), S(w, i + 2).  A tile's scores are
+        // there a whole block before its softmax asks for them, in the buffer that its last weights have left.  (One block ahead, behind the
+        // other tile's weights, a softmax stood still for a fifth of its time.)  The warp stays together around what one lane issues, so that descriptors
+        // lie in uniform registers (a lane by itself took 95 clocks for each instruction).
         const bool elected = elect_one();
         const unsigned long long q_desc = desc_kmajor(q_s), k_desc = desc_kmajor(kv_s), v_desc = desc_mnmajor(kv_s + TILE, ATOM);
         auto wait = [&](unsigned bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, err, TC_ERR_TIMEOUT_PREFILL)) != 0; };
-        auto issue_s = [&](int w, int i, int st) {
+        auto issue_s = [&](int w, int i) {
             if (!elected) return;
+            const int st = i % STAGES;
             const unsigned long long qd = q_desc + w * (Z::Q_TILE >> 4), kd = k_desc + (unsigned)st * (2 * TILE >> 4);
             const unsigned to = tmem + w * TILE_COLS + (i & 1) * S_COLS;
 #pragma unroll
@@ -216,24 +219,15 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             mma_commit(s_full0 + 8 * (2 * w + (i & 1)));
             if (w == (i < nb[1] ? 1 : 0)) mma_commit(k_empty0 + 8 * st);            // the last tile that reads the stage
         };
-        bool alive = n_blocks > 0 && wait(q_full, 0) && wait(k_full0, 0);
-        if (alive) {
+        bool alive = n_blocks > 0 && wait(q_full, 0);
+        for (int i = 0; i < 2 && i < n_blocks && alive; i++) {
+            if (!(alive = wait(k_full0 + 8 * i, 0))) break;
             tc_fence_after();
 #pragma unroll
             for (int w = 0; w < 2; w++)
-                if (nb[w] > 0) issue_s(w, 0, 0);
+                if (i < nb[w]) issue_s(w, i);
         }
         for (int i = 0; i < n_blocks && alive; i++) {
-            if (i + 1 < n_blocks) {
-                const int st = (i + 1) % STAGES;
-                if (!(alive = wait(k_full0 + 8 * st, (i + 1) / STAGES))) break;
-                tc_fence_after();
-                // (both tiles' next scores before the wait for either's weights: otherwise the second tile's softmax stands still until the first
-                // one's is through)
-#pragma unroll
-                for (int w = 0; w < 2; w++)
-                    if (i + 1 < nb[w]) issue_s(w, i + 1, st);
-            }
             const int st = i % STAGES;
             if (!(alive = wait(v_full0 + 8 * st, i / STAGES))) break;
 #pragma unroll
@@ -241,20 +235,26 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (i >= nb[w] || !alive) continue;
                 if (!(alive = wait(p_full0 + 8 * (2 * w + (i & 1)), i >> 1))) continue;
                 tc_fence_after();
-                if (!elected) continue;
-                const unsigned long long vd = v_desc + (unsigned)st * (2 * TILE >> 4);
-                const unsigned p_at = tmem + w * TILE_COLS + (i & 1) * S_COLS;
+                if (elected) {
+                    const unsigned long long vd = v_desc + (unsigned)st * (2 * TILE >> 4);
+                    const unsigned p_at = tmem + w * TILE_COLS + (i & 1) * S_COLS;
 #pragma unroll
-                for (int ks = 0; ks < TL_BN / 16; ks++)
-                    mma_bf16_ts(tmem + w * TILE_COLS + O_COL, p_at + ks * 8, vd + ks * (16 * 128 >> 4), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
-                if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
-                mma_commit(pv_done0 + 8 * w);
+                    for (int ks = 0; ks < TL_BN / 16; ks++)
+                        mma_bf16_ts(tmem + w * TILE_COLS + O_COL, p_at + ks * 8, vd + ks * (16 * 128 >> 4), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
+                    if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
+                    mma_commit(pv_done0 + 8 * (2 * w + (i & 1)));
+                }
+                if (i + 2 < nb[w]) {
+                    if (!(alive = wait(k_full0 + 8 * ((i + 2) % STAGES), (i + 2) / STAGES))) continue;
+                    tc_fence_after();
+                    issue_s(w, i + 2);
+                }
             }
         }
     } else if (Q8 && warp >= TL_WIDEN_WARP) {
         // ---- bytes to bfloat16, and the factors of the scores (with the softmax's scale) and of the weights.  Keys outside the block's range, where
-        // another sequence's may lie, have factors of zero.  The ring of factors has four places: those of block i + 4 come once the
-        // products of block i + 1 are done (v_empty), so behind every softmax of block i.
+        // another sequence's may lie, have factors of zero.  The ring of factors has four places: those of block i + 4 come behind the
+        // wait for the products of block i + 1 (v_empty), so behind every softmax of block i.
         const int ct = threadIdx.x - TL_WIDEN_WARP * 32;
         auto widen = [&](const unsigned char* raw, unsigned dst) {
 #pragma unroll
@@ -270,26 +270,31 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tl_store16(at + (((p + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
             }
         };
-        for (int i = 0; i < n_blocks; i++) {
+        // in the order in which the products ask: K(0), K(1), V(0), K(2), V(1), ...
+        auto keys = [&](int i) {
             const int rs = i % TL_RAW, st = i % STAGES, key0 = (jb0 + i) * TL_BN;
-            const unsigned char* raw = smem_raw + (raw_s - base) + rs * 2 * Z::RAW_TILE;
-            const float* ks = reinterpret_cast<const float*>(smem_raw + (sc_s - base) + rs * Z::SCALES);
-            const float* vs = ks + TL_BN;
-            const unsigned kd = kv_s + st * 2 * TILE, vd = kd + TILE;
-            if (!mbar_wait(raw_full0 + 8 * rs, (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
+            if (!mbar_wait(raw_full0 + 8 * rs, (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL)) return false;
             if (ct < TL_BN) {
+                const float* ks = reinterpret_cast<const float*>(smem_raw + (sc_s - base) + rs * Z::SCALES);
+                const float* vs = ks + TL_BN;
                 const bool in = key0 + ct >= first_key && key0 + ct <= last_key, number = fabsf(ks[ct]) < INFINITY && fabsf(vs[ct]) < INFINITY;
                 float* f = reinterpret_cast<float*>(smem_raw + (f_s - base) + rs * Z::SCALES);
                 f[ct] = !in ? 0.f : number ? ks[ct] * scale_log2e : __uint_as_float(0x7fffffffu);
                 f[TL_BN + ct] = in && number ? vs[ct] : 0.f;
                 tl_arrive(f_full0 + 8 * rs);
             }
-            if (i >= STAGES && !mbar_wait(k_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
-            widen(raw, kd);
+            if (i >= STAGES && !mbar_wait(k_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) return false;
+            widen(smem_raw + (raw_s - base) + rs * 2 * Z::RAW_TILE, kv_s + st * 2 * TILE);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tl_arrive(k_full0 + 8 * st);
-            if (i >= STAGES && !mbar_wait(v_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)) break;
-            widen(raw + Z::RAW_TILE, vd);
+            return true;
+        };
+        bool alive = n_blocks > 0 && keys(0);
+        for (int i = 0; i < n_blocks && alive; i++) {
+            if (i + 1 < n_blocks && !(alive = keys(i + 1))) break;
+            const int rs = i % TL_RAW, st = i % STAGES;
+            if (i >= STAGES && !(alive = mbar_wait(v_empty0 + 8 * st, ((i / STAGES) - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL))) break;
+            widen(smem_raw + (raw_s - base) + rs * 2 * Z::RAW_TILE + Z::RAW_TILE, kv_s + st * 2 * TILE + TILE);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tl_arrive(v_full0 + 8 * st);
             tl_arrive(raw_empty0 + 8 * rs);
@@ -328,6 +333,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const int tile_first = PREFIX ? last_key : past + (row0 + w * TL_BM) / G, tile_last = PREFIX ? last_key : past + (row0 + min(n_rows, (w + 1) * TL_BM) - 1) / G;
         const int lo_pos = PREFIX ? 0 : nbw > 0 ? first_visible(pos, work.span) : 0, lo_last = PREFIX || nbw == 0 ? 0 : first_visible(tile_last, work.span);
         const float unit = Q8 ? 1.f : scale_log2e;
+        // (pv_done has a barrier for even and one for odd blocks and is waited for only where the output is touched: the scores of block i come behind the
+        // products of block i - 2, so when this thread has them, the phase in question is the next one to end)
         float m_ref = -INFINITY, l_run = 0.f;
         bool alive = true;
         for (int i = 0; i < nbw; i++) {
@@ -369,12 +376,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * unit);
             const bool grown = m_new > m_ref + TL_RESCALE_STEP;      // true for m_ref = -inf, m_new finite
-            bool pv_seen = false;
             if (__any_sync(0xffffffffu, grown)) {
                 if (i > 0) {
-                    pv_seen = true;
                     const float corr = m_new == -INFINITY ? 1.f : m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new);
-                    alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (i - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+                    alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (2 * w + ((i - 1) & 1)), ((i - 1) >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
                     if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -434,13 +439,11 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         for (int c = 0; c < 8; c++) tl_store16(kv_s + st * 2 * TILE + TILE + a * ATOM + r * 128 + c * 16, 0u, 0u, 0u, 0u);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            // (every phase of pv_done is observed, in order, before this thread lets the next one begin)
-            if (i > 0 && !pv_seen) alive = __all_sync(0xffffffffu, alive && mbar_wait(pv_done0 + 8 * w, (i - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
             if (!alive) break;
             tc_fence_before();
             tl_arrive(p_full0 + 8 * (2 * w + (i & 1)));
         }
-        if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (nbw - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+        if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (2 * w + ((nbw - 1) & 1)), ((nbw - 1) >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
         const size_t head = (size_t)token * nh + h;
         if (PREFIX) {
             const size_t share = head * work.slots + work.slot0 + blockIdx.x;
