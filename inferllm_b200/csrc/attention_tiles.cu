@@ -9,9 +9,10 @@
 // bytes from a ring of four raw stages become u - 128 in bfloat16, exactly, in the swizzled layout that the products read.  Widening
 // costs about two instructions an element, which is why the tiles share it; two rows five apart (r and r XOR 5) go to a quarter of a warp, so that neither
 // its loads nor its stores meet in a bank.  The rows' scales are factors of the scores and, the values', of the softmax weights.
-// Tensor memory of a tile, 256 columns: two score buffers of 64 and the output.  As in attention_prefill_tc.cu the scores
-// of the next keys are made while the softmax works on the last ones, the weights stay in tensor memory in place of their scores,
-// and the output is rescaled only when a row's maximum has grown by more than 2^8.
+// Tensor memory: the tiles' outputs, their scores of 64 keys, their weights (32 columns) and the first tile's queries, 512 columns at head size 128.
+// With both operands in shared memory a product of 128 x 64 x 16 took about 95 clocks, as much again as one of twice the size whose rows come from
+// tensor memory, and 256 rows were bound by that.  The scores of the next keys are made while the softmax works on the last ones; the output is rescaled
+// only when a row's maximum has grown by more than 2^8.
 // Rounded to bfloat16 are the softmax weights (times the value's scale) and the results; scores, sums and the running output are float32.  (Rows
 // widened with their scales in them, and so rounded, put the results 0.006 of their norm off at scores of spread 2; like this it is 0.002.)
 // A key whose row reads back as NaN has its score NaN instead, so that it reaches the queries that see it and no others.
@@ -25,9 +26,9 @@
 #define TL_BN 64
 #define TL_RAW 4                        // raw stages (eight bits)
 #define TL_SOFTMAX 8                    // warps
-#define TL_MMA_WARP 8
-#define TL_TMA_WARP 9
-#define TL_WIDEN_WARP 10                // the first of four
+#define TL_MMA_WARP 8                   // the first of two, one for each tile
+#define TL_TMA_WARP 10
+#define TL_WIDEN_WARP 11                // the first of four
 #define TL_ERR_PAGE 8
 #define TL_RESCALE_STEP 8.0f
 
@@ -45,7 +46,7 @@ template <int D, bool Q8> struct TlSizes {
     static constexpr int STAGES = Q8 ? 2 : 4, TILE = TL_BN * D * 2, Q_TILE = TL_BM * D * 2;
     static constexpr int RAW_TILE = TL_BN * D, RAW = Q8 ? TL_RAW : 0, SCALES = 2 * TL_BN * 4;
     static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + RAW * (2 * RAW_TILE + 2 * SCALES) + 512;
-    static constexpr int THREADS = (Q8 ? 14 : 10) * 32;
+    static constexpr int THREADS = (Q8 ? 15 : 11) * 32;
 };
 
 namespace {
@@ -85,7 +86,10 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                        int nh, int nkv, int page_size, float scale_log2e, int* __restrict__ err) {
     using Z = TlSizes<D, Q8>;
     constexpr int STAGES = Z::STAGES, TILE = Z::TILE, NA = D / 64;
-    constexpr unsigned ATOM = TL_BN * 128, Q_ATOM = TL_BM * 128, S_COLS = TL_BN, O_COL = 2 * TL_BN, TILE_COLS = 256;
+    constexpr unsigned ATOM = TL_BN * 128, Q_ATOM = TL_BM * 128;
+    // columns of tensor memory: outputs, scores, weights, and the queries of the first tile (of both where they fit)
+    constexpr unsigned S_COL = 2 * D, P_COL = S_COL + 2 * TL_BN, Q_COL = P_COL + TL_BN, TMEM_COLS = 512;
+    constexpr bool BOTH_Q = Q_COL + D <= TMEM_COLS;
     constexpr unsigned IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TL_BN >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     constexpr unsigned IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(D >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -94,7 +98,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const unsigned f_s = sc_s + Z::RAW * Z::SCALES;         // the factors of a block's scores and weights
     const unsigned bars0 = f_s + Z::RAW * Z::SCALES;
     const unsigned q_full = bars0, k_full0 = q_full + 8, k_empty0 = k_full0 + 8 * STAGES, v_full0 = k_empty0 + 8 * STAGES, v_empty0 = v_full0 + 8 * STAGES;
-    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, p_full0 = s_full0 + 32, pv_done0 = p_full0 + 32, f_full0 = pv_done0 + 32;
+    const unsigned raw_full0 = v_empty0 + 8 * STAGES, raw_empty0 = raw_full0 + 8 * TL_RAW, s_full0 = raw_empty0 + 8 * TL_RAW, s_read0 = s_full0 + 16, p_full0 = s_read0 + 16, pv_done0 = p_full0 + 16, f_full0 = pv_done0 + 16;
     unsigned* holder = reinterpret_cast<unsigned*>(smem_raw + (f_full0 + 8 * TL_RAW - base));
     if ((base & 1023u) != 0) {          // cannot happen without static shared memory; never run misaligned
         if (threadIdx.x == 0) atomicExch(err, TC_ERR_MISALIGNED_SMEM);
@@ -106,24 +110,25 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < STAGES; i++) {
             mbar_init(k_full0 + 8 * i, Q8 ? 128 : 1);
             mbar_init(v_full0 + 8 * i, Q8 ? 128 : 1);
-            mbar_init(k_empty0 + 8 * i, 1);
-            mbar_init(v_empty0 + 8 * i, 1);
+            mbar_init(k_empty0 + 8 * i, 2);        // both tiles
+            mbar_init(v_empty0 + 8 * i, 2);
         }
         for (int i = 0; i < TL_RAW; i++) {
             mbar_init(raw_full0 + 8 * i, 1);
             mbar_init(raw_empty0 + 8 * i, 128);
             mbar_init(f_full0 + 8 * i, TL_BN);
         }
-        for (int i = 0; i < 4; i++) {
-            mbar_init(s_full0 + 8 * i, 1);
-            mbar_init(p_full0 + 8 * i, TL_BM);
+        for (int w = 0; w < 2; w++) {
+            mbar_init(s_full0 + 8 * w, 1);
+            mbar_init(s_read0 + 8 * w, TL_BM);
+            mbar_init(p_full0 + 8 * w, TL_BM);
+            mbar_init(pv_done0 + 8 * w, 1);
         }
-        for (int i = 0; i < 4; i++) mbar_init(pv_done0 + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == TL_MMA_WARP) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(holder)), "r"(2 * TILE_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(holder)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -200,55 +205,56 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 }
             }
         }
-    } else if (warp == TL_MMA_WARP) {
-        // ---- products, in this order: S(0, 0) S(1, 0) S(0, 1) S(1, 1), then per block i and tile w  O(w) += P(w, i) V(i), S(w, i + 2).  A tile's scores are
-        // there a whole block before its softmax asks for them, in the buffer that its last weights have left.  (One block ahead, behind the
-        // other tile's weights, a softmax stood still for a fifth of its time.)  The warp stays together around what one lane issues, so that descriptors
-        // lie in uniform registers (a lane by itself took 95 clocks for each instruction).
-        const bool elected = elect_one();
-        const unsigned long long q_desc = desc_kmajor(q_s), k_desc = desc_kmajor(kv_s), v_desc = desc_mnmajor(kv_s + TILE, ATOM);
+    } else if (warp == TL_MMA_WARP || warp == TL_MMA_WARP + 1) {
+        // ---- products, a warp for each tile (one for both was busy with its waits and commits for longer than a softmax).  The scores of block i + 1 are made
+        // as soon as the softmax has taken those of block i into its registers, and so are there when it comes back.  The warp stays together around what one
+        // lane issues, so that descriptors lie in uniform registers (a lane by itself took 95 clocks for each instruction).
+        const int w = warp - TL_MMA_WARP, nbw = nb[w];
+        const bool elected = elect_one(), q_in_tmem = w == 0 || BOTH_Q;
+        const unsigned long long q_desc = desc_kmajor(q_s + w * Z::Q_TILE), k_desc = desc_kmajor(kv_s), v_desc = desc_mnmajor(kv_s + TILE, ATOM);
+        const unsigned s_at = tmem + S_COL + w * TL_BN, p_at = tmem + P_COL + w * (TL_BN / 2), o_at = tmem + w * D, q_at = tmem + Q_COL + w * (D / 2);
         auto wait = [&](unsigned bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, err, TC_ERR_TIMEOUT_PREFILL)) != 0; };
-        auto issue_s = [&](int w, int i) {
-            if (!elected) return;
+        auto scores = [&](int i) {
             const int st = i % STAGES;
-            const unsigned long long qd = q_desc + w * (Z::Q_TILE >> 4), kd = k_desc + (unsigned)st * (2 * TILE >> 4);
-            const unsigned to = tmem + w * TILE_COLS + (i & 1) * S_COLS;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++)
-                mma_bf16_ss(to, qd + (kk >> 2) * (Q_ATOM >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (ATOM >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
-            mma_commit(s_full0 + 8 * (2 * w + (i & 1)));
-            if (w == (i < nb[1] ? 1 : 0)) mma_commit(k_empty0 + 8 * st);            // the last tile that reads the stage
-        };
-        bool alive = n_blocks > 0 && wait(q_full, 0);
-        for (int i = 0; i < 2 && i < n_blocks && alive; i++) {
-            if (!(alive = wait(k_full0 + 8 * i, 0))) break;
+            if (!wait(k_full0 + 8 * st, i / STAGES)) return false;
+            if (i >= nbw) {                                  // the other tile's alone
+                if (elected) tl_arrive(k_empty0 + 8 * st);
+                return true;
+            }
+            if (i > 0 && !wait(s_read0 + 8 * w, i - 1)) return false;
             tc_fence_after();
+            if (elected) {
+                const unsigned long long kd = k_desc + (unsigned)st * (2 * TILE >> 4);
+                if (q_in_tmem) {
 #pragma unroll
-            for (int w = 0; w < 2; w++)
-                if (i < nb[w]) issue_s(w, i);
-        }
+                    for (int kk = 0; kk < D / 16; kk++) mma_bf16_ts(s_at, q_at + kk * 8, kd + (kk >> 2) * (ATOM >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++)
+                        mma_bf16_ss(s_at, q_desc + (kk >> 2) * (Q_ATOM >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (ATOM >> 4) + (kk & 3) * 2, IDESC_S, kk > 0);
+                }
+                mma_commit(s_full0 + 8 * w);
+                mma_commit(k_empty0 + 8 * st);
+            }
+            return true;
+        };
+        bool alive = n_blocks > 0 && wait(q_full, 0) && scores(0);
         for (int i = 0; i < n_blocks && alive; i++) {
+            if (i + 1 < n_blocks && !(alive = scores(i + 1))) break;
             const int st = i % STAGES;
             if (!(alive = wait(v_full0 + 8 * st, i / STAGES))) break;
+            if (i >= nbw) {
+                if (elected) tl_arrive(v_empty0 + 8 * st);
+                continue;
+            }
+            if (!(alive = wait(p_full0 + 8 * w, i))) break;
+            tc_fence_after();
+            if (elected) {
+                const unsigned long long vd = v_desc + (unsigned)st * (2 * TILE >> 4);
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                if (i >= nb[w] || !alive) continue;
-                if (!(alive = wait(p_full0 + 8 * (2 * w + (i & 1)), i >> 1))) continue;
-                tc_fence_after();
-                if (elected) {
-                    const unsigned long long vd = v_desc + (unsigned)st * (2 * TILE >> 4);
-                    const unsigned p_at = tmem + w * TILE_COLS + (i & 1) * S_COLS;
-#pragma unroll
-                    for (int ks = 0; ks < TL_BN / 16; ks++)
-                        mma_bf16_ts(tmem + w * TILE_COLS + O_COL, p_at + ks * 8, vd + ks * (16 * 128 >> 4), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
-                    if (w == (i < nb[1] ? 1 : 0)) mma_commit(v_empty0 + 8 * st);
-                    mma_commit(pv_done0 + 8 * (2 * w + (i & 1)));
-                }
-                if (i + 2 < nb[w]) {
-                    if (!(alive = wait(k_full0 + 8 * ((i + 2) % STAGES), (i + 2) / STAGES))) continue;
-                    tc_fence_after();
-                    issue_s(w, i + 2);
-                }
+                for (int ks = 0; ks < TL_BN / 16; ks++) mma_bf16_ts(o_at, p_at + ks * 8, vd + ks * (16 * 128 >> 4), IDESC_O, (i > 0 || ks > 0) ? 1u : 0u);
+                mma_commit(pv_done0 + 8 * w);
+                mma_commit(v_empty0 + 8 * st);
             }
         }
     } else if (Q8 && warp >= TL_WIDEN_WARP) {
@@ -270,7 +276,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tl_store16(at + (((p + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
             }
         };
-        // in the order in which the products ask: K(0), K(1), V(0), K(2), V(1), ...
+        // in the order in which the products ask for them: K(0), K(1), V(0), K(2), V(1), ...
         auto keys = [&](int i) {
             const int rs = i % TL_RAW, st = i % STAGES, key0 = (jb0 + i) * TL_BN;
             if (!mbar_wait(raw_full0 + 8 * rs, (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL)) return false;
@@ -315,38 +321,53 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 pos = past + i;
             }
         }
-        // the row's query into the swizzled tile; rows behind the last one are zeros
+        const unsigned lane_addr = tmem + ((unsigned)((warp & 3) * 32) << 16), s_addr = lane_addr + S_COL + w * TL_BN, p_addr = lane_addr + P_COL + w * (TL_BN / 2),
+                       o_addr = lane_addr + w * D;
+        // the row's query into tensor memory or, the second tile's, into a swizzled tile of shared memory; rows behind the last one are zeros
         {
             const bf16* src = q + (size_t)token * q_stride + (size_t)h * D;
 #pragma unroll
-            for (int c = 0; c < D / 8; c++) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (valid) v = *reinterpret_cast<const uint4*>(src + c * 8);
-                tl_store16(q_s + w * Z::Q_TILE + (c >> 3) * Q_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+            for (int c0 = 0; c0 < D / 64; c0++) {
+                unsigned x[32];
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (valid) v = *reinterpret_cast<const uint4*>(src + c0 * 64 + c * 8);
+                    x[c * 4] = v.x;
+                    x[c * 4 + 1] = v.y;
+                    x[c * 4 + 2] = v.z;
+                    x[c * 4 + 3] = v.w;
+                }
+                if (w == 0 || BOTH_Q) {
+                    tmem_st32(lane_addr + Q_COL + w * (D / 2) + c0 * 32, x);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) tl_store16(q_s + w * Z::Q_TILE + c0 * Q_ATOM + r * 128 + ((c ^ (r & 7)) << 4), x[c * 4], x[c * 4 + 1], x[c * 4 + 2], x[c * 4 + 3]);
+                }
             }
+            tmem_wait_st();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_fence_before();
             tl_arrive(q_full);
         }
-        const unsigned lane_addr = tmem + w * TILE_COLS + ((unsigned)((warp & 3) * 32) << 16);
         const int nbw = nb[w];
         // what the tile's rows see: everything in blocks between the last row's first key and the first row's last one
         const int tile_first = PREFIX ? last_key : past + (row0 + w * TL_BM) / G, tile_last = PREFIX ? last_key : past + (row0 + min(n_rows, (w + 1) * TL_BM) - 1) / G;
         const int lo_pos = PREFIX ? 0 : nbw > 0 ? first_visible(pos, work.span) : 0, lo_last = PREFIX || nbw == 0 ? 0 : first_visible(tile_last, work.span);
         const float unit = Q8 ? 1.f : scale_log2e;
-        // (pv_done has a barrier for even and one for odd blocks and is waited for only where the output is touched: the scores of block i come behind the
-        // products of block i - 2, so when this thread has them, the phase in question is the next one to end)
         float m_ref = -INFINITY, l_run = 0.f;
         bool alive = true;
         for (int i = 0; i < nbw; i++) {
             const int key0 = (jb0 + i) * TL_BN;
-            alive = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (2 * w + (i & 1)), (i >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+            alive = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * w, i & 1, err, TC_ERR_TIMEOUT_PREFILL));
             if (!alive) break;
             tc_fence_after();
-            const unsigned s_addr = lane_addr + (i & 1) * S_COLS;
             unsigned sr[TL_BN];
             tmem_ld32_issue(s_addr, sr);
             tmem_ld32_issue(s_addr + 32, sr + 32);
             tmem_wait_ld<TL_BN>(sr);
+            tc_fence_before();
+            tl_arrive(s_read0 + 8 * w);
             const unsigned f_at = f_s + (i % TL_RAW) * Z::SCALES;
             if (Q8) {
                 alive = __all_sync(0xffffffffu, mbar_wait(f_full0 + 8 * (i % TL_RAW), (i / TL_RAW) & 1, err, TC_ERR_TIMEOUT_PREFILL));
@@ -376,20 +397,20 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * unit);
             const bool grown = m_new > m_ref + TL_RESCALE_STEP;      // true for m_ref = -inf, m_new finite
+            // the products of the block before: their weights lie where this block's go, and the output may be touched
+            if (i > 0 && !(alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (i - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL)))) break;
             if (__any_sync(0xffffffffu, grown)) {
                 if (i > 0) {
                     const float corr = m_new == -INFINITY ? 1.f : m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_new);
-                    alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (2 * w + ((i - 1) & 1)), ((i - 1) >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
-                    if (!alive) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         unsigned o[32];
-                        tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                        tmem_ld32_issue(o_addr + c0, o);
                         tmem_wait_ld<32>(o);
 #pragma unroll
                         for (int c = 0; c < 32; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-                        tmem_st32(lane_addr + O_COL + c0, o);
+                        tmem_st32(o_addr + c0, o);
                     }
                     tmem_wait_st();
                     l_run *= corr;
@@ -426,7 +447,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 f2_unpack(psb, b0, b1);
                 l_run += (a0 + a1) + (b0 + b1);
             }
-            tmem_st32(s_addr, pr);
+            tmem_st32(p_addr, pr);
             tmem_wait_st();
             if (!Q8 && key0 + TL_BN - 1 > last_key) {
                 // behind the prefix the page may hold anything: those rows of V are cleared (both tiles write the same zeros)
@@ -441,9 +462,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             if (!alive) break;
             tc_fence_before();
-            tl_arrive(p_full0 + 8 * (2 * w + (i & 1)));
+            tl_arrive(p_full0 + 8 * w);
         }
-        if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (2 * w + ((nbw - 1) & 1)), ((nbw - 1) >> 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
+        if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (nbw - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
         const size_t head = (size_t)token * nh + h;
         if (PREFIX) {
             const size_t share = head * work.slots + work.slot0 + blockIdx.x;
@@ -454,7 +475,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     unsigned o[32];
-                    tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                    tmem_ld32_issue(o_addr + c0, o);
                     tmem_wait_ld<32>(o);
                     if (valid)
 #pragma unroll
@@ -470,7 +491,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 unsigned o[32];
-                tmem_ld32_issue(lane_addr + O_COL + c0, o);
+                tmem_ld32_issue(o_addr + c0, o);
                 tmem_wait_ld<32>(o);
                 if (valid)
 #pragma unroll
@@ -487,7 +508,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     __syncthreads();
     if (warp == TL_MMA_WARP) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
 }
 
