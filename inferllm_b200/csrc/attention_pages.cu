@@ -114,7 +114,7 @@ template <int D, bool Q8> struct PgRing {
     static constexpr int STAGES = Q8 ? (D == 128 ? 4 : 6) : 256 / D, BYTES = STAGES * (2 * TILE + SCALES) + 1024;
 };
 
-// grid: (splits, kv heads, prefix tiles and tokens).  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
+// grid: prefix tiles times kv heads times pre_splits, then tokens times kv heads times own_splits.  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
 // a token's own first.  No part_acc: the blocks of a (token, kv head) are a cluster that joins them through shared memory and writes `out`.
 template <int D, bool Q8, int NT>
 __global__ void __launch_bounds__(PG_THREADS)
@@ -143,20 +143,20 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     pdl_grid_sync();
 
     // ---- which rows and keys
-    const int split = blockIdx.x, hk = blockIdx.y, G = nh / nkv, slots = own_splits + pre_splits;
-    const bool prefix = (int)blockIdx.z < plan.n_tiles;
-    const int n_splits = prefix ? pre_splits : own_splits;
-    if (split >= n_splits) return;
+    // the blocks of one (prefix tile or token, kv head) follow one another, then come the other kv heads, whose rows lie in the same pages
+    const int G = nh / nkv, slots = own_splits + pre_splits, own0 = plan.n_tiles * nkv * pre_splits;
+    const bool prefix = (int)blockIdx.x < own0;
+    const int n_splits = prefix ? pre_splits : own_splits, at = (int)blockIdx.x - (prefix ? 0 : own0), split = at % n_splits, hk = at / n_splits % nkv, item = at / n_splits / nkv;
     int t = 0, first = 0, count = 1, p, lo = 0;
     if (prefix) {
-        const int4 tile = plan.tiles[blockIdx.z];
+        const int4 tile = plan.tiles[item];
         first = tile.x;
         count = tile.y;
         p = tile.z - 1;
         if (count <= 0 || p < 0) return;
         t = plan.members[first];
     } else {
-        t = blockIdx.z - plan.n_tiles;
+        t = item;
         p = token_pos[t];
         lo = p < 0 ? 0 : first_visible(p, span);
         if (plan.start) lo = max(lo, plan.start[t]);
@@ -583,9 +583,10 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
     const int smem = PgRing<D, Q8>::BYTES;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    const bool shares = own_splits > PG_MAX_CLUSTER || plan.start;
-    if (!shares) part_acc = part_ml = nullptr;
-    rc = illm_launch_cluster(kern, dim3(own_splits > pre_splits ? own_splits : pre_splits, nkv, plan.n_tiles + T), dim3(PG_THREADS), shares ? 1 : own_splits, smem, s, mk, mv, mk16,
+    const bool shares = part_acc != nullptr;
+    const long long blocks = (long long)nkv * ((long long)plan.n_tiles * pre_splits + (long long)T * own_splits);
+    if (blocks > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;
+    rc = illm_launch_cluster(kern, dim3((unsigned)blocks), dim3(PG_THREADS), shares ? 1 : own_splits, smem, s, mk, mv, mk16,
                              mv16, ksc, vsc, (const bf16*)q, q_stride, block_table, max_pages, (int)n_pages, token_pos, token_seq, plan, part_acc, part_ml, (bf16*)out,
                              own_splits, pre_splits, nh, nkv, page_size, span, scale * 1.4426950408889634f, err);
     if (rc || !shares) return rc;
@@ -597,19 +598,21 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 // Single tokens: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages
 // [n_pages, nkv, page_size, d] of bytes with their scales ksc, vsc, or (ksc, vsc nullptr) of bfloat16; page_size a multiple of 64, d 64
 // or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most 16 rows (members times nh / nkv),
-// are walked here, with n_tiles 0 their shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  own_splits, pre_splits: at most 32 each,
-// pre_splits 0 without a plan.  Scratch with a plan or more than 8 splits: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  err: 7 a wait
-// ran out, 8 a visible position without a page.
+// are walked here, with n_tiles 0 their pre_splits shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  own_splits, pre_splits: at most 32 each,
+// pre_splits 0 without a plan.  Scratch: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2], or, without a plan and with up to 8 splits,
+// nullptr: then the blocks of a (token, kv head) are a cluster and there is no second kernel.  That is the faster way while the blocks find room together (one
+// sequence of 8 kv heads at 1,777 keys 7.3 us and 9), and the slower one where they have to wait for one another's places (64 sequences of 32 kv heads at 300
+// keys in two parts 60 us and 46).  err: 7 a wait ran out, 8 a visible position without a page.
 extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                     const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles,
                                     const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,
                                     int span, float scale, int own_splits, int pre_splits, int* err, void* stream) {
     if (T <= 0) return 0;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || T > 65535 || nkv > 65535 || n_tiles < 0 || n_tiles + T > 65535 || (q_stride & 7) || page_size <= 0 ||
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || T > 65535 || nkv > 65535 || n_tiles < 0 || n_tiles > 65535 || (q_stride & 7) || page_size <= 0 ||
         page_size % PG_BN || max_pages <= 0 || n_pages <= 0 || n_pages * nkv * page_size > 0x7fffffffLL || own_splits < 1 || own_splits > PG_MAX_SPLITS || pre_splits < 0 ||
         pre_splits > PG_MAX_SPLITS || !q || ((uintptr_t)q & 15) || !kc || !vc || ((uintptr_t)kc & 15) || ((uintptr_t)vc & 15) || (!ksc) != (!vsc) || ((uintptr_t)ksc & 15) ||
         ((uintptr_t)vsc & 15) || !err || (plan_start && (span != 0 || pre_splits < 1)) || (!plan_start && (n_tiles > 0 || pre_splits != 0)) ||
-        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || ((own_splits > PG_MAX_CLUSTER || plan_start) && (!part_acc || !part_ml || ((uintptr_t)part_ml & 7))) || !out || !token_pos || !token_seq || !block_table)
+        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || ((own_splits > PG_MAX_CLUSTER || plan_start) && !part_acc) || (!part_acc) != (!part_ml) || ((uintptr_t)part_ml & 7) || !out || !token_pos || !token_seq || !block_table)
         return ILLM_ERR_BAD_ARG;
     const PgPlan plan = {plan_start, reinterpret_cast<const int4*>(plan_tiles), plan_members, n_tiles};
     cudaStream_t s = (cudaStream_t)stream;

@@ -30,6 +30,7 @@
 #define TL_TMA_WARP 10
 #define TL_WIDEN_WARP 11                // the first of four
 #define TL_ERR_PAGE 8
+#define TL_CLUSTER 4                    // parts of a prefix that join their shares: of clusters of eight such blocks only 15 find room, of four 33
 #define TL_RESCALE_STEP 8.0f
 
 // Which rows and keys: prompts (PREFIX false) or the tiles of a plan of common prefixes (attention_pages.cu).
@@ -39,6 +40,7 @@ struct TlWork {
     const int4* tiles;                  // prefixes: first member, number of members, positions, 0
     const int *members, *token_seq;
     int slots, slot0;                   // shares of a (token, head) and the first of them that is the prefix's
+    int cluster;                        // blocks (parts of a prefix) that join their shares
     float *part_acc, *part_ml;
 };
 
@@ -72,6 +74,15 @@ __device__ __forceinline__ void tl_widen(const unsigned (&w)[4], unsigned (&out)
             out[i * 2 + h] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
         }
 }
+// four floats of the same place in another block of the cluster
+__device__ __forceinline__ float4 tl_remote4(unsigned at, unsigned rank) {
+    unsigned a;
+    float4 f;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+    return f;
+}
+__device__ __forceinline__ void tl_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // four floats of shared memory, the same for all lanes
 __device__ __forceinline__ void tl_load4(unsigned at, float* f) {
     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(at));
@@ -90,6 +101,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // columns of tensor memory: outputs, scores, weights, and the queries of the first tile (of both where they fit)
     constexpr unsigned S_COL = 2 * D, P_COL = S_COL + 2 * TL_BN, Q_COL = P_COL + TL_BN, TMEM_COLS = 512;
     constexpr bool BOTH_Q = Q_COL + D <= TMEM_COLS;
+    constexpr int SHARE_ROW = (D + 4) * 4;      // bytes of a row of a prefix's share: accumulators, maximum and sum
+    static_assert(!PREFIX || 2 * TL_BM * SHARE_ROW <= 2 * Z::Q_TILE + STAGES * 2 * TILE + Z::RAW * 2 * Z::RAW_TILE, "the shares must fit the tiles' memory");
     constexpr unsigned IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TL_BN >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     constexpr unsigned IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(D >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -467,23 +480,21 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (alive && nbw > 0) alive = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * w, (nbw - 1) & 1, err, TC_ERR_TIMEOUT_PREFILL));
         const size_t head = (size_t)token * nh + h;
         if (PREFIX) {
-            const size_t share = head * work.slots + work.slot0 + blockIdx.x;
-            if (valid) *reinterpret_cast<float2*>(work.part_ml + share * 2) = nbw > 0 ? make_float2(m_ref, l_run) : make_float2(-INFINITY, 0.f);
-            if (alive && nbw > 0) {
+            // the block's share of a row into shared memory: all products of both tiles have to be through with what lies there
+            asm volatile("bar.sync 1, %0;" ::"n"(TL_SOFTMAX * 32) : "memory");
+            const unsigned dst = base + br * SHARE_ROW;
+            if (nbw > 0) {
                 tc_fence_after();
-                float* dst = work.part_acc + share * D;
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     unsigned o[32];
                     tmem_ld32_issue(o_addr + c0, o);
                     tmem_wait_ld<32>(o);
-                    if (valid)
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4)
-                            *reinterpret_cast<float4*>(dst + c0 + c) =
-                                make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+                    for (int c = 0; c < 32; c += 4) tl_store16(dst + (c0 + c) * 4, o[c], o[c + 1], o[c + 2], o[c + 3]);
                 }
             }
+            tl_store16(dst + D * 4, __float_as_uint(nbw > 0 ? m_ref : -INFINITY), __float_as_uint(nbw > 0 ? l_run : 0.f), 0u, 0u);
         } else if (alive && nbw > 0) {
             tc_fence_after();
             const float inv = 1.0f / l_run;
@@ -506,6 +517,42 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     tc_fence_before();
     __syncthreads();
+    if (PREFIX) {
+        // the cluster's shares of a row (ascending) become one; every block makes a part of the rows, four columns to a thread
+        const int n = work.cluster, rank = (int)blockIdx.x % n;
+        if (n > 1) tl_cluster_sync();
+        for (int idx = rank * (int)blockDim.x + (int)threadIdx.x; idx < n_rows * (D / 4); idx += n * (int)blockDim.x) {
+            const int br = idx / (D / 4), c = idx % (D / 4);
+            const unsigned at = base + br * SHARE_ROW;
+            float4 ml[TL_CLUSTER], v[TL_CLUSTER];
+            float M = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < TL_CLUSTER; k++) {
+                ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+                if (k >= n) continue;
+                ml[k] = tl_remote4(at + D * 4, k);
+                if (ml[k].y != 0.f) v[k] = tl_remote4(at + c * 16, k);
+                M = fmaxf(M, ml[k].x);
+            }
+            const float ref = M == -INFINITY ? 0.f : M;
+            float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+            float den = 0.f;
+#pragma unroll
+            for (int k = 0; k < TL_CLUSTER; k++) {
+                if (ml[k].y == 0.f) continue;                       // no keys; a sum that is no number goes on
+                const float f = ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - ref);
+                num.x += f * v[k].x;
+                num.y += f * v[k].y;
+                num.z += f * v[k].z;
+                num.w += f * v[k].w;
+                den += f * ml[k].y;
+            }
+            const size_t share = ((size_t)work.members[tile.x + br / G] * nh + hk * G + br % G) * work.slots + work.slot0 + blockIdx.x / n;
+            *reinterpret_cast<float4*>(work.part_acc + share * D + c * 4) = num;
+            if (c == 0) *reinterpret_cast<float2*>(work.part_ml + share * 2) = make_float2(M, den);
+        }
+        if (n > 1) tl_cluster_sync();               // the others may still read this block's rows
+    }
     if (warp == TL_MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
@@ -547,9 +594,8 @@ static int tl_launch(dim3 grid, const void* q, int q_stride, const void* kc, con
     const int smem = TlSizes<D, Q8>::SMEM;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    illm_launch(kern, grid, dim3(TlSizes<D, Q8>::THREADS), smem, s, mk, mv, ksc, vsc, (const bf16*)q, q_stride, block_table, max_pages, (int)n_pages, work, (bf16*)out, nh, nkv,
-                page_size, scale * 1.4426950408889634f, err);
-    return illm_launch_status();
+    return illm_launch_cluster(kern, grid, dim3(TlSizes<D, Q8>::THREADS), PREFIX ? work.cluster : 1, smem, s, mk, mv, ksc, vsc, (const bf16*)q, q_stride, block_table, max_pages,
+                               (int)n_pages, work, (bf16*)out, nh, nkv, page_size, scale * 1.4426950408889634f, err);
 }
 
 static bool tl_bad(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, int max_pages, int nh, int nkv, int page_size,
@@ -585,16 +631,19 @@ extern "C" int illm_attention_tiles_int8(const void* q, int q_stride, const void
     return ILLM_ERR_BAD_ARG;
 }
 
-// The shares of common prefixes (ksc, vsc nullptr: bfloat16 pages): for every tile of the plan (at most 256 / (nh / nkv) members) and every one of `splits` parts of its
-// positions, for every (member, head) the accumulators, maximum (in units of log2) and sum at share slot0 + part of `slots`: part_acc float [T, nh, slots, d],
-// part_ml float [T, nh, slots, 2].  illm_attention_pages_join adds them up with the others.
+// Parts of a prefix that are joined before they leave: up to four, whole clusters.
+extern "C" int illm_attention_tiles_cluster(int splits) { return splits < TL_CLUSTER ? (splits < 1 ? 1 : splits) : splits % TL_CLUSTER == 0 ? TL_CLUSTER : splits % 2 == 0 ? 2 : 1; }
+
+// The shares of common prefixes (ksc, vsc nullptr: bfloat16 pages): for every tile of the plan (at most 256 / (nh / nkv) members), whose positions are cut into `splits` parts,
+// of which every c = illm_attention_tiles_cluster(splits) are joined: for every (member, head) accumulators, maximum (in units of log2) and sum at share slot0 + part / c of
+// `slots`: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  illm_attention_pages adds them up with a token's own.
 extern "C" int illm_attention_tiles_prefix(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                            const int* block_table, int max_pages, const int* token_seq, const int* plan_tiles, const int* plan_members, int n_tiles,
                                            float* part_acc, float* part_ml, int nh, int nkv, int d, int page_size, float scale, int slots, int slot0, int splits, int* err,
                                            void* stream) {
     if (n_tiles <= 0) return 0;
-    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || nh / nkv > 2 * TL_BM || n_tiles > 65535 || splits < 1 || splits > 65535 || slot0 < 0 ||
-        slot0 + splits > slots || !part_acc || !part_ml || ((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || !plan_tiles || ((uintptr_t)plan_tiles & 15) || !plan_members)
+    if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || nh / nkv > 2 * TL_BM || n_tiles > 65535 || splits < 1 || splits > 256 ||
+        slot0 < 0 || slot0 + splits / illm_attention_tiles_cluster(splits) > slots || !part_acc || !part_ml || ((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || !plan_tiles || ((uintptr_t)plan_tiles & 15) || !plan_members)
         return ILLM_ERR_BAD_ARG;
     TlWork work = {};
     work.tiles = reinterpret_cast<const int4*>(plan_tiles);
@@ -602,6 +651,7 @@ extern "C" int illm_attention_tiles_prefix(const void* q, int q_stride, const vo
     work.token_seq = token_seq;
     work.slots = slots;
     work.slot0 = slot0;
+    work.cluster = illm_attention_tiles_cluster(splits);
     work.part_acc = part_acc;
     work.part_ml = part_ml;
     const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)n_tiles);

@@ -49,6 +49,7 @@ int illm_attention_pages(const void* q, int q_stride, const void* kc, const void
 
 // attention_tiles.cu
 int illm_attention_tiles_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d, int page_size, int span, float scale, int tile_rows, int* err, void* stream);
+int illm_attention_tiles_cluster(int splits);
 int illm_attention_tiles_prefix(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* token_seq, const int* plan_tiles, const int* plan_members, int n_tiles, float* part_acc, float* part_ml, int nh, int nkv, int d, int page_size, float scale, int slots, int slot0, int splits, int* err, void* stream);
 
 // attention_prefill.cu

@@ -119,12 +119,20 @@ int attention_decode_ring_splits(long long T, int n_kv_heads, long long max_len,
 }
 
 int attention_pages_splits(long long pairs, long long keys, int n_sms) {
-    const long long most = std::min<long long>(kRingDecodeMaxSplits, std::max<long long>(1, ceil_div(keys, 128)));
-    return (int)std::max<long long>(1, std::min<long long>(most, 2LL * n_sms / std::max<long long>(1, pairs)));
+    const long long tiles = std::max<long long>(1, ceil_div(keys, 64)), slots = 3LL * n_sms;
+    pairs = std::max<long long>(1, pairs);
+    long long n;
+    if (pairs >= slots) n = keys >= 4096 ? 4 : keys >= 2048 ? 2 : 1;
+    else n = std::min(ceil_div(2 * slots, pairs), std::max<long long>(1, ceil_div(keys, 512)));
+    // few blocks: a cluster's worth of them, more where every one still has eight tiles
+    if (pairs * 8 <= 2LL * n_sms) n = keys <= 3000 ? 8 : std::min<long long>(32, std::max<long long>(8, keys / 512));
+    return (int)std::max<long long>(1, std::min<long long>({n, tiles, (long long)kRingDecodeMaxSplits}));
 }
 int attention_prefix_splits(long long pairs, long long keys, int n_sms) {
     const long long most = std::min<long long>(kRingDecodeMaxSplits, std::max<long long>(1, ceil_div(keys, 128)));
-    return (int)std::max<long long>(1, std::min<long long>(most, (long long)n_sms / std::max<long long>(1, pairs)));
+    // (clusters of four blocks, each alone on its SM, fill seven eighths of the SMs)
+    const long long n = std::max<long long>(1, std::min<long long>(most, n_sms * 7LL / 8 / std::max<long long>(1, pairs)));
+    return (int)(n > 4 ? n / 4 * 4 : n);
 }
 bool attention_int8_tc_supported(DType dtype, int nh, int nkv, int d, int page_size, bool decode) {
     return dtype == DType::BF16 && nkv > 0 && nh % nkv == 0 && (d == 64 || d == 128) && page_size > 0 && page_size % 64 == 0 && (!decode || nh / nkv <= 16);

@@ -67,6 +67,7 @@ _KERNEL_SIGNATURES = {
     "illm_attention_int8": [P_, I_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, P_, P_],
     "illm_attention_pages": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, F_, I_, I_, P_, P_],
     "illm_attention_tiles_int8": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, I_, P_, P_],
+    "illm_attention_tiles_cluster": [I_],
     "illm_attention_tiles_prefix": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, P_, P_, I_, I_, I_, I_, F_, I_, I_, I_, P_, P_],
     "illm_attention_prefill": [P_, I_, P_, P_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, P_],
     "illm_gemm_bf16_tc": [P_, P_, P_, I_, I_, I_, I_, P_, I_, P_, P_, I_],
@@ -1103,7 +1104,12 @@ def pages_splits(pairs, keys, wide, n_sms) -> int:
     return int(_b.lib().illm_policy_pages_splits(int(pairs), int(keys), int(wide), int(n_sms)))
 
 
-MAX_CLUSTER_SPLITS = 8      # of attention_pages: more of them leave their shares in memory
+MAX_CLUSTER_SPLITS = 8
+
+
+def _in_cluster(pairs, splits, device):
+    """Whether the blocks of a (token, kv head) join their shares in a cluster (the engine's rule): where all blocks find room at once."""
+    return splits <= MAX_CLUSTER_SPLITS and pairs * splits <= 2 * _sms[device.index]
 
 
 def _shares(T, n_heads, slots, d, device):
@@ -1136,8 +1142,9 @@ def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, 
         run, keys, err, stream = load().illm_attention_pages, min(max_len, abs(span)) if span else max_len, _error_word(device), _stream()
         for t0 in range(0, T, 65535):
             n = min(T - t0, 65535)
-            s = _splits(n * nkv, keys, False, device) if splits is None else int(splits)
-            ws, acc, ml = _shares(n, n_heads, s, d, device) if s > MAX_CLUSTER_SPLITS else (None, None, None)
+            s = _splits(n * nkv, keys, False, device)
+            s = s if splits is None else int(splits)
+            ws, acc, ml = (None, None, None) if s == 1 or _in_cluster(n * nkv, s, device) else _shares(n, n_heads, s, d, device)
             _check(run(q.data_ptr() + t0 * stride * 2, stride, *cache.pointers, cache.pages, block_table.data_ptr(), width, token_pos.data_ptr() + 4 * t0,
                        token_seq.data_ptr() + 4 * t0, None, None, None, 0, acc, ml, out.data_ptr() + t0 * n_heads * d * 2, n, n_heads, nkv, d, cache.page_size, span,
                        float(scale), s, 0, err, stream), "attention_decode_int8")
@@ -1215,15 +1222,16 @@ def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n
         common = plan.tiles > 0
         own = _splits(T * nkv, max(1, plan.longest_rest), False, device) if own_splits is None else int(own_splits)
         pre = (_splits(plan.tiles * nkv, plan.longest_prefix, plan.wide, device) if pre_splits is None else int(pre_splits)) if common else 0
-        ws, acc, ml = _shares(T, n_heads, own + pre, d, device) if common or own > MAX_CLUSTER_SPLITS else (None, None, None)
+        kept = pre // load().illm_attention_tiles_cluster(pre) if plan.wide and pre > 0 else pre           # shares of the prefixes that are left in memory
+        ws, acc, ml = _shares(T, n_heads, own + kept, d, device) if common or own > 1 else (None, None, None)
         start, tiles, members = plan.pointers if common else (None, None, None)
         h, err, stream = load(), _error_word(device), _stream()
         at, table, pos, seq = q.data_ptr(), block_table.data_ptr(), token_pos.data_ptr(), token_seq.data_ptr()
         if common and plan.wide:
             _check(h.illm_attention_tiles_prefix(at, stride, *pointers, pages, table, width, seq, tiles, members, plan.tiles, acc, ml, n_heads, nkv, d, page_size,
-                                                 float(scale), own + pre, own, pre, err, stream), "attention_decode_shared")
+                                                 float(scale), own + kept, own, pre, err, stream), "attention_decode_shared")
         _check(h.illm_attention_pages(at, stride, *pointers, pages, table, width, pos, seq, start, tiles, members, 0 if plan.wide else plan.tiles, acc, ml,
-                                      out.data_ptr(), T, n_heads, nkv, d, page_size, 0, float(scale), own, pre, err, stream), "attention_decode_shared")
+                                      out.data_ptr(), T, n_heads, nkv, d, page_size, 0, float(scale), own, kept, err, stream), "attention_decode_shared")
     return out
 
 
