@@ -108,22 +108,24 @@ struct PgPlan {
     int n_tiles;
 };
 
-// stages that leave two blocks to an SM
-template <int D, bool Q8> struct PgRing {
+// Stages: as many as leave four blocks to an SM (five at head size 64, three of bfloat16 rows), or with sixteen rows, whose registers leave two blocks, more.  The blocks
+// are short (one takes a few tiles after it has waited for its first), so that more of them are worth more than deeper rings: 64 sequences of 32 kv heads at
+// 300 keys 37.8 us with two blocks of six stages, 31.7 with three of four, 28.0 with four of three.
+template <int D, bool Q8, int NT> struct PgRing {
     static constexpr int TILE = PG_BN * D * (Q8 ? 1 : 2), SCALES = Q8 ? 2 * PG_BN * 4 : 0;
-    static constexpr int STAGES = Q8 ? (D == 128 ? 4 : 6) : 256 / D, BYTES = STAGES * (2 * TILE + SCALES) + 1024;
+    static constexpr int STAGES = !Q8 ? 256 / D : NT == 1 ? (D == 128 ? 3 : 4) : (D == 128 ? 4 : 6), BYTES = STAGES * (2 * TILE + SCALES) + 1024;
 };
 
 // grid: prefix tiles times kv heads times pre_splits, then tokens times kv heads times own_splits.  Shares: part_acc [T, nh, slots, D], part_ml [T, nh, slots, 2] with slots = own_splits + pre_splits,
 // a token's own first.  No part_acc: the blocks of a (token, kv head) are a cluster that joins them through shared memory and writes `out`.
 template <int D, bool Q8, int NT>
-__global__ void __launch_bounds__(PG_THREADS)
+__global__ void __launch_bounds__(PG_THREADS, NT == 2 ? 2 : Q8 ? 4 : 3)
 attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
                        const __grid_constant__ CUtensorMap map_v16, const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ q,
                        int q_stride, const int* __restrict__ block_table, int max_pages, int n_pages, const int* __restrict__ token_pos,
                        const int* __restrict__ token_seq, const PgPlan plan, float* __restrict__ part_acc, float* __restrict__ part_ml, bf16* __restrict__ out,
                        int own_splits, int pre_splits, int nh, int nkv, int page_size, int span, float scale_log2e, int* __restrict__ err) {
-    using R = PgRing<D, Q8>;
+    using R = PgRing<D, Q8, NT>;
     constexpr int KS = D / 16, STAGES = R::STAGES, TILE = R::TILE;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * STAGES];
@@ -579,8 +581,9 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
         (rc = pg_make_map(&mv16, vc, rows, D, 16, Q8)))
         return rc;
     // eight rows in a block's products where no block has more
-    auto kern = plan.n_tiles == 0 && nh / nkv <= 8 ? attention_pages_kernel<D, Q8, 1> : attention_pages_kernel<D, Q8, 2>;
-    const int smem = PgRing<D, Q8>::BYTES;
+    const bool eight = plan.n_tiles == 0 && nh / nkv <= 8;
+    auto kern = eight ? attention_pages_kernel<D, Q8, 1> : attention_pages_kernel<D, Q8, 2>;
+    const int smem = eight ? PgRing<D, Q8, 1>::BYTES : PgRing<D, Q8, 2>::BYTES;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     const bool shares = part_acc != nullptr;

@@ -19,22 +19,44 @@
 #define KQ_THREADS 256
 #define KQ_TINY 7.888609e-31f       // 2^-100
 
-// channels 8c .. 8c+7 of a row of d values that starts at element `row` of the projection (or the sum of its K slices)
-template <typename TA, bool PARTIALS>
-__device__ __forceinline__ void kq_fetch(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at, float* f) {
-    if (!PARTIALS) {
-        load8(x + at, f);
-        return;
-    }
+// eight channels as they lie in memory, and as numbers
+template <typename TA, bool PARTIALS> struct KqPiece {
+    uint4 v[PARTIALS ? 2 : sizeof(TA) / 2];
+    // from element `at` of the projection, or the sum of its K slices there
+    __device__ __forceinline__ void fetch(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
+        if (!PARTIALS) {
 #pragma unroll
-    for (int k = 0; k < 8; k++) f[k] = 0.f;
-    for (int z = 0; z < splits; z++) {
-        float p[8];
-        load8(partials + (size_t)z * stride + at, p);
+            for (int i = 0; i < (int)(sizeof(TA) / 2); i++) v[i] = reinterpret_cast<const uint4*>(x + at)[i];
+            return;
+        }
+        float f[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) f[k] += p[k];
+        for (int k = 0; k < 8; k++) f[k] = 0.f;
+        for (int z = 0; z < splits; z++) {
+            float p[8];
+            load8(partials + (size_t)z * stride + at, p);
+#pragma unroll
+            for (int k = 0; k < 8; k++) f[k] += p[k];
+        }
+        v[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        v[PARTIALS ? 1 : 0] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
     }
-}
+    __device__ __forceinline__ void numbers(float* f) const {
+        if (PARTIALS || sizeof(TA) == 4) {
+            const uint4 b = v[PARTIALS || sizeof(TA) == 4 ? 1 : 0];
+            const unsigned u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; k++) f[k] = __uint_as_float(u[k]);
+        } else {
+            const unsigned u[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                f[2 * k] = __uint_as_float(u[k] << 16);
+                f[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+            }
+        }
+    }
+};
 template <typename TA, bool PARTIALS>
 __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
     if (!PARTIALS) return to_f32(x[at]);
@@ -44,14 +66,15 @@ __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float
 }
 
 // LANES: lanes of a row.  WIDE: the rotated halves are whole pieces of eight channels (rot a multiple of 16); otherwise a thread
-// fetches its channels' partners one by one.  A block takes `per_block` heads of one token.
-template <typename TA, bool PARTIALS, bool WIDE, int LANES>
+// fetches its channels' partners one by one.  A block takes ROUNDS times KQ_THREADS / LANES heads of one token, a thread's loads of all its rounds in flight
+// together (4,096 tokens of 32 + 16 heads of 128, 92 MB: with one round's loads at a time 32 us).
+template <typename TA, bool PARTIALS, bool WIDE, int LANES, int ROUNDS>
 __global__ void __launch_bounds__(KQ_THREADS)
 kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ partials, int splits, long long split_stride, TA* __restrict__ q_out,
                      const float2* __restrict__ cs, const int* __restrict__ token_pos, const int* __restrict__ token_seq,
                      const int* __restrict__ block_table, int max_pages, int n_pages, unsigned char* __restrict__ kc, unsigned char* __restrict__ vc,
                      float* __restrict__ ksc, float* __restrict__ vsc, int nh, int nkv, int d, int rot, int page_size, int write_kv,
-                     int table_positions, int per_block, int* __restrict__ err) {
+                     int table_positions, int* __restrict__ err) {
     pdl_grid_sync();
     const int t = blockIdx.x, c = threadIdx.x & (LANES - 1), half = rot >> 1, n_slots = nh + 2 * nkv;
     const bool active = c * 8 < d;
@@ -80,29 +103,42 @@ kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ parti
             turn[k + 1] = make_float2(v.z, v.w);
         }
     }
-    const int s0 = blockIdx.y * per_block + threadIdx.x / LANES, s1 = min(n_slots, (int)(blockIdx.y + 1) * per_block);
-    // (the lanes of a row run together: s0 is the same for all of them, and shuffles stay within the row)
+    // (the lanes of a row run together: its slot is the same for all of them, and shuffles stay within the row)
     const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) & ~(LANES - 1));
-    for (int slot = s0; slot < s1; slot += KQ_THREADS / LANES) {
+    constexpr int AT_ONCE = KQ_THREADS / LANES;
+    const int s0 = blockIdx.y * (AT_ONCE * ROUNDS) + threadIdx.x / LANES;
+    const int s1 = page < 0 ? nh : n_slots;         // queries come first
+    KqPiece<TA, PARTIALS> own[ROUNDS], other[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        const int slot = s0 + i * AT_ONCE;
+        if (slot >= s1 || !active) continue;
+        const size_t at = ((size_t)t * n_slots + slot) * d;
+        own[i].fetch(qkv, partials, splits, split_stride, at + c * 8);
+        if (WIDE && turned && slot < nh + nkv) other[i].fetch(qkv, partials, splits, split_stride, at + (c < hc ? c + hc : c - hc) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        const int slot = s0 + i * AT_ONCE;
+        if (slot >= s1) break;
         const bool is_q = slot < nh, is_k = !is_q && slot < nh + nkv;
-        if (!is_q && page < 0) break;           // queries come first
         const size_t at = ((size_t)t * n_slots + slot) * d;
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (active) kq_fetch<TA, PARTIALS>(qkv, partials, splits, split_stride, at + c * 8, x);
+        if (active) own[i].numbers(x);
         if (turned && (is_q || is_k)) {
             if (WIDE) {
                 float y[8];
-                kq_fetch<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (c < hc ? c + hc : c - hc) * 8, y);
+                other[i].numbers(y);
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] = c < hc ? x[k] * turn[k].x - y[k] * turn[k].y : y[k] * turn[k].y + x[k] * turn[k].x;
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const int i = c * 8 + k, j = i < half ? i : i - half;
-                    if (i >= rot) continue;
+                    const int ch = c * 8 + k, j = ch < half ? ch : ch - half;
+                    if (ch >= rot) continue;
                     const float2 w = cs[(size_t)p * half + j];
-                    const float y = kq_fetch1<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (i < half ? i + half : j));
-                    x[k] = i < half ? x[k] * w.x - y * w.y : y * w.y + x[k] * w.x;
+                    const float y = kq_fetch1<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (ch < half ? ch + half : j));
+                    x[k] = ch < half ? x[k] * w.x - y * w.y : y * w.y + x[k] * w.x;
                 }
             }
         }
@@ -176,32 +212,41 @@ extern "C" int illm_kv_write_int8(const void* qkv, const float* partials, int sp
     const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, at_once = KQ_THREADS / lanes;
     const int n_slots = nh + (write_kv ? 2 * nkv : 0), rounds_all = (n_slots + at_once - 1) / at_once;
     // several heads to a thread once that leaves eight blocks to every SM
+    const bool wide = (rot & 15) == 0;
     int rounds = 1;
-    while (rounds < rounds_all && (long long)T * ((rounds_all + rounds) / (rounds + 1)) >= 8LL * illm_sm_count()) rounds++;
+    if (wide && !partials)
+        while (rounds < 4 && rounds < rounds_all && (long long)T * ((rounds_all + rounds) / (rounds + 1)) >= 8LL * illm_sm_count()) rounds++;
     const dim3 grid((unsigned)T, (unsigned)((rounds_all + rounds - 1) / rounds));
     if (grid.y > 65535) return ILLM_ERR_BAD_ARG;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool wide = (rot & 15) == 0;
-#define KQ_RUN(TA, PART, W, L)                                                                                                                  \
-    illm_launch(kv_write_int8_kernel<TA, PART, W, L>, grid, dim3(KQ_THREADS), 0, s, (const TA*)qkv, partials, splits, split_stride, (TA*)q_out, \
+#define KQ_RUN(TA, PART, W, L, N)                                                                                                               \
+    illm_launch(kv_write_int8_kernel<TA, PART, W, L, N>, grid, dim3(KQ_THREADS), 0, s, (const TA*)qkv, partials, splits, split_stride, (TA*)q_out, \
                 (const float2*)cos_sin, token_pos, token_seq, block_table, max_pages, (int)n_pages, (unsigned char*)kc, (unsigned char*)vc, ksc, vsc, nh, \
-                nkv, d, rot, page_size, write_kv, table_positions, rounds * at_once, err)
-#define KQ_LANES(TA, PART, W)                  \
-    do {                                       \
-        if (lanes == 8) KQ_RUN(TA, PART, W, 8); \
-        else if (lanes == 16) KQ_RUN(TA, PART, W, 16); \
-        else KQ_RUN(TA, PART, W, 32);          \
+                nkv, d, rot, page_size, write_kv, table_positions, err)
+#define KQ_LANES(TA, PART, W, N)                       \
+    do {                                               \
+        if (lanes == 8) KQ_RUN(TA, PART, W, 8, N);     \
+        else if (lanes == 16) KQ_RUN(TA, PART, W, 16, N); \
+        else KQ_RUN(TA, PART, W, 32, N);               \
     } while (0)
-#define KQ_WIDE(TA, PART)                  \
-    do {                                   \
-        if (wide) KQ_LANES(TA, PART, true); \
-        else KQ_LANES(TA, PART, false);    \
+#define KQ_ROUNDS(TA)                                  \
+    do {                                               \
+        if (!wide) KQ_LANES(TA, false, false, 1);      \
+        else if (rounds == 1) KQ_LANES(TA, false, true, 1); \
+        else if (rounds == 2) KQ_LANES(TA, false, true, 2); \
+        else if (rounds == 3) KQ_LANES(TA, false, true, 3); \
+        else KQ_LANES(TA, false, true, 4);             \
     } while (0)
-    if (act_dtype == ILLM_BF16 && partials) KQ_WIDE(bf16, true);
-    else if (act_dtype == ILLM_BF16) KQ_WIDE(bf16, false);
-    else if (partials) return ILLM_ERR_BAD_ARG;
-    else KQ_WIDE(float, false);
-#undef KQ_WIDE
+    if (partials) {
+        if (act_dtype != ILLM_BF16) return ILLM_ERR_BAD_ARG;
+        if (wide) KQ_LANES(bf16, true, true, 1);
+        else KQ_LANES(bf16, true, false, 1);
+    } else if (act_dtype == ILLM_BF16) {
+        KQ_ROUNDS(bf16);
+    } else {
+        KQ_ROUNDS(float);
+    }
+#undef KQ_ROUNDS
 #undef KQ_LANES
 #undef KQ_RUN
     return illm_launch_status();
