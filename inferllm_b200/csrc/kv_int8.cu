@@ -13,50 +13,42 @@
 // activations' type, in a matrix of their own.
 // Memory bounds it: a projection row is read once, 1 + 4 / d bytes per element are written.  A row belongs to the fewest lanes
 // (8, 16 or 32) that hold it with eight channels each, so that the maximum is a few shuffles, and a thread keeps its channels'
-// cos and sin for several heads of its token.
+// cos and sin for up to four heads of its token, whose loads are in flight together.
 #include "common.cuh"
 
 #define KQ_THREADS 256
 #define KQ_TINY 7.888609e-31f       // 2^-100
 
-// eight channels as they lie in memory, and as numbers
-template <typename TA, bool PARTIALS> struct KqPiece {
-    uint4 v[PARTIALS ? 2 : sizeof(TA) / 2];
-    // from element `at` of the projection, or the sum of its K slices there
-    __device__ __forceinline__ void fetch(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
-        if (!PARTIALS) {
-#pragma unroll
-            for (int i = 0; i < (int)(sizeof(TA) / 2); i++) v[i] = reinterpret_cast<const uint4*>(x + at)[i];
-            return;
-        }
-        float f[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) f[k] = 0.f;
+// Four neighbouring channels, as they lie in memory and as numbers.
+__device__ __forceinline__ void kq_numbers(uint2 u, float* f) {
+    f[0] = __uint_as_float(u.x << 16);
+    f[1] = __uint_as_float(u.x & 0xffff0000u);
+    f[2] = __uint_as_float(u.y << 16);
+    f[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+__device__ __forceinline__ void kq_numbers(float4 u, float* f) { f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w; }
+__device__ __forceinline__ void kq_store4(bf16* p, const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+__device__ __forceinline__ void kq_store4(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+template <typename TA, bool PARTIALS> struct KqFour { using Raw = float4; };
+template <> struct KqFour<bf16, false> { using Raw = uint2; };
+
+// of the projection at element `at`, or the sum of its K slices there
+template <typename TA, bool PARTIALS>
+__device__ __forceinline__ typename KqFour<TA, PARTIALS>::Raw kq_fetch4(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
+    if constexpr (!PARTIALS) {
+        return *reinterpret_cast<const typename KqFour<TA, PARTIALS>::Raw*>(x + at);
+    } else {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int z = 0; z < splits; z++) {
-            float p[8];
-            load8(partials + (size_t)z * stride + at, p);
-#pragma unroll
-            for (int k = 0; k < 8; k++) f[k] += p[k];
+            const float4 p = *reinterpret_cast<const float4*>(partials + (size_t)z * stride + at);
+            f.x += p.x, f.y += p.y, f.z += p.z, f.w += p.w;
         }
-        v[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-        v[PARTIALS ? 1 : 0] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+        return f;
     }
-    __device__ __forceinline__ void numbers(float* f) const {
-        if (PARTIALS || sizeof(TA) == 4) {
-            const uint4 b = v[PARTIALS || sizeof(TA) == 4 ? 1 : 0];
-            const unsigned u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int k = 0; k < 8; k++) f[k] = __uint_as_float(u[k]);
-        } else {
-            const unsigned u[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                f[2 * k] = __uint_as_float(u[k] << 16);
-                f[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-            }
-        }
-    }
-};
+}
 template <typename TA, bool PARTIALS>
 __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float* __restrict__ partials, int splits, long long stride, size_t at) {
     if (!PARTIALS) return to_f32(x[at]);
@@ -65,85 +57,88 @@ __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float
     return f;
 }
 
-// LANES: lanes of a row.  WIDE: the rotated halves are whole pieces of eight channels (rot a multiple of 16); otherwise a thread
-// fetches its channels' partners one by one.  A block takes ROUNDS times KQ_THREADS / LANES heads of one token, a thread's loads of all its rounds in flight
-// together (4,096 tokens of 32 + 16 heads of 128, 92 MB: with one round's loads at a time 32 us).
+// LANES: lanes of a row, eight channels each.  WIDE (rot a multiple of 8): a lane of the rotated part has four channels and the four that they are turned with, so
+// that it needs no other lane's and each of its cosines once (with eight neighbours a lane, and their partners fetched beside them, 4,096 tokens of 32 + 16
+// heads of 128 took 27 us).  Otherwise it has eight neighbours and fetches their partners one by one.  A block takes ROUNDS times
+// KQ_THREADS / LANES heads of one token.
 template <typename TA, bool PARTIALS, bool WIDE, int LANES, int ROUNDS>
-__global__ void __launch_bounds__(KQ_THREADS)
+__global__ void __launch_bounds__(KQ_THREADS, WIDE && !PARTIALS && sizeof(TA) == 2 ? 5 : 4)
 kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ partials, int splits, long long split_stride, TA* __restrict__ q_out,
                      const float2* __restrict__ cs, const int* __restrict__ token_pos, const int* __restrict__ token_seq,
                      const int* __restrict__ block_table, int max_pages, int n_pages, unsigned char* __restrict__ kc, unsigned char* __restrict__ vc,
                      float* __restrict__ ksc, float* __restrict__ vsc, int nh, int nkv, int d, int rot, int page_size, int write_kv,
                      int table_positions, int* __restrict__ err) {
     pdl_grid_sync();
+    constexpr int AT_ONCE = KQ_THREADS / LANES;
     const int t = blockIdx.x, c = threadIdx.x & (LANES - 1), half = rot >> 1, n_slots = nh + 2 * nkv;
-    const bool active = c * 8 < d;
+    const bool active = c * 8 < d, turned = c * 8 < rot;
+    const int ch0 = WIDE && turned ? c * 4 : c * 8, ch1 = WIDE && turned ? half + c * 4 : c * 8 + 4;
+    // (the lanes of a row run together: its slot is the same for all of them, and shuffles stay within the row)
+    const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) & ~(LANES - 1));
+    const int s0 = blockIdx.y * (AT_ONCE * ROUNDS) + threadIdx.x / LANES, all = write_kv ? n_slots : nh;
+    const size_t row0 = ((size_t)t * n_slots + s0) * d;
+    // the rows first: where they go is looked up behind their loads
+    typename KqFour<TA, PARTIALS>::Raw raw[ROUNDS][2];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        raw[i][0] = raw[i][1] = {};
+        if (s0 + i * AT_ONCE >= all || !active) continue;
+        raw[i][0] = kq_fetch4<TA, PARTIALS>(qkv, partials, splits, split_stride, row0 + i * (AT_ONCE * d) + ch0);
+        raw[i][1] = kq_fetch4<TA, PARTIALS>(qkv, partials, splits, split_stride, row0 + i * (AT_ONCE * d) + ch1);
+    }
     const int p = token_pos[t];
     if (p < 0 || (half > 0 && p >= table_positions)) {
         if (threadIdx.x == 0) atomicExch(err, 3);
         return;
     }
     int page = -1;
+    const int logical = (int)((unsigned)p / (unsigned)page_size), offset = p - logical * page_size;
     if (write_kv) {
-        if (p / page_size < max_pages) page = block_table[(size_t)token_seq[t] * max_pages + p / page_size];
+        if (logical < max_pages) page = block_table[(size_t)token_seq[t] * max_pages + logical];
         if (page < 0 || page >= n_pages) {
             if (threadIdx.x == 0) atomicExch(err, 2);
             page = -1;
         }
     }
-    const int hc = half >> 3;                   // WIDE: pieces of a rotated half
-    const bool turned = active && c * 8 < rot;
-    float2 turn[8];
+    const int end = page < 0 ? nh : n_slots;         // queries come first
+    float2 turn[4];
     if (WIDE && turned) {
-        const float2* row = cs + (size_t)p * half + (c < hc ? c : c - hc) * 8;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-            const float4 v = *reinterpret_cast<const float4*>(row + k);
-            turn[k] = make_float2(v.x, v.y);
-            turn[k + 1] = make_float2(v.z, v.w);
-        }
-    }
-    // (the lanes of a row run together: its slot is the same for all of them, and shuffles stay within the row)
-    const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << ((threadIdx.x & 31) & ~(LANES - 1));
-    constexpr int AT_ONCE = KQ_THREADS / LANES;
-    const int s0 = blockIdx.y * (AT_ONCE * ROUNDS) + threadIdx.x / LANES;
-    const int s1 = page < 0 ? nh : n_slots;         // queries come first
-    KqPiece<TA, PARTIALS> own[ROUNDS], other[ROUNDS];
-#pragma unroll
-    for (int i = 0; i < ROUNDS; i++) {
-        const int slot = s0 + i * AT_ONCE;
-        if (slot >= s1 || !active) continue;
-        const size_t at = ((size_t)t * n_slots + slot) * d;
-        own[i].fetch(qkv, partials, splits, split_stride, at + c * 8);
-        if (WIDE && turned && slot < nh + nkv) other[i].fetch(qkv, partials, splits, split_stride, at + (c < hc ? c + hc : c - hc) * 8);
+        const float4 v0 = *reinterpret_cast<const float4*>(cs + (size_t)p * half + c * 4), v1 = *reinterpret_cast<const float4*>(cs + (size_t)p * half + c * 4 + 2);
+        turn[0] = make_float2(v0.x, v0.y), turn[1] = make_float2(v0.z, v0.w), turn[2] = make_float2(v1.x, v1.y), turn[3] = make_float2(v1.z, v1.w);
     }
 #pragma unroll
     for (int i = 0; i < ROUNDS; i++) {
         const int slot = s0 + i * AT_ONCE;
-        if (slot >= s1) break;
+        if (slot >= end) break;
         const bool is_q = slot < nh, is_k = !is_q && slot < nh + nkv;
-        const size_t at = ((size_t)t * n_slots + slot) * d;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (active) own[i].numbers(x);
+        float x[8];
+        kq_numbers(raw[i][0], x);
+        kq_numbers(raw[i][1], x + 4);
         if (turned && (is_q || is_k)) {
             if (WIDE) {
-                float y[8];
-                other[i].numbers(y);
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = c < hc ? x[k] * turn[k].x - y[k] * turn[k].y : y[k] * turn[k].y + x[k] * turn[k].x;
+                for (int k = 0; k < 4; k++) {
+                    const float a = x[k], b = x[k + 4];
+                    x[k] = a * turn[k].x - b * turn[k].y;
+                    x[k + 4] = a * turn[k].y + b * turn[k].x;
+                }
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const int ch = c * 8 + k, j = ch < half ? ch : ch - half;
                     if (ch >= rot) continue;
                     const float2 w = cs[(size_t)p * half + j];
-                    const float y = kq_fetch1<TA, PARTIALS>(qkv, partials, splits, split_stride, at + (ch < half ? ch + half : j));
+                    const float y = kq_fetch1<TA, PARTIALS>(qkv, partials, splits, split_stride, row0 + i * (AT_ONCE * d) + (ch < half ? ch + half : j));
                     x[k] = ch < half ? x[k] * w.x - y * w.y : y * w.y + x[k] * w.x;
                 }
             }
         }
         if (is_q) {
-            if (active) store8(q_out + ((size_t)t * nh + slot) * d + c * 8, x);
+            TA* to = q_out + ((size_t)t * nh + slot) * d;
+            if (active) {
+                kq_store4(to + ch0, x);
+                kq_store4(to + ch1, x + 4);
+            }
             continue;
         }
         // the largest magnitude as bits: unsigned order is that of the values, with infinities and then NaNs above them
@@ -156,13 +151,19 @@ kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ parti
         const bool finite = top < 0x7f800000u, tiny = finite && a < KQ_TINY;
         const float scale = !finite ? __uint_as_float(0x7fffffffu) : tiny ? 0.f : a / 127.f, inv = !finite || tiny ? 0.f : 127.f / a;
         const int hk = is_k ? slot - nh : slot - nh - nkv;
-        const size_t row = ((size_t)page * nkv + hk) * page_size + p % page_size;
+        const size_t row = ((size_t)page * nkv + hk) * page_size + offset;
+        // u = 128 + round(x / s): added to 1.5 x 2^23 + 128 in one rounding the quotient, at most 127 and a little, is the lowest byte of the sum
         unsigned u[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) u[k] = finite ? (unsigned)(128 + min(127, max(-127, __float2int_rn(x[k] * inv)))) : 128u;
-        if (active)
-            *reinterpret_cast<uint2*>((is_k ? kc : vc) + row * d + c * 8) =
-                make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24, u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
+        for (int k = 0; k < 8; k++) u[k] = __float_as_uint(fmaf(x[k], inv, 12583040.f));
+        unsigned lo = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+        unsigned hi = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
+        if (!finite) lo = hi = 0x80808080u;
+        if (active) {
+            unsigned char* to = (is_k ? kc : vc) + row * d;
+            *reinterpret_cast<unsigned*>(to + ch0) = lo;
+            *reinterpret_cast<unsigned*>(to + ch1) = hi;
+        }
         if (c == 0) (is_k ? ksc : vsc)[row] = scale;
     }
 }
@@ -174,15 +175,15 @@ kv_read_int8_kernel(const unsigned char* __restrict__ kc, const unsigned char* _
                     const int* __restrict__ token_pos, const int* __restrict__ token_seq, const int* __restrict__ block_table, int max_pages, int n_pages,
                     TA* __restrict__ k_out, TA* __restrict__ v_out, long long n, int nkv, int d, int page_size) {
     pdl_grid_sync();
-    const long long i = (long long)blockIdx.x * KQ_THREADS + threadIdx.x;
-    const int pieces = d >> 3;
-    if (i >= n * nkv * pieces) return;
-    const int c = (int)(i % pieces), hk = (int)(i / pieces % nkv);
-    const long long t = i / pieces / nkv;
-    const int p = token_pos[t];
-    const int page = p >= 0 && p / page_size < max_pages ? block_table[(size_t)token_seq[t] * max_pages + p / page_size] : -1;
+    // a block takes pieces of eight channels of one position (blockIdx.x)
+    const int pieces = d >> 3, i = blockIdx.y * KQ_THREADS + threadIdx.x;
+    if (i >= nkv * pieces) return;
+    const int hk = i / pieces, c = i - hk * pieces;
+    const long long t = blockIdx.x;
+    const int p = token_pos[t], logical = p < 0 ? max_pages : (int)((unsigned)p / (unsigned)page_size);
+    const int page = logical < max_pages ? block_table[(size_t)token_seq[t] * max_pages + logical] : -1;
     const bool held = page >= 0 && page < n_pages;
-    const size_t row = held ? ((size_t)page * nkv + hk) * page_size + p % page_size : 0;
+    const size_t row = held ? ((size_t)page * nkv + hk) * page_size + (p - logical * page_size) : 0;
     const float nan = __uint_as_float(0x7fffffffu);
     auto one = [&](const unsigned char* cache, const float* scales, TA* out) {
         const uint2 v = *reinterpret_cast<const uint2*>(cache + row * d + c * 8);
@@ -212,7 +213,7 @@ extern "C" int illm_kv_write_int8(const void* qkv, const float* partials, int sp
     const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, at_once = KQ_THREADS / lanes;
     const int n_slots = nh + (write_kv ? 2 * nkv : 0), rounds_all = (n_slots + at_once - 1) / at_once;
     // several heads to a thread once that leaves eight blocks to every SM
-    const bool wide = (rot & 15) == 0;
+    const bool wide = (rot & 7) == 0;
     int rounds = 1;
     if (wide && !partials)
         while (rounds < 4 && rounds < rounds_all && (long long)T * ((rounds_all + rounds) / (rounds + 1)) >= 8LL * illm_sm_count()) rounds++;
@@ -260,14 +261,15 @@ extern "C" int illm_kv_read_int8(const void* kc, const void* vc, const float* ks
     if (nkv <= 0 || d <= 0 || d > 256 || (d & 7) || page_size <= 0 || max_pages <= 0 || n_pages <= 0 || n_pages > 0x7fffffffLL || !kc || !vc || !ksc || !vsc || ((uintptr_t)kc & 7) ||
         ((uintptr_t)vc & 7) || ((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || (dtype != ILLM_BF16 && dtype != ILLM_F32))
         return ILLM_ERR_BAD_ARG;
-    const long long blocks = (n * nkv * (d / 8) + KQ_THREADS - 1) / KQ_THREADS;
-    if (blocks > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;
+    const int items = nkv * (d / 8), threads = items >= KQ_THREADS ? KQ_THREADS : (items + 31) / 32 * 32;
+    if (n > 0x7fffffffLL || items > 65535 * KQ_THREADS) return ILLM_ERR_BAD_ARG;
+    const dim3 grid((unsigned)n, (unsigned)((items + KQ_THREADS - 1) / KQ_THREADS));
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == ILLM_BF16)
-        illm_launch(kv_read_int8_kernel<bf16>, dim3((unsigned)blocks), dim3(KQ_THREADS), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
+        illm_launch(kv_read_int8_kernel<bf16>, grid, dim3(threads), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
                     token_seq, block_table, max_pages, (int)n_pages, (bf16*)k_out, (bf16*)v_out, n, nkv, d, page_size);
     else
-        illm_launch(kv_read_int8_kernel<float>, dim3((unsigned)blocks), dim3(KQ_THREADS), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
+        illm_launch(kv_read_int8_kernel<float>, grid, dim3(threads), 0, s, (const unsigned char*)kc, (const unsigned char*)vc, ksc, vsc, token_pos,
                     token_seq, block_table, max_pages, (int)n_pages, (float*)k_out, (float*)v_out, n, nkv, d, page_size);
     return illm_launch_status();
 }
