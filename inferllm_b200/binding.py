@@ -80,6 +80,7 @@ _SIGNATURES = {
     "illm_ledger_release_beyond": [P, I, LL], "illm_ledger_row": [P, I, I, PI], "illm_ledger_check": [P],
     "illm_ledger_pool": [P], "illm_ledger_pages": [P, I, PI, PI, I],
     "illm_cache_create": [S, I, I, I, LL, PP], "illm_cache_wrap": [P], "illm_cache_free_handle": [P],
+    "illm_cache_fork_slot": [P, I, LL, PI], "illm_cache_common_prefixes": [P, PI, I, PP], "illm_engine_fork_sequence": [P, I, LL, PI],
     "illm_cache_alloc_slot": [P, PI], "illm_cache_free_slot": [P, I], "illm_cache_reset": [P], "illm_cache_check": [P],
     "illm_cache_plan_step": [P, PI, PI, I, PI, PLL, PI], "illm_cache_commit_step": [P, I], "illm_cache_abandon_step": [P, I],
     "illm_cache_stats": [P, PP],
@@ -104,7 +105,7 @@ _SIGNATURES = {
     "illm_test_device": [P, PP], "illm_test_device_rewind": [P], "illm_test_device_info": [P, PI, PP, PP],
     "illm_copy_device": [P, P, P, LL], "illm_op_linear": [P, S, P, LL, LL, P, LL, I, I, I, PP, PP, PI],
     "illm_op_linear_gated": [P, S, P, LL, LL, P, LL, I, PP], "illm_policy_gemm_tc_splits": [LL, LL, LL, I],
-    "illm_policy_pages_splits": [LL, LL, I, I],
+    "illm_policy_pages_splits": [LL, LL, I, I], "illm_policy_pages_in_cluster": [LL, I, I],
     "illm_policy_ring_splits": [LL, I, LL, I, I], "illm_policy_attention_diff_splits": [LL, I, LL, I], "illm_policy_attention_supported": [I, I, I, I, I, I],
     "illm_policy_attention_generic": [PI, I, I, I, PI],
     "illm_policy_scan_form": [I, LL, I, I, I, I, I],

@@ -53,6 +53,9 @@ ILLM_API int illm_engine_load_folder(void* e, const char* folder) {
 ILLM_API int illm_engine_load_random(void* e, unsigned long long seed) {
     return guard([&] { ((Engine*)e)->load_random(seed); });
 }
+ILLM_API int illm_engine_fork_sequence(void* e, int slot, long long length, int* forked) {
+    return guard([&] { *forked = ((Engine*)e)->fork_sequence(slot, length); });
+}
 ILLM_API int illm_engine_new_sequence(void* e, int* slot) {
     return guard([&] { *slot = ((Engine*)e)->new_sequence(); });
 }
@@ -255,6 +258,8 @@ ILLM_API int illm_model_create(const char* config_json, const char* model_name, 
         if (j.at("max_batch").is_int()) c.max_batch = (int)j.at("max_batch").as_int();
         if (j.at("page_size").is_int()) c.page_size = (int)j.at("page_size").as_int();
         if (j.at("cuda_graphs").is_bool()) c.cuda_graphs = j.at("cuda_graphs").as_bool();
+        if (j.has("cache_dtype") && j.at("cache_dtype").is_string()) c.cache_dtype = j.at("cache_dtype").as_string();
+        if (j.has("share_prefixes") && j.at("share_prefixes").is_bool()) c.share_prefixes = j.at("share_prefixes").as_bool();
         if (j.at("max_adapters").is_int()) c.max_adapters = (int)j.at("max_adapters").as_int();
         if (j.at("adapter_rank").is_int()) c.adapter_rank = (int)j.at("adapter_rank").as_int();
         if (j.at("gemm").is_string()) c.gemm = j.at("gemm").as_string();
@@ -414,6 +419,7 @@ ILLM_API int illm_policy_ring_splits(long long T, int n_kv_heads, long long max_
 ILLM_API int illm_policy_pages_splits(long long pairs, long long keys, int wide, int n_sms) {
     return wide ? ops::attention_prefix_splits(pairs, keys, n_sms) : ops::attention_pages_splits(pairs, keys, n_sms);
 }
+ILLM_API int illm_policy_pages_in_cluster(long long pairs, int splits, int n_sms) { return ops::attention_pages_in_cluster(pairs, splits, n_sms); }
 ILLM_API int illm_policy_attention_diff_splits(long long T, int head_groups, long long max_seq_len, int n_sms) {
     return ops::attention_diff_splits(T, head_groups, max_seq_len, n_sms);
 }

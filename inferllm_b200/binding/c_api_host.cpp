@@ -320,6 +320,23 @@ ILLM_API void illm_cache_free_handle(void* h) { delete (CacheHandle*)h; }
 ILLM_API int illm_cache_alloc_slot(void* h, int* slot) {
     return guard([&] { *slot = ((CacheHandle*)h)->cache->alloc_slot(); });
 }
+ILLM_API int illm_cache_fork_slot(void* h, int from, long long length, int* slot) {
+    return guard([&] { *slot = ((CacheHandle*)h)->cache->fork_slot(from, length); });
+}
+// The common prefixes of sequences, as JSON: [[positions, [places in `slots`]], ...].
+ILLM_API int illm_cache_common_prefixes(void* h, const int* slots, int n, char** out) {
+    return guard([&] {
+        Json a = Json::array();
+        for (auto& g : ((CacheHandle*)h)->cache->common_prefixes(std::vector<int>(slots, slots + n))) {
+            Json e = Json::array(), members = Json::array();
+            for (int i : g.second) members.push(i);
+            e.push(g.first);
+            e.push(members);
+            a.push(e);
+        }
+        *out = dup_string(a.dump());
+    });
+}
 ILLM_API int illm_cache_free_slot(void* h, int slot) {
     return guard([&] { ((CacheHandle*)h)->cache->free_slot(slot); });
 }
@@ -397,6 +414,11 @@ ILLM_API int illm_cache_stats(void* hh, char** out) {
             o.set("pages", pages);
             o.set("k", (long long)(uintptr_t)g.k);
             o.set("v", (long long)(uintptr_t)g.v);
+            if (g.k_scale) {
+                o.set("k_scale", (long long)(uintptr_t)g.k_scale);
+                o.set("v_scale", (long long)(uintptr_t)g.v_scale);
+                o.set("scale_entry_bytes", (long long)g.scale_entry_bytes);
+            }
             paged.push(o);
         }
         for (auto& g : c.states) {

@@ -24,6 +24,7 @@ class PagedKV:
     window: Optional[int] = None
     keys_only: bool = False
     chunk: Optional[int] = None
+    int8: bool = False            # rows of eight bits with a scale per row
 
     def to_json(self):
         j = {"kind": "kv", "n_kv_heads": self.n_kv_heads, "head_dim": self.head_dim, "window": self.window}
@@ -31,6 +32,8 @@ class PagedKV:
             j["keys_only"] = True
         if self.chunk:
             j["chunk"] = self.chunk
+        if self.int8:
+            j["int8"] = True
         return j
 
 
@@ -186,6 +189,16 @@ class SequenceCache:
         out = ctypes.c_int()
         _b.check(_b.lib().illm_cache_alloc_slot(self._ptr, ctypes.byref(out)))
         return out.value
+
+    def fork_slot(self, slot: int, length: int) -> int:
+        """A sequence that begins with the first `length` positions of another (whole pages, which both hold then)."""
+        out = ctypes.c_int()
+        _b.check(_b.lib().illm_cache_fork_slot(self._ptr, slot, length, ctypes.byref(out)))
+        return out.value
+
+    def common_prefixes(self, slots: Sequence[int]) -> List[Tuple[int, List[int]]]:
+        """Of these sequences those that hold their first pages in common: (positions, places in `slots`) per group."""
+        return [(n, m) for n, m in _b.call_json(_b.lib().illm_cache_common_prefixes, self._ptr, _b.ints(slots), len(slots))]
 
     def free_slot(self, slot: int) -> None:
         _b.check(_b.lib().illm_cache_free_slot(self._ptr, slot))

@@ -42,7 +42,7 @@ CacheRequest CacheRequest::state(std::vector<long long> shape, DType dtype) {
 }
 bool CacheRequest::operator==(const CacheRequest& o) const {
     return kind == o.kind && n_kv_heads == o.n_kv_heads && head_dim == o.head_dim && v_head_dim == o.v_head_dim && window == o.window && chunk == o.chunk &&
-           keys_only == o.keys_only && shape == o.shape &&
+           keys_only == o.keys_only && int8 == o.int8 && shape == o.shape &&
            (kind != FixedState || dtype == o.dtype);
 }
 Json CacheRequest::to_json() const {
@@ -56,6 +56,7 @@ Json CacheRequest::to_json() const {
         if (keys_only) j.set("keys_only", true);
         j.set("window", window ? Json(window) : Json());
         if (chunk) j.set("chunk", chunk);
+        if (int8) j.set("int8", true);
     } else {
         j.set("kind", "state");
         Json s = Json::array();
@@ -71,13 +72,17 @@ CacheRequest CacheRequest::from_json(const Json& j) {
     const int chunk = j.has("chunk") && j.at("chunk").is_int() ? (int)j.at("chunk").as_int() : 0;
     if (chunk < 0 || (chunk > 0 && j.has("window") && j.at("window").is_int() && j.at("window").as_int() > 0))
         throw CacheError("a cache request has a window or a chunk, not both, and neither is negative");
+    if (kind == "kv" && j.has("int8") && j.at("int8").is_bool() && j.at("int8").as_bool() && j.has("keys_only") && j.at("keys_only").is_bool() && j.at("keys_only").as_bool())
+        throw CacheError("a keys-only entry is not kept in eight bits");
     if (kind == "kv" && j.has("keys_only") && j.at("keys_only").is_bool() && j.at("keys_only").as_bool())
         return paged_keys_only((int)j.at("n_kv_heads").as_int(), (int)j.at("head_dim").as_int(),
                                j.at("window").is_int() ? (int)j.at("window").as_int() : 0).in_chunks(chunk);
-    if (kind == "kv")
-        return paged((int)j.at("n_kv_heads").as_int(), (int)j.at("head_dim").as_int(),
-                     j.at("window").is_int() ? (int)j.at("window").as_int() : 0,
-                     j.has("v_head_dim") && j.at("v_head_dim").is_int() ? (int)j.at("v_head_dim").as_int() : 0).in_chunks(chunk);
+    if (kind == "kv") {
+        const CacheRequest r = paged((int)j.at("n_kv_heads").as_int(), (int)j.at("head_dim").as_int(),
+                                     j.at("window").is_int() ? (int)j.at("window").as_int() : 0,
+                                     j.has("v_head_dim") && j.at("v_head_dim").is_int() ? (int)j.at("v_head_dim").as_int() : 0).in_chunks(chunk);
+        return j.has("int8") && j.at("int8").is_bool() && j.at("int8").as_bool() ? r.in_int8() : r;
+    }
     if (kind == "state") {
         std::vector<long long> shape;
         for (const Json& d : j.at("shape").items()) shape.push_back(d.as_int());
@@ -130,7 +135,28 @@ void IndexPool::check() const {
 // ---- PageLedger
 
 PageLedger::PageLedger(int num_pages, int page_size_, int num_slots, int window_, int chunk_)
-        : pool(num_pages, "page"), page_size(page_size_), window(window_), chunk(chunk_), pages((size_t)num_slots), n_logical((size_t)num_slots, 0) {}
+        : pool(num_pages, "page"), page_size(page_size_), window(window_), chunk(chunk_), pages((size_t)num_slots), n_logical((size_t)num_slots, 0),
+          holders((size_t)std::max(num_pages, 0), 0) {}
+
+void PageLedger::drop(std::vector<int>& physical) {
+    std::vector<int> back;
+    for (int p : physical)
+        if (--holders[(size_t)p] == 0) back.push_back(p);
+    physical.swap(back);
+    pool.free(physical);
+}
+void PageLedger::share(int from, int to, int count) {
+    if (!pages[to].empty() || n_logical[to]) throw CacheError("slot " + std::to_string(to) + " holds pages of its own");
+    for (int lp = 0; lp < count; lp++) {
+        auto it = pages[from].find(lp);
+        if (it == pages[from].end()) throw CacheError("slot " + std::to_string(from) + " does not hold its page " + std::to_string(lp) + " any more");
+    }
+    for (int lp = 0; lp < count; lp++) {
+        pages[to][lp] = pages[from][lp];
+        holders[(size_t)pages[from][lp]]++;
+    }
+    n_logical[to] = count;
+}
 
 static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -141,7 +167,10 @@ void PageLedger::reserve(int slot, long long new_len) {
     const int want = (int)ceil_div(new_len, page_size), first = n_logical[slot];
     if (want > first) {
         std::vector<int> got = pool.alloc(want - first);
-        for (int lp = first; lp < want; lp++) pages[slot][lp] = got[lp - first];
+        for (int lp = first; lp < want; lp++) {
+            pages[slot][lp] = got[lp - first];
+            holders[(size_t)got[lp - first]] = 1;
+        }
         n_logical[slot] = want;
     }
 }
@@ -157,13 +186,13 @@ std::vector<int> PageLedger::release_outside_window(int slot, long long seq_len)
         gone.push_back(it->second);
         it = have.erase(it);
     }
-    pool.free(gone);
+    drop(gone);
     return gone;
 }
 std::vector<int> PageLedger::release_all(int slot) {
     std::vector<int> gone;
     for (auto& p : pages[slot]) gone.push_back(p.second);
-    pool.free(gone);
+    drop(gone);
     pages[slot].clear();
     n_logical[slot] = 0;
     return gone;
@@ -176,7 +205,7 @@ std::vector<int> PageLedger::release_beyond(int slot, long long seq_len) {
         gone.push_back(it->second);
         it = have.erase(it);
     }
-    pool.free(gone);
+    drop(gone);
     if (n_logical[slot] > keep) n_logical[slot] = keep;
     return gone;
 }
@@ -187,16 +216,15 @@ void PageLedger::row(int slot, int width, int* out) const {
 }
 void PageLedger::check() const {
     pool.check();
-    std::set<int> held;
-    size_t n = 0;
+    std::map<int, int> held;
     for (auto& d : pages)
-        for (auto& p : d) {
-            held.insert(p.second);
-            n++;
-        }
-    if (held.size() != n) throw CacheError("a page is held by two sequences");
-    if ((int)n != pool.n_held())
-        throw CacheError(std::to_string(pool.n_held()) + " pages are out of the pool but sequences hold " + std::to_string(n));
+        for (auto& p : d) held[p.second]++;
+    for (auto& h : held)
+        if (h.second != holders[(size_t)h.first])
+            throw CacheError(h.second > holders[(size_t)h.first] ? "a page is held by two sequences"
+                                                                 : "page " + std::to_string(h.first) + " has fewer holders than it was given to");
+    if ((int)held.size() != pool.n_held())
+        throw CacheError(std::to_string(pool.n_held()) + " pages are out of the pool but sequences hold " + std::to_string(held.size()));
 }
 
 // ---- SequenceCache
@@ -205,7 +233,8 @@ size_t SequenceCache::bytes_per_token(const std::map<int, CacheRequest>& request
     size_t n = 0;
     for (auto& r : requests)
         if (r.second.kind == CacheRequest::PagedKV)
-            n += (size_t)r.second.n_kv_heads * (r.second.head_dim + (r.second.keys_only ? 0 : r.second.v_head_dim)) * dtype_size(dtype);
+            n += (size_t)r.second.n_kv_heads * (r.second.int8 ? (size_t)r.second.head_dim + r.second.v_head_dim + 2 * sizeof(float)
+                                                              : (r.second.head_dim + (r.second.keys_only ? 0 : r.second.v_head_dim)) * dtype_size(dtype));
     return n;
 }
 
@@ -247,10 +276,15 @@ SequenceCache::SequenceCache(const std::map<int, CacheRequest>& requests, int nu
         }
     }
     for (PagedGroup& g : paged) {
-        g.page_bytes = (size_t)g.request.n_kv_heads * page_size * g.request.head_dim * dtype_size(dtype);
+        const size_t size = dtype_size(g.request.int8 ? DType::U8 : dtype);
+        if (g.request.int8 && g.request.keys_only) throw CacheError("a keys-only entry is not kept in eight bits");
+        g.page_bytes = (size_t)g.request.n_kv_heads * page_size * g.request.head_dim * size;
         g.entry_bytes = g.page_bytes * num_pages;
-        g.v_page_bytes = g.request.keys_only ? 0 : (size_t)g.request.n_kv_heads * page_size * g.request.v_head_dim * dtype_size(dtype);
+        g.v_page_bytes = g.request.keys_only ? 0 : (size_t)g.request.n_kv_heads * page_size * g.request.v_head_dim * size;
         g.v_entry_bytes = g.v_page_bytes * num_pages;
+        // (entries' scales begin on 16-byte boundaries, which bulk copies want)
+        g.scale_page_bytes = g.request.int8 ? (size_t)g.request.n_kv_heads * page_size * sizeof(float) : 0;
+        g.scale_entry_bytes = (g.scale_page_bytes * num_pages + 255) / 256 * 256;
     }
     for (StateGroup& g : states) g.entry_bytes = (size_t)num_slots * g.request.elements() * dtype_size(g.request.dtype);
     if (!device_) return;
@@ -269,6 +303,12 @@ SequenceCache::SequenceCache(const std::map<int, CacheRequest>& requests, int nu
             check_cuda(cudaMemsetAsync(g.k, 0xFF, g.entry_bytes * g.entries.size(), device_->stream()), "poisoning the cache");
             if (g.v) check_cuda(cudaMemsetAsync(g.v, 0xFF, g.v_entry_bytes * g.entries.size(), device_->stream()), "poisoning the cache");
         }
+        if (!g.scale_entry_bytes) continue;
+        g.k_scale = (float*)device_->alloc_persistent(g.scale_entry_bytes * g.entries.size(), "the scales of the cache's keys", !poison);
+        g.v_scale = (float*)device_->alloc_persistent(g.scale_entry_bytes * g.entries.size(), "the scales of the cache's values", !poison);
+        if (poison)
+            for (float* s : {g.k_scale, g.v_scale})
+                check_cuda(cudaMemsetAsync(s, 0xFF, g.scale_entry_bytes * g.entries.size(), device_->stream()), "poisoning the cache");
     }
     for (StateGroup& g : states) g.state = device_->alloc_persistent(g.entry_bytes * g.entries.size(), "the per-sequence state", true);
 }
@@ -278,6 +318,8 @@ SequenceCache::~SequenceCache() {
     for (PagedGroup& g : paged) {
         device_->free_persistent(g.k);
         if (g.v) device_->free_persistent(g.v);
+        if (g.k_scale) device_->free_persistent(g.k_scale);
+        if (g.v_scale) device_->free_persistent(g.v_scale);
     }
     for (StateGroup& g : states) device_->free_persistent(g.state);
     device_->free_persistent(poison_list_);
@@ -297,7 +339,16 @@ void SequenceCache::poison_pages(PagedGroup& g, const std::vector<int>& pages) {
     std::copy(pages.begin(), pages.end(), poison_host_);
     check_cuda(cudaMemcpyAsync(poison_list_, poison_host_, pages.size() * 4, cudaMemcpyHostToDevice, device_->stream()),
                "uploading the pages to poison");
-    if (!g.v) {        // keys only
+    if (g.scale_page_bytes % 16 == 0 && g.k_scale) {        // an eight-bit row reads as NaN once its scale does
+        check_kernel(illm_poison_pages(g.k_scale, g.v_scale, (long long)g.scale_entry_bytes, (int)g.entries.size(), (long long)g.scale_page_bytes, poison_list_,
+                                       (int)pages.size(), device_->stream()),
+                     "poison_pages");
+    } else if (g.k_scale) {
+        for (size_t e = 0; e < g.entries.size(); e++)
+            for (int p : pages)
+                for (float* s : {g.k_scale, g.v_scale})
+                    check_cuda(cudaMemsetAsync((char*)s + e * g.scale_entry_bytes + (size_t)p * g.scale_page_bytes, 0xFF, g.scale_page_bytes, device_->stream()), "poisoning a page");
+    } else if (!g.v) {        // keys only
         check_kernel(illm_poison_pages(g.k, g.k, (long long)g.entry_bytes, (int)g.entries.size(), (long long)g.page_bytes, poison_list_,
                                        (int)pages.size(), device_->stream()),
                      "poison_pages");
@@ -333,6 +384,51 @@ int SequenceCache::alloc_slot() {
             }
         }
     return slot;
+}
+
+bool SequenceCache::can_fork() const {
+    if (!states.empty() || paged.empty()) return false;
+    for (const PagedGroup& g : paged)
+        if (g.request.window > 0 || g.request.chunk > 0) return false;
+    return true;
+}
+
+int SequenceCache::fork_slot(int from, long long length) {
+    if (!slots.is_held(from)) throw CacheError("slot " + std::to_string(from) + " is not live");
+    if (!can_fork()) throw CacheError("positions cannot be shared: this model keeps a window of them, chunks of them or per-sequence state");
+    if (length < page_size || length % page_size || length > seq_len[from])
+        throw CacheError("slot " + std::to_string(from) + ": " + std::to_string(length) + " positions cannot be shared (a multiple of the page size " +
+                         std::to_string(page_size) + ", up to the sequence's " + std::to_string(seq_len[from]) + ")");
+    const int slot = alloc_slot();
+    for (PagedGroup& g : paged) g.ledger->share(from, slot, (int)(length / page_size));
+    seq_len[slot] = length;
+    return slot;
+}
+
+std::vector<std::pair<int, std::vector<int>>> SequenceCache::common_prefixes(const std::vector<int>& step_slots) const {
+    std::vector<std::pair<int, std::vector<int>>> out;
+    if (!can_fork() || step_slots.size() < 2) return out;
+    const PageLedger& l = *paged[0].ledger;        // (pages are shared in all groups alike)
+    std::map<int, std::vector<int>> by_first;
+    for (size_t i = 0; i < step_slots.size(); i++) {
+        const auto& pages = l.pages[(size_t)step_slots[i]];
+        if (!pages.empty() && l.holders[(size_t)pages.begin()->second] > 1) by_first[pages.begin()->second].push_back((int)i);
+    }
+    for (auto& g : by_first) {
+        if (g.second.size() < 2) continue;
+        const auto& first = l.pages[(size_t)step_slots[(size_t)g.second[0]]];
+        int common = (int)first.size();
+        for (int i : g.second) {
+            const auto& pages = l.pages[(size_t)step_slots[(size_t)i]];
+            common = std::min(common, (int)pages.size());
+            auto a = first.begin(), b = pages.begin();
+            int n = 0;
+            while (n < common && a->second == b->second) ++a, ++b, ++n;
+            common = n;
+        }
+        out.emplace_back(common * page_size, g.second);
+    }
+    return out;
 }
 
 void SequenceCache::free_slot(int slot) {
@@ -432,6 +528,11 @@ KVView SequenceCache::kv_view(int entry, const int* table_dev) const {
     v.head_dim = g.request.head_dim;
     v.v_head_dim = g.request.v_head_dim;
     v.dtype = dtype_;
+    if (g.request.int8) {
+        v.dtype = DType::U8;
+        v.k_scale = g.k_scale ? (float*)((char*)g.k_scale + (size_t)it->second.index * g.scale_entry_bytes) : nullptr;
+        v.v_scale = g.v_scale ? (float*)((char*)g.v_scale + (size_t)it->second.index * g.scale_entry_bytes) : nullptr;
+    }
     return v;
 }
 
@@ -456,7 +557,7 @@ std::vector<int> SequenceCache::pages_free() const {
 }
 size_t SequenceCache::storage_bytes() const {
     size_t n = 0;
-    for (const PagedGroup& g : paged) n += (g.entry_bytes + g.v_entry_bytes) * g.entries.size();
+    for (const PagedGroup& g : paged) n += (g.entry_bytes + g.v_entry_bytes + 2 * g.scale_entry_bytes) * g.entries.size();
     return n;
 }
 

@@ -6,13 +6,15 @@
 // schedule) with equal requests form a group; every group has storage, a page pool and page tables
 // of its own, so groups with different needs (all keys, a window of them, another head size) live
 // side by side.  Device storage of a paged group: k : [entries, pages, kv heads, page_size,
-// head_dim], v likewise with its own row size, in the engine's dtype; of a state group: [entries, slots, elements].
+// head_dim], v likewise with its own row size, in the engine's dtype or, an eight-bit group, in bytes with a float32 scale per row beside them
+// (csrc/kv_int8.cu); of a state group: [entries, slots, elements].
 //
 // Life of a sequence: alloc_slot() (state zeroed) -> plan_step() / commit_step() once per step
 // (pages are reserved before the step runs and the length advances after it; abandon_step() gives
 // back what a step that failed had reserved) -> free_slot() (pages and slot go back to the pools
-// for the next sequence).  Nothing of the bookkeeping touches the device; its invariants (no slot
-// or page lost, held twice or freed twice) are checked on every call.
+// for the next sequence).  fork_slot() begins a sequence with another's first positions: both then hold the same pages, which
+// nobody writes any more (they are full) and which go back with the last of their holders.  Nothing of the bookkeeping touches the device; its
+// invariants (no slot or page lost, held by more sequences than it was given to or freed twice) are checked on every call.
 //
 // The reference has one implicit sequence per model: KvStorage keeps a single index of the tokens
 // stored (m_store_id, src/core/kvstorage.h:40-49) in one growable float32 tensor per layer
@@ -43,6 +45,8 @@ struct CacheRequest {
     // PagedKV with keys_only: one row per position that serves as key and as value (a shared latent); no value
     // pages are kept, and a view's `v` is its `k`
     bool keys_only = false;
+    // PagedKV with int8: rows of eight bits, one byte per value and a float32 scale per row
+    bool int8 = false;
     // FixedState: `elements` values of `dtype` per sequence, zeroed when a slot is handed out
     std::vector<long long> shape;
     DType dtype = DType::F32;
@@ -50,6 +54,7 @@ struct CacheRequest {
     static CacheRequest paged(int n_kv_heads, int head_dim, int window = 0, int v_head_dim = 0);
     static CacheRequest paged_keys_only(int n_kv_heads, int head_dim, int window = 0);
     CacheRequest in_chunks(int size) const { CacheRequest r = *this; r.chunk = size; return r; }
+    CacheRequest in_int8() const { CacheRequest r = *this; r.int8 = true; return r; }
     // the request widened to what a second reader with this window or chunk (0, 0: all positions) needs as well
     CacheRequest reaching(int window2, int chunk2) const;
     static CacheRequest state(std::vector<long long> shape, DType dtype = DType::F32);
@@ -89,12 +94,17 @@ public:
     std::vector<int> release_outside_window(int slot, long long seq_len);   // after a step; returns the pages given back
     std::vector<int> release_all(int slot);
     std::vector<int> release_beyond(int slot, long long seq_len);     // pages reserved for positions >= seq_len (a step that failed)
+    void share(int from, int to, int count);                          // `to`, which holds nothing, holds the first `count` pages of `from` too
     void row(int slot, int width, int* out) const;                    // logical -> physical table, -1 = no page
     void check() const;
     IndexPool pool;
     int page_size, window, chunk;
     std::vector<std::map<int, int>> pages;     // per slot: logical page -> physical page
     std::vector<int> n_logical;                // logical pages ever reserved by the slot's sequence
+    std::vector<int> holders;                  // per physical page: sequences that hold it
+
+private:
+    void drop(std::vector<int>& physical);     // one holder less each; keeps those that go back to the pool
 };
 
 struct StepPlan {
@@ -115,6 +125,9 @@ struct KVView {
     // 0 all, w > 0 the last w, -c < 0 those of its own chunk of c.
     int span() const { return chunk > 0 ? -chunk : window; }
     DType dtype = DType::BF16;
+    // rows of eight bits (dtype U8): float32 [pages, kv heads, page_size] beside k and v
+    float *k_scale = nullptr, *v_scale = nullptr;
+    bool int8() const { return dtype == DType::U8; }
     bool writes = true;
 };
 struct StateView {
@@ -136,6 +149,13 @@ public:
     ~SequenceCache();
 
     int alloc_slot();
+    // A sequence that begins with the first `length` positions of `from` (a multiple of the page size, at least one page and at most what `from`
+    // holds): their pages are held by both.  CacheError where they cannot be shared: a window or chunk group, whose pages go back one by one, or
+    // per-sequence state.
+    int fork_slot(int from, long long length);
+    bool can_fork() const;
+    // Of a step's sequences those that hold their first pages in common: groups of at least two (places in `slots`) with the positions of those pages.
+    std::vector<std::pair<int, std::vector<int>>> common_prefixes(const std::vector<int>& slots) const;
     void free_slot(int slot);
     void reset();
     StepPlan plan_step(const std::vector<int>& slots, const std::vector<int>& q_lens);   // all or nothing
@@ -150,6 +170,8 @@ public:
         void *k = nullptr, *v = nullptr;
         size_t entry_bytes = 0, page_bytes = 0;          // of the keys
         size_t v_entry_bytes = 0, v_page_bytes = 0;      // of the values
+        float *k_scale = nullptr, *v_scale = nullptr;    // eight-bit groups
+        size_t scale_entry_bytes = 0, scale_page_bytes = 0;
     };
     struct StateGroup {
         CacheRequest request;

@@ -29,6 +29,8 @@ class EngineOptions:
     page_size: int = 64
     cuda_graphs: bool = True       # replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     gemm: str = "auto"             # bfloat16 products: "auto" | "tc" | "library"
+    cache_dtype: str = "auto"      # keys and values: "auto" (as `dtype`) or "int8" (a byte each and a scale per row, where a layer can)
+    share_prefixes: bool = False   # `generate` runs the first positions that all prompts of a batch have in common once
     max_adapters: int = 0          # low-rank adapters that may be loaded together (`Engine.add_adapter`)
     adapter_rank: int = 16         # the largest rank of one (at most 85)
     poison_freed_pages: bool = False    # fill pages that go back to the pool with NaN (a check, not for serving)
@@ -141,6 +143,15 @@ class Engine:
         _b.check(_b.lib().illm_engine_new_sequence(self._ptr, ctypes.byref(out)))
         return out.value
 
+    def fork_sequence(self, slot: int, length: int) -> int:
+        """A sequence that begins with the first `length` positions of a live one (a multiple of the page size): both hold the same pages of the cache
+        (the last of them to end gives them back), and decode steps of several such sequences read them once.  Refused (CacheError) for models that
+        keep a window of positions or per-sequence state.  Low-rank adapters make keys of their own: sequences that share positions should run with the
+        adapter that made them."""
+        out = ctypes.c_int()
+        _b.check(_b.lib().illm_engine_fork_sequence(self._ptr, slot, int(length), ctypes.byref(out)))
+        return out.value
+
     def end_sequence(self, slot: int) -> None:
         _b.check(_b.lib().illm_engine_end_sequence(self._ptr, slot))
 
@@ -235,11 +246,16 @@ class Engine:
 
     def cache_tensors(self, group: int = 0):
         """(k, v) of a paged group as torch tensors [entries, pages, kv heads, page_size, head_dim]
-        that view the engine's own storage."""
+        that view the engine's own storage; of an eight-bit group (k, v, k_scale, v_scale), uint8 and the float32 scales
+        [entries, pages, kv heads, page_size] (`kernels.ops.CacheInt8`)."""
         import torch
         st = self.cache.stats()
         g = st["paged"][group]
         shape = (len(g["entries"]), st["num_pages"], g["request"]["n_kv_heads"], st["page_size"], g["request"]["head_dim"])
+        if "k_scale" in g:
+            rows = shape[1] * shape[2] * shape[3]
+            scales = [device_view(g[name], (shape[0], g["scale_entry_bytes"] // 4), torch.float32, self.device_id)[:, :rows].view(*shape[:-1]) for name in ("k_scale", "v_scale")]
+            return tuple(device_view(g[name], shape, torch.uint8, self.device_id) for name in ("k", "v")) + tuple(scales)
         dtype = torch.float32 if self.info()["dtype"] == "float32" else torch.bfloat16
         return tuple(device_view(g[name], shape, dtype, self.device_id) for name in ("k", "v"))
 
@@ -433,6 +449,8 @@ class ModelConfig:
     page_size: int = 64
     cuda_graphs: bool = True
     gemm: str = "auto"
+    cache_dtype: str = "auto"
+    share_prefixes: bool = False
     max_adapters: int = 0
     adapter_rank: int = 16
     poison_freed_pages: bool = False

@@ -26,6 +26,8 @@ EngineOptions EngineOptions::from_json(const Json& j) {
     if (j.at("cuda_graphs").is_bool()) o.cuda_graphs = j.at("cuda_graphs").as_bool();
     if (j.at("gemm").is_string()) o.gemm = j.at("gemm").as_string();
     if (j.at("poison_freed_pages").is_bool()) o.poison_freed_pages = j.at("poison_freed_pages").as_bool();
+    if (j.has("cache_dtype") && j.at("cache_dtype").is_string()) o.cache_dtype = j.at("cache_dtype").as_string();
+    if (j.has("share_prefixes") && j.at("share_prefixes").is_bool()) o.share_prefixes = j.at("share_prefixes").as_bool();
     if (j.at("stream").is_int()) o.stream = (void*)(uintptr_t)j.at("stream").as_int();
     return o;
 }
@@ -52,6 +54,7 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     if (options.max_adapters < 0 || options.max_adapters > 4096) throw EngineError("max_adapters must be in [0, 4096]");
     if (options.max_adapters > 0 && (options.adapter_rank < 1 || options.adapter_rank > ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces))
         throw EngineError("adapter_rank must be in [1, " + std::to_string(ADAPTER_GROUP * ADAPTER_MAX_GROUPS / kAdapterPieces) + "]");
+    if (options.cache_dtype != "auto" && options.cache_dtype != "int8") throw EngineError("cache_dtype '" + options.cache_dtype + "' is not supported (auto or int8)");
     device_.reset(new Device(options.device_id, (cudaStream_t)options.stream));
     device_->set_weights_settled(true);
     rt_.dev = device_.get();
@@ -67,11 +70,18 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
         model_->make_adapters(options.max_adapters, options.adapter_rank);
         adapter_ranks_.assign((size_t)options.max_adapters, 0);
     }
+    const std::map<int, CacheRequest> requests = model_->cache_requests(options.cache_dtype == "int8");
+    if (options.cache_dtype == "int8") {
+        bool any = false;
+        for (auto& r : requests) any = any || r.second.int8;
+        if (!any) throw EngineError("cache_dtype int8: no layer of this model keeps its keys and values in eight bits");
+    }
+    prefix_heads_ = model_->prefix_heads();
     long long max_tokens = options.max_tokens;
     if (max_tokens <= 0) max_tokens = tokens_that_fit(options.mem_fraction);
     const int num_pages = (int)std::max<long long>(1, ceil_div(max_tokens, options.page_size));
     const int num_slots = options.max_batch > 0 ? options.max_batch : num_pages;
-    cache_.reset(new SequenceCache(model_->cache_requests(), num_slots, num_pages, options.page_size, max_seq, device_.get(), dtype,
+    cache_.reset(new SequenceCache(requests, num_slots, num_pages, options.page_size, max_seq, device_.get(), dtype,
                                    options.poison_freed_pages));
     builder_.reset(new StepContextBuilder(device_.get(), &rt_));
     for (TokRead& t : tok_reads_) check_cuda(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming), "cudaEventCreate");
@@ -133,7 +143,7 @@ long long Engine::tokens_that_fit(double fraction) const {
     const size_t elem = dtype_size(rt_.dtype);
     size_t weights = 0;
     for (auto& d : model_->tensor_decls()) weights += (size_t)d.second.numel() * elem;
-    const size_t per_token = SequenceCache::bytes_per_token(model_->cache_requests(), rt_.dtype);
+    const size_t per_token = SequenceCache::bytes_per_token(model_->cache_requests(options_.cache_dtype == "int8"), rt_.dtype);
     const size_t free_b = device_->mem_free();
     if (per_token == 0) return options_.page_size;
     const double room = ((double)free_b - (double)weights) * fraction;
@@ -149,6 +159,10 @@ long long Engine::tokens_that_fit(double fraction) const {
 int Engine::new_sequence() {
     device_->make_current();
     return cache_->alloc_slot();
+}
+int Engine::fork_sequence(int slot, long long length) {
+    device_->make_current();
+    return cache_->fork_slot(slot, length);
 }
 void Engine::end_sequence(int slot) {
     device_->make_current();
@@ -224,10 +238,38 @@ void Engine::size_adapters(StepAdapters& a, bool fixed, bool one_sequence) const
 }
 
 StepContext Engine::make_context(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows, int* into,
-                                 std::vector<const int*>* tables_dev, const StepAdapters* adapters) {
-    StepContext ctx = builder_->build(*cache_, plan, ids, want_rows, into, tables_dev, adapters);
+                                 std::vector<const int*>* tables_dev, const StepAdapters* adapters, const StepPrefixes* prefixes) {
+    StepContext ctx = builder_->build(*cache_, plan, ids, want_rows, into, tables_dev, adapters, prefixes);
     last_upload_bytes_ = builder_->last_upload_bytes;
     return ctx;
+}
+
+// The common prefixes of a decode step's sequences, where walking them once saves more than the second launch of it costs.  What the launches depend on
+// (tiles, the splits that follow from the lengths) is rounded up, so that captured steps of growing sequences can be replayed.
+bool Engine::find_prefixes(const StepPlan& plan, StepPrefixes* out) const {
+    if (!prefix_heads_ || plan.slots.size() < 2) return false;
+    long long saved = 0;
+    for (auto& g : cache_->common_prefixes(plan.slots)) {
+        saved += (long long)g.first * ((long long)g.second.size() - 1);
+        ops::PrefixGroup group;
+        group.prefix = g.first;
+        group.members = g.second;
+        out->groups.push_back(std::move(group));
+    }
+    if (saved < kSharedPrefixMinSaved) return false;
+    std::vector<int> lens;
+    for (size_t i = 0; i < plan.slots.size(); i++) lens.push_back((int)(plan.past[i] + 1));
+    out->heads = prefix_heads_;
+    out->sizes = ops::prefix_plan_sizes(out->groups, lens.data(), (int)lens.size(), prefix_heads_);
+    auto up = [](int n) {
+        int p = 1;
+        while (p < n) p *= 2;
+        return p;
+    };
+    out->sizes.tiles = up(out->sizes.tiles);
+    out->sizes.longest_rest = up(out->sizes.longest_rest);
+    out->sizes.longest_prefix = up(out->sizes.longest_prefix);
+    return true;
 }
 
 LogitsRef Engine::run_forward(const StepContext& ctx, const std::vector<const int*>& tables) {
@@ -279,15 +321,17 @@ LogitsRef Engine::step(const std::vector<StepItem>& items, const int* device_ids
     }
     StepPlan plan = cache_->plan_step(slots, q_lens);
     LogitsRef logits;
+    StepPrefixes step_prefixes;
+    const StepPrefixes* prefixes = ids.size() == items.size() && find_prefixes(plan, &step_prefixes) ? &step_prefixes : nullptr;
     try {
         if (options_.cuda_graphs && ids.size() == items.size() && graph_safe_) {
             if (adapters) size_adapters(*adapters, true, false);
-            logits = decode_step_graphed(plan, ids, want_rows, device_ids, adapters);
+            logits = decode_step_graphed(plan, ids, want_rows, device_ids, adapters, prefixes);
         } else {
             if (adapters) size_adapters(*adapters, false, false);
             device_->arena_rewind();
             std::vector<const int*> tables;
-            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
+            StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters, prefixes);
             if (device_ids)
                 check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                            "copying the step's token ids");
@@ -317,16 +361,18 @@ void Engine::drop_graphs(bool keep_seen) {
 }
 
 LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, const std::vector<int>& ids,
-                                  const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters) {
+                                  const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes) {
     if (graphs_.size() > 64) drop_graphs(true);
     std::unique_ptr<GraphEntry> e(new GraphEntry);
     int T = 0;
     for (int q : plan.q_lens) T += q;
     e->ctx_buf = (int*)device_->alloc_persistent(
-            (context_ints(T, (int)plan.slots.size(), (int)want_rows.size()) + (adapters ? adapters->ints() : 0)) * sizeof(int), "the inputs of a captured step");
+            (context_ints(T, (int)plan.slots.size(), (int)want_rows.size()) + (adapters ? (adapters->ints() + 3) / 4 * 4 : 0) + (prefixes ? (size_t)prefixes->sizes.ints() : 0)) *
+                    sizeof(int),
+            "the inputs of a captured step");
     device_->arena_rewind();
     std::vector<const int*> tables;
-    StepContext ctx = make_context(plan, ids, want_rows, e->ctx_buf, &tables, adapters);
+    StepContext ctx = make_context(plan, ids, want_rows, e->ctx_buf, &tables, adapters, prefixes);
     if (device_ids)
         check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                    "copying the step's token ids");
@@ -363,9 +409,9 @@ LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, 
 }
 
 LogitsRef Engine::replay(GraphEntry& e, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                         const int* device_ids, const StepAdapters* adapters) {
+                         const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes) {
     std::vector<const int*> tables;
-    StepContext ctx = make_context(plan, ids, want_rows, e.ctx_buf, &tables, adapters);
+    StepContext ctx = make_context(plan, ids, want_rows, e.ctx_buf, &tables, adapters, prefixes);
     if (device_ids)
         check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                    "copying the step's token ids");
@@ -425,21 +471,23 @@ bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const
 // in device memory), so the step is captured in a CUDA graph the second time a batch size is seen and
 // replayed from then on.
 LogitsRef Engine::decode_step_graphed(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                                      const int* device_ids, const StepAdapters* adapters) {
-    const std::string key = std::string(adapters ? "da/" : "d/") + std::to_string(ids.size()) + "/" + std::to_string(want_rows.size());
+                                      const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes) {
+    std::string key = std::string(adapters ? "da/" : "d/") + std::to_string(ids.size()) + "/" + std::to_string(want_rows.size());
+    if (prefixes)
+        for (int n : {prefixes->sizes.tiles, prefixes->sizes.wide ? 1 : 0, prefixes->sizes.longest_prefix, prefixes->sizes.longest_rest}) key += "/" + std::to_string(n);
     auto it = graphs_.find(key);
     if (it == graphs_.end()) {
         graphs_[key].reset(new GraphEntry);
         device_->arena_rewind();
         std::vector<const int*> tables;
-        StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
+        StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters, prefixes);
         if (device_ids)
             check_cuda(cudaMemcpyAsync((void*)ctx.ids, device_ids, ids.size() * sizeof(int), cudaMemcpyDeviceToDevice, device_->stream()),
                        "copying the step's token ids");
         return run_forward(ctx, tables);
     }
-    if (!it->second->exec) return capture_and_run(key, plan, ids, want_rows, device_ids, adapters);
-    return replay(*it->second, plan, ids, want_rows, device_ids, adapters);
+    if (!it->second->exec) return capture_and_run(key, plan, ids, want_rows, device_ids, adapters, prefixes);
+    return replay(*it->second, plan, ids, want_rows, device_ids, adapters, prefixes);
 }
 
 void Engine::read_logits(const LogitsRef& logits, float* host) {
@@ -524,9 +572,10 @@ void Engine::check_device_errors() {
         const char* what;
         switch (words.first) {
             case 4: what = "a wait inside the tensor-core matrix product (gemm_tc, gemm_tc2) timed out"; break;
-            case 5: what = "a wait inside the tensor-core prompt attention (attention_prefill_tc) timed out"; break;
+            case 5: what = "a wait inside the tensor-core prompt attention (attention_prefill_tc, attention_tiles) timed out"; break;
             case 6: what = "a tensor-core kernel found its shared memory misaligned and did not run"; break;
-            case 7: what = "a wait inside the decode attention (attention_decode_ring) timed out"; break;
+            case 7: what = "a wait inside the decode attention (attention_decode_ring, attention_pages) timed out"; break;
+            case 8: what = "an attention kernel met a visible position whose page the sequence does not hold"; break;
             default: what = nullptr;
         }
         throw EngineError((what ? std::string(what) : "a tensor-core kernel reported error " + std::to_string(words.first)) +

@@ -32,6 +32,8 @@ struct EngineOptions {
     int max_batch = 0;                  // slots; 0: max_tokens / page_size
     int page_size = 64;
     bool cuda_graphs = true;            // replay one-token-per-sequence steps and single prompts from captured CUDA graphs
+    std::string cache_dtype = "auto";   // keys and values: "auto" (as the compute dtype) or "int8" (a byte each and a scale per row, where a layer can)
+    bool share_prefixes = false;        // the generation loop runs the first positions that all prompts of a batch have in common once
     int max_adapters = 0;               // low-rank adapters that may be loaded together (Engine::add_adapter)
     int adapter_rank = 16;              // the largest rank of one (at most 85: q, k and v stand side by side)
     std::string gemm = "auto";          // bfloat16 products: "auto" | "tc" | "library" (see ops::GemmBackend)
@@ -61,6 +63,8 @@ struct LogitsRef {
     long long rows = 0, vocab = 0;
 };
 
+// Positions that a decode step's common prefixes must save (a prefix counts once for every sequence but one) to be walked by themselves.
+constexpr long long kSharedPrefixMinSaved = 1024;
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
 
@@ -75,6 +79,10 @@ public:
     void load_random(unsigned long long seed);
 
     int new_sequence();
+    // A sequence that begins with the first `length` positions of a live one (a multiple of the page size): both hold the same pages, and decode steps of
+    // several such sequences read them once (ops::attention_shared).  CacheError for models that keep a window or per-sequence state.
+    int fork_sequence(int slot, long long length);
+    bool can_fork() const { return cache_->can_fork(); }
     void end_sequence(int slot);
     long long sequence_length(int slot) const;
     Limits limits() const;
@@ -126,16 +134,17 @@ private:
     struct GraphEntry;
     long long tokens_that_fit(double fraction) const;
     StepContext make_context(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows, int* into,
-                             std::vector<const int*>* tables_dev, const StepAdapters* adapters);
+                             std::vector<const int*>* tables_dev, const StepAdapters* adapters, const StepPrefixes* prefixes = nullptr);
+    bool find_prefixes(const StepPlan& plan, StepPrefixes* out) const;
     void size_adapters(StepAdapters& a, bool fixed, bool one_sequence) const;
     LogitsRef run_forward(const StepContext& ctx, const std::vector<const int*>& tables);
     bool prompt_step_graphed(int slot, const std::vector<int>& ids, const std::vector<int>& want_rows, StepAdapters* adapters, LogitsRef* out);
     LogitsRef decode_step_graphed(const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                                  const int* device_ids, const StepAdapters* adapters);
+                                  const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes);
     LogitsRef capture_and_run(const std::string& key, const StepPlan& plan, const std::vector<int>& ids,
-                              const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters);
+                              const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes = nullptr);
     LogitsRef replay(GraphEntry& e, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                     const int* device_ids, const StepAdapters* adapters);
+                     const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes = nullptr);
     void drop_graphs(bool keep_seen);
     size_t context_ints(int T, int B, int K) const;
 
@@ -147,7 +156,7 @@ private:
     std::unique_ptr<SequenceCache> cache_;
     bool loaded_ = false;
     std::vector<int> adapter_ranks_;        // 0: free
-    int pad_safe_ = -1, graph_safe_ = -1;
+    int pad_safe_ = -1, graph_safe_ = -1, prefix_heads_ = 0;
     size_t last_upload_bytes_ = 0;
 
     std::unique_ptr<StepContextBuilder> builder_;

@@ -96,11 +96,30 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
         std::map<int, int> slots;
         std::map<int, long long> n_fed;         // tokens of a request that the cache holds
         try {
-            for (int r : batch) {
-                slots[r] = backend.new_sequence();
-                n_fed[r] = (long long)prompts[(size_t)r].size();
-            }
             double t0 = clock();
+            // whole pages that all prompts of the batch begin with (a prompt keeps a token of its own, and an adapter makes keys of its own)
+            long long common = 0;
+            if (const int page = batch.size() > 1 ? backend.share_page() : 0) {
+                const std::vector<int>& first = prompts[(size_t)batch[0]];
+                common = (long long)first.size() - 1;
+                for (int r : batch) {
+                    const std::vector<int>& p = prompts[(size_t)r];
+                    common = std::min<long long>(common, (long long)p.size() - 1);
+                    common = std::mismatch(first.begin(), first.begin() + common, p.begin()).first - first.begin();
+                    if (adapters && (*adapters)[(size_t)r] != (*adapters)[(size_t)batch[0]]) common = 0;
+                }
+                common = common / page * page;
+            }
+            for (int r : batch) {
+                slots[r] = common == 0 || r == batch[0] ? backend.new_sequence() : backend.fork_sequence(slots[batch[0]], common);
+                n_fed[r] = (long long)prompts[(size_t)r].size();
+                if (common == 0 || r != batch[0]) continue;
+                StepItem it;
+                it.slot = slots[r];
+                it.tokens.assign(prompts[(size_t)r].begin(), prompts[(size_t)r].begin() + common);
+                if (adapters) it.adapter = (*adapters)[(size_t)r];
+                backend.step({it}, nullptr);
+            }
             // the requests of a batch are stepped longest prompt first (all grow by one token per step, so
             // the order holds): the attention kernels hand out their blocks in the order of the step's
             // sequences, and the blocks with the most keys should start first; results are kept by request
@@ -111,8 +130,8 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
             for (int r : order) {
                 StepItem it;
                 it.slot = slots[r];
-                it.tokens = prompts[(size_t)r];
-                it.want = {(int)prompts[(size_t)r].size() - 1};
+                it.tokens.assign(prompts[(size_t)r].begin() + common, prompts[(size_t)r].end());
+                it.want = {(int)it.tokens.size() - 1};
                 if (adapters) it.adapter = (*adapters)[(size_t)r];
                 items.push_back(std::move(it));
                 hist.push_back(prompts[(size_t)r]);

@@ -52,6 +52,9 @@ public:
     virtual int read_tokens_async(const TokensRef& toks) = 0;        // a ticket
     virtual std::vector<int> finish_read(int ticket) = 0;
     virtual TokensRef select(const TokensRef& toks, const std::vector<int>& idx) = 0;   // toks[idx]
+    // The page size of a backend whose batches are to run the first positions that all their prompts have in common once; 0: they are not.
+    virtual int share_page() { return 0; }
+    virtual int fork_sequence(int slot, long long length) { throw EngineError("this backend shares no positions"); }
 };
 
 class Chooser {
@@ -84,6 +87,8 @@ public:
     int read_tokens_async(const TokensRef& t) override { return e_->read_tokens_async(t.p, t.n); }
     std::vector<int> finish_read(int ticket) override { return e_->finish_read(ticket); }
     TokensRef select(const TokensRef& toks, const std::vector<int>& idx) override;
+    int share_page() override { return e_->options().share_prefixes && e_->can_fork() ? e_->options().page_size : 0; }
+    int fork_sequence(int slot, long long length) override { return e_->fork_sequence(slot, length); }
 
 private:
     Engine* e_;

@@ -32,6 +32,8 @@ EngineOptions Model::options() const {
     o.page_size = config_.page_size;
     o.cuda_graphs = config_.cuda_graphs;
     o.gemm = config_.gemm;
+    o.cache_dtype = config_.cache_dtype;
+    o.share_prefixes = config_.share_prefixes;
     o.max_adapters = config_.max_adapters;
     o.adapter_rank = config_.adapter_rank;
     o.poison_freed_pages = config_.poison_freed_pages;

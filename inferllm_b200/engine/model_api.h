@@ -33,6 +33,8 @@ struct ModelConfig {
     int page_size = 64;
     bool cuda_graphs = true;
     std::string gemm = "auto";
+    std::string cache_dtype = "auto";
+    bool share_prefixes = false;
     int max_adapters = 0, adapter_rank = 16;
     bool poison_freed_pages = false;
     void* stream = nullptr;

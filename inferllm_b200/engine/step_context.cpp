@@ -24,7 +24,7 @@ size_t StepContextBuilder::ints(int T, int B, int K, size_t n_groups, int width)
 
 StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan& plan, const std::vector<int>& ids,
                                       const std::vector<int>& want_rows, int* into, std::vector<const int*>* tables_dev,
-                                      const StepAdapters* adapters) {
+                                      const StepAdapters* adapters, const StepPrefixes* prefixes) {
     const int B = (int)plan.slots.size(), K = (int)want_rows.size();
     int T = 0, max_q = 0;
     long long max_len = 0;
@@ -33,7 +33,8 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
         max_q = std::max(max_q, plan.q_lens[i]);
         max_len = std::max(max_len, plan.past[i] + plan.q_lens[i]);
     }
-    const size_t own = ints(T, B, K, cache.paged.size(), cache.width), total = own + (adapters ? adapters->ints() : 0);
+    const size_t own = ints(T, B, K, cache.paged.size(), cache.width), plans = adapters ? adapters->ints() : 0,
+                 total = own + pad4(plans) + (prefixes ? (size_t)prefixes->sizes.ints() : 0);
     // one asynchronous copy for all of a step's index arrays, from a small ring of pinned staging
     // buffers: the host may prepare the next steps while the GPU still runs this one, and waits only
     // when it comes back to a buffer whose copy has not left yet
@@ -83,6 +84,8 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
             off += (size_t)adapter_plan_layout(adapters->sizes[p]).total;
         }
     }
+    const size_t o_prefix = own + pad4(plans);
+    if (prefixes) ops::prefix_plan_fill(prefixes->groups, prefixes->sizes, prefixes->heads, h + o_prefix);
     int* buf = into ? into : dev_->alloc_n<int>(total);
     check_cuda(cudaMemcpyAsync(buf, h, total * sizeof(int), cudaMemcpyHostToDevice, dev_->stream()), "uploading a step's index arrays");
     check_cuda(cudaEventRecord(st.busy, dev_->stream()), "cudaEventRecord");
@@ -108,6 +111,11 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
     ctx.err = dev_->step_error_word();
     ctx.adapted = adapters != nullptr;
     for (int p = 0; adapters && p < kAdapterPieces; p++) ctx.adapters[p] = AdapterView{buf + o_plan[p], adapters->sizes[p]};
+    if (prefixes) {
+        ctx.prefix_plan = buf + o_prefix;
+        ctx.prefix = prefixes->sizes;
+        ctx.prefix_heads = prefixes->heads;
+    }
     ctx.dev = dev_;
     ctx.rt = rt_;
     ctx.q_lens = plan.q_lens;

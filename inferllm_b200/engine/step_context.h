@@ -26,6 +26,13 @@ struct StepAdapters {
     }
 };
 
+// The common prefixes of a decode step's sequences and what is set aside for their plan.
+struct StepPrefixes {
+    std::vector<ops::PrefixGroup> groups;
+    ops::PrefixPlanSizes sizes;
+    int heads = 0;                  // query heads per kv head of the layers that use it
+};
+
 class StepContextBuilder {
 public:
     StepContextBuilder(Device* dev, Runtime* rt);
@@ -36,7 +43,7 @@ public:
     // a captured graph); nullptr takes a fresh one from the step arena.  tables_dev gets, per paged
     // group of the cache, the device address of the step's page table [B, width].
     StepContext build(const SequenceCache& cache, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
-                      int* into, std::vector<const int*>* tables_dev, const StepAdapters* adapters = nullptr);
+                      int* into, std::vector<const int*>* tables_dev, const StepAdapters* adapters = nullptr, const StepPrefixes* prefixes = nullptr);
     size_t last_upload_bytes = 0;
 
 private:

@@ -128,6 +128,7 @@ int attention_pages_splits(long long pairs, long long keys, int n_sms) {
     if (pairs * 8 <= 2LL * n_sms) n = keys <= 3000 ? 8 : std::min<long long>(32, std::max<long long>(8, keys / 512));
     return (int)std::max<long long>(1, std::min<long long>({n, tiles, (long long)kRingDecodeMaxSplits}));
 }
+bool attention_pages_in_cluster(long long pairs, int splits, int n_sms) { return splits <= 8 && pairs * splits <= 2LL * n_sms; }
 int attention_prefix_splits(long long pairs, long long keys, int n_sms) {
     const long long most = std::min<long long>(kRingDecodeMaxSplits, std::max<long long>(1, ceil_div(keys, 128)));
     // (clusters of four blocks, each alone on its SM, fill seven eighths of the SMs)
@@ -1007,6 +1008,104 @@ int attention_diff_splits(long long T, int head_groups, long long max_seq_len, i
     long long s = std::max<long long>(1, 2LL * n_sms / pairs);
     s = std::min<long long>(s, std::max<long long>(1, ceil_div(max_seq_len, 256)));
     return (int)std::max<long long>(1, std::min<long long>(s, 64));
+}
+
+// ---- eight-bit entries and common prefixes
+
+static void check_cache_int8(const KVView& kv, Geometry g, const char* what) {
+    check_cache(kv, DType::U8, g, what);
+    if (!kv.k_scale || !kv.v_scale) throw KernelError(std::string(what) + ": the cache entry has no scales");
+    if (kv.v_head_dim > 0 && kv.v_head_dim != g.head_dim) throw KernelError(std::string(what) + ": values of another size than the keys are not kept in eight bits");
+}
+
+Mat kv_write_int8(Device& dev, const MatOrPartials& in, const float* cos_sin, int rot_dim, long long n_pos, const StepView& ctx, const KVView& kv, Geometry g,
+                  DType act_dtype) {
+    check_cache_int8(kv, g, "kv_write_int8");
+    if (in.cols() != (long long)(g.n_heads + 2 * g.n_kv_heads) * g.head_dim)
+        throw KernelError("qkv width " + std::to_string(in.cols()) + " is not (heads + 2 kv heads) * head_dim");
+    if (rot_dim && !cos_sin) throw KernelError("kv_write_int8: a rotation needs its cos/sin table");
+    if (!in.is_partials()) need(in.m, "qkv", true, act_dtype);
+    const long long T = in.rows();
+    Mat q = new_mat(dev, T, (long long)g.n_heads * g.head_dim, act_dtype);
+    check_kernel(illm_kv_write_int8(in.is_partials() ? nullptr : in.m.p, in.is_partials() ? in.part.ws : nullptr, in.is_partials() ? in.part.splits : 0, in.stride(), q.p,
+                                    rot_dim ? cos_sin : nullptr, ctx.token_pos, ctx.token_seq, kv.block_table, kv.width, kv.num_pages, kv.k, kv.v, kv.k_scale, kv.v_scale,
+                                    code_of(act_dtype, "kv_write_int8"), (int)T, g.n_heads, g.n_kv_heads, g.head_dim, rot_dim, kv.page_size, kv.writes ? 1 : 0,
+                                    (int)(rot_dim ? n_pos : 0), ctx.err, dev.stream()),
+                 "kv_write_int8");
+    return q;
+}
+
+// Scratch of attention_pages for `slots` shares per (token, head); the sums follow the accumulators.
+static float* shares(Device& dev, long long T, Geometry g, int slots, float** ml) {
+    float* acc = dev.alloc_n<float>((size_t)T * g.n_heads * slots * g.head_dim);
+    *ml = dev.alloc_n<float>((size_t)T * g.n_heads * slots * 2);
+    return acc;
+}
+
+Mat attention_int8(Device& dev, const Mat& q, const KVView& kv, const StepView& ctx, Geometry g, float scale) {
+    need(q, "q");
+    check_cache_int8(kv, g, "attention_int8");
+    const long long T = q.rows;
+    if (!attention_int8_tc_supported(q.dtype, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, ctx.is_decode)) {
+        Mat out = new_mat(dev, T, (long long)g.n_heads * g.head_dim, q.dtype);
+        check_kernel(illm_attention_int8(q.p, (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.block_table, kv.width, kv.num_pages, ctx.token_pos, ctx.token_seq, out.p,
+                                         code_of(q.dtype, "attention_int8"), (int)T, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, kv.span(), scale,
+                                         dev.tc_error_word(), dev.stream()),
+                     "attention_int8");
+        return out;
+    }
+    if (!ctx.is_decode) {
+        Mat out = new_mat(dev, T, (long long)g.n_heads * g.head_dim, DType::BF16);
+        check_kernel(illm_attention_tiles_int8(q.p, (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.cu_q, ctx.seq_lens, out.p,
+                                               ctx.B, ctx.max_q, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, kv.span(), scale, 0, dev.tc_error_word(),
+                                               dev.stream()),
+                     "attention_tiles_int8");
+        return out;
+    }
+    Mat out = new_mat_exact(dev, T, (long long)g.n_heads * g.head_dim, DType::BF16);
+    const long long span = std::abs((long long)kv.span()), keys = span ? std::min<long long>(ctx.max_seq_len, span) : ctx.max_seq_len;
+    for (long long t0 = 0; t0 < T; t0 += 65535) {
+        const long long n = std::min<long long>(T - t0, 65535), pairs = n * g.n_kv_heads;
+        const int splits = attention_pages_splits(pairs, keys, dev.n_sms());
+        float *acc = nullptr, *ml = nullptr;
+        if (splits > 1 && !attention_pages_in_cluster(pairs, splits, dev.n_sms())) acc = shares(dev, n, g, splits, &ml);
+        check_kernel(illm_attention_pages(row_ptr(q, t0), (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.token_pos + t0,
+                                          ctx.token_seq + t0, nullptr, nullptr, nullptr, 0, acc, ml, row_ptr(out, t0), (int)n, g.n_heads, g.n_kv_heads, g.head_dim,
+                                          kv.page_size, kv.span(), scale, splits, 0, dev.tc_error_word(), dev.stream()),
+                     "attention_pages");
+    }
+    return out;
+}
+
+bool attention_shared_supported(DType dtype, const KVView& kv, const StepView& ctx, Geometry g) {
+    return ctx.prefix_plan && ctx.prefix.tiles > 0 && kv.span() == 0 && g.n_kv_heads > 0 && g.n_heads == ctx.prefix_heads * g.n_kv_heads &&
+           (kv.v_head_dim == 0 || kv.v_head_dim == g.head_dim) && attention_int8_tc_supported(dtype, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, true);
+}
+
+Mat attention_shared(Device& dev, const Mat& q, const KVView& kv, const StepView& ctx, Geometry g, float scale) {
+    need(q, "q", true, DType::BF16);
+    if (kv.int8()) check_cache_int8(kv, g, "attention_shared");
+    else check_cache(kv, DType::BF16, g, "attention_shared");
+    if (!attention_shared_supported(q.dtype, kv, ctx, g) || ctx.prefix.T != q.rows) throw KernelError("attention_shared: the step's plan is not for these heads and tokens");
+    const long long T = q.rows;
+    const PrefixPlanSizes& s = ctx.prefix;
+    Mat out = new_mat_exact(dev, T, (long long)g.n_heads * g.head_dim, DType::BF16);
+    const int own = attention_pages_splits(T * g.n_kv_heads, std::max(1, s.longest_rest), dev.n_sms());
+    const long long pairs = (long long)s.tiles * g.n_kv_heads;
+    const int pre = s.wide ? attention_prefix_splits(pairs, s.longest_prefix, dev.n_sms()) : attention_pages_splits(pairs, s.longest_prefix, dev.n_sms());
+    const int kept = s.wide ? pre / illm_attention_tiles_cluster(pre) : pre;
+    float *ml, *acc = shares(dev, T, g, own + kept, &ml);
+    const int *start = ctx.prefix_plan + s.start_at(), *members = ctx.prefix_plan + s.members_at();
+    if (s.wide)
+        check_kernel(illm_attention_tiles_prefix(q.p, (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.token_seq, ctx.prefix_plan,
+                                                 members, s.tiles, acc, ml, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, scale, own + kept, own, pre,
+                                                 dev.tc_error_word(), dev.stream()),
+                     "attention_tiles_prefix");
+    check_kernel(illm_attention_pages(q.p, (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.token_pos, ctx.token_seq, start,
+                                      ctx.prefix_plan, members, s.wide ? 0 : s.tiles, acc, ml, out.p, (int)T, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, 0, scale,
+                                      own, kept, dev.tc_error_word(), dev.stream()),
+                 "attention_pages");
+    return out;
 }
 
 Mat attention(Device& dev, const Mat& qkv, const KVView& kv, const StepView& ctx, Geometry g, float scale) {

@@ -14,6 +14,7 @@
 #include "cache/cache.h"
 #include "csrc/adapters.h"
 #include "device/device.h"
+#include "kernels/prefix_plan.h"
 
 namespace illm {
 
@@ -87,6 +88,10 @@ struct StepView {
     int* err = nullptr;               // the step's error word
     bool adapted = false;             // some of the step's sequences have a low-rank adapter: adapters[p - 1] is the plan for
     AdapterView adapters[kAdapterPieces];      // projections packed of p pieces
+    // a decode step whose sequences hold first positions in common: the plan (kernels/prefix_plan.h) for layers with prefix_heads query heads per kv head
+    const int* prefix_plan = nullptr;
+    ops::PrefixPlanSizes prefix;
+    int prefix_heads = 0;
 };
 
 namespace ops {
@@ -140,6 +145,8 @@ int attention_prefix_splits(long long pairs, long long keys, int n_sms);
 // The tensor-core kernels over rows of eight bits: bfloat16 queries, head size 64 or 128, pages of a multiple of 64 positions; single tokens
 // also need at most 16 query heads per kv head.
 bool attention_int8_tc_supported(DType dtype, int nh, int nkv, int d, int page_size, bool decode);
+// Whether the blocks of a (token, kv head) of attention_pages join their shares as a cluster (all of them find room at once), or a second kernel does.
+bool attention_pages_in_cluster(long long pairs, int splits, int n_sms);
 bool attention_decode_ring_supported(DType dtype, int nh, int nkv, int d, int page_size);
 bool attention_decode_supported(DType dtype, int nh, int nkv, int d, int page_size);
 bool attention_decode_gqa_supported(DType dtype, int nh, int nkv, int d);
@@ -211,6 +218,16 @@ struct Geometry { int n_heads, n_kv_heads, head_dim; };
 // as unreduced slices, a new one (the slices are added up on the way).
 Mat rope_kv_write(Device& dev, const MatOrPartials& qkv, const float* cos_sin, int rot_dim, long long n_pos, const StepView& ctx,
                   const KVView& kv, Geometry g);
+// Rotate Q and K of the packed projection (finished or as unreduced slices) and store K and V in the pages of an eight-bit cache entry; returns the rotated
+// queries [T, n_heads * head_dim], a new matrix (csrc/kv_int8.cu).
+Mat kv_write_int8(Device& dev, const MatOrPartials& qkv, const float* cos_sin, int rot_dim, long long n_pos, const StepView& ctx, const KVView& kv, Geometry g,
+                  DType act_dtype);
+// Attention over an eight-bit cache entry, prompts or single tokens, window or chunk included: the tensor-core kernels where they take the sizes
+// (attention_int8_tc_supported), the plain one otherwise.
+Mat attention_int8(Device& dev, const Mat& q, const KVView& kv, const StepView& ctx, Geometry g, float scale);
+// Attention of a decode step with a plan of common prefixes over a bfloat16 or eight-bit entry: their keys are read once for a group.
+bool attention_shared_supported(DType dtype, const KVView& kv, const StepView& ctx, Geometry g);
+Mat attention_shared(Device& dev, const Mat& q, const KVView& kv, const StepView& ctx, Geometry g, float scale);
 // Options of the attention kernels beyond the plain softmax attention: a per-head sink in the softmax denominator
 // (float32 [n_heads]; zeros add one to it), an output gate, sigmoid(gate[t * gate_stride + h]) for whole heads or, with
 // wide_gate, sigmoid(gate[t * gate_stride + h * dv + c]) element by element (float32), and a soft cap on the scaled

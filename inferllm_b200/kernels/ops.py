@@ -1104,12 +1104,10 @@ def pages_splits(pairs, keys, wide, n_sms) -> int:
     return int(_b.lib().illm_policy_pages_splits(int(pairs), int(keys), int(wide), int(n_sms)))
 
 
-MAX_CLUSTER_SPLITS = 8
-
-
-def _in_cluster(pairs, splits, device):
-    """Whether the blocks of a (token, kv head) join their shares in a cluster (the engine's rule): where all blocks find room at once."""
-    return splits <= MAX_CLUSTER_SPLITS and pairs * splits <= 2 * _sms[device.index]
+@functools.lru_cache(maxsize=4096)
+def _in_cluster(pairs, splits, n_sms):
+    """Whether the blocks of a (token, kv head) join their shares as a cluster (`ops::attention_pages_in_cluster`)."""
+    return bool(_b.lib().illm_policy_pages_in_cluster(pairs, splits, n_sms))
 
 
 def _shares(T, n_heads, slots, d, device):
@@ -1144,7 +1142,7 @@ def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, 
             n = min(T - t0, 65535)
             s = _splits(n * nkv, keys, False, device)
             s = s if splits is None else int(splits)
-            ws, acc, ml = (None, None, None) if s == 1 or _in_cluster(n * nkv, s, device) else _shares(n, n_heads, s, d, device)
+            ws, acc, ml = (None, None, None) if s == 1 or _in_cluster(n * nkv, s, _sms[device.index]) else _shares(n, n_heads, s, d, device)
             _check(run(q.data_ptr() + t0 * stride * 2, stride, *cache.pointers, cache.pages, block_table.data_ptr(), width, token_pos.data_ptr() + 4 * t0,
                        token_seq.data_ptr() + 4 * t0, None, None, None, 0, acc, ml, out.data_ptr() + t0 * n_heads * d * 2, n, n_heads, nkv, d, cache.page_size, span,
                        float(scale), s, 0, err, stream), "attention_decode_int8")

@@ -96,7 +96,17 @@ void DecoderModel::put_adapter(int i, const AdapterFactors& f) {
     }
 }
 
-std::map<int, CacheRequest> DecoderModel::cache_requests() const {
+int DecoderModel::prefix_heads() const {
+    int heads = 0;
+    for (const Layer& l : layers_) {
+        const int n = l.mixer->prefix_heads();
+        if (n && heads && n != heads) return 0;
+        if (n) heads = n;
+    }
+    return heads;
+}
+
+std::map<int, CacheRequest> DecoderModel::cache_requests(bool int8) const {
     std::map<int, CacheRequest> out;
     for (const ScheduleEntry& e : spec.schedule)
         if (e.writes) {
@@ -111,6 +121,15 @@ std::map<int, CacheRequest> DecoderModel::cache_requests() const {
         const Mixer::Reach r = layers_[(size_t)e.layer].mixer->reach();
         auto it = out.find(e.cache);
         if (r.known && it != out.end() && it->second.kind == CacheRequest::PagedKV) it->second = it->second.reaching(r.window, r.chunk);
+    }
+    if (int8) {
+        std::map<int, bool> takes;
+        for (const ScheduleEntry& e : spec.schedule) {
+            const bool t = layers_[(size_t)e.layer].mixer->takes_int8_cache();
+            takes[e.cache] = takes.count(e.cache) ? takes[e.cache] && t : t;
+        }
+        for (auto& r : out)
+            if (r.second.kind == CacheRequest::PagedKV && !r.second.keys_only && takes[r.first]) r.second = r.second.in_int8();
     }
     const CacheRequest er = embedding_->cache_request();
     if (er.kind != CacheRequest::None) out[kEmbeddingCacheEntry] = er;

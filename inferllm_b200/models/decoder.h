@@ -39,7 +39,10 @@ public:
     // them, one part at a time.
     void load_tensors(const std::function<std::unique_ptr<TensorSource>(const std::string& prefix)>& open);
     // Cache entry number -> what its writing layer's mixer asks for.
-    std::map<int, CacheRequest> cache_requests() const;
+    // int8: keys and values in eight bits wherever every layer that uses the entry can (Mixer::takes_int8_cache).
+    std::map<int, CacheRequest> cache_requests(bool int8 = false) const;
+    // Query heads per kv head of the layers that walk common prefixes once (Mixer::prefix_heads); 0: no layer does, or they differ.
+    int prefix_heads() const;
     // Run the tokens of one step; float32 logits [ctx.K, vocab] (rows == 0 when nothing is wanted).
     Mat forward(const StepContext& ctx, const SequenceCache& cache, const std::vector<const int*>& tables_dev);
     // Low-rank adapters: the names (as in the weight file) of the matrices beside which they can stand, with their shapes; room

@@ -649,6 +649,17 @@ struct Attention : Mixer {
         return own_kv ? CacheRequest::paged(n_kv_heads, maps * head_dim, window, v_head_dim).in_chunks(chunk) : CacheRequest();
     }
 
+    bool takes_int8_cache() const override {
+        const float* table = nullptr;
+        int rot = 0;
+        long long n_pos = 0;
+        return !values_are_keys && !general() && head_dim % 8 == 0 && head_dim <= 256 && position->rotation_table(&table, &rot, &n_pos);
+    }
+    int prefix_heads() const override {
+        return !values_are_keys && !general() && window == 0 && rt && ops::attention_int8_tc_supported(rt->dtype, n_heads, n_kv_heads, head_dim, rt->page_size, true)
+                       ? n_heads / n_kv_heads
+                       : 0;
+    }
     Reach reach() const override {
         Reach r;
         r.known = true;
@@ -774,6 +785,18 @@ struct Attention : Mixer {
         int rot = 0;
         long long n_pos = 0;
         const bool rotation = position->rotation_table(&table, &rot, &n_pos);
+        if (kv.int8()) {
+            MatOrPartials qkv = project_qkv(h, ctx, true);
+            Mat q = ops::kv_write_int8(dev, qkv, table, rot, n_pos, ctx, kv, g, h.dtype);
+            Mat o = ctx.is_decode && ops::attention_shared_supported(h.dtype, kv, ctx, g) ? ops::attention_shared(dev, q, kv, ctx, g, scale)
+                                                                                          : ops::attention_int8(dev, q, kv, ctx, g, scale);
+            return project_o(o, ctx, may_defer);
+        }
+        if (ctx.is_decode && ops::attention_shared_supported(h.dtype, kv, ctx, g)) {
+            MatOrPartials qkv = project_qkv(h, ctx, position->takes_partials());
+            Mat q = position->encode_and_store(qkv, g, ctx, kv);
+            return project_o(ops::attention_shared(dev, q, kv, ctx, g, scale), ctx, may_defer);
+        }
         if (ctx.is_decode && rotation && rot % 16 == 0 && ops::attention_decode_ring_supported(h.dtype, n_heads, n_kv_heads, head_dim, kv.page_size)) {
             // one token per sequence: the attention kernel itself adds up the K slices of the projection,
             // rotates Q and the new K row and writes K and V into the cache

@@ -271,6 +271,11 @@ public:
     // A second cache entry, of fixed per-sequence state, beside the first (a mixer with keys and values AND a few
     // rows of state, say): the decoder gives it an entry number of its own and hands it over as CacheView::aux.
     virtual CacheRequest aux_cache_request() const { return CacheRequest(); }
+    // true: the mixer can write and read its keys and values in eight bits (KVView::int8)
+    virtual bool takes_int8_cache() const { return false; }
+    // Query heads per kv head of a mixer whose decode steps can walk positions that sequences hold in common once for all of them
+    // (StepView::prefix_plan); 0: it cannot, and reads them for every sequence.
+    virtual int prefix_heads() const { return 0; }
     // Which earlier positions the mixer's queries see (0, 0: all; as in CacheRequest), for a mixer that attends to keys and
     // values which another layer wrote: the cache keeps every position that one of the entry's readers still needs.
     struct Reach { bool known = false; int window = 0, chunk = 0; };

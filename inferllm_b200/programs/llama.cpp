@@ -56,6 +56,8 @@ static const char* kHelp =
     "  --prompt-ids IDS         comma-separated token ids (repeatable)\n"
     "  --prompt-file FILE       one request (comma- or space-separated ids) per line\n"
     "  --random-prompts LENS    comma-separated prompt lengths of random ids\n"
+    "  --cache-dtype TYPE       keys and values: auto (as the compute dtype) | int8 (default auto)\n"
+    "  --share-prefixes         run the first tokens that all requests have in common once\n"
     "  --max-tokens N           tokens the cache holds (default: fits all requests at once, up to 64 Ki)\n"
     "  --config FILE            config.json for --random-weights / --write-random-model\n"
     "  --random-weights SEED    run a model with random weights made on the device\n"
@@ -67,6 +69,8 @@ static int run(int argc, char** argv) {
     long long ctx = 2048, seed = -1, n_predict = 128, max_tokens = 0, random_weights = 0;
     int top_k = 40, repeat_last_n = 64, threads = 4;
     float top_p = 0.95f, temp = 0.10f, repeat_penalty = 1.30f;
+    std::string cache_dtype = "auto";
+    bool share_prefixes = false;
     bool has_random_weights = false, no_stop = false, mmap_flag = false;
     std::vector<std::string> prompt_ids;
     for (int i = 1; i < argc; i++) {
@@ -93,6 +97,8 @@ static int run(int argc, char** argv) {
         else if (a == "--prompt-ids") prompt_ids.push_back(value());
         else if (a == "--prompt-file") prompt_file = value();
         else if (a == "--random-prompts") random_prompts = value();
+        else if (a == "--cache-dtype") cache_dtype = value();
+        else if (a == "--share-prefixes") share_prefixes = true;
         else if (a == "--max-tokens") max_tokens = atoll(value().c_str());
         else if (a == "--config") config_file = value();
         else if (a == "--random-weights") { random_weights = atoll(value().c_str()); has_random_weights = true; }
@@ -168,6 +174,8 @@ static int run(int argc, char** argv) {
     mc.nr_ctx = (unsigned)ctx;
     mc.device_id = device_id;
     mc.enable_mmap = mmap_flag;
+    mc.cache_dtype = cache_dtype;
+    mc.share_prefixes = share_prefixes;
     mc.max_tokens = max_tokens > 0 ? max_tokens : std::min<long long>(need, 65536);
     Model model(mc);
     if (has_random_weights && cfg) {

@@ -36,7 +36,7 @@ inline bool dtype_from_name(const std::string& s, DType* out) {
 inline const char* dtype_word(DType t) {   // the names of config.json and of the command lines
     switch (t) {
         case DType::F32: return "float32"; case DType::BF16: return "bfloat16"; case DType::F16: return "float16";
-        case DType::I32: return "int32"; default: return dtype_name(t);
+        case DType::I32: return "int32"; case DType::U8: return "uint8"; default: return dtype_name(t);
     }
 }
 

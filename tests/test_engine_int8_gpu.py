@@ -1,0 +1,259 @@
+"""The engine with a cache of eight-bit rows, and sequences that share their first positions (GPU).
+
+The plain implementation is given the same rounding of keys and values.  A value that lies on the border between two steps may
+fall to either side in the engine, which moves it by 1/127 of its row's largest: less than what rounding every activation to bfloat16 does, whose bounds
+therefore serve the float32 mode here too."""
+import subprocess
+
+import numpy as np
+import plain_llama as plain
+import pytest
+import torch
+from conftest import ROOT, TINY, random_prompt
+from util import assert_close
+
+from inferllm_b200 import CacheError, Engine, EngineError, EngineOptions, Model, ModelConfig, StepItem
+from inferllm_b200.kernels import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def eight_bits(x):
+    s = np.abs(x).max(-1, keepdims=True) / 127
+    return np.rint(x / np.where(s > 0, s, 1)) * s
+
+
+@pytest.fixture
+def rounded(monkeypatch):
+    """The plain implementation over keys and values of eight bits."""
+    scores, values = plain.attention_scores, plain.weighted_values
+    monkeypatch.setattr(plain, "attention_scores", lambda q, k, *a: scores(q, eight_bits(k), *a))
+    monkeypatch.setattr(plain, "weighted_values", lambda p, v, *a: values(p, eight_bits(v), *a))
+
+
+def engine(folder, dtype="bfloat16", cache="int8", **kw):
+    return Engine.from_folder(folder, EngineOptions(dtype=dtype, cache_dtype=cache, max_tokens=kw.pop("max_tokens", 4096), max_batch=kw.pop("max_batch", 16), **kw))
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "B", "C", "D"])
+def test_logits(name, dtype, graphs, model_folders, plain_models, rounded):
+    """Three prompts in one step, then single tokens (the second such step is captured, the others replay it)."""
+    cfg, w = plain_models[name]
+    e = engine(model_folders[name], dtype, cuda_graphs=graphs, poison_freed_pages=True)
+    prompts, after = [random_prompt(name, n, 30 + n) for n in (17, 70, 9)], [random_prompt(name, 5, 40 + i) for i in range(3)]
+    slots = [e.new_sequence() for _ in prompts]
+    got, at = e.step([StepItem(s, p, list(range(len(p)))) for s, p in zip(slots, prompts)]).cpu().numpy(), 0
+    for p in prompts:
+        assert_close(got[at:at + len(p)], plain.forward(cfg, w, p), "bfloat16", "prompt")
+        at += len(p)
+    want = [plain.forward(cfg, w, p + t)[len(p):] for p, t in zip(prompts, after)]
+    for j in range(5):
+        got = e.step([StepItem(s, [t[j]], [0]) for s, t in zip(slots, after)]).cpu().numpy()
+        for i in range(3):
+            assert_close(got[i:i + 1], want[i][j:j + 1], "bfloat16", f"token {j} of request {i}")
+    e.check_device_errors()
+    # a page that comes back from the pool is another sequence's no more
+    for s in slots:
+        e.end_sequence(s)
+    p = random_prompt(name, 33, 77)
+    assert_close(e.step([StepItem(e.new_sequence(), p, list(range(33)))]).cpu().numpy(), plain.forward(cfg, w, p), "bfloat16", "reused pages")
+    e.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["B", "C", "D"])
+def test_a_prompt_in_pieces(name, dtype, model_folders):
+    """At once, in pieces and token by token: the same rows end up in the cache.  Single prompts are padded and replayed from graphs too."""
+    e = engine(model_folders[name], dtype)
+    p = random_prompt(name, 130, 5)
+    for _ in range(3):
+        whole = e.step([StepItem(s := e.new_sequence(), p, [129])])
+        e.end_sequence(s)
+    s = e.new_sequence()
+    for a, b in ((0, 50), (50, 51), (51, 129)):
+        e.step([StepItem(s, p[a:b], [])])
+    pieces = e.step([StepItem(s, p[129:], [0])])
+    s = e.new_sequence()
+    for t in p[:-1]:
+        e.step([StepItem(s, [t], [])])
+    singles = e.step([StepItem(s, p[-1:], [0])])
+    e.check_device_errors()
+    for other in (pieces, singles):
+        assert_close(other.cpu().numpy(), whole.cpu().numpy(), "bfloat16")
+
+
+def test_what_lies_in_the_cache(model_folders, plain_models):
+    """The first layer's rows: the plain implementation's keys and values in eight bits."""
+    name = "C"
+    cfg, w = plain_models[name]
+    e = engine(model_folders[name], "float32")
+    p = random_prompt(name, 100, 3)
+    s = e.new_sequence()
+    e.step([StepItem(s, p, [99])])
+    k, v, ks, vs = e.cache_tensors(0)
+    assert k.dtype == torch.uint8 and ks.shape == k.shape[:-1]
+    layer = ops.CacheInt8(k[0], v[0], ks[0], vs[0])
+    pages = e.cache.pages_of(0, s)
+    table = torch.tensor([[pages[i] for i in range(2)]], dtype=torch.int32).cuda()
+    got = ops.kv_read_int8(layer, torch.arange(100, dtype=torch.int32).cuda(), torch.zeros(100, dtype=torch.int32).cuda(), table, torch.float32)
+    h = plain.rms_norm(plain.embed(p, w["model.embed_tokens.weight"]), w["model.layers.0.input_layernorm.weight"], cfg["rms_norm_eps"])
+    shape = (100, cfg["num_key_value_heads"], cfg["head_dim"])
+    want_k = plain.rope_rotate_half(plain.linear(h, w["model.layers.0.self_attn.k_proj.weight"]).reshape(shape), np.arange(100), cfg["rope_theta"])
+    want_v = plain.linear(h, w["model.layers.0.self_attn.v_proj.weight"]).reshape(shape)
+    for g, x in zip(got, (want_k, want_v)):
+        # half a step, and float32's way to the row (a few hundred roundings of 2^-24)
+        step = np.abs(x).max(-1, keepdims=True) / 127
+        assert (np.abs(g.cpu().numpy() - x) <= step * (0.5 + 0.01)).all()
+
+
+# ---------------------------------------------------------------- shared positions
+
+SHARED = {"C": (640, 512), "D": (400, 320)}
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("cache", ["auto", "int8"])
+@pytest.mark.parametrize("name", ["C", "D"])
+@pytest.mark.parametrize("n", [4, 14])
+def test_forks_answer_as_if_they_were_alone(name, cache, graphs, n, model_folders, plain_models, monkeypatch, request):
+    """Sequences that share a prefix with the one that made it, each with tokens of its own, beside one that shares nothing: enough of them that their
+    steps walk the prefix once (4: rows of one narrow tile's size, 14: wide ones)."""
+    if cache == "int8":
+        request.getfixturevalue("rounded")
+    cfg, w = plain_models[name]
+    e = engine(model_folders[name], cache=cache, cuda_graphs=graphs, max_tokens=8192, max_batch=n + 3)
+    prompt = random_prompt(name, SHARED[name][0], 11)
+    common = SHARED[name][1]
+    slots = [e.new_sequence()]
+    e.step([StepItem(slots[0], prompt, [])])
+    slots += [e.fork_sequence(slots[0], common) for _ in range(n - 1)]
+    texts = [prompt] + [prompt[:common] + random_prompt(name, 3 + i, 200 + i) for i in range(n - 1)]
+    lone = random_prompt(name, 21, 12)
+    slots.append(e.new_sequence())
+    texts.append(lone)
+    # the forks' own tokens as short prompts
+    items = [StepItem(s, t[common:], [len(t) - common - 1]) for s, t in zip(slots[1:n], texts[1:n])] + [StepItem(slots[n], lone, [20])]
+    got = e.step(items).cpu().numpy()
+    some = [1, n - 1, n]
+    for i in some:
+        assert_close(got[i - 1:i], plain.forward(cfg, w, texts[i])[-1:], "bfloat16", f"prompt of {i}")
+    for j in range(4):
+        tokens = [random_prompt(name, 1, 300 + 20 * j + i) for i in range(n + 1)]
+        texts = [t + x for t, x in zip(texts, tokens)]
+        got = e.step([StepItem(s, x, [0]) for s, x in zip(slots, tokens)]).cpu().numpy()
+        for i in [0] + some:
+            assert_close(got[i:i + 1], plain.forward(cfg, w, texts[i])[-1:], "bfloat16", f"token {j} of {i}")
+    e.check_device_errors()
+    # the sequence that made the prefix ends first, in a step of other sizes
+    e.end_sequence(slots[0])
+    tokens = [random_prompt(name, 1, 500 + i) for i in range(n + 1)]
+    texts = [t + x for t, x in zip(texts, tokens)]
+    order = list(range(n, 0, -1))
+    got = e.step([StepItem(slots[i], tokens[i], [0]) for i in order]).cpu().numpy()
+    for i in some:
+        at = order.index(i)
+        assert_close(got[at:at + 1], plain.forward(cfg, w, texts[i])[-1:], "bfloat16", f"after the end, {i}")
+    e.check_device_errors()
+    for s in slots[1:]:
+        e.end_sequence(s)
+    e.cache.check()
+    assert e.cache.pages_free() == [e.limits().num_pages]
+
+
+@pytest.mark.parametrize("name, dtype, cache", [("A", "float32", "int8"), ("B", "float32", "auto"), ("B", "bfloat16", "int8"), ("D", "float32", "int8")])
+def test_forks_on_the_plain_kernels(name, dtype, cache, model_folders):
+    """Sizes and types that read a shared prefix for every sequence: a fork answers as the same tokens in a sequence of their own."""
+    e = engine(model_folders[name], dtype, cache=cache, page_size=16)
+    prompt, tail = random_prompt(name, 70, 1), random_prompt(name, 6, 2)
+    a, b = e.new_sequence(), e.new_sequence()
+    e.step([StepItem(a, prompt, [])])
+    e.step([StepItem(b, prompt[:64], [])])
+    c = e.fork_sequence(a, 64)
+    for t in tail:
+        got = e.step([StepItem(b, [t], [0]), StepItem(c, [t], [0])]).cpu()
+        assert_close(got[:1].numpy(), got[1:].numpy(), dtype)
+    e.check_device_errors()
+
+
+def test_generate_runs_common_positions_once(model_folders):
+    """The same tokens with and without, in float32, where a row's result does not depend on what else is in the step; and fewer tokens to run."""
+    name = "C"
+    head = random_prompt(name, 150, 1)
+    prompts = [head + random_prompt(name, 2 + i, 50 + i) for i in range(5)] + [head[:149]]
+    results = []
+    for share in (False, True):
+        m = Model(ModelConfig(compt_type="float32", nr_ctx=512, max_tokens=4096, share_prefixes=share))
+        m.load(model_folders[name])
+        m.init(top_k=40, top_p=0.95, temp=0.0, repeat_penalty=1.0, repeat_last_n=64, seed=1, end_token=2)
+        results.append(m.generate(prompts, max_new_tokens=8, stop_ids=[]).tokens)
+        m.engine.check_device_errors()
+        assert m.engine.cache.pages_free() == [m.engine.limits().num_pages]
+    assert results[0] == results[1]
+    # bfloat16 and eight bits together, one request alone, prompts that have nothing in common
+    m = Model(ModelConfig(nr_ctx=512, max_tokens=4096, share_prefixes=True, cache_dtype="int8"))
+    m.load(model_folders[name])
+    m.init(top_k=40, top_p=0.95, temp=0.0, repeat_penalty=1.0, repeat_last_n=64, seed=1, end_token=2)
+    for ps in (prompts, prompts[:1], [random_prompt(name, 70, 9), random_prompt(name, 80, 10)], [head, head, head]):
+        out = m.generate(ps, max_new_tokens=6, stop_ids=[])
+        assert [len(t) for t in out.tokens] == [6] * len(ps)
+        m.engine.check_device_errors()
+    assert out.tokens[0] == out.tokens[1] == out.tokens[2]
+
+
+def test_adapters_and_shared_positions(model_folders):
+    """Requests with different adapters share nothing: an adapter makes keys of its own."""
+    name = "C"
+    head = random_prompt(name, 150, 1)
+    prompts = [head + random_prompt(name, 2 + i, 50 + i) for i in range(3)]
+    tokens = []
+    for share in (False, True):
+        m = Model(ModelConfig(compt_type="float32", nr_ctx=512, max_tokens=4096, share_prefixes=share, max_adapters=2, adapter_rank=4))
+        m.load(model_folders[name])
+        m.init(top_k=40, top_p=0.95, temp=0.0, repeat_penalty=1.0, repeat_last_n=64, seed=1, end_token=2)
+        g = torch.Generator().manual_seed(3)
+        numbers = []
+        for _ in range(2):
+            names = {k: v for k, v in m.engine.adapted().items() if "k_proj" in k or "v_proj" in k}
+            numbers.append(m.engine.add_adapter({k: (torch.randn((4, v[1]), generator=g) * v[1] ** -0.5, torch.randn((v[0], 4), generator=g) * 0.2) for k, v in names.items()}))
+        tokens.append([m.generate(prompts, 6, stop_ids=[], adapters=a).tokens for a in ([numbers[0], numbers[1], -1], [numbers[1]] * 3)])
+        m.engine.check_device_errors()
+    assert tokens[0] == tokens[1]
+
+
+def test_the_cache_takes_half_the_room(model_folders):
+    pages = [engine(model_folders["C"], cache=c, max_tokens=None, mem_fraction=0.02, max_batch=4).limits().num_pages for c in ("auto", "int8")]
+    assert 1.85 <= pages[1] / pages[0] <= 2 * 128 / 132 + 0.01
+
+
+def test_refusals(model_folders):
+    with pytest.raises(EngineError, match="cache_dtype"):
+        engine(model_folders["A"], cache="int4")
+    with pytest.raises(EngineError, match="eight bits"):
+        Engine.from_config(_windowless_none(), EngineOptions(cache_dtype="int8", max_tokens=256))
+    e = engine(model_folders["D"])
+    s = e.new_sequence()
+    e.step([StepItem(s, random_prompt("D", 100, 1), [])])
+    for length in (0, 1, 63, 65, 128, -64):
+        with pytest.raises(CacheError):
+            e.fork_sequence(s, length)
+    with pytest.raises(CacheError):
+        e.fork_sequence(s + 1, 64)
+    assert e.sequence_length(e.fork_sequence(s, 64)) == 64
+
+
+def _windowless_none():
+    """A model none of whose layers keeps plain keys and values."""
+    from plain_kudonex import random_config
+    from inferllm_b200 import config_from_dict
+    return config_from_dict(random_config(("mlstm", "attention")))
+
+
+def test_command_line(model_folders):
+    out = subprocess.run([f"{ROOT}/bin/llama", "-m", model_folders["C"], "-g", "GPU", "--prompt-ids", ",".join(map(str, range(1, 80))), "--prompt-ids",
+                          ",".join(map(str, range(1, 70))), "-n", "4", "--temp", "0", "--cache-dtype", "int8", "--share-prefixes", "-c", "256", "--no-stop"],
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    bad = subprocess.run([f"{ROOT}/bin/llama", "-m", model_folders["C"], "--prompt-ids", "1,2", "-n", "1", "--cache-dtype", "int3"], capture_output=True, text=True, timeout=300)
+    assert bad.returncode != 0 and "cache_dtype" in bad.stderr
