@@ -30,6 +30,7 @@
 #define TL_TMA_WARP 10
 #define TL_WIDEN_WARP 11                // the first of four
 #define TL_ERR_PAGE 8
+#define TL_ORDERED 128                  // sequences that are put in order
 #define TL_CLUSTER 4                    // parts of a prefix that join their shares: of clusters of eight such blocks only 15 find room, of four 33
 #define TL_RESCALE_STEP 8.0f
 
@@ -168,9 +169,25 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         nb[0] = n_rows > 0 ? n : 0;
         nb[1] = n_rows > TL_BM ? n : 0;
     } else {
-        // blocks with the most keys before them start first
+        // Blocks with the most keys before them start first: the longest sequences (of up to 128, by counting those that come before), and of each the last tile.
+        // (Sixteen unequal prompts of 2,048 tokens together, in the order of the step: 75 us.)
         hk = blockIdx.x;
         seq = blockIdx.z;
+        if (gridDim.z > 1 && gridDim.z <= TL_ORDERED) {
+            int* chosen = reinterpret_cast<int*>(holder + 1);
+            const int n = gridDim.z, b = threadIdx.x;
+            if (b < n) {
+                const int len = work.seq_lens[b];
+                int before = 0;
+                for (int j = 0; j < n; j++) {
+                    const int other = work.seq_lens[j];
+                    before += other > len || (other == len && j < b);
+                }
+                if (before == (int)blockIdx.z) *chosen = b;
+            }
+            __syncthreads();
+            seq = *chosen;
+        }
         token0 = work.cu_q[seq];
         const int q_len = work.cu_q[seq + 1] - token0, all_rows = q_len * G;
         past = work.seq_lens[seq] - q_len;
