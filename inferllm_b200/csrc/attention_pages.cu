@@ -100,7 +100,7 @@ __device__ __forceinline__ void pg_bulk(unsigned dst, const void* src, unsigned 
 }  // namespace
 
 // A plan of common prefixes (attention_decode_shared): int32 on the device.  `start` [T]: the positions that a token leaves to its
-// group; `tiles` [n_tiles][4]: first member, number of members, positions of the prefix, 0; `members`: tokens.
+// group; `tiles` [n_tiles][4]: number of members, positions of the prefix, 0, 0; `members` [n_tiles][16 / (nh / nkv)]: tokens.
 struct PgPlan {
     const int* start;
     const int4* tiles;
@@ -152,9 +152,9 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     int t = 0, first = 0, count = 1, p, lo = 0;
     if (prefix) {
         const int4 tile = plan.tiles[item];
-        first = tile.x;
-        count = tile.y;
-        p = tile.z - 1;
+        first = item * (16 / G);
+        count = tile.x;
+        p = tile.y - 1;
         if (count <= 0 || p < 0) return;
         t = plan.members[first];
     } else {

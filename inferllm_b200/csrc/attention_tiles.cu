@@ -38,8 +38,8 @@
 struct TlWork {
     const int *cu_q, *seq_lens;         // prompts: [B + 1], [B]
     int span, tile_rows;                // tile_rows: rows of a block, 128 (its first tile alone) or 256
-    const int4* tiles;                  // prefixes: first member, number of members, positions, 0
-    const int *members, *token_seq;
+    const int4* tiles;                  // prefixes: members, positions, 0, 0
+    const int *members, *token_seq;     // 256 / (nh / nkv) places for the members of each tile
     int slots, slot0;                   // shares of a (token, head) and the first of them that is the prefix's
     int cluster;                        // blocks (parts of a prefix) that join their shares
     float *part_acc, *part_ml;
@@ -103,7 +103,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     constexpr unsigned S_COL = 2 * D, P_COL = S_COL + 2 * TL_BN, Q_COL = P_COL + TL_BN, TMEM_COLS = 512;
     constexpr bool BOTH_Q = Q_COL + D <= TMEM_COLS;
     constexpr int SHARE_ROW = (D + 4) * 4;      // bytes of a row of a prefix's share: accumulators, maximum and sum
-    static_assert(!PREFIX || 2 * TL_BM * SHARE_ROW <= 2 * Z::Q_TILE + STAGES * 2 * TILE + Z::RAW * 2 * Z::RAW_TILE, "the shares must fit the tiles' memory");
+    static_assert(!PREFIX || 2 * TL_BM * (SHARE_ROW + TL_CLUSTER * 4) <= 2 * Z::Q_TILE + STAGES * 2 * TILE + Z::RAW * 2 * Z::RAW_TILE, "the shares must fit the tiles' memory");
     constexpr unsigned IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(TL_BN >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     constexpr unsigned IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(D >> 3) << 17) | ((unsigned)(TL_BM >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -153,18 +153,21 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
     // ---- which rows and keys
     const int G = nh / nkv;
+    int member0 = 0;
     int hk, row0 = 0, n_rows, token0, past = 0, seq, jb0, last_key, nb[2], first_key;       // of the block: its rows, from row0 of its (sequence or tile)'s
     int4 tile = make_int4(0, 0, 0, 0);
     if (PREFIX) {
         hk = blockIdx.y;
+        member0 = blockIdx.z * (2 * TL_BM / G);
+        const int first_member = work.members[member0];
         tile = work.tiles[blockIdx.z];
-        n_rows = tile.y > 0 && tile.z > 0 ? tile.y * G : 0;
+        n_rows = tile.x > 0 && tile.y > 0 ? tile.x * G : 0;
         token0 = 0;
-        seq = n_rows ? work.token_seq[work.members[tile.x]] : 0;
-        const int all = (tile.z + TL_BN - 1) / TL_BN, per = (all + gridDim.x - 1) / gridDim.x;
+        seq = n_rows ? work.token_seq[first_member] : 0;
+        const int all = (tile.y + TL_BN - 1) / TL_BN, per = (all + gridDim.x - 1) / gridDim.x;
         jb0 = blockIdx.x * per;
         first_key = jb0 * TL_BN;
-        last_key = tile.z - 1;
+        last_key = tile.y - 1;
         const int n = max(0, min(per, all - jb0));
         nb[0] = n_rows > 0 ? n : 0;
         nb[1] = n_rows > TL_BM ? n : 0;
@@ -342,7 +345,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         int token = 0, h = hk * G, pos = last_key;
         if (valid) {
             if (PREFIX) {
-                token = work.members[tile.x + br / G];
+                token = work.members[member0 + br / G];
                 h = hk * G + br % G;
             } else {
                 const int i = (row0 + br) / G;
@@ -353,29 +356,35 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         const unsigned lane_addr = tmem + ((unsigned)((warp & 3) * 32) << 16), s_addr = lane_addr + S_COL + w * TL_BN, p_addr = lane_addr + P_COL + w * (TL_BN / 2),
                        o_addr = lane_addr + w * D;
-        // the row's query into tensor memory or, the second tile's, into a swizzled tile of shared memory; rows behind the last one are zeros
+        // the queries into a swizzled tile of shared memory, whole rows at a time, and the first tile's from there into tensor memory; rows behind the last one are
+        // zeros
         {
-            const bf16* src = q + (size_t)token * q_stride + (size_t)h * D;
-#pragma unroll
-            for (int c0 = 0; c0 < D / 64; c0++) {
-                unsigned x[32];
-#pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (valid) v = *reinterpret_cast<const uint4*>(src + c0 * 64 + c * 8);
-                    x[c * 4] = v.x;
-                    x[c * 4 + 1] = v.y;
-                    x[c * 4 + 2] = v.z;
-                    x[c * 4 + 3] = v.w;
-                }
-                if (w == 0 || BOTH_Q) {
-                    tmem_st32(lane_addr + Q_COL + w * (D / 2) + c0 * 32, x);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; c++) tl_store16(q_s + w * Z::Q_TILE + c0 * Q_ATOM + r * 128 + ((c ^ (r & 7)) << 4), x[c * 4], x[c * 4 + 1], x[c * 4 + 2], x[c * 4 + 3]);
-                }
+            const long long mine = valid ? (long long)token * q_stride + (long long)h * D : -1;
+            const unsigned tile_s = q_s + w * Z::Q_TILE;
+            constexpr int LINE = D / 8, ROWS = 32 / LINE;           // lanes of a row, rows at a time
+            // (asynchronous copies, in a loop that stays one: unrolled, its instructions alone, fetched anew by every block's first warps, took longer than the rows)
+            const int c = lane % LINE;
+#pragma unroll 1
+            for (int k = 0; k < LINE; k++) {
+                const int rr = k * ROWS + lane / LINE, row = (warp & 3) * 32 + rr;
+                const long long from = __shfl_sync(0xffffffffu, mine, rr);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile_s + (c >> 3) * Q_ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)),
+                             "l"(q + (from >= 0 ? from : 0) + c * 8), "r"(from >= 0 ? 16 : 0) : "memory");
             }
-            tmem_wait_st();
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (w == 0 || BOTH_Q) {
+                __syncwarp();
+#pragma unroll 1
+                for (int c0 = 0; c0 < D / 64; c0++) {
+                    unsigned x[32];
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[c * 4]), "=r"(x[c * 4 + 1]), "=r"(x[c * 4 + 2]), "=r"(x[c * 4 + 3])
+                                     : "r"(tile_s + c0 * Q_ATOM + r * 128 + ((c ^ (r & 7)) << 4)) : "memory");
+                    tmem_st32(lane_addr + Q_COL + w * (D / 2) + c0 * 32, x);
+                }
+                tmem_wait_st();
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before();
             tl_arrive(q_full);
@@ -535,38 +544,48 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     tc_fence_before();
     __syncthreads();
     if (PREFIX) {
-        // the cluster's shares of a row (ascending) become one; every block makes a part of the rows, four columns to a thread
-        const int n = work.cluster, rank = (int)blockIdx.x % n;
+        // the cluster's shares of a row (ascending) become one; every block makes a part of the rows: first their factors, then four columns to a thread
+        const int n = work.cluster, rank = (int)blockIdx.x % n, rows_each = (n_rows + n - 1) / n, r0 = rank * rows_each, r1 = min(n_rows, r0 + rows_each);
+        const unsigned factors = base + 2 * TL_BM * SHARE_ROW;              // [row of the part][TL_CLUSTER]
         if (n > 1) tl_cluster_sync();
-        for (int idx = rank * (int)blockDim.x + (int)threadIdx.x; idx < n_rows * (D / 4); idx += n * (int)blockDim.x) {
-            const int br = idx / (D / 4), c = idx % (D / 4);
-            const unsigned at = base + br * SHARE_ROW;
-            float4 ml[TL_CLUSTER], v[TL_CLUSTER];
-            float M = -INFINITY;
+        for (int br = r0 + (int)threadIdx.x; br < r1; br += (int)blockDim.x) {
+            float4 ml[TL_CLUSTER];
+            float M = -INFINITY, f[TL_CLUSTER], den = 0.f;
 #pragma unroll
             for (int k = 0; k < TL_CLUSTER; k++) {
-                ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-                if (k >= n) continue;
-                ml[k] = tl_remote4(at + D * 4, k);
-                if (ml[k].y != 0.f) v[k] = tl_remote4(at + c * 16, k);
+                ml[k] = k < n ? tl_remote4(base + br * SHARE_ROW + D * 4, k) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
                 M = fmaxf(M, ml[k].x);
             }
-            const float ref = M == -INFINITY ? 0.f : M;
-            float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-            float den = 0.f;
 #pragma unroll
             for (int k = 0; k < TL_CLUSTER; k++) {
-                if (ml[k].y == 0.f) continue;                       // no keys; a sum that is no number goes on
-                const float f = ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - ref);
-                num.x += f * v[k].x;
-                num.y += f * v[k].y;
-                num.z += f * v[k].z;
-                num.w += f * v[k].w;
-                den += f * ml[k].y;
+                // (no keys: no factor; a sum that is no number goes on)
+                f[k] = ml[k].y == 0.f ? 0.f : ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - M);
+                if (ml[k].y != 0.f) den += f[k] * ml[k].y;
             }
-            const size_t share = ((size_t)work.members[tile.x + br / G] * nh + hk * G + br % G) * work.slots + work.slot0 + blockIdx.x / n;
+            tl_store16(factors + (br - r0) * (TL_CLUSTER * 4), __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+            const size_t share = ((size_t)work.members[member0 + br / G] * nh + hk * G + br % G) * work.slots + work.slot0 + blockIdx.x / n;
+            *reinterpret_cast<float2*>(work.part_ml + share * 2) = make_float2(M, den);
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int idx = (int)threadIdx.x; idx < (r1 - r0) * (D / 4); idx += (int)blockDim.x) {
+            const int i = idx / (D / 4), br = r0 + i, c = idx % (D / 4);
+            float f[TL_CLUSTER];
+            tl_load4(factors + i * (TL_CLUSTER * 4), f);
+            float4 v[TL_CLUSTER], num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < TL_CLUSTER; k++)
+                if (f[k] != 0.f) v[k] = tl_remote4(base + br * SHARE_ROW + c * 16, k);
+#pragma unroll
+            for (int k = 0; k < TL_CLUSTER; k++) {
+                if (f[k] == 0.f) continue;
+                num.x += f[k] * v[k].x;
+                num.y += f[k] * v[k].y;
+                num.z += f[k] * v[k].z;
+                num.w += f[k] * v[k].w;
+            }
+            const size_t share = ((size_t)work.members[member0 + br / G] * nh + hk * G + br % G) * work.slots + work.slot0 + blockIdx.x / n;
             *reinterpret_cast<float4*>(work.part_acc + share * D + c * 4) = num;
-            if (c == 0) *reinterpret_cast<float2*>(work.part_ml + share * 2) = make_float2(M, den);
         }
         if (n > 1) tl_cluster_sync();               // the others may still read this block's rows
     }

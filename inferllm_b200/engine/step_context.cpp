@@ -85,7 +85,7 @@ StepContext StepContextBuilder::build(const SequenceCache& cache, const StepPlan
         }
     }
     const size_t o_prefix = own + pad4(plans);
-    if (prefixes) ops::prefix_plan_fill(prefixes->groups, prefixes->sizes, prefixes->heads, h + o_prefix);
+    if (prefixes) ops::prefix_plan_fill(prefixes->groups, prefixes->sizes, h + o_prefix);
     int* buf = into ? into : dev_->alloc_n<int>(total);
     check_cuda(cudaMemcpyAsync(buf, h, total * sizeof(int), cudaMemcpyHostToDevice, dev_->stream()), "uploading a step's index arrays");
     check_cuda(cudaEventRecord(st.busy, dev_->stream()), "cudaEventRecord");

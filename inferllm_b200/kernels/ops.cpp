@@ -131,9 +131,13 @@ int attention_pages_splits(long long pairs, long long keys, int n_sms) {
 bool attention_pages_in_cluster(long long pairs, int splits, int n_sms) { return splits <= 8 && pairs * splits <= 2LL * n_sms; }
 int attention_prefix_splits(long long pairs, long long keys, int n_sms) {
     const long long most = std::min<long long>(kRingDecodeMaxSplits, std::max<long long>(1, ceil_div(keys, 128)));
-    // (clusters of four blocks, each alone on its SM, fill seven eighths of the SMs)
-    const long long n = std::max<long long>(1, std::min<long long>(most, n_sms * 7LL / 8 / std::max<long long>(1, pairs)));
-    return (int)(n > 4 ? n / 4 * 4 : n);
+    pairs = std::max<long long>(1, pairs);
+    // a block is alone on its SM: clusters of four find room on nine tenths of the SMs, of two on all
+    const long long four = n_sms * 9LL / 10 / pairs / 4 * 4, two = n_sms / pairs / 2 * 2;
+    long long n = four >= 8 || two < four + four / 4 ? four : two;
+    if (n < 1) n = 1;
+    if (n > most) n = most > 4 ? most / 4 * 4 : most;
+    return (int)n;
 }
 bool attention_int8_tc_supported(DType dtype, int nh, int nkv, int d, int page_size, bool decode) {
     return dtype == DType::BF16 && nkv > 0 && nh % nkv == 0 && (d == 64 || d == 128) && page_size > 0 && page_size % 64 == 0 && (!decode || nh / nkv <= 16);

@@ -1184,7 +1184,7 @@ class SharedPrefixes:
         lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
         self.T, self.group_heads = len(lens), int(group_heads)
         self.device = torch.empty(0, device="cuda" if device is None else device).device
-        sizes, total = (ctypes.c_int * 6)(), ctypes.c_int()
+        sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
         args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), self.T,
                 self.group_heads, sizes, ctypes.byref(total))
         _b.check(_b.lib().illm_prefix_plan(*args, None))

@@ -35,7 +35,8 @@ PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const 
         s.longest_prefix = std::max(s.longest_prefix, g.prefix);
     }
     s.wide = rows > kNarrowMost;
-    for (const PrefixGroup& g : groups) s.tiles += ((int)g.members.size() + per_tile(s.wide, G) - 1) / per_tile(s.wide, G);
+    s.per_tile = per_tile(s.wide, G);
+    for (const PrefixGroup& g : groups) s.tiles += ((int)g.members.size() + s.per_tile - 1) / s.per_tile;
     for (int t = 0; t < T; t++) {
         if (lens[t] < 1) throw KernelError("token " + std::to_string(t) + " sees no position");
         s.longest_rest = std::max(s.longest_rest, lens[t] - start[(size_t)t]);
@@ -43,21 +44,20 @@ PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const 
     return s;
 }
 
-void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& s, int G, int* out) {
+void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& s, int* out) {
     std::fill(out, out + s.ints(), 0);
-    int tile = 0, member = 0;
-    const int per = per_tile(s.wide, G);
+    int tile = 0;
+    const int per = s.per_tile;
     for (const PrefixGroup& g : groups)
         for (size_t i = 0; i < g.members.size(); i += (size_t)per) {
             const int n = std::min(per, (int)(g.members.size() - i));
-            int* t = out + 4 * tile++;
-            t[0] = member;
-            t[1] = n;
-            t[2] = g.prefix;
+            out[4 * tile] = n;
+            out[4 * tile + 1] = g.prefix;
             for (int k = 0; k < n; k++) {
-                out[s.members_at() + member++] = g.members[i + (size_t)k];
+                out[s.members_at() + tile * per + k] = g.members[i + (size_t)k];
                 out[s.start_at() + g.members[i + (size_t)k]] = g.prefix;
             }
+            tile++;
         }
 }
 

@@ -18,8 +18,9 @@ struct PrefixPlanSizes {
     bool wide = false;          // pieces of 256 rows (attention_tiles.cu) or of 16 (attention_pages.cu)
     int longest_prefix = 0;     // positions
     int longest_rest = 0;       // the most positions that a token has for itself
-    int ints() const { return 4 * tiles + 2 * ((T + 3) / 4 * 4); }
-    // where its arrays begin: tiles [tiles][4], start [T], members [T]
+    int per_tile = 0;           // members that fit a tile
+    int ints() const { return members_at() + (tiles * per_tile + 3) / 4 * 4; }
+    // where its arrays begin: tiles [tiles][4], start [T], members [tiles][per_tile]
     int start_at() const { return 4 * tiles; }
     int members_at() const { return 4 * tiles + (T + 3) / 4 * 4; }
 };
@@ -28,7 +29,7 @@ struct PrefixPlanSizes {
 // two groups, an empty group, a prefix that is not positive or longer than a member sees.
 PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G);
 // Fills out[0 .. sizes.ints()); sizes.tiles may be larger than the plan needs (the rest are empty tiles).
-void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& sizes, int G, int* out);
+void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& sizes, int* out);
 
 }  // namespace ops
 }  // namespace illm

@@ -8,7 +8,7 @@ from inferllm_b200.binding import KernelError
 
 
 def plan(groups, lens, G):
-    sizes, total = (ctypes.c_int * 6)(), ctypes.c_int()
+    sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
     args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), len(lens), G,
             sizes, ctypes.byref(total))
     _b.check(_b.lib().illm_prefix_plan(*args, None))
@@ -16,15 +16,15 @@ def plan(groups, lens, G):
     _b.check(_b.lib().illm_prefix_plan(*args, out))
     flat = list(out)[:total.value]
     tiles = [flat[4 * i:4 * i + 4] for i in range(sizes[0])]
-    return dict(tiles=tiles, wide=bool(sizes[1]), longest_prefix=sizes[2], longest_rest=sizes[3], start=flat[sizes[4]:sizes[4] + len(lens)], members=flat[sizes[5]:])
+    return dict(tiles=tiles, wide=bool(sizes[1]), longest_prefix=sizes[2], longest_rest=sizes[3], start=flat[sizes[4]:sizes[4] + len(lens)], members=flat[sizes[5]:], per=sizes[6])
 
 
 def covered(p):
     """token -> positions of the prefix that a tile walks for it."""
     got = {}
-    for first, n, length, zero in p["tiles"]:
-        assert zero == 0
-        for t in p["members"][first:first + n]:
+    for i, (n, length, *zeros) in enumerate(p["tiles"]):
+        assert zeros == [0, 0] and n <= p["per"]
+        for t in p["members"][i * p["per"]:i * p["per"] + n]:
             assert t not in got
             got[t] = length
     return got
@@ -46,7 +46,7 @@ def test_every_member_is_in_one_tile_that_fits(G, counts):
     assert covered(p) == want
     assert p["start"] == [want.get(t, 0) for t in range(tokens)]
     most = 256 if p["wide"] else 16
-    assert all(1 <= n and n * G <= most for _, n, _, _ in p["tiles"])
+    assert p["per"] == most // G and all(1 <= n for n, *_ in p["tiles"])
     assert p["longest_prefix"] == 64 * len(counts)
     assert p["longest_rest"] == max(n - want.get(t, 0) for t, n in enumerate(lens))
 
