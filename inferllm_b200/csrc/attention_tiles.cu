@@ -521,15 +521,18 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 }
             }
             tl_store16(dst + D * 4, __float_as_uint(nbw > 0 ? m_ref : -INFINITY), __float_as_uint(nbw > 0 ? l_run : 0.f), 0u, 0u);
-        } else if (alive && nbw > 0) {
+        } else if (alive) {
+            // (a row that sees nothing, one before the first position of its sequence, is zeros)
             tc_fence_after();
-            const float inv = 1.0f / l_run;
+            const float inv = nbw > 0 && l_run != 0.f ? 1.0f / l_run : 0.f;
             bf16* dst = out + head * D;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
-                unsigned o[32];
-                tmem_ld32_issue(o_addr + c0, o);
-                tmem_wait_ld<32>(o);
+                unsigned o[32] = {};
+                if (nbw > 0) {
+                    tmem_ld32_issue(o_addr + c0, o);
+                    tmem_wait_ld<32>(o);
+                }
                 if (valid)
 #pragma unroll
                     for (int c = 0; c < 32; c += 8) {

@@ -1019,40 +1019,40 @@ def kv_write_int8(qkv, cos_sin, rot_dim, token_pos, token_seq, block_table, cach
     such a token's rows are not written.  Two tokens of one call must not name the same position."""
     if not isinstance(cache, CacheInt8):
         raise KernelError("kv_write_int8 writes a CacheInt8")
-    d, nkv = cache.head_dim, cache.n_kv_heads
-    partials = qkv if isinstance(qkv, SplitKPartials) else None
-    dtype = torch.bfloat16 if partials is not None else qkv.dtype
-    if partials is None:
+    device, d, nkv = cache.device, cache.head_dim, cache.n_kv_heads
+    if isinstance(qkv, SplitKPartials):
+        dtype, at, parts, splits, apart = torch.bfloat16, None, qkv.ws.data_ptr(), qkv.splits, qkv.rows * qkv.cols
+    else:
         _need(qkv, "qkv", None, 2)
+        dtype, at, parts, splits, apart = qkv.dtype, qkv.data_ptr(), None, 0, 0
     code = act_code(dtype)
-    if tuple(qkv.shape)[1] != (n_heads + 2 * nkv) * d or n_heads < 1:
-        raise KernelError(f"qkv width {tuple(qkv.shape)[1]} is not (heads + 2 kv heads) * head_dim")
-    if qkv.device != cache.device or err.device != cache.device:
+    T, columns = qkv.shape
+    if columns != (n_heads + 2 * nkv) * d or n_heads < 1:
+        raise KernelError(f"qkv width {columns} is not (heads + 2 kv heads) * head_dim")
+    if qkv.device != device or err.device != device:
         raise KernelError("qkv, err and the cache must be on one device")
-    T = qkv.shape[0]
     _need(err, "err", torch.int32)
-    width = _block_table(block_table, cache.device)
-    _step_array(token_pos, "token_pos", T, cache.device)
-    _step_array(token_seq, "token_seq", T, cache.device)
+    width = _block_table(block_table, device)
+    _step_array(token_pos, "token_pos", T, device)
+    _step_array(token_seq, "token_seq", T, device)
     if rot_dim < 0 or rot_dim > d or rot_dim % 2:
         raise KernelError(f"rot_dim {rot_dim} must be even and at most the head size {d}")
-    n_pos = 0
+    n_pos, turns = 0, None
     if rot_dim:
         if cos_sin is None:
             raise KernelError("a rotation needs its cos/sin table")
         _need(cos_sin, "cos_sin", torch.float32, 3)
-        if cos_sin.shape[1] != rot_dim // 2 or cos_sin.shape[2] != 2 or cos_sin.device != cache.device:
+        n_pos, half, two = cos_sin.shape
+        if half != rot_dim // 2 or two != 2 or cos_sin.device != device:
             raise KernelError("cos_sin table does not match rot_dim")
-        if cos_sin.data_ptr() & 15:
+        turns = cos_sin.data_ptr()
+        if turns & 15:
             raise KernelError("cos_sin must start on a 16-byte boundary")
-        n_pos = cos_sin.shape[0]
-    with _on(cache.device):
-        q = _rows(T, n_heads * d, dtype, cache.device)
+    with _on(device):
+        q = _rows(T, n_heads * d, dtype, device)
         _check(load().illm_kv_write_int8(
-            None if partials is not None else _ptr(qkv), None if partials is None else _ptr(partials.ws), 0 if partials is None else partials.splits,
-            0 if partials is None else partials.rows * partials.cols, _ptr(q), _ptr(cos_sin) if rot_dim else None, _ptr(token_pos), _ptr(token_seq),
-            _ptr(block_table), width, cache.pages, *cache.pointers, code, T, n_heads, nkv, d, rot_dim, cache.page_size, 1, n_pos, _ptr(err),
-            _stream()), "kv_write_int8")
+            at, parts, splits, apart, q.data_ptr(), turns, token_pos.data_ptr(), token_seq.data_ptr(), block_table.data_ptr(), width, cache.pages, *cache.pointers, code, T,
+            n_heads, nkv, d, rot_dim, cache.page_size, 1, n_pos, err.data_ptr(), _stream()), "kv_write_int8")
     return q
 
 
@@ -1067,8 +1067,7 @@ def kv_read_int8(cache, token_pos, token_seq, block_table, dtype=torch.bfloat16)
     with _on(cache.device):
         k = torch.empty((n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
         v = torch.empty_like(k)
-        _check(load().illm_kv_read_int8(*cache.pointers, _ptr(token_pos), _ptr(token_seq), _ptr(block_table), width, cache.pages, _ptr(k), _ptr(v),
-                                        code, n, cache.n_kv_heads, cache.head_dim, cache.page_size, _stream()), "kv_read_int8")
+        _check(load().illm_kv_read_int8(*cache.pointers, token_pos.data_ptr(), token_seq.data_ptr(), block_table.data_ptr(), width, cache.pages, k.data_ptr(), v.data_ptr(), code, n, cache.n_kv_heads, cache.head_dim, cache.page_size, _stream()), "kv_read_int8")
     return k, v
 
 

@@ -446,6 +446,25 @@ def test_prompts(ops, nh, nkv, d, page, new, past, window, tile_rows):
     assert take_error(ops) == 0
 
 
+def test_prompt_rows_before_the_first_position_are_zeros(ops):
+    """A sequence said to be shorter than its new tokens: those before position 0 see nothing (of the first 40, 20 and 260 tokens a part of a tile, and more
+    than a tile of two sequences' heads)."""
+    nh, nkv, d, scale = 4, 2, 64, 0.125
+    new, lens = [100, 30, 300], [60, 10, 40]
+    pages = Pages(71, lens, nkv, d)
+    T = sum(new)
+    q = queries(73, T, nh * d)
+    cu = torch.tensor([0, 100, 130, 430], dtype=torch.int32).cuda()
+    for tile_rows in (128, 256):
+        got = ops.attention_prompts_int8(q.cuda(), pages.cache(ops), pages.table.cuda(), cu, torch.tensor(lens, dtype=torch.int32).cuda(), 300, nh, 0, scale, tile_rows=tile_rows)
+        assert take_error(ops) == 0
+        for i, (n, length) in enumerate(zip(new, lens)):
+            first = sum(new[:i])
+            assert (got[first:first + n - length] == 0).all()
+            mine = slice(first + n - length, first + n)
+            want, tol = expected(pages, q[mine], [(i, j) for j in range(length)], nh, 0, scale, B16)
+            near(got[mine], want, tol)
+
 def test_a_row_that_is_not_a_number_reaches_later_queries_only(ops):
     nh, nkv, d, n = 4, 2, 64, 150
     for which in ("k", "v"):
@@ -606,6 +625,51 @@ def test_on_another_stream_and_captured(ops):
     torch.cuda.synchronize()
     for (_, _, out), w in zip(graphs, (want, other)):
         assert all(torch.equal(a, b) for a, b in zip(w, out))
+    assert take_error(ops) == 0
+
+
+def test_two_calls_at_once(ops):
+    """Calls on two streams, none of which waits for the other, have scratch of their own: each gives what it gives alone."""
+    nh, nkv, d, n = 32, 8, 128, 40
+    lens = [600 + 7 * i for i in range(n)]
+    common = [(0, None)] + [(512, 0)] * (n - 1)
+    pages = Pages(91, lens, nkv, d, common=common)
+    cache, table = pages.cache(ops), pages.table.cuda()
+    pos, seq = torch.tensor(lens, dtype=torch.int32).cuda() - 1, torch.arange(n, dtype=torch.int32).cuda()
+    plan = ops.SharedPrefixes([(512, list(range(n)))], lens, nh // nkv)
+    q = [queries(s, n, nh * d).cuda() for s in (93, 97)]
+    cu, ln = torch.arange(0, n + 1, dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    runs = [lambda x: ops.attention_decode_shared(x, cache, table, pos, seq, plan, nh, 0.09, max(lens)),
+            lambda x: ops.attention_decode_int8(x, cache, table, pos, seq, nh, 0, 0.09, max(lens), splits=16),
+            lambda x: ops.attention_decode_int8(x, cache, table, pos, seq, nh, 0, 0.09, max(lens), splits=4),
+            lambda x: ops.attention_prompts_int8(x, cache, table, cu, ln, 1, nh, 0, 0.09)]
+    for run in runs:
+        alone = [run(x) for x in q]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in q]
+        got = [[], []]
+        for _ in range(4):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(run(q[i]))
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(alone[i], g) for g in got[i])
+    assert take_error(ops) == 0
+
+
+def test_more_tokens_than_a_grid_has_rows(ops):
+    """65,540 single tokens go in two launches."""
+    lens = [1, 70, 129]
+    pages = Pages(101, lens, 1, 64)
+    few = queries(103, 3, 64)
+    T = 65540
+    seq = (torch.arange(T) % 3).int()
+    args = pages.cache(ops), pages.table.cuda()
+    last = torch.tensor(lens, dtype=torch.int32) - 1
+    got = ops.attention_decode_int8(few[seq.long()].contiguous().cuda(), *args, last[seq.long()].cuda(), seq.cuda(), 1, 0, 0.125, 129, splits=2)
+    want = ops.attention_decode_int8(few.cuda(), *args, last.cuda(), torch.arange(3, dtype=torch.int32).cuda(), 1, 0, 0.125, 129, splits=2)
+    assert torch.equal(got, want[seq.long().cuda()])
     assert take_error(ops) == 0
 
 

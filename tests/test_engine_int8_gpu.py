@@ -4,6 +4,7 @@ The plain implementation is given the same rounding of keys and values.  A value
 fall to either side in the engine, which moves it by 1/127 of its row's largest: less than what rounding every activation to bfloat16 does, whose bounds
 therefore serve the float32 mode here too."""
 import subprocess
+from dataclasses import dataclass
 
 import numpy as np
 import plain_llama as plain
@@ -12,8 +13,10 @@ import torch
 from conftest import ROOT, TINY, random_prompt
 from util import assert_close
 
-from inferllm_b200 import CacheError, Engine, EngineError, EngineOptions, Model, ModelConfig, StepItem
+from inferllm_b200 import CacheError, Engine, EngineError, EngineOptions, Model, ModelConfig, StepItem, write_random_model
+from inferllm_b200.config import ArchConfig, LayerSpec, ModelSpec, PartSpec, ScheduleEntry, register_architecture, unregister_architecture
 from inferllm_b200.kernels import ops
+from inferllm_b200.parts import PositionEncoding, register_position, unregister_part
 
 pytestmark = pytest.mark.gpu
 
@@ -82,6 +85,109 @@ def test_a_prompt_in_pieces(name, dtype, model_folders):
     e.check_device_errors()
     for other in (pieces, singles):
         assert_close(other.cpu().numpy(), whole.cpu().numpy(), "bfloat16")
+
+
+HIDDEN, HEADS, KV_HEADS, SIZE, WORDS, WINDOW, BASE = 96, 4, 2, 64, 90, 70, 1e4
+
+
+@register_position("pairs_of_a_test")
+class Pairs(PositionEncoding):
+    """An encoding of its own, which writes rows of the activations' type: its layer's entry stays wide."""
+
+    def encode_and_store(self, qkv, geometry, ctx, kv):
+        nh, nkv, d = geometry
+        ops.rope_kv_write(qkv, None, 0, ctx.token_pos, ctx.token_seq, kv.block_table, kv.k, kv.v, nh, nkv, d, kv.page_size, True, ctx.err)
+        return qkv
+
+
+@dataclass
+class ManyKinds(ArchConfig):
+    """Attention with a window and without, a layer that reads another's entry and, `own`, one that cannot keep eight bits."""
+    own: bool = False
+
+    @classmethod
+    def from_dict(cls, d):
+        return cls(own=d["own"])
+
+    def to_dict(self):
+        return {"architectures": ["ManyKindsForCausalLM"], "own": self.own}
+
+    def model_spec(self):
+        norm = PartSpec("rmsnorm", {"size": HIDDEN, "eps": 1e-5})
+        shape = {"hidden_size": HIDDEN, "n_heads": HEADS, "n_kv_heads": KV_HEADS, "head_dim": SIZE}
+        half = PartSpec("rope_half", {"head_dim": SIZE, "theta": BASE, "max_positions": 512})
+        mixers = [PartSpec("attention", dict(shape, window=w, position=p)) for w, p in
+                  [(None, half), (WINDOW, half), (None, half), (None, PartSpec("pairs_of_a_test", {}))][:4 if self.own else 3]]
+        ffn = PartSpec("gated_mlp", {"hidden_size": HIDDEN, "intermediate_size": 128})
+        layers = [LayerSpec("prenorm", m, ffn, {"norm1": norm, "norm2": norm}, f"blocks.{i}.", {"mixer": "mixer.", "ffn": "ffn.", "norm1": "ln1.", "norm2": "ln2."})
+                  for i, m in enumerate(mixers)]
+        schedule = [ScheduleEntry(0, 0), ScheduleEntry(1, 1), ScheduleEntry(2, 0, writes=False)] + ([ScheduleEntry(3, 2)] if self.own else [])
+        return ModelSpec(HIDDEN, WORDS, layers, schedule, PartSpec("embedding", {"name": "emb.", "vocab_size": WORDS, "hidden_size": HIDDEN}),
+                         PartSpec("rmsnorm", {"name": "ln_f.", "size": HIDDEN, "eps": 1e-5}),
+                         PartSpec("lm_head", {"name": "head.", "tied": True, "vocab_size": WORDS, "hidden_size": HIDDEN}), 512, None, [])
+
+
+def plain_many(w, ids, own):
+    pos, x, kept = np.arange(len(ids)), plain.embed(ids, w["emb.weight"]), {}
+    for layer, entry in [(0, 0), (1, 1), (2, 0), (3, 2)][:4 if own else 3]:
+        p = f"blocks.{layer}."
+        h = plain.rms_norm(x, w[p + "ln1.weight"], 1e-5)
+        weights = [w[p + f"mixer.{n}_proj.weight"] for n in "qkvo"]
+        if layer == 3:
+            q, k, v = (plain.linear(h, m).reshape(len(ids), -1, SIZE) for m in weights[:3])
+            s = plain.scale_and_mask(plain.attention_scores(q, k, HEADS, KV_HEADS), SIZE ** -0.5)
+            a = plain.linear(plain.weighted_values(plain.softmax_rows(s), v, HEADS, KV_HEADS), weights[3])
+        else:
+            shape = pos, HEADS, KV_HEADS, SIZE, BASE
+            if layer < 2:
+                kept[entry] = tuple(eight_bits(t) for t in plain.self_attention(h, *weights, *shape)[1])
+            a, _ = plain.self_attention(h, *weights, *shape, window=WINDOW if layer == 1 else None, kv_override=kept[entry])
+        x = x + a
+        h = plain.rms_norm(x, w[p + "ln2.weight"], 1e-5)
+        x = x + plain.swiglu_ffn(h, *(w[p + f"ffn.{n}_proj.weight"] for n in ("gate", "up", "down")))
+    return plain.linear(plain.rms_norm(x, w["ln_f.weight"], 1e-5), w["emb.weight"])
+
+
+@pytest.fixture(scope="module", params=[False, True])
+def many_kinds(request, tmp_path_factory):
+    register_architecture("ManyKindsForCausalLM", ManyKinds)
+    d = str(tmp_path_factory.mktemp("many"))
+    write_random_model(ManyKinds(own=request.param), d, seed=5, dtype=torch.bfloat16)
+    yield d, request.param
+    unregister_architecture("ManyKindsForCausalLM")
+    if request.param:
+        unregister_part("position", "pairs_of_a_test")
+
+
+@pytest.mark.parametrize("dtype, page", [("float32", 16), ("bfloat16", 64), ("bfloat16", 16)])
+def test_windows_and_entries_that_layers_share(many_kinds, dtype, page):
+    """Past the window, where pages go back (and are poisoned) while the sequences grow; entries in eight bits beside one that stays wide."""
+    folder, own = many_kinds
+    _, w = plain.load_weights(folder)
+    e = engine(folder, dtype, page_size=page, poison_freed_pages=True)
+    assert [g.get("k_scale") is not None for g in e.cache.stats()["paged"]].count(True) == 2
+    rng = np.random.default_rng(7)
+    texts = [rng.integers(0, WORDS, n).tolist() for n in (230, 60, 150)]
+    first = [200, 30, 1]
+    slots = [e.new_sequence() for _ in texts]
+    refs = [plain_many(w, t, own) for t in texts]
+    got, at = e.step([StepItem(s, t[:n], list(range(n))) for s, t, n in zip(slots, texts, first)]).cpu().numpy(), 0
+    for r, n in zip(refs, first):
+        assert_close(got[at:at + n], r[:n], "bfloat16", "prompt")
+        at += n
+    for j in range(30):
+        got = e.step([StepItem(s, [t[n + j]], [0]) for s, t, n in zip(slots, texts, first)]).cpu().numpy()
+        for i in range(3):
+            assert_close(got[i:i + 1], refs[i][first[i] + j:first[i] + j + 1], "bfloat16", f"token {j} of request {i}")
+    # the last one's next tokens in one step, on top of what is there
+    got = e.step([StepItem(slots[2], texts[2][31:], list(range(119)))]).cpu().numpy()
+    assert_close(got, refs[2][31:], "bfloat16", "a longer piece")
+    e.check_device_errors()
+    with pytest.raises(CacheError):
+        e.fork_sequence(slots[0], 64)
+    for s in slots:
+        e.end_sequence(s)
+    e.cache.check()
 
 
 def test_what_lies_in_the_cache(model_folders, plain_models):
