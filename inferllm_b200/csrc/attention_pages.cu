@@ -82,13 +82,31 @@ template <int D, bool Q8> __device__ __forceinline__ unsigned pg_off(int r, int 
     if (D == 128) return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4));
     return (unsigned)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
-// a float of the same place in another block of the cluster
-__device__ __forceinline__ float pg_remote(unsigned at, unsigned rank) {
+// two and four floats of the same place in another block of the cluster
+__device__ __forceinline__ float2 pg_remote2(unsigned at, unsigned rank) {
     unsigned a;
-    float f;
+    float2 f;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(a) : "memory");
     return f;
+}
+__device__ __forceinline__ float4 pg_remote4(unsigned at, unsigned rank) {
+    unsigned a;
+    float4 f;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+    return f;
+}
+__device__ __forceinline__ void pg_add(float4& sum, float4 v, float f) {
+    sum.x += v.x * f;
+    sum.y += v.y * f;
+    sum.z += v.z * f;
+    sum.w += v.w * f;
+}
+// four channels of a result; a row without keys is zeros
+__device__ __forceinline__ void pg_result(bf16* to, float4 num, float den) {
+    const bool none = den == 0.f;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pg_bf162(none ? 0.f : num.x / den, none ? 0.f : num.y / den), pg_bf162(none ? 0.f : num.z / den, none ? 0.f : num.w / den));
 }
 __device__ __forceinline__ void pg_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -142,7 +160,11 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    pdl_grid_sync();
+    // Behind wide tiles this kernel needs nothing of theirs, and what comes before them is through when they let it start (attention_tiles.cu): it runs beside
+    // them and waits for them at its end, for the sake of what follows both.
+    const bool beside = plan.start && plan.n_tiles == 0;
+    if (beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    else pdl_grid_sync();
 
     // ---- which rows and keys
     // the blocks of one (prefix tile or token, kv head) follow one another, then come the other kv heads, whose rows lie in the same pages
@@ -173,6 +195,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int slot = prefix ? own_splits + split : split;
     if (part_acc && n_my == 0) {
         if (tid < rows) *reinterpret_cast<float2*>(part_ml + (row_head(tid) * slots + slot) * 2) = make_float2(-INFINITY, 0.f);
+        if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
@@ -448,62 +471,66 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (g == 0) *reinterpret_cast<float4*>(dst + D) = make_float4(m[nt][e], l[nt][e], mv[nt][e], 0.f);
         }
     asm volatile("bar.sync 1, %0;" ::"n"(PG_CONSUMERS * 32) : "memory");
-    // the block's share of every row: accumulators relative to m, m and l; a row without keys has l = 0
+    // the block's share of every row: accumulators relative to m, m and l; a row without keys has l = 0.  A thread makes four channels (one by one the
+    // warps' factors cost more than the sums: 16 rows behind a common prefix of 128 positions 13.1 us).
     float* share = joined + (size_t)PG_CONSUMERS * 16 * ROW;        // [16][ROW]
     const bool alone = !part_acc && n_splits == 1;
-    for (int idx = tid; idx < rows * D; idx += PG_CONSUMERS * 32) {
-        const int r = idx / D, c = idx - r * D;
-        float4 w[PG_CONSUMERS];
+    for (int idx = tid; idx < rows * (D / 4); idx += PG_CONSUMERS * 32) {
+        const int r = idx / (D / 4), c = (idx - r * (D / 4)) * 4;
+        float4 w[PG_CONSUMERS], v[PG_CONSUMERS];
         float M = -INFINITY;
 #pragma unroll
         for (int k = 0; k < PG_CONSUMERS; k++) {
             w[k] = *reinterpret_cast<const float4*>(joined + ((size_t)k * 16 + r) * ROW + D);
+            v[k] = *reinterpret_cast<const float4*>(joined + ((size_t)k * 16 + r) * ROW + c);
             M = fmaxf(M, w[k].x);
         }
         const float ref = M == -INFINITY ? 0.f : M;
-        float num = 0.f, den = 0.f;
+        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
 #pragma unroll
         for (int k = 0; k < PG_CONSUMERS; k++) {
             if (w[k].y == 0.f) continue;                        // no visible keys; a sum that is no number goes on
-            num += joined[((size_t)k * 16 + r) * ROW + c] * (w[k].z == -INFINITY ? 1.f : fast_exp2(w[k].z - ref));
+            pg_add(num, v[k], w[k].z == -INFINITY ? 1.f : fast_exp2(w[k].z - ref));
             den += w[k].y * (w[k].x == -INFINITY ? 1.f : fast_exp2(w[k].x - ref));
         }
         if (alone) {
-            out[row_head(r) * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+            pg_result(out + row_head(r) * D + c, num, den);
         } else if (part_acc) {
             const size_t at = row_head(r) * slots + slot;
-            part_acc[at * D + c] = num;
+            *reinterpret_cast<float4*>(part_acc + at * D + c) = num;
             if (c == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(M, den);
         } else {
-            share[r * ROW + c] = num;
+            *reinterpret_cast<float4*>(share + r * ROW + c) = num;
             if (c == 0) *reinterpret_cast<float2*>(share + r * ROW + D) = make_float2(M, den);
         }
     }
+    if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (alone || part_acc) return;
     // ---- join the cluster's shares (ascending): every block writes a part of the rows
     pg_cluster_sync();
     const unsigned share_at = tc_smem_u32(share);
-    for (int idx = split * (PG_CONSUMERS * 32) + tid; idx < rows * D; idx += n_splits * (PG_CONSUMERS * 32)) {
-        const int r = idx / D, c = idx - r * D;
+    for (int idx = split * (PG_CONSUMERS * 32) + tid; idx < rows * (D / 4); idx += n_splits * (PG_CONSUMERS * 32)) {
+        const int r = idx / (D / 4), c = (idx - r * (D / 4)) * 4;
         const unsigned row_at = share_at + r * ROW * 4;
-        float ms[PG_MAX_CLUSTER], ls[PG_MAX_CLUSTER], v[PG_MAX_CLUSTER], M = -INFINITY;
+        float4 v[PG_MAX_CLUSTER], num = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 ml[PG_MAX_CLUSTER];
+        float M = -INFINITY, den = 0.f;
 #pragma unroll
         for (int k = 0; k < PG_MAX_CLUSTER; k++) {
-            ms[k] = k < n_splits ? pg_remote(row_at + D * 4, k) : -INFINITY;
-            ls[k] = k < n_splits ? pg_remote(row_at + D * 4 + 4, k) : 0.f;
-            v[k] = k < n_splits ? pg_remote(row_at + c * 4, k) : 0.f;
-            M = fmaxf(M, ms[k]);
+            ml[k] = k < n_splits ? pg_remote2(row_at + D * 4, k) : make_float2(-INFINITY, 0.f);
+            v[k] = k < n_splits ? pg_remote4(row_at + c * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            M = fmaxf(M, ml[k].x);
         }
         const float ref = M == -INFINITY ? 0.f : M;
-        float num = 0.f, den = 0.f;
 #pragma unroll
         for (int k = 0; k < PG_MAX_CLUSTER; k++) {
-            if (k >= n_splits || ls[k] == 0.f) continue;
-            const float f = ms[k] == -INFINITY ? 1.f : fast_exp2(ms[k] - ref);
-            num += f * v[k];
-            den += f * ls[k];
+            if (k >= n_splits || ml[k].y == 0.f) continue;
+            const float f = ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - ref);
+            pg_add(num, v[k], f);
+            den += f * ml[k].y;
         }
-        out[row_head(r) * D + c] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+        pg_result(out + row_head(r) * D + c, num, den);
     }
     pg_cluster_sync();              // the others may still read this block's shares
 }
@@ -601,7 +628,8 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 // Single tokens: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages
 // [n_pages, nkv, page_size, d] of bytes with their scales ksc, vsc, or (ksc, vsc nullptr) of bfloat16; page_size a multiple of 64, d 64
 // or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most 16 rows (members times nh / nkv),
-// are walked here, with n_tiles 0 their pre_splits shares are there already (illm_attention_tiles_prefix, slot0 = own_splits).  own_splits, pre_splits: at most 32 each,
+// are walked here; with n_tiles 0
+// their pre_splits shares are what the launch before this one makes, which has to be illm_attention_tiles_prefix's (slot0 = own_splits): the two run side by side.  own_splits, pre_splits: at most 32 each,
 // pre_splits 0 without a plan.  Scratch: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2], or, without a plan and with up to 8 splits,
 // nullptr: then the blocks of a (token, kv head) are a cluster and there is no second kernel.  That is the faster way while the blocks find room together (one
 // sequence of 8 kv heads at 1,777 keys 7.3 us and 9), and the slower one where they have to wait for one another's places (64 sequences of 32 kv heads at 300

@@ -149,7 +149,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = *holder;
-    pdl_grid_sync();
+    if (PREFIX) {
+        // in this order, for attention_pages.cu runs beside this kernel without a wait of its own: what comes before is through once it starts
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    } else {
+        pdl_grid_sync();
+    }
 
     // ---- which rows and keys
     const int G = nh / nkv;
