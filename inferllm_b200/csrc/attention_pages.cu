@@ -118,12 +118,12 @@ __device__ __forceinline__ void pg_bulk(unsigned dst, const void* src, unsigned 
 }  // namespace
 
 // A plan of common prefixes (attention_decode_shared): int32 on the device.  `start` [T]: the positions that a token leaves to its
-// group; `tiles` [n_tiles][4]: number of members, positions of the prefix, 0, 0; `members` [n_tiles][16 / (nh / nkv)]: tokens.
+// group; `tiles` [n_tiles][4]: number of members, positions of the prefix, 0, 0; `members` [n_tiles][per_tile]: tokens.
 struct PgPlan {
     const int* start;
     const int4* tiles;
     const int* members;
-    int n_tiles;
+    int n_tiles, per_tile;
 };
 
 // Stages: as many as leave four blocks to an SM (five at head size 64, three of bfloat16 rows), or with sixteen rows, whose registers leave two blocks, more.  The blocks
@@ -174,8 +174,8 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     int t = 0, first = 0, count = 1, p, lo = 0;
     if (prefix) {
         const int4 tile = plan.tiles[item];
-        first = item * (16 / G);
-        count = tile.x;
+        first = item * plan.per_tile;
+        count = min(tile.x, plan.per_tile);
         p = tile.y - 1;
         if (count <= 0 || p < 0) return;
         t = plan.members[first];
@@ -608,7 +608,7 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
         (rc = pg_make_map(&mv16, vc, rows, D, 16, Q8)))
         return rc;
     // eight rows in a block's products where no block has more
-    const bool eight = plan.n_tiles == 0 && nh / nkv <= 8;
+    const bool eight = nh / nkv * (plan.n_tiles ? plan.per_tile : 1) <= 8;
     auto kern = eight ? attention_pages_kernel<D, Q8, 1> : attention_pages_kernel<D, Q8, 2>;
     const int smem = eight ? PgRing<D, Q8, 1>::BYTES : PgRing<D, Q8, 2>::BYTES;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -627,7 +627,7 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 
 // Single tokens: q, rows of q_stride bfloat16 elements whose first nh * d are the query heads; kc, vc one entry's pages
 // [n_pages, nkv, page_size, d] of bytes with their scales ksc, vsc, or (ksc, vsc nullptr) of bfloat16; page_size a multiple of 64, d 64
-// or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most 16 rows (members times nh / nkv),
+// or 128, at most 16 query heads per kv head.  plan_start nullptr, or a plan (PgPlan; then span 0): its n_tiles tiles, of at most per_tile members and 16 rows (members times nh / nkv),
 // are walked here; with n_tiles 0
 // their pre_splits shares are what the launch before this one makes, which has to be illm_attention_tiles_prefix's (slot0 = own_splits): the two run side by side.  own_splits, pre_splits: at most 32 each,
 // pre_splits 0 without a plan.  Scratch: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2], or, without a plan and with up to 8 splits,
@@ -636,16 +636,16 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 // keys in two parts 60 us and 46).  err: 7 a wait ran out, 8 a visible position without a page.
 extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                     const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles,
-                                    const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,
+                                    const int* plan_members, int n_tiles, int per_tile, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,
                                     int span, float scale, int own_splits, int pre_splits, int* err, void* stream) {
     if (T <= 0) return 0;
     if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || T > 65535 || nkv > 65535 || n_tiles < 0 || n_tiles > 65535 || (q_stride & 7) || page_size <= 0 ||
         page_size % PG_BN || max_pages <= 0 || n_pages <= 0 || n_pages * nkv * page_size > 0x7fffffffLL || own_splits < 1 || own_splits > PG_MAX_SPLITS || pre_splits < 0 ||
         pre_splits > PG_MAX_SPLITS || !q || ((uintptr_t)q & 15) || !kc || !vc || ((uintptr_t)kc & 15) || ((uintptr_t)vc & 15) || (!ksc) != (!vsc) || ((uintptr_t)ksc & 15) ||
         ((uintptr_t)vsc & 15) || !err || (plan_start && (span != 0 || pre_splits < 1)) || (!plan_start && (n_tiles > 0 || pre_splits != 0)) ||
-        (n_tiles > 0 && (!plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || ((own_splits > PG_MAX_CLUSTER || plan_start) && !part_acc) || (!part_acc) != (!part_ml) || ((uintptr_t)part_ml & 7) || !out || !token_pos || !token_seq || !block_table)
+        (n_tiles > 0 && (per_tile < 1 || per_tile > 16 || per_tile * (nh / nkv) > 16 || !plan_tiles || !plan_members || ((uintptr_t)plan_tiles & 15))) || ((own_splits > PG_MAX_CLUSTER || plan_start) && !part_acc) || (!part_acc) != (!part_ml) || ((uintptr_t)part_ml & 7) || !out || !token_pos || !token_seq || !block_table)
         return ILLM_ERR_BAD_ARG;
-    const PgPlan plan = {plan_start, reinterpret_cast<const int4*>(plan_tiles), plan_members, n_tiles};
+    const PgPlan plan = {plan_start, reinterpret_cast<const int4*>(plan_tiles), plan_members, n_tiles, per_tile};
     cudaStream_t s = (cudaStream_t)stream;
 #define PG_CASE(DD, QQ)                                                                                                                                        \
     if (d == DD && (ksc != nullptr) == QQ)                                                                                                                     \

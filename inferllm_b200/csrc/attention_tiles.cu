@@ -167,7 +167,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         member0 = blockIdx.z * (2 * TL_BM / G);
         const int first_member = work.members[member0];
         tile = work.tiles[blockIdx.z];
-        n_rows = tile.x > 0 && tile.y > 0 ? tile.x * G : 0;
+        n_rows = tile.x > 0 && tile.y > 0 ? min(tile.x, 2 * TL_BM / G) * G : 0;
         token0 = 0;
         seq = n_rows ? work.token_seq[first_member] : 0;
         const int all = (tile.y + TL_BN - 1) / TL_BN, per = (all + gridDim.x - 1) / gridDim.x;

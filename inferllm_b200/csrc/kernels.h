@@ -45,7 +45,7 @@ int illm_kv_read_int8(const void* kc, const void* vc, const float* ksc, const fl
 int illm_attention_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, const int* block_table, int max_pages, long long n_pages, const int* token_pos, const int* token_seq, void* out, int act_dtype, int T, int nh, int nkv, int d, int page_size, int span, float scale, int* err, void* stream);
 
 // attention_pages.cu
-int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles, const int* plan_members, int n_tiles, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size, int span, float scale, int own_splits, int pre_splits, int* err, void* stream);
+int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles, const int* plan_members, int n_tiles, int per_tile, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size, int span, float scale, int own_splits, int pre_splits, int* err, void* stream);
 
 // attention_tiles.cu
 int illm_attention_tiles_int8(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages, const int* cu_q, const int* seq_lens, void* out, int B, int max_q, int nh, int nkv, int d, int page_size, int span, float scale, int tile_rows, int* err, void* stream);

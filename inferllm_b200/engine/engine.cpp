@@ -28,6 +28,7 @@ EngineOptions EngineOptions::from_json(const Json& j) {
     if (j.at("poison_freed_pages").is_bool()) o.poison_freed_pages = j.at("poison_freed_pages").as_bool();
     if (j.has("cache_dtype") && j.at("cache_dtype").is_string()) o.cache_dtype = j.at("cache_dtype").as_string();
     if (j.has("share_prefixes") && j.at("share_prefixes").is_bool()) o.share_prefixes = j.at("share_prefixes").as_bool();
+    if (j.has("shared_prefix_bytes") && j.at("shared_prefix_bytes").is_int()) o.shared_prefix_bytes = j.at("shared_prefix_bytes").as_int();
     if (j.at("stream").is_int()) o.stream = (void*)(uintptr_t)j.at("stream").as_int();
     return o;
 }
@@ -248,19 +249,21 @@ StepContext Engine::make_context(const StepPlan& plan, const std::vector<int>& i
 // (tiles, the splits that follow from the lengths) is rounded up, so that captured steps of growing sequences can be replayed.
 bool Engine::find_prefixes(const StepPlan& plan, StepPrefixes* out) const {
     if (!prefix_heads_ || plan.slots.size() < 2) return false;
+    const SequenceCache::PagedGroup& kept = cache_->paged[0];
     long long saved = 0;
     for (auto& g : cache_->common_prefixes(plan.slots)) {
-        saved += (long long)g.first * ((long long)g.second.size() - 1);
+        saved += g.first / cache_->page_size * (long long)(kept.page_bytes + kept.v_page_bytes) * ((long long)g.second.size() - 1);
         ops::PrefixGroup group;
         group.prefix = g.first;
         group.members = g.second;
         out->groups.push_back(std::move(group));
     }
-    if (saved < kSharedPrefixMinSaved) return false;
+    if (out->groups.empty() || saved < (options_.shared_prefix_bytes >= 0 ? options_.shared_prefix_bytes : kSharedPrefixBytes + (long long)plan.slots.size() * kSharedPrefixBytesEach))
+        return false;
     std::vector<int> lens;
     for (size_t i = 0; i < plan.slots.size(); i++) lens.push_back((int)(plan.past[i] + 1));
     out->heads = prefix_heads_;
-    out->sizes = ops::prefix_plan_sizes(out->groups, lens.data(), (int)lens.size(), prefix_heads_);
+    out->sizes = ops::prefix_plan_sizes(out->groups, lens.data(), (int)lens.size(), prefix_heads_, kept.request.n_kv_heads);
     auto up = [](int n) {
         int p = 1;
         while (p < n) p *= 2;
@@ -474,7 +477,7 @@ LogitsRef Engine::decode_step_graphed(const StepPlan& plan, const std::vector<in
                                       const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes) {
     std::string key = std::string(adapters ? "da/" : "d/") + std::to_string(ids.size()) + "/" + std::to_string(want_rows.size());
     if (prefixes)
-        for (int n : {prefixes->sizes.tiles, prefixes->sizes.wide ? 1 : 0, prefixes->sizes.longest_prefix, prefixes->sizes.longest_rest}) key += "/" + std::to_string(n);
+        for (int n : {prefixes->sizes.tiles, prefixes->sizes.per_tile, prefixes->sizes.longest_prefix, prefixes->sizes.longest_rest}) key += "/" + std::to_string(n);
     auto it = graphs_.find(key);
     if (it == graphs_.end()) {
         graphs_[key].reset(new GraphEntry);

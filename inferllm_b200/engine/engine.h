@@ -34,6 +34,7 @@ struct EngineOptions {
     bool cuda_graphs = true;            // replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     std::string cache_dtype = "auto";   // keys and values: "auto" (as the compute dtype) or "int8" (a byte each and a scale per row, where a layer can)
     bool share_prefixes = false;        // the generation loop runs the first positions that all prompts of a batch have in common once
+    long long shared_prefix_bytes = -1; // decode steps walk common positions once where that saves so many bytes of a layer's cache; -1: by a rule
     int max_adapters = 0;               // low-rank adapters that may be loaded together (Engine::add_adapter)
     int adapter_rank = 16;              // the largest rank of one (at most 85: q, k and v stand side by side)
     std::string gemm = "auto";          // bfloat16 products: "auto" | "tc" | "library" (see ops::GemmBackend)
@@ -63,8 +64,11 @@ struct LogitsRef {
     long long rows = 0, vocab = 0;
 };
 
-// Positions that a decode step's common prefixes must save (a prefix counts once for every sequence but one) to be walked by themselves.
-constexpr long long kSharedPrefixMinSaved = 1024;
+// Bytes of keys and values (of a layer) that a decode step of n sequences must not have to read again to walk common prefixes by themselves: kSharedPrefixBytes
+// + n kSharedPrefixBytesEach (a prefix counts once for every sequence but one).  Measured per layer with rows of 128 bytes, 100 positions behind the prefix:
+// 4 sequences with 32 / 8 heads behind 2,048 positions (12.6 MB saved) 11.4 us, one by one 10.2, behind 4,096 (25 MB) 14.4 and 14.5; 16 with 32 / 32 heads behind 512
+// (63 MB) 21.1 and 15.6, behind 1,024 (126 MB) 21.9 and 25.0; 64 with 32 / 32 behind 128 (66 MB) 28.6 and 26.2, behind 256 (132 MB) 29.7 and 33.8.
+constexpr long long kSharedPrefixBytes = 10 << 20, kSharedPrefixBytesEach = 5 << 19;
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
 

@@ -1074,7 +1074,7 @@ Mat attention_int8(Device& dev, const Mat& q, const KVView& kv, const StepView& 
         float *acc = nullptr, *ml = nullptr;
         if (splits > 1 && !attention_pages_in_cluster(pairs, splits, dev.n_sms())) acc = shares(dev, n, g, splits, &ml);
         check_kernel(illm_attention_pages(row_ptr(q, t0), (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.token_pos + t0,
-                                          ctx.token_seq + t0, nullptr, nullptr, nullptr, 0, acc, ml, row_ptr(out, t0), (int)n, g.n_heads, g.n_kv_heads, g.head_dim,
+                                          ctx.token_seq + t0, nullptr, nullptr, nullptr, 0, 0, acc, ml, row_ptr(out, t0), (int)n, g.n_heads, g.n_kv_heads, g.head_dim,
                                           kv.page_size, kv.span(), scale, splits, 0, dev.tc_error_word(), dev.stream()),
                      "attention_pages");
     }
@@ -1106,7 +1106,7 @@ Mat attention_shared(Device& dev, const Mat& q, const KVView& kv, const StepView
                                                  dev.tc_error_word(), dev.stream()),
                      "attention_tiles_prefix");
     check_kernel(illm_attention_pages(q.p, (int)q.cols, kv.k, kv.v, kv.k_scale, kv.v_scale, kv.num_pages, kv.block_table, kv.width, ctx.token_pos, ctx.token_seq, start,
-                                      ctx.prefix_plan, members, s.wide ? 0 : s.tiles, acc, ml, out.p, (int)T, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, 0, scale,
+                                      ctx.prefix_plan, members, s.wide ? 0 : s.tiles, s.per_tile, acc, ml, out.p, (int)T, g.n_heads, g.n_kv_heads, g.head_dim, kv.page_size, 0, scale,
                                       own, kept, dev.tc_error_word(), dev.stream()),
                  "attention_pages");
     return out;

@@ -65,7 +65,7 @@ _KERNEL_SIGNATURES = {
     "illm_kv_write_int8": [P_, P_, I_, LL_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, I_, I_, P_, P_],
     "illm_kv_read_int8": [P_, P_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, I_, LL_, I_, I_, I_, P_],
     "illm_attention_int8": [P_, I_, P_, P_, P_, P_, P_, I_, LL_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, P_, P_],
-    "illm_attention_pages": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, F_, I_, I_, P_, P_],
+    "illm_attention_pages": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, P_, P_, I_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, F_, I_, I_, P_, P_],
     "illm_attention_tiles_int8": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, I_, I_, I_, I_, I_, I_, F_, I_, P_, P_],
     "illm_attention_tiles_cluster": [I_],
     "illm_attention_tiles_prefix": [P_, I_, P_, P_, P_, P_, LL_, P_, I_, P_, P_, P_, I_, P_, P_, I_, I_, I_, I_, F_, I_, I_, I_, P_, P_],
@@ -1143,7 +1143,7 @@ def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, 
             s = s if splits is None else int(splits)
             ws, acc, ml = (None, None, None) if s == 1 or _in_cluster(n * nkv, s, _sms[device.index]) else _shares(n, n_heads, s, d, device)
             _check(run(q.data_ptr() + t0 * stride * 2, stride, *cache.pointers, cache.pages, block_table.data_ptr(), width, token_pos.data_ptr() + 4 * t0,
-                       token_seq.data_ptr() + 4 * t0, None, None, None, 0, acc, ml, out.data_ptr() + t0 * n_heads * d * 2, n, n_heads, nkv, d, cache.page_size, span,
+                       token_seq.data_ptr() + 4 * t0, None, None, None, 0, 0, acc, ml, out.data_ptr() + t0 * n_heads * d * 2, n, n_heads, nkv, d, cache.page_size, span,
                        float(scale), s, 0, err, stream), "attention_decode_int8")
     return out
 
@@ -1176,20 +1176,20 @@ def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads
 class SharedPrefixes:
     """Which tokens of a step (one per sequence) see their first positions in common: `groups` of (positions, [tokens]), whose block tables name
     the same pages for those positions; `lens` [T] on the host: the positions that each token sees, its own included; `group_heads`: query heads per kv
-    head (at most 16).  Made once per step and used for every layer.  Tokens in no group are served too."""
+    head (at most 16); `n_kv_heads` only helps to choose between kernels.  Made once per step and used for every layer.  Tokens in no group are served too."""
 
-    def __init__(self, groups, lens, group_heads, device=None):
+    def __init__(self, groups, lens, group_heads, device=None, n_kv_heads=8):
         groups = [(int(p), [int(t) for t in m]) for p, m in groups]
         lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
         self.T, self.group_heads = len(lens), int(group_heads)
         self.device = torch.empty(0, device="cuda" if device is None else device).device
         sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
         args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), self.T,
-                self.group_heads, sizes, ctypes.byref(total))
+                self.group_heads, int(n_kv_heads), sizes, ctypes.byref(total))
         _b.check(_b.lib().illm_prefix_plan(*args, None))
         host = torch.zeros(max(1, total.value), dtype=torch.int32)
         _b.check(_b.lib().illm_prefix_plan(*args, ctypes.cast(host.data_ptr(), _b.PI)))
-        self.tiles, self.wide, self.longest_prefix, self.longest_rest = sizes[0], bool(sizes[1]), sizes[2], sizes[3]
+        self.tiles, self.wide, self.longest_prefix, self.longest_rest, self.per_tile = sizes[0], bool(sizes[1]), sizes[2], sizes[3], sizes[6]
         self.longest = max(lens)
         self.host = host
         self.plan = host.to(self.device)
@@ -1227,7 +1227,7 @@ def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n
         if common and plan.wide:
             _check(h.illm_attention_tiles_prefix(at, stride, *pointers, pages, table, width, seq, tiles, members, plan.tiles, acc, ml, n_heads, nkv, d, page_size,
                                                  float(scale), own + kept, own, pre, err, stream), "attention_decode_shared")
-        _check(h.illm_attention_pages(at, stride, *pointers, pages, table, width, pos, seq, start, tiles, members, 0 if plan.wide else plan.tiles, acc, ml,
+        _check(h.illm_attention_pages(at, stride, *pointers, pages, table, width, pos, seq, start, tiles, members, 0 if plan.wide else plan.tiles, plan.per_tile, acc, ml,
                                       out.data_ptr(), T, n_heads, nkv, d, page_size, 0, float(scale), own, kept, err, stream), "attention_decode_shared")
     return out
 

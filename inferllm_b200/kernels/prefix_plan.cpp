@@ -8,15 +8,15 @@
 namespace illm {
 namespace ops {
 
-static constexpr int kNarrowRows = 16, kWideRows = 256;
-// Groups of more rows than this take the wide tiles.
-static constexpr int kNarrowMost = 32;
+// Rows (members times G) of a tile, and up to which group the first of them are taken.
+static constexpr int kFewRows = 8, kFewMost = 8, kNarrowRows = 16, kWideRows = 256;
+// Narrow tiles times key/value heads from which on wide ones are taken where a group has more rows than a narrow one.
+static constexpr int kNarrowMost = 24;
 
-static int per_tile(bool wide, int G) { return (wide ? kWideRows : kNarrowRows) / G; }
-
-PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G) {
+PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G, int kv_heads) {
     if (T < 1 || T > 65535) throw KernelError("a plan of common prefixes takes 1 to 65535 tokens, found " + std::to_string(T));
     if (G < 1 || G > kNarrowRows) throw KernelError("a plan of common prefixes takes 1 to 16 query heads per key/value head, found " + std::to_string(G));
+    if (kv_heads < 1) throw KernelError("a plan of common prefixes needs at least one key/value head, found " + std::to_string(kv_heads));
     PrefixPlanSizes s;
     s.T = T;
     std::vector<int> start((size_t)T, 0);
@@ -34,9 +34,14 @@ PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const 
         rows = std::max(rows, (int)g.members.size() * G);
         s.longest_prefix = std::max(s.longest_prefix, g.prefix);
     }
-    s.wide = rows > kNarrowMost;
-    s.per_tile = per_tile(s.wide, G);
-    for (const PrefixGroup& g : groups) s.tiles += ((int)g.members.size() + s.per_tile - 1) / s.per_tile;
+    auto tiles_of = [&](int per) {
+        int n = 0;
+        for (const PrefixGroup& g : groups) n += ((int)g.members.size() + per - 1) / per;
+        return n;
+    };
+    s.wide = rows > kNarrowRows && (long long)tiles_of(kNarrowRows / G) * kv_heads >= kNarrowMost;
+    s.per_tile = (s.wide ? kWideRows : rows <= kFewMost && G <= kFewRows ? kFewRows : kNarrowRows) / G;
+    s.tiles = tiles_of(s.per_tile);
     for (int t = 0; t < T; t++) {
         if (lens[t] < 1) throw KernelError("token " + std::to_string(t) + " sees no position");
         s.longest_rest = std::max(s.longest_rest, lens[t] - start[(size_t)t]);

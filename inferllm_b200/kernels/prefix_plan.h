@@ -15,7 +15,7 @@ struct PrefixGroup {
 struct PrefixPlanSizes {
     int T = 0;                  // tokens of the step
     int tiles = 0;              // groups in pieces that fit the rows of a block's products
-    bool wide = false;          // pieces of 256 rows (attention_tiles.cu) or of 16 (attention_pages.cu)
+    bool wide = false;          // pieces of 256 rows (attention_tiles.cu) or of 8 or 16 (attention_pages.cu)
     int longest_prefix = 0;     // positions
     int longest_rest = 0;       // the most positions that a token has for itself
     int per_tile = 0;           // members that fit a tile
@@ -25,9 +25,9 @@ struct PrefixPlanSizes {
     int members_at() const { return 4 * tiles + (T + 3) / 4 * 4; }
 };
 
-// lens[t]: the positions that token t sees; G: query heads per key/value head, at most 16.  KernelError for a token outside the step or in
+// lens[t]: the positions that token t sees; G: query heads per key/value head, at most 16; kv_heads: key/value heads (for the choice of tiles alone).  KernelError for a token outside the step or in
 // two groups, an empty group, a prefix that is not positive or longer than a member sees.
-PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G);
+PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G, int kv_heads);
 // Fills out[0 .. sizes.ints()); sizes.tiles may be larger than the plan needs (the rest are empty tiles).
 void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& sizes, int* out);
 

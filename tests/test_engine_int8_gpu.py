@@ -222,20 +222,20 @@ SHARED = {"C": (640, 512), "D": (400, 320)}
 @pytest.mark.parametrize("graphs", [True, False])
 @pytest.mark.parametrize("cache", ["auto", "int8"])
 @pytest.mark.parametrize("name", ["C", "D"])
-@pytest.mark.parametrize("n", [4, 14])
+@pytest.mark.parametrize("n", [4, 14, 100])
 def test_forks_answer_as_if_they_were_alone(name, cache, graphs, n, model_folders, plain_models, monkeypatch, request):
     """Sequences that share a prefix with the one that made it, each with tokens of its own, beside one that shares nothing: enough of them that their
-    steps walk the prefix once (4: rows of one narrow tile's size, 14: wide ones)."""
+    steps walk the prefix once (in tiles of 8, 16 and 256 rows)."""
     if cache == "int8":
         request.getfixturevalue("rounded")
     cfg, w = plain_models[name]
-    e = engine(model_folders[name], cache=cache, cuda_graphs=graphs, max_tokens=8192, max_batch=n + 3)
+    e = engine(model_folders[name], cache=cache, cuda_graphs=graphs, max_tokens=8192 if n < 100 else 32768, max_batch=n + 3, shared_prefix_bytes=0)
     prompt = random_prompt(name, SHARED[name][0], 11)
     common = SHARED[name][1]
     slots = [e.new_sequence()]
     e.step([StepItem(slots[0], prompt, [])])
     slots += [e.fork_sequence(slots[0], common) for _ in range(n - 1)]
-    texts = [prompt] + [prompt[:common] + random_prompt(name, 3 + i, 200 + i) for i in range(n - 1)]
+    texts = [prompt] + [prompt[:common] + random_prompt(name, 3 + i % 40, 200 + i) for i in range(n - 1)]
     lone = random_prompt(name, 21, 12)
     slots.append(e.new_sequence())
     texts.append(lone)
@@ -266,6 +266,24 @@ def test_forks_answer_as_if_they_were_alone(name, cache, graphs, n, model_folder
         e.end_sequence(s)
     e.cache.check()
     assert e.cache.pages_free() == [e.limits().num_pages]
+
+
+def test_common_positions_are_walked_once_where_that_saves_enough(model_folders):
+    """A narrow tile adds the kernel that joins the shares, a wide one its own kernel too; a step that would save less is as before."""
+    launches = {}
+    for least in (0, 256 * 2 * 4 * 128 * 128, -1):
+        e = engine(model_folders["C"], cache="int8", cuda_graphs=False, max_batch=16, shared_prefix_bytes=least)
+        a = e.new_sequence()
+        e.step([StepItem(a, random_prompt("C", 256, 1), [])])
+        slots = [a] + [e.fork_sequence(a, 256) for _ in range(2)]
+        items = [StepItem(s, random_prompt("C", 1, 2 + i), [0]) for i, s in enumerate(slots)]
+        e.step(items)
+        before = ops.launch_count()
+        e.step(items)
+        launches[least] = ops.launch_count() - before
+        e.check_device_errors()
+    few, some, rule = launches.values()
+    assert few > some == rule
 
 
 @pytest.mark.parametrize("name, dtype, cache", [("A", "float32", "int8"), ("B", "float32", "auto"), ("B", "bfloat16", "int8"), ("D", "float32", "int8")])
