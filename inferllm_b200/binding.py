@@ -85,7 +85,7 @@ _SIGNATURES = {
     "illm_cache_plan_step": [P, PI, PI, I, PI, PLL, PI], "illm_cache_commit_step": [P, I], "illm_cache_abandon_step": [P, I],
     "illm_cache_stats": [P, PP],
     "illm_generate_with_callbacks": [P, I, PI, PI, LL, PI, I, PP], "illm_plan_batches": [PI, I, LL, I, I, I, LL, PP],
-    "illm_adapter_plan": [PI, I, PI, I, PI, PI, PI], "illm_prefix_plan": [I, PI, PI, PI, PI, I, I, I, PI, PI, PI],
+    "illm_adapter_plan": [PI, I, PI, I, PI, PI, PI], "illm_prefix_plan": [I, PI, PI, PI, PI, I, I, PI, PI, PI],
     "illm_engine_create": [P, S, PP], "illm_engine_from_folder": [S, S, S, PP], "illm_engine_free": [P],
     "illm_engine_load_folder": [P, S], "illm_engine_load_random": [P, ULL], "illm_engine_new_sequence": [P, PI],
     "illm_engine_end_sequence": [P, I], "illm_engine_sequence_length": [P, I, PLL], "illm_engine_limits": [P, PLL],

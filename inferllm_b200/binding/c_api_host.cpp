@@ -570,7 +570,7 @@ ILLM_API int illm_adapter_plan(const int* index, int T, const int* ranks, int co
 
 // The plan of a step's common prefixes: n_groups groups, group i with prefixes[i] positions and counts[i] members, which follow one another in
 // `members`; lens [T].  sizes: tiles, wide, longest prefix, longest rest, where start and members begin, members to a tile; out: nullptr, or `total` ints.
-ILLM_API int illm_prefix_plan(int n_groups, const int* prefixes, const int* counts, const int* members, const int* lens, int T, int G, int kv_heads, int* sizes, int* total, int* out) {
+ILLM_API int illm_prefix_plan(int n_groups, const int* prefixes, const int* counts, const int* members, const int* lens, int T, int G, int* sizes, int* total, int* out) {
     return guard([&] {
         std::vector<ops::PrefixGroup> groups((size_t)std::max(n_groups, 0));
         for (auto& g : groups) {
@@ -579,7 +579,7 @@ ILLM_API int illm_prefix_plan(int n_groups, const int* prefixes, const int* coun
             g.members.assign(members, members + std::max(counts[i], 0));
             members += std::max(counts[i], 0);
         }
-        const ops::PrefixPlanSizes s = ops::prefix_plan_sizes(groups, lens, T, G, kv_heads);
+        const ops::PrefixPlanSizes s = ops::prefix_plan_sizes(groups, lens, T, G);
         sizes[0] = s.tiles, sizes[1] = s.wide ? 1 : 0, sizes[2] = s.longest_prefix, sizes[3] = s.longest_rest, sizes[4] = s.start_at(), sizes[5] = s.members_at(), sizes[6] = s.per_tile;
         *total = s.ints();
         if (out) ops::prefix_plan_fill(groups, s, out);

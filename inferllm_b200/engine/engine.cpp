@@ -263,7 +263,7 @@ bool Engine::find_prefixes(const StepPlan& plan, StepPrefixes* out) const {
     std::vector<int> lens;
     for (size_t i = 0; i < plan.slots.size(); i++) lens.push_back((int)(plan.past[i] + 1));
     out->heads = prefix_heads_;
-    out->sizes = ops::prefix_plan_sizes(out->groups, lens.data(), (int)lens.size(), prefix_heads_, kept.request.n_kv_heads);
+    out->sizes = ops::prefix_plan_sizes(out->groups, lens.data(), (int)lens.size(), prefix_heads_);
     auto up = [](int n) {
         int p = 1;
         while (p < n) p *= 2;

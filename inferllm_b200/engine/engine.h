@@ -65,10 +65,10 @@ struct LogitsRef {
 };
 
 // Bytes of keys and values (of a layer) that a decode step of n sequences must not have to read again to walk common prefixes by themselves: kSharedPrefixBytes
-// + n kSharedPrefixBytesEach (a prefix counts once for every sequence but one).  Measured per layer with rows of 128 bytes, 100 positions behind the prefix:
-// 4 sequences with 32 / 8 heads behind 2,048 positions (12.6 MB saved) 11.4 us, one by one 10.2, behind 4,096 (25 MB) 14.4 and 14.5; 16 with 32 / 32 heads behind 512
-// (63 MB) 21.1 and 15.6, behind 1,024 (126 MB) 21.9 and 25.0; 64 with 32 / 32 behind 128 (66 MB) 28.6 and 26.2, behind 256 (132 MB) 29.7 and 33.8.
-constexpr long long kSharedPrefixBytes = 10 << 20, kSharedPrefixBytesEach = 5 << 19;
+// + n kSharedPrefixBytesEach (a prefix counts once for every sequence but one).  Measured with eight-bit rows of 128, a common prefix and 100 positions behind it, once
+// for all and one by one: 4 sequences of 32 / 32 heads at 256 positions (6 MB saved) 7.3 and 7.5 us, at 1,024 9.2 and 12.1, of 32 / 8 heads at 1,024 (6 MB) 8.8 and 8.0;
+// 16 of 32 / 8 at 1,024 (30 MB) 12.8 and 11.6, at 2,048 17.8 and 20.0; 64 of 32 / 8 at 512 (63 MB) 23 and 16, at 1,024 (126 MB) 23.7 and 25.4, at 2,048 24 and 44.
+constexpr long long kSharedPrefixBytes = 4 << 20, kSharedPrefixBytesEach = 3 << 19;
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
 

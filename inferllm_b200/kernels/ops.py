@@ -1176,16 +1176,16 @@ def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads
 class SharedPrefixes:
     """Which tokens of a step (one per sequence) see their first positions in common: `groups` of (positions, [tokens]), whose block tables name
     the same pages for those positions; `lens` [T] on the host: the positions that each token sees, its own included; `group_heads`: query heads per kv
-    head (at most 16); `n_kv_heads` only helps to choose between kernels.  Made once per step and used for every layer.  Tokens in no group are served too."""
+    head (at most 16).  Made once per step and used for every layer.  Tokens in no group are served too."""
 
-    def __init__(self, groups, lens, group_heads, device=None, n_kv_heads=8):
+    def __init__(self, groups, lens, group_heads, device=None):
         groups = [(int(p), [int(t) for t in m]) for p, m in groups]
         lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
         self.T, self.group_heads = len(lens), int(group_heads)
         self.device = torch.empty(0, device="cuda" if device is None else device).device
         sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
         args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), self.T,
-                self.group_heads, int(n_kv_heads), sizes, ctypes.byref(total))
+                self.group_heads, sizes, ctypes.byref(total))
         _b.check(_b.lib().illm_prefix_plan(*args, None))
         host = torch.zeros(max(1, total.value), dtype=torch.int32)
         _b.check(_b.lib().illm_prefix_plan(*args, ctypes.cast(host.data_ptr(), _b.PI)))

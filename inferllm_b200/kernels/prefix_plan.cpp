@@ -8,19 +8,20 @@
 namespace illm {
 namespace ops {
 
-// Rows (members times G) of a tile, and up to which group the first of them are taken.
-static constexpr int kFewRows = 8, kFewMost = 8, kNarrowRows = 16, kWideRows = 256;
-// Narrow tiles times key/value heads from which on wide ones are taken where a group has more rows than a narrow one.
-static constexpr int kNarrowMost = 24;
+// Rows (members times G) of a tile: wide, or narrow.  Narrow tiles of eight rows leave a block half the registers of sixteen, so that twice as many share an SM, and are
+// taken while they hold two members (16 sequences of 32 / 32 heads behind 2,048 positions 17.0 us and 23.2; of 32 / 8 heads 13.9 and 17.1).
+static constexpr int kFewRows = 8, kNarrowRows = 16, kWideRows = 256;
+// Wide tiles where a group takes more narrow ones than this: 32 / 32 heads behind 8,192 positions, 32 sequences 52 us narrow and 54 wide, 48 sequences 71 and 59, 128
+// sequences 180 and 86; 32 / 8 heads, 8 sequences 20 and 19, 16 sequences 30 and 24; behind 512 positions the two are nearly alike.
+static constexpr int kNarrowMost = 4;
 
-PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G, int kv_heads) {
+PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G) {
     if (T < 1 || T > 65535) throw KernelError("a plan of common prefixes takes 1 to 65535 tokens, found " + std::to_string(T));
     if (G < 1 || G > kNarrowRows) throw KernelError("a plan of common prefixes takes 1 to 16 query heads per key/value head, found " + std::to_string(G));
-    if (kv_heads < 1) throw KernelError("a plan of common prefixes needs at least one key/value head, found " + std::to_string(kv_heads));
     PrefixPlanSizes s;
     s.T = T;
     std::vector<int> start((size_t)T, 0);
-    int rows = 0;
+    int most = 0;               // members of a group
     for (const PrefixGroup& g : groups) {
         if (g.members.empty()) throw KernelError("a group of tokens with a common prefix needs at least one token");
         if (g.prefix < 1) throw KernelError("a common prefix must have at least one position, found " + std::to_string(g.prefix));
@@ -31,17 +32,13 @@ PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const 
                 throw KernelError("token " + std::to_string(t) + " sees " + std::to_string(lens[t]) + " positions, fewer than the common prefix of " + std::to_string(g.prefix));
             start[(size_t)t] = g.prefix;
         }
-        rows = std::max(rows, (int)g.members.size() * G);
+        most = std::max(most, (int)g.members.size());
         s.longest_prefix = std::max(s.longest_prefix, g.prefix);
     }
-    auto tiles_of = [&](int per) {
-        int n = 0;
-        for (const PrefixGroup& g : groups) n += ((int)g.members.size() + per - 1) / per;
-        return n;
-    };
-    s.wide = rows > kNarrowRows && (long long)tiles_of(kNarrowRows / G) * kv_heads >= kNarrowMost;
-    s.per_tile = (s.wide ? kWideRows : rows <= kFewMost && G <= kFewRows ? kFewRows : kNarrowRows) / G;
-    s.tiles = tiles_of(s.per_tile);
+    const int narrow = (2 * G <= kFewRows ? kFewRows : kNarrowRows) / G;
+    s.wide = most > kNarrowMost * narrow;
+    s.per_tile = s.wide ? kWideRows / G : narrow;
+    for (const PrefixGroup& g : groups) s.tiles += ((int)g.members.size() + s.per_tile - 1) / s.per_tile;
     for (int t = 0; t < T; t++) {
         if (lens[t] < 1) throw KernelError("token " + std::to_string(t) + " sees no position");
         s.longest_rest = std::max(s.longest_rest, lens[t] - start[(size_t)t]);

@@ -25,9 +25,9 @@ struct PrefixPlanSizes {
     int members_at() const { return 4 * tiles + (T + 3) / 4 * 4; }
 };
 
-// lens[t]: the positions that token t sees; G: query heads per key/value head, at most 16; kv_heads: key/value heads (for the choice of tiles alone).  KernelError for a token outside the step or in
+// lens[t]: the positions that token t sees; G: query heads per key/value head, at most 16.  KernelError for a token outside the step or in
 // two groups, an empty group, a prefix that is not positive or longer than a member sees.
-PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G, int kv_heads);
+PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const int* lens, int T, int G);
 // Fills out[0 .. sizes.ints()); sizes.tiles may be larger than the plan needs (the rest are empty tiles).
 void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& sizes, int* out);
 

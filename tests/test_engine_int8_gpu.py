@@ -225,7 +225,7 @@ SHARED = {"C": (640, 512), "D": (400, 320)}
 @pytest.mark.parametrize("n", [4, 14, 100])
 def test_forks_answer_as_if_they_were_alone(name, cache, graphs, n, model_folders, plain_models, monkeypatch, request):
     """Sequences that share a prefix with the one that made it, each with tokens of its own, beside one that shares nothing: enough of them that their
-    steps walk the prefix once (in tiles of 8, 16 and 256 rows)."""
+    steps walk the prefix once (in tiles of 8 and 256 rows)."""
     if cache == "int8":
         request.getfixturevalue("rounded")
     cfg, w = plain_models[name]

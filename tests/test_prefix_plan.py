@@ -7,9 +7,9 @@ from inferllm_b200 import binding as _b
 from inferllm_b200.binding import KernelError
 
 
-def plan(groups, lens, G, kv_heads=8):
+def plan(groups, lens, G):
     sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
-    args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), len(lens), G, kv_heads,
+    args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), len(lens), G,
             sizes, ctypes.byref(total))
     _b.check(_b.lib().illm_prefix_plan(*args, None))
     out = (ctypes.c_int * max(1, total.value))()
@@ -45,8 +45,7 @@ def test_every_member_is_in_one_tile_that_fits(G, counts):
     want = {t: length for length, m in groups for t in m}
     assert covered(p) == want
     assert p["start"] == [want.get(t, 0) for t in range(tokens)]
-    most = max(counts) * G
-    assert p["per"] == (256 if p["wide"] else 8 if most <= 8 else 16) // G and all(1 <= n for n, *_ in p["tiles"])
+    assert p["per"] == (256 if p["wide"] else 8 if G <= 4 else 16) // G and all(1 <= n for n, *_ in p["tiles"])
     assert p["longest_prefix"] == 64 * len(counts)
     assert p["longest_rest"] == max(n - want.get(t, 0) for t, n in enumerate(lens))
 
@@ -54,9 +53,8 @@ def test_every_member_is_in_one_tile_that_fits(G, counts):
 def test_groups_of_many_rows_take_wide_tiles():
     assert not plan([(64, [0, 1])], [65, 65], 16)["wide"]
     assert plan([(64, list(range(64)))], [65] * 64, 4)["wide"]
-    # where there are enough of them
-    assert not plan([(64, list(range(8)))], [65] * 8, 4)["wide"] and plan([(64, list(range(8)))], [65] * 8, 4, 32)["wide"]
-    assert not plan([(64, list(range(16)))], [65] * 16, 1, 32)["wide"]
+    for G, most in ((1, 32), (4, 8), (5, 12), (16, 4)):
+        assert not plan([(64, list(range(most))), (64, [most + 1])], [65] * (most + 2), G)["wide"] and plan([(64, list(range(most + 1)))], [65] * (most + 1), G)["wide"]
 
 
 def test_no_groups_is_a_plan():
