@@ -632,8 +632,8 @@ static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc
 // their pre_splits shares are what the launch before this one makes, which has to be illm_attention_tiles_prefix's (slot0 = own_splits): the two run side by side.  own_splits, pre_splits: at most 32 each,
 // pre_splits 0 without a plan.  Scratch: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2], or, without a plan and with up to 8 splits,
 // nullptr: then the blocks of a (token, kv head) are a cluster and there is no second kernel.  That is the faster way while the blocks find room together (one
-// sequence of 8 kv heads at 1,777 keys 7.3 us and 9), and the slower one where they have to wait for one another's places (64 sequences of 32 kv heads at 300
-// keys in two parts 60 us and 46).  err: 7 a wait ran out, 8 a visible position without a page.
+// sequence of 8 kv heads at 1,777 keys 6.6 us and 7.3), and the slower one where they have to wait for one another's places (64 sequences of 32 kv heads at 300
+// keys in two parts 57 us and 47).  err: 7 a wait ran out, 8 a visible position without a page.
 extern "C" int illm_attention_pages(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                     const int* block_table, int max_pages, const int* token_pos, const int* token_seq, const int* plan_start, const int* plan_tiles,
                                     const int* plan_members, int n_tiles, int per_tile, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int d, int page_size,

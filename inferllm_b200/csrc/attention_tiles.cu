@@ -179,7 +179,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         nb[1] = n_rows > TL_BM ? n : 0;
     } else {
         // Blocks with the most keys before them start first: the longest sequences (of up to 128, by counting those that come before), and of each the last tile.
-        // (Sixteen unequal prompts of 2,048 tokens together, in the order of the step: 75 us.)
+        // (Sixteen unequal prompts of 2,048 tokens together 70 us, in the order of the step 74.)
         hk = blockIdx.x;
         seq = blockIdx.z;
         if (gridDim.z > 1 && gridDim.z <= TL_ORDERED) {
@@ -660,7 +660,8 @@ extern "C" int illm_attention_tiles_int8(const void* q, int q_stride, const void
     if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || !ksc || B > 65535 || (tile_rows && tile_rows != TL_BM && tile_rows != 2 * TL_BM) || !out ||
         ((uintptr_t)out & 15))
         return ILLM_ERR_BAD_ARG;
-    // two tiles a block over the same keys, or one while that leaves SMs without a block
+    // two tiles a block over the same keys, or one while that leaves SMs without a block (32 / 8 heads: one prompt of 200 tokens 8.7 us with one tile, 11.3 with two;
+    // sixteen of 2,048 together 93 and 70)
     if (tile_rows == 0) tile_rows = ((long long)max_q * (nh / nkv) + 2 * TL_BM - 1) / (2 * TL_BM) * nkv * B < illm_sm_count() ? TL_BM : 2 * TL_BM;
     const long long tiles = ((long long)max_q * (nh / nkv) + tile_rows - 1) / tile_rows;
     if (tiles > 65535 || (long long)max_q * (nh / nkv) > 0x7fffffffLL) return ILLM_ERR_BAD_ARG;

@@ -212,7 +212,8 @@ extern "C" int illm_kv_write_int8(const void* qkv, const float* partials, int sp
     if (((uintptr_t)qkv & 15) || ((uintptr_t)partials & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)cos_sin & 15)) return ILLM_ERR_BAD_ARG;
     const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, at_once = KQ_THREADS / lanes;
     const int n_slots = nh + (write_kv ? 2 * nkv : 0), rounds_all = (n_slots + at_once - 1) / at_once;
-    // several heads to a thread once that leaves eight blocks to every SM
+    // several heads to a thread once that leaves eight blocks to every SM (4,096 tokens of 32 + 16 heads written and read back 31.3 us, one head to a thread 37.1; 8 tokens
+    // of 32 + 64 heads 4.2 with one, 4.9 with four)
     const bool wide = (rot & 7) == 0;
     int rounds = 1;
     if (wide && !partials)
