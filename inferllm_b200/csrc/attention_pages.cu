@@ -128,7 +128,7 @@ struct PgPlan {
 
 // Stages: as many as leave four blocks to an SM (five at head size 64, three of bfloat16 rows), or with sixteen rows, whose registers leave two blocks, more.  The blocks
 // are short (one takes a few tiles after it has waited for its first), so that more of them are worth more than deeper rings: 64 sequences of 32 kv heads at
-// 300 keys 37.8 us with two blocks of six stages, 31.7 with three of four, 28.0 with four of three.
+// 300 keys 46.7 us with two blocks of six stages, 38.3 with three of four, 37.1 with four of three (64 sequences of 8 kv heads at up to 8,192 keys 130, 115 and 118).
 template <int D, bool Q8, int NT> struct PgRing {
     static constexpr int TILE = PG_BN * D * (Q8 ? 1 : 2), SCALES = Q8 ? 2 * PG_BN * 4 : 0;
     static constexpr int STAGES = !Q8 ? 256 / D : NT == 1 ? (D == 128 ? 3 : 4) : (D == 128 ? 4 : 6), BYTES = STAGES * (2 * TILE + SCALES) + 1024;

@@ -58,8 +58,8 @@ __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float
 }
 
 // LANES: lanes of a row, eight channels each.  WIDE (rot a multiple of 8): a lane of the rotated part has four channels and the four that they are turned with, so
-// that it needs no other lane's and each of its cosines once (with eight neighbours a lane, and their partners fetched beside them, 4,096 tokens of 32 + 16
-// heads of 128 took 27 us).  Otherwise it has eight neighbours and fetches their partners one by one.  A block takes ROUNDS times
+// that it needs no other lane's and each of its cosines once (4,096 tokens of 32 + 16 heads of 128 take 24 us, bound by instructions, 64 % of the issue slots; with eight
+// neighbours a lane, and their partners fetched beside them, 27).  Otherwise it has eight neighbours and fetches their partners one by one.  A block takes ROUNDS times
 // KQ_THREADS / LANES heads of one token.
 template <typename TA, bool PARTIALS, bool WIDE, int LANES, int ROUNDS>
 __global__ void __launch_bounds__(KQ_THREADS, WIDE && !PARTIALS && sizeof(TA) == 2 ? 5 : 4)

@@ -1,5 +1,6 @@
 #include "engine/engine.h"
 
+#include <climits>
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -28,7 +29,8 @@ EngineOptions EngineOptions::from_json(const Json& j) {
     if (j.at("poison_freed_pages").is_bool()) o.poison_freed_pages = j.at("poison_freed_pages").as_bool();
     if (j.has("cache_dtype") && j.at("cache_dtype").is_string()) o.cache_dtype = j.at("cache_dtype").as_string();
     if (j.has("share_prefixes") && j.at("share_prefixes").is_bool()) o.share_prefixes = j.at("share_prefixes").as_bool();
-    if (j.has("shared_prefix_bytes") && j.at("shared_prefix_bytes").is_int()) o.shared_prefix_bytes = j.at("shared_prefix_bytes").as_int();
+    if (j.has("shared_prefix_bytes") && j.at("shared_prefix_bytes").is_number())      // (numbers of 19 digits come as float64)
+        o.shared_prefix_bytes = j.at("shared_prefix_bytes").as_double() >= 9e18 ? LLONG_MAX : j.at("shared_prefix_bytes").as_int();
     if (j.at("stream").is_int()) o.stream = (void*)(uintptr_t)j.at("stream").as_int();
     return o;
 }
