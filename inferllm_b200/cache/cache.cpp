@@ -407,6 +407,8 @@ int SequenceCache::fork_slot(int from, long long length) {
 
 std::vector<std::pair<int, std::vector<int>>> SequenceCache::common_prefixes(const std::vector<int>& step_slots) const {
     std::vector<std::pair<int, std::vector<int>>> out;
+    for (int s : step_slots)
+        if (!slots.is_held(s)) throw CacheError("slot " + std::to_string(s) + " is not live");
     if (!can_fork() || step_slots.size() < 2) return out;
     const PageLedger& l = *paged[0].ledger;        // (pages are shared in all groups alike)
     std::map<int, std::vector<int>> by_first;

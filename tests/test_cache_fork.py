@@ -88,6 +88,9 @@ def test_refusals():
     for slot in (1, 5, -1):
         with pytest.raises(CacheError):
             c.fork_slot(slot, 4)
+    for slots in ([a, 1], [a, 2], [-1, a], [2 ** 31 - 1, a]):
+        with pytest.raises(CacheError, match="not live"):
+            c.common_prefixes(slots)
     c.fork_slot(a, 4)
     with pytest.raises(CacheFull):
         c.fork_slot(a, 4)

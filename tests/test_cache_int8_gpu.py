@@ -338,6 +338,47 @@ def test_scales_of_any_size(ops, power):
     near(got, want, tol)
 
 
+@pytest.mark.parametrize("power", [-100, 100])
+def test_scales_of_any_size_on_wide_tiles(ops, power):
+    """The same for prompts and for a common prefix of many rows, whose weights carry the values' scales in bfloat16's range."""
+    nh, nkv, d, n = 8, 2, 128, 20
+    lens = [150 + i for i in range(n)]
+    pages = Pages(17, lens, nkv, d, common=[(128, 0)] * n)
+    pages.vs *= 2.0 ** power
+    pages.ks *= 2.0 ** -power
+    scale = d ** -0.5 * 2.0 ** power
+    pos, seq = torch.tensor(lens, dtype=torch.int32).cuda() - 1, torch.arange(n, dtype=torch.int32).cuda()
+    q = queries(3, n, nh * d)
+    want, tol = expected(pages, q, [(i, m - 1) for i, m in enumerate(lens)], nh, 0, scale, B16)
+    plan = ops.SharedPrefixes([(128, list(range(n)))], lens, nh // nkv)
+    assert plan.wide
+    near(ops.attention_decode_shared(q.cuda(), pages.cache(ops), pages.table.cuda(), pos, seq, plan, nh, scale, max(lens)), want, tol)
+    cu = torch.arange(0, n + 1, dtype=torch.int32).cuda()
+    near(ops.attention_prompts_int8(q.cuda(), pages.cache(ops), pages.table.cuda(), cu, pos + 1, 1, nh, 0, scale), want, tol)
+    assert take_error(ops) == 0
+
+
+def test_launches_that_wait_for_the_whole_of_the_one_before(ops):
+    """Without programmatic launches the kernels of a call follow one another: the same bits."""
+    nh, nkv, d, n = 8, 2, 64, 40
+    lens = [300 + 3 * i for i in range(n)]
+    pages = Pages(23, lens, nkv, d, common=[(256, 0)] * n)
+    pos, seq = torch.tensor(lens, dtype=torch.int32).cuda() - 1, torch.arange(n, dtype=torch.int32).cuda()
+    q, cache, table = queries(5, n, nh * d).cuda(), pages.cache(ops), pages.table.cuda()
+    for groups in ([(256, list(range(n)))], [(256, list(range(i, i + 4))) for i in range(0, n, 4)]):
+        plan = ops.SharedPrefixes(groups, lens, nh // nkv)
+        got = []
+        try:
+            for on in (True, False):
+                ops.set_pdl(on)
+                got.append([ops.attention_decode_shared(q, cache, table, pos, seq, plan, nh, 0.1, max(lens)) for _ in range(3)])
+                torch.cuda.synchronize()
+        finally:
+            ops.set_pdl(True)
+        assert all(torch.equal(got[0][0], g) for row in got for g in row)
+    assert take_error(ops) == 0
+
+
 def test_queries_of_any_size(ops):
     for power in (-120, -60, 60, 100):
         pages = Pages(17, [300, 64], 2, 64)
@@ -632,8 +673,7 @@ def test_two_calls_at_once(ops):
     """Calls on two streams, none of which waits for the other, have scratch of their own: each gives what it gives alone."""
     nh, nkv, d, n = 32, 8, 128, 40
     lens = [600 + 7 * i for i in range(n)]
-    common = [(0, None)] + [(512, 0)] * (n - 1)
-    pages = Pages(91, lens, nkv, d, common=common)
+    pages = Pages(91, lens, nkv, d, common=[(512, 0)] * n)
     cache, table = pages.cache(ops), pages.table.cuda()
     pos, seq = torch.tensor(lens, dtype=torch.int32).cuda() - 1, torch.arange(n, dtype=torch.int32).cuda()
     plan = ops.SharedPrefixes([(512, list(range(n)))], lens, nh // nkv)
