@@ -171,7 +171,7 @@ class SequenceCache:
         return cls(None, 0, 0, 0, 0, _wrap=sequence_cache_ptr, _owner=owner)
 
     def __del__(self):
-        if self._ptr and _b._lib is not None:
+        if getattr(self, "_ptr", None) and _b._lib is not None:
             _b._lib.illm_cache_free_handle(self._ptr)
 
     def stats(self) -> dict:
