@@ -346,6 +346,58 @@ def test_adapters_and_shared_positions(model_folders):
     assert tokens[0] == tokens[1]
 
 
+def some_adapters(e, n):
+    g = torch.Generator().manual_seed(5)
+    shapes = {k: v for k, v in e.adapted().items() if "k_proj" in k or "q_proj" in k or "down_proj" in k}
+    return [e.add_adapter({k: (torch.randn((4, v[1]), generator=g) * v[1] ** -0.5, torch.randn((v[0], 4), generator=g) * 0.2) for k, v in shapes.items()}) for _ in range(n)]
+
+
+@pytest.mark.parametrize("cache", ["auto", "int8"])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_adapters_beside_a_plan_of_common_positions(cache, graphs, model_folders):
+    """Steps that bring both plans, eager and captured, with groups that change: as the steps that walk every sequence by itself."""
+    name, got = "C", []
+    prompt = random_prompt(name, 300, 1)
+    for least in (0, 2 ** 62):
+        e = engine(model_folders[name], cache=cache, cuda_graphs=graphs, max_batch=8, shared_prefix_bytes=least, max_adapters=2, adapter_rank=4)
+        one, two = some_adapters(e, 2)
+        a = e.new_sequence()
+        e.step([StepItem(a, prompt, [], one)])
+        slots = [a] + [e.fork_sequence(a, 256) for _ in range(4)]
+        lone = e.new_sequence()
+        e.step([StepItem(s, random_prompt(name, 3 + i, 10 + i), [], one) for i, s in enumerate(slots[1:])] + [StepItem(lone, prompt[:40], [], two)])
+        out = []
+        for j in range(6):
+            order = slots + [lone] if j != 4 else [lone] + slots[::-1]
+            logits = e.step([StepItem(s, random_prompt(name, 1, 100 + 10 * j + slots.index(s) if s != lone else 99), [0], two if s == lone else one) for s in order]).cpu().numpy()
+            out += [logits[order.index(s)] for s in slots + [lone]]
+        e.check_device_errors()
+        got.append(np.stack(out))
+    assert_close(got[0], got[1], "bfloat16")
+
+
+def test_adapters_over_rows_of_eight_bits(model_folders):
+    """In float32 a request's tokens do not depend on what else is in the step."""
+    e = engine(model_folders["C"], "float32", max_batch=8, max_adapters=2, adapter_rank=4)
+    one, two = some_adapters(e, 2)
+    requests = [(random_prompt("C", 40 + 9 * i, i), a) for i, a in enumerate((one, two, -1))]
+
+    def run(some):
+        slots, out = [e.new_sequence() for _ in some], []
+        out.append(e.step([StepItem(s, p, [len(p) - 1], a) for s, (p, a) in zip(slots, some)]).cpu())
+        for j in range(4):
+            out.append(e.step([StepItem(s, random_prompt("C", 1, 50 + j), [0], a) for s, (_, a) in zip(slots, some)]).cpu())
+        for s in slots:
+            e.end_sequence(s)
+        return torch.stack(out, 1)
+
+    together = run(requests)
+    for i, r in enumerate(requests):
+        assert_close(run([r])[0].numpy(), together[i].numpy(), "float32")
+    assert (together[0] - together[2]).abs().max() > 0
+    e.check_device_errors()
+
+
 def test_the_cache_takes_half_the_room(model_folders):
     pages = [engine(model_folders["C"], cache=c, max_tokens=None, mem_fraction=0.02, max_batch=4).limits().num_pages for c in ("auto", "int8")]
     assert 1.85 <= pages[1] / pages[0] <= 2 * 128 / 132 + 0.01
