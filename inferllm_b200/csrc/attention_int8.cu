@@ -3,15 +3,17 @@
 //
 // o = sum_j p_j s^v_j (u^v_j - 128), p = softmax over the visible j of scale s^k_j sum_c q_c (u^k_jc - 128)
 // (src/kern/naive/naive.cpp:576-604, :531-553, :209-240, :634-662).
-// A block takes one (token, head).  Its four warps walk the visible keys 32 at a time: a lane makes the score of one key alone (its
+// A block takes one (token, head).  Its eight warps walk the visible keys 32 at a time: a lane makes the score of one key alone (its
 // row in eight-byte pieces, the query from shared memory), the warp agrees on the running maximum, and for the values the lanes
 // change roles, a lane for eight channels; what the warps have is added up at the end in ascending order.  A score and a weight
-// are float32.  Bound by its loads, which lie a row apart between lanes (a lane's 16 loads of a row of 128 share its four sectors).
+// are float32.  Bound by its loads, which lie a row apart between lanes (a lane's 16 loads of a row of 128 share its four sectors), four of
+// them in flight: 8 sequences of up to 4,096 positions with 32 / 32 heads of 128 in float32 223 us, 64 of 2,048 with heads of 96 in bfloat16 400 and one 53 (one load
+// at a time 350, 646 and 85; four warps besides 660, 651 and 160; sixteen warps 336, 1,140 and 49).
 #include <math.h>
 
 #include "common.cuh"
 
-#define AI_WARPS 4
+#define AI_WARPS 8
 
 template <typename TA>
 __global__ void __launch_bounds__(AI_WARPS * 32)
@@ -39,6 +41,7 @@ attention_int8_kernel(const TA* __restrict__ q, int q_stride, const unsigned cha
         if (row >= 0) {
             float dot = 0.f;
             const unsigned char* k = kc + row * d;
+#pragma unroll 4
             for (int c = 0; c < pieces; c++) {
                 const uint2 w = *reinterpret_cast<const uint2*>(k + c * 8);
 #pragma unroll
@@ -54,11 +57,11 @@ attention_int8_kernel(const TA* __restrict__ q, int q_stride, const unsigned cha
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[i] *= keep;
         const int n = min(32, p - j0 + 1);
+#pragma unroll 4
         for (int i = 0; i < n; i++) {
             const float f = __shfl_sync(0xffffffffu, wv, i);
             const long long r = __shfl_sync(0xffffffffu, row, i);
-            if (r < 0 || lane >= pieces) continue;
-            const uint2 v = *reinterpret_cast<const uint2*>(vc + r * d + lane * 8);
+            const uint2 v = r < 0 || lane >= pieces ? make_uint2(0x80808080u, 0x80808080u) : *reinterpret_cast<const uint2*>(vc + r * d + lane * 8);
 #pragma unroll
             for (int k = 0; k < 8; k++) acc[k] = fmaf(f, (float)((int)((k < 4 ? v.x : v.y) >> (8 * (k & 3)) & 255u) - 128), acc[k]);
         }
