@@ -86,6 +86,12 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     const int num_slots = options.max_batch > 0 ? options.max_batch : num_pages;
     cache_.reset(new SequenceCache(requests, num_slots, num_pages, options.page_size, max_seq, device_.get(), dtype,
                                    options.poison_freed_pages));
+    for (int entry : model_->prefix_entries()) {
+        if (cache_->kind_of(entry) != SequenceCache::KV) continue;
+        const SequenceCache::PagedGroup& g = cache_->paged[(size_t)cache_->group_of(entry)];
+        const long long bytes = (long long)(g.page_bytes + g.v_page_bytes);
+        prefix_page_bytes_ = prefix_page_bytes_ ? std::min(prefix_page_bytes_, bytes) : bytes;
+    }
     builder_.reset(new StepContextBuilder(device_.get(), &rt_));
     for (TokRead& t : tok_reads_) check_cuda(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming), "cudaEventCreate");
     // say once which attention kernels the model's layers get: a head size that the tensor-core kernels
@@ -250,11 +256,10 @@ StepContext Engine::make_context(const StepPlan& plan, const std::vector<int>& i
 // The common prefixes of a decode step's sequences, where walking them once saves more than the second launch of it costs.  What the launches depend on
 // (tiles, the splits that follow from the lengths) is rounded up, so that captured steps of growing sequences can be replayed.
 bool Engine::find_prefixes(const StepPlan& plan, StepPrefixes* out) const {
-    if (!prefix_heads_ || plan.slots.size() < 2) return false;
-    const SequenceCache::PagedGroup& kept = cache_->paged[0];
+    if (!prefix_heads_ || plan.slots.size() < 2 || plan.slots.size() > kSharedPrefixSequences) return false;
     long long saved = 0;
     for (auto& g : cache_->common_prefixes(plan.slots)) {
-        saved += g.first / cache_->page_size * (long long)(kept.page_bytes + kept.v_page_bytes) * ((long long)g.second.size() - 1);
+        saved += g.first / cache_->page_size * prefix_page_bytes_ * ((long long)g.second.size() - 1);
         ops::PrefixGroup group;
         group.prefix = g.first;
         group.members = g.second;
@@ -326,9 +331,9 @@ LogitsRef Engine::step(const std::vector<StepItem>& items, const int* device_ids
     }
     StepPlan plan = cache_->plan_step(slots, q_lens);
     LogitsRef logits;
-    StepPrefixes step_prefixes;
-    const StepPrefixes* prefixes = ids.size() == items.size() && find_prefixes(plan, &step_prefixes) ? &step_prefixes : nullptr;
     try {
+        StepPrefixes step_prefixes;
+        const StepPrefixes* prefixes = ids.size() == items.size() && find_prefixes(plan, &step_prefixes) ? &step_prefixes : nullptr;
         if (options_.cuda_graphs && ids.size() == items.size() && graph_safe_) {
             if (adapters) size_adapters(*adapters, true, false);
             logits = decode_step_graphed(plan, ids, want_rows, device_ids, adapters, prefixes);

@@ -69,6 +69,7 @@ struct LogitsRef {
 // for all and one by one: 4 sequences of 32 / 32 heads at 256 positions (6 MB saved) 7.3 and 7.5 us, at 1,024 9.2 and 12.1, of 32 / 8 heads at 1,024 (6 MB) 8.8 and 8.0;
 // 16 of 32 / 8 at 1,024 (30 MB) 12.8 and 11.6, at 2,048 17.8 and 20.0; 64 of 32 / 8 at 512 (63 MB) 23 and 16, at 1,024 (126 MB) 23.7 and 25.4, at 2,048 24 and 44.
 constexpr long long kSharedPrefixBytes = 4 << 20, kSharedPrefixBytesEach = 3 << 19;
+constexpr size_t kSharedPrefixSequences = 32768;       // a plan's tiles, rounded up to a power of two, still are rows of a grid; larger steps read every sequence by itself
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
 
@@ -161,6 +162,7 @@ private:
     bool loaded_ = false;
     std::vector<int> adapter_ranks_;        // 0: free
     int pad_safe_ = -1, graph_safe_ = -1, prefix_heads_ = 0;
+    long long prefix_page_bytes_ = 0;       // of a page of keys and values in the entries of the layers that walk common prefixes (the least, where they differ)
     size_t last_upload_bytes_ = 0;
 
     std::unique_ptr<StepContextBuilder> builder_;

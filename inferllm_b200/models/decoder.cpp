@@ -106,6 +106,13 @@ int DecoderModel::prefix_heads() const {
     return heads;
 }
 
+std::set<int> DecoderModel::prefix_entries() const {
+    std::set<int> out;
+    for (const ScheduleEntry& e : spec.schedule)
+        if (layers_[(size_t)e.layer].mixer->prefix_heads()) out.insert(e.cache);
+    return out;
+}
+
 std::map<int, CacheRequest> DecoderModel::cache_requests(bool int8) const {
     std::map<int, CacheRequest> out;
     for (const ScheduleEntry& e : spec.schedule)

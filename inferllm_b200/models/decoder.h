@@ -9,6 +9,7 @@
 #include <functional>
 #include <map>
 #include <memory>
+#include <set>
 #include <string>
 #include <vector>
 
@@ -43,6 +44,8 @@ public:
     std::map<int, CacheRequest> cache_requests(bool int8 = false) const;
     // Query heads per kv head of the layers that walk common prefixes once (Mixer::prefix_heads); 0: no layer does, or they differ.
     int prefix_heads() const;
+    // The cache entries of those layers.
+    std::set<int> prefix_entries() const;
     // Run the tokens of one step; float32 logits [ctx.K, vocab] (rows == 0 when nothing is wanted).
     Mat forward(const StepContext& ctx, const SequenceCache& cache, const std::vector<const int*>& tables_dev);
     // Low-rank adapters: the names (as in the weight file) of the matrices beside which they can stand, with their shapes; room

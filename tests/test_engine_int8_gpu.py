@@ -433,3 +433,22 @@ def test_command_line(model_folders):
     assert out.returncode == 0, out.stderr
     bad = subprocess.run([f"{ROOT}/bin/llama", "-m", model_folders["C"], "--prompt-ids", "1,2", "-n", "1", "--cache-dtype", "int3"], capture_output=True, text=True, timeout=300)
     assert bad.returncode != 0 and "cache_dtype" in bad.stderr
+
+
+def test_a_step_of_more_sequences_than_a_plan_takes(model_folders):
+    """It reads common positions for every sequence, and the pages that it brings are the sequences' own."""
+    n = 65600
+    e = engine(model_folders["C"], max_tokens=64 * (n + 70), max_batch=n + 2, max_seq_len=192, shared_prefix_bytes=0)
+    prompt, last = random_prompt("C", 64, 1), random_prompt("C", 1, 2)
+    a = e.new_sequence()
+    e.step([StepItem(a, prompt, [])])
+    slots = [e.fork_sequence(a, 64) for _ in range(n)]
+    free = e.cache.pages_free()
+    some = [0, 1, 32768, 65535, 65536, n - 1]
+    got = e.step([StepItem(s, last, [0] if i in some else []) for i, s in enumerate(slots)]).cpu().numpy()
+    e.check_device_errors()
+    assert e.cache.pages_free() == [f - n for f in free]
+    alone = e.step([StepItem(a, last, [0])]).cpu().numpy()
+    for i in range(len(some)):
+        assert_close(got[i:i + 1], alone, "bfloat16", f"sequence {some[i]}")
+    e.cache.check()
