@@ -949,10 +949,21 @@ def _rows_beside(x, M, cols, dtype):
     return x.new_empty(M, cols) if x.dtype is dtype else x.new_empty(M, cols, dtype=dtype)
 
 
-class CacheInt8:
+class _Fixed:
+    """What a call takes from it (sizes, addresses) is looked up once, so it stays as it was made: to have other tensors make another."""
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} is not changed: make another")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} is not taken away")
+
+
+class CacheInt8(_Fixed):
     """Keys and values of one cache entry in eight bits: `k`, `v` uint8 [pages, kv heads, page_size, head_dim] and `k_scale`,
     `v_scale` float32 [pages, kv heads, page_size].  A row (the values of one position and kv head) stands for
-    (u - 128) * scale; `kv_write_int8` makes it with scale = max|x| / 127."""
+    (u - 128) * scale; `kv_write_int8` makes it with scale = max|x| / 127.  The tensors are held and written in place; none can be put in
+    another's place."""
 
     def __init__(self, k, v, k_scale, v_scale):
         for name, t in (("k", k), ("v", v)):
@@ -965,14 +976,15 @@ class CacheInt8:
                 raise KernelError(f"cache: {name} {tuple(t.shape)} does not fit pages {tuple(k.shape)}")
         if any(t.data_ptr() & 15 for t in (k, v, k_scale, v_scale)):
             raise KernelError("cache: pages and scales must start on 16-byte boundaries")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
-        if min(k.shape) < 1 or self.head_dim % 8 or self.head_dim > MAX_HEAD_DIM_GENERIC:
+        pages, n_kv_heads, page_size, head_dim = k.shape
+        if min(k.shape) < 1 or head_dim % 8 or head_dim > MAX_HEAD_DIM_GENERIC:
             raise KernelError(f"cache: pages {tuple(k.shape)}: head sizes are multiples of 8 up to {MAX_HEAD_DIM_GENERIC}")
-        if k.numel() // self.head_dim >= 2 ** 31:
+        if k.numel() // head_dim >= 2 ** 31:
             raise KernelError(f"cache: pages {tuple(k.shape)} have more than 2^31 rows")
-        self.device = k.device
-        self.pointers = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+        # (tensors of its own over the same memory: one that a user points elsewhere leaves these, and the addresses, as they are)
+        k, v, k_scale, v_scale = (t.detach() for t in (k, v, k_scale, v_scale))
+        self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, pages=pages, n_kv_heads=n_kv_heads, page_size=page_size, head_dim=head_dim, device=k.device,
+                             pointers=(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()))
 
     @classmethod
     def empty(cls, pages, n_kv_heads, page_size, head_dim, device="cuda"):
@@ -1185,7 +1197,7 @@ def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads
     return out
 
 
-class SharedPrefixes:
+class SharedPrefixes(_Fixed):
     """Which tokens of a step (one per sequence) see their first positions in common: `groups` of (positions, [tokens]), whose block tables name
     the same pages for those positions; `lens` [T] on the host: the positions that each token sees, its own included; `group_heads`: query heads per kv
     head (at most 16).  Made once per step and used for every layer.  Tokens in no group are served too."""
@@ -1193,20 +1205,18 @@ class SharedPrefixes:
     def __init__(self, groups, lens, group_heads, device=None):
         groups = [(int(p), [int(t) for t in m]) for p, m in groups]
         lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
-        self.T, self.group_heads = len(lens), int(group_heads)
-        self.device = torch.empty(0, device="cuda" if device is None else device).device
+        T, group_heads = len(lens), int(group_heads)
+        device = torch.empty(0, device="cuda" if device is None else device).device
         sizes, total = (ctypes.c_int * 7)(), ctypes.c_int()
-        args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), self.T,
-                self.group_heads, sizes, ctypes.byref(total))
+        args = (len(groups), _b.ints(p for p, _ in groups), _b.ints(len(m) for _, m in groups), _b.ints(t for _, m in groups for t in m), _b.ints(lens), T, group_heads, sizes,
+                ctypes.byref(total))
         _b.check(_b.lib().illm_prefix_plan(*args, None))
         host = torch.zeros(max(1, total.value), dtype=torch.int32)
         _b.check(_b.lib().illm_prefix_plan(*args, ctypes.cast(host.data_ptr(), _b.PI)))
-        self.tiles, self.wide, self.longest_prefix, self.longest_rest, self.per_tile = sizes[0], bool(sizes[1]), sizes[2], sizes[3], sizes[6]
-        self.longest = max(lens)
-        self.host = host
-        self.plan = host.to(self.device)
-        at = self.plan.data_ptr()
-        self.pointers = at + 4 * sizes[4], at, at + 4 * sizes[5]         # start, tiles, members
+        plan = host.to(device)
+        at = plan.data_ptr()
+        self.__dict__.update(T=T, group_heads=group_heads, device=device, tiles=sizes[0], wide=bool(sizes[1]), longest_prefix=sizes[2], longest_rest=sizes[3], per_tile=sizes[6],
+                             longest=max(lens), host=host, plan=plan, pointers=(at + 4 * sizes[4], at, at + 4 * sizes[5]))         # start, tiles, members
 
 
 def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n_heads, scale, max_len, own_splits=None, pre_splits=None):

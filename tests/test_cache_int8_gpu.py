@@ -800,3 +800,29 @@ def test_positions_beyond_32_bits_of_elements(ops):
     f = q[99:].float()
     assert torch.equal(ops.attention_decode_int8(f, cache, last, *one, 32, 0, 0.1, 100), ops.attention_decode_int8(f, small, first, *one, 32, 0, 0.1, 100))
     assert int(err.item()) == 0 and take_error(ops) == 0
+
+
+def test_what_a_call_reads_stays_as_it_was_made(ops):
+    """Addresses are taken once: another tensor in place of one that they belong to is refused, and one that is pointed elsewhere keeps its memory for the calls."""
+    k, v = (torch.full((3, 2, 64, 64), 128 + i, dtype=torch.uint8, device="cuda") for i in (3, 5))
+    ks, vs = (torch.ones((3, 2, 64), device="cuda") for _ in range(2))
+    cache = ops.CacheInt8(k, v, ks, vs)
+    plan = ops.SharedPrefixes([(64, [0, 1])], [65, 70], 2)
+    for thing, names in ((cache, ("k", "v", "k_scale", "v_scale", "pointers", "pages", "n_kv_heads", "page_size", "head_dim", "device")),
+                         (plan, ("plan", "pointers", "T", "group_heads", "tiles", "wide", "per_tile", "longest", "longest_prefix", "longest_rest", "device"))):
+        for name in names:
+            before = getattr(thing, name)
+            with pytest.raises(AttributeError):
+                setattr(thing, name, before)
+            with pytest.raises(AttributeError):
+                delattr(thing, name)
+            assert getattr(thing, name) is before
+    at = cache.pointers
+    for t in (k, v, ks, vs):
+        t.data = torch.empty(0, dtype=t.dtype, device="cuda")
+    assert tuple(t.data_ptr() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)) == at
+    torch.full((3, 2, 64, 64), 0, dtype=torch.uint8, device="cuda")         # (memory that was given back would be this one's)
+    table = torch.arange(3, dtype=torch.int32, device="cuda").view(1, 3)
+    pos = torch.tensor([0, 130], dtype=torch.int32, device="cuda")
+    rows = ops.kv_read_int8(cache, pos, torch.zeros(2, dtype=torch.int32, device="cuda"), table)
+    assert (rows[0] == 3).all() and (rows[1] == 5).all()
