@@ -26,7 +26,8 @@ attention_int8_kernel(const TA* __restrict__ q, int q_stride, const unsigned cha
     const int t = blockIdx.x, h = blockIdx.y, hk = h / (nh / nkv), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = d >> 3;
     for (int c = threadIdx.x; c < d; c += AI_WARPS * 32) qs[c] = to_f32(q[(size_t)t * q_stride + (size_t)h * d + c]);
     __syncthreads();
-    const int p = token_pos[t], lo = p < 0 ? 0 : first_visible(p, span);
+    const int place = token_pos[t], p = min(place, last_in_table(max_pages, page_size)), lo = p < 0 ? 0 : min(first_visible(place, span), p + 1);
+    if (p < place && threadIdx.x == 0) atomicExch(err, 8);
     const int* bt = block_table + (size_t)token_seq[t] * max_pages;
     float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j0 = lo + warp * 32; j0 <= p; j0 += AI_WARPS * 32) {

@@ -192,7 +192,9 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const int tok = prefix ? plan.members[first + r / G] : t;
         return (size_t)tok * nh + hk * G + r % G;
     };
-    const int tile_lo = lo / PG_BN, n_tiles = p < lo ? 0 : p / PG_BN - tile_lo + 1;
+    const int last = last_in_table(max_pages, page_size);
+    if (p > last && tid == 0) atomicExch(err, PG_ERR_PAGE);
+    const int tile_lo = lo / PG_BN, n_tiles = p < lo ? 0 : min(p, last) / PG_BN - tile_lo + 1;
     const int n_my = n_tiles > split ? (n_tiles - split + n_splits - 1) / n_splits : 0;
     const int slot = prefix ? own_splits + split : split;
     if (part_acc && n_my == 0) {

@@ -164,11 +164,16 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     int member0 = 0;
     int hk, row0 = 0, n_rows, token0, past = 0, seq, jb0, last_key, nb[2], first_key;       // of the block: its rows, from row0 of its (sequence or tile)'s
     int4 tile = make_int4(0, 0, 0, 0);
+    const int end = last_in_table(max_pages, page_size);
     if (PREFIX) {
         hk = blockIdx.y;
         member0 = blockIdx.z * (2 * TL_BM / G);
         const int first_member = work.members[member0];
         tile = work.tiles[blockIdx.z];
+        if (tile.y - 1 > end) {
+            if (threadIdx.x == 0) atomicExch(err, TL_ERR_PAGE);
+            tile.y = end + 1;
+        }
         n_rows = tile.x > 0 && tile.y > 0 ? min(tile.x, 2 * TL_BM / G) * G : 0;
         token0 = 0;
         seq = n_rows ? work.token_seq[first_member] : 0;
@@ -208,8 +213,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         first_key = n_rows > 0 ? max(0, first_visible(past + row0 / G, work.span)) : 0;
         jb0 = first_key / TL_BN;
         last_key = n_rows > 0 ? past + (row0 + n_rows - 1) / G : -1;
-        nb[0] = n_rows > 0 ? (past + (row0 + min(n_rows, TL_BM) - 1) / G) / TL_BN - jb0 + 1 : 0;
-        nb[1] = n_rows > TL_BM ? last_key / TL_BN - jb0 + 1 : 0;
+        nb[0] = n_rows > 0 ? min(past + (row0 + min(n_rows, TL_BM) - 1) / G, end) / TL_BN - jb0 + 1 : 0;
+        nb[1] = n_rows > TL_BM ? min(last_key, end) / TL_BN - jb0 + 1 : 0;
+        if (last_key > end && threadIdx.x == 0) atomicExch(err, TL_ERR_PAGE);
     }
     const int n_blocks = max(nb[0], nb[1]);         // the second tile, where it has rows, sees at least as far as the first
 

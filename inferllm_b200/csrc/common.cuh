@@ -51,6 +51,9 @@ __device__ __forceinline__ int first_visible(int p, int span) {
     return (span > 0 && p - span + 1 > 0) ? p - span + 1 : 0;
 }
 
+// The last position that a row of the block table can name (and a whole tile below the last int): no walk goes further, whatever a position says.
+__device__ __forceinline__ int last_in_table(int max_pages, int page_size) { return (int)min((long long)max_pages * page_size, 0x7fffff00LL) - 1; }
+
 // cap * tanh(s / cap) by the special-function unit, for scores that a kernel of the bfloat16 mode made: tanh x =
 // 1 - 2 / (1 + e^(2x)), absolute error a few 2^-23 of the cap.  two_log2e_over_cap = 2 log2(e) / cap.
 __device__ __forceinline__ float soft_cap_fast(float s, float cap, float two_log2e_over_cap) {

@@ -826,3 +826,48 @@ def test_what_a_call_reads_stays_as_it_was_made(ops):
     pos = torch.tensor([0, 130], dtype=torch.int32, device="cuda")
     rows = ops.kv_read_int8(cache, pos, torch.zeros(2, dtype=torch.int32, device="cuda"), table)
     assert (rows[0] == 3).all() and (rows[1] == 5).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 32])
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 31 - 300, 2 ** 30, 257])
+def test_positions_beyond_the_table_are_reported_and_not_walked(ops, d, far):
+    """A token whose position no page of the table can hold sees the positions that it can, or with a window none of them; the walk ends with the table."""
+    pages = Pages(53, [256, 256], 2, d)
+    cache, table, seq = pages.cache(ops), pages.table[:, :4].contiguous().cuda(), torch.arange(2, dtype=torch.int32).cuda()
+    q = queries(54, 2, 4 * d).cuda()
+    there, beyond = (torch.tensor([p, 99], dtype=torch.int32).cuda() for p in (255, far))
+    assert take_error(ops) == 0
+    for splits in (1, 3):
+        want = ops.attention_decode_int8(q, cache, table, there, seq, 4, 0, 0.1, 256, splits=splits)
+        assert take_error(ops) == 0
+        got = ops.attention_decode_int8(q, cache, table, beyond, seq, 4, 0, 0.1, 256, splits=splits)
+        assert take_error(ops) == 8 and torch.equal(got, want)
+        for window in (1, -1):
+            got = ops.attention_decode_int8(q, cache, table, beyond, seq, 4, window, 0.1, 256, splits=splits)
+            assert take_error(ops) == 8 and (got[0] == 0).all() and (got[1] != 0).any()
+    if d == 32:
+        return
+    cu, lens = torch.arange(3, dtype=torch.int32).cuda(), [torch.tensor([p + 1 if p + 1 < 2 ** 31 else p, 100], dtype=torch.int32).cuda() for p in (255, far)]
+    want = ops.attention_prompts_int8(q, cache, table, cu, lens[0], 1, 4, 0, 0.1)
+    assert take_error(ops) == 0
+    got = ops.attention_prompts_int8(q, cache, table, cu, lens[1], 1, 4, 0, 0.1)
+    assert take_error(ops) == 8 and torch.equal(got, want)
+    got = ops.attention_prompts_int8(q, cache, table, cu, lens[1], 1, 4, 1, 0.1)
+    assert take_error(ops) == 8 and (got[0] == 0).all() and (got[1] != 0).any()
+
+
+@pytest.mark.parametrize("members", [2, 40])
+@pytest.mark.parametrize("prefix", [2 ** 31 - 64, 2 ** 20])
+def test_a_plan_that_goes_beyond_the_table_is_reported(ops, members, prefix):
+    """Tiles of eight rows and of 256: the common positions that the table can name are walked, and the rest of a token's is empty."""
+    pages = Pages(57, [256] * members, 2, 64)
+    cache, table = pages.cache(ops), pages.table[:1, :4].expand(members, 4).contiguous().cuda()
+    q, seq = queries(58, members, 4 * 64).cuda(), torch.arange(members, dtype=torch.int32).cuda()
+    there, beyond = (torch.full((members,), p, dtype=torch.int32).cuda() for p in (255, prefix))
+    made = [ops.SharedPrefixes([(p, list(range(members)))], [p + 1] * members, 2) for p in (192, prefix)]
+    assert made[1].wide == (members == 40)
+    want = ops.attention_decode_int8(q, cache, table, there, seq, 4, 0, 0.1, 256)
+    assert take_error(ops) == 0
+    got = ops.attention_decode_shared(q, cache, table, beyond, seq, made[1], 4, 0.1, prefix + 1, own_splits=2, pre_splits=4)
+    assert take_error(ops) == 8
+    assert (got.double() - want.double()).norm() <= 0.01 * want.double().norm()
