@@ -105,7 +105,7 @@ _SIGNATURES = {
     "illm_test_device": [P, PP], "illm_test_device_rewind": [P], "illm_test_device_info": [P, PI, PP, PP],
     "illm_copy_device": [P, P, P, LL], "illm_op_linear": [P, S, P, LL, LL, P, LL, I, I, I, PP, PP, PI],
     "illm_op_linear_gated": [P, S, P, LL, LL, P, LL, I, PP], "illm_policy_gemm_tc_splits": [LL, LL, LL, I],
-    "illm_policy_pages_splits": [LL, LL, I, I], "illm_policy_pages_in_cluster": [LL, I, I],
+    "illm_policy_shared_prefix_pays": [LL, LL, I], "illm_policy_pages_splits": [LL, LL, I, I], "illm_policy_pages_in_cluster": [LL, I, I],
     "illm_policy_ring_splits": [LL, I, LL, I, I], "illm_policy_attention_diff_splits": [LL, I, LL, I], "illm_policy_attention_supported": [I, I, I, I, I, I],
     "illm_policy_attention_generic": [PI, I, I, I, PI],
     "illm_policy_scan_form": [I, LL, I, I, I, I, I],

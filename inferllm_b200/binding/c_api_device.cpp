@@ -419,6 +419,7 @@ ILLM_API int illm_policy_ring_splits(long long T, int n_kv_heads, long long max_
 ILLM_API int illm_policy_pages_splits(long long pairs, long long keys, int wide, int n_sms) {
     return wide ? ops::attention_prefix_splits(pairs, keys, n_sms) : ops::attention_pages_splits(pairs, keys, n_sms);
 }
+ILLM_API int illm_policy_shared_prefix_pays(long long saved_rows, long long sequences, int int8) { return ops::shared_prefix_pays(saved_rows, sequences, int8 != 0); }
 ILLM_API int illm_policy_pages_in_cluster(long long pairs, int splits, int n_sms) { return ops::attention_pages_in_cluster(pairs, splits, n_sms); }
 ILLM_API int illm_policy_attention_diff_splits(long long T, int head_groups, long long max_seq_len, int n_sms) {
     return ops::attention_diff_splits(T, head_groups, max_seq_len, n_sms);

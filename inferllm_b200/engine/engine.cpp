@@ -89,8 +89,7 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     for (int entry : model_->prefix_entries()) {
         if (cache_->kind_of(entry) != SequenceCache::KV) continue;
         const SequenceCache::PagedGroup& g = cache_->paged[(size_t)cache_->group_of(entry)];
-        const long long bytes = (long long)(g.page_bytes + g.v_page_bytes);
-        prefix_page_bytes_ = prefix_page_bytes_ ? std::min(prefix_page_bytes_, bytes) : bytes;
+        prefix_entries_.insert({g.request.n_kv_heads, (long long)(g.page_bytes + g.v_page_bytes), g.request.int8});
     }
     builder_.reset(new StepContextBuilder(device_.get(), &rt_));
     for (TokRead& t : tok_reads_) check_cuda(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming), "cudaEventCreate");
@@ -257,16 +256,19 @@ StepContext Engine::make_context(const StepPlan& plan, const std::vector<int>& i
 // (tiles, the splits that follow from the lengths) is rounded up, so that captured steps of growing sequences can be replayed.
 bool Engine::find_prefixes(const StepPlan& plan, StepPrefixes* out) const {
     if (!prefix_heads_ || plan.slots.size() < 2 || plan.slots.size() > kSharedPrefixSequences) return false;
-    long long saved = 0;
+    long long saved = 0;        // positions
     for (auto& g : cache_->common_prefixes(plan.slots)) {
-        saved += g.first / cache_->page_size * prefix_page_bytes_ * ((long long)g.second.size() - 1);
+        saved += g.first * ((long long)g.second.size() - 1);
         ops::PrefixGroup group;
         group.prefix = g.first;
         group.members = g.second;
         out->groups.push_back(std::move(group));
     }
-    if (out->groups.empty() || saved < (options_.shared_prefix_bytes >= 0 ? options_.shared_prefix_bytes : kSharedPrefixBytes + (long long)plan.slots.size() * kSharedPrefixBytesEach))
-        return false;
+    if (out->groups.empty()) return false;
+    for (const PrefixEntry& e : prefix_entries_)
+        if (options_.shared_prefix_bytes >= 0 ? saved / cache_->page_size * e.page_bytes < options_.shared_prefix_bytes
+                                              : !ops::shared_prefix_pays(saved * e.rows, (long long)plan.slots.size(), e.int8))
+            return false;
     std::vector<int> lens;
     for (size_t i = 0; i < plan.slots.size(); i++) lens.push_back((int)(plan.past[i] + 1));
     out->heads = prefix_heads_;

@@ -12,7 +12,9 @@
 #pragma once
 #include <map>
 #include <memory>
+#include <set>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "cache/cache.h"
@@ -34,7 +36,7 @@ struct EngineOptions {
     bool cuda_graphs = true;            // replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     std::string cache_dtype = "auto";   // keys and values: "auto" (as the compute dtype) or "int8" (a byte each and a scale per row, where a layer can)
     bool share_prefixes = false;        // the generation loop runs the first positions that all prompts of a batch have in common once
-    long long shared_prefix_bytes = -1; // decode steps walk common positions once where that saves so many bytes of a layer's cache; -1: by a rule
+    long long shared_prefix_bytes = -1; // decode steps walk common positions once where that saves so many bytes of a layer's cache; -1: by a rule (ops::shared_prefix_pays)
     int max_adapters = 0;               // low-rank adapters that may be loaded together (Engine::add_adapter)
     int adapter_rank = 16;              // the largest rank of one (at most 85: q, k and v stand side by side)
     std::string gemm = "auto";          // bfloat16 products: "auto" | "tc" | "library" (see ops::GemmBackend)
@@ -64,11 +66,6 @@ struct LogitsRef {
     long long rows = 0, vocab = 0;
 };
 
-// Bytes of keys and values (of a layer) that a decode step of n sequences must not have to read again to walk common prefixes by themselves: kSharedPrefixBytes
-// + n kSharedPrefixBytesEach (a prefix counts once for every sequence but one).  Measured with eight-bit rows of 128, a common prefix and 100 positions behind it, once
-// for all and one by one: 4 sequences of 32 / 32 heads at 256 positions (6 MB saved) 7.3 and 7.5 us, at 1,024 9.2 and 12.1, of 32 / 8 heads at 1,024 (6 MB) 8.8 and 8.0;
-// 16 of 32 / 8 at 1,024 (30 MB) 12.8 and 11.6, at 2,048 17.8 and 20.0; 64 of 32 / 8 at 512 (63 MB) 23 and 16, at 1,024 (126 MB) 23.7 and 25.4, at 2,048 24 and 44.
-constexpr long long kSharedPrefixBytes = 4 << 20, kSharedPrefixBytesEach = 3 << 19;
 constexpr size_t kSharedPrefixSequences = 32768;       // a plan's tiles, rounded up to a power of two, still are rows of a grid; larger steps read every sequence by itself
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
@@ -162,7 +159,13 @@ private:
     bool loaded_ = false;
     std::vector<int> adapter_ranks_;        // 0: free
     int pad_safe_ = -1, graph_safe_ = -1, prefix_heads_ = 0;
-    long long prefix_page_bytes_ = 0;       // of a page of keys and values in the entries of the layers that walk common prefixes (the least, where they differ)
+    // the entries of the layers that walk common prefixes, where they differ: rows of a position (kv heads), bytes of keys and values of a page
+    struct PrefixEntry {
+        long long rows, page_bytes;
+        bool int8;
+        bool operator<(const PrefixEntry& o) const { return std::tie(rows, page_bytes, int8) < std::tie(o.rows, o.page_bytes, o.int8); }
+    };
+    std::set<PrefixEntry> prefix_entries_;
     size_t last_upload_bytes_ = 0;
 
     std::unique_ptr<StepContextBuilder> builder_;

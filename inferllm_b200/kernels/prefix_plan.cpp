@@ -46,6 +46,10 @@ PrefixPlanSizes prefix_plan_sizes(const std::vector<PrefixGroup>& groups, const 
     return s;
 }
 
+bool shared_prefix_pays(long long saved_rows, long long sequences, bool int8) {
+    return saved_rows >= std::min<long long>(int8 ? 32768 + 8192 * sequences : 131072 + 12288 * sequences, 393216);
+}
+
 void prefix_plan_fill(const std::vector<PrefixGroup>& groups, const PrefixPlanSizes& s, int* out) {
     std::fill(out, out + s.ints(), 0);
     int tile = 0;

@@ -452,3 +452,23 @@ def test_a_step_of_more_sequences_than_a_plan_takes(model_folders):
     for i in range(len(some)):
         assert_close(got[i:i + 1], alone, "bfloat16", f"sequence {some[i]}")
     e.cache.check()
+
+
+@pytest.mark.parametrize("cache", ["auto", "int8"])
+def test_steps_follow_the_rule_of_what_common_positions_save(cache, model_folders):
+    """Behind 960 positions of two kv heads 300 sequences are on one side of the rule and 100 on the other, whatever the rows' type."""
+    e = engine(model_folders["C"], cache=cache, cuda_graphs=False, max_tokens=64 * 330, max_batch=301)
+    other = engine(model_folders["C"], cache=cache, cuda_graphs=False, max_tokens=64 * 330, max_batch=301, shared_prefix_bytes=2 ** 62)
+    prompt, launches, got = random_prompt("C", 960, 1), {}, {}
+    for which, x in (("rule", e), ("one by one", other)):
+        a = x.new_sequence()
+        x.step([StepItem(a, prompt, [])])
+        slots = [x.fork_sequence(a, 960) for _ in range(300)]
+        for n in (300, 100):
+            before = ops.launch_count()
+            got[which, n] = x.step([StepItem(s, [5], [0]) for s in slots[:n]]).cpu().numpy()
+            launches[which, n] = ops.launch_count() - before
+        x.check_device_errors()
+    assert launches["rule", 300] > launches["one by one", 300] and launches["rule", 100] == launches["one by one", 100]
+    for n in (300, 100):
+        assert_close(got["rule", n], got["one by one", n], "bfloat16", f"{n} sequences")

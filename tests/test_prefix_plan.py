@@ -78,3 +78,16 @@ def test_no_groups_is_a_plan():
 def test_refusals(groups, lens, G, words):
     with pytest.raises(KernelError, match=words):
         plan(groups, lens, G)
+
+
+@pytest.mark.parametrize("int8, sequences, positions, kv_heads, once", [
+    # as measured, on both sides of the border: bfloat16 rows ...
+    (0, 2, 8192, 8, False), (0, 3, 8192, 8, False), (0, 4, 4096, 8, False), (0, 4, 8192, 8, True), (0, 4, 1024, 32, False), (0, 4, 2048, 32, True), (0, 7, 4096, 8, False),
+    (0, 8, 2048, 8, False), (0, 8, 4096, 8, True), (0, 16, 2048, 8, False), (0, 16, 4096, 8, True), (0, 32, 1024, 8, False), (0, 32, 2048, 8, True),
+    (0, 64, 512, 8, False), (0, 64, 1024, 8, True), (0, 64, 256, 32, True),
+    # ... and rows of eight bits
+    (1, 2, 4096, 8, False), (1, 2, 8192, 8, True), (1, 4, 256, 32, False), (1, 4, 1024, 32, True), (1, 4, 4096, 8, True), (1, 16, 1024, 8, False), (1, 16, 4096, 8, True),
+    (1, 32, 512, 8, False), (1, 32, 2048, 8, True), (1, 64, 512, 8, False), (1, 64, 1024, 8, True),
+])
+def test_where_common_positions_are_walked_once(int8, sequences, positions, kv_heads, once):
+    assert bool(_b.lib().illm_policy_shared_prefix_pays((sequences - 1) * positions * kv_heads, sequences, int8)) == once
