@@ -456,6 +456,8 @@ struct illm_loop_callbacks {
     int (*select)(void* user, long long tokens, const int* idx, int n, long long* out);
     double (*clock)(void* user);
     void (*on_token)(void* user, int request, int token);
+    int (*share_page)(void* user, int* page);          // both or neither: GenBackend::share_page and fork_sequence
+    int (*fork_sequence)(void* user, int slot, long long length, int* forked);
 };
 
 namespace {
@@ -475,6 +477,16 @@ struct CallbackBackend : GenBackend, Chooser {
     }
     void end_sequence(int slot) override {
         if (cb.end_sequence(cb.user, slot)) callback_failed("end_sequence");
+    }
+    int share_page() override {
+        int page = 0;
+        if (cb.share_page && cb.fork_sequence && cb.share_page(cb.user, &page)) callback_failed("share_page");
+        return page;
+    }
+    int fork_sequence(int slot, long long length) override {
+        int s = -1;
+        if (cb.fork_sequence(cb.user, slot, length, &s)) callback_failed("fork_sequence");
+        return s;
     }
     LogitsRef step(const std::vector<StepItem>& items, const TokensRef* ids) override {
         std::vector<int> slots, nt, toks, nw, want;

@@ -303,7 +303,8 @@ class GenerationResult:
     tokens: List[List[int]]                    # generated ids per request (stop token included)
     finish: List[str]                          # "stop" | "length" | "context"
     batches: List[List[int]]                   # which requests ran together
-    prefill_tokens: int = 0
+    prefill_tokens: int = 0                    # that ran
+    shared_tokens: int = 0                     # of the prompts, held in common with another request's and not run again
     prefill_s: float = 0.0
     decode_tokens: int = 0
     decode_s: float = 0.0
@@ -313,8 +314,9 @@ class GenerationResult:
     def summary(self) -> str:
         pf = self.prefill_tokens / self.prefill_s if self.prefill_s > 0 else 0.0
         dc = self.decode_tokens / self.decode_s if self.decode_s > 0 else 0.0
+        common = f", {self.shared_tokens} more held in common" if self.shared_tokens else ""
         return (f"prefill: {self.prefill_tokens} tokens in {self.prefill_s * 1e3:.1f} ms "
-                f"({pf:.1f} tok/s); decode: {self.decode_tokens} tokens in {self.decode_steps} steps, "
+                f"({pf:.1f} tok/s){common}; decode: {self.decode_tokens} tokens in {self.decode_steps} steps, "
                 f"{self.decode_s * 1e3:.1f} ms ({dc:.1f} tok/s)")
 
 
@@ -327,7 +329,7 @@ def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, limits: Limits
 
 class _LoopCallbacks(ctypes.Structure):
     _fields_ = [("user", ctypes.c_void_p)] + [(n, ctypes.c_void_p) for n in (
-        "limits", "new_sequence", "end_sequence", "step", "choose", "read_async", "finish_read", "select", "clock", "on_token")]
+        "limits", "new_sequence", "end_sequence", "step", "choose", "read_async", "finish_read", "select", "clock", "on_token", "share_page", "fork_sequence")]
 
 
 def generate(backend, prompts: Sequence[Sequence[int]], choose: Callable, max_new_tokens: int, stop_ids: Sequence[int] = (),
@@ -335,7 +337,8 @@ def generate(backend, prompts: Sequence[Sequence[int]], choose: Callable, max_ne
     """The library's generation loop over a backend and a chooser written in Python (stand-ins in
     tests, or an engine driven from Python).  `backend` has `limits()`, `new_sequence()`,
     `end_sequence(slot)`, `step(items, device_ids=None)` and may have `read_tokens_async(toks)` (returns
-    a function that gives the list); `choose(logits, requests, steps, histories)` returns one token per
+    a function that gives the list) and `share_page()` with `fork_sequence(slot, length)` (batches then run
+    what their prompts have in common once, in whole pages of that size); `choose(logits, requests, steps, histories)` returns one token per
     row (a list, or anything with `tolist()`; indexable by a list of rows if it is no list)."""
     I, LL, P = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
     PI, PLL = ctypes.POINTER(I), ctypes.POINTER(LL)
@@ -407,6 +410,13 @@ def generate(backend, prompts: Sequence[Sequence[int]], choose: Callable, max_ne
         t, rows = objects[tokens], [idx[i] for i in range(n)]
         out[0] = keep([t[i] for i in rows] if isinstance(t, (list, tuple)) else t[rows])
 
+    def cb_share_page(_u, page):
+        page[0] = backend.share_page()
+
+    def cb_fork(_u, slot, length, forked):
+        forked[0] = backend.fork_sequence(slot, length)
+
+    shares = hasattr(backend, "share_page")
     table = _LoopCallbacks()
     funcs = [
         ctypes.CFUNCTYPE(I, P, PLL)(guarded(cb_limits)), ctypes.CFUNCTYPE(I, P, PI)(guarded(cb_new)),
@@ -414,7 +424,8 @@ def generate(backend, prompts: Sequence[Sequence[int]], choose: Callable, max_ne
         ctypes.CFUNCTYPE(I, P, LL, I, PI, PI, I, PI, PI, PLL)(guarded(cb_choose)), ctypes.CFUNCTYPE(I, P, LL, PI)(guarded(cb_read)),
         ctypes.CFUNCTYPE(I, P, I, PI, I, PI)(guarded(cb_finish)), ctypes.CFUNCTYPE(I, P, LL, PI, I, PLL)(guarded(cb_select)),
         ctypes.CFUNCTYPE(ctypes.c_double, P)(lambda _u: float(clock())) if clock else None,
-        ctypes.CFUNCTYPE(None, P, I, I)(lambda _u, r, t: on_token(r, t)) if on_token else None]
+        ctypes.CFUNCTYPE(None, P, I, I)(lambda _u, r, t: on_token(r, t)) if on_token else None,
+        ctypes.CFUNCTYPE(I, P, PI)(guarded(cb_share_page)) if shares else None, ctypes.CFUNCTYPE(I, P, I, LL, PI)(guarded(cb_fork)) if shares else None]
     for name, f in zip([n for n, _ in _LoopCallbacks._fields_[1:]], funcs):
         setattr(table, name, ctypes.cast(f, P) if f is not None else None)
     lens = [len(p) for p in prompts]

@@ -11,9 +11,10 @@ namespace illm {
 
 std::string GenerationResult::summary() const {
     const double pf = prefill_s > 0 ? prefill_tokens / prefill_s : 0.0, dc = decode_s > 0 ? decode_tokens / decode_s : 0.0;
-    char buf[256];
-    snprintf(buf, sizeof buf, "prefill: %lld tokens in %.1f ms (%.1f tok/s); decode: %lld tokens in %lld steps, %.1f ms (%.1f tok/s)",
-             prefill_tokens, prefill_s * 1e3, pf, decode_tokens, decode_steps, decode_s * 1e3, dc);
+    const std::string common = shared_tokens ? ", " + std::to_string(shared_tokens) + " more held in common" : "";
+    char buf[320];
+    snprintf(buf, sizeof buf, "prefill: %lld tokens in %.1f ms (%.1f tok/s)%s; decode: %lld tokens in %lld steps, %.1f ms (%.1f tok/s)",
+             prefill_tokens, prefill_s * 1e3, pf, common.c_str(), decode_tokens, decode_steps, decode_s * 1e3, dc);
     return buf;
 }
 
@@ -35,6 +36,7 @@ Json GenerationResult::to_json() const {
     j.set("finish", fin);
     j.set("batches", bat);
     j.set("prefill_tokens", prefill_tokens);
+    j.set("shared_tokens", shared_tokens);
     j.set("prefill_s", prefill_s);
     j.set("decode_tokens", decode_tokens);
     j.set("decode_s", decode_s);
@@ -189,6 +191,9 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
                 if (first) {
                     res.prefill_s += now - t0;
                     for (int r : batch) res.prefill_tokens += (long long)prompts[(size_t)r].size();
+                    const long long shared = common * ((long long)batch.size() - 1);
+                    res.prefill_tokens -= shared;
+                    res.shared_tokens += shared;
                     first = false;
                 } else {
                     res.step_s.push_back(now - t0);

@@ -34,7 +34,8 @@ struct GenerationResult {
     std::vector<std::vector<int>> tokens;       // generated ids per request (stop token included)
     std::vector<std::string> finish;            // "stop" | "length" | "context"
     std::vector<std::vector<int>> batches;      // which requests ran together
-    long long prefill_tokens = 0, decode_tokens = 0, decode_steps = 0;
+    long long prefill_tokens = 0, decode_tokens = 0, decode_steps = 0;       // tokens that ran
+    long long shared_tokens = 0;                // of the prompts, held in common with another request's and not run again
     double prefill_s = 0, decode_s = 0;
     std::vector<double> step_s;                 // wall time of every decode step, in order
     std::string summary() const;

@@ -472,3 +472,28 @@ def test_steps_follow_the_rule_of_what_common_positions_save(cache, model_folder
     assert launches["rule", 300] > launches["one by one", 300] and launches["rule", 100] == launches["one by one", 100]
     for n in (300, 100):
         assert_close(got["rule", n], got["one by one", n], "bfloat16", f"{n} sequences")
+
+
+def test_shared_positions_are_not_run_again(model_folders):
+    """What the loop ran, by its own counts and the cache's: with and without sharing, with one adapter for all requests and with several, and through the command."""
+    name = "C"
+    head = random_prompt(name, 150, 1)
+    prompts = [head + random_prompt(name, 2 + i, 50 + i) for i in range(5)]
+    total = sum(map(len, prompts))
+    for share in (False, True):
+        m = Model(ModelConfig(compt_type="float32", nr_ctx=512, max_tokens=4096, share_prefixes=share, max_adapters=2, adapter_rank=4))
+        m.load(model_folders[name])
+        m.init(top_k=40, top_p=0.95, temp=0.0, repeat_penalty=1.0, repeat_last_n=64, seed=1, end_token=2)
+        one, two = some_adapters(m.engine, 2)
+        for adapters, shared in ((None, True), ([one] * 5, True), ([one, one, two, one, one], False), ([one, -1, -1, -1, -1], False)):
+            used = []
+            res = m.generate(prompts, 4, stop_ids=[], adapters=adapters, on_token=lambda r, t: used.append(m.engine.limits().num_pages - m.engine.cache.pages_free()[0]))
+            n = 4 * 128 if share and shared else 0
+            assert (res.prefill_tokens, res.shared_tokens) == (total - n, n)
+            assert max(used) == 5 * 3 - n // 64
+    for extra in ([], ["--share-prefixes"]):
+        ids = [x for i in range(5) for x in ("--prompt-ids", ",".join(map(str, list(range(1, 80)) + [100 + i])))]
+        out = subprocess.run([f"{ROOT}/bin/llama", "-m", model_folders[name], "-g", "GPU", *ids, "-n", "4", "--temp", "0", "-c", "256", "--no-stop", *extra],
+                             capture_output=True, text=True, timeout=300)
+        assert out.returncode == 0, out.stderr
+        assert (f"prefill: {5 * 80 - 4 * 64} tokens" in out.stderr and "256 more held in common" in out.stderr) if extra else f"prefill: {5 * 80} tokens" in out.stderr

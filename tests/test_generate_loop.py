@@ -209,3 +209,62 @@ def test_timing_uses_the_callers_clock():
 
     res = generate(FakeBackend(), [[1, 2]], scripted({0: [5, 6, 7]}), max_new_tokens=3, clock=clock)
     assert res.decode_steps == 2 and res.prefill_s > 0 and res.decode_s > 0 and len(res.step_s) == 2
+
+
+class SharingBackend(FakeBackend):
+    """Sequences may begin with the first pages of another."""
+
+    def __init__(self, page=64, **kw):
+        super().__init__(max_batch=8, num_pages=200, page_size=page, max_seq_len=4096, **kw)
+        self.forks = []
+        self.began = set()
+
+    def share_page(self):
+        return self.lim.page_size
+
+    def fork_sequence(self, slot, length):
+        assert length % self.lim.page_size == 0 and 0 < length <= self.len[slot]
+        s = self.new_sequence()
+        self.len[s] = length
+        self.forks.append((slot, s, length))
+        return s
+
+    def step(self, items, device_ids=None):
+        # a prompt may come in two pieces: what is common, and the rest
+        pieces = {it.slot: self.len[it.slot] for it in items if len(it.tokens) > 1}
+        for s in pieces:
+            self.len[s] = 0
+        out = super().step(items, device_ids)
+        for s, n in pieces.items():
+            self.len[s] += n
+        return out
+
+
+def test_common_positions_run_once_and_are_counted_once():
+    head = list(range(150))
+    prompts = [head + [500 + i] * (2 + i) for i in range(5)] + [head[:149]]
+    script = {r: [7] * 4 for r in range(6)}
+    alone, be = FakeBackend(max_batch=8, num_pages=200, page_size=64, max_seq_len=4096), SharingBackend()
+    want = generate(alone, prompts, scripted(script), max_new_tokens=3)
+    res = generate(be, prompts, scripted(script), max_new_tokens=3)
+    assert res.tokens == want.tokens and res.finish == want.finish
+    assert be.forks == [(0, i, 128) for i in range(1, 6)] and be.len == {}
+    total = sum(map(len, prompts))
+    assert (want.prefill_tokens, want.shared_tokens) == (total, 0)
+    assert (res.prefill_tokens, res.shared_tokens) == (total - 5 * 128, 5 * 128)
+    # what ran: the common pages for the first request, then what every prompt has for itself, the longest first
+    assert be.log[0] == [(0, 128)] and sorted(be.log[1]) == sorted((i, len(p) - 128) for i, p in enumerate(prompts))
+    assert sum(n for step in be.log[:2] for _, n in step) == res.prefill_tokens
+    assert "640 more held in common" in res.summary() and "common" not in want.summary()
+
+
+@pytest.mark.parametrize("prompts", [
+    [list(range(300))],                                                  # one request
+    [list(range(300)), [1] + list(range(299))],                          # nothing in common
+    [list(range(63)) + [900 + i] * 300 for i in range(6)],               # less than a page
+    [list(range(64)) for _ in range(6)],                                 # a prompt keeps a token of its own
+])
+def test_prompts_without_a_common_page_run_as_they_are(prompts):
+    be = SharingBackend()
+    res = generate(be, prompts, scripted({r: [7] * 3 for r in range(6)}), max_new_tokens=2)
+    assert be.forks == [] and res.shared_tokens == 0 and res.prefill_tokens == sum(map(len, prompts)) and len(be.log[0]) == len(prompts)
