@@ -30,7 +30,7 @@ class EngineOptions:
     cuda_graphs: bool = True       # replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     gemm: str = "auto"             # bfloat16 products: "auto" | "tc" | "library"
     cache_dtype: str = "auto"      # keys and values: "auto" (as `dtype`) or "int8" (a byte each and a scale per row, where a layer can)
-    share_prefixes: bool = False   # `generate` runs the first positions that all prompts of a batch have in common once
+    share_prefixes: bool = False   # `generate` runs the first positions that all prompts of a batch have in common once, where that saves 256 tokens or more
     shared_prefix_bytes: int = -1  # decode steps walk common positions once where that saves so many bytes of a layer's cache; -1: by a rule
     max_adapters: int = 0          # low-rank adapters that may be loaded together (`Engine.add_adapter`)
     adapter_rank: int = 16         # the largest rank of one (at most 85)

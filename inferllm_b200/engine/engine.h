@@ -35,7 +35,7 @@ struct EngineOptions {
     int page_size = 64;
     bool cuda_graphs = true;            // replay one-token-per-sequence steps and single prompts from captured CUDA graphs
     std::string cache_dtype = "auto";   // keys and values: "auto" (as the compute dtype) or "int8" (a byte each and a scale per row, where a layer can)
-    bool share_prefixes = false;        // the generation loop runs the first positions that all prompts of a batch have in common once
+    bool share_prefixes = false;        // the generation loop runs the first positions that all prompts of a batch have in common once, where that saves 256 tokens or more
     long long shared_prefix_bytes = -1; // decode steps walk common positions once where that saves so many bytes of a layer's cache; -1: by a rule (ops::shared_prefix_pays)
     int max_adapters = 0;               // low-rank adapters that may be loaded together (Engine::add_adapter)
     int adapter_rank = 16;              // the largest rank of one (at most 85: q, k and v stand side by side)

@@ -111,6 +111,7 @@ GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int
                     if (adapters && (*adapters)[(size_t)r] != (*adapters)[(size_t)batch[0]]) common = 0;
                 }
                 common = common / page * page;
+                if (common * ((long long)batch.size() - 1) < kSharedTokensLeast) common = 0;
             }
             for (int r : batch) {
                 slots[r] = common == 0 || r == batch[0] ? backend.new_sequence() : backend.fork_sequence(slots[batch[0]], common);

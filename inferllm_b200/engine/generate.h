@@ -53,7 +53,8 @@ public:
     virtual int read_tokens_async(const TokensRef& toks) = 0;        // a ticket
     virtual std::vector<int> finish_read(int ticket) = 0;
     virtual TokensRef select(const TokensRef& toks, const std::vector<int>& idx) = 0;   // toks[idx]
-    // The page size of a backend whose batches are to run the first positions that all their prompts have in common once; 0: they are not.
+    // The page size of a backend whose batches are to run the first positions that all their prompts have in common once, where that saves enough
+    // (kSharedTokensLeast); 0: they are not.
     virtual int share_page() { return 0; }
     virtual int fork_sequence(int slot, long long length) { throw EngineError("this backend shares no positions"); }
 };
@@ -69,6 +70,12 @@ public:
 // sequence's worst case (prompt + new tokens, capped by the longest sequence), so that a batch that
 // has started never runs out of cache.  RequestTooLong for a request that can never fit.
 std::vector<std::vector<int>> plan_batches(const std::vector<int>& prompt_lens, long long max_new_tokens, const Limits& limits);
+
+// Tokens that a batch must not have to run for what its prompts have in common to be run by itself first: a step of a few tokens is one reading of the weights, which
+// is the time of about so many tokens' arithmetic (at the measured rates the bfloat16 products of 261 tokens take as long as one reading).  Prompts of 32 layers of a hidden size of 4,096
+// with 20 tokens of their own, together / common part first, ms: 2 prompts behind 64 tokens 4.7 / 7.0, 192 (saved) 7.1 / 8.3, 256 9.2 / 8.5, 512 15.7 / 11.9; 4 behind 64
+// (192 saved) 6.6 / 7.7, 128 (384) 9.8 / 8.3; 8 behind 64 (448) 10.4 / 8.5.  With 200 tokens of their own: 2 behind 64 10.2 / 11.3, 256 14.8 / 12.8; 4 behind 64 15.6 / 17.5, 128 19.5 / 17.7.
+constexpr long long kSharedTokensLeast = 256;
 
 using TokenCallback = std::function<void(int request, int token)>;
 GenerationResult generate(GenBackend& backend, const std::vector<std::vector<int>>& prompts, Chooser& chooser, long long max_new_tokens,

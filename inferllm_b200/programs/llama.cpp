@@ -57,7 +57,7 @@ static const char* kHelp =
     "  --prompt-file FILE       one request (comma- or space-separated ids) per line\n"
     "  --random-prompts LENS    comma-separated prompt lengths of random ids\n"
     "  --cache-dtype TYPE       keys and values: auto (as the compute dtype) | int8 (default auto)\n"
-    "  --share-prefixes         run the first tokens that all requests have in common once\n"
+    "  --share-prefixes         run the first tokens that all requests of a batch have in common once, where that saves 256 or more\n"
     "  --max-tokens N           tokens the cache holds (default: fits all requests at once, up to 64 Ki)\n"
     "  --config FILE            config.json for --random-weights / --write-random-model\n"
     "  --random-weights SEED    run a model with random weights made on the device\n"

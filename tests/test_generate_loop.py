@@ -268,3 +268,12 @@ def test_prompts_without_a_common_page_run_as_they_are(prompts):
     be = SharingBackend()
     res = generate(be, prompts, scripted({r: [7] * 3 for r in range(6)}), max_new_tokens=2)
     assert be.forks == [] and res.shared_tokens == 0 and res.prefill_tokens == sum(map(len, prompts)) and len(be.log[0]) == len(prompts)
+
+
+@pytest.mark.parametrize("requests, common, shared", [(2, 64, False), (2, 192, False), (2, 256, True), (4, 64, False), (4, 128, True), (5, 64, True), (8, 64, True)])
+def test_common_positions_run_by_themselves_where_that_saves_a_step(requests, common, shared):
+    be = SharingBackend()
+    prompts = [list(range(common)) + [900 + i] * (10 + i) for i in range(requests)]
+    res = generate(be, prompts, scripted({r: [7] * 3 for r in range(requests)}), max_new_tokens=2)
+    assert res.tokens == [[7, 7]] * requests
+    assert res.shared_tokens == ((requests - 1) * common if shared else 0) and len(be.forks) == (requests - 1 if shared else 0)
