@@ -448,3 +448,7 @@ ILLM_API int illm_policy_attention_supported(int which, int dtype, int nh, int n
 ILLM_API int illm_policy_attention_kernels(int dtype, int nh, int nkv, int d, int page_size, char** out) {
     return guard([&] { *out = dup_string(ops::attention_kernels_for((DType)dtype, nh, nkv, d, page_size)); });
 }
+// of a layer whose cache entry is kept in eight bits
+ILLM_API int illm_policy_attention_kernels_int8(int dtype, int nh, int nkv, int d, int page_size, char** out) {
+    return guard([&] { *out = dup_string(ops::attention_kernels_for((DType)dtype, nh, nkv, d, page_size, true)); });
+}

@@ -96,18 +96,29 @@ Engine::Engine(std::unique_ptr<ArchConfig> config, const EngineOptions& options)
     // say once which attention kernels the model's layers get: a head size that the tensor-core kernels
     // do not take falls to the general kernel, which is right but far slower on prompts
     std::set<std::string> said;
-    for (const LayerSpec& ls : spec.layers) {
+    std::set<int> int8_layers;
+    for (const ScheduleEntry& s : spec.schedule)
+        if (cache_->kind_of(s.cache) == SequenceCache::KV && cache_->paged[(size_t)cache_->group_of(s.cache)].request.int8) int8_layers.insert(s.layer);
+    if (options.cache_dtype == "int8") {
+        size_t paged = 0, int8 = 0;
+        for (const SequenceCache::PagedGroup& g : cache_->paged) paged += g.entries.size(), int8 += g.request.int8 ? g.entries.size() : 0;
+        log_line(LogLevel::Info, "cache: %zu of %zu entries in eight bits", int8, paged);
+    }
+    for (size_t i = 0; i < spec.layers.size(); i++) {
+        const LayerSpec& ls = spec.layers[i];
         if (ls.mixer.kind != "attention" || !ls.mixer.has("n_heads")) continue;
         // a layer with sinks, gates, biases or norms of its own takes the general path (ops::attention_ex), which this line does not describe
         if (ls.mixer.get_bool("sink", false) || ls.mixer.get_bool("qkv_bias", false) || ls.mixer.has("out_gate") || ls.mixer.has("qk_norm")) continue;
         const int nh = (int)ls.mixer.get_int("n_heads"), nkv = (int)ls.mixer.get_int("n_kv_heads", nh), d = (int)ls.mixer.get_int("head_dim", 0);
-        const std::string what = ops::attention_kernels_for(dtype, nh, nkv, d, options.page_size);
+        const std::string what = ops::attention_kernels_for(dtype, nh, nkv, d, options.page_size, int8_layers.count((int)i) != 0);
         const std::string line = std::to_string(nh) + " heads over " + std::to_string(nkv) + " of size " + std::to_string(d) + ", pages of " +
                                  std::to_string(options.page_size) + ": " + what;
         if (!said.insert(line).second) continue;
-        const bool slow = dtype == DType::BF16 && what.find("prompts: generic") != std::string::npos;
+        const bool slow = dtype == DType::BF16 && (what.find("prompts: generic") != std::string::npos || what.find("plain") != std::string::npos);
         log_line(slow ? LogLevel::Warning : LogLevel::Info, "attention, %s%s", line.c_str(),
-                 slow ? " (head sizes 64 and 128 get the tensor-core kernels)" : "");
+                 !slow                        ? ""
+                 : int8_layers.count((int)i) ? " (head sizes 64 and 128 with pages of a multiple of 64 and, for single tokens, up to 16 heads per kv head get the tensor-core kernels)"
+                                             : " (head sizes 64 and 128 get the tensor-core kernels)");
     }
 }
 

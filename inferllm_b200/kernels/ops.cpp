@@ -157,7 +157,12 @@ bool attention_prefill_supported(DType dtype, int nh, int nkv, int d) {
 bool attention_prefill_tc_supported(DType dtype, int nh, int nkv, int d, int page_size) {
     return dtype == DType::BF16 && (d == 64 || d == 128) && nkv > 0 && nh % nkv == 0 && page_size % 64 == 0;
 }
-std::string attention_kernels_for(DType dtype, int nh, int nkv, int d, int page_size) {
+std::string attention_kernels_for(DType dtype, int nh, int nkv, int d, int page_size, bool int8) {
+    if (int8) {
+        auto plain = [&](bool decode) { return !attention_int8_tc_supported(dtype, nh, nkv, d, page_size, decode); };
+        return std::string("rows of eight bits, prompts: ") + (plain(false) ? "plain (float32 SIMT, every token its own reads)" : "tiles (tcgen05)") +
+               "; single tokens: " + (plain(true) ? "plain (float32 SIMT)" : "pages (TMA ring)");
+    }
     const int group = nkv ? nh / nkv : 0;
     std::string prompt = attention_prefill_tc_supported(dtype, nh, nkv, d, page_size) ? "prefill_tc (tcgen05)"
                          : attention_prefill_supported(dtype, nh, nkv, d)             ? "prefill (mma.sync)"

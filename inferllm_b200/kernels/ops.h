@@ -162,7 +162,7 @@ void count_token_tiles(const int* q_lens, int B, int& dense, int& sparse);
 int attention_generic_form(int dense_tiles, int sparse_tiles, int n_heads, int n_sms);
 // Which attention kernel a configuration gets for prompts and for single tokens (for the log line at
 // engine start): "prefill_tc/decode_ring", "generic/generic", ...
-std::string attention_kernels_for(DType dtype, int nh, int nkv, int d, int page_size);
+std::string attention_kernels_for(DType dtype, int nh, int nkv, int d, int page_size, bool int8 = false);
 
 // ---- kernels
 

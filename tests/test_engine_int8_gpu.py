@@ -3,6 +3,7 @@
 The plain implementation is given the same rounding of keys and values.  A value that lies on the border between two steps may
 fall to either side in the engine, which moves it by 1/127 of its row's largest: less than what rounding every activation to bfloat16 does, whose bounds
 therefore serve the float32 mode here too."""
+import os
 import subprocess
 from dataclasses import dataclass
 
@@ -497,3 +498,17 @@ def test_shared_positions_are_not_run_again(model_folders):
                              capture_output=True, text=True, timeout=300)
         assert out.returncode == 0, out.stderr
         assert (f"prefill: {5 * 80 - 4 * 64} tokens" in out.stderr and "256 more held in common" in out.stderr) if extra else f"prefill: {5 * 80} tokens" in out.stderr
+
+
+def test_the_engine_names_the_kernels_of_rows_in_eight_bits(model_folders):
+    """What it says of itself: the kernels of the cache that it has, and a warning where these are the plain ones."""
+    def says(name, *extra, **env):
+        out = subprocess.run([f"{ROOT}/bin/llama", "-m", model_folders[name], "-g", "GPU", "--prompt-ids", "1,2,3", "-n", "1", "-c", "128", "--no-stop", *extra],
+                             capture_output=True, text=True, timeout=300, env={**os.environ, **env})
+        assert out.returncode == 0, out.stderr
+        return out.stderr
+    assert "rows of eight bits, prompts: tiles (tcgen05); single tokens: pages (TMA ring)" in says("C", "--cache-dtype", "int8", ILLM_LOG="info")
+    assert "cache: 2 of 2 entries in eight bits" in says("C", "--cache-dtype", "int8", ILLM_LOG="info")
+    assert "eight bits" not in says("C", ILLM_LOG="info") and "warning" not in says("C", "--cache-dtype", "int8")
+    told = says("B", "--cache-dtype", "int8")
+    assert "warning" in told and "rows of eight bits, prompts: plain" in told
