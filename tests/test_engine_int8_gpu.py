@@ -512,3 +512,80 @@ def test_the_engine_names_the_kernels_of_rows_in_eight_bits(model_folders):
     assert "eight bits" not in says("C", ILLM_LOG="info") and "warning" not in says("C", "--cache-dtype", "int8")
     told = says("B", "--cache-dtype", "int8")
     assert "warning" in told and "rows of eight bits, prompts: plain" in told
+
+
+@dataclass
+class WideBeside(ArchConfig):
+    """A layer with biases, whose entry stays in the activations' type, between two that can keep eight bits."""
+
+    @classmethod
+    def from_dict(cls, d):
+        return cls()
+
+    def to_dict(self):
+        return {"architectures": ["WideBesideForCausalLM"]}
+
+    def model_spec(self):
+        norm = PartSpec("rmsnorm", {"size": HIDDEN, "eps": 1e-5})
+        half = PartSpec("rope_half", {"head_dim": SIZE, "theta": BASE, "max_positions": 512})
+        shape = {"hidden_size": HIDDEN, "n_heads": HEADS, "n_kv_heads": KV_HEADS, "head_dim": SIZE, "position": half}
+        ffn = PartSpec("gated_mlp", {"hidden_size": HIDDEN, "intermediate_size": 128})
+        layers = [LayerSpec("prenorm", PartSpec("attention", dict(shape, **more)), ffn, {"norm1": norm, "norm2": norm}, f"blocks.{i}.",
+                            {"mixer": "mixer.", "ffn": "ffn.", "norm1": "ln1.", "norm2": "ln2."}) for i, more in enumerate(({}, {"qkv_bias": True}, {}))]
+        return ModelSpec(HIDDEN, WORDS, layers, [ScheduleEntry(i, i) for i in range(3)], PartSpec("embedding", {"name": "emb.", "vocab_size": WORDS, "hidden_size": HIDDEN}),
+                         PartSpec("rmsnorm", {"name": "ln_f.", "size": HIDDEN, "eps": 1e-5}),
+                         PartSpec("lm_head", {"name": "head.", "tied": True, "vocab_size": WORDS, "hidden_size": HIDDEN}), 512, None, [])
+
+
+def plain_beside(w, ids, rounds):
+    pos, x = np.arange(len(ids)), plain.embed(ids, w["emb.weight"])
+    for layer in range(3):
+        p = f"blocks.{layer}."
+        h = plain.rms_norm(x, w[p + "ln1.weight"], 1e-5)
+        q, k, v = (plain.linear(h, w[p + f"mixer.{n}_proj.weight"]) + (w[p + f"mixer.{n}_proj.bias"] if layer == 1 else 0) for n in "qkv")
+        q, k, v = (t.reshape(len(ids), -1, SIZE) for t in (q, k, v))
+        angle = pos[:, None] * BASE ** (-np.arange(0, SIZE, 2) / SIZE)
+
+        def turn(t):
+            a, b, c, s = t[..., :SIZE // 2], t[..., SIZE // 2:], np.cos(angle)[:, None], np.sin(angle)[:, None]
+            return np.concatenate([a * c - b * s, a * s + b * c], -1)
+        q, k = turn(q), turn(k)
+        if rounds and layer != 1:
+            k, v = eight_bits(k), eight_bits(v)
+        s = plain.scale_and_mask(plain.attention_scores(q, k, HEADS, KV_HEADS), SIZE ** -0.5)
+        x = x + plain.linear(plain.weighted_values(plain.softmax_rows(s), v, HEADS, KV_HEADS), w[p + "mixer.o_proj.weight"])
+        h = plain.rms_norm(x, w[p + "ln2.weight"], 1e-5)
+        x = x + plain.swiglu_ffn(h, *(w[p + f"ffn.{n}_proj.weight"] for n in ("gate", "up", "down")))
+    return plain.linear(plain.rms_norm(x, w["ln_f.weight"], 1e-5), w["emb.weight"])
+
+
+@pytest.mark.parametrize("cache", ["auto", "int8"])
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("n", [3, 60])
+def test_common_positions_beside_a_layer_that_reads_them_one_by_one(cache, graphs, n, tmp_path):
+    """Forks in a model whose layers differ: entries in eight bits, one that stays wide and whose layer takes no plan."""
+    register_architecture("WideBesideForCausalLM", WideBeside)
+    try:
+        write_random_model(WideBeside(), str(tmp_path), seed=7, dtype=torch.bfloat16)
+        _, w = plain.load_weights(str(tmp_path))
+        e = engine(str(tmp_path), cache=cache, cuda_graphs=graphs, max_tokens=64 * (2 * n + 8), max_batch=n + 2, shared_prefix_bytes=0)
+        groups = e.cache.stats()["paged"]
+        assert sorted((bool(g["request"].get("int8")), len(g["entries"])) for g in groups) == ([(False, 1), (True, 2)] if cache == "int8" else [(False, 3)])
+        R = np.random.default_rng(3)
+        prompt = R.integers(0, WORDS, 150).tolist()
+        a = e.new_sequence()
+        e.step([StepItem(a, prompt, [])])
+        slots, texts = [a] + [e.fork_sequence(a, 128) for _ in range(n - 1)], [list(prompt)] + [prompt[:128] for _ in range(n - 1)]
+        more = [R.integers(0, WORDS, 1 + i % 9).tolist() for i in range(n - 1)]
+        e.step([StepItem(s, t, []) for s, t in zip(slots[1:], more)])
+        texts[1:] = [t + m for t, m in zip(texts[1:], more)]
+        for j in range(4):
+            tokens = [[int(t)] for t in R.integers(0, WORDS, n)]
+            texts = [t + x for t, x in zip(texts, tokens)]
+            got = e.step([StepItem(s, x, [0]) for s, x in zip(slots, tokens)]).cpu().numpy()
+            for i in (0, 1, n - 1):
+                assert_close(got[i:i + 1], plain_beside(w, texts[i], cache == "int8")[-1:], "bfloat16", f"token {j} of {i}")
+        e.check_device_errors()
+        assert (e.info()["graphs_captured"] > 0) == graphs
+    finally:
+        unregister_architecture("WideBesideForCausalLM")
