@@ -383,9 +383,16 @@ void Engine::drop_graphs(bool keep_seen) {
     }
 }
 
+// A kind of step is captured the second time it comes.  Kinds that never came again are forgotten together; they take no room from those that were captured.
+void Engine::seen_once(const std::string& key) {
+    if (graphs_.size() > (size_t)kKindsMost + kGraphsMost)
+        for (auto it = graphs_.begin(); it != graphs_.end();) it = it->second->exec ? std::next(it) : graphs_.erase(it);
+    graphs_[key].reset(new GraphEntry);
+}
+
 LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, const std::vector<int>& ids,
                                   const std::vector<int>& want_rows, const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes) {
-    if (graphs_.size() > 64) drop_graphs(true);
+    if (graphs_captured() > kGraphsMost) drop_graphs(true);
     std::unique_ptr<GraphEntry> e(new GraphEntry);
     int T = 0;
     for (int q : plan.q_lens) T += q;
@@ -471,7 +478,7 @@ bool Engine::prompt_step_graphed(int slot, const std::vector<int>& ids_in, const
         }
         auto it = graphs_.find(key);
         if (it == graphs_.end()) {
-            graphs_[key].reset(new GraphEntry);       // seen once
+            seen_once(key);
             device_->arena_rewind();
             std::vector<const int*> tables;
             StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters);
@@ -500,7 +507,7 @@ LogitsRef Engine::decode_step_graphed(const StepPlan& plan, const std::vector<in
         for (int n : {prefixes->sizes.tiles, prefixes->sizes.per_tile, prefixes->sizes.longest_prefix, prefixes->sizes.longest_rest}) key += "/" + std::to_string(n);
     auto it = graphs_.find(key);
     if (it == graphs_.end()) {
-        graphs_[key].reset(new GraphEntry);
+        seen_once(key);
         device_->arena_rewind();
         std::vector<const int*> tables;
         StepContext ctx = make_context(plan, ids, want_rows, nullptr, &tables, adapters, prefixes);

@@ -67,6 +67,7 @@ struct LogitsRef {
 };
 
 constexpr size_t kSharedPrefixSequences = 32768;       // a plan's tiles, rounded up to a power of two, still are rows of a grid; larger steps read every sequence by itself
+constexpr int kGraphsMost = 64, kKindsMost = 4096;       // captured steps that are kept, and kinds of steps that came once
 constexpr int kPromptBucket = 64;               // tokens; also the rows the library's products are rounded up to
 constexpr int kPromptGraphMaxTokens = 1024;     // longer prompts keep the GPU busy longer than the host needs to issue them
 
@@ -148,6 +149,7 @@ private:
     LogitsRef replay(GraphEntry& e, const StepPlan& plan, const std::vector<int>& ids, const std::vector<int>& want_rows,
                      const int* device_ids, const StepAdapters* adapters, const StepPrefixes* prefixes = nullptr);
     void drop_graphs(bool keep_seen);
+    void seen_once(const std::string& key);
     size_t context_ints(int T, int B, int K) const;
 
     std::unique_ptr<ArchConfig> config_;

@@ -589,3 +589,19 @@ def test_common_positions_beside_a_layer_that_reads_them_one_by_one(cache, graph
         assert (e.info()["graphs_captured"] > 0) == graphs
     finally:
         unregister_architecture("WideBesideForCausalLM")
+
+
+def test_kinds_of_steps_that_came_once_do_not_push_captured_ones_out(model_folders):
+    """Sequences that grow and batches that shrink make steps of many kinds; those that come again are replayed all the same."""
+    e = engine(model_folders["C"], max_tokens=64 * 200, max_batch=80, shared_prefix_bytes=0)
+    a = e.new_sequence()
+    e.step([StepItem(a, random_prompt("C", 64, 1), [])])
+    slots = [a] + [e.fork_sequence(a, 64) for _ in range(79)]
+    for n in range(2, 80):                # 78 kinds, once each
+        e.step([StepItem(s, [5], [0]) for s in slots[:n]])
+    assert e.info()["graphs_captured"] == 0
+    for _ in range(3):
+        for n in (3, 40):
+            got = e.step([StepItem(s, [5], [0]) for s in slots[-n:]])
+    assert e.info()["graphs_captured"] >= 2 and torch.isfinite(got).all()
+    e.check_device_errors()
