@@ -162,3 +162,37 @@ def test_random_lives(seed):
     c.reset()
     c.check()
     assert c.pages_free() == [40, 40]
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_common_prefixes_are_the_pages_that_all_hold(seed):
+    """Forks of forks at any length, some of whose origins have ended: against a comparison page by page."""
+    rng = random.Random(seed)
+    c, live = cache(num_pages=400, slots=30, page=4, longest=120), []
+    for _ in range(4):
+        s = c.alloc_slot()
+        grow(c, [s], [rng.randint(4, 100)])
+        live.append(s)
+    for _ in range(60):
+        if len(live) > 25 or (len(live) > 6 and rng.random() < 0.25):
+            c.free_slot(live.pop(rng.randrange(len(live))))
+            continue
+        s = rng.choice(live)
+        t = c.fork_slot(s, rng.randint(1, int(c.seq_len[s]) // 4) * 4)
+        if c.seq_len[t] < 110:
+            grow(c, [t], [rng.randint(1, 9)])
+        live.append(t)
+        some = rng.sample(live, rng.randint(1, len(live)))
+        pages = [[p for _, p in sorted(c.pages_of(0, s).items())] for s in some]
+        groups = {}
+        for i, p in enumerate(pages):
+            groups.setdefault(p[0], []).append(i)
+        want = []
+        for m in groups.values():
+            if len(m) > 1:
+                n = 0
+                while all(len(pages[i]) > n and pages[i][n] == pages[m[0]][n] for i in m):
+                    n += 1
+                want.append((4 * n, m))
+        assert sorted(c.common_prefixes(some)) == sorted(want)
+        c.check()
