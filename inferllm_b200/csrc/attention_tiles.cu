@@ -306,8 +306,8 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     } else if (Q8 && warp >= TL_WIDEN_WARP) {
         // ---- bytes to bfloat16, and the factors of the scores (with the softmax's scale) and of the weights.  Keys outside the block's range, where
-        // another sequence's may lie, have factors of zero.  The ring of factors has four places: those of block i + 4 come behind the
-        // wait for the products of block i + 1 (v_empty), so behind every softmax of block i.
+        // another sequence's may lie, have factors of zero.  The ring of factors has four places: those of block i + 4 are made behind
+        // the wait for the stage of V(i + 2), which the products of block i leave (v_empty of both tiles), so behind every softmax of block i.
         const int ct = threadIdx.x - TL_WIDEN_WARP * 32;
         auto widen = [&](const unsigned char* raw, unsigned dst) {
 #pragma unroll

@@ -1,7 +1,9 @@
 // Rows of keys and values in eight bits: rotated, rounded and written into the paged cache in one pass, and read back.
 //
 // A row is the d values of one position and kv head.  With a = max |x| over it, its scale is s = a / 127 and a value is kept as
-// u = 128 + round(x / s) (ties to even), so that it stands for (u - 128) s: at most a / 254 from x.  Pages: u
+// u = 128 + round(x (127 / a)) (ties to even), so that it stands for (u - 128) s: at most a / 254 from x, and four roundings of float32.  That is round(x / s) but for
+// quotients within 2^-15 of the border of two steps, which may fall to either: x (127 / a) and x / (a / 127) are rounded apart (of bfloat16 rows, which often hold a / 2
+// and so 63.5 steps, 0.13 % of the values; both steps are as near).  Pages: u
 // [pages, kv heads, page_size, d] bytes, scales float32 [pages, kv heads, page_size] beside them.  The zero point of 128 keeps u
 // unsigned: an attention kernel makes 1024 + u in half precision by putting the byte into the mantissa.
 // One scale per row, not per page: rows come one at a time and are never rounded again.  A row whose largest value is below
@@ -152,7 +154,7 @@ kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ parti
         const float scale = !finite ? __uint_as_float(0x7fffffffu) : tiny ? 0.f : a / 127.f, inv = !finite || tiny ? 0.f : 127.f / a;
         const int hk = is_k ? slot - nh : slot - nh - nkv;
         const size_t row = ((size_t)page * nkv + hk) * page_size + offset;
-        // u = 128 + round(x / s): added to 1.5 x 2^23 + 128 in one rounding the quotient, at most 127 and a little, is the lowest byte of the sum
+        // u = 128 + round(x (127 / a)): added to 1.5 x 2^23 + 128 in one rounding the quotient, at most 127 and a little, is the lowest byte of the sum
         unsigned u[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) u[k] = __float_as_uint(fmaf(x[k], inv, 12583040.f));

@@ -140,6 +140,9 @@ int attention_decode_ring_splits(long long T, int n_kv_heads, long long max_len,
                                  double stream_bytes_per_us = 6.6e6);
 // Blocks per (token, kv head) of attention_pages for `pairs` of them that walk up to `keys` positions.  Measured in us with heads of 128: 8 pairs of 1,777 positions in
 // 1 / 4 / 8 / 16 / 28 blocks 18.5 / 8.0 / 6.6 / 6.6 / 7.7; 256 of 4,096 in 1 / 2 / 4 / 8 64.7 / 43.7 / 39.8 / 42.0; 512 of up to 8,192 in 1 / 2 / 4 / 8 144 / 131 / 118 / 117.
+// On both sides of its borders, caches that no L2 holds: 8 pairs of 2,900 in 8 / 16 8.2 / 7.6, 3,100 8.8 / 8.2, 6,144 in 8 / 12 / 16 12.6 / 11.8 / 10.1; 448 of up to 4,000 in 1 / 2 / 4
+// 73.2 / 71.2 / 59.4, all of them 4,000 81.0 / 89.4 / 81.4; 512 of 2,000 or more, all alike, in 1 / 2 48.4 / 55.9 (2,100), 85.5 / 93.5 (4,000).  Where it misses most: 128 of 2,100 in 5 (its
+// choice) / 3 23.5 / 18.1, 384 of 1,000 in 2 / 1 30.9 / 24.8, 64 of 2,000 in 4 / 8 14.0 / 11.7.
 int attention_pages_splits(long long pairs, long long keys, int n_sms);
 // Parts of a common prefix of `keys` positions that attention_tiles walks for `pairs` (tile, kv head): a block is alone on its SM.  64 sequences behind 8,192 positions
 // (8 pairs) in 2 / 4 / 8 / 12 / 16 / 18 parts, the whole call, us: 98 / 72 / 53 / 47.6 / 44.4 / 45.2.

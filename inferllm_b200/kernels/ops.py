@@ -1174,7 +1174,8 @@ def attention_decode_int8(q, cache, block_table, token_pos, token_seq, n_heads, 
 
 def attention_prompts_int8(q, cache, block_table, cu_q, seq_lens, max_q, n_heads, window, scale, tile_rows=None):
     """Attention of whole prompts (or chunks that continue a sequence) over a cache of eight-bit rows, the step's own rows written already.
-    `cu_q` int32 [B + 1], `seq_lens` int32 [B] (after the step) and `max_q` as for `attention_prefill_tc`.  Returns [T, heads * head_dim].  bfloat16 with head
+    `cu_q` int32 [B + 1], `seq_lens` int32 [B] (after the step) and `max_q` as for `attention_prefill_tc` (at least the most new tokens of a sequence: rows
+    behind it are not written, nor are those behind the last sequence).  Returns [T, heads * head_dim].  bfloat16 with head
     sizes 64 and 128 and pages of a multiple of 64 positions."""
     if not isinstance(cache, CacheInt8):
         raise KernelError("attention_prompts_int8 reads a CacheInt8")
