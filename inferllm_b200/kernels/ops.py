@@ -985,6 +985,7 @@ class CacheInt8(_Fixed):
         k, v, k_scale, v_scale = (t.detach() for t in (k, v, k_scale, v_scale))
         self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, pages=pages, n_kv_heads=n_kv_heads, page_size=page_size, head_dim=head_dim, device=k.device,
                              pointers=(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()))
+        _error_word(k.device)       # (made here: a call that is captured first of all could not)
 
     @classmethod
     def empty(cls, pages, n_kv_heads, page_size, head_dim, device="cuda"):
@@ -1218,6 +1219,7 @@ class SharedPrefixes(_Fixed):
         at = plan.data_ptr()
         self.__dict__.update(T=T, group_heads=group_heads, device=device, tiles=sizes[0], wide=bool(sizes[1]), longest_prefix=sizes[2], longest_rest=sizes[3], per_tile=sizes[6],
                              longest=max(lens), host=host, plan=plan, pointers=(at + 4 * sizes[4], at, at + 4 * sizes[5]))         # start, tiles, members
+        _error_word(device)         # (as in CacheInt8)
 
 
 def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n_heads, scale, max_len, own_splits=None, pre_splits=None):

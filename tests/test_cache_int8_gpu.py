@@ -6,9 +6,12 @@ much: the scores are sums of d products in float32 on tensor cores (2^-22 a step
 sign; a second one, for the norm of the whole result, takes the two roundings to bfloat16 (weights, results) as independent: a rounding is off by 2^-8 / sqrt(12) on the average of its
 range at most."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
+from conftest import ROOT
 
 from inferllm_b200.binding import KernelError
 
@@ -871,3 +874,46 @@ def test_a_plan_that_goes_beyond_the_table_is_reported(ops, members, prefix):
     got = ops.attention_decode_shared(q, cache, table, beyond, seq, made[1], 4, 0.1, prefix + 1, own_splits=2, pre_splits=4)
     assert take_error(ops) == 8
     assert (got.double() - want.double()).norm() <= 0.01 * want.double().norm()
+
+
+CAPTURED_FIRST = """
+import sys
+import torch
+from inferllm_b200.kernels import ops
+kind, d, nh, n = sys.argv[1], 64, 4, 3
+g = torch.Generator("cuda").manual_seed(1)
+q = torch.randn((n, nh * d), generator=g, device="cuda").bfloat16()
+qkv = torch.randn((n, (nh + 4) * d), generator=g, device="cuda").bfloat16()
+table = torch.tensor([[0, 1], [0, 2], [0, 3]], dtype=torch.int32, device="cuda")
+pos, seq = torch.tensor([70, 80, 127], dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+cu, lens, err = torch.arange(n + 1, dtype=torch.int32, device="cuda"), pos + 1, torch.zeros(1, dtype=torch.int32, device="cuda")
+if kind != "wide":
+    cache = ops.CacheInt8(*(torch.randint(0, 256, (4, 2, 64, d), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)),
+                          *(torch.rand((4, 2, 64), generator=g, device="cuda") * 0.02 for _ in range(2)))
+if kind in ("shared", "wide"):
+    plan = ops.SharedPrefixes([(64, [0, 1, 2])], [71, 81, 128], nh // 2)
+    pair = cache if kind == "shared" else tuple(torch.randn((4, 2, 64, d), generator=g, device="cuda").bfloat16() for _ in range(2))
+call = {"decode": lambda: ops.attention_decode_int8(q, cache, table, pos, seq, nh, 0, 0.125, 128),
+        "plain": lambda: ops.attention_decode_int8(q.float(), cache, table, pos, seq, nh, 0, 0.125, 128),
+        "prompts": lambda: ops.attention_prompts_int8(q, cache, table, cu, lens, 1, nh, 0, 0.125),
+        "rows": lambda: (ops.kv_write_int8(qkv, None, 0, pos, seq, table, cache, nh, err),) + ops.kv_read_int8(cache, pos, seq, table),
+        "shared": lambda: ops.attention_decode_shared(q, pair, table, pos, seq, plan, nh, 0.125, 128),
+        "wide": lambda: ops.attention_decode_shared(q, pair, table, pos, seq, plan, nh, 0.125, 128)}[kind]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = call()
+graph.replay()
+torch.cuda.synchronize()
+want = call()
+for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+    assert torch.equal(a, b) and (a != 0).any()
+print("same")
+"""
+
+
+@pytest.mark.parametrize("kind", ["decode", "plain", "prompts", "rows", "shared", "wide"])
+def test_a_call_that_is_captured_first_of_all(kind):
+    """A process whose first call of the library goes into a graph: nothing is left to be made then."""
+    out = subprocess.run([sys.executable, "-c", CAPTURED_FIRST, kind], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("same"), out.stderr[-2000:]
