@@ -690,14 +690,15 @@ extern "C" int illm_attention_tiles_cluster(int splits) { return splits < TL_CLU
 
 // The shares of common prefixes (ksc, vsc nullptr: bfloat16 pages): for every tile of the plan (at most 256 / (nh / nkv) members), whose positions are cut into `splits` parts,
 // of which every c = illm_attention_tiles_cluster(splits) are joined: for every (member, head) accumulators, maximum (in units of log2) and sum at share slot0 + part / c of
-// `slots`: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  illm_attention_pages adds them up with a token's own.
+// `slots`: part_acc float [T, nh, slots, d], part_ml float [T, nh, slots, 2].  illm_attention_pages adds them up with a token's own.  bfloat16 rows: a scale below zero
+// is refused (the softmax takes its reference from the largest score before the scale).
 extern "C" int illm_attention_tiles_prefix(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages,
                                            const int* block_table, int max_pages, const int* token_seq, const int* plan_tiles, const int* plan_members, int n_tiles,
                                            float* part_acc, float* part_ml, int nh, int nkv, int d, int page_size, float scale, int slots, int slot0, int splits, int* err,
                                            void* stream) {
     if (n_tiles <= 0) return 0;
     if (tl_bad(q, q_stride, kc, vc, ksc, vsc, n_pages, max_pages, nh, nkv, page_size, err) || nh / nkv > 2 * TL_BM || n_tiles > 65535 || splits < 1 || splits > 256 ||
-        slot0 < 0 || slot0 + splits / illm_attention_tiles_cluster(splits) > slots || !part_acc || !part_ml || ((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || !plan_tiles || ((uintptr_t)plan_tiles & 15) || !plan_members)
+        (!ksc && !(scale >= 0.f)) || slot0 < 0 || slot0 + splits / illm_attention_tiles_cluster(splits) > slots || !part_acc || !part_ml || ((uintptr_t)part_acc & 15) || ((uintptr_t)part_ml & 7) || !plan_tiles || ((uintptr_t)plan_tiles & 15) || !plan_members)
         return ILLM_ERR_BAD_ARG;
     TlWork work = {};
     work.tiles = reinterpret_cast<const int4*>(plan_tiles);

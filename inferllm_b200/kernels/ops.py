@@ -1237,6 +1237,8 @@ def attention_decode_shared(q, cache, block_table, token_pos, token_seq, plan, n
                           f"found {q.dtype}, {d}, {page_size} and {n_heads} over {nkv}")
     if plan.T != T or plan.device != device or plan.group_heads != n_heads // nkv:
         raise KernelError(f"attention_decode_shared: the plan is for {plan.T} tokens with {plan.group_heads} query heads per kv head on {plan.device}")
+    if not float(scale) >= 0.0:
+        raise KernelError(f"attention_decode_shared: the scale {scale} must not be negative")
     if int(max_len) < plan.longest:
         raise KernelError(f"attention_decode_shared: max_len {max_len} is below the plan's longest sequence {plan.longest}")
     with _on(device):

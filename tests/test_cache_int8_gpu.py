@@ -917,3 +917,22 @@ def test_a_call_that_is_captured_first_of_all(kind):
     """A process whose first call of the library goes into a graph: nothing is left to be made then."""
     out = subprocess.run([sys.executable, "-c", CAPTURED_FIRST, kind], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip().endswith("same"), out.stderr[-2000:]
+
+
+def test_scales_below_zero(ops):
+    """A negative scale is computed where scores are scaled before their maximum is taken, and refused over common positions."""
+    nh, nkv, d, n = 8, 2, 64, 20
+    pages = Pages(61, [200 + i for i in range(n)], nkv, d, common=[(128, 0)] * n)
+    cache, table = pages.cache(ops), pages.table.cuda()
+    pos, seq = torch.tensor([199 + i for i in range(n)], dtype=torch.int32).cuda(), torch.arange(n, dtype=torch.int32).cuda()
+    q = queries(62, n, nh * d)
+    want, _ = expected(pages, q, [(i, 199 + i) for i in range(n)], nh, 0, -4.0, B8H)
+    cu, lens = torch.arange(n + 1, dtype=torch.int32).cuda(), pos + 1
+    for got in (ops.attention_decode_int8(q.cuda(), cache, table, pos, seq, nh, 0, -4.0, 256), ops.attention_prompts_int8(q.cuda(), cache, table, cu, lens, 1, nh, 0, -4.0)):
+        assert torch.isfinite(got).all() and (got.double().cpu() - want).norm() <= 0.01 * want.norm()
+    plan = ops.SharedPrefixes([(128, list(range(n)))], [200 + i for i in range(n)], nh // nkv)
+    assert plan.wide
+    for scale in (-0.1, float("nan")):
+        with pytest.raises(KernelError, match="scale"):
+            ops.attention_decode_shared(q.cuda(), cache, table, pos, seq, plan, nh, scale, 256)
+    assert take_error(ops) == 0
