@@ -1029,8 +1029,8 @@ def _query_rows(q, device, n_heads, n_kv_heads, head_dim):
     (T, width), (apart, side) = q.shape, q.stride()
     if width < n_heads * head_dim:
         raise KernelError(f"q has {width} columns, {n_heads} heads of {head_dim} need {n_heads * head_dim}")
-    if T and (side != 1 or (T > 1 and apart < width)):
-        raise KernelError("q: a row's elements must lie side by side, and rows apart")
+    if T and (side != 1 or (T > 1 and not width <= apart < 2 ** 31)):
+        raise KernelError("q: a row's elements must lie side by side, and rows apart, by less than 2^31")
     if T and (q.data_ptr() & 15 or (T > 1 and apart * q.element_size() & 15)):
         raise KernelError("q: rows must start on 16-byte boundaries")
     return T, apart if T > 1 else -(-width // 8) * 8

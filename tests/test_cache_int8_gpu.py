@@ -936,3 +936,11 @@ def test_scales_below_zero(ops):
         with pytest.raises(KernelError, match="scale"):
             ops.attention_decode_shared(q.cuda(), cache, table, pos, seq, plan, nh, scale, 256)
     assert take_error(ops) == 0
+
+
+def test_rows_further_apart_than_a_launch_can_say(ops):
+    cache = ops.CacheInt8.empty(2, 2, 64, 64)
+    q = torch.empty(2 ** 31 + 512, dtype=torch.bfloat16, device="cuda").as_strided((2, 512), (2 ** 31, 1))
+    table, pos, seq = torch.zeros((2, 1), dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.arange(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(KernelError, match="apart"):
+        ops.attention_decode_int8(q, cache, table, pos, seq, 8, 0, 0.1, 64)
