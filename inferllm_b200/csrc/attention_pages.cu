@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include "paged_rows.cuh"
 #include "tc_common.cuh"
 
 #define PG_BN 64                        // keys per tile
@@ -84,19 +85,12 @@ template <int D, bool Q8> __device__ __forceinline__ unsigned pg_off(int r, int 
     if (D == 128) return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4));
     return (unsigned)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
-// two and four floats of the same place in another block of the cluster
+// two floats of the same place in another block of the cluster
 __device__ __forceinline__ float2 pg_remote2(unsigned at, unsigned rank) {
     unsigned a;
     float2 f;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
     asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(a) : "memory");
-    return f;
-}
-__device__ __forceinline__ float4 pg_remote4(unsigned at, unsigned rank) {
-    unsigned a;
-    float4 f;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
     return f;
 }
 __device__ __forceinline__ void pg_add(float4& sum, float4 v, float f) {
@@ -109,12 +103,6 @@ __device__ __forceinline__ void pg_add(float4& sum, float4 v, float f) {
 __device__ __forceinline__ void pg_result(bf16* to, float4 num, float den) {
     const bool none = den == 0.f;
     *reinterpret_cast<uint2*>(to) = make_uint2(pg_bf162(none ? 0.f : num.x / den, none ? 0.f : num.y / den), pg_bf162(none ? 0.f : num.z / den, none ? 0.f : num.w / den));
-}
-__device__ __forceinline__ void pg_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void pg_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 }  // namespace
@@ -221,8 +209,8 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 const int groups = min(PG_BN / 16, (p - key0) / 16 + 1);       // of 16 keys, as many as hold a visible one
                 mbar_expect_tx(bar, (unsigned)groups * (2 * TILE / (PG_BN / 16)) + (unsigned)R::SCALES);
                 if (Q8) {
-                    pg_bulk(scales + s * R::SCALES, ksc + row, PG_BN * 4, bar);
-                    pg_bulk(scales + s * R::SCALES + PG_BN * 4, vsc + row, PG_BN * 4, bar);
+                    rows_bulk(scales + s * R::SCALES, ksc + row, PG_BN * 4, bar);
+                    rows_bulk(scales + s * R::SCALES + PG_BN * 4, vsc + row, PG_BN * 4, bar);
                 }
 #pragma unroll
                 for (int hx = 0; hx < (Q8 ? 1 : D / 64); hx++) {
@@ -241,8 +229,8 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         __syncwarp();
         if (!part_acc && n_splits > 1) {        // the cluster's two meetings, at the end
-            pg_cluster_sync();
-            pg_cluster_sync();
+            rows_cluster_sync();
+            rows_cluster_sync();
         }
         return;
     }
@@ -512,7 +500,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (alone || part_acc) return;
     // ---- join the cluster's shares (ascending): every block writes a part of the rows
-    pg_cluster_sync();
+    rows_cluster_sync();
     const unsigned share_at = tc_smem_u32(share);
     for (int idx = split * (PG_CONSUMERS * 32) + tid; idx < rows * (D / 4); idx += n_splits * (PG_CONSUMERS * 32)) {
         const int r = idx / (D / 4), c = (idx - r * (D / 4)) * 4;
@@ -523,7 +511,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int k = 0; k < PG_MAX_CLUSTER; k++) {
             ml[k] = k < n_splits ? pg_remote2(row_at + D * 4, k) : make_float2(-INFINITY, 0.f);
-            v[k] = k < n_splits ? pg_remote4(row_at + c * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[k] = k < n_splits ? rows_remote4(row_at + c * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
             M = fmaxf(M, ml[k].x);
         }
         const float ref = M == -INFINITY ? 0.f : M;
@@ -536,7 +524,7 @@ attention_pages_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         pg_result(out + row_head(r) * D + c, num, den);
     }
-    pg_cluster_sync();              // the others may still read this block's shares
+    rows_cluster_sync();              // the others may still read this block's shares
 }
 
 // out[t, h] = sum over the shares (ascending) of acc 2^(m - M) / sum of l 2^(m - M): a token's own and, where it has a prefix in common with
@@ -575,41 +563,16 @@ attention_pages_join_kernel(const float* __restrict__ part_acc, const float* __r
 
 // ---- host side
 
-typedef CUresult (*PgEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static PgEncodeTiledFn pg_encode_fn() {
-    static const PgEncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess ? (PgEncodeTiledFn)p
-                                                                                                                                         : (PgEncodeTiledFn) nullptr;
-    }();
-    return fn;
-}
-// an entry's pages as a matrix [pages * kv heads * page_size, d]; boxes of `box_rows` rows of 128 bytes (eight bits: of d)
-static int pg_make_map(CUtensorMap* map, const void* ptr, long long rows, int d, int box_rows, bool q8) {
-    PgEncodeTiledFn fn = pg_encode_fn();
-    if (!fn) return ILLM_ERR_BAD_ARG;
-    cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)d * (q8 ? 1 : 2)};
-    cuuint32_t box[2] = {q8 ? (cuuint32_t)d : 64u, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, q8 && d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : ILLM_ERR_BAD_ARG;
-}
-
 template <int D, bool Q8>
 static int pg_launch(const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table, int max_pages,
                      const int* token_pos, const int* token_seq, const PgPlan& plan, float* part_acc, float* part_ml, void* out, int T, int nh, int nkv, int page_size,
                      int span, float scale, int own_splits, int pre_splits, int* err, cudaStream_t s) {
     CUtensorMap mk, mv, mk16, mv16;
     const long long rows = n_pages * nkv * page_size;
+    const CUtensorMapSwizzle swizzle = Q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     int rc;
-    if ((rc = pg_make_map(&mk, kc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mv, vc, rows, D, PG_BN, Q8)) || (rc = pg_make_map(&mk16, kc, rows, D, 16, Q8)) ||
-        (rc = pg_make_map(&mv16, vc, rows, D, 16, Q8)))
+    if ((rc = rows_make_map(&mk, kc, rows, D, PG_BN, Q8, swizzle)) || (rc = rows_make_map(&mv, vc, rows, D, PG_BN, Q8, swizzle)) || (rc = rows_make_map(&mk16, kc, rows, D, 16, Q8, swizzle)) ||
+        (rc = rows_make_map(&mv16, vc, rows, D, 16, Q8, swizzle)))
         return rc;
     // eight rows in a block's products where no block has more
     const bool eight = nh / nkv * (plan.n_tiles ? plan.per_tile : 1) <= 8;

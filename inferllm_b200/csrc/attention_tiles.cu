@@ -22,6 +22,7 @@
 #include <math.h>
 
 #include "attention_tc.cuh"
+#include "paged_rows.cuh"
 #include "tc_common.cuh"
 
 #define TL_BM 128
@@ -56,9 +57,6 @@ template <int D, bool Q8> struct TlSizes {
 
 namespace {
 
-__device__ __forceinline__ void tl_bulk(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void tl_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void tl_store16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -77,15 +75,6 @@ __device__ __forceinline__ void tl_widen(const unsigned (&w)[4], unsigned (&out)
             out[i * 2 + h] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
         }
 }
-// four floats of the same place in another block of the cluster
-__device__ __forceinline__ float4 tl_remote4(unsigned at, unsigned rank) {
-    unsigned a;
-    float4 f;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
-    return f;
-}
-__device__ __forceinline__ void tl_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // four floats of shared memory, the same for all lanes
 __device__ __forceinline__ void tl_load4(unsigned at, float* f) {
     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(at));
@@ -237,9 +226,9 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     const unsigned bar = raw_full0 + 8 * st, dst = raw_s + st * 2 * Z::RAW_TILE;
                     mbar_expect_tx(bar, 2 * Z::RAW_TILE + Z::SCALES);
                     tma_load_2d(dst, &map_k, 0, row, bar);
-                    tl_bulk(sc_s + st * Z::SCALES, ksc + row, TL_BN * 4, bar);
+                    rows_bulk(sc_s + st * Z::SCALES, ksc + row, TL_BN * 4, bar);
                     tma_load_2d(dst + Z::RAW_TILE, &map_v, 0, row, bar);
-                    tl_bulk(sc_s + st * Z::SCALES + TL_BN * 4, vsc + row, TL_BN * 4, bar);
+                    rows_bulk(sc_s + st * Z::SCALES + TL_BN * 4, vsc + row, TL_BN * 4, bar);
                 } else {
                     const int st = i % STAGES;
                     const unsigned kd = kv_s + st * 2 * TILE, vd = kd + TILE;
@@ -564,13 +553,13 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         // the cluster's shares of a row (ascending) become one; every block makes a part of the rows: first their factors, then four columns to a thread
         const int n = work.cluster, rank = (int)blockIdx.x % n, rows_each = (n_rows + n - 1) / n, r0 = rank * rows_each, r1 = min(n_rows, r0 + rows_each);
         const unsigned factors = base + 2 * TL_BM * SHARE_ROW;              // [row of the part][TL_CLUSTER]
-        if (n > 1) tl_cluster_sync();
+        if (n > 1) rows_cluster_sync();
         for (int br = r0 + (int)threadIdx.x; br < r1; br += (int)blockDim.x) {
             float4 ml[TL_CLUSTER];
             float M = -INFINITY, f[TL_CLUSTER], den = 0.f;
 #pragma unroll
             for (int k = 0; k < TL_CLUSTER; k++) {
-                ml[k] = k < n ? tl_remote4(base + br * SHARE_ROW + D * 4, k) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+                ml[k] = k < n ? rows_remote4(base + br * SHARE_ROW + D * 4, k) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
                 M = fmaxf(M, ml[k].x);
             }
 #pragma unroll
@@ -592,7 +581,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             float4 v[TL_CLUSTER], num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < TL_CLUSTER; k++)
-                if (f[k] != 0.f) v[k] = tl_remote4(base + br * SHARE_ROW + c * 16, k);
+                if (f[k] != 0.f) v[k] = rows_remote4(base + br * SHARE_ROW + c * 16, k);
 #pragma unroll
             for (int k = 0; k < TL_CLUSTER; k++) {
                 if (f[k] == 0.f) continue;
@@ -604,7 +593,7 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             const size_t share = ((size_t)work.members[member0 + br / G] * nh + hk * G + br % G) * work.slots + work.slot0 + blockIdx.x / n;
             *reinterpret_cast<float4*>(work.part_acc + share * D + c * 4) = num;
         }
-        if (n > 1) tl_cluster_sync();               // the others may still read this block's rows
+        if (n > 1) rows_cluster_sync();               // the others may still read this block's rows
     }
     if (warp == TL_MMA_WARP) {
         tc_fence_after();
@@ -614,35 +603,14 @@ attention_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
 // ---- host side
 
-typedef CUresult (*TlEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// an entry's pages as a matrix [pages * kv heads * page_size, d]; boxes of 64 rows of 128 bytes (eight bits: of d)
-static int tl_make_map(CUtensorMap* map, const void* ptr, long long rows, int d, bool q8) {
-    static const TlEncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess ? (TlEncodeTiledFn)p
-                                                                                                                                         : (TlEncodeTiledFn) nullptr;
-    }();
-    if (!fn) return ILLM_ERR_BAD_ARG;
-    cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)d * (q8 ? 1 : 2)};
-    cuuint32_t box[2] = {q8 ? (cuuint32_t)d : 64u, TL_BN};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, q8 && d == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : ILLM_ERR_BAD_ARG;
-}
-
 template <int D, bool Q8, bool PREFIX>
 static int tl_launch(dim3 grid, const void* q, int q_stride, const void* kc, const void* vc, const float* ksc, const float* vsc, long long n_pages, const int* block_table,
                      int max_pages, const TlWork& work, void* out, int nh, int nkv, int page_size, float scale, int* err, cudaStream_t s) {
     CUtensorMap mk, mv;
     const long long rows = n_pages * nkv * page_size;
+    const CUtensorMapSwizzle swizzle = Q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     int rc;
-    if ((rc = tl_make_map(&mk, kc, rows, D, Q8)) || (rc = tl_make_map(&mv, vc, rows, D, Q8))) return rc;
+    if ((rc = rows_make_map(&mk, kc, rows, D, TL_BN, Q8, swizzle)) || (rc = rows_make_map(&mv, vc, rows, D, TL_BN, Q8, swizzle))) return rc;
     auto kern = attention_tiles_kernel<D, Q8, PREFIX>;
     const int smem = TlSizes<D, Q8>::SMEM;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
