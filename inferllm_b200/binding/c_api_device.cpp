@@ -46,7 +46,9 @@ ILLM_API int illm_engine_from_folder(const char* folder, const char* options_jso
                        .release();
     });
 }
-ILLM_API void illm_engine_free(void* e) { delete (Engine*)e; }
+ILLM_API void illm_engine_free(void* e) {
+    after_captures([e] { delete (Engine*)e; });
+}
 ILLM_API int illm_engine_load_folder(void* e, const char* folder) {
     return guard([&] { ((Engine*)e)->load_folder(folder); });
 }
@@ -268,7 +270,9 @@ ILLM_API int illm_model_create(const char* config_json, const char* model_name, 
         *out = new Model(c, model_name ? model_name : "");
     });
 }
-ILLM_API void illm_model_free(void* m) { delete (Model*)m; }
+ILLM_API void illm_model_free(void* m) {
+    after_captures([m] { delete (Model*)m; });
+}
 ILLM_API int illm_model_load(void* m, const char* path) {
     return guard([&] { ((Model*)m)->load(path); });
 }

@@ -304,7 +304,9 @@ ILLM_API int illm_sandbox_create(const char* requests_json, const char* dtype, i
         *out = sb.release();
     });
 }
-ILLM_API void illm_sandbox_free(void* sb) { delete (Sandbox*)sb; }
+ILLM_API void illm_sandbox_free(void* sb) {
+    after_captures([sb] { delete (Sandbox*)sb; });
+}
 ILLM_API void* illm_sandbox_cache(void* sb) { return ((Sandbox*)sb)->cache.get(); }
 ILLM_API void* illm_sandbox_device(void* sb) { return ((Sandbox*)sb)->dev.get(); }
 

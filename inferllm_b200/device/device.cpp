@@ -4,8 +4,45 @@
 
 #include <algorithm>
 #include <cstring>
+#include <mutex>
+#include <utility>
 
 namespace illm {
+
+namespace {
+struct Captures {
+    std::mutex lock;
+    int open = 0;
+    std::vector<std::function<void()>> waiting;
+};
+Captures& captures() {
+    static Captures* c = new Captures;      // (never torn down: what is freed at the process's end still asks it)
+    return *c;
+}
+}  // namespace
+
+Capture::Capture() {
+    std::lock_guard<std::mutex> hold(captures().lock);
+    captures().open++;
+}
+Capture::~Capture() {
+    std::vector<std::function<void()>> now;
+    {
+        std::lock_guard<std::mutex> hold(captures().lock);
+        if (--captures().open == 0) now.swap(captures().waiting);
+    }
+    for (auto& f : now) f();
+}
+void after_captures(std::function<void()> f) {
+    {
+        std::lock_guard<std::mutex> hold(captures().lock);
+        if (captures().open > 0) {
+            captures().waiting.push_back(std::move(f));
+            return;
+        }
+    }
+    f();
+}
 
 void check_kernel(int code, const char* what) {
     if (code == 0) return;

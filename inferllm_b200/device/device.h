@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 
 #include <cstddef>
+#include <functional>
 #include <string>
 #include <vector>
 
@@ -32,6 +33,17 @@ namespace illm {
 void check_kernel(int code, const char* what);
 // Raises EngineError for a CUDA runtime error.
 void check_cuda(cudaError_t e, const char* what);
+
+// While one lives a stream of this process is being captured.  What a device's end does (the library's handle waits for the whole device) would end the capture with an
+// error, and it may come at any moment: from another thread, or from a collector of garbage that runs inside a part written in another language.
+class Capture {
+public:
+    Capture();
+    ~Capture();         // runs what waited for the last capture
+    Capture(const Capture&) = delete;
+};
+// Now, or when the captures that are going on have ended.
+void after_captures(std::function<void()> f);
 
 class Device {
 public:

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import json
+import weakref
 from dataclasses import asdict, dataclass, field
 from typing import Callable, List, Optional, Sequence
 
@@ -91,7 +92,7 @@ class Engine:
     def __init__(self, config: ArchConfig, options: EngineOptions, _ptr=None, _owner=None):
         self.options = options
         self._owner = _owner
-        self._cache = None
+        self._cache = None        # weak reference: the cache's face holds the engine, which so goes when the last of both is let go, not when a collector comes
         self._children = []       # weak references to samplers made on this engine: they go before it does
         if _ptr is None:
             out = ctypes.c_void_p()
@@ -105,7 +106,6 @@ class Engine:
         self.device_id = info["device"]
 
     def _adopt(self, child) -> None:
-        import weakref
         self._children.append(weakref.ref(child))
 
     def _release_children(self) -> None:
@@ -237,9 +237,11 @@ class Engine:
 
     @property
     def cache(self) -> SequenceCache:
-        if self._cache is None:
-            self._cache = SequenceCache.wrap(_b.lib().illm_engine_cache(self._ptr), self)
-        return self._cache
+        cache = self._cache() if self._cache is not None else None
+        if cache is None:
+            cache = SequenceCache.wrap(_b.lib().illm_engine_cache(self._ptr), self)
+            self._cache = weakref.ref(cache)
+        return cache
 
     @property
     def last_upload_bytes(self) -> int:

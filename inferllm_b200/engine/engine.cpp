@@ -408,6 +408,7 @@ LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, 
                    "copying the step's token ids");
     device_->synchronize();
     const long long before = ops::launch_count();
+    std::unique_ptr<Capture> going_on(new Capture);
     cudaError_t rc = cudaStreamBeginCapture(device_->stream(), cudaStreamCaptureModeRelaxed);
     if (rc != cudaSuccess) {
         device_->free_persistent(e->ctx_buf);
@@ -424,6 +425,8 @@ LogitsRef Engine::capture_and_run(const std::string& key, const StepPlan& plan, 
         throw;
     }
     rc = cudaStreamEndCapture(device_->stream(), &e->graph);
+    going_on.reset();
+    device_->make_current();            // (what waited may have been another device's)
     if (rc == cudaSuccess) rc = cudaGraphInstantiate(&e->exec, e->graph, 0);
     if (rc != cudaSuccess) {
         if (e->graph) cudaGraphDestroy(e->graph);

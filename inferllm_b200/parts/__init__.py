@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import json
+import weakref
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -379,13 +380,20 @@ class PartSandbox:
         _b.check(_b.lib().illm_sandbox_create(json.dumps(reqs).encode(), dtype.encode(), num_slots, num_pages, page_size, max_seq_len,
                                               ctypes.c_void_p(torch.cuda.current_stream().cuda_stream or 1), ctypes.byref(out)))
         self._ptr = out
-        self.cache = SequenceCache.wrap(_b.lib().illm_sandbox_cache(out), self)
+        self._cache = None       # weak reference: the cache's face holds the sandbox
         self._dev = ctypes.c_void_p(_b.lib().illm_sandbox_device(out))
         self.B = 0
         self._children = []      # weak references to parts, streams and blocks: they go before the device does
 
+    @property
+    def cache(self) -> SequenceCache:
+        cache = self._cache() if self._cache is not None else None
+        if cache is None:
+            cache = SequenceCache.wrap(_b.lib().illm_sandbox_cache(self._ptr), self)
+            self._cache = weakref.ref(cache)
+        return cache
+
     def _adopt(self, child) -> None:
-        import weakref
         self._children.append(weakref.ref(child))
 
     def __del__(self):
@@ -394,7 +402,6 @@ class PartSandbox:
             if child is not None:
                 child._free()
         if getattr(self, "_ptr", None) and _b._lib is not None:
-            self.cache = None
             _b._lib.illm_sandbox_free(self._ptr)
         self._ptr = None
 
