@@ -171,6 +171,12 @@ class PositionEncoding(Part):
 
 
 _REGISTERED = {}     # (family, kind) -> everything that has to stay alive while the kind is registered
+_UNREGISTERED = []   # the same of kinds that are not any more, while parts of theirs are there (a live engine's): they still call it
+
+
+def _retire(family: str, kind: str):
+    old = _REGISTERED.pop((family, kind), None)
+    _UNREGISTERED[:] = [e for e in _UNREGISTERED + ([old] if old else []) if e[2]]
 
 
 def _register(family: str, kind: str, cls):
@@ -264,6 +270,7 @@ def _register(family: str, kind: str, cls):
     for name, f in funcs.items():
         setattr(table, name, ctypes.cast(f, P))
     _b.check(_b.lib().illm_register_foreign_part(family.encode(), kind.encode(), ctypes.byref(table)))
+    _retire(family, kind)
     _REGISTERED[(family, kind)] = (table, funcs, instances, texts, errors)
     return cls
 
@@ -282,7 +289,7 @@ def register_position(kind: str):
 
 def unregister_part(family: str, kind: str):
     _b.check(_b.lib().illm_unregister_part(family.encode(), kind.encode()))
-    _REGISTERED.pop((family, kind), None)
+    _retire(family, kind)
 
 
 def registered_parts(family: str):

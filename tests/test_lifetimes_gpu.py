@@ -108,3 +108,27 @@ def test_what_goes_while_a_step_is_captured_waits_for_its_end(one_part, model_fo
         assert (gone[0]() is None) == (LetsGo.captures > 0) == (gone[1]() is None)
     assert LetsGo.captures == 1 and e.info()["graphs_captured"] == 1
     e.check_device_errors()
+
+
+def test_a_part_that_is_no_longer_registered_serves_the_engines_that_have_it(tmp_path):
+    """Its callbacks stay until the last such engine has gone; the same kind may be registered anew beside it."""
+    from inferllm_b200 import parts
+    LetsGo.others = []
+    made = []
+    for _ in range(2):
+        register_architecture("OnePartForCausalLM", OnePart)
+        register_position("lets_go_of_a_test")(LetsGo)
+        write_random_model(OnePart(), str(tmp_path), seed=3, dtype=torch.bfloat16)
+        e = Engine.from_folder(str(tmp_path), EngineOptions(dtype="float32", max_tokens=256, max_batch=2))
+        made.append((e, e.new_sequence()))
+        unregister_architecture("OnePartForCausalLM")
+        unregister_part("position", "lets_go_of_a_test")
+        gc.collect()
+    for t in range(4):
+        a, b = (e.step([StepItem(s, [t + 1], [0])]).cpu() for e, s in made)
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+    assert len(parts._UNREGISTERED) >= 2
+    del e, made
+    gc.collect()
+    parts._retire("position", "none of this kind")
+    assert not any(isinstance(x, LetsGo) for entry in parts._UNREGISTERED for x in entry[2].values())
