@@ -1,9 +1,7 @@
 // Rows of keys and values in eight bits: rotated, rounded and written into the paged cache in one pass, and read back.
 //
 // A row is the d values of one position and kv head.  With a = max |x| over it, its scale is s = a / 127 and a value is kept as
-// u = 128 + round(x (127 / a)) (ties to even), so that it stands for (u - 128) s: at most a / 254 from x, and four roundings of float32.  That is round(x / s) but for
-// quotients within 2^-15 of the border of two steps, which may fall to either: x (127 / a) and x / (a / 127) are rounded apart (of bfloat16 rows, which often hold a / 2
-// and so 63.5 steps, 0.13 % of the values; both steps are as near).  Pages: u
+// u = 128 + round(127 x / a) (ties to even), so that it stands for (u - 128) s: at most a / 254 from x, and the scale's rounding.  Pages: u
 // [pages, kv heads, page_size, d] bytes, scales float32 [pages, kv heads, page_size] beside them.  The zero point of 128 keeps u
 // unsigned: an attention kernel makes 1024 + u in half precision by putting the byte into the mantissa.
 // One scale per row, not per page: rows come one at a time and are never rounded again.  A row whose largest value is below
@@ -151,13 +149,17 @@ kv_write_int8_kernel(const TA* __restrict__ qkv, const float* __restrict__ parti
         for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
         const float a = __uint_as_float(top);
         const bool finite = top < 0x7f800000u, tiny = finite && a < KQ_TINY;
-        const float scale = !finite ? __uint_as_float(0x7fffffffu) : tiny ? 0.f : a / 127.f, inv = !finite || tiny ? 0.f : 127.f / a;
+        const float scale = !finite ? __uint_as_float(0x7fffffffu) : tiny ? 0.f : a / 127.f, inv = !finite || tiny ? 0.f : 1.f / a;
         const int hk = is_k ? slot - nh : slot - nh - nkv;
         const size_t row = ((size_t)page * nkv + hk) * page_size + offset;
-        // u = 128 + round(x (127 / a)): added to 1.5 x 2^23 + 128 in one rounding the quotient, at most 127 and a little, is the lowest byte of the sum
+        // u = 128 + round(127 x / a): (127 / 128) x / a, rounded once (the remainder of the first quotient corrects it: P. Markstein, 1990; with the reciprocal alone
+        // exact halves, which rows of bfloat16 often hold, fell to either side: 0.13 % of their values), and 128 times that added to 1.5 x 2^23 + 128 in one rounding, whose sum's lowest byte it is
         unsigned u[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) u[k] = __float_as_uint(fmaf(x[k], inv, 12583040.f));
+        for (int k = 0; k < 8; k++) {
+            const float y = x[k] * 0.9921875f, q = y * inv;
+            u[k] = __float_as_uint(fmaf(fmaf(fmaf(-q, a, y), inv, q), 128.f, 12583040.f));
+        }
         unsigned lo = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
         unsigned hi = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
         if (!finite) lo = hi = 0x80808080u;

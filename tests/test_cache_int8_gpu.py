@@ -944,3 +944,31 @@ def test_rows_further_apart_than_a_launch_can_say(ops):
     table, pos, seq = torch.zeros((2, 1), dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.arange(2, dtype=torch.int32, device="cuda")
     with pytest.raises(KernelError, match="apart"):
         ops.attention_decode_int8(q, cache, table, pos, seq, 8, 0, 0.1, 64)
+
+
+@pytest.mark.parametrize("nh, nkv, d, slices", [(4, 2, 64, 0), (32, 8, 128, 0), (3, 1, 24, 0), (2, 2, 256, 0), (32, 8, 128, 2)])
+def test_values_fall_to_the_nearest_step(ops, nh, nkv, d, slices):
+    """u = 128 + round(127 x / max |x|), halves to even, for rows as they come (bfloat16, not rotated), against whole numbers in 64 bits: 127 x is exact in float32 and a quotient of
+    bfloat16 numbers that is no half is further from one than its rounding.  Rows hold their largest and its half, whose quotient is 63.5."""
+    T = 500
+    g = torch.Generator().manual_seed(nh * d)
+    x = torch.randn((T, nh + 2 * nkv, d), generator=g) * torch.exp(4 * torch.randn((T, nh + 2 * nkv, 1), generator=g))
+    x = x.bfloat16()
+    top = x.float().abs().amax(-1, keepdim=True)
+    x[:, :, 1:2] = (top / 2).bfloat16()
+    x[:, :, 2:3] = (-top / 2).bfloat16()
+    cache = ops.CacheInt8.empty(-(-T // 64), nkv, 64, d)
+    pos, seq = torch.arange(T, dtype=torch.int32).cuda(), torch.zeros(T, dtype=torch.int32).cuda()
+    table, err = torch.arange(cache.pages, dtype=torch.int32).cuda().view(1, -1), torch.zeros(1, dtype=torch.int32, device="cuda")
+    qkv = x.reshape(T, -1).cuda()
+    if slices:          # the first slice is the row, the others add nothing
+        qkv = ops.SplitKPartials(torch.cat([qkv.float()[None], torch.zeros((slices - 1,) + qkv.shape, device="cuda")]).contiguous())
+    ops.kv_write_int8(qkv, None, 0, pos, seq, table, cache, nh, err)
+    for got, scale, rows in ((cache.k, cache.k_scale, x[:, nh:nh + nkv]), (cache.v, cache.v_scale, x[:, nh + nkv:])):
+        a = rows.double().abs().amax(-1, keepdim=True)
+        want = torch.round(127 * rows.double() / a) + 128
+        u = got.cpu().transpose(1, 2).reshape(-1, nkv, d)[:T].double()
+        assert torch.equal(u, want)
+        s = scale.cpu().transpose(1, 2).reshape(-1, nkv)[:T]
+        assert torch.equal(s, a[..., 0].float() / torch.full((T, nkv), 127.0))
+    assert int(err.item()) == 0
