@@ -58,8 +58,8 @@ __device__ __forceinline__ float kq_fetch1(const TA* __restrict__ x, const float
 }
 
 // LANES: lanes of a row, eight channels each.  WIDE (rot a multiple of 8): a lane of the rotated part has four channels and the four that they are turned with, so
-// that it needs no other lane's and each of its cosines once (4,096 tokens of 32 + 16 heads of 128 take 24 us, bound by instructions, 64 % of the issue slots; with eight
-// neighbours a lane, and their partners fetched beside them, 27).  Otherwise it has eight neighbours and fetches their partners one by one.  A block takes ROUNDS times
+// that it needs no other lane's and each of its cosines once (4,096 tokens of 32 + 16 heads of 128 take 22 us, floor 14, mostly instructions, 70 % of the issue slots; with eight
+// neighbours a lane, and their partners fetched beside them, 3 us more).  Otherwise it has eight neighbours and fetches their partners one by one.  A block takes ROUNDS times
 // KQ_THREADS / LANES heads of one token.
 template <typename TA, bool PARTIALS, bool WIDE, int LANES, int ROUNDS>
 __global__ void __launch_bounds__(KQ_THREADS, WIDE && !PARTIALS && sizeof(TA) == 2 ? 5 : 4)
@@ -216,7 +216,7 @@ extern "C" int illm_kv_write_int8(const void* qkv, const float* partials, int sp
     if (((uintptr_t)qkv & 15) || ((uintptr_t)partials & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)cos_sin & 15)) return ILLM_ERR_BAD_ARG;
     const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, at_once = KQ_THREADS / lanes;
     const int n_slots = nh + (write_kv ? 2 * nkv : 0), rounds_all = (n_slots + at_once - 1) / at_once;
-    // several heads to a thread once that leaves eight blocks to every SM (4,096 tokens of 32 + 16 heads written and read back 31.3 us, one head to a thread 37.1; 8 tokens
+    // several heads to a thread once that leaves eight blocks to every SM (4,096 tokens of 32 + 16 heads written and read back 29.2 us, one head to a thread 37.6; 8 tokens
     // of 32 + 64 heads 4.2 with one, 4.9 with four)
     const bool wide = (rot & 7) == 0;
     int rounds = 1;
