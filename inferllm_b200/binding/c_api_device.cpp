@@ -224,7 +224,9 @@ ILLM_API int illm_sampler_create(void* engine, const char* params_json, void** o
         *out = j.kind() == Json::Array ? new Sampler(dev, each_from(j)) : new Sampler(dev, params_from(j));
     });
 }
-ILLM_API void illm_sampler_free(void* s) { delete (Sampler*)s; }
+ILLM_API void illm_sampler_free(void* s) {
+    after_captures([s] { delete (Sampler*)s; });
+}
 // logits: float32 [B, V] on the device; hist_lens == nullptr: no histories.  *tokens: int32 [B] on the
 // device, valid for the sampler's next three calls.
 ILLM_API int illm_sampler_choose(void* s, const float* logits, int B, long long V, const int* requests, const int* steps,

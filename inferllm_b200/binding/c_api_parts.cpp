@@ -328,7 +328,9 @@ ILLM_API int illm_sandbox_build(void* sbp, const char* family, const char* spec_
         *out = h.release();
     });
 }
-ILLM_API void illm_part_free(void* p) { delete (PartHandle*)p; }
+ILLM_API void illm_part_free(void* p) {
+    after_captures([p] { delete (PartHandle*)p; });
+}
 ILLM_API int illm_part_describe(void* p, char** out) {
     return guard([&] {
         PartHandle* h = (PartHandle*)p;
@@ -496,7 +498,9 @@ ILLM_API int illm_sandbox_block(void* sbp, const char* kind, void* mixer, void* 
         *out = b.release();
     });
 }
-ILLM_API void illm_block_free(void* b) { delete (BlockHandle*)b; }
+ILLM_API void illm_block_free(void* b) {
+    after_captures([b] { delete (BlockHandle*)b; });
+}
 ILLM_API int illm_block_norm_roles(const char* kind, char** out) {
     return guard([&] {
         Json a = Json::array();

@@ -132,3 +132,20 @@ def test_a_part_that_is_no_longer_registered_serves_the_engines_that_have_it(tmp
     gc.collect()
     parts._retire("position", "none of this kind")
     assert not any(isinstance(x, LetsGo) for entry in parts._UNREGISTERED for x in entry[2].values())
+
+
+def test_a_sampler_that_goes_while_its_engine_captures_waits_too(one_part):
+    """Its buffers are freed behind what the engine's stream holds, which a stream that is being captured cannot be waited for."""
+    from inferllm_b200.sampling import Sampler, SamplingParams
+    e = Engine.from_folder(one_part, EngineOptions(dtype="float32", max_tokens=256, max_batch=2))
+    sampler = Sampler(e, SamplingParams(temp=0.0, repeat_penalty=1.1, repeat_last_n=8))
+    slot = e.new_sequence()
+    logits = e.step([StepItem(slot, [1, 2, 3], [2])])
+    token = sampler.choose(logits, [0], [0], [[1, 2, 3]])
+    LetsGo.others, LetsGo.captures = [sampler], 0
+    gone = weakref.ref(sampler)
+    del sampler
+    for t in range(4):
+        got = e.step([StepItem(slot, [t + 1], [0])])
+    assert LetsGo.captures == 1 and gone() is None and torch.isfinite(got).all() and 0 <= int(token[0]) < WORDS
+    e.check_device_errors()
