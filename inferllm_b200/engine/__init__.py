@@ -237,6 +237,8 @@ class Engine:
 
     @property
     def cache(self) -> SequenceCache:
+        if not self._ptr:
+            raise EngineError("the model has loaded other weights, and this engine has gone")
         cache = self._cache() if self._cache is not None else None
         if cache is None:
             cache = SequenceCache.wrap(_b.lib().illm_engine_cache(self._ptr), self)

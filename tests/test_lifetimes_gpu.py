@@ -149,3 +149,15 @@ def test_a_sampler_that_goes_while_its_engine_captures_waits_too(one_part):
         got = e.step([StepItem(slot, [t + 1], [0])])
     assert LetsGo.captures == 1 and gone() is None and torch.isfinite(got).all() and 0 <= int(token[0]) < WORDS
     e.check_device_errors()
+
+
+def test_the_cache_of_an_engine_that_has_gone_is_refused(model_folders):
+    from inferllm_b200 import EngineError
+    m = Model(ModelConfig(nr_ctx=128, max_tokens=256))
+    m.load(model_folders["A"])
+    old = m.engine
+    assert old.cache.pages_free() == [4]
+    m.load(model_folders["B"])
+    with pytest.raises(EngineError, match="gone"):
+        old.cache
+    assert m.engine is not old and m.engine.cache.pages_free() == [4]
